@@ -322,6 +322,112 @@ LF_API int lf_gather_signals(int batch, int n_q, int world);
 LF_API int lf_gather_wait(uint32_t* flags, int layer, uint32_t expected, uint64_t limit_ns, int32_t* status,
                           lf_stream_t stream);
 
+/*
+ * ---- The 4-bit paged cache ------------------------------------------------
+ *
+ * A second cache beside the tiered one above: Key and Value both at 4 bits,
+ * quantized token by token as they are written, so it needs no calibrated
+ * policy and holds no original-dtype residual page (no counterpart in the
+ * reference, whose packed backend stores Value at 2 bits and Key by an offline
+ * tier map, layout.py:71-129).  Each group of 32 channels of a token has an
+ * fp16 scale s and minimum z; a code c in 0..15 stands for c * s + z (fp32).
+ *
+ * A pool holds records of 64-token pages, one per (page, KV head), of
+ * 20 * head_dim int32 words: Key codes (8 * head_dim words), Key parameters
+ * (2 * head_dim), Value codes, Value parameters.  Token k of the page, group G
+ * (channels 32 G .. 32 G + 31):
+ *   Key:    channel 32 G + 8 t + n is nibble n of word k * D/8 + t * D/32 + G
+ *   Value:  channel 64 w + 32 u + 4 g + n of token 8 b + 2 t + o is nibble 4 u + n
+ *           of word b * D + g * D/8 + t * D/32 + o * D/64 + w
+ *   parameters: word k * D/32 + G, s in the low half, z in the high half
+ * The page table gives sequence b's logical page j as pool page
+ * table[b * table_stride + j]; sequences may share pages.  An entry outside
+ * [0, n_pages) is never followed: the tokens there are skipped (written
+ * nowhere, read as zero, not attended) and LF_ERR_OUT_OF_RANGE goes to *status
+ * (device int32, may be NULL).
+ *
+ * Bounds records (optional, int8; a sparse call needs them):
+ * 2 * head_dim + 1 bytes or more per (page, KV head): upper and lower bound of
+ * every Key channel over the page's tokens, in steps of 2^e, then e.  They
+ * are written when slot 63 of a page is.
+ */
+typedef struct lf_int4_pool {
+  int32_t* pages;        /* records, 16-byte aligned                              */
+  const int32_t* table;  /* [batch][table_width] pool pages                      */
+  int64_t page_stride;   /* words between pages, multiple of 4                   */
+  int64_t head_stride;   /* words between KV heads, multiple of 4                */
+  int64_t table_stride;  /* entries between sequences                            */
+  int32_t table_width;   /* logical pages per sequence                           */
+  int32_t n_pages;       /* pages in the pool                                    */
+  int32_t kv_heads;
+  int32_t batch;
+} lf_int4_pool;
+
+/*
+ * Quantize and store tokens: token i of sequence b (i < counts[b], or i <
+ * tokens where counts is NULL) goes to position start[b] + i.
+ * key/value [batch][kv_heads][tokens][head_dim] with the given element
+ * strides (channel stride 1, rows 16-byte aligned), dtype F32, F16 or BF16.
+ * bounds (may be NULL) with strides in bytes.  A group whose scale or minimum
+ * is not a finite fp16 number reads back as NaN.
+ */
+LF_API int lf_int4_write(const lf_int4_pool* pool, int head_dim, const void* key, const void* value, int dtype,
+                         int64_t k_seq_stride, int64_t k_head_stride, int64_t k_tok_stride, int64_t v_seq_stride,
+                         int64_t v_head_stride, int64_t v_tok_stride, int tokens, const int32_t* start,
+                         const int32_t* counts, int8_t* bounds, int64_t bounds_page_stride,
+                         int64_t bounds_head_stride, int32_t* status, lf_stream_t stream);
+
+/* Read positions start[b] .. start[b] + tokens - 1 back into out_k/out_v
+ * [batch][kv_heads][tokens][head_dim] (contiguous, 16-byte aligned); token i is zero
+ * from counts[b] on (counts may be NULL). */
+LF_API int lf_int4_read(const lf_int4_pool* pool, int head_dim, const int32_t* start, const int32_t* counts,
+                        int tokens, void* out_k, void* out_v, int out_dtype, int32_t* status, lf_stream_t stream);
+
+/* Bounds records as fp32 values: out [n_pages][kv_heads][2][head_dim], upper then lower. */
+LF_API int lf_int4_read_bounds(const int8_t* bounds, int64_t page_stride, int64_t head_stride, int n_pages,
+                               int kv_heads, int head_dim, float* out, lf_stream_t stream);
+
+/*
+ * The pages a sparse call reads, for each sequence b, query token i and KV
+ * head h.  Query token i sees v = max(0, lengths[b] - c + 1 + i) tokens, c =
+ * counts[b] (q_len where counts is NULL; a token i >= c sees none), n =
+ * ceil(v / 64) pages: the first sink_pages and the last recent_pages always, and of
+ * the rest the top_pages with the largest
+ * score (ties to the lower page).  With the group's queries scaled by the
+ * power of two 2^-f that brings the largest magnitude among them to 127 at
+ * most, and rounded to whole numbers Q (half to even; a non-finite one counts
+ * as 0), the score of a page is fp32(I) * 2^e,
+ *   I = sum_channels upper * sum_heads max(Q, 0) + lower * sum_heads min(Q, 0),
+ * an upper bound of the group's summed scores in units of 2^f, exact in whole
+ * numbers: the choice does not depend on the order of any sum.
+ * picked [batch][q_len][kv_heads][sink + recent + top] int32: logical pages in
+ * ascending order, -1 after the last.  Candidate pages need their bounds record.
+ * q [batch][n_q][q_len][head_dim], dtype F16 or BF16.
+ */
+LF_API int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void* q, int q_dtype, int64_t q_seq_stride,
+                          int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int8_t* bounds,
+                          int64_t bounds_page_stride, int64_t bounds_head_stride, const int32_t* lengths,
+                          const int32_t* counts, int top_pages, int sink_pages, int recent_pages, int32_t* picked, int32_t* status,
+                          lf_stream_t stream);
+
+/*
+ * Attention of q [batch][n_q][q_len][head_dim] over the cached tokens: query
+ * token i sees positions 0 .. lengths[b] - c + i, c = counts[b] (q_len where
+ * counts is NULL; a token i >= c sees none): the causal mask of
+ * reference.py:18-27 over a cache that the new tokens were written to first.
+ * q-head j reads KV head j / (n_q / kv_heads).  With picked not NULL ([batch][q_len][kv_heads]
+ * [slots], as lf_int4_select writes it) only the tokens of those pages.  A query
+ * token that sees nothing gets zeros.  out as q, same dtype (F16 or BF16).
+ * workspace: lf_int4_workspace_bytes bytes, 16-byte aligned, zero before its first
+ * use and left so by every call; calls that overlap on the GPU need one each.
+ */
+LF_API int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q, int dtype, int64_t q_seq_stride,
+                          int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int32_t* lengths,
+                          const int32_t* counts, const int32_t* picked, int slots, float scaling, void* out, int64_t out_seq_stride,
+                          int64_t out_head_stride, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
+                          int32_t* status, lf_stream_t stream);
+LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);
+
 /* Human-readable text of a status code; detail of the last failure on this thread. */
 LF_API const char* lf_status_string(int status);
 LF_API const char* lf_last_error(void);

@@ -1,0 +1,483 @@
+"""A 4-bit paged Key/Value cache, attention over it, and attention over the
+pages that matter.
+
+The tiered cache of :mod:`logitfill_b200.packed` needs a Key policy from an
+offline calibration and stores Value at 2 bits.  This one needs none: Key and
+Value are both held at 4 bits, quantized token by token as they are written
+(an fp16 scale and minimum for every 32 channels: 5 bits per element in all),
+in 64-token pages that a page table orders into sequences.
+
+* :func:`int4_write` / :func:`int4_read` quantize tokens into the pages and
+  read them back;
+* :func:`int4_attention` attends query tokens over the cached tokens;
+* :func:`int4_select` scores a sequence's pages by a bound on their attention
+  scores and picks the best for each query token and KV head, and
+  :func:`int4_sparse_attention` attends over the picked pages only;
+* :class:`Int4KVCache` keeps the pools, the page table and the lengths of a
+  batch of sequences, for every layer of a model.
+
+The functions take the tensors themselves: ``pages`` int32 ``[n_pages, n_kv,
+20 * head_dim]`` (see ``include/logitfill_b200.h`` for the record),
+``page_table`` int32 ``[batch, width]``, lengths and positions int32
+``[batch]``, all on the GPU.  A page table entry outside the pool is never
+followed; with ``status`` (int32 ``[1]`` on the GPU) given, such an access sets
+it to a non-zero ``lf_status``.  Every launch goes to the current stream.
+There is no CPU or dense fallback; what the kernels do not implement raises
+``NotImplementedError``, malformed arguments ``ValueError``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from logitfill_b200 import _lib
+
+PAGE_TOKENS = 64   # tokens of a page
+GROUP = 32         # channels that share a scale and a minimum
+
+
+def record_words(head_dim: int) -> int:
+    """int32 words of one page and KV head."""
+    return 20 * int(head_dim)
+
+
+def bounds_bytes(head_dim: int) -> int:
+    """int8 entries of the bounds record of one page and KV head."""
+    return 2 * int(head_dim) + 16
+
+
+def alloc_pages(n_pages: int, n_kv: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """An empty pool (zeros) of ``n_pages`` pages."""
+    return torch.zeros(n_pages, n_kv, record_words(head_dim), dtype=torch.int32, device=device)
+
+
+def alloc_bounds(n_pages: int, n_kv: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Bounds records (zeros) of ``n_pages`` pages."""
+    return torch.zeros(n_pages, n_kv, bounds_bytes(head_dim), dtype=torch.int8, device=device)
+
+
+def _pool(pages: torch.Tensor, page_table: torch.Tensor):
+    """The C ABI's pool of ``pages`` and ``page_table``, and the head_dim."""
+    if pages.dim() != 3 or pages.dtype != torch.int32 or pages.stride(2) != 1:
+        raise ValueError(f"pages must be int32 [n_pages, n_kv, words] with word stride 1, got {pages.dtype} "
+                         f"{tuple(pages.shape)}")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+        raise ValueError(f"page_table must be int32 [batch, width] with entry stride 1, got {page_table.dtype} "
+                         f"{tuple(page_table.shape)}")
+    if not pages.is_cuda:
+        raise RuntimeError("the 4-bit cache needs CUDA tensors (there is no CPU path)")
+    if page_table.device != pages.device:
+        raise RuntimeError(f"page_table is on {page_table.device}, pages on {pages.device}")
+    n, H, words = pages.shape
+    if words % 20:
+        raise ValueError(f"a record of {words} words belongs to no head_dim (20 * head_dim words)")
+    B, W = page_table.shape
+    return _lib.LfInt4Pool(pages.data_ptr(), page_table.data_ptr(), pages.stride(0) if n > 1 else H * words,
+                           pages.stride(1) if H > 1 else words, page_table.stride(0) if B > 1 else W, W, n, H, B), words // 20
+
+
+def _per_sequence(name: str, t: torch.Tensor | None, batch: int, device) -> int:
+    """Address of an int32 [batch] tensor (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.shape != (batch,) or not (t.is_contiguous() and t.device == device):
+        raise ValueError(f"{name} must be a contiguous int32 [{batch}] tensor on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _status(t: torch.Tensor | None, device) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.numel() < 1 or t.device != device:
+        raise ValueError(f"status must be an int32 tensor on {device}")
+    return t.data_ptr()
+
+
+def _bounds(bounds: torch.Tensor, pages: torch.Tensor, head_dim: int):
+    n, H = pages.shape[0], pages.shape[1]
+    if (bounds.dtype != torch.int8 or bounds.dim() != 3 or bounds.shape[0] != n or bounds.shape[1] != H
+            or bounds.shape[2] < 2 * head_dim + 1 or bounds.stride(2) != 1 or bounds.device != pages.device):
+        raise ValueError(f"bounds must be int8 [{n}, {H}, {bounds_bytes(head_dim)}] on {pages.device}, got {bounds.dtype} "
+                         f"{tuple(bounds.shape)} on {bounds.device}")
+    return bounds.data_ptr(), bounds.stride(0) if n > 1 else H * bounds.shape[2], \
+        bounds.stride(1) if H > 1 else bounds.shape[2]
+
+
+def _aligned_rows(t: torch.Tensor):
+    """``t`` [B, H, T, D] with 16-byte aligned rows of channel stride 1 (a copy
+    where it is not), and its first three strides (0 where the extent is 1)."""
+    unit = 16 // t.element_size()
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in strides):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = list(t.stride()[:3])
+    return t, strides
+
+
+class _on:
+    """Makes ``device`` current for a launch (nothing to do when it is)."""
+
+    def __init__(self, device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor,
+               start: torch.Tensor, counts: torch.Tensor | None = None, bounds: torch.Tensor | None = None,
+               status: torch.Tensor | None = None) -> None:
+    """Quantize ``key``/``value`` ``[batch, n_kv, T, head_dim]`` (fp32, fp16 or
+    bf16, any strides) into the pages: token ``i`` of sequence ``b`` goes to
+    position ``start[b] + i``, for ``i < counts[b]`` (all ``T`` where ``counts``
+    is None).  With ``bounds`` given, the record of every page whose last slot
+    is written is brought up to date (a sparse call needs it).  A group of 32
+    channels whose scale or minimum is no finite fp16 number (a NaN, an
+    infinity, a range past 15 * 65504) reads back as NaN."""
+    pool, D = _pool(pages, page_table)
+    B, H = pool.batch, pool.kv_heads
+    if key.dim() != 4 or key.shape != value.shape or (key.shape[0], key.shape[1], key.shape[3]) != (B, H, D):
+        raise ValueError(f"key and value must be [{B}, {H}, T, {D}], got {tuple(key.shape)} and {tuple(value.shape)}")
+    if key.dtype != value.dtype:
+        raise ValueError(f"key is {key.dtype}, value {value.dtype}")
+    dev = pages.device
+    if key.device != dev or value.device != dev:
+        raise RuntimeError(f"key and value must be on {dev}")
+    code = _lib.dtype_code(key.dtype)
+    addresses = (_per_sequence("start", start, B, dev), _per_sequence("counts", counts, B, dev))
+    if key.shape[2] == 0:
+        return
+    key, ks = _aligned_rows(key)
+    value, vs = _aligned_rows(value)
+    bp, b0, b1 = (0, 0, 0) if bounds is None else _bounds(bounds, pages, D)
+    with _on(dev):
+        _lib.check(_lib.lib().lf_int4_write(
+            ctypes.byref(pool), D, key.data_ptr(), value.data_ptr(), code, *ks, *vs, key.shape[2],
+            *addresses, bp, b0, b1,
+            _status(status, dev), _lib.stream_handle(dev)), "lf_int4_write")
+
+
+def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor, tokens: int,
+              counts: torch.Tensor | None = None, dtype=torch.float32, status: torch.Tensor | None = None):
+    """Positions ``start[b] .. start[b] + tokens - 1`` of every sequence as Key and
+    Value ``[batch, n_kv, tokens, head_dim]`` in ``dtype`` (fp32, fp16 or
+    bf16); tokens ``i >= counts[b]`` are zeros."""
+    pool, D = _pool(pages, page_table)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"cannot read {tokens} tokens")
+    dev, code = pages.device, _lib.dtype_code(dtype)
+    out = torch.empty(2, pool.batch, pool.kv_heads, tokens, D, dtype=dtype, device=dev)
+    key, value = out.unbind(0)
+    addresses = (_per_sequence("start", start, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev))
+    if tokens:
+        with _on(dev):
+            _lib.check(_lib.lib().lf_int4_read(
+                ctypes.byref(pool), D, *addresses, tokens, key.data_ptr(), value.data_ptr(), code, _status(status, dev),
+                _lib.stream_handle(dev)), "lf_int4_read")
+    return key, value
+
+
+def int4_read_bounds(bounds: torch.Tensor) -> torch.Tensor:
+    """fp32 ``[n_pages, n_kv, 2, head_dim]`` of the bounds records: every Key
+    channel's upper, then its lower bound over a page's tokens."""
+    if bounds.dim() != 3 or bounds.dtype != torch.int8 or bounds.stride(2) != 1 or bounds.shape[2] % 2:
+        raise ValueError(f"bounds must be int8 [n_pages, n_kv, 2 * head_dim + 16], got {bounds.dtype} {tuple(bounds.shape)}")
+    if not bounds.is_cuda:
+        raise RuntimeError("the 4-bit cache needs CUDA tensors (there is no CPU path)")
+    n, H, width = bounds.shape
+    D = (width - 16) // 2
+    out = torch.empty(n, H, 2, D, dtype=torch.float32, device=bounds.device)
+    with _on(bounds.device):
+        _lib.check(_lib.lib().lf_int4_read_bounds(
+            bounds.data_ptr(), bounds.stride(0) if n > 1 else H * width, bounds.stride(1) if H > 1 else width, n, H, D,
+            out.data_ptr(), _lib.stream_handle(bounds.device)), "lf_int4_read_bounds")
+    return out
+
+
+_workspaces: dict = {}
+
+
+def _workspace(need: int, device) -> torch.Tensor:
+    """Scratch of an attention call, zero before its first use and left so by
+    every call.  Calls on one stream share one buffer (they run in order);
+    a call being captured in a CUDA graph gets its own, which the graph keeps
+    and clears, so replays on any stream do not meet."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(need, dtype=torch.uint8, device=device)
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < need:
+        ws = _workspaces[key] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
+    return ws
+
+
+def _query(query: torch.Tensor, pool, head_dim: int, device):
+    """The query as [B, n_q, q_len, D] with channel stride 1, checked."""
+    q = query.unsqueeze(2) if query.dim() == 3 else query
+    if q.dim() != 4 or q.shape[0] != pool.batch or q.shape[3] != head_dim or q.shape[1] < 1 or q.shape[2] < 1:
+        raise ValueError(f"query must be [{pool.batch}, n_q, {head_dim}] or [{pool.batch}, n_q, q_len, {head_dim}], got "
+                         f"{tuple(query.shape)}")
+    if q.shape[1] % pool.kv_heads:
+        raise ValueError(f"{q.shape[1]} query heads do not divide into {pool.kv_heads} KV heads")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"the 4-bit cache's attention takes fp16 or bf16 queries, got {q.dtype}")
+    if q.device != device:
+        raise RuntimeError(f"query is on {q.device}, pages on {device}")
+    return q if q.stride(3) == 1 else q.contiguous()
+
+
+def _attend(query, pages, page_table, lengths, scaling, counts, picked, out, status):
+    pool, D = _pool(pages, page_table)
+    dev = pages.device
+    q = _query(query, pool, D, dev)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride(-1) != 1:
+        raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} on {dev} with channel stride 1")
+    o = out.unsqueeze(2) if out.dim() == 3 else out
+    n_q, q_len = q.shape[1], q.shape[2]
+    slots = 0
+    if picked is not None:
+        if picked.dtype != torch.int32 or picked.shape[:-1] != (pool.batch, q_len, pool.kv_heads) \
+                or not picked.is_contiguous() or picked.device != dev:
+            raise ValueError(f"picked must be contiguous int32 [{pool.batch}, {q_len}, {pool.kv_heads}, slots] on {dev}, got "
+                             f"{picked.dtype} {tuple(picked.shape)} on {picked.device}")
+        slots = picked.shape[-1]
+    so = _lib.lib()
+    with _on(dev):
+        ws = _workspace(so.lf_int4_workspace_bytes(pool.batch, pool.kv_heads, n_q, q_len, D), dev)
+        _lib.check(so.lf_int4_attend(
+            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), q_len, n_q,
+            _per_sequence("lengths", lengths, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev),
+            _lib.ptr(picked), slots, float(scaling), o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), ws.data_ptr(),
+            ws.numel(), _status(status, dev), _lib.stream_handle(dev)), "lf_int4_attend")
+    return out
+
+
+def int4_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                   scaling: float, counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                   status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``query`` ``[batch, n_q, head_dim]`` (one token per
+    sequence) or ``[batch, n_q, q_len, head_dim]`` over the cached tokens, fp16
+    or bf16, in the query's shape and type.  ``lengths[b]`` tokens are cached,
+    the query's own among them (written first): query token ``i`` sees
+    positions ``0 .. lengths[b] - q_len + i``.  With ``counts`` (int32
+    ``[batch]``) sequence ``b`` has only its first ``counts[b]`` query tokens;
+    the others, and those that see nothing, get zeros."""
+    return _attend(query, pages, page_table, lengths, scaling, counts, None, out, status)
+
+
+def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
+                lengths: torch.Tensor, top_pages: int, sink_pages: int = 1, recent_pages: int = 2,
+                counts: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """The logical pages each query token and KV head reads in a sparse call:
+    int32 ``[batch, q_len, n_kv, sink + recent + top]``, ascending, -1 after the
+    last.  The first ``sink_pages`` and the last ``recent_pages`` (at least 1:
+    the page being filled) are always in; of the rest the ``top_pages`` with
+    the largest bound on the scores of the KV head's queries (summed over its
+    query heads; ties to the lower page)."""
+    pool, D = _pool(pages, page_table)
+    dev = pages.device
+    q = _query(query, pool, D, dev)
+    n_q, q_len = q.shape[1], q.shape[2]
+    top, sink, recent = int(top_pages), int(sink_pages), int(recent_pages)
+    if top < 0 or sink < 0 or recent < 1:
+        raise ValueError(f"top {top} and sink {sink} must not be negative, recent {recent} at least 1")
+    bp, b0, b1 = _bounds(bounds, pages, D)
+    picked = torch.empty(pool.batch, q_len, pool.kv_heads, sink + recent + top, dtype=torch.int32, device=dev)
+    with _on(dev):
+        _lib.check(_lib.lib().lf_int4_select(
+            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), q_len, n_q,
+            bp, b0, b1, _per_sequence("lengths", lengths, pool.batch, dev),
+            _per_sequence("counts", counts, pool.batch, dev), top, sink, recent, picked.data_ptr(), _status(status, dev),
+            _lib.stream_handle(dev)), "lf_int4_select")
+    return picked
+
+
+def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
+                          lengths: torch.Tensor, scaling: float, top_pages: int, sink_pages: int = 1,
+                          recent_pages: int = 2, counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                          status: torch.Tensor | None = None):
+    """:func:`int4_select`, then :func:`int4_attention` over the picked pages
+    only: ``(out, picked)``.  With ``sink + recent + top`` pages or fewer
+    visible, every page is read and the result is the dense one."""
+    picked = int4_select(query, pages, bounds, page_table, lengths, top_pages, sink_pages, recent_pages, counts, status)
+    return _attend(query, pages, page_table, lengths, scaling, counts, picked, out, status), picked
+
+
+class Int4KVCache:
+    """4-bit cache of ``batch`` sequences for ``n_layers`` layers: a pool of
+    ``n_pages`` 64-token pages per layer, shared by the sequences through one
+    page table (a sequence's token positions are the same in every layer).
+
+    A step is ``extend(counts)``, then for every layer ``write(layer, key,
+    value)`` and ``attend(layer, query, scaling)``: ``extend`` makes room for
+    the step's tokens, ``write`` stores them behind the tokens of the steps
+    before, ``attend`` sees both.  Pages come from a free list and go back with
+    ``release``.
+
+    Capturing a step in a CUDA graph: ``reserve`` pages for all tokens to come,
+    capture ``extend(n)`` (an int) with the rest of the step, and call
+    ``advance_host(n)`` for each replay."""
+
+    def __init__(self, n_layers: int, batch: int, n_q: int, n_kv: int, head_dim: int, n_pages: int,
+                 max_tokens: int, device="cuda", bounds: bool = True):
+        if n_q % n_kv:
+            raise ValueError("query heads must divide into KV heads")
+        if head_dim not in (64, 128):
+            raise NotImplementedError(f"the 4-bit cache takes head_dim 64 or 128, got {head_dim}")
+        if n_layers < 1 or batch < 1 or n_pages < 1 or max_tokens < 1:
+            raise ValueError("layers, batch, pages and max_tokens must be positive")
+        self.batch, self.n_q, self.n_kv, self.head_dim = int(batch), int(n_q), int(n_kv), int(head_dim)
+        self.n_pages = int(n_pages)
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.width = -(-int(max_tokens) // PAGE_TOKENS)
+        self.pages = [alloc_pages(n_pages, n_kv, head_dim, self.device) for _ in range(n_layers)]
+        self.bounds = [alloc_bounds(n_pages, n_kv, head_dim, self.device) for _ in range(n_layers)] if bounds else None
+        self.page_table = torch.full((batch, self.width), -1, dtype=torch.int32, device=self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        spans = torch.zeros(3, batch, dtype=torch.int32, device=self.device)
+        self.start, self.end, self.counts = spans.unbind(0)     # device: first new position, length, new tokens
+        self._spans = spans
+        self._table = np.full((batch, self.width), -1, np.int32)  # host, authoritative
+        self._owned = np.zeros(batch, np.int64)                   # pages each sequence holds
+        self._end = np.zeros(batch, np.int64)
+        self._start = np.zeros(batch, np.int64)
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def n_layers(self) -> int:
+        return len(self.pages)
+
+    @property
+    def lengths(self) -> np.ndarray:
+        """Tokens of each sequence, the current step's among them (host)."""
+        return self._end.copy()
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, tokens) -> None:
+        """Hold pages for ``tokens`` tokens in all (an int, or one per
+        sequence).  Raises ``RuntimeError`` when the pool has too few; nothing
+        changes then."""
+        want = -(-np.broadcast_to(np.asarray(tokens, np.int64), (self.batch,)) // PAGE_TOKENS)
+        if want.max(initial=0) > self.width:
+            raise ValueError(f"{int(np.max(tokens))} tokens exceed the cache's {self.width * PAGE_TOKENS} per sequence")
+        need = np.maximum(want - self._owned, 0)
+        if not need.any():
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("reserve the pages before the capture")
+        if need.sum() > len(self._free):
+            raise RuntimeError(f"{int(need.sum())} pages are needed, {len(self._free)} are free")
+        for b in np.flatnonzero(need):
+            for j in range(int(self._owned[b]), int(want[b])):
+                self._table[b, j] = self._free.pop()
+            self._owned[b] = want[b]
+        self._upload(self.page_table, self._table)
+
+    def _upload(self, device_tensor: torch.Tensor, host: np.ndarray) -> None:
+        # Pinned, non-blocking: ordered on the stream without stalling the host.
+        device_tensor.copy_(torch.from_numpy(host.astype(np.int32)).pin_memory(), non_blocking=True)
+
+    def extend(self, counts) -> None:
+        """Open a step of ``counts`` new tokens (an int, or one per sequence,
+        0 for a sequence that pauses) behind those of the step before."""
+        uniform = np.ndim(counts) == 0
+        n = np.broadcast_to(np.asarray(counts, np.int64), (self.batch,))
+        if (n < 0).any():
+            raise ValueError("counts must not be negative")
+        self.reserve(self._end + n)
+        if torch.cuda.is_current_stream_capturing():
+            if not uniform:
+                raise RuntimeError("a captured step takes the same number of tokens for every sequence")
+        else:
+            self._start, self._end = self._end, self._end + n
+            if not uniform:
+                self._upload(self._spans, np.stack([self._start, self._end, n]))
+                return
+        self.start.copy_(self.end)
+        self.end.add_(int(counts))
+        self.counts.fill_(int(counts))
+
+    def advance_host(self, count: int) -> None:
+        """Mirror one replay of a captured ``extend(count)`` in the host lengths."""
+        self._start, self._end = self._end, self._end + int(count)
+
+    def truncate(self, lengths) -> None:
+        """Drop the tokens past ``lengths`` (an int, or one per sequence), e.g.
+        rejected drafts; the pages stay with their sequences."""
+        n = np.broadcast_to(np.asarray(lengths, np.int64), (self.batch,))
+        if (n < 0).any() or (n > self._end).any():
+            raise ValueError("truncate() takes lengths between 0 and the present ones")
+        self._start, self._end = n.copy(), n.copy()
+        self._upload(self._spans, np.stack([self._start, self._end, np.zeros_like(n)]))
+
+    def release(self, seqs=None) -> None:
+        """Empty the sequences ``seqs`` (default: all) and return their pages."""
+        for b in range(self.batch) if seqs is None else seqs:
+            for j in range(int(self._owned[b]) - 1, -1, -1):
+                self._free.append(int(self._table[b, j]))
+            self._table[b, :] = -1
+            self._owned[b] = self._start[b] = self._end[b] = 0
+        self._upload(self.page_table, self._table)
+        self._upload(self._spans, np.stack([self._start, self._end, self._end - self._start]))
+
+    def write(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Store this step's tokens of one layer: ``[batch, n_kv, T, head_dim]``,
+        the first ``counts[b]`` of sequence ``b``."""
+        int4_write(key, value, self.pages[layer], self.page_table, self.start, self.counts,
+                   None if self.bounds is None else self.bounds[layer], self.status)
+
+    def read(self, layer: int, start: int = 0, stop: int | None = None, dtype=torch.float32):
+        """Positions ``start .. stop - 1`` (default: to the longest sequence's
+        end) of every sequence as ``[batch, n_kv, stop - start, head_dim]``;
+        zeros past a sequence's end."""
+        stop = int(self._end.max()) if stop is None else int(stop)
+        if start < 0 or stop < start:
+            raise ValueError(f"cannot read positions {start} .. {stop}")
+        first = torch.full_like(self.start, start)
+        return int4_read(self.pages[layer], self.page_table, first, stop - start, self.end - first, dtype, self.status)
+
+    def attend(self, layer: int, query: torch.Tensor, scaling: float, out: torch.Tensor | None = None) -> torch.Tensor:
+        """:func:`int4_attention` of this step's query tokens (the first
+        ``counts[b]`` of sequence ``b``)."""
+        self._check_heads(query)
+        return int4_attention(query, self.pages[layer], self.page_table, self.end, scaling, self.counts, out, self.status)
+
+    def attend_sparse(self, layer: int, query: torch.Tensor, scaling: float, top_pages: int, sink_pages: int = 1,
+                      recent_pages: int = 2, out: torch.Tensor | None = None):
+        """:func:`int4_sparse_attention` of this step's query tokens."""
+        self._check_heads(query)
+        if self.bounds is None:
+            raise RuntimeError("a sparse call needs a cache made with bounds=True")
+        return int4_sparse_attention(query, self.pages[layer], self.bounds[layer], self.page_table, self.end, scaling,
+                                     top_pages, sink_pages, recent_pages, self.counts, out, self.status)
+
+    def _check_heads(self, query: torch.Tensor) -> None:
+        if query.dim() < 3 or query.shape[1] != self.n_q:
+            raise ValueError(f"query must have {self.n_q} heads, got {tuple(query.shape)}")
+
+    def check_status(self) -> None:
+        """Raise if a kernel met a position outside its sequence's pages (synchronises)."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            _lib.check(code, "4-bit cache kernel")
+
+
+__all__ = ["PAGE_TOKENS", "GROUP", "record_words", "bounds_bytes", "alloc_pages", "alloc_bounds", "int4_write",
+           "int4_read", "int4_read_bounds", "int4_attention", "int4_select", "int4_sparse_attention", "Int4KVCache"]
