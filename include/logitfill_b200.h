@@ -418,8 +418,10 @@ LF_API int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void* q,
  * q-head j reads KV head j / (n_q / kv_heads).  With picked not NULL ([batch][q_len][kv_heads]
  * [slots], as lf_int4_select writes it) only the tokens of those pages.  A query
  * token that sees nothing gets zeros.  out as q, same dtype (F16 or BF16).
- * workspace: lf_int4_workspace_bytes bytes, 16-byte aligned, zero before its first
- * use and left so by every call; calls that overlap on the GPU need one each.
+ * q rows 16-byte aligned.  workspace: lf_int4_workspace_bytes bytes (of the
+ * current device), 16-byte aligned, zero from byte lf_int4_workspace_clear_from on
+ * before its first use and left so by every call, of any shape; calls that
+ * overlap on the GPU need one each.
  */
 LF_API int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q, int dtype, int64_t q_seq_stride,
                           int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int32_t* lengths,
@@ -427,6 +429,7 @@ LF_API int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q,
                           int64_t out_head_stride, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
                           int32_t* status, lf_stream_t stream);
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);
+LF_API size_t lf_int4_workspace_clear_from(void);
 
 /* Human-readable text of a status code; detail of the last failure on this thread. */
 LF_API const char* lf_status_string(int status);

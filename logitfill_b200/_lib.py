@@ -21,7 +21,7 @@ EXPORTS = (
     "lf_decode", "lf_decode_multi", "lf_decode_max_splits_multi", "lf_commit_token", "lf_selftest_wait", "lf_selftest_divide",
     "lf_ipc_alloc", "lf_ipc_free", "lf_ipc_handle", "lf_ipc_open", "lf_ipc_close", "lf_decode_merge_gather",
     "lf_gather_signals", "lf_gather_wait", "lf_int4_write", "lf_int4_read", "lf_int4_read_bounds", "lf_int4_select",
-    "lf_int4_attend", "lf_int4_workspace_bytes", "lf_status_string", "lf_last_error",
+    "lf_int4_attend", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from", "lf_status_string", "lf_last_error",
 )
 
 
@@ -104,6 +104,7 @@ def lib() -> ctypes.CDLL:
                                    P, P, c_int, c_int, c_int, P, P, P]),
         "lf_int4_attend": (c_int, [Q, c_int, P, c_int, c_int64, c_int64, c_int64, c_int, c_int, P, P, P, c_int,
                                    c_float, P, c_int64, c_int64, c_int64, P, c_size_t, P, P]),
+        "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
         "lf_status_string": (c_char_p, [c_int]),
         "lf_last_error": (c_char_p, []),

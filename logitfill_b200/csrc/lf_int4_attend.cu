@@ -1,9 +1,34 @@
 // Attention over the 4-bit paged cache (lf_int4_attend): dense over a
 // sequence's pages, or over a list of picked ones.
 //
-// One CTA per (q-head, query token, sequence), one pass over its pages with a
-// running maximum and sum: two threads per token form the scores of a page,
-// one thread per channel sums the Values.
+// Mathematics.  A unit is one KV head of one sequence (of one query token in a
+// sparse call) with up to 8 NT query columns (q-head, query token).  With codes
+// c, scales s and minima z per token and group G of 32 channels,
+//   score[k][col] = sum_G s_kG * (sum_{d in G} c_kd q_d) + sum_G z_kG * (sum_{d in G} q_d)
+//   out[col][d]   = sum_k p_k (c_kd s_kG + z_kG)
+// Keys: the tensor cores multiply the raw codes.  A nibble needs no conversion:
+// in the fp16 pair w & 0x000f000f each half is the subnormal code * 2^-24, in
+// w & 0x00f000f0 it is 16 code * 2^-24, and m16n8k16 takes subnormals exactly.
+// The queries are scaled by a power of two per column (and 1/16 for the odd
+// nibbles), so a bf16 or fp16 query enters exactly; products are summed in fp32.
+// Values: code * s + z is rounded once to fp16 (one fma on the exact code), and
+// so is p: each costs 2^-11 of a token's share p |value| at most, below the
+// output's own rounding.  (Multiplying raw codes by p s instead would round a
+// number that may be many times p |value|.)
+//
+// The work is one pass over the pages with a running maximum and sum.  The
+// maximum is moved only when a score passes it by 2^8 (p <= 2^8 fits), so most
+// tiles skip the rescaling.
+//
+// Split.  All pages of all units form one line, cut into equal ranges, one per
+// CTA (the lengths are read on the device, so nothing is planned on the host).
+// Each of a CTA's four warps takes 16 tokens of every page of the range through
+// its own ring of cp.async stages: no barrier until the range's end.  A unit
+// that lies in one range is finished there; otherwise each CTA leaves a partial
+// (maximum, sum, accumulator) and the last one to arrive (an atomic ticket)
+// merges them in the order of the ranges, so results do not depend on timing.
+#include <type_traits>
+
 #include "lf_int4.cuh"
 
 namespace lf {
@@ -19,87 +44,676 @@ struct AttendParams {
   float scale_log2;
   void* out;
   int64_t out_seq, out_head, out_tok;
+  int rows, cols, col_tiles;  // sequences (or query tokens), query columns of a unit, column tiles
+  float* partials;
+  uint32_t* tickets;
   int32_t* status;
 };
 
-constexpr int kAttendThreads = 128;
+constexpr int kAttendWarps = 4;
+constexpr int kAttendThreads = 32 * kAttendWarps;
+constexpr int kTile = kInt4Page / kAttendWarps;  // tokens of a page that one warp takes
+constexpr float kSlack = 8.0f;                   // log2 a score may pass the running maximum by
+constexpr float kNoMax = -1e30f;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttendThreads) int4_attend_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ float q_s[D], p_s[kInt4Page];
-  const int head = blockIdx.x, i = blockIdx.y, b = blockIdx.z, h = head / p.group, tid = threadIdx.x;
-  const int seen = int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i);
-  const T* q = static_cast<const T*>(p.q) + b * p.q_seq + head * p.q_head + i * p.q_tok;
-  if (tid < D) q_s[tid] = Scalar<T>::load(q + tid) * p.scale_log2;
-  __syncthreads();
-  const int n = (seen + kInt4Page - 1) / kInt4Page;
-  const int32_t* picked =
-      p.picked == nullptr ? nullptr : p.picked + ((static_cast<int64_t>(b) * p.q_len + i) * p.pool.kv_heads + h) * p.slots;
-  const int todo = picked == nullptr ? n : p.slots;
-  float m = -1e30f, l = 0.0f, acc = 0.0f;
-  for (int s = 0; s < todo; ++s) {
-    const int page = picked == nullptr ? s : picked[s];
-    if (page < 0 || page >= n) continue;
-    const int id = int4_page_id(p.pool, b, page);
-    if (id < 0) {
-      if (tid == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
-      continue;
-    }
-    const uint32_t* rec = reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
-    const int k = tid >> 1, half = tid & 1;
-    float dot = 0.0f;
-    for (int w = half * (D / 16); w < (half + 1) * (D / 16); ++w) {
-      const int t = w / (D / 32), G = w % (D / 32);
-      const uint32_t c = rec[k * (D / 8) + w], kp = rec[8 * D + k * (D / 32) + G];
-      for (int x = 0; x < 8; ++x)
-        dot += q_s[32 * G + 8 * t + x] * fmaf(static_cast<float>((c >> (4 * x)) & 15u), half_lo(kp), half_hi(kp));
-    }
-    dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-    if (page * kInt4Page + k >= seen) dot = -INFINITY;
-    __syncthreads();
-    if (half == 0) p_s[k] = dot;
-    __syncthreads();
-    float top = m;
-    for (int x = 0; x < kInt4Page; ++x) top = fmaxf(top, p_s[x]);
-    const float fix = exp2f(m - top);
-    m = top;
-    l *= fix;
-    acc *= fix;
-    const int w = (tid % D) >> 6, u = (tid >> 5) & 1, g = (tid & 31) >> 2, x = tid & 3, G = (tid % D) >> 5;
-    for (int tok = 0; tok < min(kInt4Page, seen - page * kInt4Page); ++tok) {
-      const float pr = exp2f(p_s[tok] - m);
-      l += pr;
-      const uint32_t c = rec[10 * D + (tok >> 3) * D + g * (D / 8) + ((tok & 7) >> 1) * (D / 32) + (tok & 1) * (D / 64) + w];
-      const uint32_t vp = rec[18 * D + tok * (D / 32) + G];
-      acc += pr * fmaf(static_cast<float>((c >> (4 * (4 * u + x))) & 15u), half_lo(vp), half_hi(vp));
-    }
-  }
-  T* out = static_cast<T*>(p.out) + b * p.out_seq + head * p.out_head + i * p.out_tok;
-  if (tid < D) Scalar<T>::store(out + tid, l == 0.0f ? 0.0f : acc / l);
+template <int D, int NT> struct AttendCfg {
+  static constexpr int kStages = D == 128 ? 6 : 10;
+  static constexpr int kCtas = NT == 1 ? 3 : 2;
+  static constexpr int kTileBytes = kTile * (D + D / 4);
+  static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
+  static constexpr int kRing = kAttendWarps * kStages * kTileBytes;
+  static constexpr int kMerge = kAttendWarps * 8 * NT * (kPad + 2) * 4;
+  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T>
-static int launch_attend(const AttendParams& p, int D, cudaStream_t stream) {
-  const dim3 grid(p.group * p.pool.kv_heads, p.q_len, p.pool.batch);
-  if (D == 128)
-    int4_attend_kernel<T, 128><<<grid, kAttendThreads, 0, stream>>>(p);
-  else
-    int4_attend_kernel<T, 64><<<grid, kAttendThreads, 0, stream>>>(p);
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Codes of bits 0-3 (4-7) of both halves as exact fp16 numbers: 1024 + c (+ 16 c)
+// by its bit pattern, brought back by one fma.
+__device__ __forceinline__ uint32_t even_code(uint32_t x) {
+  return hfma2((x & 0x000f000fu) | 0x64006400u, 0x3C003C00u, 0xE400E400u);  // * 1 - 1024
+}
+__device__ __forceinline__ uint32_t odd_code(uint32_t x) {
+  return hfma2((x & 0x00f000f0u) | 0x64006400u, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
+}
+__device__ __forceinline__ bool is_nan_param(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
+// Scale above 2048 or |minimum| of 2^15 and more.
+__device__ __forceinline__ bool is_wide_param(uint32_t w) {
+  return (w & 0x7FFFu) > 0x6800u || (w & 0x7FFF0000u) >= 0x78000000u;
+}
+// Parameter words of token k of a warp's tile.
+template <int kG>
+__device__ __forceinline__ void load_params(const uint8_t* par, int k, uint32_t (&w)[kG]) {
+  if constexpr (kG == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(par + k * 16);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(par + k * 8);
+    w[0] = x.x; w[1] = x.y;
+  }
+}
+
+// Tokens that row r (a sequence, or a query token of one) sees at most.
+template <bool kSparse>
+__device__ __forceinline__ int row_tokens(const AttendParams& p, int r) {
+  const int b = kSparse ? r / p.q_len : r;
+  const int length = p.lengths[b], count = p.counts != nullptr ? p.counts[b] : p.q_len;
+  return int4_seen(length, count, kSparse ? r - b * p.q_len : max(0, min(count, p.q_len) - 1));
+}
+// Pages of a row that sees `tokens`, at least 1, so that an empty row is visited
+// and zeroed.
+template <bool kSparse>
+__device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
+  const int n = tokens / kInt4Page + (tokens % kInt4Page != 0);
+  return max(1, min(n, kSparse ? p.slots : p.pool.table_width));
+}
+
+template <typename T, int D, int NT, bool kSparse>
+__global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
+    int4_attend_kernel(const __grid_constant__ AttendParams p) {
+  using C = AttendCfg<D, NT>;
+  constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int meta_s[kAttendWarps][kStages];  // first token of each stage's page, -1: nothing to do
+  __shared__ float weight_s[kAttendWarps][kCol], top_s[kCol], sum_s[kCol];
+  __shared__ int last_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int per_row = p.pool.kv_heads * p.col_tiles;
+
+  // The line of pages: its length, and the row where this CTA's range begins.
+  int total = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += 32) {
+    const int n = r0 + lane < p.rows ? row_pages<kSparse>(p, row_tokens<kSparse>(p, r0 + lane)) * per_row : 0;
+    total += __reduce_add_sync(0xffffffffu, n);
+  }
+  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int begin = blockIdx.x * per, end = min(total, begin + per);
+  if (begin >= end) return;
+  int row = 0, row_base = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += 32) {
+    const int n = r0 + lane < p.rows ? row_pages<kSparse>(p, row_tokens<kSparse>(p, r0 + lane)) * per_row : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, row_base + upto > begin);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      row = r0 + l;
+      row_base += __shfl_sync(0xffffffffu, upto - n, l);
+      break;
+    }
+    row_base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+
+  uint8_t* ring = smem + warp * kStages * C::kTileBytes;
+  const uint32_t ring_a = smem_addr(ring);
+  int at = begin;
+  while (at < end) {
+    // ------------------------------------------------------------ one unit
+    const int seen_max = row_tokens<kSparse>(p, row), n_pages = row_pages<kSparse>(p, seen_max);
+    const int in_row = at - row_base, unit_in_row = in_row / n_pages;
+    const int unit_begin = row_base + unit_in_row * n_pages, unit_end = unit_begin + n_pages;
+    const int h = unit_in_row / p.col_tiles, c0 = (unit_in_row - h * p.col_tiles) * kCol;
+    const int first = at - unit_begin, stop = min(end, unit_end) - unit_begin;
+    const int b = kSparse ? row / p.q_len : row;
+    const int i0 = kSparse ? row - b * p.q_len : 0;
+    const int length = p.lengths[b], count = p.counts != nullptr ? p.counts[b] : p.q_len;
+    if (tid == 0 && p.status != nullptr && (seen_max - 1) / kInt4Page >= p.pool.table_width)
+      atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+
+    // Page ids of 32 pages at a time, one per lane, loaded a window ahead.
+    auto load_ids = [&](int j0, int& id, int& logical) {
+      const int j = j0 + lane;
+      id = logical = -1;
+      if (j < stop) {
+        logical = j;
+        if constexpr (kSparse)
+          logical = p.picked[(static_cast<int64_t>(row) * p.pool.kv_heads + h) * p.slots + j];
+        if (logical >= 0 && static_cast<int64_t>(logical) * kInt4Page < seen_max) {
+          id = int4_page_id(p.pool, b, logical);
+          if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+        }
+      }
+    };
+    int ids, logicals, ids_next, logicals_next;
+    load_ids(first, ids, logicals);
+    load_ids(first + 32, ids_next, logicals_next);
+    int window = first;
+    auto issue = [&](int j) {
+      if (j < stop) {
+        if (j - window == 32) {
+          window += 32;
+          ids = ids_next;
+          logicals = logicals_next;
+          load_ids(window + 32, ids_next, logicals_next);
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, j - window);
+        const int logical = __shfl_sync(0xffffffffu, logicals, j - window);
+        const int st = (j - first) % kStages;
+        if (lane == 0) meta_s[warp][st] = id < 0 ? -1 : logical * kInt4Page + warp * kTile;
+        if (id >= 0) {
+          const uint8_t* rec = reinterpret_cast<const uint8_t*>(p.pool.words + int4_record(p.pool, id, h));
+          const uint32_t dst = ring_a + st * C::kTileBytes;
+          constexpr int kCodes = kTile * D / 2, kPar = kTile * D / 8;  // bytes of one warp's tile
+          const uint8_t* kc = rec + warp * kCodes + lane * 16;
+#pragma unroll
+          for (int x = 0; x < kCodes / 512; ++x) {
+            cp_async16(dst + lane * 16 + x * 512, kc + x * 512);
+            cp_async16(dst + kCodes + lane * 16 + x * 512, kc + 40 * D + x * 512);
+          }
+          constexpr int kParLanes = kPar / 16;
+          if (lane < 2 * kParLanes) {
+            const int v = lane / kParLanes;
+            cp_async16(dst + 2 * kCodes + lane * 16, rec + 32 * D + v * 40 * D + warp * kPar + (lane - v * kParLanes) * 16);
+          }
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(first + s);
+
+    // Query fragments, sums and scales of this unit's columns.
+    uint32_t qf[NT][2 * kG][2], qz[NT];
+    float c2[NT][2];
+    int vis[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = c0 + nt * 8 + g, i = c / p.group;
+      const bool live = c < p.cols;
+      const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (h * p.group + c - i * p.group) * p.q_head + (i0 + i) * p.q_tok;
+      float x[kG][8], most = 0.0f;
+#pragma unroll
+      for (int G = 0; G < kG; ++G) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (live) w = *reinterpret_cast<const uint4*>(q + 32 * G + 8 * t);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+            x[G][2 * k] = half_lo(v[k]);
+            x[G][2 * k + 1] = half_hi(v[k]);
+          } else {
+            x[G][2 * k] = __uint_as_float(v[k] << 16);
+            x[G][2 * k + 1] = __uint_as_float(v[k] & 0xFFFF0000u);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[G][k]));
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // 2^kq brings the column's largest magnitude to [2^13, 2^14)
+      const int kq = most > 0.0f && most < INFINITY
+                         ? max(-100, min(100, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127)))
+                         : 0;
+      const float up = pow2(kq);
+      float sums[kG];
+#pragma unroll
+      for (int G = 0; G < kG; ++G) {
+        sums[G] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          sums[G] += x[G][k];
+          x[G][k] *= up;
+        }
+        sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 1);
+        sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 2);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          qf[nt][2 * G + k][0] = pack_half2(x[G][2 * k], x[G][2 * k + 4]);
+          qf[nt][2 * G + k][1] = pack_half2(x[G][2 * k + 1] * 0.0625f, x[G][2 * k + 5] * 0.0625f);
+        }
+      }
+      // The column's sum over group t's channels as two fp16 limbs (22 bits).
+      float mine = 0.0f;
+#pragma unroll
+      for (int G = 0; G < kG; ++G) mine = t == G ? sums[G] : mine;
+      mine *= pow2(kq - 10);
+      const float hi = __half2float(__float2half_rn(mine));
+      qz[nt] = pack_half2(hi, mine - hi);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int kc = __shfl_sync(0xffffffffu, kq, (2 * t + k) * 4);
+        c2[nt][k] = pow2(10 - kc) * p.scale_log2;
+        const int col = min(c0 + nt * 8 + 2 * t + k, p.cols - 1);
+        vis[nt][k] = int4_seen(length, count, i0 + col / p.group);
+      }
+    }
+    int vis_min = INT32_MAX;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) vis_min = min(vis_min, min(vis[nt][0], vis[nt][1]));
+    vis_min = __reduce_min_sync(0xffffffffu, vis_min);
+
+    float acc[NT][2 * kG][4], m[NT][2], l[NT][2];
+    float big = 1.0f;  // 1/32 once a Value past the fp16 range may have been met
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        m[nt][k] = kNoMax;
+        l[nt][k] = 0.0f;
+      }
+#pragma unroll
+      for (int x = 0; x < 2 * kG; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[nt][x][k] = 0.0f;
+    }
+
+    // ------------------------------------------------------- its pages
+    int st = 0;
+    for (int j = first; j < stop; ++j) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      issue(j + kStages - 1);
+      const int base = meta_s[warp][st];
+      const uint8_t* tile = ring + st * C::kTileBytes;
+      st = st + 1 == kStages ? 0 : st + 1;
+      if (base < 0 || base >= seen_max) continue;
+      constexpr int kCodes = kTile * D / 2, kPar = kTile * D / 8;
+      const uint8_t *kcode = tile, *vcode = tile + kCodes, *kpar = tile + 2 * kCodes, *vpar = kpar + kPar;
+
+      // Scores of 16 tokens (rows g and g + 8 of the fragment).
+      uint32_t kw[2][kG], ks[2][kG], kz[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (D == 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kcode + r * 512 + lane * 16);
+          const uint4 s = *reinterpret_cast<const uint4*>(kpar + (8 * r + g) * 16);
+          kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
+          ks[r][0] = s.x; ks[r][1] = s.y; ks[r][2] = s.z; ks[r][3] = s.w;
+          kz[r] = *reinterpret_cast<const uint32_t*>(kpar + r * 128 + lane * 4);
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(kcode + r * 256 + lane * 8);
+          const uint2 s = *reinterpret_cast<const uint2*>(kpar + (8 * r + g) * 8);
+          kw[r][0] = w.x; kw[r][1] = w.y;
+          ks[r][0] = s.x; ks[r][1] = s.y;
+          kz[r] = t < kG ? *reinterpret_cast<const uint32_t*>(kpar + (8 * r + g) * 8 + t * 4) : 0u;
+        }
+        kz[r] = __byte_perm(kz[r], 0, 0x3232);
+      }
+      float sc[NT][4], dot[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sc[nt][k] = dot[nt][k] = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma1688(sc[nt], kz[0], kz[1], qz[nt]);
+#pragma unroll
+      for (int G = 0; G < kG; ++G) {
+        const uint32_t a[2][2] = {{kw[0][G], kw[1][G]}, {kw[0][G] >> 8, kw[1][G] >> 8}};
+        const float s0 = half_lo(ks[0][G]), s1 = half_lo(ks[1][G]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            mma16816(d, a[k][0] & 0x000f000fu, a[k][1] & 0x000f000fu, a[k][0] & 0x00f000f0u, a[k][1] & 0x00f000f0u,
+                     qf[nt][2 * G + k][0], qf[nt][2 * G + k][1]);
+          dot[nt][0] = fmaf(d[0], s0, dot[nt][0]);
+          dot[nt][1] = fmaf(d[1], s0, dot[nt][1]);
+          dot[nt][2] = fmaf(d[2], s1, dot[nt][2]);
+          dot[nt][3] = fmaf(d[3], s1, dot[nt][3]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sc[nt][k] = fmaf(dot[nt][k], 16384.0f, sc[nt][k]) * c2[nt][k & 1];
+
+      // Scales and minima of this lane's four tokens, 2t and 2t + 1 of each half.
+      uint32_t vp[2][2][kG];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) load_params<kG>(vpar, 8 * r + 2 * t + o, vp[r][o]);
+
+      const bool masked = base + kTile > vis_min;
+      if (masked) {
+        // Tokens that not every column sees.  What an unwritten slot holds must
+        // not be read; a NaN that only some columns see goes to those columns'
+        // weights, so that it does not reach the others through the product.
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int tok = base + g + 8 * r;
+          bool nan = false;
+          if (tok >= vis_min && tok < seen_max) {
+            uint32_t w[kG];
+            load_params<kG>(vpar, g + 8 * r, w);
+#pragma unroll
+            for (int G = 0; G < kG; ++G) nan |= is_nan_param(w[G]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if (nan) sc[nt][2 * r + k] = NAN;
+              if (tok >= vis[nt][k]) sc[nt][2 * r + k] = -INFINITY;
+            }
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const int mine = base + 8 * r + 2 * t + o;
+#pragma unroll
+            for (int G = 0; G < kG; ++G)
+              if (mine >= seen_max || (mine >= vis_min && is_nan_param(vp[r][o][G]))) vp[r][o][G] = 0;
+          }
+        }
+      }
+
+      // The running maxima, where a score passes one by the slack.
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) move |= sc[nt][k] > m[nt][k & 1] + kSlack;
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float fix[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(sc[nt][k], sc[nt][k + 2]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m[nt][k]);
+            fix[k] = ex2(m[nt][k] - top);
+            m[nt][k] = top;
+            l[nt][k] *= fix[k];
+          }
+#pragma unroll
+          for (int x = 0; x < 2 * kG; ++x)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[nt][x][k] *= fix[k & 1];
+        }
+      }
+      uint32_t pb[NT][2];  // weights as the product's B operand: columns by tokens
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float pr[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          pr[k] = ex2(sc[nt][k] - m[nt][k & 1]);
+          l[nt][k & 1] += pr[k];
+        }
+        pb[nt][0] = transpose8x8(pack_half2(pr[0], pr[1]));
+        pb[nt][1] = transpose8x8(pack_half2(pr[2], pr[3]));
+      }
+
+      // Values past the fp16 range (a scale above 2048 or a minimum above 2^15 in
+      // magnitude can give one) are held at 1/32, from the first such tile on.
+      bool wide = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+          for (int G = 0; G < kG; ++G) wide |= G % 2 == (g & 1) && is_wide_param(vp[r][o][G]);
+      if (big != 1.0f || __any_sync(0xffffffffu, wide)) {
+        if (big == 1.0f) {
+          big = 0.03125f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2 * kG; ++x)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[nt][x][k] *= 0.03125f;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int G = 0; G < kG; ++G) vp[r][o][G] = hmul2(vp[r][o][G], 0x28002800u);
+      }
+
+      // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half.
+      uint32_t vw[2][2][D / 64];  // half, even/odd token, word
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (D == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vcode + r * 512 + lane * 16);
+          vw[r][0][0] = x.x; vw[r][0][1] = x.y; vw[r][1][0] = x.z; vw[r][1][1] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(vcode + r * 256 + lane * 8);
+          vw[r][0][0] = x.x; vw[r][1][0] = x.y;
+        }
+      }
+#pragma unroll
+      for (int G = 0; G < kG; ++G) {
+        uint32_t v[2][4];  // half, channel 4 g + n of the group
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t s = __byte_perm(vp[r][0][G], vp[r][1][G], 0x5410), z = __byte_perm(vp[r][0][G], vp[r][1][G], 0x7632);
+          const uint32_t x = __byte_perm(vw[r][0][G >> 1], vw[r][1][G >> 1], (G & 1) ? 0x7632 : 0x5410);
+          v[r][0] = hfma2(even_code(x), s, z);
+          v[r][1] = hfma2(odd_code(x), s, z);
+          v[r][2] = hfma2(even_code(x >> 8), s, z);
+          v[r][3] = hfma2(odd_code(x >> 8), s, z);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][0], pb[nt][1]);
+          mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][0], pb[nt][1]);
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();  // the rings are free: the merge buffer takes their place
+
+    // ---------------------------------------- the four warps' results, merged
+    float* merge = reinterpret_cast<float*>(smem);
+    float* top_w = merge + kAttendWarps * kCol * C::kPad;
+    float* sum_w = top_w + kAttendWarps * kCol;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float sum = l[nt][k];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int col = warp * kCol + nt * 8 + 2 * t + k;
+        if (g == 0) {
+          top_w[col] = m[nt][k];
+          sum_w[col] = sum;
+        }
+        const float back = big == 1.0f ? 1.0f : 32.0f;
+#pragma unroll
+        for (int G = 0; G < kG; ++G)
+          *reinterpret_cast<float4*>(merge + col * C::kPad + 32 * G + 4 * g) =
+              make_float4(acc[nt][2 * G][k] * back, acc[nt][2 * G][k + 2] * back, acc[nt][2 * G + 1][k] * back,
+                          acc[nt][2 * G + 1][k + 2] * back);
+      }
+    __syncthreads();
+    if (tid < kCol) {
+      float top = top_w[tid], sum = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kAttendWarps; ++w) top = fmaxf(top, top_w[w * kCol + tid]);
+#pragma unroll
+      for (int w = 0; w < kAttendWarps; ++w) {
+        const float f = ex2(top_w[w * kCol + tid] - top);
+        weight_s[w][tid] = f;
+        sum = fmaf(f, sum_w[w * kCol + tid], sum);
+      }
+      top_s[tid] = top;
+      sum_s[tid] = sum;
+    }
+    __syncthreads();
+
+    const bool whole = first == 0 && stop == n_pages;
+    T* out = static_cast<T*>(p.out) + b * p.out_seq;
+    auto store = [&](int col, int d, float4 v, float inv) {
+      const int c = c0 + col, i = c / p.group;
+      if (c >= p.cols) return;
+      T* o = out + (h * p.group + c - i * p.group) * p.out_head + (i0 + i) * p.out_tok + d;
+      Scalar<T>::store(o, v.x * inv);
+      Scalar<T>::store(o + 1, v.y * inv);
+      Scalar<T>::store(o + 2, v.z * inv);
+      Scalar<T>::store(o + 3, v.w * inv);
+    };
+    // The partial of range x of this unit: the range that begins inside the unit
+    // uses its CTA's first record, the unit's first range the second.
+    const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per;
+    auto record = [&](int x) { return p.partials + (2 * static_cast<int64_t>(x) + (x == first_cta)) * C::kRecord; };
+    float* mine = record(blockIdx.x);
+    for (int item = tid; item < kCol * D / 4; item += kAttendThreads) {
+      const int col = item / (D / 4), d = item % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kAttendWarps; ++w) {
+        const float f = weight_s[w][col];
+        const float4 x = *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d);
+        v.x = fmaf(f, x.x, v.x);
+        v.y = fmaf(f, x.y, v.y);
+        v.z = fmaf(f, x.z, v.z);
+        v.w = fmaf(f, x.w, v.w);
+      }
+      if (whole) {
+        const float sum = sum_s[col];
+        store(col, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+      } else {
+        *reinterpret_cast<float4*>(mine + 2 * kCol + col * D + d) = v;
+      }
+    }
+    if (!whole) {
+      if (tid < kCol) {
+        mine[tid] = top_s[tid];
+        mine[kCol + tid] = sum_s[tid];
+      }
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const uint32_t parts = last_cta - first_cta + 1;
+        uint32_t* ticket = p.tickets + static_cast<int64_t>(row) * per_row + unit_in_row;
+        const uint32_t n = atomicAdd(ticket, 1u) + 1;
+        if (n == parts) *ticket = 0;  // every range has arrived: ready for the next call
+        last_s = n == parts;
+      }
+      __syncthreads();
+      if (last_s) {
+        __threadfence();
+        for (int item = tid; item < kCol * D / 4; item += kAttendThreads) {
+          const int col = item / (D / 4), d = item % (D / 4) * 4;
+          float top = kNoMax, sum = 0.0f;
+          for (int x = first_cta; x <= last_cta; ++x) top = fmaxf(top, __ldcg(record(x) + col));
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int x = first_cta; x <= last_cta; ++x) {
+            const float* rec = record(x);
+            const float f = ex2(__ldcg(rec + col) - top);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
+            sum = fmaf(f, __ldcg(rec + kCol + col), sum);
+            v.x = fmaf(f, y.x, v.x);
+            v.y = fmaf(f, y.y, v.y);
+            v.z = fmaf(f, y.z, v.z);
+            v.w = fmaf(f, y.w, v.w);
+          }
+          store(col, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+        }
+      }
+    }
+    at = unit_begin + stop;
+    if (at - row_base == n_pages * per_row) {
+      row_base = at;
+      ++row;
+    }
+    __syncthreads();  // the merge buffer is free for the next unit's stages
+  }
+}
+
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return n;
+}
+// The partials: two records per CTA of the largest grid (the records of 16 columns are twice those of 8).
+static size_t partial_bytes(int sms) {
+  return static_cast<size_t>(sms) * 2 * AttendCfg<128, 2>::kCtas * AttendCfg<128, 2>::kRecord * sizeof(float);
+}
+static_assert(AttendCfg<128, 2>::kCtas * AttendCfg<128, 2>::kRecord >= AttendCfg<128, 1>::kCtas * AttendCfg<128, 1>::kRecord,
+              "the partials of every variant fit");
+
+template <typename T, int D, int NT, bool kSparse>
+static int launch_attend(const AttendParams& p, int sms, cudaStream_t stream) {
+  using C = AttendCfg<D, NT>;
+  auto kern = int4_attend_kernel<T, D, NT, kSparse>;
+  if (raise_smem_limit(reinterpret_cast<const void*>(kern), C::kSmem, true) != cudaSuccess)
+    return launch_status("lf_int4_attend");
+  // No more CTAs than pages there can be.
+  const int64_t most = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles * (kSparse ? p.slots : p.pool.table_width);
+  const int grid = static_cast<int>(most < static_cast<int64_t>(sms) * C::kCtas ? most : static_cast<int64_t>(sms) * C::kCtas);
+  kern<<<grid, kAttendThreads, C::kSmem, stream>>>(p);
   return launch_status("lf_int4_attend");
 }
+template <typename T, int D>
+static int launch_attend_by(const AttendParams& p, int sms, cudaStream_t stream) {
+  if (p.cols <= 8)
+    return p.picked ? launch_attend<T, D, 1, true>(p, sms, stream) : launch_attend<T, D, 1, false>(p, sms, stream);
+  return p.picked ? launch_attend<T, D, 2, true>(p, sms, stream) : launch_attend<T, D, 2, false>(p, sms, stream);
+}
+static int tile_columns(int cols) { return cols <= 8 ? 8 : 16; }
 
 }  // namespace lf
 
+extern "C" size_t lf_int4_workspace_clear_from(void) { return lf::partial_bytes(lf::sm_count()); }
+
 extern "C" size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim) {
-  if (batch <= 0 || kv_heads <= 0 || n_q <= 0 || q_len <= 0 || head_dim <= 0) return 0;
-  return 16;
+  if (batch <= 0 || kv_heads <= 0 || n_q < kv_heads || q_len <= 0 || head_dim <= 0) return 0;
+  // one ticket per unit: the dense and the sparse call's units, whichever are more
+  const int64_t group = n_q / kv_heads;
+  const int64_t dense = (group * q_len + 15) / 16, sparse = (group + 15) / 16 * q_len;
+  const int64_t units = static_cast<int64_t>(batch) * kv_heads * (dense > sparse ? dense : sparse);
+  return lf::partial_bytes(lf::sm_count()) + (static_cast<size_t>(units) * 4 + 15) / 16 * 16;
 }
 
 extern "C" int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q, int dtype, int64_t q_seq_stride,
                               int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int32_t* lengths,
-                              const int32_t* counts, const int32_t* picked, int slots, float scaling, void* out, int64_t out_seq_stride,
-                              int64_t out_head_stride, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
-                              int32_t* status, lf_stream_t stream) {
+                              const int32_t* counts, const int32_t* picked, int slots, float scaling, void* out,
+                              int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void* workspace,
+                              size_t workspace_bytes, int32_t* status, lf_stream_t stream) {
   lf::AttendParams p;
   const int bad = lf::check_int4_pool("lf_int4_attend", pool, head_dim, p.pool);
   if (bad != LF_OK) return bad;
@@ -108,8 +722,13 @@ extern "C" int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void
   LF_CHECK_ARG(q_len > 0 && q_len <= 65535 && n_q > 0 && n_q % p.pool.kv_heads == 0,
                "lf_int4_attend: q_len %d, %d query heads on %d KV heads", q_len, n_q, p.pool.kv_heads);
   LF_CHECK_ARG(picked == nullptr || slots > 0, "lf_int4_attend: %d slots", slots);
-  LF_CHECK_ARG(workspace && workspace_bytes >= lf_int4_workspace_bytes(p.pool.batch, p.pool.kv_heads, n_q, q_len, head_dim),
-               "lf_int4_attend: workspace of %zu bytes is too small", workspace_bytes);
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_seq_stride | q_head_stride | q_tok_stride) % 8 == 0,
+               "lf_int4_attend: query rows must be 16-byte aligned");
+  const int sms = lf::sm_count();
+  if (sms <= 0) return lf::launch_status("lf_int4_attend");
+  LF_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
+                   workspace_bytes >= lf_int4_workspace_bytes(p.pool.batch, p.pool.kv_heads, n_q, q_len, head_dim),
+               "lf_int4_attend: workspace of %zu bytes is missing, misaligned or too small", workspace_bytes);
   p.q = q;
   p.q_seq = q_seq_stride;
   p.q_head = q_head_stride;
@@ -125,7 +744,19 @@ extern "C" int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void
   p.out_seq = out_seq_stride;
   p.out_head = out_head_stride;
   p.out_tok = out_tok_stride;
+  p.rows = picked ? p.pool.batch * q_len : p.pool.batch;
+  p.cols = picked ? p.group : p.group * q_len;
+  p.col_tiles = (p.cols + lf::tile_columns(p.cols) - 1) / lf::tile_columns(p.cols);
+  LF_CHECK_SUPPORTED(static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles <=
+                         (1 << 30) / (picked ? slots : p.pool.table_width),
+                     "lf_int4_attend: %d sequences of %d pages are too many for one call", p.pool.batch,
+                     p.pool.table_width);
+  p.partials = static_cast<float*>(workspace);
+  p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + lf::partial_bytes(sms));
   p.status = status;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == LF_F16 ? lf::launch_attend<__half>(p, head_dim, s) : lf::launch_attend<__nv_bfloat16>(p, head_dim, s);
+  if (dtype == LF_F16)
+    return head_dim == 128 ? lf::launch_attend_by<__half, 128>(p, sms, s) : lf::launch_attend_by<__half, 64>(p, sms, s);
+  return head_dim == 128 ? lf::launch_attend_by<__nv_bfloat16, 128>(p, sms, s)
+                         : lf::launch_attend_by<__nv_bfloat16, 64>(p, sms, s);
 }

@@ -207,21 +207,24 @@ _workspaces: dict = {}
 
 
 def _workspace(need: int, device) -> torch.Tensor:
-    """Scratch of an attention call, zero before its first use and left so by
-    every call.  Calls on one stream share one buffer (they run in order);
+    """Scratch of an attention call: partial results, then tickets that are zero
+    between calls.  Calls on one stream share one buffer (they run in order);
     a call being captured in a CUDA graph gets its own, which the graph keeps
     and clears, so replays on any stream do not meet."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[_lib.lib().lf_int4_workspace_clear_from():].zero_()
+        return ws
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < need:
-        ws = _workspaces[key] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
+        ws = _workspaces[key] = torch.zeros(need + need // 8, dtype=torch.uint8, device=device)
     return ws
 
 
 def _query(query: torch.Tensor, pool, head_dim: int, device):
-    """The query as [B, n_q, q_len, D] with channel stride 1, checked."""
+    """The query, checked, as [B, n_q, q_len, D] with 16-byte aligned rows of
+    channel stride 1, and its first three strides."""
     q = query.unsqueeze(2) if query.dim() == 3 else query
     if q.dim() != 4 or q.shape[0] != pool.batch or q.shape[3] != head_dim or q.shape[1] < 1 or q.shape[2] < 1:
         raise ValueError(f"query must be [{pool.batch}, n_q, {head_dim}] or [{pool.batch}, n_q, q_len, {head_dim}], got "
@@ -232,13 +235,13 @@ def _query(query: torch.Tensor, pool, head_dim: int, device):
         raise NotImplementedError(f"the 4-bit cache's attention takes fp16 or bf16 queries, got {q.dtype}")
     if q.device != device:
         raise RuntimeError(f"query is on {q.device}, pages on {device}")
-    return q if q.stride(3) == 1 else q.contiguous()
+    return _aligned_rows(q)
 
 
 def _attend(query, pages, page_table, lengths, scaling, counts, picked, out, status):
     pool, D = _pool(pages, page_table)
     dev = pages.device
-    q = _query(query, pool, D, dev)
+    q, qs = _query(query, pool, D, dev)
     if out is None:
         out = torch.empty(query.shape, dtype=query.dtype, device=dev)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride(-1) != 1:
@@ -256,7 +259,7 @@ def _attend(query, pages, page_table, lengths, scaling, counts, picked, out, sta
     with _on(dev):
         ws = _workspace(so.lf_int4_workspace_bytes(pool.batch, pool.kv_heads, n_q, q_len, D), dev)
         _lib.check(so.lf_int4_attend(
-            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), q_len, n_q,
+            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), *qs, q_len, n_q,
             _per_sequence("lengths", lengths, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev),
             _lib.ptr(picked), slots, float(scaling), o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), ws.data_ptr(),
             ws.numel(), _status(status, dev), _lib.stream_handle(dev)), "lf_int4_attend")
@@ -287,7 +290,7 @@ def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, 
     query heads; ties to the lower page)."""
     pool, D = _pool(pages, page_table)
     dev = pages.device
-    q = _query(query, pool, D, dev)
+    q, qs = _query(query, pool, D, dev)
     n_q, q_len = q.shape[1], q.shape[2]
     top, sink, recent = int(top_pages), int(sink_pages), int(recent_pages)
     if top < 0 or sink < 0 or recent < 1:
@@ -296,7 +299,7 @@ def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, 
     picked = torch.empty(pool.batch, q_len, pool.kv_heads, sink + recent + top, dtype=torch.int32, device=dev)
     with _on(dev):
         _lib.check(_lib.lib().lf_int4_select(
-            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), q_len, n_q,
+            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), *qs, q_len, n_q,
             bp, b0, b1, _per_sequence("lengths", lengths, pool.batch, dev),
             _per_sequence("counts", counts, pool.batch, dev), top, sink, recent, picked.data_ptr(), _status(status, dev),
             _lib.stream_handle(dev)), "lf_int4_select")
