@@ -346,7 +346,7 @@ LF_API int lf_gather_wait(uint32_t* flags, int layer, uint32_t expected, uint64_
  * nowhere, read as zero, not attended) and LF_ERR_OUT_OF_RANGE goes to *status
  * (device int32, may be NULL).
  *
- * Bounds records (optional, int8; a sparse call needs them):
+ * Bounds records (optional, int8, 8-byte aligned; a sparse call needs them):
  * 2 * head_dim + 1 bytes or more per (page, KV head): upper and lower bound of
  * every Key channel over the page's tokens, in steps of 2^e, then e.  They
  * are written when slot 63 of a page is.

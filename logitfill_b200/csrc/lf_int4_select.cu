@@ -1,9 +1,19 @@
 // Which pages a sparse attention call reads: a bound on the scores of each page
 // from its Key bounds, and the best of them (lf_int4_select).
 //
-// One CTA per (query token, KV head).  The bound is a dot product of whole
-// numbers, so every page's score is exact and the choice is the same on every
-// run.
+// Mathematics.  For a page with channel bounds low_d <= K_d <= upper_d every
+// score q . K is at most sum_d max(q_d, 0) upper_d + min(q_d, 0) low_d; summed over
+// the heads that share the KV head, that is one dot product of the record's 2 D
+// int8 entries with 2 D weights.  The weights are whole numbers (the queries
+// scaled by one power of two per group and rounded), so the sum is exact in
+// int32 and the choice the same on every run.
+//
+// One cluster per (query token, KV head): its CTAs share the candidate pages, a
+// warp per record (a lane holds the weights of its 8 channels, two int16 x int8
+// products an instruction, one warp sum), and put the scores into the first
+// CTA's shared memory; that CTA then narrows the range of the top-th best score
+// (a histogram of 256 steps over the range that is left, four rounds at most)
+// and writes the chosen pages in order.
 #include "lf_int4.cuh"
 
 namespace lf {
@@ -16,96 +26,253 @@ struct SelectParams {
   const int8_t* bounds;
   int64_t bounds_page, bounds_head;
   const int32_t *lengths, *counts;
-  int top, sink, recent;
+  int top, sink, recent, cluster;
   int32_t* picked;
   int32_t* status;
 };
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxSelectPages = 32768;  // candidates whose scores fit in shared memory
+constexpr int kPagesAtOnce = 8;         // records a warp has in flight
+
+// A float's bits as an unsigned number of the same order.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Stores into the shared memory of the cluster's first CTA, at this CTA's address of p.
+__device__ __forceinline__ void store_first(uint32_t* p, uint32_t v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
+// Sum of x over the threads before this one, and over all of them.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* warp_sum, uint32_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t upto = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  __syncthreads();  // warp_sum may still be read from the scan before
+  if (lane == 31) warp_sum[warp] = upto;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  return before + upto - x;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __grid_constant__ SelectParams p) {
-  extern __shared__ float score_s[];
-  __shared__ int plus_s[D], minus_s[D];
-  __shared__ float most_s[kSelectThreads / 32];
-  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
+  extern __shared__ uint32_t key_s[];
+  __shared__ __align__(16) int16_t weight_s[2 * D];
+  __shared__ float most_s[kSelectWarps];
+  __shared__ uint32_t hist_s[256], sum_s[kSelectWarps], low_s[kSelectWarps], high_s[kSelectWarps], pick_s[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int h = blockIdx.x / p.cluster, i = blockIdx.y, b = blockIdx.z;
   const int slots = p.top + p.sink + p.recent;
   int32_t* picked = p.picked + ((static_cast<int64_t>(b) * p.q_len + i) * p.pool.kv_heads + h) * slots;
-  const int n = min((int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i) + kInt4Page - 1) / kInt4Page, p.pool.table_width);
-  if (n <= slots) {
-    for (int s = threadIdx.x; s < slots; s += kSelectThreads) picked[s] = s < n ? s : -1;
+  const int seen = int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i);
+  const int n = min(seen / kInt4Page + (seen % kInt4Page != 0), p.pool.table_width);
+  if (n <= slots || p.top == 0) {  // nothing to choose (the same in every CTA of the cluster)
+    const int head = n <= slots ? n : p.sink;
+    if (rank == 0)
+      for (int s = tid; s < slots; s += kSelectThreads) picked[s] = s < head ? s : n <= slots ? -1 : n - slots + s;
     return;
   }
+
+  if (p.cluster > 1) cluster_arrive();  // that every CTA of the cluster runs, before any stores to the first
+
+  // Weights: the group's queries in whole numbers, split by sign.
   const T* q = static_cast<const T*>(p.q) + b * p.q_seq + static_cast<int64_t>(h) * p.group * p.q_head + i * p.q_tok;
   float most = 0.0f;
-  for (int x = threadIdx.x; x < p.group * D; x += kSelectThreads) {
+  for (int x = tid; x < p.group * D; x += kSelectThreads) {
     const float v = fabsf(Scalar<T>::load(q + (x / D) * p.q_head + x % D));
     most = isfinite(v) ? fmaxf(most, v) : most;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
+  if (lane == 0) most_s[warp] = most;
   __syncthreads();
-  for (int w = 0; w < kSelectThreads / 32; ++w) most = fmaxf(most, most_s[w]);
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) most = fmaxf(most, most_s[w]);
   const int f = exponent127(most);
-  if (threadIdx.x < D) {
+  const float scale = pow2(-f);
+  if (tid < D) {
     int plus = 0, minus = 0;
     for (int j = 0; j < p.group; ++j) {
-      const float v = Scalar<T>::load(q + j * p.q_head + threadIdx.x);
-      const int c = isfinite(v) ? __float2int_rn(scalbnf(v, -f)) : 0;
+      const float v = Scalar<T>::load(q + j * p.q_head + tid);
+      const int c = isfinite(v) ? __float2int_rn(v * scale) : 0;
       plus += max(c, 0);
       minus += min(c, 0);
     }
-    plus_s[threadIdx.x] = plus;
-    minus_s[threadIdx.x] = minus;
+    weight_s[tid] = static_cast<int16_t>(plus);
+    weight_s[D + tid] = static_cast<int16_t>(minus);
   }
   __syncthreads();
-  const int first = p.sink, count = n - p.sink - p.recent;  // candidates: pages first .. first + count - 1
-  for (int c = threadIdx.x; c < count; c += kSelectThreads) {
-    const int id = int4_page_id(p.pool, b, first + c);
-    float score = -INFINITY;
-    if (id >= 0) {
-      const int8_t* rec = p.bounds + id * p.bounds_page + h * p.bounds_head;
-      int sum = 0;
-      for (int d = 0; d < D; ++d) sum += rec[d] * plus_s[d] + rec[D + d] * minus_s[d];
-      score = __int2float_rn(sum) * pow2(rec[2 * D]);
-    } else if (p.status != nullptr) {
-      atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+
+  // Scores of this CTA's candidates (pages sink .. n - recent - 1, dealt warp by warp).
+  constexpr int kBytes = 2 * D / 32, kPairs = kBytes / 2;  // a lane's record entries and its weight pairs
+  int wt[kPairs];
+#pragma unroll
+  for (int x = 0; x < kPairs; ++x) wt[x] = reinterpret_cast<const int*>(weight_s)[lane * kPairs + x];
+  const int first = p.sink, count = n - p.sink - p.recent;
+  if (p.cluster > 1) cluster_wait();
+  const int step = p.cluster * kSelectWarps * kPagesAtOnce;
+  for (int c0 = (rank * kSelectWarps + warp) * kPagesAtOnce; c0 < count; c0 += step) {
+    int id = -1;
+    if (lane < kPagesAtOnce && c0 + lane < count) {
+      id = int4_page_id(p.pool, b, first + c0 + lane);
+      if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
     }
-    score_s[c] = score;
-  }
-  __syncthreads();
-  // A candidate's place: how many are better.  Then the chosen ones in order.
-  for (int c = threadIdx.x; c < count; c += kSelectThreads) {
-    const float mine = score_s[c];
-    int better = 0;
-    for (int o = 0; o < count; ++o) better += score_s[o] > mine || (score_s[o] == mine && o < c);
-    if (better < p.top) {
-      int place = 0;  // chosen candidates before this one
-      for (int o = 0; o < c; ++o) {
-        int r = 0;
-        for (int x = 0; x < count; ++x) r += score_s[x] > score_s[o] || (score_s[x] == score_s[o] && x < o);
-        place += r < p.top;
+    const int e = id < 0 ? 0 : p.bounds[id * p.bounds_page + h * p.bounds_head + 2 * D];
+    uint32_t w[kPagesAtOnce][kBytes / 4];
+#pragma unroll
+    for (int x = 0; x < kPagesAtOnce; ++x) {
+      const int page = __shfl_sync(0xffffffffu, id, x);
+      const int8_t* rec = p.bounds + max(page, 0) * p.bounds_page + h * p.bounds_head;
+      if constexpr (D == 128) {
+        const uint2 y = *reinterpret_cast<const uint2*>(rec + lane * 8);
+        w[x][0] = y.x;
+        w[x][1] = y.y;
+      } else {
+        w[x][0] = *reinterpret_cast<const uint32_t*>(rec + lane * 4);
       }
-      picked[p.sink + place] = first + c;
+    }
+    int mine = 0;
+#pragma unroll
+    for (int x = 0; x < kPagesAtOnce; ++x) {
+      int sum = 0;
+#pragma unroll
+      for (int y = 0; y < kBytes / 4; ++y) {
+        sum = __dp2a_lo(wt[2 * y], static_cast<int>(w[x][y]), sum);
+        sum = __dp2a_hi(wt[2 * y + 1], static_cast<int>(w[x][y]), sum);
+      }
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      mine = lane == x ? sum : mine;
+    }
+    if (lane < kPagesAtOnce && c0 + lane < count) {
+      const uint32_t key = id < 0 ? 0u : ordered(__int2float_rn(mine) * pow2(e));
+      if (p.cluster > 1)
+        store_first(key_s + c0 + lane, key);
+      else
+        key_s[c0 + lane] = key;
     }
   }
-  for (int s = threadIdx.x; s < p.sink; s += kSelectThreads) picked[s] = s;
-  for (int s = threadIdx.x; s < p.recent; s += kSelectThreads) picked[p.sink + p.top + s] = n - p.recent + s;
+  if (p.cluster > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+
+  // The top-th best key: narrow [low, high] to one key.  `want` keys of the
+  // range are still to be chosen, all above it are.
+  uint32_t low = UINT32_MAX, high = 0;
+  for (int c = tid; c < count; c += kSelectThreads) {
+    low = min(low, key_s[c]);
+    high = max(high, key_s[c]);
+  }
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) {
+    low_s[warp] = low;
+    high_s[warp] = high;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) {
+    low = min(low, low_s[w]);
+    high = max(high, high_s[w]);
+  }
+  uint32_t want = p.top;
+  while (low < high) {  // at most 4 rounds: the range loses 8 bits each
+    const int shift = max(0, 24 - __clz(high - low));  // (high - low) >> shift is at most 255
+    hist_s[tid] = 0;
+    __syncthreads();
+    for (int c = tid; c < count; c += kSelectThreads) {
+      const uint32_t k = key_s[c];
+      if (k >= low && k <= high) atomicAdd(&hist_s[255 - ((k - low) >> shift)], 1u);  // best step first
+    }
+    __syncthreads();
+    const uint32_t mine = hist_s[tid];
+    uint32_t total;
+    const uint32_t before = scan_before(mine, sum_s, total);
+    if (before < want && want <= before + mine) {
+      pick_s[0] = 255 - tid;
+      pick_s[1] = want - before;
+    }
+    __syncthreads();
+    want = pick_s[1];
+    low += pick_s[0] << shift;
+    high = low + min(high - low, (1u << shift) - 1u);
+    __syncthreads();
+  }
+
+  // Every key above it, and the first `want` equal to it, in order.
+  const int each = (count + kSelectThreads - 1) / kSelectThreads;
+  const int from = min(count, tid * each), to = min(count, from + each);
+  uint32_t found = 0;  // keys above in the low half, equal ones in the high half
+  for (int c = from; c < to; ++c) found += key_s[c] > low ? 1u : key_s[c] == low ? 0x10000u : 0u;
+  uint32_t total;
+  uint32_t place = scan_before(found, sum_s, total);
+  for (int c = from; c < to; ++c) {
+    const uint32_t k = key_s[c], equal = place >> 16;
+    if (k > low || (k == low && equal < want)) picked[p.sink + (place & 0xFFFFu) + min(equal, want)] = first + c;
+    place += k > low ? 1u : k == low ? 0x10000u : 0u;
+  }
+  for (int s = tid; s < p.sink; s += kSelectThreads) picked[s] = s;
+  for (int s = tid; s < p.recent; s += kSelectThreads) picked[p.sink + p.top + s] = n - p.recent + s;
 }
 
-template <typename T>
-static int launch_select(const SelectParams& p, int D, cudaStream_t stream) {
-  const dim3 grid(p.pool.kv_heads, p.q_len, p.pool.batch);
-  const int smem = p.pool.table_width * static_cast<int>(sizeof(float));
-  const void* kern = D == 128 ? reinterpret_cast<const void*>(int4_select_kernel<T, 128>)
-                              : reinterpret_cast<const void*>(int4_select_kernel<T, 64>);
-  if (raise_smem_limit(kern, smem, false) != cudaSuccess) return launch_status("lf_int4_select");
-  if (D == 128)
-    int4_select_kernel<T, 128><<<grid, kSelectThreads, smem, stream>>>(p);
-  else
-    int4_select_kernel<T, 64><<<grid, kSelectThreads, smem, stream>>>(p);
+template <typename T, int D>
+static int launch_select(SelectParams p, cudaStream_t stream) {
+  const void* kern = reinterpret_cast<const void*>(int4_select_kernel<T, D>);
+  const int smem = p.pool.table_width * static_cast<int>(sizeof(uint32_t));
+  cudaError_t err = raise_smem_limit(kern, smem, false);
+  if (err != cudaSuccess) {
+    set_error("lf_int4_select: %s", cudaGetErrorString(err));
+    return LF_ERR_CUDA;
+  }
+  // More CTAs per unit while the units alone leave SMs idle and a CTA keeps a
+  // round of records for each of its warps.
+  const int64_t units = static_cast<int64_t>(p.pool.kv_heads) * p.q_len * p.pool.batch;
+  p.cluster = 1;
+  while (p.cluster < 8 && units * p.cluster < 148 && p.pool.table_width > p.cluster * kSelectWarps * kPagesAtOnce) p.cluster *= 2;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.pool.kv_heads * p.cluster, p.q_len, p.pool.batch);
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&p};
+  err = cudaLaunchKernelExC(&cfg, kern, args);
+  if (err != cudaSuccess) {
+    set_error("lf_int4_select: %s", cudaGetErrorString(err));
+    return LF_ERR_LAUNCH;
+  }
   return launch_status("lf_int4_select");
 }
 
@@ -130,6 +297,8 @@ extern "C" int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void
                "lf_int4_select: top %d, sink %d, recent %d pages (recent at least 1)", top_pages, sink_pages, recent_pages);
   LF_CHECK_ARG(bounds_page_stride > 2 * head_dim && bounds_head_stride > 2 * head_dim,
                "lf_int4_select: bounds records overlap");
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(bounds) & 7) == 0 && (bounds_page_stride | bounds_head_stride) % 8 == 0,
+               "lf_int4_select: bounds records must be 8-byte aligned");
   LF_CHECK_SUPPORTED(p.pool.table_width <= lf::kMaxSelectPages, "lf_int4_select: %d pages per sequence (%d at most)",
                      p.pool.table_width, lf::kMaxSelectPages);
   p.q = q;
@@ -149,5 +318,7 @@ extern "C" int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void
   p.picked = picked;
   p.status = status;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return q_dtype == LF_F16 ? lf::launch_select<__half>(p, head_dim, s) : lf::launch_select<__nv_bfloat16>(p, head_dim, s);
+  if (q_dtype == LF_F16)
+    return head_dim == 128 ? lf::launch_select<__half, 128>(p, s) : lf::launch_select<__half, 64>(p, s);
+  return head_dim == 128 ? lf::launch_select<__nv_bfloat16, 128>(p, s) : lf::launch_select<__nv_bfloat16, 64>(p, s);
 }

@@ -99,7 +99,7 @@ def _status(t: torch.Tensor | None, device) -> int:
 def _bounds(bounds: torch.Tensor, pages: torch.Tensor, head_dim: int):
     n, H = pages.shape[0], pages.shape[1]
     if (bounds.dtype != torch.int8 or bounds.dim() != 3 or bounds.shape[0] != n or bounds.shape[1] != H
-            or bounds.shape[2] < 2 * head_dim + 1 or bounds.stride(2) != 1 or bounds.device != pages.device):
+            or bounds.shape[2] != 2 * head_dim + 16 or bounds.stride(2) != 1 or bounds.device != pages.device):
         raise ValueError(f"bounds must be int8 [{n}, {H}, {bounds_bytes(head_dim)}] on {pages.device}, got {bounds.dtype} "
                          f"{tuple(bounds.shape)} on {bounds.device}")
     return bounds.data_ptr(), bounds.stride(0) if n > 1 else H * bounds.shape[2], \
