@@ -22,11 +22,12 @@
 //
 // Split.  All pages of all units form one line, cut into equal ranges, one per
 // CTA (the lengths are read on the device, so nothing is planned on the host).
-// Each of a CTA's four warps takes 16 tokens of every page of the range through
-// its own ring of cp.async stages: no barrier until the range's end.  A unit
-// that lies in one range is finished there; otherwise each CTA leaves a partial
-// (maximum, sum, accumulator) and the last one to arrive (an atomic ticket)
-// merges them in the order of the ranges, so results do not depend on timing.
+// A CTA fills an SM; two of its warps share a page, 32 tokens each, and each
+// warp copies its half pages through its own ring of cp.async stages: no barrier
+// until the range's end.  A unit that lies in one range is finished there;
+// otherwise each CTA leaves a partial (maximum, sum, accumulator) and the last
+// one to arrive (an atomic ticket) merges them in the order of the ranges, so
+// results do not depend on timing.
 #include <type_traits>
 
 #include "lf_int4.cuh"
@@ -50,19 +51,27 @@ struct AttendParams {
   int32_t* status;
 };
 
-constexpr int kAttendWarps = 4;
-constexpr int kAttendThreads = 32 * kAttendWarps;
-constexpr int kTile = kInt4Page / kAttendWarps;  // tokens of a page that one warp takes
-constexpr float kSlack = 8.0f;                   // log2 a score may pass the running maximum by
+constexpr int kHalfPage = kInt4Page / 2;  // tokens of a page that one warp takes
+constexpr int kTile = 16;                 // tokens of one tensor-core step
+constexpr float kSlack = 8.0f;            // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
+constexpr int kMinPages = 3;  // pages of a range at least: below, merging costs more than the pages
+#ifndef LF_UNROLL
+#define LF_UNROLL 1
+#endif
+constexpr int kUnroll = LF_UNROLL;
 
+// Warps and stages per CTA: what the registers (12 warps of 168, or 8 of 255 with
+// 16 columns at D 128) and 227 KB of shared memory hold.
 template <int D, int NT> struct AttendCfg {
-  static constexpr int kStages = D == 128 ? 6 : 10;
-  static constexpr int kCtas = NT == 1 ? 3 : 2;
-  static constexpr int kTileBytes = kTile * (D + D / 4);
+  static constexpr int kWarps = D == 128 && NT == 2 ? 8 : 12;
+  static constexpr int kThreads = 32 * kWarps, kPairs = kWarps / 2;
+  static constexpr int kStages = D == 64 ? 6 : kWarps == 8 ? 5 : 3;
+  static constexpr int kCodes = kHalfPage * D / 2, kPar = kHalfPage * D / 8;  // bytes of a half page, Key or Value
+  static constexpr int kStageBytes = 2 * (kCodes + kPar);
   static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
-  static constexpr int kRing = kAttendWarps * kStages * kTileBytes;
-  static constexpr int kMerge = kAttendWarps * 8 * NT * (kPad + 2) * 4;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kMerge = kWarps * 8 * NT * (kPad + 2) * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
   static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial
 };
@@ -118,20 +127,33 @@ __device__ __forceinline__ uint32_t odd_code(uint32_t x) {
   return hfma2((x & 0x00f000f0u) | 0x64006400u, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
 }
 __device__ __forceinline__ bool is_nan_param(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
-// Scale above 2048 or |minimum| of 2^15 and more.
-__device__ __forceinline__ bool is_wide_param(uint32_t w) {
-  return (w & 0x7FFFu) > 0x6800u || (w & 0x7FFF0000u) >= 0x78000000u;
+// Larger magnitude of each half (a NaN gives way to a number).
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7FFF7FFFu), "r"(b & 0x7FFF7FFFu));
+  return r;
 }
-// Parameter words of token k of a warp's tile.
-template <int kG>
-__device__ __forceinline__ void load_params(const uint8_t* par, int k, uint32_t (&w)[kG]) {
-  if constexpr (kG == 4) {
-    const uint4 x = *reinterpret_cast<const uint4*>(par + k * 16);
+// kWords (2 or 4) words of shared memory in one load.
+template <int kWords>
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[kWords]) {
+  if constexpr (kWords == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(at);
     w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
   } else {
-    const uint2 x = *reinterpret_cast<const uint2*>(par + k * 8);
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
     w[0] = x.x; w[1] = x.y;
   }
+}
+// Whether a Value group of position tok holds NaN (read from the record).
+template <int kG>
+__device__ __noinline__ bool value_has_nan(const AttendParams& p, int h, int b, int tok) {
+  const int id = int4_page_id(p.pool, b, tok / kInt4Page);
+  if (id < 0) return false;
+  const uint32_t* par = reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h) + 18 * 32 * kG +
+                        tok % kInt4Page * kG;
+  bool nan = false;
+  for (int G = 0; G < kG; ++G) nan |= is_nan_param(par[G]);
+  return nan;
 }
 
 // Tokens that row r (a sequence, or a query token of one) sees at most.
@@ -150,16 +172,18 @@ __device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
 }
 
 template <typename T, int D, int NT, bool kSparse>
-__global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
+__global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
     int4_attend_kernel(const __grid_constant__ AttendParams p) {
   using C = AttendCfg<D, NT>;
-  constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages;
+  constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
+  constexpr int kCodes = C::kCodes, kPar = C::kPar;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int meta_s[kAttendWarps][kStages];  // first token of each stage's page, -1: nothing to do
-  __shared__ float weight_s[kAttendWarps][kCol], top_s[kCol], sum_s[kCol];
+  __shared__ int meta_s[kWarps][kStages];  // first token of each stage's half page, -1: nothing to do
+  __shared__ float weight_s[kWarps][kCol], top_s[kCol], sum_s[kCol];
   __shared__ int last_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = p.pool.kv_heads * p.col_tiles;
+  grid_dep_wait();
 
   // The line of pages: its length, and the row where this CTA's range begins.
   int total = 0;
@@ -167,7 +191,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     const int n = r0 + lane < p.rows ? row_pages<kSparse>(p, row_tokens<kSparse>(p, r0 + lane)) * per_row : 0;
     total += __reduce_add_sync(0xffffffffu, n);
   }
-  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int per = max(kMinPages, static_cast<int>((total + gridDim.x - 1) / gridDim.x));
   const int begin = blockIdx.x * per, end = min(total, begin + per);
   if (begin >= end) return;
   int row = 0, row_base = 0;
@@ -189,8 +213,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     row_base += __shfl_sync(0xffffffffu, upto, 31);
   }
 
-  uint8_t* ring = smem + warp * kStages * C::kTileBytes;
-  const uint32_t ring_a = smem_addr(ring);
+  uint8_t* ring = smem + warp * kStages * C::kStageBytes;
+  const uint32_t ring_a = smem_addr(ring) + lane * 16;
+  const int pair = warp >> 1, half = warp & 1;
+  // Byte offsets in a record of this lane's pieces: Key codes (Value codes 40 D
+  // later), and parameters, the first half of the lanes Key's, the others Value's.
+  constexpr int kParLanes = kPar / 16;  // lanes' worth of a half page's Key parameters
+  const int code_at = half * kCodes + lane * 16;
   int at = begin;
   while (at < end) {
     // ------------------------------------------------------------ one unit
@@ -205,14 +234,16 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     if (tid == 0 && p.status != nullptr && (seen_max - 1) / kInt4Page >= p.pool.table_width)
       atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
 
-    // Page ids of 32 pages at a time, one per lane, loaded a window ahead.
-    auto load_ids = [&](int j0, int& id, int& logical) {
-      const int j = j0 + lane;
+    // This warp's pages: first + pair, then every kPairs-th.  Their ids, 32 at a
+    // time, one per lane, loaded a window ahead.
+    const int mine_n = first + pair < stop ? (stop - first - pair + C::kPairs - 1) / C::kPairs : 0;
+    auto load_ids = [&](int x0, int& id, int& logical) {
+      const int x = x0 + lane;
       id = logical = -1;
-      if (j < stop) {
-        logical = j;
+      if (x < mine_n) {
+        logical = first + pair + x * C::kPairs;
         if constexpr (kSparse)
-          logical = p.picked[(static_cast<int64_t>(row) * p.pool.kv_heads + h) * p.slots + j];
+          logical = p.picked[(static_cast<int64_t>(row) * p.pool.kv_heads + h) * p.slots + logical];
         if (logical >= 0 && static_cast<int64_t>(logical) * kInt4Page < seen_max) {
           id = int4_page_id(p.pool, b, logical);
           if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
@@ -220,47 +251,50 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
       }
     };
     int ids, logicals, ids_next, logicals_next;
-    load_ids(first, ids, logicals);
-    load_ids(first + 32, ids_next, logicals_next);
-    int window = first;
-    auto issue = [&](int j) {
-      if (j < stop) {
-        if (j - window == 32) {
-          window += 32;
+    load_ids(0, ids, logicals);
+    load_ids(32, ids_next, logicals_next);
+    int issued = 0, into = 0;  // pages issued, the stage of the next
+    const uint8_t* head_words = reinterpret_cast<const uint8_t*>(p.pool.words + h * p.pool.head_stride);
+    auto issue = [&]() {
+      if (issued < mine_n) {
+        if (issued != 0 && (issued & 31) == 0) {
           ids = ids_next;
           logicals = logicals_next;
-          load_ids(window + 32, ids_next, logicals_next);
+          load_ids(issued + 32, ids_next, logicals_next);
         }
-        const int id = __shfl_sync(0xffffffffu, ids, j - window);
-        const int logical = __shfl_sync(0xffffffffu, logicals, j - window);
-        const int st = (j - first) % kStages;
-        if (lane == 0) meta_s[warp][st] = id < 0 ? -1 : logical * kInt4Page + warp * kTile;
+        const int id = __shfl_sync(0xffffffffu, ids, issued & 31);
+        const int logical = __shfl_sync(0xffffffffu, logicals, issued & 31);
+        if (lane == 0) meta_s[warp][into] = id < 0 ? -1 : logical * kInt4Page + half * kHalfPage;
         if (id >= 0) {
-          const uint8_t* rec = reinterpret_cast<const uint8_t*>(p.pool.words + int4_record(p.pool, id, h));
-          const uint32_t dst = ring_a + st * C::kTileBytes;
-          constexpr int kCodes = kTile * D / 2, kPar = kTile * D / 8;  // bytes of one warp's tile
-          const uint8_t* kc = rec + warp * kCodes + lane * 16;
+          const uint8_t* rec = head_words + id * p.pool.page_stride * 4;
+          const uint32_t dst = ring_a + into * C::kStageBytes;
+          const uint8_t* kc = rec + code_at;
 #pragma unroll
           for (int x = 0; x < kCodes / 512; ++x) {
-            cp_async16(dst + lane * 16 + x * 512, kc + x * 512);
-            cp_async16(dst + kCodes + lane * 16 + x * 512, kc + 40 * D + x * 512);
+            cp_async16(dst + x * 512, kc + x * 512);
+            cp_async16(dst + kCodes + x * 512, kc + 40 * D + x * 512);
           }
-          constexpr int kParLanes = kPar / 16;
-          if (lane < 2 * kParLanes) {
+          if constexpr (kParLanes == 32) {
+            cp_async16(dst + 2 * kCodes, rec + 32 * D + half * kPar + lane * 16);
+            cp_async16(dst + 2 * kCodes + 512, rec + 72 * D + half * kPar + lane * 16);
+          } else {
             const int v = lane / kParLanes;
-            cp_async16(dst + 2 * kCodes + lane * 16, rec + 32 * D + v * 40 * D + warp * kPar + (lane - v * kParLanes) * 16);
+            cp_async16(dst + 2 * kCodes, rec + 32 * D + v * 40 * D + half * kPar + (lane - v * kParLanes) * 16);
           }
         }
+        ++issued;
+        into = into + 1 == kStages ? 0 : into + 1;
       }
       cp_commit();
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(first + s);
+    for (int s = 0; s < kStages - 1; ++s) issue();
 
     // Query fragments, sums and scales of this unit's columns.
     uint32_t qf[NT][2 * kG][2], qz[NT];
     float c2[NT][2];
     int vis[NT][2];
+    const float flip = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int c = c0 + nt * 8 + g, i = c / p.group;
@@ -274,7 +308,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+          if constexpr (std::is_same<T, __half>::value) {
             x[G][2 * k] = half_lo(v[k]);
             x[G][2 * k + 1] = half_hi(v[k]);
           } else {
@@ -291,7 +325,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
       const int kq = most > 0.0f && most < INFINITY
                          ? max(-100, min(100, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127)))
                          : 0;
-      const float up = pow2(kq);
+      const float up = pow2(kq) * flip;
       float sums[kG];
 #pragma unroll
       for (int G = 0; G < kG; ++G) {
@@ -313,13 +347,14 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
       float mine = 0.0f;
 #pragma unroll
       for (int G = 0; G < kG; ++G) mine = t == G ? sums[G] : mine;
-      mine *= pow2(kq - 10);
+      mine *= pow2(kq - 10) * flip;
       const float hi = __half2float(__float2half_rn(mine));
       qz[nt] = pack_half2(hi, mine - hi);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int kc = __shfl_sync(0xffffffffu, kq, (2 * t + k) * 4);
-        c2[nt][k] = pow2(10 - kc) * p.scale_log2;
+        // positive, so that a masked score's -inf stays one
+        c2[nt][k] = fmaxf(pow2(10 - kc) * fabsf(p.scale_log2), 1e-36f);
         const int col = min(c0 + nt * 8 + 2 * t + k, p.cols - 1);
         vis[nt][k] = int4_seen(length, count, i0 + col / p.group);
       }
@@ -330,7 +365,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
     float acc[NT][2 * kG][4], m[NT][2], l[NT][2];
-    float big = 1.0f;  // 1/32 once a Value past the fp16 range may have been met
+    float back = 1.0f;  // 32 once a Value past the fp16 range may have been met
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -344,210 +379,218 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
         for (int k = 0; k < 4; ++k) acc[nt][x][k] = 0.0f;
     }
 
-    // ------------------------------------------------------- its pages
+    // ------------------------------------------------------- its half pages
     int st = 0;
-    for (int j = first; j < stop; ++j) {
+    for (int j = 0; j < mine_n; ++j) {
       cp_wait<kStages - 2>();
       __syncwarp();
-      issue(j + kStages - 1);
+      issue();
       const int base = meta_s[warp][st];
-      const uint8_t* tile = ring + st * C::kTileBytes;
+      uint8_t* stage = ring + st * C::kStageBytes;
       st = st + 1 == kStages ? 0 : st + 1;
       if (base < 0 || base >= seen_max) continue;
-      constexpr int kCodes = kTile * D / 2, kPar = kTile * D / 8;
-      const uint8_t *kcode = tile, *vcode = tile + kCodes, *kpar = tile + 2 * kCodes, *vpar = kpar + kPar;
+      const bool masked = base + kHalfPage > vis_min;  // tokens here that not every column sees
 
-      // Scores of 16 tokens (rows g and g + 8 of the fragment).
-      uint32_t kw[2][kG], ks[2][kG], kz[2];
+      // Value parameters in pairs of tokens, as the fragments take them: in place
+      // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
+      {
+        constexpr int kQ = kG / 2;  // words of each token a lane holds: its groups q kQ .. q kQ + kQ - 1
+        const int x = lane >> 1, q = lane & 1;
+        uint32_t* par = reinterpret_cast<uint32_t*>(stage + 2 * kCodes + kPar);
+        uint32_t e[kQ], o[kQ];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if constexpr (D == 128) {
-          const uint4 w = *reinterpret_cast<const uint4*>(kcode + r * 512 + lane * 16);
-          const uint4 s = *reinterpret_cast<const uint4*>(kpar + (8 * r + g) * 16);
-          kw[r][0] = w.x; kw[r][1] = w.y; kw[r][2] = w.z; kw[r][3] = w.w;
-          ks[r][0] = s.x; ks[r][1] = s.y; ks[r][2] = s.z; ks[r][3] = s.w;
-          kz[r] = *reinterpret_cast<const uint32_t*>(kpar + r * 128 + lane * 4);
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(kcode + r * 256 + lane * 8);
-          const uint2 s = *reinterpret_cast<const uint2*>(kpar + (8 * r + g) * 8);
-          kw[r][0] = w.x; kw[r][1] = w.y;
-          ks[r][0] = s.x; ks[r][1] = s.y;
-          kz[r] = t < kG ? *reinterpret_cast<const uint32_t*>(kpar + (8 * r + g) * 8 + t * 4) : 0u;
+        for (int k = 0; k < kQ; ++k) {
+          e[k] = par[2 * x * kG + q * kQ + k];
+          o[k] = par[(2 * x + 1) * kG + q * kQ + k];
         }
-        kz[r] = __byte_perm(kz[r], 0, 0x3232);
-      }
-      float sc[NT][4], dot[NT][4];
+        if (masked) {
+          // What an unwritten slot holds must not be read; a NaN that only some
+          // columns see goes to their weights (below), not through the product.
+          const int tok = base + 2 * x;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sc[nt][k] = dot[nt][k] = 0.0f;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma1688(sc[nt], kz[0], kz[1], qz[nt]);
-#pragma unroll
-      for (int G = 0; G < kG; ++G) {
-        const uint32_t a[2][2] = {{kw[0][G], kw[1][G]}, {kw[0][G] >> 8, kw[1][G] >> 8}};
-        const float s0 = half_lo(ks[0][G]), s1 = half_lo(ks[1][G]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            mma16816(d, a[k][0] & 0x000f000fu, a[k][1] & 0x000f000fu, a[k][0] & 0x00f000f0u, a[k][1] & 0x00f000f0u,
-                     qf[nt][2 * G + k][0], qf[nt][2 * G + k][1]);
-          dot[nt][0] = fmaf(d[0], s0, dot[nt][0]);
-          dot[nt][1] = fmaf(d[1], s0, dot[nt][1]);
-          dot[nt][2] = fmaf(d[2], s1, dot[nt][2]);
-          dot[nt][3] = fmaf(d[3], s1, dot[nt][3]);
+          for (int k = 0; k < kQ; ++k) {
+            if (tok >= seen_max || (tok >= vis_min && is_nan_param(e[k]))) e[k] = 0;
+            if (tok + 1 >= seen_max || (tok + 1 >= vis_min && is_nan_param(o[k]))) o[k] = 0;
+          }
         }
-      }
+        uint32_t s2[kQ], z2[kQ], most = 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int k = 0; k < kQ; ++k) {
+          s2[k] = __byte_perm(e[k], o[k], 0x5410);
+          z2[k] = __byte_perm(e[k], o[k], 0x7632);
+          most = max_abs2(most, hmul2(s2[k], 0x4C004C00u));  // 16 s
+          most = max_abs2(most, z2[k]);
+        }
+        // code * s + z may pass the fp16 range only where 16 s or |z| is 2^15 or
+        // more: Values are held at 1/32 from the first such half page on.
+        const bool wide = (most & 0x7FFFu) >= 0x7800u || (most & 0x7FFF0000u) >= 0x78000000u;
+        if (__any_sync(0xffffffffu, wide) || back != 1.0f) {
+          if (back == 1.0f) {
+            back = 32.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sc[nt][k] = fmaf(dot[nt][k], 16384.0f, sc[nt][k]) * c2[nt][k & 1];
-
-      // Scales and minima of this lane's four tokens, 2t and 2t + 1 of each half.
-      uint32_t vp[2][2][kG];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+              for (int y = 0; y < 2 * kG; ++y)
 #pragma unroll
-        for (int o = 0; o < 2; ++o) load_params<kG>(vpar, 8 * r + 2 * t + o, vp[r][o]);
-
-      const bool masked = base + kTile > vis_min;
-      if (masked) {
-        // Tokens that not every column sees.  What an unwritten slot holds must
-        // not be read; a NaN that only some columns see goes to those columns'
-        // weights, so that it does not reach the others through the product.
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int tok = base + g + 8 * r;
-          bool nan = false;
-          if (tok >= vis_min && tok < seen_max) {
-            uint32_t w[kG];
-            load_params<kG>(vpar, g + 8 * r, w);
-#pragma unroll
-            for (int G = 0; G < kG; ++G) nan |= is_nan_param(w[G]);
+                for (int k = 0; k < 4; ++k) acc[nt][y][k] *= 0.03125f;
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int k = 0; k < kQ; ++k) {
+            s2[k] = hmul2(s2[k], 0x28002800u);
+            z2[k] = hmul2(z2[k], 0x28002800u);
+          }
+        }
+        __syncwarp();  // every lane has read its words
+        if constexpr (kQ == 2)
+          *reinterpret_cast<uint4*>(par + 4 * lane) = make_uint4(s2[0], z2[0], s2[1], z2[1]);
+        else
+          *reinterpret_cast<uint2*>(par + 2 * lane) = make_uint2(s2[0], z2[0]);
+        __syncwarp();
+      }
+
+#pragma unroll kUnroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const uint8_t* kcode = stage + sub * (kCodes / 2);
+        const uint8_t* vcode = kcode + kCodes;
+        const uint8_t* kpar = stage + 2 * kCodes + sub * (kPar / 2);
+        const uint8_t* vpair = kpar + kPar;
+
+        // Scores of 16 tokens (rows g and g + 8 of the fragment).
+        uint32_t kw[2][kG], ks[2][kG], kz[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              if (nan) sc[nt][2 * r + k] = NAN;
-              if (tok >= vis[nt][k]) sc[nt][2 * r + k] = -INFINITY;
+        for (int r = 0; r < 2; ++r) {
+          load_words<kG>(kcode + r * (4 * D) + lane * (4 * kG), kw[r]);
+          load_words<kG>(kpar + (8 * r + g) * (4 * kG), ks[r]);
+          kz[r] = t < kG ? *reinterpret_cast<const uint32_t*>(kpar + (8 * r + g) * (4 * kG) + t * 4) : 0u;
+          kz[r] = __byte_perm(kz[r], 0, 0x3232);
+        }
+        float x[NT][4], dot[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[nt][k] = dot[nt][k] = 0.0f;
+          mma1688(x[nt], kz[0], kz[1], qz[nt]);
+        }
+#pragma unroll
+        for (int G = 0; G < kG; ++G) {
+          const uint32_t a[2][2] = {{kw[0][G], kw[1][G]}, {kw[0][G] >> 8, kw[1][G] >> 8}};
+          const float s0 = half_lo(ks[0][G]), s1 = half_lo(ks[1][G]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              mma16816(d, a[k][0] & 0x000f000fu, a[k][1] & 0x000f000fu, a[k][0] & 0x00f000f0u, a[k][1] & 0x00f000f0u,
+                       qf[nt][2 * G + k][0], qf[nt][2 * G + k][1]);
+            dot[nt][0] = fmaf(d[0], s0, dot[nt][0]);
+            dot[nt][1] = fmaf(d[1], s0, dot[nt][1]);
+            dot[nt][2] = fmaf(d[2], s1, dot[nt][2]);
+            dot[nt][3] = fmaf(d[3], s1, dot[nt][3]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[nt][k] = fmaf(dot[nt][k], 16384.0f, x[nt][k]);
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int tok = base + sub * kTile + 8 * r + g;
+            bool nan = false;
+            if (tok >= vis_min && tok < seen_max) {
+              // the Value pairs hold 0 for a NaN by now: look at the record
+              nan = value_has_nan<kG>(p, h, b, tok);
             }
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            const int mine = base + 8 * r + 2 * t + o;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int G = 0; G < kG; ++G)
-              if (mine >= seen_max || (mine >= vis_min && is_nan_param(vp[r][o][G]))) vp[r][o][G] = 0;
+              for (int k = 0; k < 2; ++k) {
+                if (nan) x[nt][2 * r + k] = NAN;
+                if (tok >= vis[nt][k]) x[nt][2 * r + k] = -INFINITY;
+              }
           }
         }
-      }
 
-      // The running maxima, where a score passes one by the slack.
-      bool move = false;
+        // Distances from the running maxima, moved where one passes the slack.
+        float pr[NT][4];
+        bool move = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) move |= sc[nt][k] > m[nt][k & 1] + kSlack;
-      if (__any_sync(0xffffffffu, move)) {
+          for (int k = 0; k < 4; ++k) {
+            pr[nt][k] = fmaf(x[nt][k], c2[nt][k & 1], -m[nt][k & 1]);
+            move |= pr[nt][k] > kSlack;
+          }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float fix[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float top = fmaxf(x[nt][k], x[nt][k + 2]) * c2[nt][k];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              top = fmaxf(top, m[nt][k]);
+              fix[k] = ex2(m[nt][k] - top);
+              m[nt][k] = top;
+              l[nt][k] *= fix[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pr[nt][k] = fmaf(x[nt][k], c2[nt][k & 1], -m[nt][k & 1]);
+#pragma unroll
+            for (int y = 0; y < 2 * kG; ++y)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[nt][y][k] *= fix[k & 1];
+          }
+        }
+        uint32_t pb[NT][2];  // weights as the product's B operand: columns by tokens
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float fix[2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(sc[nt][k], sc[nt][k + 2]);
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m[nt][k]);
-            fix[k] = ex2(m[nt][k] - top);
-            m[nt][k] = top;
-            l[nt][k] *= fix[k];
+          for (int k = 0; k < 4; ++k) {
+            pr[nt][k] = ex2(pr[nt][k]);
+            l[nt][k & 1] += pr[nt][k];
           }
-#pragma unroll
-          for (int x = 0; x < 2 * kG; ++x)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[nt][x][k] *= fix[k & 1];
+          pb[nt][0] = transpose8x8(pack_half2(pr[nt][0], pr[nt][1]));
+          pb[nt][1] = transpose8x8(pack_half2(pr[nt][2], pr[nt][3]));
         }
-      }
-      uint32_t pb[NT][2];  // weights as the product's B operand: columns by tokens
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float pr[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          pr[k] = ex2(sc[nt][k] - m[nt][k & 1]);
-          l[nt][k & 1] += pr[k];
-        }
-        pb[nt][0] = transpose8x8(pack_half2(pr[0], pr[1]));
-        pb[nt][1] = transpose8x8(pack_half2(pr[2], pr[3]));
-      }
 
-      // Values past the fp16 range (a scale above 2048 or a minimum above 2^15 in
-      // magnitude can give one) are held at 1/32, from the first such tile on.
-      bool wide = false;
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int o = 0; o < 2; ++o)
-#pragma unroll
-          for (int G = 0; G < kG; ++G) wide |= G % 2 == (g & 1) && is_wide_param(vp[r][o][G]);
-      if (big != 1.0f || __any_sync(0xffffffffu, wide)) {
-        if (big == 1.0f) {
-          big = 0.03125f;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 2 * kG; ++x)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) acc[nt][x][k] *= 0.03125f;
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int o = 0; o < 2; ++o)
-#pragma unroll
-            for (int G = 0; G < kG; ++G) vp[r][o][G] = hmul2(vp[r][o][G], 0x28002800u);
-      }
-
-      // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half.
-      uint32_t vw[2][2][D / 64];  // half, even/odd token, word
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if constexpr (D == 128) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vcode + r * 512 + lane * 16);
-          vw[r][0][0] = x.x; vw[r][0][1] = x.y; vw[r][1][0] = x.z; vw[r][1][1] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(vcode + r * 256 + lane * 8);
-          vw[r][0][0] = x.x; vw[r][1][0] = x.y;
-        }
-      }
-#pragma unroll
-      for (int G = 0; G < kG; ++G) {
-        uint32_t v[2][4];  // half, channel 4 g + n of the group
+        // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half, and their parameters.
+        uint32_t vw[2][kG], sz[2][2 * kG];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t s = __byte_perm(vp[r][0][G], vp[r][1][G], 0x5410), z = __byte_perm(vp[r][0][G], vp[r][1][G], 0x7632);
-          const uint32_t x = __byte_perm(vw[r][0][G >> 1], vw[r][1][G >> 1], (G & 1) ? 0x7632 : 0x5410);
-          v[r][0] = hfma2(even_code(x), s, z);
-          v[r][1] = hfma2(odd_code(x), s, z);
-          v[r][2] = hfma2(even_code(x >> 8), s, z);
-          v[r][3] = hfma2(odd_code(x >> 8), s, z);
+          load_words<kG>(vcode + r * (4 * D) + lane * (4 * kG), vw[r]);
+          load_words<kG>(vpair + (4 * r + t) * (8 * kG), *reinterpret_cast<uint32_t(*)[kG]>(&sz[r][0]));
+          load_words<kG>(vpair + (4 * r + t) * (8 * kG) + 4 * kG, *reinterpret_cast<uint32_t(*)[kG]>(&sz[r][kG]));
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][0], pb[nt][1]);
-          mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][0], pb[nt][1]);
+        for (int G = 0; G < kG; ++G) {
+          uint32_t v[2][4];  // half, channel 4 g + n of the group
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t s2 = sz[r][2 * G], z2 = sz[r][2 * G + 1];
+            // codes of the even and the odd token: words [token][w]
+            const uint32_t y = __byte_perm(vw[r][G >> 1], vw[r][kG / 2 + (G >> 1)], (G & 1) ? 0x7632 : 0x5410);
+            v[r][0] = hfma2(even_code(y), s2, z2);
+            v[r][1] = hfma2(odd_code(y), s2, z2);
+            v[r][2] = hfma2(even_code(y >> 8), s2, z2);
+            v[r][3] = hfma2(odd_code(y >> 8), s2, z2);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][0], pb[nt][1]);
+            mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][0], pb[nt][1]);
+          }
         }
       }
     }
     cp_wait<0>();
     __syncthreads();  // the rings are free: the merge buffer takes their place
 
-    // ---------------------------------------- the four warps' results, merged
+    // ------------------------------------------ the warps' results, merged
     float* merge = reinterpret_cast<float*>(smem);
-    float* top_w = merge + kAttendWarps * kCol * C::kPad;
-    float* sum_w = top_w + kAttendWarps * kCol;
+    float* top_w = merge + kWarps * kCol * C::kPad;
+    float* sum_w = top_w + kWarps * kCol;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -560,7 +603,6 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
           top_w[col] = m[nt][k];
           sum_w[col] = sum;
         }
-        const float back = big == 1.0f ? 1.0f : 32.0f;
 #pragma unroll
         for (int G = 0; G < kG; ++G)
           *reinterpret_cast<float4*>(merge + col * C::kPad + 32 * G + 4 * g) =
@@ -571,9 +613,9 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     if (tid < kCol) {
       float top = top_w[tid], sum = 0.0f;
 #pragma unroll
-      for (int w = 1; w < kAttendWarps; ++w) top = fmaxf(top, top_w[w * kCol + tid]);
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, top_w[w * kCol + tid]);
 #pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float f = ex2(top_w[w * kCol + tid] - top);
         weight_s[w][tid] = f;
         sum = fmaf(f, sum_w[w * kCol + tid], sum);
@@ -596,20 +638,20 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
     };
     // The partial of range x of this unit: the range that begins inside the unit
     // uses its CTA's first record, the unit's first range the second.
-    const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per;
+    const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per, parts = last_cta - first_cta + 1;
     auto record = [&](int x) { return p.partials + (2 * static_cast<int64_t>(x) + (x == first_cta)) * C::kRecord; };
     float* mine = record(blockIdx.x);
-    for (int item = tid; item < kCol * D / 4; item += kAttendThreads) {
+    for (int item = tid; item < kCol * D / 4; item += C::kThreads) {
       const int col = item / (D / 4), d = item % (D / 4) * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float f = weight_s[w][col];
-        const float4 x = *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d);
-        v.x = fmaf(f, x.x, v.x);
-        v.y = fmaf(f, x.y, v.y);
-        v.z = fmaf(f, x.z, v.z);
-        v.w = fmaf(f, x.w, v.w);
+        const float4 y = *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d);
+        v.x = fmaf(f, y.x, v.x);
+        v.y = fmaf(f, y.y, v.y);
+        v.z = fmaf(f, y.z, v.z);
+        v.w = fmaf(f, y.w, v.w);
       }
       if (whole) {
         const float sum = sum_s[col];
@@ -626,30 +668,46 @@ __global__ void __launch_bounds__(kAttendThreads, AttendCfg<D, NT>::kCtas)
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        const uint32_t parts = last_cta - first_cta + 1;
         uint32_t* ticket = p.tickets + static_cast<int64_t>(row) * per_row + unit_in_row;
         const uint32_t n = atomicAdd(ticket, 1u) + 1;
-        if (n == parts) *ticket = 0;  // every range has arrived: ready for the next call
-        last_s = n == parts;
+        if (n == static_cast<uint32_t>(parts)) *ticket = 0;  // every range has arrived: ready for the next call
+        last_s = n == static_cast<uint32_t>(parts);
       }
       __syncthreads();
       if (last_s) {
         __threadfence();
-        for (int item = tid; item < kCol * D / 4; item += kAttendThreads) {
-          const int col = item / (D / 4), d = item % (D / 4) * 4;
+        // Weights of the parts (and their sum, by column), then their weighted sum.
+        float* part_w = reinterpret_cast<float*>(smem);  // [parts][kCol], the merge buffer is free
+        for (int x = tid; x < parts * kCol; x += C::kThreads) part_w[x] = __ldcg(record(first_cta + x / kCol) + x % kCol);
+        __syncthreads();
+        for (int col = warp; col < kCol; col += kWarps) {
           float top = kNoMax, sum = 0.0f;
-          for (int x = first_cta; x <= last_cta; ++x) top = fmaxf(top, __ldcg(record(x) + col));
+          for (int x = lane; x < parts; x += 32) top = fmaxf(top, part_w[x * kCol + col]);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int x = lane; x < parts; x += 32) {
+            const float f = ex2(part_w[x * kCol + col] - top);
+            part_w[x * kCol + col] = f;
+            sum = fmaf(f, __ldcg(record(first_cta + x) + kCol + col), sum);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (lane == 0) sum_s[col] = sum;
+        }
+        __syncthreads();
+        for (int item = tid; item < kCol * D / 4; item += C::kThreads) {
+          const int col = item / (D / 4), d = item % (D / 4) * 4;
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int x = first_cta; x <= last_cta; ++x) {
-            const float* rec = record(x);
-            const float f = ex2(__ldcg(rec + col) - top);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
-            sum = fmaf(f, __ldcg(rec + kCol + col), sum);
+#pragma unroll 8
+          for (int x = 0; x < parts; ++x) {
+            const float f = part_w[x * kCol + col];
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(record(first_cta + x) + 2 * kCol + col * D + d));
             v.x = fmaf(f, y.x, v.x);
             v.y = fmaf(f, y.y, v.y);
             v.z = fmaf(f, y.z, v.z);
             v.w = fmaf(f, y.w, v.w);
           }
+          const float sum = sum_s[col];
           store(col, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
         }
       }
@@ -669,23 +727,30 @@ static int sm_count() {
     return 0;
   return n;
 }
-// The partials: two records per CTA of the largest grid (the records of 16 columns are twice those of 8).
+// The partials: two records per CTA, one CTA per SM, of 16 columns at most.
 static size_t partial_bytes(int sms) {
-  return static_cast<size_t>(sms) * 2 * AttendCfg<128, 2>::kCtas * AttendCfg<128, 2>::kRecord * sizeof(float);
+  return static_cast<size_t>(sms) * 2 * AttendCfg<128, 2>::kRecord * sizeof(float);
 }
-static_assert(AttendCfg<128, 2>::kCtas * AttendCfg<128, 2>::kRecord >= AttendCfg<128, 1>::kCtas * AttendCfg<128, 1>::kRecord,
-              "the partials of every variant fit");
 
 template <typename T, int D, int NT, bool kSparse>
-static int launch_attend(const AttendParams& p, int sms, cudaStream_t stream) {
+static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
   using C = AttendCfg<D, NT>;
-  auto kern = int4_attend_kernel<T, D, NT, kSparse>;
-  if (raise_smem_limit(reinterpret_cast<const void*>(kern), C::kSmem, true) != cudaSuccess)
-    return launch_status("lf_int4_attend");
-  // No more CTAs than pages there can be.
-  const int64_t most = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles * (kSparse ? p.slots : p.pool.table_width);
-  const int grid = static_cast<int>(most < static_cast<int64_t>(sms) * C::kCtas ? most : static_cast<int64_t>(sms) * C::kCtas);
-  kern<<<grid, kAttendThreads, C::kSmem, stream>>>(p);
+  const void* kern = reinterpret_cast<const void*>(int4_attend_kernel<T, D, NT, kSparse>);
+  cudaError_t err = raise_smem_limit(kern, C::kSmem, true);
+  if (err != cudaSuccess) {
+    set_error("lf_int4_attend: %s", cudaGetErrorString(err));
+    return LF_ERR_CUDA;
+  }
+  // No more CTAs than ranges there can be.
+  const int64_t pages = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles * (kSparse ? p.slots : p.pool.table_width);
+  const int64_t ranges = (pages + kMinPages - 1) / kMinPages;
+  void* args[] = {&p};
+  err = launch_programmatic(kern, dim3(static_cast<unsigned>(ranges < sms ? ranges : sms)), dim3(C::kThreads), C::kSmem,
+                            stream, args);
+  if (err != cudaSuccess) {
+    set_error("lf_int4_attend: %s", cudaGetErrorString(err));
+    return LF_ERR_LAUNCH;
+  }
   return launch_status("lf_int4_attend");
 }
 template <typename T, int D>
