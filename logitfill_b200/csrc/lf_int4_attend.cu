@@ -22,12 +22,14 @@
 //
 // Split.  All pages of all units form one line, cut into equal ranges, one per
 // CTA (the lengths are read on the device, so nothing is planned on the host).
-// A CTA fills an SM; two of its warps share a page, 32 tokens each, and each
-// warp copies its half pages through its own ring of cp.async stages: no barrier
-// until the range's end.  A unit that lies in one range is finished there;
-// otherwise each CTA leaves a partial (maximum, sum, accumulator) and the last
-// one to arrive (an atomic ticket) merges them in the order of the ranges, so
-// results do not depend on timing.
+// Before each unit's pages lie kUnitCost empty places, the cost of taking up
+// another unit in pages: a CTA whose range goes on into the next unit gets that
+// many fewer, and short ranges end at the units' ends.  Two warps share a page,
+// 32 tokens each, and each warp copies its half pages through its own ring of
+// cp.async stages: no barrier until the unit's end.  A unit that lies in one
+// range is finished there; otherwise each CTA leaves a partial (maximum, sum,
+// accumulator) and the last one to arrive (an atomic ticket) merges them in the
+// order of the ranges, so results do not depend on timing.
 #include <type_traits>
 
 #include "lf_int4.cuh"
@@ -45,6 +47,7 @@ struct AttendParams {
   float scale_log2;
   void* out;
   int64_t out_seq, out_head, out_tok;
+  bool out_aligned;           // four channels of an output row can be stored at once
   int rows, cols, col_tiles;  // sequences (or query tokens), query columns of a unit, column tiles
   float* partials;
   uint32_t* tickets;
@@ -55,25 +58,35 @@ constexpr int kHalfPage = kInt4Page / 2;  // tokens of a page that one warp take
 constexpr int kTile = 16;                 // tokens of one tensor-core step
 constexpr float kSlack = 8.0f;            // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
-constexpr int kMinPages = 3;  // pages of a range at least: below, merging costs more than the pages
+#ifndef LF_CTAS
+#define LF_CTAS 3
+#define LF_ST 3
+#endif
+#ifndef LF_MINP
+#define LF_MINP 4
+#define LF_COST 6
+#endif
+constexpr int kMinPages = LF_MINP;  // places of a range at least: one page for each pair of warps
+constexpr int kUnitCost = LF_COST;
 #ifndef LF_UNROLL
 #define LF_UNROLL 1
 #endif
 constexpr int kUnroll = LF_UNROLL;
 
-// Warps and stages per CTA: what the registers (12 warps of 168, or 8 of 255 with
-// 16 columns at D 128) and 227 KB of shared memory hold.
+// CTAs of four warps; as many per SM as the registers hold (168 a thread, or 255
+// with 16 columns at D 128), and the stages that 227 KB of shared memory hold.
+// Three or two CTAs hide each other's start and merge.
 template <int D, int NT> struct AttendCfg {
-  static constexpr int kWarps = D == 128 && NT == 2 ? 8 : 12;
-  static constexpr int kThreads = 32 * kWarps, kPairs = kWarps / 2;
-  static constexpr int kStages = D == 64 ? 6 : kWarps == 8 ? 5 : 3;
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kPairs = kWarps / 2;
+  static constexpr int kCtas = D == 128 && NT == 2 ? 2 : LF_CTAS;
+  static constexpr int kStages = kCtas == 2 ? 5 : (D == 64 ? 2 : 1) * (LF_CTAS == 3 ? 3 : LF_ST);
   static constexpr int kCodes = kHalfPage * D / 2, kPar = kHalfPage * D / 8;  // bytes of a half page, Key or Value
   static constexpr int kStageBytes = 2 * (kCodes + kPar);
   static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kMerge = kWarps * 8 * NT * (kPad + 2) * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial
+  static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial: maxima, sums, accumulators
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -156,6 +169,13 @@ __device__ __noinline__ bool value_has_nan(const AttendParams& p, int h, int b, 
   return nan;
 }
 
+__device__ __forceinline__ void add_scaled(float4& v, float f, float4 y) {
+  v.x = fmaf(f, y.x, v.x);
+  v.y = fmaf(f, y.y, v.y);
+  v.z = fmaf(f, y.z, v.z);
+  v.w = fmaf(f, y.w, v.w);
+}
+
 // Tokens that row r (a sequence, or a query token of one) sees at most.
 template <bool kSparse>
 __device__ __forceinline__ int row_tokens(const AttendParams& p, int r) {
@@ -172,31 +192,31 @@ __device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
 }
 
 template <typename T, int D, int NT, bool kSparse>
-__global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
+__global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::kCtas)
     int4_attend_kernel(const __grid_constant__ AttendParams p) {
   using C = AttendCfg<D, NT>;
   constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int meta_s[kWarps][kStages];  // first token of each stage's half page, -1: nothing to do
-  __shared__ float weight_s[kWarps][kCol], top_s[kCol], sum_s[kCol];
   __shared__ int last_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = p.pool.kv_heads * p.col_tiles;
   grid_dep_wait();
 
   // The line of pages: its length, and the row where this CTA's range begins.
-  int total = 0;
-  for (int r0 = 0; r0 < p.rows; r0 += 32) {
-    const int n = r0 + lane < p.rows ? row_pages<kSparse>(p, row_tokens<kSparse>(p, r0 + lane)) * per_row : 0;
-    total += __reduce_add_sync(0xffffffffu, n);
-  }
+  auto places = [&](int r) {
+    return r < p.rows ? (row_pages<kSparse>(p, row_tokens<kSparse>(p, r)) + kUnitCost) * per_row : 0;
+  };
+  const int places0 = places(lane);
+  int total = __reduce_add_sync(0xffffffffu, places0);
+  for (int r0 = 32; r0 < p.rows; r0 += 32) total += __reduce_add_sync(0xffffffffu, places(r0 + lane));
   const int per = max(kMinPages, static_cast<int>((total + gridDim.x - 1) / gridDim.x));
   const int begin = blockIdx.x * per, end = min(total, begin + per);
   if (begin >= end) return;
   int row = 0, row_base = 0;
   for (int r0 = 0; r0 < p.rows; r0 += 32) {
-    const int n = r0 + lane < p.rows ? row_pages<kSparse>(p, row_tokens<kSparse>(p, r0 + lane)) * per_row : 0;
+    const int n = r0 == 0 ? places0 : places(r0 + lane);
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -224,15 +244,35 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
   while (at < end) {
     // ------------------------------------------------------------ one unit
     const int seen_max = row_tokens<kSparse>(p, row), n_pages = row_pages<kSparse>(p, seen_max);
-    const int in_row = at - row_base, unit_in_row = in_row / n_pages;
-    const int unit_begin = row_base + unit_in_row * n_pages, unit_end = unit_begin + n_pages;
+    const int in_row = at - row_base, unit_in_row = in_row / (n_pages + kUnitCost);
+    const int unit_begin = row_base + unit_in_row * (n_pages + kUnitCost) + kUnitCost;  // its first page's place
+    const int unit_end = unit_begin + n_pages;
+    const int first = max(0, at - unit_begin), stop = min(end, unit_end) - unit_begin;
     const int h = unit_in_row / p.col_tiles, c0 = (unit_in_row - h * p.col_tiles) * kCol;
-    const int first = at - unit_begin, stop = min(end, unit_end) - unit_begin;
-    const int b = kSparse ? row / p.q_len : row;
-    const int i0 = kSparse ? row - b * p.q_len : 0;
+    at = unit_begin + stop;
+    const int row_now = row;
+    if (at - row_base == (n_pages + kUnitCost) * per_row) {
+      row_base = at;
+      ++row;
+    }
+    if (stop <= first) continue;
+    const int b = kSparse ? row_now / p.q_len : row_now;
+    const int i0 = kSparse ? row_now - b * p.q_len : 0;
     const int length = p.lengths[b], count = p.counts != nullptr ? p.counts[b] : p.q_len;
     if (tid == 0 && p.status != nullptr && (seen_max - 1) / kInt4Page >= p.pool.table_width)
       atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+
+    // Query column c of the unit is query token i0 + c / group of q-head h * group + c % group.
+    auto token_of = [&](int c) { return kSparse || p.q_len == 1 ? 0 : c / p.group; };
+    uint4 qw[NT][kG];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = c0 + nt * 8 + g, i = token_of(c);
+      const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (h * p.group + c - i * p.group) * p.q_head + (i0 + i) * p.q_tok;
+#pragma unroll
+      for (int G = 0; G < kG; ++G)
+        qw[nt][G] = c < p.cols ? *reinterpret_cast<const uint4*>(q + 32 * G + 8 * t) : make_uint4(0, 0, 0, 0);
+    }
 
     // This warp's pages: first + pair, then every kPairs-th.  Their ids, 32 at a
     // time, one per lane, loaded a window ahead.
@@ -243,7 +283,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
       if (x < mine_n) {
         logical = first + pair + x * C::kPairs;
         if constexpr (kSparse)
-          logical = p.picked[(static_cast<int64_t>(row) * p.pool.kv_heads + h) * p.slots + logical];
+          logical = p.picked[(static_cast<int64_t>(row_now) * p.pool.kv_heads + h) * p.slots + logical];
         if (logical >= 0 && static_cast<int64_t>(logical) * kInt4Page < seen_max) {
           id = int4_page_id(p.pool, b, logical);
           if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
@@ -297,15 +337,10 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
     const float flip = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int c = c0 + nt * 8 + g, i = c / p.group;
-      const bool live = c < p.cols;
-      const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (h * p.group + c - i * p.group) * p.q_head + (i0 + i) * p.q_tok;
       float x[kG][8], most = 0.0f;
 #pragma unroll
       for (int G = 0; G < kG; ++G) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (live) w = *reinterpret_cast<const uint4*>(q + 32 * G + 8 * t);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t v[4] = {qw[nt][G].x, qw[nt][G].y, qw[nt][G].z, qw[nt][G].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if constexpr (std::is_same<T, __half>::value) {
@@ -356,7 +391,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
         // positive, so that a masked score's -inf stays one
         c2[nt][k] = fmaxf(pow2(10 - kc) * fabsf(p.scale_log2), 1e-36f);
         const int col = min(c0 + nt * 8 + 2 * t + k, p.cols - 1);
-        vis[nt][k] = int4_seen(length, count, i0 + col / p.group);
+        vis[nt][k] = int4_seen(length, count, i0 + token_of(col));
       }
     }
     int vis_min = INT32_MAX;
@@ -610,112 +645,104 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, 1)
                           acc[nt][2 * G + 1][k + 2] * back);
       }
     __syncthreads();
-    if (tid < kCol) {
-      float top = top_w[tid], sum = 0.0f;
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, top_w[w * kCol + tid]);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(top_w[w * kCol + tid] - top);
-        weight_s[w][tid] = f;
-        sum = fmaf(f, sum_w[w * kCol + tid], sum);
-      }
-      top_s[tid] = top;
-      sum_s[tid] = sum;
-    }
-    __syncthreads();
 
     const bool whole = first == 0 && stop == n_pages;
     T* out = static_cast<T*>(p.out) + b * p.out_seq;
-    auto store = [&](int col, int d, float4 v, float inv) {
-      const int c = c0 + col, i = c / p.group;
+    auto store = [&](int col, int d, float4 v, float sum) {
+      const int c = c0 + col, i = token_of(c);
       if (c >= p.cols) return;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a column that sees nothing
       T* o = out + (h * p.group + c - i * p.group) * p.out_head + (i0 + i) * p.out_tok + d;
-      Scalar<T>::store(o, v.x * inv);
-      Scalar<T>::store(o + 1, v.y * inv);
-      Scalar<T>::store(o + 2, v.z * inv);
-      Scalar<T>::store(o + 3, v.w * inv);
+      if (p.out_aligned) {
+        struct alignas(4 * sizeof(T)) Four { T x[4]; } f;
+        Scalar<T>::store(f.x, v.x * inv);
+        Scalar<T>::store(f.x + 1, v.y * inv);
+        Scalar<T>::store(f.x + 2, v.z * inv);
+        Scalar<T>::store(f.x + 3, v.w * inv);
+        *reinterpret_cast<Four*>(o) = f;
+      } else {
+        Scalar<T>::store(o, v.x * inv);
+        Scalar<T>::store(o + 1, v.y * inv);
+        Scalar<T>::store(o + 2, v.z * inv);
+        Scalar<T>::store(o + 3, v.w * inv);
+      }
     };
     // The partial of range x of this unit: the range that begins inside the unit
     // uses its CTA's first record, the unit's first range the second.
     const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per, parts = last_cta - first_cta + 1;
     auto record = [&](int x) { return p.partials + (2 * static_cast<int64_t>(x) + (x == first_cta)) * C::kRecord; };
     float* mine = record(blockIdx.x);
-    for (int item = tid; item < kCol * D / 4; item += C::kThreads) {
-      const int col = item / (D / 4), d = item % (D / 4) * 4;
+    constexpr int kItems = kCol * D / 4 / C::kThreads;  // (column, four channels) a thread merges
+#pragma unroll
+    for (int it = 0; it < kItems; ++it) {
+      const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
+      float top = top_w[col], sum = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, top_w[w * kCol + col]);
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = weight_s[w][col];
-        const float4 y = *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d);
-        v.x = fmaf(f, y.x, v.x);
-        v.y = fmaf(f, y.y, v.y);
-        v.z = fmaf(f, y.z, v.z);
-        v.w = fmaf(f, y.w, v.w);
+        const float f = ex2(top_w[w * kCol + col] - top);
+        sum = fmaf(f, sum_w[w * kCol + col], sum);
+        add_scaled(v, f, *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d));
       }
       if (whole) {
-        const float sum = sum_s[col];
-        store(col, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+        store(col, d, v, sum);
       } else {
         *reinterpret_cast<float4*>(mine + 2 * kCol + col * D + d) = v;
+        if (d == 0) {
+          mine[col] = top;
+          mine[kCol + col] = sum;
+        }
       }
     }
     if (!whole) {
-      if (tid < kCol) {
-        mine[tid] = top_s[tid];
-        mine[kCol + tid] = sum_s[tid];
-      }
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
-        uint32_t* ticket = p.tickets + static_cast<int64_t>(row) * per_row + unit_in_row;
+        __threadfence();  // the CTA's partial, ordered before by the barrier, is visible before its ticket
+        uint32_t* ticket = p.tickets + static_cast<int64_t>(row_now) * per_row + unit_in_row;
         const uint32_t n = atomicAdd(ticket, 1u) + 1;
         if (n == static_cast<uint32_t>(parts)) *ticket = 0;  // every range has arrived: ready for the next call
+        __threadfence();
         last_s = n == static_cast<uint32_t>(parts);
       }
       __syncthreads();
       if (last_s) {
-        __threadfence();
-        // Weights of the parts (and their sum, by column), then their weighted sum.
-        float* part_w = reinterpret_cast<float*>(smem);  // [parts][kCol], the merge buffer is free
-        for (int x = tid; x < parts * kCol; x += C::kThreads) part_w[x] = __ldcg(record(first_cta + x / kCol) + x % kCol);
-        __syncthreads();
-        for (int col = warp; col < kCol; col += kWarps) {
+#pragma unroll 1
+        for (int it = 0; it < kItems; ++it) {
+          const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
+          constexpr int kAtOnce = 8;  // parts whose loads are in flight together
           float top = kNoMax, sum = 0.0f;
-          for (int x = lane; x < parts; x += 32) top = fmaxf(top, part_w[x * kCol + col]);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          for (int x = lane; x < parts; x += 32) {
-            const float f = ex2(part_w[x * kCol + col] - top);
-            part_w[x * kCol + col] = f;
-            sum = fmaf(f, __ldcg(record(first_cta + x) + kCol + col), sum);
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (lane == 0) sum_s[col] = sum;
-        }
-        __syncthreads();
-        for (int item = tid; item < kCol * D / 4; item += C::kThreads) {
-          const int col = item / (D / 4), d = item % (D / 4) * 4;
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-          for (int x = 0; x < parts; ++x) {
-            const float f = part_w[x * kCol + col];
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(record(first_cta + x) + 2 * kCol + col * D + d));
-            v.x = fmaf(f, y.x, v.x);
-            v.y = fmaf(f, y.y, v.y);
-            v.z = fmaf(f, y.z, v.z);
-            v.w = fmaf(f, y.w, v.w);
+          for (int x0 = 0; x0 < parts; x0 += kAtOnce) {
+            float tops[kAtOnce], sums[kAtOnce];
+            float4 y[kAtOnce];
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+              const float* rec = record(first_cta + min(x0 + x, parts - 1));
+              tops[x] = __ldcg(rec + col);
+              sums[x] = __ldcg(rec + kCol + col);
+              y[x] = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
+            }
+            float now = top;
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) now = fmaxf(now, tops[x]);
+            const float fix = ex2(top - now);
+            top = now;
+            sum *= fix;
+            v = make_float4(v.x * fix, v.y * fix, v.z * fix, v.w * fix);
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+              const float f = x0 + x < parts ? ex2(tops[x] - top) : 0.0f;
+              if (x0 + x < parts) {
+                sum = fmaf(f, sums[x], sum);
+                add_scaled(v, f, y[x]);
+              }
+            }
           }
-          const float sum = sum_s[col];
-          store(col, d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+          store(col, d, v, sum);
         }
       }
-    }
-    at = unit_begin + stop;
-    if (at - row_base == n_pages * per_row) {
-      row_base = at;
-      ++row;
     }
     __syncthreads();  // the merge buffer is free for the next unit's stages
   }
@@ -727,9 +754,14 @@ static int sm_count() {
     return 0;
   return n;
 }
-// The partials: two records per CTA, one CTA per SM, of 16 columns at most.
+// The partials: two records per CTA of the largest grid.
 static size_t partial_bytes(int sms) {
-  return static_cast<size_t>(sms) * 2 * AttendCfg<128, 2>::kRecord * sizeof(float);
+  using A = AttendCfg<128, 1>;
+  using B = AttendCfg<128, 2>;
+  using E = AttendCfg<64, 2>;
+  constexpr int a = A::kCtas * A::kRecord, b = B::kCtas * B::kRecord, e = E::kCtas * E::kRecord;
+  constexpr int most = a > b ? (a > e ? a : e) : (b > e ? b : e);
+  return static_cast<size_t>(sms) * 2 * most * sizeof(float);
 }
 
 template <typename T, int D, int NT, bool kSparse>
@@ -742,10 +774,11 @@ static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
     return LF_ERR_CUDA;
   }
   // No more CTAs than ranges there can be.
-  const int64_t pages = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles * (kSparse ? p.slots : p.pool.table_width);
-  const int64_t ranges = (pages + kMinPages - 1) / kMinPages;
+  const int64_t units = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles;
+  const int64_t pages = units * (kSparse ? p.slots : p.pool.table_width);
+  const int64_t ranges = (pages + units * kUnitCost + kMinPages - 1) / kMinPages, slots = static_cast<int64_t>(sms) * C::kCtas;
   void* args[] = {&p};
-  err = launch_programmatic(kern, dim3(static_cast<unsigned>(ranges < sms ? ranges : sms)), dim3(C::kThreads), C::kSmem,
+  err = launch_programmatic(kern, dim3(static_cast<unsigned>(ranges < slots ? ranges : slots)), dim3(C::kThreads), C::kSmem,
                             stream, args);
   if (err != cudaSuccess) {
     set_error("lf_int4_attend: %s", cudaGetErrorString(err));
@@ -809,11 +842,12 @@ extern "C" int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void
   p.out_seq = out_seq_stride;
   p.out_head = out_head_stride;
   p.out_tok = out_tok_stride;
+  p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && (out_seq_stride | out_head_stride | out_tok_stride) % 4 == 0;
   p.rows = picked ? p.pool.batch * q_len : p.pool.batch;
   p.cols = picked ? p.group : p.group * q_len;
   p.col_tiles = (p.cols + lf::tile_columns(p.cols) - 1) / lf::tile_columns(p.cols);
   LF_CHECK_SUPPORTED(static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles <=
-                         (1 << 30) / (picked ? slots : p.pool.table_width),
+                         (1 << 30) / ((picked ? slots : p.pool.table_width) + lf::kUnitCost),
                      "lf_int4_attend: %d sequences of %d pages are too many for one call", p.pool.batch,
                      p.pool.table_width);
   p.partials = static_cast<float*>(workspace);
