@@ -54,14 +54,9 @@ struct AttendParams {
   int32_t* status;
 };
 
-constexpr int kHalfPage = kInt4Page / 2;  // tokens of a page that one warp takes
-constexpr int kTile = 16;                 // tokens of one tensor-core step
+constexpr int kTile = 16;  // tokens of one tensor-core step
 constexpr float kSlack = 8.0f;            // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
-#ifndef LF_CTAS
-#define LF_CTAS 3
-#define LF_ST 3
-#endif
 #ifndef LF_MINP
 #define LF_MINP 4
 #define LF_COST 6
@@ -69,18 +64,24 @@ constexpr float kNoMax = -1e30f;
 constexpr int kMinPages = LF_MINP;  // places of a range at least: one page for each pair of warps
 constexpr int kUnitCost = LF_COST;
 #ifndef LF_UNROLL
-#define LF_UNROLL 1
+#define LF_UNROLL 2
 #endif
 constexpr int kUnroll = LF_UNROLL;
 
 // CTAs of four warps; as many per SM as the registers hold (168 a thread, or 255
 // with 16 columns at D 128), and the stages that 227 KB of shared memory hold.
 // Three or two CTAs hide each other's start and merge.
+#ifndef LF_PART
+#define LF_PART 32
+#define LF_CTAS 3
+#define LF_ST 3
+#endif
 template <int D, int NT> struct AttendCfg {
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kPairs = kWarps / 2;
+  static constexpr int kPart = LF_PART, kShare = kInt4Page / kPart;  // tokens of a page that a warp takes, warps that share it
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kTeams = kWarps / kShare;
   static constexpr int kCtas = D == 128 && NT == 2 ? 2 : LF_CTAS;
-  static constexpr int kStages = kCtas == 2 ? 5 : (D == 64 ? 2 : 1) * (LF_CTAS == 3 ? 3 : LF_ST);
-  static constexpr int kCodes = kHalfPage * D / 2, kPar = kHalfPage * D / 8;  // bytes of a half page, Key or Value
+  static constexpr int kStages = kCtas == 2 ? 5 : (D == 64 ? 2 : 1) * LF_ST;
+  static constexpr int kCodes = kPart * D / 2, kPar = kPart * D / 8;  // bytes of a warp's part, Key or Value
   static constexpr int kStageBytes = 2 * (kCodes + kPar);
   static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
   static constexpr int kRing = kWarps * kStages * kStageBytes;
@@ -101,10 +102,17 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+// The same from zero.
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma1688_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -131,13 +139,13 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// Codes of bits 0-3 (4-7) of both halves as exact fp16 numbers: 1024 + c (+ 16 c)
-// by its bit pattern, brought back by one fma.
-__device__ __forceinline__ uint32_t even_code(uint32_t x) {
-  return hfma2((x & 0x000f000fu) | 0x64006400u, 0x3C003C00u, 0xE400E400u);  // * 1 - 1024
-}
-__device__ __forceinline__ uint32_t odd_code(uint32_t x) {
-  return hfma2((x & 0x00f000f0u) | 0x64006400u, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
+// Codes n0 and n1 of a byte n0 + 16 n1 in both halves, as exact fp16 numbers, from
+// x = 1024 + byte: 1024 + 16 n1 by its bits, brought back by one fma, and what it
+// leaves of x.
+__device__ __forceinline__ void two_codes(uint32_t x, uint32_t& even, uint32_t& odd) {
+  const uint32_t high = x & 0xFFF0FFF0u;
+  odd = hfma2(high, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(even) : "r"(x), "r"(high));
 }
 __device__ __forceinline__ bool is_nan_param(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
 // Larger magnitude of each half (a NaN gives way to a number).
@@ -235,11 +243,11 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
   uint8_t* ring = smem + warp * kStages * C::kStageBytes;
   const uint32_t ring_a = smem_addr(ring) + lane * 16;
-  const int pair = warp >> 1, half = warp & 1;
+  const int team = warp / C::kShare, part = warp % C::kShare;
   // Byte offsets in a record of this lane's pieces: Key codes (Value codes 40 D
   // later), and parameters, the first half of the lanes Key's, the others Value's.
   constexpr int kParLanes = kPar / 16;  // lanes' worth of a half page's Key parameters
-  const int code_at = half * kCodes + lane * 16;
+  const int code_at = part * kCodes + lane * 16;
   int at = begin;
   while (at < end) {
     // ------------------------------------------------------------ one unit
@@ -274,14 +282,14 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         qw[nt][G] = c < p.cols ? *reinterpret_cast<const uint4*>(q + 32 * G + 8 * t) : make_uint4(0, 0, 0, 0);
     }
 
-    // This warp's pages: first + pair, then every kPairs-th.  Their ids, 32 at a
+    // This warp's pages: first + team, then every kTeams-th.  Their ids, 32 at a
     // time, one per lane, loaded a window ahead.
-    const int mine_n = first + pair < stop ? (stop - first - pair + C::kPairs - 1) / C::kPairs : 0;
+    const int mine_n = first + team < stop ? (stop - first - team + C::kTeams - 1) / C::kTeams : 0;
     auto load_ids = [&](int x0, int& id, int& logical) {
       const int x = x0 + lane;
       id = logical = -1;
       if (x < mine_n) {
-        logical = first + pair + x * C::kPairs;
+        logical = first + team + x * C::kTeams;
         if constexpr (kSparse)
           logical = p.picked[(static_cast<int64_t>(row_now) * p.pool.kv_heads + h) * p.slots + logical];
         if (logical >= 0 && static_cast<int64_t>(logical) * kInt4Page < seen_max) {
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         }
         const int id = __shfl_sync(0xffffffffu, ids, issued & 31);
         const int logical = __shfl_sync(0xffffffffu, logicals, issued & 31);
-        if (lane == 0) meta_s[warp][into] = id < 0 ? -1 : logical * kInt4Page + half * kHalfPage;
+        if (lane == 0) meta_s[warp][into] = id < 0 ? -1 : logical * kInt4Page + part * C::kPart;
         if (id >= 0) {
           const uint8_t* rec = head_words + id * p.pool.page_stride * 4;
           const uint32_t dst = ring_a + into * C::kStageBytes;
@@ -315,11 +323,12 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             cp_async16(dst + kCodes + x * 512, kc + 40 * D + x * 512);
           }
           if constexpr (kParLanes == 32) {
-            cp_async16(dst + 2 * kCodes, rec + 32 * D + half * kPar + lane * 16);
-            cp_async16(dst + 2 * kCodes + 512, rec + 72 * D + half * kPar + lane * 16);
+            cp_async16(dst + 2 * kCodes, rec + 32 * D + part * kPar + lane * 16);
+            cp_async16(dst + 2 * kCodes + 512, rec + 72 * D + part * kPar + lane * 16);
           } else {
             const int v = lane / kParLanes;
-            cp_async16(dst + 2 * kCodes, rec + 32 * D + v * 40 * D + half * kPar + (lane - v * kParLanes) * 16);
+            if (kParLanes == 16 || lane < 2 * kParLanes)
+              cp_async16(dst + 2 * kCodes, rec + 32 * D + v * 40 * D + part * kPar + (lane - v * kParLanes) * 16);
           }
         }
         ++issued;
@@ -424,19 +433,21 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       uint8_t* stage = ring + st * C::kStageBytes;
       st = st + 1 == kStages ? 0 : st + 1;
       if (base < 0 || base >= seen_max) continue;
-      const bool masked = base + kHalfPage > vis_min;  // tokens here that not every column sees
+      const bool masked = base + C::kPart > vis_min;  // tokens here that not every column sees
 
       // Value parameters in pairs of tokens, as the fragments take them: in place
       // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
       {
-        constexpr int kQ = kG / 2;  // words of each token a lane holds: its groups q kQ .. q kQ + kQ - 1
-        const int x = lane >> 1, q = lane & 1;
+        // lanes per pair of tokens (16 or 8 pairs), and the groups of a lane
+        constexpr int kLanes = C::kPart == 32 ? 2 : kG, kQ = kG / kLanes;
+        const int x = lane / kLanes, q = lane % kLanes;
+        const bool busy = x < C::kPart / 2;
         uint32_t* par = reinterpret_cast<uint32_t*>(stage + 2 * kCodes + kPar);
         uint32_t e[kQ], o[kQ];
 #pragma unroll
         for (int k = 0; k < kQ; ++k) {
-          e[k] = par[2 * x * kG + q * kQ + k];
-          o[k] = par[(2 * x + 1) * kG + q * kQ + k];
+          e[k] = busy ? par[2 * x * kG + q * kQ + k] : 0;
+          o[k] = busy ? par[(2 * x + 1) * kG + q * kQ + k] : 0;
         }
         if (masked) {
           // What an unwritten slot holds must not be read; a NaN that only some
@@ -478,16 +489,16 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         __syncwarp();  // every lane has read its words
         if constexpr (kQ == 2)
           *reinterpret_cast<uint4*>(par + 4 * lane) = make_uint4(s2[0], z2[0], s2[1], z2[1]);
-        else
+        else if (busy)
           *reinterpret_cast<uint2*>(par + 2 * lane) = make_uint2(s2[0], z2[0]);
         __syncwarp();
       }
 
 #pragma unroll kUnroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const uint8_t* kcode = stage + sub * (kCodes / 2);
+      for (int sub = 0; sub < C::kPart / kTile; ++sub) {
+        const uint8_t* kcode = stage + sub * (kTile * D / 2);
         const uint8_t* vcode = kcode + kCodes;
-        const uint8_t* kpar = stage + 2 * kCodes + sub * (kPar / 2);
+        const uint8_t* kpar = stage + 2 * kCodes + sub * (kTile * D / 8);
         const uint8_t* vpair = kpar + kPar;
 
         // Scores of 16 tokens (rows g and g + 8 of the fragment).
@@ -502,9 +513,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         float x[NT][4], dot[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          mma1688_zero(x[nt], kz[0], kz[1], qz[nt]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[nt][k] = dot[nt][k] = 0.0f;
-          mma1688(x[nt], kz[0], kz[1], qz[nt]);
+          for (int k = 0; k < 4; ++k) dot[nt][k] = 0.0f;
         }
 #pragma unroll
         for (int G = 0; G < kG; ++G) {
@@ -512,11 +523,11 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           const float s0 = half_lo(ks[0][G]), s1 = half_lo(ks[1][G]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              mma16816(d, a[k][0] & 0x000f000fu, a[k][1] & 0x000f000fu, a[k][0] & 0x00f000f0u, a[k][1] & 0x00f000f0u,
-                       qf[nt][2 * G + k][0], qf[nt][2 * G + k][1]);
+            float d[4];
+            mma16816_zero(d, a[0][0] & 0x000f000fu, a[0][1] & 0x000f000fu, a[0][0] & 0x00f000f0u, a[0][1] & 0x00f000f0u,
+                          qf[nt][2 * G][0], qf[nt][2 * G][1]);
+            mma16816(d, a[1][0] & 0x000f000fu, a[1][1] & 0x000f000fu, a[1][0] & 0x00f000f0u, a[1][1] & 0x00f000f0u,
+                     qf[nt][2 * G + 1][0], qf[nt][2 * G + 1][1]);
             dot[nt][0] = fmaf(d[0], s0, dot[nt][0]);
             dot[nt][1] = fmaf(d[1], s0, dot[nt][1]);
             dot[nt][2] = fmaf(d[2], s1, dot[nt][2]);
@@ -604,12 +615,15 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const uint32_t s2 = sz[r][2 * G], z2 = sz[r][2 * G + 1];
-            // codes of the even and the odd token: words [token][w]
-            const uint32_t y = __byte_perm(vw[r][G >> 1], vw[r][kG / 2 + (G >> 1)], (G & 1) ? 0x7632 : 0x5410);
-            v[r][0] = hfma2(even_code(y), s2, z2);
-            v[r][1] = hfma2(odd_code(y), s2, z2);
-            v[r][2] = hfma2(even_code(y >> 8), s2, z2);
-            v[r][3] = hfma2(odd_code(y >> 8), s2, z2);
+            // bytes of the even and the odd token (words [token][w]), as 1024 + byte
+            const uint32_t y = __byte_perm(vw[r][G >> 1], vw[r][kG / 2 + (G >> 1)], (G & 1) ? 0x7362 : 0x5140);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t even, odd;
+              two_codes(__byte_perm(y, 0x64646464u, k == 0 ? 0x4140 : 0x4342), even, odd);
+              v[r][2 * k] = hfma2(even, s2, z2);
+              v[r][2 * k + 1] = hfma2(odd, s2, z2);
+            }
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {

@@ -36,6 +36,7 @@ from logitfill_b200 import _lib
 
 PAGE_TOKENS = 64   # tokens of a page
 GROUP = 32         # channels that share a scale and a minimum
+_CODE = {torch.float32: _lib.LF_F32, torch.float16: _lib.LF_F16, torch.bfloat16: _lib.LF_BF16}
 
 
 def record_words(head_dim: int) -> int:
@@ -59,30 +60,32 @@ def alloc_bounds(n_pages: int, n_kv: int, head_dim: int, device="cuda") -> torch
 
 
 def _pool(pages: torch.Tensor, page_table: torch.Tensor):
-    """The C ABI's pool of ``pages`` and ``page_table``, and the head_dim."""
-    if pages.dim() != 3 or pages.dtype != torch.int32 or pages.stride(2) != 1:
-        raise ValueError(f"pages must be int32 [n_pages, n_kv, words] with word stride 1, got {pages.dtype} "
-                         f"{tuple(pages.shape)}")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+    """The C ABI's pool of ``pages`` and ``page_table``, the head_dim and the device."""
+    shape, strides = pages.shape, pages.stride()
+    if len(shape) != 3 or pages.dtype != torch.int32 or strides[2] != 1:
+        raise ValueError(f"pages must be int32 [n_pages, n_kv, words] with word stride 1, got {pages.dtype} {tuple(shape)}")
+    table_shape, table_strides = page_table.shape, page_table.stride()
+    if len(table_shape) != 2 or page_table.dtype != torch.int32 or table_strides[1] != 1:
         raise ValueError(f"page_table must be int32 [batch, width] with entry stride 1, got {page_table.dtype} "
-                         f"{tuple(page_table.shape)}")
-    if not pages.is_cuda:
+                         f"{tuple(table_shape)}")
+    device = pages.device
+    if device.type != "cuda":
         raise RuntimeError("the 4-bit cache needs CUDA tensors (there is no CPU path)")
-    if page_table.device != pages.device:
-        raise RuntimeError(f"page_table is on {page_table.device}, pages on {pages.device}")
-    n, H, words = pages.shape
+    if page_table.device != device:
+        raise RuntimeError(f"page_table is on {page_table.device}, pages on {device}")
+    n, H, words = shape
+    B, W = table_shape
     if words % 20:
         raise ValueError(f"a record of {words} words belongs to no head_dim (20 * head_dim words)")
-    B, W = page_table.shape
-    return _lib.LfInt4Pool(pages.data_ptr(), page_table.data_ptr(), pages.stride(0) if n > 1 else H * words,
-                           pages.stride(1) if H > 1 else words, page_table.stride(0) if B > 1 else W, W, n, H, B), words // 20
+    return _lib.LfInt4Pool(pages.data_ptr(), page_table.data_ptr(), strides[0] if n > 1 else H * words,
+                           strides[1] if H > 1 else words, table_strides[0] if B > 1 else W, W, n, H, B), words // 20, device
 
 
 def _per_sequence(name: str, t: torch.Tensor | None, batch: int, device) -> int:
     """Address of an int32 [batch] tensor (0 for None)."""
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.shape != (batch,) or not (t.is_contiguous() and t.device == device):
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [{batch}] tensor on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -109,19 +112,25 @@ def _bounds(bounds: torch.Tensor, pages: torch.Tensor, head_dim: int):
 def _aligned_rows(t: torch.Tensor):
     """``t`` [B, H, T, D] with 16-byte aligned rows of channel stride 1 (a copy
     where it is not), and its first three strides (0 where the extent is 1)."""
-    unit = 16 // t.element_size()
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in strides):
+    (s0, s1, s2, s3), (n0, n1, n2, _) = t.stride(), t.shape
+    s0, s1, s2 = s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+    if s3 != 1 or t.data_ptr() % 16 or (s0 | s1 | s2) * t.element_size() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = list(t.stride()[:3])
-    return t, strides
+        s0, s1, s2, _ = t.stride()
+    return t, s0, s1, s2
+
+
+def _stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _on:
     """Makes ``device`` current for a launch (nothing to do when it is)."""
 
+    __slots__ = ("guard",)
+
     def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
@@ -142,27 +151,26 @@ def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page
     is written is brought up to date (a sparse call needs it).  A group of 32
     channels whose scale or minimum is no finite fp16 number (a NaN, an
     infinity, a range past 15 * 65504) reads back as NaN."""
-    pool, D = _pool(pages, page_table)
+    pool, D, dev = _pool(pages, page_table)
     B, H = pool.batch, pool.kv_heads
     if key.dim() != 4 or key.shape != value.shape or (key.shape[0], key.shape[1], key.shape[3]) != (B, H, D):
         raise ValueError(f"key and value must be [{B}, {H}, T, {D}], got {tuple(key.shape)} and {tuple(value.shape)}")
     if key.dtype != value.dtype:
         raise ValueError(f"key is {key.dtype}, value {value.dtype}")
-    dev = pages.device
     if key.device != dev or value.device != dev:
         raise RuntimeError(f"key and value must be on {dev}")
     code = _lib.dtype_code(key.dtype)
     addresses = (_per_sequence("start", start, B, dev), _per_sequence("counts", counts, B, dev))
     if key.shape[2] == 0:
         return
-    key, ks = _aligned_rows(key)
-    value, vs = _aligned_rows(value)
+    key, *ks = _aligned_rows(key)
+    value, *vs = _aligned_rows(value)
     bp, b0, b1 = (0, 0, 0) if bounds is None else _bounds(bounds, pages, D)
     with _on(dev):
         _lib.check(_lib.lib().lf_int4_write(
             ctypes.byref(pool), D, key.data_ptr(), value.data_ptr(), code, *ks, *vs, key.shape[2],
             *addresses, bp, b0, b1,
-            _status(status, dev), _lib.stream_handle(dev)), "lf_int4_write")
+            _status(status, dev), _stream(dev)), "lf_int4_write")
 
 
 def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor, tokens: int,
@@ -170,19 +178,19 @@ def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor
     """Positions ``start[b] .. start[b] + tokens - 1`` of every sequence as Key and
     Value ``[batch, n_kv, tokens, head_dim]`` in ``dtype`` (fp32, fp16 or
     bf16); tokens ``i >= counts[b]`` are zeros."""
-    pool, D = _pool(pages, page_table)
+    pool, D, dev = _pool(pages, page_table)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"cannot read {tokens} tokens")
-    dev, code = pages.device, _lib.dtype_code(dtype)
+    code = _lib.dtype_code(dtype)
     out = torch.empty(2, pool.batch, pool.kv_heads, tokens, D, dtype=dtype, device=dev)
-    key, value = out.unbind(0)
+    key, value = out[0], out[1]
     addresses = (_per_sequence("start", start, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev))
     if tokens:
         with _on(dev):
             _lib.check(_lib.lib().lf_int4_read(
                 ctypes.byref(pool), D, *addresses, tokens, key.data_ptr(), value.data_ptr(), code, _status(status, dev),
-                _lib.stream_handle(dev)), "lf_int4_read")
+                _stream(dev)), "lf_int4_read")
     return key, value
 
 
@@ -199,71 +207,92 @@ def int4_read_bounds(bounds: torch.Tensor) -> torch.Tensor:
     with _on(bounds.device):
         _lib.check(_lib.lib().lf_int4_read_bounds(
             bounds.data_ptr(), bounds.stride(0) if n > 1 else H * width, bounds.stride(1) if H > 1 else width, n, H, D,
-            out.data_ptr(), _lib.stream_handle(bounds.device)), "lf_int4_read_bounds")
+            out.data_ptr(), _stream(bounds.device)), "lf_int4_read_bounds")
     return out
 
 
 _workspaces: dict = {}
 
 
-def _workspace(need: int, device) -> torch.Tensor:
+def _workspace(pool, n_q: int, q_len: int, head_dim: int, device) -> torch.Tensor:
     """Scratch of an attention call: partial results, then tickets that are zero
     between calls.  Calls on one stream share one buffer (they run in order);
     a call being captured in a CUDA graph gets its own, which the graph keeps
     and clears, so replays on any stream do not meet."""
-    if torch.cuda.is_current_stream_capturing():
+    key = (device.index, _stream(device))
+    # a ticket for each column tile of 16 at most, of each query token and KV head
+    units = pool.batch * pool.kv_heads * q_len * (n_q // pool.kv_heads + 15)
+    held = _workspaces.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
+    if held is not None and held[1] >= units and not capturing:
+        return held[0]
+    so = _lib.lib()
+    need = so.lf_int4_workspace_bytes(pool.batch, pool.kv_heads, n_q, q_len, head_dim)
+    if capturing:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        ws[_lib.lib().lf_int4_workspace_clear_from():].zero_()
+        ws[so.lf_int4_workspace_clear_from():].zero_()
         return ws
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < need:
-        ws = _workspaces[key] = torch.zeros(need + need // 8, dtype=torch.uint8, device=device)
+    units = max(units, 1 << 16)
+    ws = torch.zeros(max(need, so.lf_int4_workspace_clear_from() + 4 * units), dtype=torch.uint8, device=device)
+    _workspaces[key] = ws, units
     return ws
 
 
 def _query(query: torch.Tensor, pool, head_dim: int, device):
     """The query, checked, as [B, n_q, q_len, D] with 16-byte aligned rows of
     channel stride 1, and its first three strides."""
-    q = query.unsqueeze(2) if query.dim() == 3 else query
-    if q.dim() != 4 or q.shape[0] != pool.batch or q.shape[3] != head_dim or q.shape[1] < 1 or q.shape[2] < 1:
+    q = query if query.dim() == 4 else query.unsqueeze(2)
+    if q.dim() != 4:
+        raise ValueError(f"query must be [batch, n_q, head_dim] or [batch, n_q, q_len, head_dim], got {tuple(query.shape)}")
+    B, n_q, q_len, D = q.shape
+    if B != pool.batch or D != head_dim or n_q < 1 or q_len < 1:
         raise ValueError(f"query must be [{pool.batch}, n_q, {head_dim}] or [{pool.batch}, n_q, q_len, {head_dim}], got "
                          f"{tuple(query.shape)}")
-    if q.shape[1] % pool.kv_heads:
-        raise ValueError(f"{q.shape[1]} query heads do not divide into {pool.kv_heads} KV heads")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    if n_q % pool.kv_heads:
+        raise ValueError(f"{n_q} query heads do not divide into {pool.kv_heads} KV heads")
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise NotImplementedError(f"the 4-bit cache's attention takes fp16 or bf16 queries, got {q.dtype}")
     if q.device != device:
         raise RuntimeError(f"query is on {q.device}, pages on {device}")
     return _aligned_rows(q)
 
 
-def _attend(query, pages, page_table, lengths, scaling, counts, picked, out, status):
-    pool, D = _pool(pages, page_table)
-    dev = pages.device
-    q, qs = _query(query, pool, D, dev)
+def _out(query: torch.Tensor, out: torch.Tensor | None, device) -> torch.Tensor:
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride(-1) != 1:
-        raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} on {dev} with channel stride 1")
-    o = out.unsqueeze(2) if out.dim() == 3 else out
-    n_q, q_len = q.shape[1], q.shape[2]
-    slots = 0
-    if picked is not None:
-        if picked.dtype != torch.int32 or picked.shape[:-1] != (pool.batch, q_len, pool.kv_heads) \
-                or not picked.is_contiguous() or picked.device != dev:
-            raise ValueError(f"picked must be contiguous int32 [{pool.batch}, {q_len}, {pool.kv_heads}, slots] on {dev}, got "
-                             f"{picked.dtype} {tuple(picked.shape)} on {picked.device}")
-        slots = picked.shape[-1]
-    so = _lib.lib()
-    with _on(dev):
-        ws = _workspace(so.lf_int4_workspace_bytes(pool.batch, pool.kv_heads, n_q, q_len, D), dev)
-        _lib.check(so.lf_int4_attend(
-            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), *qs, q_len, n_q,
-            _per_sequence("lengths", lengths, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev),
-            _lib.ptr(picked), slots, float(scaling), o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), ws.data_ptr(),
-            ws.numel(), _status(status, dev), _lib.stream_handle(dev)), "lf_int4_attend")
+        return torch.empty_like(query, memory_format=torch.contiguous_format)
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1:
+        raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} on {device} with channel stride 1")
     return out
+
+
+def _attend(pool, D, dev, q, lengths: int, counts: int, picked: int, slots: int, scaling: float, out: torch.Tensor,
+            status: int) -> None:
+    """Launch the attention of ``q`` (from :func:`_query`) into ``out``; ``lengths``,
+    ``counts``, ``picked`` and ``status`` are addresses."""
+    t, s0, s1, s2 = q
+    n_q, q_len = t.shape[1], t.shape[2]
+    strides = out.stride()
+    ws = _workspace(pool, n_q, q_len, D, dev)
+    _lib.check(_lib.lib().lf_int4_attend(
+        ctypes.byref(pool), D, t.data_ptr(), _CODE[t.dtype], s0, s1, s2, q_len, n_q, lengths, counts, picked, slots,
+        scaling, out.data_ptr(), strides[0], strides[1], strides[2] if len(strides) == 4 else 0, ws.data_ptr(), ws.numel(),
+        status, _stream(dev)), "lf_int4_attend")
+
+
+def _select(pool, D, dev, q, bounds: torch.Tensor, pages: torch.Tensor, lengths: int, counts: int, top_pages: int,
+            sink_pages: int, recent_pages: int, status: int) -> torch.Tensor:
+    """Launch the page choice of ``q`` (from :func:`_query`)."""
+    t, s0, s1, s2 = q
+    n_q, q_len = t.shape[1], t.shape[2]
+    top, sink, recent = int(top_pages), int(sink_pages), int(recent_pages)
+    if top < 0 or sink < 0 or recent < 1:
+        raise ValueError(f"top {top} and sink {sink} must not be negative, recent {recent} at least 1")
+    bp, b0, b1 = _bounds(bounds, pages, D)
+    picked = torch.empty((pool.batch, q_len, pool.kv_heads, sink + recent + top), dtype=torch.int32, device=dev)
+    _lib.check(_lib.lib().lf_int4_select(
+        ctypes.byref(pool), D, t.data_ptr(), _CODE[t.dtype], s0, s1, s2, q_len, n_q, bp, b0, b1, lengths, counts, top, sink,
+        recent, picked.data_ptr(), status, _stream(dev)), "lf_int4_select")
+    return picked
 
 
 def int4_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -276,7 +305,13 @@ def int4_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.T
     positions ``0 .. lengths[b] - q_len + i``.  With ``counts`` (int32
     ``[batch]``) sequence ``b`` has only its first ``counts[b]`` query tokens;
     the others, and those that see nothing, get zeros."""
-    return _attend(query, pages, page_table, lengths, scaling, counts, None, out, status)
+    pool, D, dev = _pool(pages, page_table)
+    q = _query(query, pool, D, dev)
+    out = _out(query, out, dev)
+    with _on(dev):
+        _attend(pool, D, dev, q, _per_sequence("lengths", lengths, pool.batch, dev),
+                _per_sequence("counts", counts, pool.batch, dev), 0, 0, scaling, out, _status(status, dev))
+    return out
 
 
 def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
@@ -288,22 +323,12 @@ def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, 
     the page being filled) are always in; of the rest the ``top_pages`` with
     the largest bound on the scores of the KV head's queries (summed over its
     query heads; ties to the lower page)."""
-    pool, D = _pool(pages, page_table)
-    dev = pages.device
-    q, qs = _query(query, pool, D, dev)
-    n_q, q_len = q.shape[1], q.shape[2]
-    top, sink, recent = int(top_pages), int(sink_pages), int(recent_pages)
-    if top < 0 or sink < 0 or recent < 1:
-        raise ValueError(f"top {top} and sink {sink} must not be negative, recent {recent} at least 1")
-    bp, b0, b1 = _bounds(bounds, pages, D)
-    picked = torch.empty(pool.batch, q_len, pool.kv_heads, sink + recent + top, dtype=torch.int32, device=dev)
+    pool, D, dev = _pool(pages, page_table)
+    q = _query(query, pool, D, dev)
     with _on(dev):
-        _lib.check(_lib.lib().lf_int4_select(
-            ctypes.byref(pool), D, q.data_ptr(), _lib.dtype_code(q.dtype), *qs, q_len, n_q,
-            bp, b0, b1, _per_sequence("lengths", lengths, pool.batch, dev),
-            _per_sequence("counts", counts, pool.batch, dev), top, sink, recent, picked.data_ptr(), _status(status, dev),
-            _lib.stream_handle(dev)), "lf_int4_select")
-    return picked
+        return _select(pool, D, dev, q, bounds, pages, _per_sequence("lengths", lengths, pool.batch, dev),
+                       _per_sequence("counts", counts, pool.batch, dev), top_pages, sink_pages, recent_pages,
+                       _status(status, dev))
 
 
 def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
@@ -313,8 +338,15 @@ def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torc
     """:func:`int4_select`, then :func:`int4_attention` over the picked pages
     only: ``(out, picked)``.  With ``sink + recent + top`` pages or fewer
     visible, every page is read and the result is the dense one."""
-    picked = int4_select(query, pages, bounds, page_table, lengths, top_pages, sink_pages, recent_pages, counts, status)
-    return _attend(query, pages, page_table, lengths, scaling, counts, picked, out, status), picked
+    pool, D, dev = _pool(pages, page_table)
+    q = _query(query, pool, D, dev)
+    out = _out(query, out, dev)
+    addresses = _per_sequence("lengths", lengths, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev)
+    flag = _status(status, dev)
+    with _on(dev):
+        picked = _select(pool, D, dev, q, bounds, pages, *addresses, top_pages, sink_pages, recent_pages, flag)
+        _attend(pool, D, dev, q, *addresses, picked.data_ptr(), picked.shape[3], scaling, out, flag)
+    return out, picked
 
 
 class Int4KVCache:
