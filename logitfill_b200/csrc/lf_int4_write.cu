@@ -7,36 +7,22 @@
 //   stored value = RN(code * s + z)
 // The codes are formed with the fp16 scale and minimum that the reader uses,
 // so the minimum's rounding costs no accuracy; a group whose scale or minimum
-// is not a finite fp16 number (a NaN, an infinity, a value past 65504) reads
-// back as NaN.
+// is not a finite fp16 number (a NaN, an infinity, a range past 15 * 65504)
+// reads back as NaN.
+//
+// Both directions move 4 D bytes of 16-bit Key and Value and 1.25 D of record per
+// token and head, so they are bound by HBM once the arithmetic is kept small:
+// extremes of packed pairs, two of them in one shuffle; four fp32 operations and
+// two integer ones per code; codes read back as subnormal halves.  The writer
+// builds a page's record in shared memory and stores whole rows of it: the
+// record's order puts a token's Value words 64 bytes apart, and stored one by one
+// they would fill eight times as many sectors.
+#include <type_traits>
+
 #include "lf_int4.cuh"
 
 namespace lf {
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = half_lo(v[i]);
-    x[2 * i + 1] = half_hi(v[i]);
-  }
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(v[i] << 16);
-    x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-  }
-}
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
 template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -61,36 +47,105 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// Smallest and largest of a lane's eight channels, as (min, -max) in one word for
+// 16-bit types, joined over the four lanes of a group; NaN where one is NaN.
+template <typename T> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t min2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T> struct Chunk {  // eight 16-bit channels
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  }
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        x[2 * i] = half_lo(w[i]);
+        x[2 * i + 1] = half_hi(w[i]);
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+  __device__ __forceinline__ void extremes(float& lo, float& hi) const {
+    const uint32_t a = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3]));
+    constexpr uint32_t kSign = 0x80008000u;
+    const uint32_t b = min2<T>(min2<T>(w[0] ^ kSign, w[1] ^ kSign), min2<T>(w[2] ^ kSign, w[3] ^ kSign));
+    uint32_t both = min2<T>(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) both = min2<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+    if constexpr (std::is_same<T, __half>::value) {
+      lo = half_lo(both);
+      hi = -half_hi(both);
+    } else {
+      lo = __uint_as_float(both << 16);
+      hi = -__uint_as_float(both & 0xFFFF0000u);
+    }
+  }
+};
+template <> struct Chunk<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[i];
+  }
+  __device__ __forceinline__ void extremes(float& lo, float& hi) const {
+    lo = hi = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = min_nan(lo, v[i]);
+      hi = max_nan(hi, v[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+  }
+};
+
 // Codes (eight nibbles) and the parameter word of a lane's eight channels; the
 // four lanes of a group take its extremes together.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& param) {
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const Chunk<T>& chunk, uint32_t& param) {
+  float lo, hi;
+  chunk.extremes(lo, hi);
   const uint16_t sb = float_to_half_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   const uint16_t zb = float_to_half_bits(lo);
-  if ((sb & 0x7C00u) == 0x7C00u || (zb & 0x7C00u) == 0x7C00u) {
-    param = 0x7FFF7FFFu;
-    return 0;
-  }
-  param = sb | (static_cast<uint32_t>(zb) << 16);
+  const bool bad = (sb & 0x7C00u) == 0x7C00u || (zb & 0x7C00u) == 0x7C00u;
+  param = bad ? 0x7FFF7FFFu : sb | (static_cast<uint32_t>(zb) << 16);
   const float s = half_bits_to_float(sb), z = half_bits_to_float(zb);
-  const float r = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+  // r / 16: a power of two less, so the product is the definition's over 16 and
+  // its saturation to [0, 1] clamps to codes 0 .. 16 for free
+  const float r = s > 0.0f && !bad ? __frcp_rn(s) * 0.0625f : 0.0f;
+  float x[8];
+  chunk.unpack(x);
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], z), r), 0.0f), 15.0f);
-    w |= static_cast<uint32_t>(__float2int_rn(c)) << (4 * i);
+  for (int i = 7; i >= 0; --i) {
+    float y;
+    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y) : "f"(__fsub_rn(x[i], z)), "f"(r));
+    // 16 y + 1.5 * 2^23 rounds to a whole number, half to even, in the low bits
+    const uint32_t c = min(__float_as_uint(__fmaf_rn(y, 16.0f, 12582912.0f)), kMagicBits + 15u);
+    w = w * 16u + c;
   }
-  return w;
+  return w - kMagicBits * 0x11111111u;  // the eight magic numbers, shifted as the codes were
 }
 
 struct WriteParams {
@@ -106,13 +161,51 @@ struct WriteParams {
 
 constexpr int kWriteThreads = 128;
 
-// Channel bounds of a complete page's Key, from its record: the extremes of
-// the stored values over the tokens, rounded outwards to whole steps of 2^e.
-// Every thread of the CTA calls it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The eight codes of a word times 2^-24, in the order n, n + 4, as floats: the
+// halves of w & 0x000f000f are subnormal (16 times that in w & 0x00f000f0).
+__device__ __forceinline__ void codes8(uint32_t w, float (&even)[4], float (&odd)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t a = w & 0x000f000fu, b = w & 0x00f000f0u;
+    even[2 * i] = half_lo(a);
+    even[2 * i + 1] = half_hi(a);
+    odd[2 * i] = half_lo(b);
+    odd[2 * i + 1] = half_hi(b);
+    w >>= 8;
+  }
+}
+// RN(code * scale + min) of the eight channels of a word, in channel order.  The
+// powers of two that the codes carry go into the scale, so every product is exact.
+__device__ __forceinline__ void values8(uint32_t w, float s, float z, float (&v)[8]) {
+  float even[4], odd[4];
+  codes8(w, even, odd);
+  const float s0 = s * 0x1p24f, s1 = s * 0x1p20f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v[2 * i + 4 * j] = __fmaf_rn(even[2 * i + j], s0, z);
+      v[2 * i + 4 * j + 1] = __fmaf_rn(odd[2 * i + j], s1, z);
+    }
+}
+
+// Channel bounds of a complete page's Key from its record in shared memory: the
+// extremes of the stored values over the tokens, rounded outwards to whole steps
+// of 2^e.  Every thread of the CTA calls it.
 template <int D>
-__device__ void write_bounds(const int32_t* rec, int8_t* out) {
+__device__ void write_bounds(const uint32_t* rec, int8_t* out) {
   constexpr int kCols = D / 8, kParts = kWriteThreads / kCols, kTok = kInt4Page / kParts;
-  __shared__ float up_s[kParts][D], low_s[kParts][D];
+  __shared__ float up_s[kParts][D + 4], low_s[kParts][D + 4];
   __shared__ float most_s[kWriteThreads / 32];
   const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
   const int t = col / (D / 32), G = col % (D / 32);
@@ -122,22 +215,25 @@ __device__ void write_bounds(const int32_t* rec, int8_t* out) {
     up[i] = -INFINITY;
     low[i] = INFINITY;
   }
-  for (int k = part * kTok; k < (part + 1) * kTok; ++k) {
-    const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(rec) + k * kCols + col);
-    const uint32_t pw = __ldcg(reinterpret_cast<const uint32_t*>(rec) + 8 * D + k * (D / 32) + G);
-    const float s = half_lo(pw), z = half_hi(pw);
+#pragma unroll
+  for (int k = part * kTok; k < (part + 1) * kTok; k += 2) {
+    float v[2][8];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t p = rec[8 * D + (k + x) * (D / 32) + G];
+      if ((p & 0x7C00u) == 0x7C00u) p = 0;  // a group that holds no numbers counts as zeros
+      values8(rec[(k + x) * kCols + col] & (p == 0 ? 0u : ~0u), half_lo(p), half_hi(p), v[x]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = __fmaf_rn(static_cast<float>((w >> (4 * i)) & 15u), s, z);
-      v = isfinite(v) ? v : 0.0f;
-      up[i] = fmaxf(up[i], v);
-      low[i] = fminf(low[i], v);
+      up[i] = max3(up[i], v[0][i], v[1][i]);
+      low[i] = min3(low[i], v[0][i], v[1][i]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    up_s[part][32 * G + 8 * t + i] = up[i];
-    low_s[part][32 * G + 8 * t + i] = low[i];
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(&up_s[part][32 * G + 8 * t + i]) = make_float4(up[i], up[i + 1], up[i + 2], up[i + 3]);
+    *reinterpret_cast<float4*>(&low_s[part][32 * G + 8 * t + i]) = make_float4(low[i], low[i + 1], low[i + 2], low[i + 3]);
   }
   __syncthreads();
   const int d = threadIdx.x;
@@ -167,15 +263,31 @@ __device__ void write_bounds(const int32_t* rec, int8_t* out) {
   if (d == 0) out[2 * D] = static_cast<int8_t>(e);
 }
 
+// Word x (0 .. 20 D / 64 - 1) of token k in a record: Key codes, Key parameters,
+// Value codes, Value parameters.
+template <int D>
+__device__ __forceinline__ int token_word(int k, int x) {
+  constexpr int kC = D / 8, kP = D / 32;
+  const int v = x >= kC + kP, y = x - v * (kC + kP);
+  if (y >= kC) return v * 10 * D + 8 * D + k * kP + y - kC;
+  if (v == 0) return k * kC + y;
+  const int g = y / (D / 64), w = y % (D / 64);
+  return 10 * D + (k >> 3) * D + g * kC + ((k & 7) >> 1) * kP + (k & 1) * (D / 64) + w;
+}
+
+// One CTA per (page, KV head): its tokens of the page, and the page's bounds once
+// its last slot is written.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const __grid_constant__ WriteParams p) {
-  constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes;
-  const int b = blockIdx.z, h = blockIdx.y;
+  constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes, kWords = 20 * D / kInt4Page;
+  __shared__ __align__(16) uint32_t rec_s[20 * D];
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  grid_dep_wait();
   const int start = p.start[b];
   const int count = p.counts != nullptr ? min(p.counts[b], p.tokens) : p.tokens;
   if (count <= 0) return;
   if (start < 0 || start > INT32_MAX - count) {
-    if (threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+    if (tid == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
     return;
   }
   const int page = start / kInt4Page + blockIdx.x;
@@ -183,43 +295,54 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const __grid_
   if (first >= last) return;
   const int id = int4_page_id(p.pool, b, page);
   if (id < 0) {
-    if (threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+    if (tid == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
     return;
   }
-  int32_t* rec = p.pool.words + int4_record(p.pool, id, h);
-  const int l = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  uint32_t* rec = reinterpret_cast<uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
+  const int k0 = first - page * kInt4Page, k1 = last - page * kInt4Page;  // slots of the page to write
+  const bool whole = p.bounds != nullptr && k1 == kInt4Page;
+  if (whole) {  // the slots written before, for the bounds
+    for (int x = tid; x < k0 * (D / 8); x += kWriteThreads) rec_s[x] = __ldcg(rec + x);
+    for (int x = tid; x < k0 * (D / 32); x += kWriteThreads) rec_s[8 * D + x] = __ldcg(rec + 8 * D + x);
+  }
+
+  const int l = tid % kLanes, row = tid / kLanes;
   const T* key = static_cast<const T*>(p.key) + b * p.k_seq + h * p.k_head + 8 * l;
   const T* value = static_cast<const T*>(p.value) + b * p.v_seq + h * p.v_head + 8 * l;
+  const int64_t src0 = first - start - k0;
   const int G = l >> 2, t = l & 3, u = G & 1;
-  for (int pos0 = first; pos0 < last; pos0 += kRows) {  // whole warps stay together for the shuffles
-    const int pos = min(pos0 + row, last - 1);
-    const bool mine = pos0 + row < last;
-    const int64_t src = pos - start;
-    float xk[8], xv[8];
-    load8<T>(key + src * p.k_tok, xk);
-    load8<T>(value + src * p.v_tok, xv);
+#pragma unroll 2
+  for (int kk = k0; kk < k1; kk += kRows) {  // whole warps stay together for the shuffles
+    const int k = min(kk + row, k1 - 1);
+    Chunk<T> ck, cv;
+    ck.load(key + (src0 + k) * p.k_tok);
+    cv.load(value + (src0 + k) * p.v_tok);
     uint32_t kp, vp;
-    const uint32_t kw = quantise8(xk, kp);
-    const uint32_t vw = quantise8(xv, vp);
+    const uint32_t kw = quantise8<T>(ck, kp);
+    const uint32_t vw = quantise8<T>(cv, vp);
     // The lane's channels are 4 of chunk g = 2 t and 4 of g + 1; the lane of the
     // neighbouring group (u flipped) holds the other halves of both words.
     const uint32_t got = __shfl_xor_sync(0xffffffffu, u == 0 ? vw >> 16 : vw & 0xFFFFu, 4);
     const uint32_t vword = u == 0 ? (vw & 0xFFFFu) | (got << 16) : got | (vw & 0xFFFF0000u);
-    if (mine) {
-      const int k = pos - page * kInt4Page;
-      rec[k * (D / 8) + t * (D / 32) + G] = static_cast<int32_t>(kw);
-      const int blk = k >> 3, pair = (k & 7) >> 1, odd = k & 1;
-      rec[10 * D + blk * D + (2 * t + u) * (D / 8) + pair * (D / 32) + odd * (D / 64) + (G >> 1)] =
-          static_cast<int32_t>(vword);
-      if (t == 0) {
-        rec[8 * D + k * (D / 32) + G] = static_cast<int32_t>(kp);
-        rec[18 * D + k * (D / 32) + G] = static_cast<int32_t>(vp);
-      }
+    rec_s[k * (D / 8) + t * (D / 32) + G] = kw;  // rows past k1 repeat the last one
+    rec_s[10 * D + (k >> 3) * D + (2 * t + u) * (D / 8) + ((k & 7) >> 1) * (D / 32) + (k & 1) * (D / 64) + (G >> 1)] = vword;
+    if (t == 0) {
+      rec_s[8 * D + k * (D / 32) + G] = kp;
+      rec_s[18 * D + k * (D / 32) + G] = vp;
     }
   }
-  if (p.bounds == nullptr || last != (page + 1) * kInt4Page) return;
-  __syncthreads();  // the page is complete: this CTA's stores are visible to all its threads
-  write_bounds<D>(rec, p.bounds + id * p.bounds_page + h * p.bounds_head);
+  __syncthreads();
+  if (k1 - k0 == kInt4Page) {
+#pragma unroll
+    for (int x = tid; x < 5 * D; x += kWriteThreads)
+      reinterpret_cast<uint4*>(rec)[x] = reinterpret_cast<const uint4*>(rec_s)[x];
+  } else {
+    for (int x = tid; x < (k1 - k0) * kWords; x += kWriteThreads) {
+      const int at = token_word<D>(k0 + x / kWords, x % kWords);
+      rec[at] = rec_s[at];
+    }
+  }
+  if (whole) write_bounds<D>(rec_s, p.bounds + id * p.bounds_page + h * p.bounds_head);
 }
 
 struct ReadParams {
@@ -231,35 +354,41 @@ struct ReadParams {
 };
 
 // out [batch][kv_heads][tokens][D]: token i is position start[b] + i, zero from
-// counts[b] on.
+// counts[b] on.  One CTA per 64 tokens, which lie in two pages at most.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_constant__ ReadParams p) {
   constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes;
   const int b = blockIdx.z, h = blockIdx.y;
+  grid_dep_wait();
   const int start = p.start[b];
-  const int count = p.counts != nullptr ? p.counts[b] : p.tokens;
+  const int count = p.counts != nullptr ? min(p.counts[b], p.tokens) : p.tokens;
   const int l = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   const int G = l >> 2, t = l & 3, u = G & 1, w = G >> 1;
-  const int last = min((static_cast<int>(blockIdx.x) + 1) * kInt4Page, p.tokens);
-  for (int i = blockIdx.x * kInt4Page + row; i < last; i += kRows) {
+  const int i0 = blockIdx.x * kInt4Page, last = min(i0 + kInt4Page, p.tokens);
+  const int64_t pos0 = static_cast<int64_t>(start) + i0;
+  auto record = [&](int x) -> const uint32_t* {  // of the first page, or of the one after
+    const int64_t page = pos0 >= 0 ? pos0 / kInt4Page + x : -1;
+    const int id = page < p.pool.table_width ? int4_page_id(p.pool, b, static_cast<int>(page)) : -1;
+    return id < 0 ? nullptr : reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
+  };
+  const uint32_t *rec0 = record(0), *rec1 = record(1);
+  const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));
+#pragma unroll 4
+  for (int i = i0 + row; i < last; i += kRows) {
     float xk[8] = {}, xv[8] = {};
-    const int64_t pos = static_cast<int64_t>(start) + i;
+    const int k = k0 + i - i0;
+    const uint32_t* rec = k < kInt4Page ? rec0 : rec1;
     if (i < count) {
-      const int id = pos < 0 || pos > INT32_MAX ? -1 : int4_page_id(p.pool, b, static_cast<int>(pos / kInt4Page));
-      if (id < 0) {
+      if (rec == nullptr) {
         if (p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
       } else {
-        const uint32_t* rec = reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
-        const int k = static_cast<int>(pos % kInt4Page);
-        const uint32_t kw = rec[k * (D / 8) + t * (D / 32) + G];
-        const uint32_t kp = rec[8 * D + k * (D / 32) + G], vp = rec[18 * D + k * (D / 32) + G];
-        const uint32_t* vc = rec + 10 * D + (k >> 3) * D + 2 * t * (D / 8) + ((k & 7) >> 1) * (D / 32) + (k & 1) * (D / 64) + w;
-        const uint32_t vw = ((vc[0] >> (16 * u)) & 0xFFFFu) | ((vc[D / 8] >> (16 * u)) << 16);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          xk[n] = __fmaf_rn(static_cast<float>((kw >> (4 * n)) & 15u), half_lo(kp), half_hi(kp));
-          xv[n] = __fmaf_rn(static_cast<float>((vw >> (4 * n)) & 15u), half_lo(vp), half_hi(vp));
-        }
+        const int s = k & (kInt4Page - 1);
+        const uint32_t kw = rec[s * (D / 8) + t * (D / 32) + G];
+        const uint32_t kp = rec[8 * D + s * (D / 32) + G], vp = rec[18 * D + s * (D / 32) + G];
+        const uint32_t* vc = rec + 10 * D + (s >> 3) * D + 2 * t * (D / 8) + ((s & 7) >> 1) * (D / 32) + (s & 1) * (D / 64) + w;
+        const uint32_t vw = __byte_perm(vc[0], vc[D / 8], u == 0 ? 0x5410 : 0x7632);
+        values8(kw, half_lo(kp), half_hi(kp), xk);
+        values8(vw, half_lo(vp), half_hi(vp), xv);
       }
     }
     const int64_t dst = ((static_cast<int64_t>(b) * p.pool.kv_heads + h) * p.tokens + i) * D + 8 * l;
@@ -279,29 +408,24 @@ __global__ void int4_read_bounds_kernel(const int8_t* bounds, int64_t page_strid
   out[i] = static_cast<float>(rec[c]) * pow2(rec[2 * D]);
 }
 
-template <template <typename, int> class Launch, typename P>
-static int by_type(int dtype, int D, dim3 grid, const P& p, cudaStream_t stream) {
-  switch (dtype * 2 + (D == 128)) {
-    case LF_F32 * 2: return Launch<float, 64>::go(grid, p, stream);
-    case LF_F32 * 2 + 1: return Launch<float, 128>::go(grid, p, stream);
-    case LF_F16 * 2: return Launch<__half, 64>::go(grid, p, stream);
-    case LF_F16 * 2 + 1: return Launch<__half, 128>::go(grid, p, stream);
-    case LF_BF16 * 2: return Launch<__nv_bfloat16, 64>::go(grid, p, stream);
-    default: return Launch<__nv_bfloat16, 128>::go(grid, p, stream);
+template <typename P>
+static int launch(const void* kern, const char* what, dim3 grid, P p, cudaStream_t stream) {
+  void* args[] = {&p};
+  const cudaError_t err = launch_programmatic(kern, grid, dim3(kWriteThreads), 0, stream, args);
+  if (err != cudaSuccess) {
+    set_error("%s: %s", what, cudaGetErrorString(err));
+    return LF_ERR_LAUNCH;
   }
+  return launch_status(what);
 }
-template <typename T, int D> struct WriteLaunch {
-  static int go(dim3 grid, const WriteParams& p, cudaStream_t stream) {
-    int4_write_kernel<T, D><<<grid, kWriteThreads, 0, stream>>>(p);
-    return launch_status("lf_int4_write");
-  }
-};
-template <typename T, int D> struct ReadLaunch {
-  static int go(dim3 grid, const ReadParams& p, cudaStream_t stream) {
-    int4_read_kernel<T, D><<<grid, kWriteThreads, 0, stream>>>(p);
-    return launch_status("lf_int4_read");
-  }
-};
+template <typename T> static const void* write_kernel(int D) {
+  return D == 128 ? reinterpret_cast<const void*>(int4_write_kernel<T, 128>)
+                  : reinterpret_cast<const void*>(int4_write_kernel<T, 64>);
+}
+template <typename T> static const void* read_kernel(int D) {
+  return D == 128 ? reinterpret_cast<const void*>(int4_read_kernel<T, 128>)
+                  : reinterpret_cast<const void*>(int4_read_kernel<T, 64>);
+}
 
 int check_int4_pool(const char* what, const lf_int4_pool* pool, int head_dim, Int4Pool& out) {
   LF_CHECK_ARG(pool && pool->pages && pool->table, "%s: null pool, pages or page table", what);
@@ -364,7 +488,10 @@ extern "C" int lf_int4_write(const lf_int4_pool* pool, int head_dim, const void*
   p.status = status;
   // tokens that start anywhere in a page touch at most this many pages
   const dim3 grid((tokens + 2 * lf::kInt4Page - 2) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
-  return lf::by_type<lf::WriteLaunch>(dtype, head_dim, grid, p, reinterpret_cast<cudaStream_t>(stream));
+  const void* kern = dtype == LF_F32   ? lf::write_kernel<float>(head_dim)
+                     : dtype == LF_F16 ? lf::write_kernel<__half>(head_dim)
+                                       : lf::write_kernel<__nv_bfloat16>(head_dim);
+  return lf::launch(kern, "lf_int4_write", grid, p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lf_int4_read(const lf_int4_pool* pool, int head_dim, const int32_t* start, const int32_t* counts,
@@ -385,7 +512,10 @@ extern "C" int lf_int4_read(const lf_int4_pool* pool, int head_dim, const int32_
   p.out_v = out_v;
   p.status = status;
   const dim3 grid((tokens + lf::kInt4Page - 1) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
-  return lf::by_type<lf::ReadLaunch>(out_dtype, head_dim, grid, p, reinterpret_cast<cudaStream_t>(stream));
+  const void* kern = out_dtype == LF_F32   ? lf::read_kernel<float>(head_dim)
+                     : out_dtype == LF_F16 ? lf::read_kernel<__half>(head_dim)
+                                           : lf::read_kernel<__nv_bfloat16>(head_dim);
+  return lf::launch(kern, "lf_int4_read", grid, p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lf_int4_read_bounds(const int8_t* bounds, int64_t page_stride, int64_t head_stride, int n_pages,
