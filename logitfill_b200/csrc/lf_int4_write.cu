@@ -120,32 +120,54 @@ template <> struct Chunk<float> {
   }
 };
 
-// Codes (eight nibbles) and the parameter word of a lane's eight channels; the
-// four lanes of a group take its extremes together.
-template <typename T>
-__device__ __forceinline__ uint32_t quantise8(const Chunk<T>& chunk, uint32_t& param) {
-  float lo, hi;
-  chunk.extremes(lo, hi);
+// A group's parameters from its extremes: the stored word, z and r / 16 (0 for a
+// group that is not stored).
+struct GroupParams {
+  uint32_t word;
+  float z, r16;
+};
+__device__ __forceinline__ GroupParams group_params(float lo, float hi) {
   const uint16_t sb = float_to_half_bits(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   const uint16_t zb = float_to_half_bits(lo);
   const bool bad = (sb & 0x7C00u) == 0x7C00u || (zb & 0x7C00u) == 0x7C00u;
-  param = bad ? 0x7FFF7FFFu : sb | (static_cast<uint32_t>(zb) << 16);
-  const float s = half_bits_to_float(sb), z = half_bits_to_float(zb);
-  // r / 16: a power of two less, so the product is the definition's over 16 and
-  // its saturation to [0, 1] clamps to codes 0 .. 16 for free
-  const float r = s > 0.0f && !bad ? __frcp_rn(s) * 0.0625f : 0.0f;
+  const float s = half_bits_to_float(sb);
+  GroupParams g;
+  g.word = bad ? 0x7FFF7FFFu : sb | (static_cast<uint32_t>(zb) << 16);
+  g.z = half_bits_to_float(zb);
+  // r / 16: a power of two less, so the product with it is the definition's over
+  // 16 and its saturation to [0, 1] clamps the code to 0 .. 16 for free
+  g.r16 = s > 0.0f && !bad ? __frcp_rn(s) * 0.0625f : 0.0f;
+  return g;
+}
+
+// Codes (eight nibbles) of a lane's eight channels.  16 y + 1.5 * 2^23 rounds to a
+// whole number, half to even, in the low bits of the sum; the magic numbers,
+// shifted as the codes are, come off at the end.  Code 16 needs |min| of a
+// thousand steps or more (its fp16 rounding then shows in x - z), so the clamp to
+// 15 is a branch.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const Chunk<T>& chunk, const GroupParams& g) {
   float x[8];
   chunk.unpack(x);
-  uint32_t w = 0;
+  uint32_t c[8];
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    float y;
-    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y) : "f"(__fsub_rn(x[i], z)), "f"(r));
-    // 16 y + 1.5 * 2^23 rounds to a whole number, half to even, in the low bits
-    const uint32_t c = min(__float_as_uint(__fmaf_rn(y, 16.0f, 12582912.0f)), kMagicBits + 15u);
-    w = w * 16u + c;
+  for (int i = 0; i < 8; i += 2) {
+    const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(-g.z, -g.z));
+    float2 y;
+    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.x) : "f"(d.x), "f"(g.r16));
+    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.y) : "f"(d.y), "f"(g.r16));
+    const float2 m = __ffma2_rn(y, make_float2(16.0f, 16.0f), make_float2(12582912.0f, 12582912.0f));
+    c[i] = __float_as_uint(m.x);
+    c[i + 1] = __float_as_uint(m.y);
   }
-  return w - kMagicBits * 0x11111111u;  // the eight magic numbers, shifted as the codes were
+  if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) & 16u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = min(c[i], kMagicBits + 15u);
+  }
+  uint32_t w = c[7];
+#pragma unroll
+  for (int i = 6; i >= 0; --i) w = w * 16u + c[i];
+  return w - kMagicBits * 0x11111111u;
 }
 
 struct WriteParams {
@@ -278,7 +300,7 @@ __device__ __forceinline__ int token_word(int k, int x) {
 // One CTA per (page, KV head): its tokens of the page, and the page's bounds once
 // its last slot is written.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const __grid_constant__ WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __grid_constant__ WriteParams p) {
   constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes, kWords = 20 * D / kInt4Page;
   __shared__ __align__(16) uint32_t rec_s[20 * D];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
@@ -306,29 +328,46 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const __grid_
     for (int x = tid; x < k0 * (D / 32); x += kWriteThreads) rec_s[8 * D + x] = __ldcg(rec + 8 * D + x);
   }
 
+  // Row `row` of every kRows slots: the addresses step by constants.
   const int l = tid % kLanes, row = tid / kLanes;
-  const T* key = static_cast<const T*>(p.key) + b * p.k_seq + h * p.k_head + 8 * l;
-  const T* value = static_cast<const T*>(p.value) + b * p.v_seq + h * p.v_head + 8 * l;
-  const int64_t src0 = first - start - k0;
+  const int64_t from = page * kInt4Page - start + row;  // source token of slot `row`
+  const T* key = static_cast<const T*>(p.key) + b * p.k_seq + h * p.k_head + from * p.k_tok + 8 * l;
+  const T* value = static_cast<const T*>(p.value) + b * p.v_seq + h * p.v_head + from * p.v_tok + 8 * l;
+  const int64_t k_step = p.k_tok * kRows, v_step = p.v_tok * kRows;
   const int G = l >> 2, t = l & 3, u = G & 1;
+  const bool odd = l & 1;
+  uint32_t* kcode = rec_s + row * (D / 8) + t * (D / 32) + G;
+  uint32_t* vcode = rec_s + 10 * D + (row >> 3) * D + (2 * t + u) * (D / 8) + ((row & 7) >> 1) * (D / 32) + (row & 1) * (D / 64) +
+                    (G >> 1);
+  uint32_t* param = rec_s + (odd ? 18 : 8) * D + row * (D / 32) + G;
 #pragma unroll 2
-  for (int kk = k0; kk < k1; kk += kRows) {  // whole warps stay together for the shuffles
-    const int k = min(kk + row, k1 - 1);
-    Chunk<T> ck, cv;
-    ck.load(key + (src0 + k) * p.k_tok);
-    cv.load(value + (src0 + k) * p.v_tok);
-    uint32_t kp, vp;
-    const uint32_t kw = quantise8<T>(ck, kp);
-    const uint32_t vw = quantise8<T>(cv, vp);
+  for (int it = 0; it < kInt4Page / kRows; ++it, key += k_step, value += v_step, kcode += kRows * (D / 8),
+           vcode += kRows * (D / 8), param += kRows * (D / 32)) {
+    const int k = it * kRows;
+    if (k + kRows <= k0 || k >= k1) continue;  // whole warps stay together for the shuffles
+    const bool live = k + row >= k0 && k + row < k1;
+    Chunk<T> ck = {}, cv = {};
+    if (live) {
+      ck.load(key);
+      cv.load(value);
+    }
+    // Even lanes form the Key group's parameters, odd ones the Value group's.
+    float klo, khi, vlo, vhi;
+    ck.extremes(klo, khi);
+    cv.extremes(vlo, vhi);
+    const GroupParams mine = group_params(odd ? vlo : klo, odd ? vhi : khi);
+    GroupParams other;
+    other.z = __shfl_xor_sync(0xffffffffu, mine.z, 1);
+    other.r16 = __shfl_xor_sync(0xffffffffu, mine.r16, 1);
+    const uint32_t kw = quantise8<T>(ck, odd ? other : mine);
+    const uint32_t vw = quantise8<T>(cv, odd ? mine : other);
     // The lane's channels are 4 of chunk g = 2 t and 4 of g + 1; the lane of the
     // neighbouring group (u flipped) holds the other halves of both words.
     const uint32_t got = __shfl_xor_sync(0xffffffffu, u == 0 ? vw >> 16 : vw & 0xFFFFu, 4);
-    const uint32_t vword = u == 0 ? (vw & 0xFFFFu) | (got << 16) : got | (vw & 0xFFFF0000u);
-    rec_s[k * (D / 8) + t * (D / 32) + G] = kw;  // rows past k1 repeat the last one
-    rec_s[10 * D + (k >> 3) * D + (2 * t + u) * (D / 8) + ((k & 7) >> 1) * (D / 32) + (k & 1) * (D / 64) + (G >> 1)] = vword;
-    if (t == 0) {
-      rec_s[8 * D + k * (D / 32) + G] = kp;
-      rec_s[18 * D + k * (D / 32) + G] = vp;
+    if (live) {
+      *kcode = kw;
+      *vcode = u == 0 ? (vw & 0xFFFFu) | (got << 16) : got | (vw & 0xFFFF0000u);
+      if (t < 2) *param = mine.word;
     }
   }
   __syncthreads();
@@ -373,27 +412,38 @@ __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_c
   };
   const uint32_t *rec0 = record(0), *rec1 = record(1);
   const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));
-#pragma unroll 4
-  for (int i = i0 + row; i < last; i += kRows) {
-    float xk[8] = {}, xv[8] = {};
-    const int k = k0 + i - i0;
-    const uint32_t* rec = k < kInt4Page ? rec0 : rec1;
-    if (i < count) {
-      if (rec == nullptr) {
-        if (p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
-      } else {
-        const int s = k & (kInt4Page - 1);
-        const uint32_t kw = rec[s * (D / 8) + t * (D / 32) + G];
-        const uint32_t kp = rec[8 * D + s * (D / 32) + G], vp = rec[18 * D + s * (D / 32) + G];
+  constexpr int kAtOnce = 4;  // rows whose loads are in flight together
+  for (int r0 = row; r0 < last - i0; r0 += kAtOnce * kRows) {
+    uint32_t kw[kAtOnce], kp[kAtOnce], vp[kAtOnce], v0[kAtOnce], v1[kAtOnce];
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      const int i = r0 + y * kRows, k = k0 + i, s = k & (kInt4Page - 1);
+      const uint32_t* rec = k < kInt4Page ? rec0 : rec1;
+      const bool there = i < last - i0 && i0 + i < count;
+      kw[y] = kp[y] = vp[y] = v0[y] = v1[y] = 0;
+      if (there && rec != nullptr) {
+        kw[y] = rec[s * (D / 8) + t * (D / 32) + G];
+        kp[y] = rec[8 * D + s * (D / 32) + G];
+        vp[y] = rec[18 * D + s * (D / 32) + G];
         const uint32_t* vc = rec + 10 * D + (s >> 3) * D + 2 * t * (D / 8) + ((s & 7) >> 1) * (D / 32) + (s & 1) * (D / 64) + w;
-        const uint32_t vw = __byte_perm(vc[0], vc[D / 8], u == 0 ? 0x5410 : 0x7632);
-        values8(kw, half_lo(kp), half_hi(kp), xk);
-        values8(vw, half_lo(vp), half_hi(vp), xv);
+        v0[y] = vc[0];
+        v1[y] = vc[D / 8];
+      } else if (there && p.status != nullptr) {
+        atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
       }
     }
-    const int64_t dst = ((static_cast<int64_t>(b) * p.pool.kv_heads + h) * p.tokens + i) * D + 8 * l;
-    store8<T>(static_cast<T*>(p.out_k) + dst, xk);
-    store8<T>(static_cast<T*>(p.out_v) + dst, xv);
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      const int i = r0 + y * kRows;
+      float xk[8], xv[8];
+      values8(kw[y], half_lo(kp[y]), half_hi(kp[y]), xk);
+      values8(__byte_perm(v0[y], v1[y], u == 0 ? 0x5410 : 0x7632), half_lo(vp[y]), half_hi(vp[y]), xv);
+      const int64_t dst = ((static_cast<int64_t>(b) * p.pool.kv_heads + h) * p.tokens + i0 + i) * D + 8 * l;
+      if (i < last - i0) {
+        store8<T>(static_cast<T*>(p.out_k) + dst, xk);
+        store8<T>(static_cast<T*>(p.out_v) + dst, xv);
+      }
+    }
   }
 }
 
