@@ -363,71 +363,95 @@ typedef struct lf_int4_pool {
   int32_t batch;
 } lf_int4_pool;
 
-/*
- * Quantize and store tokens: token i of sequence b (i < counts[b], or i <
- * tokens where counts is NULL) goes to position start[b] + i.
- * key/value [batch][kv_heads][tokens][head_dim] with the given element
- * strides (channel stride 1, rows 16-byte aligned), dtype F32, F16 or BF16.
- * bounds (may be NULL) with strides in bytes.  A group whose scale or minimum
- * is not a finite fp16 number reads back as NaN.
- */
-LF_API int lf_int4_write(const lf_int4_pool* pool, int head_dim, const void* key, const void* value, int dtype,
-                         int64_t k_seq_stride, int64_t k_head_stride, int64_t k_tok_stride, int64_t v_seq_stride,
-                         int64_t v_head_stride, int64_t v_tok_stride, int tokens, const int32_t* start,
-                         const int32_t* counts, int8_t* bounds, int64_t bounds_page_stride,
-                         int64_t bounds_head_stride, int32_t* status, lf_stream_t stream);
+/* Arguments of a write or a read.  Strides in elements (bounds: bytes). */
+typedef struct lf_int4_tokens {
+  lf_int4_pool pool;
+  void* key;              /* [batch][kv_heads][tokens][head_dim], channel stride 1, rows 16-byte aligned */
+  void* value;
+  int64_t k_seq_stride, k_head_stride, k_tok_stride;
+  int64_t v_seq_stride, v_head_stride, v_tok_stride;
+  const int32_t* start;   /* [batch] position of each sequence's first token     */
+  const int32_t* counts;  /* [batch] tokens of each sequence, or NULL: all       */
+  int8_t* bounds;         /* bounds records, or NULL                             */
+  int64_t bounds_page_stride, bounds_head_stride;
+  int32_t* status;        /* device word, or NULL                                */
+  int32_t head_dim;       /* 64 or 128                                           */
+  int32_t dtype;          /* of key and value: F32, F16 or BF16                  */
+  int32_t tokens;
+} lf_int4_tokens;
 
-/* Read positions start[b] .. start[b] + tokens - 1 back into out_k/out_v
- * [batch][kv_heads][tokens][head_dim] (contiguous, 16-byte aligned); token i is zero
- * from counts[b] on (counts may be NULL). */
-LF_API int lf_int4_read(const lf_int4_pool* pool, int head_dim, const int32_t* start, const int32_t* counts,
-                        int tokens, void* out_k, void* out_v, int out_dtype, int32_t* status, lf_stream_t stream);
+/* Quantize and store tokens: token i of sequence b (i < counts[b]) goes to
+ * position start[b] + i.  With bounds, the record of every page whose slot 63 is
+ * written is brought up to date.  A group whose scale or minimum is not a finite
+ * fp16 number reads back as NaN. */
+LF_API int lf_int4_write(const lf_int4_tokens* args, lf_stream_t stream);
+
+/* Read positions start[b] .. start[b] + tokens - 1 back into key and value; token i
+ * is zero from counts[b] on. */
+LF_API int lf_int4_read(const lf_int4_tokens* args, lf_stream_t stream);
 
 /* Bounds records as fp32 values: out [n_pages][kv_heads][2][head_dim], upper then lower. */
 LF_API int lf_int4_read_bounds(const int8_t* bounds, int64_t page_stride, int64_t head_stride, int n_pages,
                                int kv_heads, int head_dim, float* out, lf_stream_t stream);
 
+/* Arguments of a page choice or an attention call.  Strides in elements (bounds:
+ * bytes); the three calls below say which fields they read. */
+typedef struct lf_int4_query {
+  lf_int4_pool pool;
+  const void* q;          /* [batch][n_q][q_len][head_dim], channel stride 1, rows 16-byte aligned */
+  int64_t q_seq_stride, q_head_stride, q_tok_stride;
+  void* out;              /* as q                                                */
+  int64_t out_seq_stride, out_head_stride, out_tok_stride;
+  const int32_t* lengths; /* [batch] tokens cached, the query's own among them   */
+  const int32_t* counts;  /* [batch] query tokens of each sequence, or NULL: q_len */
+  const int8_t* bounds;
+  int64_t bounds_page_stride, bounds_head_stride;
+  int32_t* picked;        /* [batch][q_len][kv_heads][slots] logical pages       */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status;        /* device word, or NULL                                */
+  float scaling;
+  int32_t head_dim;       /* 64 or 128                                           */
+  int32_t dtype;          /* of q and out: F16 or BF16                           */
+  int32_t n_q, q_len;
+  int32_t slots;          /* pages per list: top_pages + sink_pages + recent_pages where they are chosen */
+  int32_t sink_pages, recent_pages;
+} lf_int4_query;
+
 /*
  * The pages a sparse call reads, for each sequence b, query token i and KV
  * head h.  Query token i sees v = max(0, lengths[b] - c + 1 + i) tokens, c =
- * counts[b] (q_len where counts is NULL; a token i >= c sees none), n =
- * ceil(v / 64) pages: the first sink_pages and the last recent_pages always, and of
- * the rest the top_pages with the largest
- * score (ties to the lower page).  With the group's queries scaled by the
- * power of two 2^-f that brings the largest magnitude among them to 127 at
- * most, and rounded to whole numbers Q (half to even; a non-finite one counts
- * as 0), the score of a page is fp32(I) * 2^e,
+ * counts[b] (a token i >= c sees none), n = ceil(v / 64) pages: the first
+ * sink_pages and the last recent_pages (1 at least) always, and of the rest the
+ * slots - sink_pages - recent_pages with the largest score (ties to the lower
+ * page).  With the group's queries scaled by the power of two 2^-f that brings
+ * the largest magnitude among them to 127 at most, and rounded to whole numbers Q
+ * (half to even; a non-finite one counts as 0), the score of a page is
+ * fp32(I) * 2^e,
  *   I = sum_channels upper * sum_heads max(Q, 0) + lower * sum_heads min(Q, 0),
  * an upper bound of the group's summed scores in units of 2^f, exact in whole
  * numbers: the choice does not depend on the order of any sum.
- * picked [batch][q_len][kv_heads][sink + recent + top] int32: logical pages in
- * ascending order, -1 after the last.  Candidate pages need their bounds record.
- * q [batch][n_q][q_len][head_dim], dtype F16 or BF16.
+ * Writes picked: logical pages in ascending order, -1 after the last.  Candidate
+ * pages need their bounds record.  Not read: out, workspace, scaling.
  */
-LF_API int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void* q, int q_dtype, int64_t q_seq_stride,
-                          int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int8_t* bounds,
-                          int64_t bounds_page_stride, int64_t bounds_head_stride, const int32_t* lengths,
-                          const int32_t* counts, int top_pages, int sink_pages, int recent_pages, int32_t* picked, int32_t* status,
-                          lf_stream_t stream);
+LF_API int lf_int4_select(const lf_int4_query* args, lf_stream_t stream);
 
 /*
- * Attention of q [batch][n_q][q_len][head_dim] over the cached tokens: query
- * token i sees positions 0 .. lengths[b] - c + i, c = counts[b] (q_len where
- * counts is NULL; a token i >= c sees none): the causal mask of
- * reference.py:18-27 over a cache that the new tokens were written to first.
- * q-head j reads KV head j / (n_q / kv_heads).  With picked not NULL ([batch][q_len][kv_heads]
- * [slots], as lf_int4_select writes it) only the tokens of those pages.  A query
- * token that sees nothing gets zeros.  out as q, same dtype (F16 or BF16).
- * q rows 16-byte aligned.  workspace: lf_int4_workspace_bytes bytes (of the
- * current device), 16-byte aligned, zero from byte lf_int4_workspace_clear_from on
- * before its first use and left so by every call, of any shape; calls that
- * overlap on the GPU need one each.
+ * Attention of q over the cached tokens: query token i of sequence b sees
+ * positions 0 .. lengths[b] - c + i (a token i >= c sees none): the causal mask
+ * of reference.py:18-27 over a cache that the new tokens were written to first.
+ * q-head j reads KV head j / (n_q / kv_heads).  With picked not NULL only the
+ * tokens of those pages.  A query token that sees nothing gets zeros.
+ * workspace: lf_int4_workspace_bytes bytes (of the current device), 16-byte
+ * aligned, zero from byte lf_int4_workspace_clear_from on before its first use
+ * and left so by every call, of any shape; calls that overlap on the GPU need one
+ * each.  Not read: bounds, sink_pages, recent_pages.
  */
-LF_API int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q, int dtype, int64_t q_seq_stride,
-                          int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int32_t* lengths,
-                          const int32_t* counts, const int32_t* picked, int slots, float scaling, void* out, int64_t out_seq_stride,
-                          int64_t out_head_stride, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
-                          int32_t* status, lf_stream_t stream);
+LF_API int lf_int4_attend(const lf_int4_query* args, lf_stream_t stream);
+
+/* lf_int4_select, then lf_int4_attend over what it picked. */
+LF_API int lf_int4_attend_sparse(const lf_int4_query* args, lf_stream_t stream);
+
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);
 LF_API size_t lf_int4_workspace_clear_from(void);
 

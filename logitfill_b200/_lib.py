@@ -6,6 +6,7 @@ is no fallback: if it is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -15,13 +16,20 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblogitfill_b200.so"
  LF_ERR_CUDA) = range(7)
 LF_F32, LF_F16, LF_BF16 = 0, 1, 2
 
+# The argument structs of the 4-bit cache, packed by the caller into one bytes
+# object: a call has 20 to 35 fields, and converting them one by one would cost
+# more than the launch.  Field order as in the header.
+_POOL = "PPqqqiiii"
+INT4_TOKENS = struct.Struct("@" + _POOL + "PP6qPPPqqPiii0q")
+INT4_QUERY = struct.Struct("@" + _POOL + "P3qP3qPPPqqPPNPf7i")
+
 EXPORTS = (
     "lf_layout_init", "lf_pack_pages", "lf_dequantize", "lf_decode_workspace_bytes",
     "lf_decode_max_splits", "lf_decode_occupancy", "lf_decode_partial", "lf_decode_noalloc", "lf_decode_merge",
     "lf_decode", "lf_decode_multi", "lf_decode_max_splits_multi", "lf_commit_token", "lf_selftest_wait", "lf_selftest_divide",
     "lf_ipc_alloc", "lf_ipc_free", "lf_ipc_handle", "lf_ipc_open", "lf_ipc_close", "lf_decode_merge_gather",
     "lf_gather_signals", "lf_gather_wait", "lf_int4_write", "lf_int4_read", "lf_int4_read_bounds", "lf_int4_select",
-    "lf_int4_attend", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from", "lf_status_string", "lf_last_error",
+    "lf_int4_attend", "lf_int4_attend_sparse", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from", "lf_status_string", "lf_last_error",
 )
 
 
@@ -38,16 +46,6 @@ class LfLayout(ctypes.Structure):
     ]
 
 
-class LfInt4Pool(ctypes.Structure):
-    """Mirror of ``struct lf_int4_pool``."""
-
-    _fields_ = [
-        ("pages", c_void_p), ("table", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64),
-        ("table_stride", c_int64), ("table_width", c_int32), ("n_pages", c_int32), ("kv_heads", c_int32),
-        ("batch", c_int32),
-    ]
-
-
 _LIB = None
 
 
@@ -61,7 +59,7 @@ def lib() -> ctypes.CDLL:
             f"logitfill_b200 native library missing at {LIB_PATH}; build it with "
             "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
     so = ctypes.CDLL(str(LIB_PATH))
-    P, L, Q = c_void_p, POINTER(LfLayout), POINTER(LfInt4Pool)
+    P, L, Q = c_void_p, POINTER(LfLayout), c_char_p  # Q: an argument struct, packed
     sig = {
         "lf_layout_init": (c_int, [L, c_int, c_int, c_int, c_int, c_int, c_int, P, c_int64, c_int64]),
         "lf_pack_pages": (c_int, [L, P, P, c_int, c_int64, c_int64, c_int64, P, c_int, c_int, P, P, P, P, P]),
@@ -96,14 +94,12 @@ def lib() -> ctypes.CDLL:
                                            c_int, c_int, c_int, P]),
         "lf_gather_signals": (c_int, [c_int, c_int, c_int]),
         "lf_gather_wait": (c_int, [P, c_int, ctypes.c_uint32, ctypes.c_uint64, P, P]),
-        "lf_int4_write": (c_int, [Q, c_int, P, P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
-                                  P, P, P, c_int64, c_int64, P, P]),
-        "lf_int4_read": (c_int, [Q, c_int, P, P, c_int, P, P, c_int, P, P]),
+        "lf_int4_write": (c_int, [Q, P]),
+        "lf_int4_read": (c_int, [Q, P]),
         "lf_int4_read_bounds": (c_int, [P, c_int64, c_int64, c_int, c_int, c_int, P, P]),
-        "lf_int4_select": (c_int, [Q, c_int, P, c_int, c_int64, c_int64, c_int64, c_int, c_int, P, c_int64, c_int64,
-                                   P, P, c_int, c_int, c_int, P, P, P]),
-        "lf_int4_attend": (c_int, [Q, c_int, P, c_int, c_int64, c_int64, c_int64, c_int, c_int, P, P, P, c_int,
-                                   c_float, P, c_int64, c_int64, c_int64, P, c_size_t, P, P]),
+        "lf_int4_select": (c_int, [Q, P]),
+        "lf_int4_attend": (c_int, [Q, P]),
+        "lf_int4_attend_sparse": (c_int, [Q, P]),
         "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
         "lf_status_string": (c_char_p, [c_int]),

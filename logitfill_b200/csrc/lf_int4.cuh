@@ -82,6 +82,6 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 }
 
 // Checks the C ABI's pool and copies it for a kernel (lf_int4_write.cu).
-int check_int4_pool(const char* what, const lf_int4_pool* pool, int head_dim, Int4Pool& out);
+int check_int4_pool(const char* what, const lf_int4_pool& pool, int head_dim, Int4Pool& out);
 
 }  // namespace lf

@@ -821,55 +821,59 @@ extern "C" size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int 
   return lf::partial_bytes(lf::sm_count()) + (static_cast<size_t>(units) * 4 + 15) / 16 * 16;
 }
 
-extern "C" int lf_int4_attend(const lf_int4_pool* pool, int head_dim, const void* q, int dtype, int64_t q_seq_stride,
-                              int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int32_t* lengths,
-                              const int32_t* counts, const int32_t* picked, int slots, float scaling, void* out,
-                              int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void* workspace,
-                              size_t workspace_bytes, int32_t* status, lf_stream_t stream) {
+extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
+  LF_CHECK_ARG(a != nullptr, "lf_int4_attend: null arguments");
   lf::AttendParams p;
-  const int bad = lf::check_int4_pool("lf_int4_attend", pool, head_dim, p.pool);
+  const int bad = lf::check_int4_pool("lf_int4_attend", a->pool, a->head_dim, p.pool);
   if (bad != LF_OK) return bad;
-  LF_CHECK_ARG(q && lengths && out, "lf_int4_attend: null pointer");
-  LF_CHECK_SUPPORTED(dtype == LF_F16 || dtype == LF_BF16, "lf_int4_attend: dtype %d (fp16 or bf16)", dtype);
-  LF_CHECK_ARG(q_len > 0 && q_len <= 65535 && n_q > 0 && n_q % p.pool.kv_heads == 0,
-               "lf_int4_attend: q_len %d, %d query heads on %d KV heads", q_len, n_q, p.pool.kv_heads);
-  LF_CHECK_ARG(picked == nullptr || slots > 0, "lf_int4_attend: %d slots", slots);
-  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_seq_stride | q_head_stride | q_tok_stride) % 8 == 0,
+  LF_CHECK_ARG(a->q && a->lengths && a->out, "lf_int4_attend: null pointer");
+  LF_CHECK_SUPPORTED(a->dtype == LF_F16 || a->dtype == LF_BF16, "lf_int4_attend: dtype %d (fp16 or bf16)", a->dtype);
+  LF_CHECK_ARG(a->q_len > 0 && a->q_len <= 65535 && a->n_q > 0 && a->n_q % p.pool.kv_heads == 0,
+               "lf_int4_attend: q_len %d, %d query heads on %d KV heads", a->q_len, a->n_q, p.pool.kv_heads);
+  const bool sparse = a->picked != nullptr;
+  LF_CHECK_ARG(!sparse || a->slots > 0, "lf_int4_attend: %d slots", a->slots);
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->q) & 15) == 0 && (a->q_seq_stride | a->q_head_stride | a->q_tok_stride) % 8 == 0,
                "lf_int4_attend: query rows must be 16-byte aligned");
   const int sms = lf::sm_count();
   if (sms <= 0) return lf::launch_status("lf_int4_attend");
-  LF_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
-                   workspace_bytes >= lf_int4_workspace_bytes(p.pool.batch, p.pool.kv_heads, n_q, q_len, head_dim),
-               "lf_int4_attend: workspace of %zu bytes is missing, misaligned or too small", workspace_bytes);
-  p.q = q;
-  p.q_seq = q_seq_stride;
-  p.q_head = q_head_stride;
-  p.q_tok = q_tok_stride;
-  p.q_len = q_len;
-  p.group = n_q / p.pool.kv_heads;
-  p.lengths = lengths;
-  p.counts = counts;
-  p.picked = picked;
-  p.slots = slots;
-  p.scale_log2 = scaling * 1.4426950408889634f;
-  p.out = out;
-  p.out_seq = out_seq_stride;
-  p.out_head = out_head_stride;
-  p.out_tok = out_tok_stride;
-  p.out_aligned = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && (out_seq_stride | out_head_stride | out_tok_stride) % 4 == 0;
-  p.rows = picked ? p.pool.batch * q_len : p.pool.batch;
-  p.cols = picked ? p.group : p.group * q_len;
+  LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
+                   a->workspace_bytes >= lf_int4_workspace_bytes(p.pool.batch, p.pool.kv_heads, a->n_q, a->q_len, a->head_dim),
+               "lf_int4_attend: workspace of %zu bytes is missing, misaligned or too small", a->workspace_bytes);
+  p.q = a->q;
+  p.q_seq = a->q_seq_stride;
+  p.q_head = a->q_head_stride;
+  p.q_tok = a->q_tok_stride;
+  p.q_len = a->q_len;
+  p.group = a->n_q / p.pool.kv_heads;
+  p.lengths = a->lengths;
+  p.counts = a->counts;
+  p.picked = a->picked;
+  p.slots = a->slots;
+  p.scale_log2 = a->scaling * 1.4426950408889634f;
+  p.out = a->out;
+  p.out_seq = a->out_seq_stride;
+  p.out_head = a->out_head_stride;
+  p.out_tok = a->out_tok_stride;
+  p.out_aligned = (reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&
+                  (a->out_seq_stride | a->out_head_stride | a->out_tok_stride) % 4 == 0;
+  p.rows = sparse ? p.pool.batch * a->q_len : p.pool.batch;
+  p.cols = sparse ? p.group : p.group * a->q_len;
   p.col_tiles = (p.cols + lf::tile_columns(p.cols) - 1) / lf::tile_columns(p.cols);
   LF_CHECK_SUPPORTED(static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles <=
-                         (1 << 30) / ((picked ? slots : p.pool.table_width) + lf::kUnitCost),
+                         (1 << 30) / ((sparse ? a->slots : p.pool.table_width) + lf::kUnitCost),
                      "lf_int4_attend: %d sequences of %d pages are too many for one call", p.pool.batch,
                      p.pool.table_width);
-  p.partials = static_cast<float*>(workspace);
-  p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + lf::partial_bytes(sms));
-  p.status = status;
+  p.partials = static_cast<float*>(a->workspace);
+  p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + lf::partial_bytes(sms));
+  p.status = a->status;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == LF_F16)
-    return head_dim == 128 ? lf::launch_attend_by<__half, 128>(p, sms, s) : lf::launch_attend_by<__half, 64>(p, sms, s);
-  return head_dim == 128 ? lf::launch_attend_by<__nv_bfloat16, 128>(p, sms, s)
-                         : lf::launch_attend_by<__nv_bfloat16, 64>(p, sms, s);
+  if (a->dtype == LF_F16)
+    return a->head_dim == 128 ? lf::launch_attend_by<__half, 128>(p, sms, s) : lf::launch_attend_by<__half, 64>(p, sms, s);
+  return a->head_dim == 128 ? lf::launch_attend_by<__nv_bfloat16, 128>(p, sms, s)
+                            : lf::launch_attend_by<__nv_bfloat16, 64>(p, sms, s);
+}
+
+extern "C" int lf_int4_attend_sparse(const lf_int4_query* a, lf_stream_t stream) {
+  const int bad = lf_int4_select(a, stream);
+  return bad != LF_OK ? bad : lf_int4_attend(a, stream);
 }

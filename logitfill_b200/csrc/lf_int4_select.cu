@@ -278,47 +278,44 @@ static int launch_select(SelectParams p, cudaStream_t stream) {
 
 }  // namespace lf
 
-extern "C" int lf_int4_select(const lf_int4_pool* pool, int head_dim, const void* q, int q_dtype, int64_t q_seq_stride,
-                              int64_t q_head_stride, int64_t q_tok_stride, int q_len, int n_q, const int8_t* bounds,
-                              int64_t bounds_page_stride, int64_t bounds_head_stride, const int32_t* lengths,
-                              const int32_t* counts, int top_pages, int sink_pages, int recent_pages, int32_t* picked, int32_t* status,
-                              lf_stream_t stream) {
+extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
+  LF_CHECK_ARG(a != nullptr, "lf_int4_select: null arguments");
   lf::SelectParams p;
-  const int bad = lf::check_int4_pool("lf_int4_select", pool, head_dim, p.pool);
+  const int bad = lf::check_int4_pool("lf_int4_select", a->pool, a->head_dim, p.pool);
   if (bad != LF_OK) return bad;
-  LF_CHECK_ARG(q && bounds && lengths && picked, "lf_int4_select: null pointer");
-  LF_CHECK_SUPPORTED(q_dtype == LF_F16 || q_dtype == LF_BF16, "lf_int4_select: query dtype %d (fp16 or bf16)", q_dtype);
-  LF_CHECK_ARG(q_len > 0 && q_len <= 65535 && n_q > 0 && n_q % p.pool.kv_heads == 0,
-               "lf_int4_select: q_len %d, %d query heads on %d KV heads", q_len, n_q, p.pool.kv_heads);
-  LF_CHECK_SUPPORTED(n_q / p.pool.kv_heads <= 64, "lf_int4_select: %d query heads per KV head (64 at most)",
-                     n_q / p.pool.kv_heads);
-  LF_CHECK_ARG(top_pages >= 0 && sink_pages >= 0 && recent_pages >= 1 && top_pages <= (1 << 24) &&
-                   sink_pages <= (1 << 24) && recent_pages <= (1 << 24),
-               "lf_int4_select: top %d, sink %d, recent %d pages (recent at least 1)", top_pages, sink_pages, recent_pages);
-  LF_CHECK_ARG(bounds_page_stride > 2 * head_dim && bounds_head_stride > 2 * head_dim,
+  LF_CHECK_ARG(a->q && a->bounds && a->lengths && a->picked, "lf_int4_select: null pointer");
+  LF_CHECK_SUPPORTED(a->dtype == LF_F16 || a->dtype == LF_BF16, "lf_int4_select: query dtype %d (fp16 or bf16)", a->dtype);
+  LF_CHECK_ARG(a->q_len > 0 && a->q_len <= 65535 && a->n_q > 0 && a->n_q % p.pool.kv_heads == 0,
+               "lf_int4_select: q_len %d, %d query heads on %d KV heads", a->q_len, a->n_q, p.pool.kv_heads);
+  p.group = a->n_q / p.pool.kv_heads;
+  LF_CHECK_SUPPORTED(p.group <= 64, "lf_int4_select: %d query heads per KV head (64 at most)", p.group);
+  LF_CHECK_ARG(a->sink_pages >= 0 && a->recent_pages >= 1 && a->slots <= (1 << 24) &&
+                   static_cast<int64_t>(a->sink_pages) + a->recent_pages <= a->slots,
+               "lf_int4_select: sink %d, recent %d of %d pages (recent at least 1)", a->sink_pages, a->recent_pages,
+               a->slots);
+  LF_CHECK_ARG(a->bounds_page_stride > 2 * a->head_dim && a->bounds_head_stride > 2 * a->head_dim,
                "lf_int4_select: bounds records overlap");
-  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(bounds) & 7) == 0 && (bounds_page_stride | bounds_head_stride) % 8 == 0,
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->bounds) & 7) == 0 && (a->bounds_page_stride | a->bounds_head_stride) % 8 == 0,
                "lf_int4_select: bounds records must be 8-byte aligned");
   LF_CHECK_SUPPORTED(p.pool.table_width <= lf::kMaxSelectPages, "lf_int4_select: %d pages per sequence (%d at most)",
                      p.pool.table_width, lf::kMaxSelectPages);
-  p.q = q;
-  p.q_seq = q_seq_stride;
-  p.q_head = q_head_stride;
-  p.q_tok = q_tok_stride;
-  p.q_len = q_len;
-  p.group = n_q / p.pool.kv_heads;
-  p.bounds = bounds;
-  p.bounds_page = bounds_page_stride;
-  p.bounds_head = bounds_head_stride;
-  p.lengths = lengths;
-  p.counts = counts;
-  p.top = top_pages;
-  p.sink = sink_pages;
-  p.recent = recent_pages;
-  p.picked = picked;
-  p.status = status;
+  p.q = a->q;
+  p.q_seq = a->q_seq_stride;
+  p.q_head = a->q_head_stride;
+  p.q_tok = a->q_tok_stride;
+  p.q_len = a->q_len;
+  p.bounds = a->bounds;
+  p.bounds_page = a->bounds_page_stride;
+  p.bounds_head = a->bounds_head_stride;
+  p.lengths = a->lengths;
+  p.counts = a->counts;
+  p.top = a->slots - a->sink_pages - a->recent_pages;
+  p.sink = a->sink_pages;
+  p.recent = a->recent_pages;
+  p.picked = a->picked;
+  p.status = a->status;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (q_dtype == LF_F16)
-    return head_dim == 128 ? lf::launch_select<__half, 128>(p, s) : lf::launch_select<__half, 64>(p, s);
-  return head_dim == 128 ? lf::launch_select<__nv_bfloat16, 128>(p, s) : lf::launch_select<__nv_bfloat16, 64>(p, s);
+  if (a->dtype == LF_F16)
+    return a->head_dim == 128 ? lf::launch_select<__half, 128>(p, s) : lf::launch_select<__half, 64>(p, s);
+  return a->head_dim == 128 ? lf::launch_select<__nv_bfloat16, 128>(p, s) : lf::launch_select<__nv_bfloat16, 64>(p, s);
 }

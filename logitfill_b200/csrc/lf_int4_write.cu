@@ -170,9 +170,9 @@ __device__ __forceinline__ uint32_t quantise8(const Chunk<T>& chunk, const Group
   return w - kMagicBits * 0x11111111u;
 }
 
-struct WriteParams {
+struct TokenParams {  // of a write (key, value: sources) or a read (destinations)
   Int4Pool pool;
-  const void *key, *value;
+  void *key, *value;
   int64_t k_seq, k_head, k_tok, v_seq, v_head, v_tok;
   int tokens;
   const int32_t *start, *counts;
@@ -300,7 +300,7 @@ __device__ __forceinline__ int token_word(int k, int x) {
 // One CTA per (page, KV head): its tokens of the page, and the page's bounds once
 // its last slot is written.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __grid_constant__ WriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __grid_constant__ TokenParams p) {
   constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes, kWords = 20 * D / kInt4Page;
   __shared__ __align__(16) uint32_t rec_s[20 * D];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
@@ -384,18 +384,9 @@ __global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __g
   if (whole) write_bounds<D>(rec_s, p.bounds + id * p.bounds_page + h * p.bounds_head);
 }
 
-struct ReadParams {
-  Int4Pool pool;
-  const int32_t *start, *counts;
-  int tokens;
-  void *out_k, *out_v;
-  int32_t* status;
-};
-
-// out [batch][kv_heads][tokens][D]: token i is position start[b] + i, zero from
-// counts[b] on.  One CTA per 64 tokens, which lie in two pages at most.
+// Token i is position start[b] + i, zero from counts[b] on.  One CTA per 64 tokens, which lie in two pages at most.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_constant__ ReadParams p) {
+__global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_constant__ TokenParams p) {
   constexpr int kLanes = D / 8, kRows = kWriteThreads / kLanes;
   const int b = blockIdx.z, h = blockIdx.y;
   grid_dep_wait();
@@ -412,6 +403,8 @@ __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_c
   };
   const uint32_t *rec0 = record(0), *rec1 = record(1);
   const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));
+  T* key = static_cast<T*>(p.key) + b * p.k_seq + h * p.k_head + i0 * p.k_tok + 8 * l;
+  T* value = static_cast<T*>(p.value) + b * p.v_seq + h * p.v_head + i0 * p.v_tok + 8 * l;
   constexpr int kAtOnce = 4;  // rows whose loads are in flight together
   for (int r0 = row; r0 < last - i0; r0 += kAtOnce * kRows) {
     uint32_t kw[kAtOnce], kp[kAtOnce], vp[kAtOnce], v0[kAtOnce], v1[kAtOnce];
@@ -438,10 +431,9 @@ __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_c
       float xk[8], xv[8];
       values8(kw[y], half_lo(kp[y]), half_hi(kp[y]), xk);
       values8(__byte_perm(v0[y], v1[y], u == 0 ? 0x5410 : 0x7632), half_lo(vp[y]), half_hi(vp[y]), xv);
-      const int64_t dst = ((static_cast<int64_t>(b) * p.pool.kv_heads + h) * p.tokens + i0 + i) * D + 8 * l;
       if (i < last - i0) {
-        store8<T>(static_cast<T*>(p.out_k) + dst, xk);
-        store8<T>(static_cast<T*>(p.out_v) + dst, xv);
+        store8<T>(key + i * p.k_tok, xk);
+        store8<T>(value + i * p.v_tok, xv);
       }
     }
   }
@@ -477,94 +469,85 @@ template <typename T> static const void* read_kernel(int D) {
                   : reinterpret_cast<const void*>(int4_read_kernel<T, 64>);
 }
 
-int check_int4_pool(const char* what, const lf_int4_pool* pool, int head_dim, Int4Pool& out) {
-  LF_CHECK_ARG(pool && pool->pages && pool->table, "%s: null pool, pages or page table", what);
+int check_int4_pool(const char* what, const lf_int4_pool& pool, int head_dim, Int4Pool& out) {
+  LF_CHECK_ARG(pool.pages && pool.table, "%s: null pages or page table", what);
   LF_CHECK_SUPPORTED(head_dim == 64 || head_dim == 128, "%s: head_dim %d (64 or 128)", what, head_dim);
-  LF_CHECK_ARG(pool->kv_heads > 0 && pool->batch > 0 && pool->n_pages > 0 && pool->table_width > 0,
+  LF_CHECK_ARG(pool.kv_heads > 0 && pool.batch > 0 && pool.n_pages > 0 && pool.table_width > 0,
                "%s: empty pool, batch or page table", what);
-  LF_CHECK_SUPPORTED(pool->kv_heads <= 65535 && pool->batch <= 65535, "%s: %d KV heads, batch %d (65535 at most)", what,
-                     pool->kv_heads, pool->batch);
-  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(pool->pages) & 15) == 0 && pool->page_stride % 4 == 0 &&
-                   pool->head_stride % 4 == 0 && pool->head_stride >= 20 * head_dim &&
-                   pool->page_stride >= 20 * head_dim && pool->table_stride >= pool->table_width,
+  LF_CHECK_SUPPORTED(pool.kv_heads <= 65535 && pool.batch <= 65535, "%s: %d KV heads, batch %d (65535 at most)", what,
+                     pool.kv_heads, pool.batch);
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(pool.pages) & 15) == 0 && pool.page_stride % 4 == 0 &&
+                   pool.head_stride % 4 == 0 && pool.head_stride >= 20 * head_dim &&
+                   pool.page_stride >= 20 * head_dim && pool.table_stride >= pool.table_width,
                "%s: records must be 16-byte aligned and apart", what);
-  LF_CHECK_SUPPORTED(pool->table_width <= INT32_MAX / kInt4Page, "%s: page table width %d", what, pool->table_width);
-  out.words = pool->pages;
-  out.page_stride = pool->page_stride;
-  out.head_stride = pool->head_stride;
-  out.table = pool->table;
-  out.table_stride = pool->table_stride;
-  out.table_width = pool->table_width;
-  out.n_pages = pool->n_pages;
-  out.kv_heads = pool->kv_heads;
-  out.batch = pool->batch;
+  LF_CHECK_SUPPORTED(pool.table_width <= INT32_MAX / kInt4Page, "%s: page table width %d", what, pool.table_width);
+  out.words = pool.pages;
+  out.page_stride = pool.page_stride;
+  out.head_stride = pool.head_stride;
+  out.table = pool.table;
+  out.table_stride = pool.table_stride;
+  out.table_width = pool.table_width;
+  out.n_pages = pool.n_pages;
+  out.kv_heads = pool.kv_heads;
+  out.batch = pool.batch;
+  return LF_OK;
+}
+
+// Checks shared by writes and reads.
+static int check_tokens(const char* what, const lf_int4_tokens* a, TokenParams& p) {
+  LF_CHECK_ARG(a != nullptr, "%s: null arguments", what);
+  const int bad = check_int4_pool(what, a->pool, a->head_dim, p.pool);
+  if (bad != LF_OK) return bad;
+  LF_CHECK_ARG(a->tokens >= 0 && a->tokens <= (1 << 30), "%s: %d tokens", what, a->tokens);
+  LF_CHECK_ARG(a->tokens == 0 || (a->key && a->value && a->start), "%s: null pointer", what);
+  LF_CHECK_ARG(a->dtype == LF_F32 || a->dtype == LF_F16 || a->dtype == LF_BF16, "%s: dtype %d", what, a->dtype);
+  const int64_t unit = a->dtype == LF_F32 ? 4 : 8;  // elements in 16 bytes
+  LF_CHECK_ARG(((reinterpret_cast<uintptr_t>(a->key) | reinterpret_cast<uintptr_t>(a->value)) & 15) == 0 &&
+                   (a->k_seq_stride | a->k_head_stride | a->k_tok_stride | a->v_seq_stride | a->v_head_stride |
+                    a->v_tok_stride) % unit == 0,
+               "%s: Key and Value rows must be 16-byte aligned", what);
+  LF_CHECK_ARG(a->bounds == nullptr || (a->bounds_page_stride > 2 * a->head_dim && a->bounds_head_stride > 2 * a->head_dim),
+               "%s: bounds records overlap", what);
+  p.key = a->key;
+  p.value = a->value;
+  p.k_seq = a->k_seq_stride;
+  p.k_head = a->k_head_stride;
+  p.k_tok = a->k_tok_stride;
+  p.v_seq = a->v_seq_stride;
+  p.v_head = a->v_head_stride;
+  p.v_tok = a->v_tok_stride;
+  p.tokens = a->tokens;
+  p.start = a->start;
+  p.counts = a->counts;
+  p.bounds = a->bounds;
+  p.bounds_page = a->bounds_page_stride;
+  p.bounds_head = a->bounds_head_stride;
+  p.status = a->status;
   return LF_OK;
 }
 
 }  // namespace lf
 
-extern "C" int lf_int4_write(const lf_int4_pool* pool, int head_dim, const void* key, const void* value, int dtype,
-                             int64_t k_seq_stride, int64_t k_head_stride, int64_t k_tok_stride, int64_t v_seq_stride,
-                             int64_t v_head_stride, int64_t v_tok_stride, int tokens, const int32_t* start,
-                             const int32_t* counts, int8_t* bounds, int64_t bounds_page_stride,
-                             int64_t bounds_head_stride, int32_t* status, lf_stream_t stream) {
-  lf::WriteParams p;
-  const int bad = lf::check_int4_pool("lf_int4_write", pool, head_dim, p.pool);
-  if (bad != LF_OK) return bad;
-  LF_CHECK_ARG(key && value && start, "lf_int4_write: null pointer");
-  LF_CHECK_ARG(dtype == LF_F32 || dtype == LF_F16 || dtype == LF_BF16, "lf_int4_write: dtype %d", dtype);
-  LF_CHECK_ARG(tokens >= 0 && tokens <= (1 << 30), "lf_int4_write: %d tokens", tokens);
-  const int64_t unit = dtype == LF_F32 ? 4 : 8;  // elements in 16 bytes
-  LF_CHECK_ARG(((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) == 0 &&
-                   (k_seq_stride | k_head_stride | k_tok_stride | v_seq_stride | v_head_stride | v_tok_stride) % unit == 0,
-               "lf_int4_write: Key and Value rows must be 16-byte aligned");
-  LF_CHECK_ARG(bounds == nullptr || (bounds_page_stride > 2 * head_dim && bounds_head_stride > 2 * head_dim),
-               "lf_int4_write: bounds records overlap");
-  if (tokens == 0) return LF_OK;
-  p.key = key;
-  p.value = value;
-  p.k_seq = k_seq_stride;
-  p.k_head = k_head_stride;
-  p.k_tok = k_tok_stride;
-  p.v_seq = v_seq_stride;
-  p.v_head = v_head_stride;
-  p.v_tok = v_tok_stride;
-  p.tokens = tokens;
-  p.start = start;
-  p.counts = counts;
-  p.bounds = bounds;
-  p.bounds_page = bounds_page_stride;
-  p.bounds_head = bounds_head_stride;
-  p.status = status;
+extern "C" int lf_int4_write(const lf_int4_tokens* a, lf_stream_t stream) {
+  lf::TokenParams p;
+  const int bad = lf::check_tokens("lf_int4_write", a, p);
+  if (bad != LF_OK || a->tokens == 0) return bad;
   // tokens that start anywhere in a page touch at most this many pages
-  const dim3 grid((tokens + 2 * lf::kInt4Page - 2) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
-  const void* kern = dtype == LF_F32   ? lf::write_kernel<float>(head_dim)
-                     : dtype == LF_F16 ? lf::write_kernel<__half>(head_dim)
-                                       : lf::write_kernel<__nv_bfloat16>(head_dim);
+  const dim3 grid((a->tokens + 2 * lf::kInt4Page - 2) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
+  const void* kern = a->dtype == LF_F32   ? lf::write_kernel<float>(a->head_dim)
+                     : a->dtype == LF_F16 ? lf::write_kernel<__half>(a->head_dim)
+                                          : lf::write_kernel<__nv_bfloat16>(a->head_dim);
   return lf::launch(kern, "lf_int4_write", grid, p, reinterpret_cast<cudaStream_t>(stream));
 }
 
-extern "C" int lf_int4_read(const lf_int4_pool* pool, int head_dim, const int32_t* start, const int32_t* counts,
-                            int tokens, void* out_k, void* out_v, int out_dtype, int32_t* status, lf_stream_t stream) {
-  lf::ReadParams p;
-  const int bad = lf::check_int4_pool("lf_int4_read", pool, head_dim, p.pool);
-  if (bad != LF_OK) return bad;
-  LF_CHECK_ARG(start && out_k && out_v, "lf_int4_read: null pointer");
-  LF_CHECK_ARG(out_dtype == LF_F32 || out_dtype == LF_F16 || out_dtype == LF_BF16, "lf_int4_read: dtype %d", out_dtype);
-  LF_CHECK_ARG(tokens >= 0 && tokens <= (1 << 30), "lf_int4_read: %d tokens", tokens);
-  LF_CHECK_ARG(((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) & 15) == 0,
-               "lf_int4_read: outputs must be 16-byte aligned");
-  if (tokens == 0) return LF_OK;
-  p.start = start;
-  p.counts = counts;
-  p.tokens = tokens;
-  p.out_k = out_k;
-  p.out_v = out_v;
-  p.status = status;
-  const dim3 grid((tokens + lf::kInt4Page - 1) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
-  const void* kern = out_dtype == LF_F32   ? lf::read_kernel<float>(head_dim)
-                     : out_dtype == LF_F16 ? lf::read_kernel<__half>(head_dim)
-                                           : lf::read_kernel<__nv_bfloat16>(head_dim);
+extern "C" int lf_int4_read(const lf_int4_tokens* a, lf_stream_t stream) {
+  lf::TokenParams p;
+  const int bad = lf::check_tokens("lf_int4_read", a, p);
+  if (bad != LF_OK || a->tokens == 0) return bad;
+  const dim3 grid((a->tokens + lf::kInt4Page - 1) / lf::kInt4Page, p.pool.kv_heads, p.pool.batch);
+  const void* kern = a->dtype == LF_F32   ? lf::read_kernel<float>(a->head_dim)
+                     : a->dtype == LF_F16 ? lf::read_kernel<__half>(a->head_dim)
+                                          : lf::read_kernel<__nv_bfloat16>(a->head_dim);
   return lf::launch(kern, "lf_int4_read", grid, p, reinterpret_cast<cudaStream_t>(stream));
 }
 

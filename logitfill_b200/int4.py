@@ -27,8 +27,6 @@ There is no CPU or dense fallback; what the kernels do not implement raises
 """
 from __future__ import annotations
 
-import ctypes
-
 import numpy as np
 import torch
 
@@ -60,7 +58,8 @@ def alloc_bounds(n_pages: int, n_kv: int, head_dim: int, device="cuda") -> torch
 
 
 def _pool(pages: torch.Tensor, page_table: torch.Tensor):
-    """The C ABI's pool of ``pages`` and ``page_table``, the head_dim and the device."""
+    """The C ABI's pool of ``pages`` and ``page_table`` as a tuple (batch and
+    KV heads last), the head_dim and the device."""
     shape, strides = pages.shape, pages.stride()
     if len(shape) != 3 or pages.dtype != torch.int32 or strides[2] != 1:
         raise ValueError(f"pages must be int32 [n_pages, n_kv, words] with word stride 1, got {pages.dtype} {tuple(shape)}")
@@ -77,8 +76,8 @@ def _pool(pages: torch.Tensor, page_table: torch.Tensor):
     B, W = table_shape
     if words % 20:
         raise ValueError(f"a record of {words} words belongs to no head_dim (20 * head_dim words)")
-    return _lib.LfInt4Pool(pages.data_ptr(), page_table.data_ptr(), strides[0] if n > 1 else H * words,
-                           strides[1] if H > 1 else words, table_strides[0] if B > 1 else W, W, n, H, B), words // 20, device
+    return (pages.data_ptr(), page_table.data_ptr(), strides[0] if n > 1 else H * words, strides[1] if H > 1 else words,
+            table_strides[0] if B > 1 else W, W, n, H, B), words // 20, device
 
 
 def _per_sequence(name: str, t: torch.Tensor | None, batch: int, device) -> int:
@@ -152,7 +151,7 @@ def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page
     channels whose scale or minimum is no finite fp16 number (a NaN, an
     infinity, a range past 15 * 65504) reads back as NaN."""
     pool, D, dev = _pool(pages, page_table)
-    B, H = pool.batch, pool.kv_heads
+    H, B = pool[-2:]
     if key.dim() != 4 or key.shape != value.shape or (key.shape[0], key.shape[1], key.shape[3]) != (B, H, D):
         raise ValueError(f"key and value must be [{B}, {H}, T, {D}], got {tuple(key.shape)} and {tuple(value.shape)}")
     if key.dtype != value.dtype:
@@ -160,17 +159,14 @@ def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page
     if key.device != dev or value.device != dev:
         raise RuntimeError(f"key and value must be on {dev}")
     code = _lib.dtype_code(key.dtype)
-    addresses = (_per_sequence("start", start, B, dev), _per_sequence("counts", counts, B, dev))
-    if key.shape[2] == 0:
-        return
     key, *ks = _aligned_rows(key)
     value, *vs = _aligned_rows(value)
-    bp, b0, b1 = (0, 0, 0) if bounds is None else _bounds(bounds, pages, D)
+    args = _lib.INT4_TOKENS.pack(
+        *pool, key.data_ptr(), value.data_ptr(), *ks, *vs, _per_sequence("start", start, B, dev),
+        _per_sequence("counts", counts, B, dev), *((0, 0, 0) if bounds is None else _bounds(bounds, pages, D)),
+        _status(status, dev), D, code, key.shape[2])
     with _on(dev):
-        _lib.check(_lib.lib().lf_int4_write(
-            ctypes.byref(pool), D, key.data_ptr(), value.data_ptr(), code, *ks, *vs, key.shape[2],
-            *addresses, bp, b0, b1,
-            _status(status, dev), _stream(dev)), "lf_int4_write")
+        _lib.check(_lib.lib().lf_int4_write(args, _stream(dev)), "lf_int4_write")
 
 
 def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor, tokens: int,
@@ -183,14 +179,15 @@ def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor
     if tokens < 0:
         raise ValueError(f"cannot read {tokens} tokens")
     code = _lib.dtype_code(dtype)
-    out = torch.empty(2, pool.batch, pool.kv_heads, tokens, D, dtype=dtype, device=dev)
+    H, B = pool[-2:]
+    out = torch.empty((2, B, H, tokens, D), dtype=dtype, device=dev)
     key, value = out[0], out[1]
-    addresses = (_per_sequence("start", start, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev))
-    if tokens:
-        with _on(dev):
-            _lib.check(_lib.lib().lf_int4_read(
-                ctypes.byref(pool), D, *addresses, tokens, key.data_ptr(), value.data_ptr(), code, _status(status, dev),
-                _stream(dev)), "lf_int4_read")
+    strides = H * tokens * D, tokens * D, D
+    args = _lib.INT4_TOKENS.pack(
+        *pool, key.data_ptr(), value.data_ptr(), *strides, *strides, _per_sequence("start", start, B, dev),
+        _per_sequence("counts", counts, B, dev), 0, 0, 0, _status(status, dev), D, code, tokens)
+    with _on(dev):
+        _lib.check(_lib.lib().lf_int4_read(args, _stream(dev)), "lf_int4_read")
     return key, value
 
 
@@ -214,42 +211,46 @@ def int4_read_bounds(bounds: torch.Tensor) -> torch.Tensor:
 _workspaces: dict = {}
 
 
-def _workspace(pool, n_q: int, q_len: int, head_dim: int, device) -> torch.Tensor:
-    """Scratch of an attention call: partial results, then tickets that are zero
-    between calls.  Calls on one stream share one buffer (they run in order);
-    a call being captured in a CUDA graph gets its own, which the graph keeps
-    and clears, so replays on any stream do not meet."""
+def _workspace(pool, n_q: int, q_len: int, head_dim: int, device):
+    """Scratch of an attention call, its address and bytes: partial results,
+    then tickets that are zero between calls.  Calls on one stream share one
+    buffer (they run in order); a call being captured in a CUDA graph gets its
+    own, which the graph keeps and clears, so replays on any stream do not
+    meet."""
+    H, B = pool[-2:]
     key = (device.index, _stream(device))
     # a ticket for each column tile of 16 at most, of each query token and KV head
-    units = pool.batch * pool.kv_heads * q_len * (n_q // pool.kv_heads + 15)
+    units = B * H * q_len * (n_q // H + 15)
     held = _workspaces.get(key)
     capturing = torch.cuda.is_current_stream_capturing()
     if held is not None and held[1] >= units and not capturing:
-        return held[0]
+        return held[0], held[2], held[3]
     so = _lib.lib()
-    need = so.lf_int4_workspace_bytes(pool.batch, pool.kv_heads, n_q, q_len, head_dim)
+    need = so.lf_int4_workspace_bytes(B, H, n_q, q_len, head_dim)
     if capturing:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         ws[so.lf_int4_workspace_clear_from():].zero_()
-        return ws
+        return ws, ws.data_ptr(), need
     units = max(units, 1 << 16)
-    ws = torch.zeros(max(need, so.lf_int4_workspace_clear_from() + 4 * units), dtype=torch.uint8, device=device)
-    _workspaces[key] = ws, units
-    return ws
+    need = max(need, so.lf_int4_workspace_clear_from() + 4 * units)
+    ws = torch.zeros(need, dtype=torch.uint8, device=device)
+    _workspaces[key] = ws, units, ws.data_ptr(), need
+    return ws, ws.data_ptr(), need
 
 
 def _query(query: torch.Tensor, pool, head_dim: int, device):
     """The query, checked, as [B, n_q, q_len, D] with 16-byte aligned rows of
     channel stride 1, and its first three strides."""
     q = query if query.dim() == 4 else query.unsqueeze(2)
+    H, batch = pool[-2:]
     if q.dim() != 4:
         raise ValueError(f"query must be [batch, n_q, head_dim] or [batch, n_q, q_len, head_dim], got {tuple(query.shape)}")
     B, n_q, q_len, D = q.shape
-    if B != pool.batch or D != head_dim or n_q < 1 or q_len < 1:
-        raise ValueError(f"query must be [{pool.batch}, n_q, {head_dim}] or [{pool.batch}, n_q, q_len, {head_dim}], got "
+    if B != batch or D != head_dim or n_q < 1 or q_len < 1:
+        raise ValueError(f"query must be [{batch}, n_q, {head_dim}] or [{batch}, n_q, q_len, {head_dim}], got "
                          f"{tuple(query.shape)}")
-    if n_q % pool.kv_heads:
-        raise ValueError(f"{n_q} query heads do not divide into {pool.kv_heads} KV heads")
+    if n_q % H:
+        raise ValueError(f"{n_q} query heads do not divide into {H} KV heads")
     if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise NotImplementedError(f"the 4-bit cache's attention takes fp16 or bf16 queries, got {q.dtype}")
     if q.device != device:
@@ -257,42 +258,42 @@ def _query(query: torch.Tensor, pool, head_dim: int, device):
     return _aligned_rows(q)
 
 
-def _out(query: torch.Tensor, out: torch.Tensor | None, device) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(query, memory_format=torch.contiguous_format)
-    if out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1:
-        raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} on {device} with channel stride 1")
-    return out
-
-
-def _attend(pool, D, dev, q, lengths: int, counts: int, picked: int, slots: int, scaling: float, out: torch.Tensor,
-            status: int) -> None:
-    """Launch the attention of ``q`` (from :func:`_query`) into ``out``; ``lengths``,
-    ``counts``, ``picked`` and ``status`` are addresses."""
-    t, s0, s1, s2 = q
-    n_q, q_len = t.shape[1], t.shape[2]
-    strides = out.stride()
-    ws = _workspace(pool, n_q, q_len, D, dev)
-    _lib.check(_lib.lib().lf_int4_attend(
-        ctypes.byref(pool), D, t.data_ptr(), _CODE[t.dtype], s0, s1, s2, q_len, n_q, lengths, counts, picked, slots,
-        scaling, out.data_ptr(), strides[0], strides[1], strides[2] if len(strides) == 4 else 0, ws.data_ptr(), ws.numel(),
-        status, _stream(dev)), "lf_int4_attend")
-
-
-def _select(pool, D, dev, q, bounds: torch.Tensor, pages: torch.Tensor, lengths: int, counts: int, top_pages: int,
-            sink_pages: int, recent_pages: int, status: int) -> torch.Tensor:
-    """Launch the page choice of ``q`` (from :func:`_query`)."""
-    t, s0, s1, s2 = q
-    n_q, q_len = t.shape[1], t.shape[2]
+def _budget(top_pages: int, sink_pages: int, recent_pages: int):
     top, sink, recent = int(top_pages), int(sink_pages), int(recent_pages)
     if top < 0 or sink < 0 or recent < 1:
         raise ValueError(f"top {top} and sink {sink} must not be negative, recent {recent} at least 1")
-    bp, b0, b1 = _bounds(bounds, pages, D)
-    picked = torch.empty((pool.batch, q_len, pool.kv_heads, sink + recent + top), dtype=torch.int32, device=dev)
-    _lib.check(_lib.lib().lf_int4_select(
-        ctypes.byref(pool), D, t.data_ptr(), _CODE[t.dtype], s0, s1, s2, q_len, n_q, bp, b0, b1, lengths, counts, top, sink,
-        recent, picked.data_ptr(), status, _stream(dev)), "lf_int4_select")
-    return picked
+    return top + sink + recent, sink, recent
+
+
+def _attend(entry: str, query, pages, page_table, lengths, scaling, counts, out, status, bounds=None, budget=(0, 0, 0)):
+    """The dense (``lf_int4_attend``), the sparse (``lf_int4_attend_sparse``) or
+    only the page choice's (``lf_int4_select``) call: ``(out, picked)``."""
+    pool, D, dev = _pool(pages, page_table)
+    q, s0, s1, s2 = _query(query, pool, D, dev)
+    H, B = pool[-2:]
+    n_q, q_len = q.shape[1], q.shape[2]
+    if entry == "lf_int4_select":
+        out_args = workspace = (0, 0, 0, 0)
+    else:
+        if out is None:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride(-1) != 1:
+            raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} on {dev} with channel stride 1")
+        o = out.stride()
+        out_args = out.data_ptr(), o[0], o[1], o[2] if len(o) == 4 else 0
+        workspace = _workspace(pool, n_q, q_len, D, dev)
+    picked, picked_at, bounds_args = None, 0, (0, 0, 0)
+    if bounds is not None:
+        bounds_args = _bounds(bounds, pages, D)
+        picked = torch.empty((B, q_len, H, budget[0]), dtype=torch.int32, device=dev)
+        picked_at = picked.data_ptr()
+    args = _lib.INT4_QUERY.pack(
+        *pool, q.data_ptr(), s0, s1, s2, *out_args, _per_sequence("lengths", lengths, B, dev),
+        _per_sequence("counts", counts, B, dev), *bounds_args, picked_at, workspace[1], workspace[2], _status(status, dev),
+        scaling, D, _CODE[q.dtype], n_q, q_len, *budget)
+    with _on(dev):
+        _lib.check(getattr(_lib.lib(), entry)(args, _stream(dev)), entry)
+    return out, picked
 
 
 def int4_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -305,13 +306,7 @@ def int4_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.T
     positions ``0 .. lengths[b] - q_len + i``.  With ``counts`` (int32
     ``[batch]``) sequence ``b`` has only its first ``counts[b]`` query tokens;
     the others, and those that see nothing, get zeros."""
-    pool, D, dev = _pool(pages, page_table)
-    q = _query(query, pool, D, dev)
-    out = _out(query, out, dev)
-    with _on(dev):
-        _attend(pool, D, dev, q, _per_sequence("lengths", lengths, pool.batch, dev),
-                _per_sequence("counts", counts, pool.batch, dev), 0, 0, scaling, out, _status(status, dev))
-    return out
+    return _attend("lf_int4_attend", query, pages, page_table, lengths, scaling, counts, out, status)[0]
 
 
 def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
@@ -323,12 +318,8 @@ def int4_select(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, 
     the page being filled) are always in; of the rest the ``top_pages`` with
     the largest bound on the scores of the KV head's queries (summed over its
     query heads; ties to the lower page)."""
-    pool, D, dev = _pool(pages, page_table)
-    q = _query(query, pool, D, dev)
-    with _on(dev):
-        return _select(pool, D, dev, q, bounds, pages, _per_sequence("lengths", lengths, pool.batch, dev),
-                       _per_sequence("counts", counts, pool.batch, dev), top_pages, sink_pages, recent_pages,
-                       _status(status, dev))
+    return _attend("lf_int4_select", query, pages, page_table, lengths, 0.0, counts, None, status, bounds,
+                   _budget(top_pages, sink_pages, recent_pages))[1]
 
 
 def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor,
@@ -338,15 +329,8 @@ def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torc
     """:func:`int4_select`, then :func:`int4_attention` over the picked pages
     only: ``(out, picked)``.  With ``sink + recent + top`` pages or fewer
     visible, every page is read and the result is the dense one."""
-    pool, D, dev = _pool(pages, page_table)
-    q = _query(query, pool, D, dev)
-    out = _out(query, out, dev)
-    addresses = _per_sequence("lengths", lengths, pool.batch, dev), _per_sequence("counts", counts, pool.batch, dev)
-    flag = _status(status, dev)
-    with _on(dev):
-        picked = _select(pool, D, dev, q, bounds, pages, *addresses, top_pages, sink_pages, recent_pages, flag)
-        _attend(pool, D, dev, q, *addresses, picked.data_ptr(), picked.shape[3], scaling, out, flag)
-    return out, picked
+    return _attend("lf_int4_attend_sparse", query, pages, page_table, lengths, scaling, counts, out, status, bounds,
+                   _budget(top_pages, sink_pages, recent_pages))
 
 
 class Int4KVCache:
