@@ -400,7 +400,7 @@ typedef struct lf_int4_query {
   lf_int4_pool pool;
   const void* q;          /* [batch][n_q][q_len][head_dim], channel stride 1, rows 16-byte aligned */
   int64_t q_seq_stride, q_head_stride, q_tok_stride;
-  void* out;              /* as q                                                */
+  void* out;              /* as q, rows 8-byte aligned                            */
   int64_t out_seq_stride, out_head_stride, out_tok_stride;
   const int32_t* lengths; /* [batch] tokens cached, the query's own among them   */
   const int32_t* counts;  /* [batch] query tokens of each sequence, or NULL: q_len */

@@ -47,7 +47,6 @@ struct AttendParams {
   float scale_log2;
   void* out;
   int64_t out_seq, out_head, out_tok;
-  bool out_aligned;           // four channels of an output row can be stored at once
   int rows, cols, col_tiles;  // sequences (or query tokens), query columns of a unit, column tiles
   float* partials;
   uint32_t* tickets;
@@ -60,6 +59,9 @@ constexpr float kNoMax = -1e30f;
 #ifndef LF_MINP
 #define LF_MINP 4
 #define LF_COST 6
+#endif
+#ifndef LF_MERGE
+#define LF_MERGE 0.33f
 #endif
 constexpr int kMinPages = LF_MINP;  // places of a range at least: one page for each pair of warps
 constexpr int kUnitCost = LF_COST;
@@ -199,6 +201,13 @@ __device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
   return max(1, min(n, kSparse ? p.slots : p.pool.table_width));
 }
 
+// Places of a range below which the merge costs more than the range: with n pages
+// a unit in ranges of r, r pages take 0.3 r us and the last to arrive another 0.1 us
+// for each of n / r parts, least at r = sqrt(n / 3).
+__device__ __forceinline__ int merge_pages(int total, int units) {
+  return static_cast<int>(sqrtf(static_cast<float>(total / units) * LF_MERGE));
+}
+
 template <typename T, int D, int NT, bool kSparse>
 __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::kCtas)
     int4_attend_kernel(const __grid_constant__ AttendParams p) {
@@ -219,7 +228,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   const int places0 = places(lane);
   int total = __reduce_add_sync(0xffffffffu, places0);
   for (int r0 = 32; r0 < p.rows; r0 += 32) total += __reduce_add_sync(0xffffffffu, places(r0 + lane));
-  const int per = max(kMinPages, static_cast<int>((total + gridDim.x - 1) / gridDim.x));
+  const int per = max(kMinPages, max(static_cast<int>((total + gridDim.x - 1) / gridDim.x), merge_pages(total, p.rows * per_row)));
   const int begin = blockIdx.x * per, end = min(total, begin + per);
   if (begin >= end) return;
   int row = 0, row_base = 0;
@@ -283,32 +292,25 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     }
 
     // This warp's pages: first + team, then every kTeams-th.  Their ids, 32 at a
-    // time, one per lane, loaded a window ahead.
+    // time, one per lane.
     const int mine_n = first + team < stop ? (stop - first - team + C::kTeams - 1) / C::kTeams : 0;
-    auto load_ids = [&](int x0, int& id, int& logical) {
-      const int x = x0 + lane;
-      id = logical = -1;
-      if (x < mine_n) {
-        logical = first + team + x * C::kTeams;
-        if constexpr (kSparse)
-          logical = p.picked[(static_cast<int64_t>(row_now) * p.pool.kv_heads + h) * p.slots + logical];
-        if (logical >= 0 && static_cast<int64_t>(logical) * kInt4Page < seen_max) {
-          id = int4_page_id(p.pool, b, logical);
-          if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
-        }
-      }
-    };
-    int ids, logicals, ids_next, logicals_next;
-    load_ids(0, ids, logicals);
-    load_ids(32, ids_next, logicals_next);
+    const int32_t* listed =
+        kSparse ? p.picked + (static_cast<int64_t>(row_now) * p.pool.kv_heads + h) * p.slots : nullptr;
+    int ids = -1, logicals = -1;
     int issued = 0, into = 0;  // pages issued, the stage of the next
     const uint8_t* head_words = reinterpret_cast<const uint8_t*>(p.pool.words + h * p.pool.head_stride);
     auto issue = [&]() {
       if (issued < mine_n) {
-        if (issued != 0 && (issued & 31) == 0) {
-          ids = ids_next;
-          logicals = logicals_next;
-          load_ids(issued + 32, ids_next, logicals_next);
+        if ((issued & 31) == 0) {
+          ids = logicals = -1;
+          if (issued + lane < mine_n) {
+            logicals = first + team + (issued + lane) * C::kTeams;
+            if constexpr (kSparse) logicals = listed[logicals];
+            if (logicals >= 0 && logicals < (seen_max + kInt4Page - 1) / kInt4Page) {
+              ids = int4_page_id(p.pool, b, logicals);
+              if (ids < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+            }
+          }
         }
         const int id = __shfl_sync(0xffffffffu, ids, issued & 31);
         const int logical = __shfl_sync(0xffffffffu, logicals, issued & 31);
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       }
       cp_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) issue();
 
     // Query fragments, sums and scales of this unit's columns.
@@ -667,19 +669,12 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       if (c >= p.cols) return;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a column that sees nothing
       T* o = out + (h * p.group + c - i * p.group) * p.out_head + (i0 + i) * p.out_tok + d;
-      if (p.out_aligned) {
-        struct alignas(4 * sizeof(T)) Four { T x[4]; } f;
-        Scalar<T>::store(f.x, v.x * inv);
-        Scalar<T>::store(f.x + 1, v.y * inv);
-        Scalar<T>::store(f.x + 2, v.z * inv);
-        Scalar<T>::store(f.x + 3, v.w * inv);
-        *reinterpret_cast<Four*>(o) = f;
-      } else {
-        Scalar<T>::store(o, v.x * inv);
-        Scalar<T>::store(o + 1, v.y * inv);
-        Scalar<T>::store(o + 2, v.z * inv);
-        Scalar<T>::store(o + 3, v.w * inv);
-      }
+      struct alignas(4 * sizeof(T)) Four { T x[4]; } f;
+      Scalar<T>::store(f.x, v.x * inv);
+      Scalar<T>::store(f.x + 1, v.y * inv);
+      Scalar<T>::store(f.x + 2, v.z * inv);
+      Scalar<T>::store(f.x + 3, v.w * inv);
+      *reinterpret_cast<Four*>(o) = f;
     };
     // The partial of range x of this unit: the range that begins inside the unit
     // uses its CTA's first record, the unit's first range the second.
@@ -722,39 +717,51 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       }
       __syncthreads();
       if (last_s) {
-#pragma unroll 1
+        constexpr int kAtOnce = NT == 1 ? 8 : 4;  // parts whose loads are in flight together, for every item
+        float top[kItems], sum[kItems];
+        float4 v[kItems];
+#pragma unroll
         for (int it = 0; it < kItems; ++it) {
-          const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
-          constexpr int kAtOnce = 8;  // parts whose loads are in flight together
-          float top = kNoMax, sum = 0.0f;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int x0 = 0; x0 < parts; x0 += kAtOnce) {
-            float tops[kAtOnce], sums[kAtOnce];
-            float4 y[kAtOnce];
+          top[it] = kNoMax;
+          sum[it] = 0.0f;
+          v[it] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        for (int x0 = 0; x0 < parts; x0 += kAtOnce) {
+          float tops[kItems][kAtOnce], sums[kItems][kAtOnce];
+          float4 y[kItems][kAtOnce];
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-              const float* rec = record(first_cta + min(x0 + x, parts - 1));
-              tops[x] = __ldcg(rec + col);
-              sums[x] = __ldcg(rec + kCol + col);
-              y[x] = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
-            }
-            float now = top;
+          for (int x = 0; x < kAtOnce; ++x) {
+            const float* rec = record(first_cta + min(x0 + x, parts - 1));
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) now = fmaxf(now, tops[x]);
-            const float fix = ex2(top - now);
-            top = now;
-            sum *= fix;
-            v = make_float4(v.x * fix, v.y * fix, v.z * fix, v.w * fix);
-#pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-              const float f = x0 + x < parts ? ex2(tops[x] - top) : 0.0f;
-              if (x0 + x < parts) {
-                sum = fmaf(f, sums[x], sum);
-                add_scaled(v, f, y[x]);
-              }
+            for (int it = 0; it < kItems; ++it) {
+              const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
+              tops[it][x] = __ldcg(rec + col);
+              sums[it][x] = __ldcg(rec + kCol + col);
+              y[it][x] = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
             }
           }
-          store(col, d, v, sum);
+#pragma unroll
+          for (int it = 0; it < kItems; ++it) {
+            float now = top[it];
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) now = fmaxf(now, tops[it][x]);
+            const float fix = ex2(top[it] - now);
+            top[it] = now;
+            sum[it] *= fix;
+            v[it] = make_float4(v[it].x * fix, v[it].y * fix, v[it].z * fix, v[it].w * fix);
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x)
+              if (x0 + x < parts) {
+                const float f = ex2(tops[it][x] - now);
+                sum[it] = fmaf(f, sums[it][x], sum[it]);
+                add_scaled(v[it], f, y[it][x]);
+              }
+          }
+        }
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+          const int item = tid + it * C::kThreads;
+          store(item / (D / 4), item % (D / 4) * 4, v[it], sum[it]);
         }
       }
     }
@@ -834,6 +841,9 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
   LF_CHECK_ARG(!sparse || a->slots > 0, "lf_int4_attend: %d slots", a->slots);
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->q) & 15) == 0 && (a->q_seq_stride | a->q_head_stride | a->q_tok_stride) % 8 == 0,
                "lf_int4_attend: query rows must be 16-byte aligned");
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&
+                   (a->out_seq_stride | a->out_head_stride | a->out_tok_stride) % 4 == 0,
+               "lf_int4_attend: output rows must be 8-byte aligned");
   const int sms = lf::sm_count();
   if (sms <= 0) return lf::launch_status("lf_int4_attend");
   LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
@@ -854,8 +864,6 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
   p.out_seq = a->out_seq_stride;
   p.out_head = a->out_head_stride;
   p.out_tok = a->out_tok_stride;
-  p.out_aligned = (reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&
-                  (a->out_seq_stride | a->out_head_stride | a->out_tok_stride) % 4 == 0;
   p.rows = sparse ? p.pool.batch * a->q_len : p.pool.batch;
   p.cols = sparse ? p.group : p.group * a->q_len;
   p.col_tiles = (p.cols + lf::tile_columns(p.cols) - 1) / lf::tile_columns(p.cols);

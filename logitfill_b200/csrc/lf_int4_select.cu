@@ -33,6 +33,7 @@ struct SelectParams {
 
 constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxSelectPages = 32768;  // candidates whose scores fit in shared memory
+constexpr int kMaxGroup = 64;           // query heads per KV head
 constexpr int kPagesAtOnce = 8;         // records a warp has in flight
 
 // A float's bits as an unsigned number of the same order.
@@ -80,12 +81,14 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ uint32_t key_s[];
   __shared__ __align__(16) int16_t weight_s[2 * D];
+  __shared__ __align__(16) uint16_t query_s[kMaxGroup * D];
   __shared__ float most_s[kSelectWarps];
   __shared__ uint32_t hist_s[256], sum_s[kSelectWarps], low_s[kSelectWarps], high_s[kSelectWarps], pick_s[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int h = blockIdx.x / p.cluster, i = blockIdx.y, b = blockIdx.z;
   const int slots = p.top + p.sink + p.recent;
+  grid_dep_wait();
   int32_t* picked = p.picked + ((static_cast<int64_t>(b) * p.q_len + i) * p.pool.kv_heads + h) * slots;
   const int seen = int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i);
   const int n = min(seen / kInt4Page + (seen % kInt4Page != 0), p.pool.table_width);
@@ -98,12 +101,20 @@ __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __gri
 
   if (p.cluster > 1) cluster_arrive();  // that every CTA of the cluster runs, before any stores to the first
 
-  // Weights: the group's queries in whole numbers, split by sign.
+  // Weights: the group's queries in whole numbers, split by sign.  All heads are
+  // loaded at once, eight channels a thread.
   const T* q = static_cast<const T*>(p.q) + b * p.q_seq + static_cast<int64_t>(h) * p.group * p.q_head + i * p.q_tok;
   float most = 0.0f;
-  for (int x = tid; x < p.group * D; x += kSelectThreads) {
-    const float v = fabsf(Scalar<T>::load(q + (x / D) * p.q_head + x % D));
-    most = isfinite(v) ? fmaxf(most, v) : most;
+  for (int x = tid; x < p.group * (D / 8); x += kSelectThreads) {
+    const uint4 w = *reinterpret_cast<const uint4*>(q + x / (D / 8) * p.q_head + x % (D / 8) * 8);
+    *reinterpret_cast<uint4*>(query_s + 8 * x) = w;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t pair = k < 2 ? w.x : k < 4 ? w.y : k < 6 ? w.z : w.w;
+      const uint16_t bits = static_cast<uint16_t>(k % 2 ? pair >> 16 : pair);
+      const float v = fabsf(Scalar<T>::load(reinterpret_cast<const T*>(&bits)));
+      most = v < INFINITY ? fmaxf(most, v) : most;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -111,12 +122,11 @@ __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __gri
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSelectWarps; ++w) most = fmaxf(most, most_s[w]);
-  const int f = exponent127(most);
-  const float scale = pow2(-f);
+  const float scale = pow2(-exponent127(most));
   if (tid < D) {
     int plus = 0, minus = 0;
     for (int j = 0; j < p.group; ++j) {
-      const float v = Scalar<T>::load(q + j * p.q_head + tid);
+      const float v = Scalar<T>::load(reinterpret_cast<const T*>(query_s + j * D + tid));
       const int c = isfinite(v) ? __float2int_rn(v * scale) : 0;
       plus += max(c, 0);
       minus += min(c, 0);
@@ -255,18 +265,20 @@ static int launch_select(SelectParams p, cudaStream_t stream) {
   const int64_t units = static_cast<int64_t>(p.pool.kv_heads) * p.q_len * p.pool.batch;
   p.cluster = 1;
   while (p.cluster < 8 && units * p.cluster < 148 && p.pool.table_width > p.cluster * kSelectWarps * kPagesAtOnce) p.cluster *= 2;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.pool.kv_heads * p.cluster, p.q_len, p.pool.batch);
   cfg.blockDim = dim3(kSelectThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   void* args[] = {&p};
   err = cudaLaunchKernelExC(&cfg, kern, args);
   if (err != cudaSuccess) {
@@ -288,7 +300,7 @@ extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
   LF_CHECK_ARG(a->q_len > 0 && a->q_len <= 65535 && a->n_q > 0 && a->n_q % p.pool.kv_heads == 0,
                "lf_int4_select: q_len %d, %d query heads on %d KV heads", a->q_len, a->n_q, p.pool.kv_heads);
   p.group = a->n_q / p.pool.kv_heads;
-  LF_CHECK_SUPPORTED(p.group <= 64, "lf_int4_select: %d query heads per KV head (64 at most)", p.group);
+  LF_CHECK_SUPPORTED(p.group <= lf::kMaxGroup, "lf_int4_select: %d query heads per KV head (%d at most)", p.group, lf::kMaxGroup);
   LF_CHECK_ARG(a->sink_pages >= 0 && a->recent_pages >= 1 && a->slots <= (1 << 24) &&
                    static_cast<int64_t>(a->sink_pages) + a->recent_pages <= a->slots,
                "lf_int4_select: sink %d, recent %d of %d pages (recent at least 1)", a->sink_pages, a->recent_pages,
@@ -297,6 +309,8 @@ extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
                "lf_int4_select: bounds records overlap");
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->bounds) & 7) == 0 && (a->bounds_page_stride | a->bounds_head_stride) % 8 == 0,
                "lf_int4_select: bounds records must be 8-byte aligned");
+  LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->q) & 15) == 0 && (a->q_seq_stride | a->q_head_stride | a->q_tok_stride) % 8 == 0,
+               "lf_int4_select: query rows must be 16-byte aligned");
   LF_CHECK_SUPPORTED(p.pool.table_width <= lf::kMaxSelectPages, "lf_int4_select: %d pages per sequence (%d at most)",
                      p.pool.table_width, lf::kMaxSelectPages);
   p.q = a->q;
