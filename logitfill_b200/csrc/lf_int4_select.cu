@@ -34,7 +34,7 @@ struct SelectParams {
 constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxSelectPages = 32768;  // candidates whose scores fit in shared memory
 constexpr int kMaxGroup = 64;           // query heads per KV head
-constexpr int kPagesAtOnce = 8;         // records a warp has in flight
+constexpr int kPagesAtOnce = 16;        // records a warp has in flight
 
 // A float's bits as an unsigned number of the same order.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -78,12 +78,12 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* warp_sum, 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads, 4) int4_select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ uint32_t key_s[];
   __shared__ __align__(16) int16_t weight_s[2 * D];
   __shared__ __align__(16) uint16_t query_s[kMaxGroup * D];
   __shared__ float most_s[kSelectWarps];
-  __shared__ uint32_t hist_s[256], sum_s[kSelectWarps], low_s[kSelectWarps], high_s[kSelectWarps], pick_s[2];
+  __shared__ uint32_t hist_s[256], sum_s[kSelectWarps], low_s[kSelectWarps], high_s[kSelectWarps], pick_s[3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = p.cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int h = blockIdx.x / p.cluster, i = blockIdx.y, b = blockIdx.z;
@@ -136,47 +136,55 @@ __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __gri
   }
   __syncthreads();
 
-  // Scores of this CTA's candidates (pages sink .. n - recent - 1, dealt warp by warp).
+  // Scores of this CTA's candidates (pages sink .. n - recent - 1): an equal run of
+  // them per warp, the ids of 32 at a time, the records of kPagesAtOnce in flight.
   constexpr int kBytes = 2 * D / 32, kPairs = kBytes / 2;  // a lane's record entries and its weight pairs
   int wt[kPairs];
 #pragma unroll
   for (int x = 0; x < kPairs; ++x) wt[x] = reinterpret_cast<const int*>(weight_s)[lane * kPairs + x];
   const int first = p.sink, count = n - p.sink - p.recent;
   if (p.cluster > 1) cluster_wait();
-  const int step = p.cluster * kSelectWarps * kPagesAtOnce;
-  for (int c0 = (rank * kSelectWarps + warp) * kPagesAtOnce; c0 < count; c0 += step) {
-    int id = -1;
-    if (lane < kPagesAtOnce && c0 + lane < count) {
+  const int run = (count + p.cluster * kSelectWarps - 1) / (p.cluster * kSelectWarps);
+  const int run_end = min(count, (rank * kSelectWarps + warp + 1) * run);
+  const int8_t* head_bounds = p.bounds + h * p.bounds_head;
+  for (int c0 = (rank * kSelectWarps + warp) * run; c0 < run_end; c0 += 32) {
+    int id = -1, e = 0, mine = 0;
+    if (c0 + lane < run_end) {
       id = int4_page_id(p.pool, b, first + c0 + lane);
       if (id < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
+      if (id >= 0) e = head_bounds[id * p.bounds_page + 2 * D];
     }
-    const int e = id < 0 ? 0 : p.bounds[id * p.bounds_page + h * p.bounds_head + 2 * D];
-    uint32_t w[kPagesAtOnce][kBytes / 4];
+    for (int x0 = 0; x0 < min(32, run_end - c0); x0 += kPagesAtOnce) {
+      uint32_t w[kPagesAtOnce][kBytes / 4];
 #pragma unroll
-    for (int x = 0; x < kPagesAtOnce; ++x) {
-      const int page = __shfl_sync(0xffffffffu, id, x);
-      const int8_t* rec = p.bounds + max(page, 0) * p.bounds_page + h * p.bounds_head;
-      if constexpr (D == 128) {
-        const uint2 y = *reinterpret_cast<const uint2*>(rec + lane * 8);
-        w[x][0] = y.x;
-        w[x][1] = y.y;
-      } else {
-        w[x][0] = *reinterpret_cast<const uint32_t*>(rec + lane * 4);
+      for (int x = 0; x < kPagesAtOnce; ++x) {
+        const int page = __shfl_sync(0xffffffffu, id, x0 + x);
+#pragma unroll
+        for (int y = 0; y < kBytes / 4; ++y) w[x][y] = 0;
+        if (page >= 0) {
+          const int8_t* rec = head_bounds + page * p.bounds_page + lane * kBytes;
+          if constexpr (D == 128) {
+            const uint2 y = *reinterpret_cast<const uint2*>(rec);
+            w[x][0] = y.x;
+            w[x][1] = y.y;
+          } else {
+            w[x][0] = *reinterpret_cast<const uint32_t*>(rec);
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kPagesAtOnce; ++x) {
+        int sum = 0;
+#pragma unroll
+        for (int y = 0; y < kBytes / 4; ++y) {
+          sum = __dp2a_lo(wt[2 * y], static_cast<int>(w[x][y]), sum);
+          sum = __dp2a_hi(wt[2 * y + 1], static_cast<int>(w[x][y]), sum);
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        mine = lane == x0 + x ? sum : mine;
       }
     }
-    int mine = 0;
-#pragma unroll
-    for (int x = 0; x < kPagesAtOnce; ++x) {
-      int sum = 0;
-#pragma unroll
-      for (int y = 0; y < kBytes / 4; ++y) {
-        sum = __dp2a_lo(wt[2 * y], static_cast<int>(w[x][y]), sum);
-        sum = __dp2a_hi(wt[2 * y + 1], static_cast<int>(w[x][y]), sum);
-      }
-      sum = __reduce_add_sync(0xffffffffu, sum);
-      mine = lane == x ? sum : mine;
-    }
-    if (lane < kPagesAtOnce && c0 + lane < count) {
+    if (c0 + lane < run_end) {
       const uint32_t key = id < 0 ? 0u : ordered(__int2float_rn(mine) * pow2(e));
       if (p.cluster > 1)
         store_first(key_s + c0 + lane, key);
@@ -192,8 +200,8 @@ __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __gri
     __syncthreads();
   }
 
-  // The top-th best key: narrow [low, high] to one key.  `want` keys of the
-  // range are still to be chosen, all above it are.
+  // The top-th best key: narrow [low, high] until all the keys in it are chosen, or
+  // one value is left.  `want` keys of the range are chosen, and all above it.
   uint32_t low = UINT32_MAX, high = 0;
   for (int c = tid; c < count; c += kSelectThreads) {
     low = min(low, key_s[c]);
@@ -227,25 +235,26 @@ __global__ void __launch_bounds__(kSelectThreads) int4_select_kernel(const __gri
     if (before < want && want <= before + mine) {
       pick_s[0] = 255 - tid;
       pick_s[1] = want - before;
+      pick_s[2] = mine;
     }
     __syncthreads();
     want = pick_s[1];
     low += pick_s[0] << shift;
     high = low + min(high - low, (1u << shift) - 1u);
-    __syncthreads();
+    if (want == pick_s[2]) break;
   }
 
-  // Every key above it, and the first `want` equal to it, in order.
+  // Every key above the range, and the first `want` in it, in order.
   const int each = (count + kSelectThreads - 1) / kSelectThreads;
   const int from = min(count, tid * each), to = min(count, from + each);
-  uint32_t found = 0;  // keys above in the low half, equal ones in the high half
-  for (int c = from; c < to; ++c) found += key_s[c] > low ? 1u : key_s[c] == low ? 0x10000u : 0u;
+  uint32_t found = 0;  // keys above in the low half, those in the range in the high half
+  for (int c = from; c < to; ++c) found += key_s[c] > high ? 1u : key_s[c] >= low ? 0x10000u : 0u;
   uint32_t total;
   uint32_t place = scan_before(found, sum_s, total);
   for (int c = from; c < to; ++c) {
-    const uint32_t k = key_s[c], equal = place >> 16;
-    if (k > low || (k == low && equal < want)) picked[p.sink + (place & 0xFFFFu) + min(equal, want)] = first + c;
-    place += k > low ? 1u : k == low ? 0x10000u : 0u;
+    const uint32_t k = key_s[c], within = place >> 16;
+    if (k > high || (k >= low && within < want)) picked[p.sink + (place & 0xFFFFu) + min(within, want)] = first + c;
+    place += k > high ? 1u : k >= low ? 0x10000u : 0u;
   }
   for (int s = tid; s < p.sink; s += kSelectThreads) picked[s] = s;
   for (int s = tid; s < p.recent; s += kSelectThreads) picked[p.sink + p.top + s] = n - p.recent + s;
@@ -260,11 +269,11 @@ static int launch_select(SelectParams p, cudaStream_t stream) {
     set_error("lf_int4_select: %s", cudaGetErrorString(err));
     return LF_ERR_CUDA;
   }
-  // More CTAs per unit while the units alone leave SMs idle and a CTA keeps a
-  // round of records for each of its warps.
+  // More CTAs per unit while the units alone leave SMs idle and every warp keeps
+  // eight records.
   const int64_t units = static_cast<int64_t>(p.pool.kv_heads) * p.q_len * p.pool.batch;
   p.cluster = 1;
-  while (p.cluster < 8 && units * p.cluster < 148 && p.pool.table_width > p.cluster * kSelectWarps * kPagesAtOnce) p.cluster *= 2;
+  while (p.cluster < 8 && units * p.cluster < 148 && p.pool.table_width > p.cluster * kSelectWarps * 8) p.cluster *= 2;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
