@@ -646,3 +646,21 @@ def test_refusals():
     refuses(ValueError, cache.truncate, 66)
     refuses(RuntimeError, cache.attend_sparse, 0, q, 1.0, 4)
     refuses(ValueError, cache.attend, 0, q[:, :2], 1.0)
+
+
+def test_example_serves_dense_sparse_and_drafts():
+    """The example's batch, decoded from the 4-bit cache and from uncompressed
+    Key and Value side by side."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "int4_decode.py"
+    spec = importlib.util.spec_from_file_location("int4_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    for kwargs in (dict(), dict(draft=3), dict(top=40), dict(top=4)):
+        apart, same, cache = example.serve([300, 1, 129, 64], steps=6, **kwargs)
+        # every Key and Value element is within half a step (1/30 of its group's range, about 4
+        # standard deviations): 8 % of an element's magnitude at most in root mean square
+        assert apart < 0.16 and same > 0.5
+        assert cache.lengths.tolist() == [n + 6 * kwargs.get("draft", 1) for n in (300, 1, 129, 64)]
