@@ -12,9 +12,11 @@
 // The queries are scaled by a power of two per column (and 1/16 for the odd
 // nibbles), so a bf16 or fp16 query enters exactly; products are summed in fp32.
 // Values: code * s + z is rounded once to fp16 (one fma on the exact code), and
-// so is p: each costs 2^-11 of a token's share p |value| at most, below the
+// so is p: each costs 2^-11 of a token's share p |value| at most, below a bf16
 // output's own rounding.  (Multiplying raw codes by p s instead would round a
-// number that may be many times p |value|.)
+// number that may be many times p |value|.)  For an fp16 output, whose rounding
+// is as fine, p enters as the sum of two fp16 numbers, at two products a tile more
+// per group: error against 64 bits 1.3 times the output rounding's instead of 1.6.
 //
 // The work is one pass over the pages with a running maximum and sum.  The
 // maximum is moved only when a score passes it by 2^8 (p <= 2^8 fits), so most
@@ -30,6 +32,7 @@
 // range is finished there; otherwise each CTA leaves a partial (maximum, sum,
 // accumulator) and the last one to arrive (an atomic ticket) merges them in the
 // order of the ranges, so results do not depend on timing.
+#include <atomic>
 #include <type_traits>
 
 #include "lf_int4.cuh"
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   using C = AttendCfg<D, NT>;
   constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
+  constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 1;  // fp16 numbers that make up a weight
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int meta_s[kWarps][kStages];  // first token of each stage's half page, -1: nothing to do
   __shared__ int last_s;
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
               for (int k = 0; k < 4; ++k) acc[nt][y][k] *= fix[k & 1];
           }
         }
-        uint32_t pb[NT][2];  // weights as the product's B operand: columns by tokens
+        uint32_t pb[NT][kTerms][2];  // weights as the product's B operand: columns by tokens
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -599,8 +603,17 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             pr[nt][k] = ex2(pr[nt][k]);
             l[nt][k & 1] += pr[nt][k];
           }
-          pb[nt][0] = transpose8x8(pack_half2(pr[nt][0], pr[nt][1]));
-          pb[nt][1] = transpose8x8(pack_half2(pr[nt][2], pr[nt][3]));
+#pragma unroll
+          for (int y = 0; y < kTerms; ++y)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t w = pack_half2(pr[nt][2 * k], pr[nt][2 * k + 1]);
+              pb[nt][y][k] = transpose8x8(w);
+              if (y + 1 < kTerms) {
+                pr[nt][2 * k] -= half_lo(w);
+                pr[nt][2 * k + 1] -= half_hi(w);
+              }
+            }
         }
 
         // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half, and their parameters.
@@ -629,8 +642,11 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][0], pb[nt][1]);
-            mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][0], pb[nt][1]);
+#pragma unroll
+            for (int y = 0; y < kTerms; ++y) {
+              mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][y][0], pb[nt][y][1]);
+              mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][y][0], pb[nt][y][1]);
+            }
           }
         }
       }
@@ -769,10 +785,14 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   }
 }
 
+// SMs of the current device (0 on error), asked once per device.
 static int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 // The partials: two records per CTA of the largest grid.

@@ -123,21 +123,22 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _on:
-    """Makes ``device`` current for a launch (nothing to do when it is)."""
+def _launch(entry: str, device, *args) -> None:
+    """Call ``entry`` of the library with ``args`` and the current stream of ``device``."""
+    fn = _entries.get(entry)
+    if fn is None:
+        fn = _entries[entry] = getattr(_lib.lib(), entry)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, entry)
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device):
-        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_entries: dict = {}
 
 
 def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor,
@@ -165,8 +166,7 @@ def int4_write(key: torch.Tensor, value: torch.Tensor, pages: torch.Tensor, page
         *pool, key.data_ptr(), value.data_ptr(), *ks, *vs, _per_sequence("start", start, B, dev),
         _per_sequence("counts", counts, B, dev), *((0, 0, 0) if bounds is None else _bounds(bounds, pages, D)),
         _status(status, dev), D, code, key.shape[2])
-    with _on(dev):
-        _lib.check(_lib.lib().lf_int4_write(args, _stream(dev)), "lf_int4_write")
+    _launch("lf_int4_write", dev, args)
 
 
 def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor, tokens: int,
@@ -180,14 +180,13 @@ def int4_read(pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor
         raise ValueError(f"cannot read {tokens} tokens")
     code = _lib.dtype_code(dtype)
     H, B = pool[-2:]
-    out = torch.empty((2, B, H, tokens, D), dtype=dtype, device=dev)
-    key, value = out[0], out[1]
+    key = torch.empty((B, H, tokens, D), dtype=dtype, device=dev)
+    value = torch.empty_like(key)
     strides = H * tokens * D, tokens * D, D
     args = _lib.INT4_TOKENS.pack(
         *pool, key.data_ptr(), value.data_ptr(), *strides, *strides, _per_sequence("start", start, B, dev),
         _per_sequence("counts", counts, B, dev), 0, 0, 0, _status(status, dev), D, code, tokens)
-    with _on(dev):
-        _lib.check(_lib.lib().lf_int4_read(args, _stream(dev)), "lf_int4_read")
+    _launch("lf_int4_read", dev, args)
     return key, value
 
 
@@ -201,10 +200,8 @@ def int4_read_bounds(bounds: torch.Tensor) -> torch.Tensor:
     n, H, width = bounds.shape
     D = (width - 16) // 2
     out = torch.empty(n, H, 2, D, dtype=torch.float32, device=bounds.device)
-    with _on(bounds.device):
-        _lib.check(_lib.lib().lf_int4_read_bounds(
-            bounds.data_ptr(), bounds.stride(0) if n > 1 else H * width, bounds.stride(1) if H > 1 else width, n, H, D,
-            out.data_ptr(), _stream(bounds.device)), "lf_int4_read_bounds")
+    _launch("lf_int4_read_bounds", bounds.device, bounds.data_ptr(), bounds.stride(0) if n > 1 else H * width,
+            bounds.stride(1) if H > 1 else width, n, H, D, out.data_ptr())
     return out
 
 
@@ -226,13 +223,14 @@ def _workspace(pool, n_q: int, q_len: int, head_dim: int, device):
     if held is not None and held[1] >= units and not capturing:
         return held[0], held[2], held[3]
     so = _lib.lib()
-    need = so.lf_int4_workspace_bytes(B, H, n_q, q_len, head_dim)
+    with torch.cuda.device(device):
+        need, clear_from = so.lf_int4_workspace_bytes(B, H, n_q, q_len, head_dim), so.lf_int4_workspace_clear_from()
     if capturing:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        ws[so.lf_int4_workspace_clear_from():].zero_()
+        ws[clear_from:].zero_()
         return ws, ws.data_ptr(), need
     units = max(units, 1 << 16)
-    need = max(need, so.lf_int4_workspace_clear_from() + 4 * units)
+    need = max(need, clear_from + 4 * units)
     ws = torch.zeros(need, dtype=torch.uint8, device=device)
     _workspaces[key] = ws, units, ws.data_ptr(), need
     return ws, ws.data_ptr(), need
@@ -289,10 +287,10 @@ def _attend(entry: str, query, pages, page_table, lengths, scaling, counts, out,
         picked_at = picked.data_ptr()
     args = _lib.INT4_QUERY.pack(
         *pool, q.data_ptr(), s0, s1, s2, *out_args, _per_sequence("lengths", lengths, B, dev),
-        _per_sequence("counts", counts, B, dev), *bounds_args, picked_at, workspace[1], workspace[2], _status(status, dev),
+        0 if counts is None else _per_sequence("counts", counts, B, dev), *bounds_args, picked_at, workspace[1],
+        workspace[2], 0 if status is None else _status(status, dev),
         scaling, D, _CODE[q.dtype], n_q, q_len, *budget)
-    with _on(dev):
-        _lib.check(getattr(_lib.lib(), entry)(args, _stream(dev)), entry)
+    _launch(entry, dev, args)
     return out, picked
 
 
