@@ -33,6 +33,7 @@
 // accumulator) and the last one to arrive (an atomic ticket) merges them in the
 // order of the ranges, so results do not depend on timing.
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "lf_int4.cuh"
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           if (issued + lane < mine_n) {
             logicals = first + team + (issued + lane) * C::kTeams;
             if constexpr (kSparse) logicals = listed[logicals];
-            if (logicals >= 0 && logicals < (seen_max + kInt4Page - 1) / kInt4Page) {
+            if (logicals >= 0 && seen_max > 0 && logicals <= (seen_max - 1) / kInt4Page) {
               ids = int4_page_id(p.pool, b, logicals);
               if (ids < 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
             }
@@ -859,6 +860,7 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
                "lf_int4_attend: q_len %d, %d query heads on %d KV heads", a->q_len, a->n_q, p.pool.kv_heads);
   const bool sparse = a->picked != nullptr;
   LF_CHECK_ARG(!sparse || a->slots > 0, "lf_int4_attend: %d slots", a->slots);
+  LF_CHECK_ARG(std::isfinite(a->scaling), "lf_int4_attend: scaling is not a finite number");
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->q) & 15) == 0 && (a->q_seq_stride | a->q_head_stride | a->q_tok_stride) % 8 == 0,
                "lf_int4_attend: query rows must be 16-byte aligned");
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&

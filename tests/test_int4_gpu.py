@@ -334,6 +334,37 @@ def test_attention_ignores_what_is_not_seen_and_spreads_what_is_nan():
     assert bool(torch.isnan(int4.int4_attention(q, pages, table, _i32([T + 1]), 0.125)).all())
 
 
+@pytest.mark.parametrize("scaling", [-0.125, 0.0, 1e-30, 5.0])
+def test_attention_scaling_of_any_sign(scaling):
+    lengths, D = [130, 500], 64
+    pages, table, _, sk, sv = _filled(4, lengths, 2, D, dtype=F16)
+    q = torch.randn(2, 4, 3, D, generator=torch.Generator().manual_seed(0)).to(F16).cuda()
+    got = int4.int4_attention(q, pages, table, _i32(lengths), scaling).double().cpu().numpy()
+    want, weight = _dense_reference(q, lengths, [3, 3], sk, sv, scaling)
+    # a score of magnitude S carries fp32 sums' error of about S 2^-20
+    S = float(np.abs(q.double().cpu().numpy()).sum(-1).max() * np.abs(sk).max() * abs(scaling))
+    assert (np.abs(got - want) <= 2.0 ** -11 * np.abs(want) + (2.0 ** -10 + S * 2.0 ** -20) * weight + 2.0 ** -24).all()
+
+
+def test_attention_draft_nan_reaches_only_the_queries_that_see_it():
+    """Drafted tokens 2 and 3 of 4 hold NaN (in Value, in Key): queries 0 and 1 stay
+    clean, the others are NaN in every channel that sees it."""
+    D, T, L = 128, 70, 4
+    for which in ("value", "key"):
+        pages, table, _, sk, sv = _filled(1, [T], 2, D)
+        q = torch.randn(1, 6, L, D, generator=torch.Generator().manual_seed(0)).to(BF16).cuda()
+        clean = int4.int4_attention(q, pages, table, _i32([T]), 0.1)
+        ok = torch.zeros(1, 2, 2, D, dtype=BF16, device="cuda")
+        bad = ok.clone()
+        bad[..., 40] = float("nan")
+        int4.int4_write(bad if which == "key" else ok, bad if which == "value" else ok, pages, table, _i32([T - 2]))
+        got = int4.int4_attention(q, pages, table, _i32([T]), 0.1)
+        assert torch.equal(got[:, :, :2], clean[:, :, :2])
+        assert bool(torch.isnan(got[:, :, 2:, 32:64]).all())
+        if which == "key":
+            assert bool(torch.isnan(got[:, :, 2:]).all())
+
+
 def test_attention_is_repeatable_and_takes_strides_and_outputs():
     lengths, D = [3000, 129], 128
     pages, table, _, sk, sv = _filled(2, lengths, 4, D)
@@ -632,6 +663,8 @@ def test_refusals():
     refuses(RuntimeError, int4.int4_attention, q.cpu(), pages, table, n, 1.0)
     refuses(ValueError, int4.int4_attention, q, pages, table, n, 1.0, out=q.float())
     refuses(ValueError, int4.int4_attention, q, pages, table, n, 1.0, status=n.float())
+    refuses(ValueError, int4.int4_attention, q, pages, table, n, float("nan"))
+    refuses(ValueError, int4.int4_attention, q, pages, table, n, 1.0, out=torch.empty(2, 4, 66, dtype=BF16, device="cuda")[..., 1:65])
     refuses(ValueError, int4.int4_select, q, pages, bounds, table, n, 4, recent_pages=0)
     refuses(ValueError, int4.int4_select, q, pages, bounds, table, n, -1)
     refuses(ValueError, int4.int4_read_bounds, pages)
