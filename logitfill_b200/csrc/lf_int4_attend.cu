@@ -57,36 +57,24 @@ struct AttendParams {
   int32_t* status;
 };
 
-constexpr int kTile = 16;  // tokens of one tensor-core step
-constexpr float kSlack = 8.0f;            // log2 a score may pass the running maximum by
+constexpr int kTile = 16;             // tokens of one tensor-core step
+constexpr int kPart = kInt4Page / 2;  // tokens of a page that one warp takes
+constexpr int kSubs = kPart / kTile;
+constexpr float kSlack = 8.0f;        // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
-#ifndef LF_MINP
-#define LF_MINP 4
-#define LF_COST 6
-#endif
-#ifndef LF_MERGE
-#define LF_MERGE 0.33f
-#endif
-constexpr int kMinPages = LF_MINP;  // places of a range at least: one page for each pair of warps
-constexpr int kUnitCost = LF_COST;
-#ifndef LF_UNROLL
-#define LF_UNROLL 2
-#endif
-constexpr int kUnroll = LF_UNROLL;
+constexpr int kMinPages = 4;          // places of a range at least: two pages for each pair of warps
+constexpr int kUnitCost = 6;          // empty places before a unit's pages
 
-// CTAs of four warps; as many per SM as the registers hold (168 a thread, or 255
-// with 16 columns at D 128), and the stages that 227 KB of shared memory hold.
-// Three or two CTAs hide each other's start and merge.
-#ifndef LF_PART
-#define LF_PART 32
-#define LF_CTAS 3
-#define LF_ST 3
-#endif
+// CTAs of four warps, three an SM (168 registers a thread), or two with 16 columns
+// at D 128 (255), which hide each other's start and merge; the stages are what 227
+// KB of shared memory hold.  Measured at 8 x 32k tokens, 28 heads on 4: one CTA of
+// 12 warps 53.8 us (starts and merges lie bare), three of 4 warps 48.7 us; four
+// CTAs with two stages 55.5 us (too few bytes in flight); 16 tokens a warp instead
+// of 32 52.0 us (a page's fixed work twice as often).
 template <int D, int NT> struct AttendCfg {
-  static constexpr int kPart = LF_PART, kShare = kInt4Page / kPart;  // tokens of a page that a warp takes, warps that share it
-  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kTeams = kWarps / kShare;
-  static constexpr int kCtas = D == 128 && NT == 2 ? 2 : LF_CTAS;
-  static constexpr int kStages = kCtas == 2 ? 5 : (D == 64 ? 2 : 1) * LF_ST;
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kTeams = kWarps / 2;
+  static constexpr int kCtas = D == 128 && NT == 2 ? 2 : 3;
+  static constexpr int kStages = D == 64 ? 6 : kCtas == 2 ? 5 : 3;
   static constexpr int kCodes = kPart * D / 2, kPar = kPart * D / 8;  // bytes of a warp's part, Key or Value
   static constexpr int kStageBytes = 2 * (kCodes + kPar);
   static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
@@ -209,7 +197,7 @@ __device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
 // a unit in ranges of r, r pages take 0.3 r us and the last to arrive another 0.1 us
 // for each of n / r parts, least at r = sqrt(n / 3).
 __device__ __forceinline__ int merge_pages(int total, int units) {
-  return static_cast<int>(sqrtf(static_cast<float>(total / units) * LF_MERGE));
+  return static_cast<int>(sqrtf(static_cast<float>(total / units) / 3.0f));
 }
 
 template <typename T, int D, int NT, bool kSparse>
@@ -220,7 +208,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
   constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 1;  // fp16 numbers that make up a weight
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int meta_s[kWarps][kStages];  // first token of each stage's half page, -1: nothing to do
+  __shared__ int meta_s[kWarps][kStages];  // first token of each stage's part of a page, -1: nothing to do
   __shared__ int last_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = p.pool.kv_heads * p.col_tiles;
@@ -257,7 +245,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
   uint8_t* ring = smem + warp * kStages * C::kStageBytes;
   const uint32_t ring_a = smem_addr(ring) + lane * 16;
-  const int team = warp / C::kShare, part = warp % C::kShare;
+  const int team = warp >> 1, part = warp & 1;
   // Byte offsets in a record of this lane's pieces: Key codes (Value codes 40 D
   // later), and parameters, the first half of the lanes Key's, the others Value's.
   constexpr int kParLanes = kPar / 16;  // lanes' worth of a half page's Key parameters
@@ -319,7 +307,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         }
         const int id = __shfl_sync(0xffffffffu, ids, issued & 31);
         const int logical = __shfl_sync(0xffffffffu, logicals, issued & 31);
-        if (lane == 0) meta_s[warp][into] = id < 0 ? -1 : logical * kInt4Page + part * C::kPart;
+        if (lane == 0) meta_s[warp][into] = id < 0 ? -1 : logical * kInt4Page + part * kPart;
         if (id >= 0) {
           const uint8_t* rec = head_words + id * p.pool.page_stride * 4;
           const uint32_t dst = ring_a + into * C::kStageBytes;
@@ -334,8 +322,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             cp_async16(dst + 2 * kCodes + 512, rec + 72 * D + part * kPar + lane * 16);
           } else {
             const int v = lane / kParLanes;
-            if (kParLanes == 16 || lane < 2 * kParLanes)
-              cp_async16(dst + 2 * kCodes, rec + 32 * D + v * 40 * D + part * kPar + (lane - v * kParLanes) * 16);
+            cp_async16(dst + 2 * kCodes, rec + 32 * D + v * 40 * D + part * kPar + (lane - v * kParLanes) * 16);
           }
         }
         ++issued;
@@ -440,21 +427,19 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       uint8_t* stage = ring + st * C::kStageBytes;
       st = st + 1 == kStages ? 0 : st + 1;
       if (base < 0 || base >= seen_max) continue;
-      const bool masked = base + C::kPart > vis_min;  // tokens here that not every column sees
+      const bool masked = base + kPart > vis_min;  // tokens here that not every column sees
 
       // Value parameters in pairs of tokens, as the fragments take them: in place
       // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
       {
-        // lanes per pair of tokens (16 or 8 pairs), and the groups of a lane
-        constexpr int kLanes = C::kPart == 32 ? 2 : kG, kQ = kG / kLanes;
-        const int x = lane / kLanes, q = lane % kLanes;
-        const bool busy = x < C::kPart / 2;
+        constexpr int kQ = kG / 2;  // groups of a lane: two lanes for each of the 16 pairs
+        const int x = lane >> 1, q = lane & 1;
         uint32_t* par = reinterpret_cast<uint32_t*>(stage + 2 * kCodes + kPar);
         uint32_t e[kQ], o[kQ];
 #pragma unroll
         for (int k = 0; k < kQ; ++k) {
-          e[k] = busy ? par[2 * x * kG + q * kQ + k] : 0;
-          o[k] = busy ? par[(2 * x + 1) * kG + q * kQ + k] : 0;
+          e[k] = par[2 * x * kG + q * kQ + k];
+          o[k] = par[(2 * x + 1) * kG + q * kQ + k];
         }
         if (masked) {
           // What an unwritten slot holds must not be read; a NaN that only some
@@ -496,19 +481,17 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         __syncwarp();  // every lane has read its words
         if constexpr (kQ == 2)
           *reinterpret_cast<uint4*>(par + 4 * lane) = make_uint4(s2[0], z2[0], s2[1], z2[1]);
-        else if (busy)
+        else
           *reinterpret_cast<uint2*>(par + 2 * lane) = make_uint2(s2[0], z2[0]);
         __syncwarp();
       }
 
-#pragma unroll kUnroll
-      for (int sub = 0; sub < C::kPart / kTile; ++sub) {
+      // Scores of the part's tokens, 16 at a time (rows g and g + 8 of the fragment).
+      float x[kSubs][NT][4];
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
         const uint8_t* kcode = stage + sub * (kTile * D / 2);
-        const uint8_t* vcode = kcode + kCodes;
         const uint8_t* kpar = stage + 2 * kCodes + sub * (kTile * D / 8);
-        const uint8_t* vpair = kpar + kPar;
-
-        // Scores of 16 tokens (rows g and g + 8 of the fragment).
         uint32_t kw[2][kG], ks[2][kG], kz[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -517,10 +500,10 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           kz[r] = t < kG ? *reinterpret_cast<const uint32_t*>(kpar + (8 * r + g) * (4 * kG) + t * 4) : 0u;
           kz[r] = __byte_perm(kz[r], 0, 0x3232);
         }
-        float x[NT][4], dot[NT][4];
+        float dot[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma1688_zero(x[nt], kz[0], kz[1], qz[nt]);
+          mma1688_zero(x[sub][nt], kz[0], kz[1], qz[nt]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) dot[nt][k] = 0.0f;
         }
@@ -544,80 +527,85 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[nt][k] = fmaf(dot[nt][k], 16384.0f, x[nt][k]);
-        if (masked) {
+          for (int k = 0; k < 4; ++k) x[sub][nt][k] = fmaf(dot[nt][k], 16384.0f, x[sub][nt][k]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int tok = base + sub * kTile + 8 * r + g;
-            bool nan = false;
-            if (tok >= vis_min && tok < seen_max) {
-              // the Value pairs hold 0 for a NaN by now: look at the record
-              nan = value_has_nan<kG>(p, h, b, tok);
-            }
+            // the Value pairs hold 0 for a NaN by now: look at the record
+            const bool nan = tok >= vis_min && tok < seen_max && value_has_nan<kG>(p, h, b, tok);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                if (nan) x[nt][2 * r + k] = NAN;
-                if (tok >= vis[nt][k]) x[nt][2 * r + k] = -INFINITY;
+                if (nan) x[sub][nt][2 * r + k] = NAN;
+                if (tok >= vis[nt][k]) x[sub][nt][2 * r + k] = -INFINITY;
               }
           }
-        }
+      }
 
-        // Distances from the running maxima, moved where one passes the slack.
-        float pr[NT][4];
-        bool move = false;
+      // The running maxima, moved where a score passes one by more than the slack.
+      bool move = false;
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pr[nt][k] = fmaf(x[nt][k], c2[nt][k & 1], -m[nt][k & 1]);
-            move |= pr[nt][k] > kSlack;
+          for (int k = 0; k < 4; ++k) move |= fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]) > kSlack;
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float fix[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
+#pragma unroll
+            for (int sub = 1; sub < kSubs; ++sub) top = fmaxf(top, fmaxf(x[sub][nt][k], x[sub][nt][k + 2]));
+            top *= c2[nt][k];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m[nt][k]);
+            fix[k] = ex2(m[nt][k] - top);
+            m[nt][k] = top;
+            l[nt][k] *= fix[k];
           }
-        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float fix[2];
+          for (int y = 0; y < 2 * kG; ++y)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float top = fmaxf(x[nt][k], x[nt][k + 2]) * c2[nt][k];
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              top = fmaxf(top, m[nt][k]);
-              fix[k] = ex2(m[nt][k] - top);
-              m[nt][k] = top;
-              l[nt][k] *= fix[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) pr[nt][k] = fmaf(x[nt][k], c2[nt][k & 1], -m[nt][k & 1]);
-#pragma unroll
-            for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) acc[nt][y][k] *= fix[k & 1];
-          }
+            for (int k = 0; k < 4; ++k) acc[nt][y][k] *= fix[k & 1];
         }
+      }
+
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
         uint32_t pb[NT][kTerms][2];  // weights as the product's B operand: columns by tokens
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float pr[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            pr[nt][k] = ex2(pr[nt][k]);
-            l[nt][k & 1] += pr[nt][k];
+            pr[k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
+            l[nt][k & 1] += pr[k];
           }
 #pragma unroll
           for (int y = 0; y < kTerms; ++y)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const uint32_t w = pack_half2(pr[nt][2 * k], pr[nt][2 * k + 1]);
+              const uint32_t w = pack_half2(pr[2 * k], pr[2 * k + 1]);
               pb[nt][y][k] = transpose8x8(w);
               if (y + 1 < kTerms) {
-                pr[nt][2 * k] -= half_lo(w);
-                pr[nt][2 * k + 1] -= half_hi(w);
+                pr[2 * k] -= half_lo(w);
+                pr[2 * k + 1] -= half_hi(w);
               }
             }
         }
 
         // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half, and their parameters.
+        const uint8_t* vcode = stage + kCodes + sub * (kTile * D / 2);
+        const uint8_t* vpair = stage + 2 * kCodes + kPar + sub * (kTile * D / 8);
         uint32_t vw[2][kG], sz[2][2 * kG];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -828,6 +816,9 @@ static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
   }
   return launch_status("lf_int4_attend");
 }
+// 16 columns a unit where a unit has more than 8: the codes are then unpacked once
+// for both halves.  Measured at 8 x 16k tokens, D 128: 7 columns 27.9 us in tiles of
+// 8, 35.7 in one of 16 (fewer warps fit); 16 columns 41.3 us in two tiles, 35.9 in one.
 template <typename T, int D>
 static int launch_attend_by(const AttendParams& p, int sms, cudaStream_t stream) {
   if (p.cols <= 8)
