@@ -6,22 +6,15 @@ is no fallback: if it is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes
-import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblogitfill_b200.so"
+BINDING_PATH = LIB_PATH.with_name("int4_binding.so")
 
 (LF_OK, LF_ERR_INVALID_ARGUMENT, LF_ERR_UNSUPPORTED, LF_ERR_LAUNCH, LF_ERR_DEVICE_TIMEOUT, LF_ERR_OUT_OF_RANGE,
  LF_ERR_CUDA) = range(7)
 LF_F32, LF_F16, LF_BF16 = 0, 1, 2
-
-# The argument structs of the 4-bit cache, packed by the caller into one bytes
-# object: a call has 20 to 35 fields, and converting them one by one would cost
-# more than the launch.  Field order as in the header.
-_POOL = "PPqqqiiii"
-INT4_TOKENS = struct.Struct("@" + _POOL + "PP6qPPPqqPiii0q")
-INT4_QUERY = struct.Struct("@" + _POOL + "P3qP3qPPPqqPPNPf7i")
 
 EXPORTS = (
     "lf_layout_init", "lf_pack_pages", "lf_dequantize", "lf_decode_workspace_bytes",
@@ -59,7 +52,7 @@ def lib() -> ctypes.CDLL:
             f"logitfill_b200 native library missing at {LIB_PATH}; build it with "
             "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
     so = ctypes.CDLL(str(LIB_PATH))
-    P, L, Q = c_void_p, POINTER(LfLayout), c_char_p  # Q: an argument struct, packed
+    P, L, Q = c_void_p, POINTER(LfLayout), c_char_p  # Q: an argument struct's bytes
     sig = {
         "lf_layout_init": (c_int, [L, c_int, c_int, c_int, c_int, c_int, c_int, P, c_int64, c_int64]),
         "lf_pack_pages": (c_int, [L, P, P, c_int, c_int64, c_int64, c_int64, P, c_int, c_int, P, P, P, P, P]),
@@ -111,6 +104,30 @@ def lib() -> ctypes.CDLL:
         fn.argtypes = args
     _LIB = so
     return so
+
+
+_BINDING = None
+
+
+def int4_binding():
+    """Load the 4-bit cache's compiled binding once; raise if it has not been
+    built."""
+    global _BINDING
+    if _BINDING is None:
+        lib()
+        if not BINDING_PATH.exists():
+            raise RuntimeError(
+                f"logitfill_b200 binding missing at {BINDING_PATH}; build it with "
+                "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries are the binding's)
+
+        spec = importlib.util.spec_from_file_location("int4_binding", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _BINDING = module
+    return _BINDING
 
 
 def check(status: int, what: str) -> None:

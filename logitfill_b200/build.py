@@ -4,7 +4,8 @@
 
 nvcc cross-compiles for B200 without a GPU.  The shared library links the
 CUDA runtime statically and exports only the ``lf_*`` symbols declared in
-``include/logitfill_b200.h``.
+``include/logitfill_b200.h``.  The compiled Python binding of the 4-bit cache
+(``csrc/int4_binding.cpp``, against the installed torch) lies next to it.
 """
 from __future__ import annotations
 
@@ -19,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB_NAME = "liblogitfill_b200.so"
+BINDING_NAME = "int4_binding.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -33,7 +35,42 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
+def build_binding(verbose: bool = False, force: bool = False) -> Path:
+    """g++ of the 4-bit cache's Python binding, linked to torch and the library."""
+    src, out, lib = CSRC / "int4_binding.cpp", OUT_DIR / BINDING_NAME, OUT_DIR / LIB_NAME
+    deps = (src, ROOT / "include" / "logitfill_b200.h", Path(__file__))
+    if not force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
+        return out
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    tmp = out.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(ROOT / "include"),
+           "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda), "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp),
+           str(lib), "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if done.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{done.stdout}")
+    os.replace(tmp, out)
+    return out
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
+    """Build the library and the binding; returns the library's path."""
+    out = build_library(verbose, force)
+    build_binding(verbose, force)
+    return out
+
+
+def build_library(verbose: bool = False, force: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     out = OUT_DIR / LIB_NAME
     srcs = sources()
@@ -63,7 +100,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     if failed:
         raise RuntimeError("nvcc failed:\n" + "\n".join(failed))
     tmp = out.with_suffix(".so.tmp")
-    link = [nvcc(), *ARCH, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static"]
+    link = [nvcc(), *ARCH, "-shared", "-o", str(tmp), "-Xlinker", f"-soname={LIB_NAME}", *map(str, objs), "-cudart", "static"]
     if verbose:
         print(" ".join(link), flush=True)
     subprocess.run(link, check=True)

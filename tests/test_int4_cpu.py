@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -15,6 +16,12 @@ from tests import int4_reference as ref
 
 HEADER = (Path(__file__).resolve().parents[1] / "include" / "logitfill_b200.h").read_text()
 SIZES = {"void*": 8, "int32_t*": 8, "int8_t*": 8, "int64_t": 8, "size_t": 8, "int32_t": 4, "float": 4, "lf_int4_pool": 56}
+
+
+# The argument structs, field by field; checked against the header below.
+POOL = "PPqqqiiii"
+TOKENS = struct.Struct("@" + POOL + "PP6qPPPqqPiii0q")
+QUERY = struct.Struct("@" + POOL + "P3qP3qPPPqqPPNPf7i")
 
 
 def _fields(name):
@@ -39,13 +46,14 @@ def _size(name):
 
 
 def test_packed_structs_follow_the_header():
-    pool = "PPqqqiiii"
+    pool = POOL
     code = {"void*": "P", "int32_t*": "P", "int8_t*": "P", "int64_t": "q", "size_t": "N", "int32_t": "i", "float": "f",
             "lf_int4_pool": pool}
     assert "".join(code[k] for k, _ in _fields("lf_int4_pool")) == pool and _size("lf_int4_pool") == 56
-    for name, packed in (("lf_int4_tokens", _lib.INT4_TOKENS), ("lf_int4_query", _lib.INT4_QUERY)):
+    for name, packed in (("lf_int4_tokens", TOKENS), ("lf_int4_query", QUERY)):
         want = "".join(code[k] for k, _ in _fields(name))
-        spelled = re.sub(r"(\d+)([a-zA-Z])", lambda m: int(m.group(1)) * m.group(2), packed.format.lstrip("@"))
+        spelled = re.sub(r"(\d+)([a-zA-Z])", lambda m: int(m.group(1)) * m.group(2),
+                         packed.format.lstrip("@"))
         assert spelled == want, name
         assert packed.size == _size(name)
 
@@ -58,7 +66,7 @@ def _tokens(**over):
     f.update(over)
     s = f.pop("strides")
     v = list(f.values())
-    return _lib.INT4_TOKENS.pack(*v[:11], *s, *v[11:])
+    return TOKENS.pack(*v[:11], *s, *v[11:])
 
 
 def _query(**over):
@@ -71,7 +79,7 @@ def _query(**over):
     flat = []
     for v in f.values():
         flat += list(v) if isinstance(v, tuple) else [v]
-    return _lib.INT4_QUERY.pack(*flat)
+    return QUERY.pack(*flat)
 
 
 def test_entry_points_validate_before_launch():
