@@ -47,17 +47,20 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
   *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// Smallest and largest of a lane's eight channels, as (min, -max) in one word for
-// 16-bit types, joined over the four lanes of a group; NaN where one is NaN.
-template <typename T> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
-template <> __device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b) {
+// Smaller (larger) half of each pair, NaN where one is NaN.
+template <typename T, bool kMax> __device__ __forceinline__ uint32_t pick2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-template <> __device__ __forceinline__ uint32_t min2<__nv_bfloat16>(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  if constexpr (std::is_same<T, __half>::value) {
+    if constexpr (kMax)
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    if constexpr (kMax)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
   return r;
 }
 template <typename T> struct Chunk {  // eight 16-bit channels
@@ -79,12 +82,12 @@ template <typename T> struct Chunk {  // eight 16-bit channels
     }
   }
   __device__ __forceinline__ void extremes(float& lo, float& hi) const {
-    const uint32_t a = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3]));
-    constexpr uint32_t kSign = 0x80008000u;
-    const uint32_t b = min2<T>(min2<T>(w[0] ^ kSign, w[1] ^ kSign), min2<T>(w[2] ^ kSign, w[3] ^ kSign));
-    uint32_t both = min2<T>(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+    const uint32_t a = pick2<T, false>(pick2<T, false>(w[0], w[1]), pick2<T, false>(w[2], w[3]));
+    const uint32_t b = pick2<T, true>(pick2<T, true>(w[0], w[1]), pick2<T, true>(w[2], w[3])) ^ 0x80008000u;
+    // (min, -max) in one word: one shuffle joins both over the group's four lanes
+    uint32_t both = pick2<T, false>(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) both = min2<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+    for (int o = 1; o < 4; o <<= 1) both = pick2<T, false>(both, __shfl_xor_sync(0xffffffffu, both, o));
     if constexpr (std::is_same<T, __half>::value) {
       lo = half_lo(both);
       hi = -half_hi(both);
@@ -121,7 +124,9 @@ template <> struct Chunk<float> {
 };
 
 // A group's parameters from its extremes: the stored word, z and r / 16 (0 for a
-// group that is not stored).
+// group that is not stored; negative where the largest channel's code would be 16:
+// codes grow with x, so no other group needs the clamp to 15.  It takes a |min| of
+// a thousand steps or more, whose fp16 rounding then shows in x - z).
 struct GroupParams {
   uint32_t word;
   float z, r16;
@@ -137,30 +142,30 @@ __device__ __forceinline__ GroupParams group_params(float lo, float hi) {
   // r / 16: a power of two less, so the product with it is the definition's over
   // 16 and its saturation to [0, 1] clamps the code to 0 .. 16 for free
   g.r16 = s > 0.0f && !bad ? __frcp_rn(s) * 0.0625f : 0.0f;
+  if (__fmul_rn(__fsub_rn(hi, g.z), g.r16) >= 15.5f / 16.0f) g.r16 = -g.r16;
   return g;
 }
 
 // Codes (eight nibbles) of a lane's eight channels.  16 y + 1.5 * 2^23 rounds to a
 // whole number, half to even, in the low bits of the sum; the magic numbers,
-// shifted as the codes are, come off at the end.  Code 16 needs |min| of a
-// thousand steps or more (its fp16 rounding then shows in x - z), so the clamp to
-// 15 is a branch.
+// shifted as the codes are, come off at the end.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const Chunk<T>& chunk, const GroupParams& g) {
   float x[8];
   chunk.unpack(x);
+  const float r16 = fabsf(g.r16);
   uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(-g.z, -g.z));
     float2 y;
-    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.x) : "f"(d.x), "f"(g.r16));
-    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.y) : "f"(d.y), "f"(g.r16));
+    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.x) : "f"(d.x), "f"(r16));
+    asm("mul.rn.sat.f32 %0, %1, %2;" : "=f"(y.y) : "f"(d.y), "f"(r16));
     const float2 m = __ffma2_rn(y, make_float2(16.0f, 16.0f), make_float2(12582912.0f, 12582912.0f));
     c[i] = __float_as_uint(m.x);
     c[i + 1] = __float_as_uint(m.y);
   }
-  if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) & 16u) {
+  if (g.r16 < 0.0f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = min(c[i], kMagicBits + 15u);
   }
@@ -238,13 +243,14 @@ __device__ void write_bounds(const uint32_t* rec, int8_t* out) {
     low[i] = INFINITY;
   }
 #pragma unroll
-  for (int k = part * kTok; k < (part + 1) * kTok; k += 2) {
+  for (int i = 0; i < kTok; i += 2) {
     float v[2][8];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint32_t p = rec[8 * D + (k + x) * (D / 32) + G];
+      const int k = part + (i + x) * kParts;
+      uint32_t p = rec[8 * D + k * (D / 32) + G];
       if ((p & 0x7C00u) == 0x7C00u) p = 0;  // a group that holds no numbers counts as zeros
-      values8(rec[(k + x) * kCols + col] & (p == 0 ? 0u : ~0u), half_lo(p), half_hi(p), v[x]);
+      values8(rec[k * kCols + col] & (p == 0 ? 0u : ~0u), half_lo(p), half_hi(p), v[x]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

@@ -160,6 +160,22 @@ def test_special_values():
     assert nan.sum() == 4 and nan[4, 0] and nan[5, 1] and nan[6, 2] and nan[10, 3]
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_groups_of_nearly_equal_values(dtype):
+    """Ranges of a few fp16 roundings of the minimum: x - z is then far from x - min,
+    codes pass 15 before the clamp and fall below 0."""
+    D, T = 64, 128
+    g = torch.Generator().manual_seed(0)
+    base = torch.rand(T, 2, generator=g).repeat_interleave(32, 1) * 200 - 100
+    x = (base + torch.rand(T, D, generator=g) * torch.logspace(-4, 0.5, T).view(T, 1)).to(dtype).view(1, 1, T, D).cuda()
+    table, n = _table(0, 1, 2)
+    pages, bounds = _garbage(n, 1, D), int4.alloc_bounds(n, 1, D)
+    int4.int4_write(x, -x, pages, table, _i32([0]), bounds=bounds)
+    k, v = int4.int4_read(pages, table, _i32([0]), T)
+    assert np.array_equal(k.cpu().numpy(), ref.stored(x.double().cpu().numpy()))
+    assert np.array_equal(v.cpu().numpy(), ref.stored(-x.double().cpu().numpy()))
+
+
 def test_bounds_of_pages_with_nan_and_zeros():
     D, H = 64, 1
     k = torch.randn(1, H, 128, D, generator=torch.Generator().manual_seed(3)).cuda()
