@@ -80,8 +80,10 @@ template <int D, int NT> struct AttendCfg {
   static constexpr int kPad = D + 4;  // floats between the columns of a merge buffer
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kMerge = kWarps * 8 * NT * (kPad + 2) * 4;
-  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
   static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial: maxima, sums, accumulators
+  static constexpr int kRoom = kMerge > 64 * kRecord ? kMerge : 64 * kRecord;  // 16 partials at least
+  static constexpr int kSmem = kRing > kRoom ? kRing : kRoom;
+  static constexpr int kFit = kSmem / (4 * kRecord);  // partials that are merged at once
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -171,6 +173,13 @@ __device__ __noinline__ bool value_has_nan(const AttendParams& p, int h, int b, 
   return nan;
 }
 
+// Adds 1 and returns what was there.  What the CTA wrote before the barrier ahead
+// of it is visible to whoever takes a later ticket.
+__device__ __forceinline__ uint32_t take_ticket(uint32_t* ticket) {
+  uint32_t n;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(ticket) : "memory");
+  return n;
+}
 __device__ __forceinline__ void add_scaled(float4& v, float f, float4 y) {
   v.x = fmaf(f, y.x, v.x);
   v.y = fmaf(f, y.y, v.y);
@@ -713,16 +722,15 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     if (!whole) {
       __syncthreads();
       if (tid == 0) {
-        __threadfence();  // the CTA's partial, ordered before by the barrier, is visible before its ticket
         uint32_t* ticket = p.tickets + static_cast<int64_t>(row_now) * per_row + unit_in_row;
-        const uint32_t n = atomicAdd(ticket, 1u) + 1;
+        const uint32_t n = take_ticket(ticket) + 1;
         if (n == static_cast<uint32_t>(parts)) *ticket = 0;  // every range has arrived: ready for the next call
-        __threadfence();
         last_s = n == static_cast<uint32_t>(parts);
       }
       __syncthreads();
       if (last_s) {
-        constexpr int kAtOnce = NT == 1 ? 8 : 4;  // parts whose loads are in flight together, for every item
+        // The parts, as many as shared memory holds, in one round of copies: 14 parts
+        // take 4 us from the ticket to the end in two rounds through registers, 2.8 so.
         float top[kItems], sum[kItems];
         float4 v[kItems];
 #pragma unroll
@@ -731,37 +739,41 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           sum[it] = 0.0f;
           v[it] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        for (int x0 = 0; x0 < parts; x0 += kAtOnce) {
-          float tops[kItems][kAtOnce], sums[kItems][kAtOnce];
-          float4 y[kItems][kAtOnce];
+        for (int x0 = 0; x0 < parts; x0 += C::kFit) {
+          const int n = min(C::kFit, parts - x0);
+          for (int x = 0; x < n; ++x) {
+            const float* rec = record(first_cta + x0 + x);
+            for (int c = tid * 4; c < C::kRecord; c += C::kThreads * 4) cp_async16(smem_addr(merge + x * C::kRecord + c), rec + c);
+          }
+          cp_commit();
+          cp_wait<0>();
+          __syncthreads();
+          float now[kItems];
 #pragma unroll
-          for (int x = 0; x < kAtOnce; ++x) {
-            const float* rec = record(first_cta + min(x0 + x, parts - 1));
+          for (int it = 0; it < kItems; ++it) now[it] = top[it];
+#pragma unroll 4
+          for (int x = 0; x < n; ++x)
+#pragma unroll
+            for (int it = 0; it < kItems; ++it)
+              now[it] = fmaxf(now[it], merge[x * C::kRecord + (tid + it * C::kThreads) / (D / 4)]);
+#pragma unroll
+          for (int it = 0; it < kItems; ++it) {
+            const float fix = ex2(top[it] - now[it]);
+            top[it] = now[it];
+            sum[it] *= fix;
+            v[it] = make_float4(v[it].x * fix, v[it].y * fix, v[it].z * fix, v[it].w * fix);
+          }
+#pragma unroll 4
+          for (int x = 0; x < n; ++x)
 #pragma unroll
             for (int it = 0; it < kItems; ++it) {
               const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
-              tops[it][x] = __ldcg(rec + col);
-              sums[it][x] = __ldcg(rec + kCol + col);
-              y[it][x] = __ldcg(reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
+              const float* rec = merge + x * C::kRecord;
+              const float f = ex2(rec[col] - now[it]);
+              sum[it] = fmaf(f, rec[kCol + col], sum[it]);
+              add_scaled(v[it], f, *reinterpret_cast<const float4*>(rec + 2 * kCol + col * D + d));
             }
-          }
-#pragma unroll
-          for (int it = 0; it < kItems; ++it) {
-            float now = top[it];
-#pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) now = fmaxf(now, tops[it][x]);
-            const float fix = ex2(top[it] - now);
-            top[it] = now;
-            sum[it] *= fix;
-            v[it] = make_float4(v[it].x * fix, v[it].y * fix, v[it].z * fix, v[it].w * fix);
-#pragma unroll
-            for (int x = 0; x < kAtOnce; ++x)
-              if (x0 + x < parts) {
-                const float f = ex2(tops[it][x] - now);
-                sum[it] = fmaf(f, sums[it][x], sum[it]);
-                add_scaled(v[it], f, y[it][x]);
-              }
-          }
+          __syncthreads();
         }
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {

@@ -319,15 +319,16 @@ __global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __g
     return;
   }
   const int page = start / kInt4Page + blockIdx.x;
-  const int first = max(start, page * kInt4Page), last = min(start + count, (page + 1) * kInt4Page);
-  if (first >= last) return;
+  const int64_t base = static_cast<int64_t>(page) * kInt4Page;
+  if (base >= start + count) return;
+  // slots of the page to write
+  const int k0 = max(static_cast<int>(start - base), 0), k1 = static_cast<int>(min(start + count - base, int64_t{kInt4Page}));
   const int id = int4_page_id(p.pool, b, page);
   if (id < 0) {
     if (tid == 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_OUT_OF_RANGE);
     return;
   }
   uint32_t* rec = reinterpret_cast<uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
-  const int k0 = first - page * kInt4Page, k1 = last - page * kInt4Page;  // slots of the page to write
   const bool whole = p.bounds != nullptr && k1 == kInt4Page;
   if (whole) {  // the slots written before, for the bounds
     for (int x = tid; x < k0 * (D / 8); x += kWriteThreads) rec_s[x] = __ldcg(rec + x);
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __g
 
   // Row `row` of every kRows slots: the addresses step by constants.
   const int l = tid % kLanes, row = tid / kLanes;
-  const int64_t from = page * kInt4Page - start + row;  // source token of slot `row`
+  const int64_t from = base - start + row;  // source token of slot `row`
   const T* key = static_cast<const T*>(p.key) + b * p.k_seq + h * p.k_head + from * p.k_tok + 8 * l;
   const T* value = static_cast<const T*>(p.value) + b * p.v_seq + h * p.v_head + from * p.v_tok + 8 * l;
   const int64_t k_step = p.k_tok * kRows, v_step = p.v_tok * kRows;
