@@ -32,6 +32,13 @@
 // range is finished there; otherwise each CTA leaves a partial (maximum, sum,
 // accumulator) and the last one to arrive (an atomic ticket) merges them in the
 // order of the ranges, so results do not depend on timing.
+//
+// Measured at 8 sequences of 32k tokens, 28 heads on 4, D 128, bf16 (168 MB): 41.6
+// us, 4.0 TB/s, 62 % of a plain copy's rate.  Of it 3.5 us pass before the first
+// page is there (lengths, table and pages are dependent loads), 4 after the last one
+// (partial, ticket, merge).  The loop takes 26 to 33; its copies alone end at 25, so
+// the instructions bound it: 675 a warp for its 32 tokens, issue slots 58 % busy with
+// three warps a scheduler, the dequantisation of the Values a third of them.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -63,14 +70,14 @@ constexpr int kSubs = kPart / kTile;
 constexpr float kSlack = 8.0f;        // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
 constexpr int kMinPages = 4;          // places of a range at least: two pages for each pair of warps
-constexpr int kUnitCost = 6;          // empty places before a unit's pages
+constexpr int kUnitCost = 6;          // empty places before a unit's pages (at 8 x 32k 16 cost 2 us more, 40 2.4)
 
 // CTAs of four warps, three an SM (168 registers a thread), or two with 16 columns
 // at D 128 (255), which hide each other's start and merge; the stages are what 227
-// KB of shared memory hold.  Measured at 8 x 32k tokens, 28 heads on 4: one CTA of
-// 12 warps 53.8 us (starts and merges lie bare), three of 4 warps 48.7 us; four
-// CTAs with two stages 55.5 us (too few bytes in flight); 16 tokens a warp instead
-// of 32 52.0 us (a page's fixed work twice as often).
+// KB of shared memory hold.  Compared at 8 x 32k tokens, 28 heads on 4, before
+// the loop had its present form: one CTA of 12 warps 53.8 us (starts and merges lie
+// bare), three of 4 warps 48.7 us; four CTAs with two stages 55.5 us (too few bytes in
+// flight); 16 tokens a warp instead of 32 52.0 us (a page's fixed work twice as often).
 template <int D, int NT> struct AttendCfg {
   static constexpr int kWarps = 4, kThreads = 32 * kWarps, kTeams = kWarps / 2;
   static constexpr int kCtas = D == 128 && NT == 2 ? 2 : 3;
@@ -81,7 +88,8 @@ template <int D, int NT> struct AttendCfg {
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kMerge = kWarps * 8 * NT * (kPad + 2) * 4;
   static constexpr int kRecord = 8 * NT * (D + 2);  // floats of a partial: maxima, sums, accumulators
-  static constexpr int kRoom = kMerge > 64 * kRecord ? kMerge : 64 * kRecord;  // 16 partials at least
+  // 16 partials where that costs no CTA: 60 KB of ring would hold 14 (D 128)
+  static constexpr int kRoom = NT == 1 && kMerge < 64 * kRecord ? 64 * kRecord : kMerge;
   static constexpr int kSmem = kRing > kRoom ? kRing : kRoom;
   static constexpr int kFit = kSmem / (4 * kRecord);  // partials that are merged at once
 };
@@ -830,7 +838,9 @@ static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
 }
 // 16 columns a unit where a unit has more than 8: the codes are then unpacked once
 // for both halves.  Measured at 8 x 16k tokens, D 128: 7 columns 27.9 us in tiles of
-// 8, 35.7 in one of 16 (fewer warps fit); 16 columns 41.3 us in two tiles, 35.9 in one.
+// 8, 35.7 in one of 16 (fewer warps fit); 16 columns 41.3 us in two tiles, 35.9 in one
+// (now 26.4 and 34.8).  Four column tiles in one at D 64 do not pay: 25 columns of
+// drafts 28.2 us, 25.2 in two tiles of 16.
 template <typename T, int D>
 static int launch_attend_by(const AttendParams& p, int sms, cudaStream_t stream) {
   if (p.cols <= 8)

@@ -11,12 +11,18 @@
 // reads back as NaN.
 //
 // Both directions move 4 D bytes of 16-bit Key and Value and 1.25 D of record per
-// token and head, so they are bound by HBM once the arithmetic is kept small:
-// extremes of packed pairs, two of them in one shuffle; four fp32 operations and
-// two integer ones per code; codes read back as subnormal halves.  The writer
-// builds a page's record in shared memory and stores whole rows of it: the
-// record's order puts a token's Value words 64 bytes apart, and stored one by one
-// they would fill eight times as many sectors.
+// token and head, so HBM would bound them; what is left above that is arithmetic.
+// It is kept small by extremes of packed pairs, two of them in one shuffle; three
+// fp32 instructions (two of them on pairs) and one integer one per code; codes
+// read back as subnormal halves.  The writer builds a page's record in shared
+// memory and stores whole rows of it: the record's order puts a token's Value words
+// 64 bytes apart, and stored one by one they would fill eight times as many sectors
+// (66 us instead of 49).
+//
+// Measured for 16 sequences of 4096 bf16 tokens, 4 KV heads, D 128 (176 MB each
+// way): write 46.6 us (3.8 TB/s), of which loads and stores alone 32.9, parameters
+// 2.3, codes 5, bounds 6; the issue slots are 75 % busy.  Read 31.4 us (5.6 TB/s).
+// One token of 16 sequences: 2 to 3 us each, the latency of three dependent loads.
 #include <type_traits>
 
 #include "lf_int4.cuh"
@@ -303,7 +309,8 @@ __device__ __forceinline__ int token_word(int k, int x) {
   return 10 * D + (k >> 3) * D + g * kC + ((k & 7) >> 1) * kP + (k & 1) * (D / 64) + w;
 }
 
-// One CTA per (page, KV head): its tokens of the page, and the page's bounds once
+// One CTA per (page, KV head), so that a page's bounds need no second launch; ten
+// of them an SM hide each other's loads (eight and twelve measure the same).  Its tokens of the page, and the page's bounds once
 // its last slot is written.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads, 10) int4_write_kernel(const __grid_constant__ TokenParams p) {
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_c
   const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));
   T* key = static_cast<T*>(p.key) + b * p.k_seq + h * p.k_head + i0 * p.k_tok + 8 * l;
   T* value = static_cast<T*>(p.value) + b * p.v_seq + h * p.v_head + i0 * p.v_tok + 8 * l;
-  constexpr int kAtOnce = 4;  // rows whose loads are in flight together
+  constexpr int kAtOnce = 4;  // rows whose loads are in flight together (one: 38 us for the prompts above, four: 31.4)
   for (int r0 = row; r0 < last - i0; r0 += kAtOnce * kRows) {
     uint32_t kw[kAtOnce], kp[kAtOnce], vp[kAtOnce], v0[kAtOnce], v1[kAtOnce];
 #pragma unroll

@@ -288,6 +288,17 @@ def test_attention_lengths(dtype, lengths):
     _check_out(got, *_dense_reference(q, lengths, [L] * B, sk, sv, D ** -0.5), dtype)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nq", [3, 12])
+def test_attention_of_one_long_unit(D, nq):
+    # one KV head: its pages lie in more ranges than one round of the merge holds
+    lengths = [30001]
+    pages, table, _, sk, sv = _filled(D, lengths, 1, D)
+    q = torch.randn(1, nq, 1, D, generator=torch.Generator().manual_seed(nq)).to(BF16).cuda()
+    got = int4.int4_attention(q, pages, table, _i32(lengths), D ** -0.5)
+    _check_out(got, *_dense_reference(q, lengths, [1], sk, sv, D ** -0.5), BF16)
+
+
 def test_attention_long_queries_and_many_sequences():
     lengths, nq, H, D, L = [150, 77, 300], 6, 2, 64, 75
     pages, table, _, sk, sv = _filled(3, lengths, H, D)
