@@ -133,6 +133,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// c += a b on two fp32 numbers in one instruction.
+__device__ __forceinline__ void fma2(float& c0, float& c1, float a0, float a1, float b0, float b1) {
+  const float2 c = __ffma2_rn(make_float2(a0, a1), make_float2(b0, b1), make_float2(c0, c1));
+  c0 = c.x;
+  c1 = c.y;
+}
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -544,7 +550,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[sub][nt][k] = fmaf(dot[nt][k], 16384.0f, x[sub][nt][k]);
+          for (int k = 0; k < 4; k += 2) fma2(x[sub][nt][k], x[sub][nt][k + 1], dot[nt][k], dot[nt][k + 1], 16384.0f, 16384.0f);
       }
       if (masked) {
 #pragma unroll
@@ -566,22 +572,23 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
       // The running maxima, moved where a score passes one by more than the slack.
       bool move = false;
+      float most[NT][2];
 #pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int k = 0; k < 2; ++k) {
+          most[nt][k] = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) move |= fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]) > kSlack;
+          for (int sub = 1; sub < kSubs; ++sub) most[nt][k] = fmaxf(most[nt][k], fmaxf(x[sub][nt][k], x[sub][nt][k + 2]));
+          move |= fmaf(most[nt][k], c2[nt][k], -m[nt][k]) > kSlack;
+        }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float fix[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
-#pragma unroll
-            for (int sub = 1; sub < kSubs; ++sub) top = fmaxf(top, fmaxf(x[sub][nt][k], x[sub][nt][k + 2]));
-            top *= c2[nt][k];
+            float top = most[nt][k] * c2[nt][k];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(top, m[nt][k]);
@@ -603,9 +610,14 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         for (int nt = 0; nt < NT; ++nt) {
           float pr[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pr[k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
-            l[nt][k & 1] += pr[k];
+          for (int k = 0; k < 4; k += 2) {
+            float a0 = -m[nt][0], a1 = -m[nt][1];
+            fma2(a0, a1, x[sub][nt][k], x[sub][nt][k + 1], c2[nt][0], c2[nt][1]);
+            pr[k] = ex2(a0);
+            pr[k + 1] = ex2(a1);
+            const float2 sum = __fadd2_rn(make_float2(l[nt][0], l[nt][1]), make_float2(pr[k], pr[k + 1]));
+            l[nt][0] = sum.x;
+            l[nt][1] = sum.y;
           }
 #pragma unroll
           for (int y = 0; y < kTerms; ++y)
