@@ -37,8 +37,8 @@
 // us, 4.0 TB/s, 62 % of a plain copy's rate.  Of it 3.5 us pass before the first
 // page is there (lengths, table and pages are dependent loads), 4 after the last one
 // (partial, ticket, merge).  The loop takes 26 to 33; its copies alone end at 25, so
-// the instructions bound it: 675 a warp for its 32 tokens, issue slots 58 % busy with
-// three warps a scheduler, the dequantisation of the Values a third of them.
+// instructions and their latencies bound it: some 650 a warp for its 32 tokens, a third
+// of them the Values' dequantisation, issue slots 58 % busy with three warps a scheduler.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
