@@ -175,16 +175,16 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[kWor
     w[0] = x.x; w[1] = x.y;
   }
 }
-// Whether a Value group of position tok holds NaN (read from the record).
+// Value parameters of position tok in the record (its page is known to be there).
 template <int kG>
-__device__ __noinline__ bool value_has_nan(const AttendParams& p, int h, int b, int tok) {
+__device__ __forceinline__ const uint32_t* value_params(const AttendParams& p, int h, int b, int tok) {
   const int id = int4_page_id(p.pool, b, tok / kInt4Page);
-  if (id < 0) return false;
-  const uint32_t* par = reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h) + 18 * 32 * kG +
-                        tok % kInt4Page * kG;
-  bool nan = false;
-  for (int G = 0; G < kG; ++G) nan |= is_nan_param(par[G]);
-  return nan;
+  return reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h) + 18 * 32 * kG + tok % kInt4Page * kG;
+}
+// Bit i: token i of 32, where lanes 2 x and 2 x + 1 hold flags of tokens 2 x and 2 x + 1.
+__device__ __forceinline__ uint32_t token_bits(bool even, bool odd) {
+  const uint32_t e = __ballot_sync(0xffffffffu, even), o = __ballot_sync(0xffffffffu, odd);
+  return ((e | e >> 1) & 0x55555555u) | ((o | o << 1) & 0xAAAAAAAAu);
 }
 
 // Adds 1 and returns what was there.  What the CTA wrote before the barrier ahead
@@ -454,6 +454,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
       // Value parameters in pairs of tokens, as the fragments take them: in place
       // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
+      uint32_t apart = 0;  // tokens with a Value group that stays out of the product
       {
         constexpr int kQ = kG / 2;  // groups of a lane: two lanes for each of the 16 pairs
         const int x = lane >> 1, q = lane & 1;
@@ -465,14 +466,24 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           o[k] = par[(2 * x + 1) * kG + q * kQ + k];
         }
         if (masked) {
-          // What an unwritten slot holds must not be read; a NaN that only some
-          // columns see goes to their weights (below), not through the product.
+          // What an unwritten slot holds must not be read; a NaN group that only some
+          // columns see goes into their sums (below), not through the product.
           const int tok = base + 2 * x;
+          bool nan_e = false, nan_o = false;
 #pragma unroll
           for (int k = 0; k < kQ; ++k) {
-            if (tok >= seen_max || (tok >= vis_min && is_nan_param(e[k]))) e[k] = 0;
-            if (tok + 1 >= seen_max || (tok + 1 >= vis_min && is_nan_param(o[k]))) o[k] = 0;
+            if (tok >= seen_max) e[k] = 0;
+            if (tok + 1 >= seen_max) o[k] = 0;
+            if (tok >= vis_min && is_nan_param(e[k])) {
+              nan_e = true;
+              e[k] = 0;
+            }
+            if (tok + 1 >= vis_min && is_nan_param(o[k])) {
+              nan_o = true;
+              o[k] = 0;
+            }
           }
+          apart = token_bits(nan_e, nan_o);
         }
         uint32_t s2[kQ], z2[kQ], most = 0;
 #pragma unroll
@@ -558,16 +569,27 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int tok = base + sub * kTile + 8 * r + g;
-            // the Value pairs hold 0 for a NaN by now: look at the record
-            const bool nan = tok >= vis_min && tok < seen_max && value_has_nan<kG>(p, h, b, tok);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                if (nan) x[sub][nt][2 * r + k] = NAN;
+              for (int k = 0; k < 2; ++k)
                 if (tok >= vis[nt][k]) x[sub][nt][2 * r + k] = -INFINITY;
-              }
           }
+      }
+      // A NaN group among the tokens that only some columns see: NaN in its channels of
+      // the columns that do.  The pairs hold 0 for it by now: look at the record.
+      for (; apart != 0; apart &= apart - 1) {
+        const int tok = base + __ffs(apart) - 1;
+        const uint32_t* par = value_params<kG>(p, h, b, tok);
+#pragma unroll
+        for (int G = 0; G < kG; ++G) {
+          if (!is_nan_param(par[G])) continue;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (tok < vis[nt][k & 1]) acc[nt][2 * G][k] = acc[nt][2 * G + 1][k] = NAN;
+        }
       }
 
       // The running maxima, moved where a score passes one by more than the slack.

@@ -1,0 +1,70 @@
+"""GPU tests of the 4-bit cache at the edges of its values and arguments.  The
+reference and the helpers are those of :mod:`tests.test_int4_gpu`."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from logitfill_b200 import int4
+from tests import int4_reference as ref
+from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _i32
+
+pytestmark = pytest.mark.gpu
+
+
+def _queries(seed, B, nq, q_len, D, dtype=BF16):
+    return torch.randn(B, nq, q_len, D, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def _check(got, want, weight, dtype, extra=0.0):
+    """NaN where the definition has NaN, and elsewhere within ``u |out| + 2^-10 sum p |v|
+    + extra``, the bound of :mod:`tests.test_int4_gpu`."""
+    got = got.double().cpu().numpy()
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan)
+    over = np.abs(got - want) - (ROUND[dtype] * np.abs(want) + 2.0 ** -10 * weight + extra)
+    assert nan.all() or over[~nan].max() <= 0, f"outside the bound by {over[~nan].max():.3g}"
+
+
+# ------------------------------------------------------------ NaN among drafts
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,nq", [(64, 4), (64, 12), (128, 4), (128, 14)])
+def test_draft_nan_value_stays_in_its_channels(dtype, D, nq):
+    """Drafted tokens whose Value groups do not fit (a NaN; a range past 15 * 65504):
+    the queries that see one are NaN in that group's 32 channels and nowhere else, in
+    sequences with all and with some of the query tokens."""
+    lengths, L, H = [70, 97, 66, 130], 4, 2
+    pages, table, _, sk, sv = _filled(1, lengths, H, D, dtype=dtype)
+    value = torch.randn(4, H, 3, D, generator=torch.Generator().manual_seed(5))
+    value[0, :, 1, 40] = float("nan")     # the last but one token, group 1, both KV heads
+    value[1, 0, 2, 3] = float("nan")      # the last token, group 0, KV head 0
+    value[1, 1, 0, 63] = float("-inf")
+    value[2, 1, 1, 33] = 3e6
+    key = torch.randn(4, H, 3, D, generator=torch.Generator().manual_seed(6))
+    int4.int4_write(key.cuda(), value.cuda(), pages, table, _i32([n - 3 for n in lengths]))
+    rows = [np.arange(n - 3, n) for n in lengths]
+    wk, wv = ref.stored(key.double().numpy()), ref.stored(value.double().numpy())
+    for b in range(4):
+        sk[b][:, rows[b]], sv[b][:, rows[b]] = wk[b], wv[b]
+    assert np.isnan(sv).any()
+    q = _queries(2, 4, nq, L, D, dtype)
+    for counts in ([L] * 4, [3, L, 2, 1]):
+        got = int4.int4_attention(q, pages, table, _i32(lengths), D ** -0.5, counts=_i32(counts))
+        want, weight = _dense_reference(q, lengths, counts, sk, sv, D ** -0.5)
+        assert np.isnan(want).any() and np.isfinite(want).any()
+        _check(got, want, np.nan_to_num(weight), dtype, 2.0 ** -24)
+
+
+def test_sparse_over_every_page_has_the_dense_result_with_nan_drafts():
+    lengths, L, D = [70, 200], 3, 64
+    pages, table, bounds, _, _ = _filled(1, lengths, 1, D)
+    value = torch.zeros(2, 1, 2, D, device="cuda")
+    value[..., 1, 7] = float("nan")
+    int4.int4_write(torch.zeros_like(value), value, pages, table, _i32([n - 2 for n in lengths]), bounds=bounds)
+    q = _queries(0, 2, 4, L, D)
+    dense = int4.int4_attention(q, pages, table, _i32(lengths), 0.125)
+    sparse, _ = int4.int4_sparse_attention(q, pages, bounds, table, _i32(lengths), 0.125, top_pages=4)
+    assert torch.equal(torch.isnan(dense), torch.isnan(sparse))
+    assert bool(torch.isnan(dense[:, :, 2, :32]).all()) and bool(torch.isfinite(dense[..., 32:]).all())
