@@ -12,14 +12,17 @@
 // The queries are scaled by a power of two per column (and 1/16 for the odd
 // nibbles), so a bf16 or fp16 query enters exactly; products are summed in fp32.
 // Values: code * s + z is rounded once to fp16 (one fma on the exact code), and
-// so is p: each costs 2^-11 of a token's share p |value| at most, below a bf16
-// output's own rounding.  (Multiplying raw codes by p s instead would round a
-// number that may be many times p |value|.)  For an fp16 output, whose rounding
-// is as fine, p enters as the sum of two fp16 numbers, at two products a tile more
-// per group: error against 64 bits 1.3 times the output rounding's instead of 1.6.
+// so is p: each costs 2^-11 of a token's share p |value|, below a bf16 output's own
+// rounding.  (Multiplying raw codes by p s instead would round a number that may
+// be many times p |value|.)  For an fp16 output, whose rounding is as fine, p enters
+// as the sum of two fp16 numbers, at two products a tile more per group: error
+// against 64 bits 1.3 times the output rounding's instead of 1.6.  Small weights
+// keep fewer bits: fp16 ends at steps of 2^-24.  So that a dominant token does not
+// press the rest of its warp's tokens below that, the largest weight is put at 2^7
+// and not at 1: what is lost of a weight is then 2^-32 of the warp's largest at most.
 //
 // The work is one pass over the pages with a running maximum and sum.  The
-// maximum is moved only when a score passes it by 2^8 (p <= 2^8 fits), so most
+// maximum is moved only when a score passes it by 2^8 (p <= 2^15 fits), so most
 // tiles skip the rescaling.
 //
 // Split.  All pages of all units form one line, cut into equal ranges, one per
@@ -67,6 +70,7 @@ struct AttendParams {
 constexpr int kTile = 16;             // tokens of one tensor-core step
 constexpr int kPart = kInt4Page / 2;  // tokens of a page that one warp takes
 constexpr int kSubs = kPart / kTile;
+constexpr float kLift = 7.0f;         // log2 of the weight that a running maximum stands for
 constexpr float kSlack = 8.0f;        // log2 a score may pass the running maximum by
 constexpr float kNoMax = -1e30f;
 constexpr int kMinPages = 4;          // places of a range at least: two pages for each pair of warps
@@ -592,7 +596,8 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         }
       }
 
-      // The running maxima, moved where a score passes one by more than the slack.
+      // The running maxima (m lies kLift below), moved where a score passes one by more
+      // than the slack.
       bool move = false;
       float most[NT][2];
 #pragma unroll
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           most[nt][k] = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
 #pragma unroll
           for (int sub = 1; sub < kSubs; ++sub) most[nt][k] = fmaxf(most[nt][k], fmaxf(x[sub][nt][k], x[sub][nt][k + 2]));
-          move |= fmaf(most[nt][k], c2[nt][k], -m[nt][k]) > kSlack;
+          move |= fmaf(most[nt][k], c2[nt][k], -m[nt][k]) > kLift + kSlack;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -613,7 +618,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             float top = most[nt][k] * c2[nt][k];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m[nt][k]);
+            top = fmaxf(top - kLift, m[nt][k]);
             fix[k] = ex2(m[nt][k] - top);
             m[nt][k] = top;
             l[nt][k] *= fix[k];

@@ -8,7 +8,7 @@ import torch
 
 from logitfill_b200 import int4
 from tests import int4_reference as ref
-from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _i32
+from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _garbage, _i32, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,34 @@ def test_sparse_over_every_page_has_the_dense_result_with_nan_drafts():
     sparse, _ = int4.int4_sparse_attention(q, pages, bounds, table, _i32(lengths), 0.125, top_pages=4)
     assert torch.equal(torch.isnan(dense), torch.isnan(sparse))
     assert bool(torch.isnan(dense[:, :, 2, :32]).all()) and bool(torch.isfinite(dense[..., 32:]).all())
+
+
+# ---------------------------------------------------------------- small weights
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,H,nq,D", [(1, 2, 8, 128), (96, 4, 4, 64), (80, 4, 48, 128)])
+@pytest.mark.parametrize("gap", [9.0, 12.0, 15.0, 18.0])
+def test_weights_far_below_a_dominant_token(dtype, B, H, nq, D, gap):
+    """A first token with a score ``gap`` above the mean of the others' and a Value of
+    zero, so that the output is the sum of small weights; in units split over many CTAs
+    and in units that one CTA takes whole.
+
+    A weight is held in fp16 with its warp's largest at 2^7 at least: to 2^-11 of itself,
+    or to 2^-25 where it is subnormal, which is 2^-32 of the largest weight.  The
+    second is bounded by T 2^-32 max p max |v|."""
+    T = 700
+    g = torch.Generator().manual_seed(int(gap))
+    key, value = torch.randn(B, H, T, D, generator=g), 100.0 * (2.0 + torch.randn(B, H, T, D, generator=g))
+    q = torch.randn(B, nq, 1, D, generator=g)
+    key[..., 0], q[..., 0] = 0.0, 4.0
+    key[:, :, 0], value[:, :, 0] = 0.0, 0.0
+    key[:, :, 0, 0] = gap * D ** 0.5 / 4.0
+    key, value, q = key.to(dtype).cuda(), value.to(dtype).cuda(), q.to(dtype).cuda()
+    table, n = _table(3, B, 11)
+    pages = _garbage(n, H, D)
+    int4.int4_write(key, value, pages, table, _i32([0] * B))
+    sk, sv = ref.stored(key.double().cpu().numpy()), ref.stored(value.double().cpu().numpy())
+    got = int4.int4_attention(q, pages, table, _i32([T] * B), D ** -0.5)
+    some = list(range(0, B, 7))   # of a large batch, sequences enough
+    want, weight = _dense_reference(q[some], [T] * len(some), [1] * len(some), sk[some], sv[some], D ** -0.5)
+    _check(got[some], want, weight, dtype, T * 2.0 ** -32 * np.abs(sv).max())
