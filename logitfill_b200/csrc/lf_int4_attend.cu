@@ -20,6 +20,8 @@
 // keep fewer bits: fp16 ends at steps of 2^-24.  So that a dominant token does not
 // press the rest of its warp's tokens below that, the largest weight is put at 2^7
 // and not at 1: what is lost of a weight is then 2^-32 of the warp's largest at most.
+// A Value group that may pass the fp16 range stays out of the product and is added in
+// fp32, token by token.
 //
 // The work is one pass over the pages with a running maximum and sum.  The
 // maximum is moved only when a score passes it by 2^8 (p <= 2^15 fits), so most
@@ -162,6 +164,15 @@ __device__ __forceinline__ void two_codes(uint32_t x, uint32_t& even, uint32_t& 
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(even) : "r"(x), "r"(high));
 }
 __device__ __forceinline__ bool is_nan_param(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
+// Whether code * s + z may pass the fp16 range: only where s is 2^11 or |z| 2^15 at
+// least (else it is 15 * 2^11 + 2^15 = 63488 at most).
+__device__ __forceinline__ bool is_wide_param(uint32_t w) {
+  return ((w & 0x7FFFu) >= 0x6800u || (w & 0x7FFF0000u) >= 0x78000000u) && !is_nan_param(w);
+}
+// Whether a Value group of token tok (seen by some column) stays out of the product.
+__device__ __forceinline__ bool stays_apart(uint32_t w, int tok, int vis_min) {
+  return is_wide_param(w) || (tok >= vis_min && is_nan_param(w));
+}
 // Larger magnitude of each half (a NaN gives way to a number).
 __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -189,6 +200,47 @@ __device__ __forceinline__ const uint32_t* value_params(const AttendParams& p, i
 __device__ __forceinline__ uint32_t token_bits(bool even, bool odd) {
   const uint32_t e = __ballot_sync(0xffffffffu, even), o = __ballot_sync(0xffffffffu, odd);
   return ((e | e >> 1) & 0x55555555u) | ((o | o << 1) & 0xAAAAAAAAu);
+}
+
+// A warp's sums, weights (fragment order) and visible tokens, for add_apart.
+template <int D, int NT> struct Apart {
+  float acc[NT][D / 16][4], w[NT][4 * kSubs];
+  int vis[NT][2];
+};
+// Value groups that stay out of the product, added in fp32 to the columns that see
+// their token: those past the fp16 range (scaled to fit, they would cost the small
+// groups beside them their low bits), and NaN ones that only some columns see.
+// `apart` has the part's tokens with such groups.  The parameters are those of the
+// record: the pairs in shared memory hold 0 for these groups.  A call of its own on
+// copies: in the loop the registers it takes cost 1 % at D 128, 5 % with 16 columns.
+template <int D, int NT>
+__device__ __noinline__ void add_apart(const AttendParams& p, int h, int b, uint32_t apart, int base, int vis_min,
+                                       const uint32_t* codes, Apart<D, NT>& s) {
+  constexpr int kG = D / kInt4Group;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll 1
+  for (; apart != 0; apart &= apart - 1) {
+    const int k = __ffs(apart) - 1, tok = base + k;
+    const uint32_t* par = value_params<kG>(p, h, b, tok);
+    const uint32_t* words = codes + (k >> 3) * D + g * (D / 8) + ((k & 7) >> 1) * (D / 32) + (k & 1) * (D / 64);
+#pragma unroll 1
+    for (int col = 0; col < 2 * NT; ++col) {
+      const int nt = col >> 1, c = col & 1;
+      // row k & 7 of the scores' fragments holds the token
+      const float w = __shfl_sync(0xffffffffu, s.w[nt][2 * (k >> 3) + c], (k & 7) * 4 + t);
+      const bool seen = tok < s.vis[nt][c];
+#pragma unroll 1
+      for (int G = 0; G < kG; ++G) {
+        const uint32_t sz = par[G], four = words[G >> 1] >> (16 * (G & 1));
+        if (!seen || !stays_apart(sz, tok, vis_min)) continue;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {  // channel 4 g + n
+          float& a = s.acc[nt][2 * G + (n >> 1)][2 * (n & 1) + c];
+          a = fmaf(w, fmaf(static_cast<float>(four >> (4 * n) & 15u), half_lo(sz), half_hi(sz)), a);
+        }
+      }
+    }
+  }
 }
 
 // Adds 1 and returns what was there.  What the CTA wrote before the barrier ahead
@@ -430,7 +482,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
     float acc[NT][2 * kG][4], m[NT][2], l[NT][2];
-    float back = 1.0f;  // 32 once a Value past the fp16 range may have been met
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -458,7 +509,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
       // Value parameters in pairs of tokens, as the fragments take them: in place
       // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
-      uint32_t apart = 0;  // tokens with a Value group that stays out of the product
+      uint32_t apart = 0;  // tokens with a Value group that stays out of the product (add_apart)
       {
         constexpr int kQ = kG / 2;  // groups of a lane: two lanes for each of the 16 pairs
         const int x = lane >> 1, q = lane & 1;
@@ -469,25 +520,15 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           e[k] = par[2 * x * kG + q * kQ + k];
           o[k] = par[(2 * x + 1) * kG + q * kQ + k];
         }
-        if (masked) {
-          // What an unwritten slot holds must not be read; a NaN group that only some
-          // columns see goes into their sums (below), not through the product.
-          const int tok = base + 2 * x;
-          bool nan_e = false, nan_o = false;
+        bool any_apart = false;
+        const int tok = base + 2 * x;
+        if (masked) {  // what an unwritten slot holds must not be read
 #pragma unroll
           for (int k = 0; k < kQ; ++k) {
             if (tok >= seen_max) e[k] = 0;
             if (tok + 1 >= seen_max) o[k] = 0;
-            if (tok >= vis_min && is_nan_param(e[k])) {
-              nan_e = true;
-              e[k] = 0;
-            }
-            if (tok + 1 >= vis_min && is_nan_param(o[k])) {
-              nan_o = true;
-              o[k] = 0;
-            }
+            any_apart |= (tok >= vis_min && is_nan_param(e[k])) || (tok + 1 >= vis_min && is_nan_param(o[k]));
           }
-          apart = token_bits(nan_e, nan_o);
         }
         uint32_t s2[kQ], z2[kQ], most = 0;
 #pragma unroll
@@ -497,24 +538,23 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           most = max_abs2(most, hmul2(s2[k], 0x4C004C00u));  // 16 s
           most = max_abs2(most, z2[k]);
         }
-        // code * s + z may pass the fp16 range only where 16 s or |z| is 2^15 or
-        // more: Values are held at 1/32 from the first such half page on.
-        const bool wide = (most & 0x7FFFu) >= 0x7800u || (most & 0x7FFF0000u) >= 0x78000000u;
-        if (__any_sync(0xffffffffu, wide) || back != 1.0f) {
-          if (back == 1.0f) {
-            back = 32.0f;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[nt][y][k] *= 0.03125f;
-          }
+        any_apart |= (most & 0x7FFFu) >= 0x7800u || (most & 0x7FFF0000u) >= 0x78000000u;  // 2^15: is_wide_param of one
+        if (__any_sync(0xffffffffu, any_apart)) {
+          bool apart_e = false, apart_o = false;
 #pragma unroll
           for (int k = 0; k < kQ; ++k) {
-            s2[k] = hmul2(s2[k], 0x28002800u);
-            z2[k] = hmul2(z2[k], 0x28002800u);
+            if (stays_apart(e[k], tok, vis_min)) {
+              apart_e = true;
+              e[k] = 0;
+            }
+            if (stays_apart(o[k], tok + 1, vis_min)) {
+              apart_o = true;
+              o[k] = 0;
+            }
+            s2[k] = __byte_perm(e[k], o[k], 0x5410);
+            z2[k] = __byte_perm(e[k], o[k], 0x7632);
           }
+          apart = token_bits(apart_e, apart_o);
         }
         __syncwarp();  // every lane has read its words
         if constexpr (kQ == 2)
@@ -579,21 +619,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
               for (int k = 0; k < 2; ++k)
                 if (tok >= vis[nt][k]) x[sub][nt][2 * r + k] = -INFINITY;
           }
-      }
-      // A NaN group among the tokens that only some columns see: NaN in its channels of
-      // the columns that do.  The pairs hold 0 for it by now: look at the record.
-      for (; apart != 0; apart &= apart - 1) {
-        const int tok = base + __ffs(apart) - 1;
-        const uint32_t* par = value_params<kG>(p, h, b, tok);
-#pragma unroll
-        for (int G = 0; G < kG; ++G) {
-          if (!is_nan_param(par[G])) continue;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (tok < vis[nt][k & 1]) acc[nt][2 * G][k] = acc[nt][2 * G + 1][k] = NAN;
-        }
       }
 
       // The running maxima (m lies kLift below), moved where a score passes one by more
@@ -695,6 +720,29 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           }
         }
       }
+      if (apart != 0) {
+        Apart<D, NT> held;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int y = 0; y < 2 * kG; ++y)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) held.acc[nt][y][k] = acc[nt][y][k];
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) held.w[nt][4 * sub + k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) held.vis[nt][c] = vis[nt][c];
+        }
+        add_apart<D, NT>(p, h, b, apart, base, vis_min, reinterpret_cast<const uint32_t*>(stage + kCodes), held);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int y = 0; y < 2 * kG; ++y)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[nt][y][k] = held.acc[nt][y][k];
+      }
     }
     cp_wait<0>();
     __syncthreads();  // the rings are free: the merge buffer takes their place
@@ -718,8 +766,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
         for (int G = 0; G < kG; ++G)
           *reinterpret_cast<float4*>(merge + col * C::kPad + 32 * G + 4 * g) =
-              make_float4(acc[nt][2 * G][k] * back, acc[nt][2 * G][k + 2] * back, acc[nt][2 * G + 1][k] * back,
-                          acc[nt][2 * G + 1][k + 2] * back);
+              make_float4(acc[nt][2 * G][k], acc[nt][2 * G][k + 2], acc[nt][2 * G + 1][k], acc[nt][2 * G + 1][k + 2]);
       }
     __syncthreads();
 

@@ -99,3 +99,47 @@ def test_weights_far_below_a_dominant_token(dtype, B, H, nq, D, gap):
     some = list(range(0, B, 7))   # of a large batch, sequences enough
     want, weight = _dense_reference(q[some], [T] * len(some), [1] * len(some), sk[some], sv[some], D ** -0.5)
     _check(got[some], want, weight, dtype, T * 2.0 ** -32 * np.abs(sv).max())
+
+
+# ----------------------------------------------------------------- large Values
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,nq,L", [(64, 4, 1), (64, 12, 3), (128, 4, 1), (128, 14, 3)])
+@pytest.mark.parametrize("first", [0, 400])
+def test_values_past_the_fp16_range_beside_small_ones(dtype, D, nq, L, first):
+    """Value groups of magnitude 4e4 (and, for bf16 outputs, 6e5) from token ``first`` on,
+    in some channels of some tokens, beside groups of magnitude 2e-4."""
+    T, H = 600, 2
+    g = torch.Generator().manual_seed(D + nq)
+    key, value = torch.randn(1, H, T, D, generator=g), torch.randn(1, H, T, D, generator=g) * 2e-4
+    low, high = (-4e4, 4e4) if dtype == F16 else (-6e4, 6e5)   # the minimum has to fit fp16, the range 15 times that
+    value[:, 0, first::5, 32:64] = low + torch.rand(1, len(range(first, T, 5)), 32, generator=g) * (high - low)
+    value[:, 1, first + 1::64, :32] = 3.5e4 + torch.rand(1, len(range(first + 1, T, 64)), 32, generator=g)
+    value[:, :, T - 2, :32] = -4e4   # among the drafts
+    key, value = key.cuda(), value.cuda()
+    table, n = _table(1, 1, 10)
+    pages, bounds = _garbage(n, H, D), int4.alloc_bounds(n, H, D)
+    int4.int4_write(key, value, pages, table, _i32([0]), bounds=bounds)
+    sk, sv = ref.stored(key.double().cpu().numpy()), ref.stored(value.double().cpu().numpy())
+    assert np.abs(sv).max() > 32768
+    q = 3 * _queries(1, 1, nq, L, D, dtype)
+    got = int4.int4_attention(q, pages, table, _i32([T]), D ** -0.5)
+    _check(got, *_dense_reference(q, [T], [L], sk, sv, D ** -0.5), dtype, 2.0 ** -24)
+    got, picked = int4.int4_sparse_attention(q, pages, bounds, table, _i32([T]), D ** -0.5, top_pages=2, sink_pages=1, recent_pages=1)
+    _check(got, *_dense_reference(q, [T], [L], sk, sv, D ** -0.5, picked.cpu().numpy()), dtype, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_masked_large_value_changes_nothing(D):
+    """The slots past the length hold Values of 5e4, the seen ones 2e-4."""
+    T, H = 100, 1
+    g = torch.Generator().manual_seed(1)
+    key, value = torch.randn(1, H, 128, D, generator=g).cuda(), (torch.randn(1, H, 128, D, generator=g) * 2e-4).cuda()
+    value[:, :, T:] = 5e4
+    table, n = _table(1, 1, 2)
+    pages = _garbage(n, H, D)
+    int4.int4_write(key, value, pages, table, _i32([0]))
+    sk, sv = ref.stored(key.double().cpu().numpy()), ref.stored(value.double().cpu().numpy())
+    q = _queries(1, 1, 5, 2, D)
+    got = int4.int4_attention(q, pages, table, _i32([T]), D ** -0.5)
+    _check(got, *_dense_reference(q, [T], [2], sk, sv, D ** -0.5), BF16, 2.0 ** -24)
