@@ -449,7 +449,8 @@ LF_API int lf_int4_select(const lf_int4_query* args, lf_stream_t stream);
  */
 LF_API int lf_int4_attend(const lf_int4_query* args, lf_stream_t stream);
 
-/* lf_int4_select, then lf_int4_attend over what it picked. */
+/* lf_int4_select, then lf_int4_attend over what it picked.  With a negative scaling
+ * the pages are those of the negated queries: the largest bounds on scaling q . K. */
 LF_API int lf_int4_attend_sparse(const lf_int4_query* args, lf_stream_t stream);
 
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);

@@ -1001,8 +1001,3 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
   return a->head_dim == 128 ? lf::launch_attend_by<__nv_bfloat16, 128>(p, sms, s)
                             : lf::launch_attend_by<__nv_bfloat16, 64>(p, sms, s);
 }
-
-extern "C" int lf_int4_attend_sparse(const lf_int4_query* a, lf_stream_t stream) {
-  const int bad = lf_int4_select(a, stream);
-  return bad != LF_OK ? bad : lf_int4_attend(a, stream);
-}

@@ -36,6 +36,7 @@ struct SelectParams {
   int top, sink, recent, cluster;
   int32_t* picked;
   int32_t* status;
+  float sign;  // of the scores' scaling: -1 chooses for the negated queries
 };
 
 constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) int4_select_kernel(const __
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSelectWarps; ++w) most = fmaxf(most, most_s[w]);
-  const float scale = pow2(-exponent127(most));
+  const float scale = pow2(-exponent127(most)) * p.sign;
   if (tid < D) {
     int plus = 0, minus = 0;
     for (int j = 0; j < p.group; ++j) {
@@ -308,9 +309,10 @@ static int launch_select(SelectParams p, cudaStream_t stream) {
 
 }  // namespace lf
 
-extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
-  LF_CHECK_ARG(a != nullptr, "lf_int4_select: null arguments");
+// The choice for the queries times sign.
+static int select_pages(const lf_int4_query* a, float sign, lf_stream_t stream) {
   lf::SelectParams p;
+  p.sign = sign;
   const int bad = lf::check_int4_pool("lf_int4_select", a->pool, a->head_dim, p.pool);
   if (bad != LF_OK) return bad;
   LF_CHECK_ARG(a->q && a->bounds && a->lengths && a->picked, "lf_int4_select: null pointer");
@@ -350,4 +352,15 @@ extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
   if (a->dtype == LF_F16)
     return a->head_dim == 128 ? lf::launch_select<__half, 128>(p, s) : lf::launch_select<__half, 64>(p, s);
   return a->head_dim == 128 ? lf::launch_select<__nv_bfloat16, 128>(p, s) : lf::launch_select<__nv_bfloat16, 64>(p, s);
+}
+
+extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
+  LF_CHECK_ARG(a != nullptr, "lf_int4_select: null arguments");
+  return select_pages(a, 1.0f, stream);
+}
+
+extern "C" int lf_int4_attend_sparse(const lf_int4_query* a, lf_stream_t stream) {
+  LF_CHECK_ARG(a != nullptr, "lf_int4_attend_sparse: null arguments");
+  const int bad = select_pages(a, a->scaling < 0.0f ? -1.0f : 1.0f, stream);
+  return bad != LF_OK ? bad : lf_int4_attend(a, stream);
 }

@@ -113,8 +113,8 @@ def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torc
                           lengths: torch.Tensor, scaling: float, top_pages: int, sink_pages: int = 1,
                           recent_pages: int = 2, counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
                           status: torch.Tensor | None = None):
-    """:func:`int4_select`, then :func:`int4_attention` over the picked pages
-    only: ``(out, picked)``.  With ``sink + recent + top`` pages or fewer
+    """:func:`int4_select` (of the negated query where ``scaling`` is negative),
+    then :func:`int4_attention` over the picked pages only: ``(out, picked)``.  With ``sink + recent + top`` pages or fewer
     visible, every page is read and the result is the dense one."""
     return _lib.int4_binding().attend(query, pages, page_table, lengths, scaling, counts, out, status, bounds, top_pages,
                                       sink_pages, recent_pages)

@@ -8,7 +8,7 @@ import torch
 
 from logitfill_b200 import int4
 from tests import int4_reference as ref
-from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _garbage, _i32, _table
+from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _garbage, _i32, _picks, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,19 @@ def test_a_masked_large_value_changes_nothing(D):
     q = _queries(1, 1, 5, 2, D)
     got = int4.int4_attention(q, pages, table, _i32([T]), D ** -0.5)
     _check(got, *_dense_reference(q, [T], [2], sk, sv, D ** -0.5), BF16, 2.0 ** -24)
+
+
+# ------------------------------------------------------------ negative scalings
+
+@pytest.mark.parametrize("D,nq,H", [(128, 28, 4), (64, 8, 8)])
+def test_sparse_with_a_negative_scaling(D, nq, H):
+    """The pages with the largest bound on scaling * q . K: those of the negated query."""
+    lengths, L = [1500, 64 * 9, 130], 2
+    pages, table, bounds, sk, sv = _filled(7, lengths, H, D)
+    q = _queries(1, 3, nq, L, D)
+    got, picked = int4.int4_sparse_attention(q, pages, bounds, table, _i32(lengths), -D ** -0.5, 4, 1, 2)
+    want = _picks(-q, sk, lengths, [L] * 3, 4, 1, 2)
+    assert np.array_equal(picked.cpu().numpy(), want)
+    _check(got, *_dense_reference(q, lengths, [L] * 3, sk, sv, -D ** -0.5, want), BF16, 2.0 ** -24)
+    flipped, same = int4.int4_sparse_attention(-q, pages, bounds, table, _i32(lengths), D ** -0.5, 4, 1, 2)
+    assert torch.equal(same, picked) and torch.equal(flipped, got)
