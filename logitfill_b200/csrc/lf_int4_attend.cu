@@ -20,8 +20,8 @@
 // keep fewer bits: fp16 ends at steps of 2^-24.  So that a dominant token does not
 // press the rest of its warp's tokens below that, the largest weight is put at 2^7
 // and not at 1: what is lost of a weight is then 2^-32 of the warp's largest at most.
-// A Value group that may pass the fp16 range stays out of the product and is added in
-// fp32, token by token.
+// A Value group that may pass the fp16 range stays out of the product and gets one of
+// its own, at 1/32 (add_apart).
 //
 // The work is one pass over the pages with a running maximum and sum.  The
 // maximum is moved only when a score passes it by 2^8 (p <= 2^15 fits), so most
@@ -99,6 +99,9 @@ template <int D, int NT> struct AttendCfg {
   static constexpr int kSmem = kRing > kRoom ? kRing : kRoom;
   static constexpr int kFit = kSmem / (4 * kRecord);  // partials that are merged at once
 };
+
+// fp16 numbers that make up a weight.
+template <typename T> constexpr int kWeightTerms = std::is_same<T, __half>::value ? 2 : 1;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -190,57 +193,130 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[kWor
     w[0] = x.x; w[1] = x.y;
   }
 }
-// Value parameters of position tok in the record (its page is known to be there).
-template <int kG>
-__device__ __forceinline__ const uint32_t* value_params(const AttendParams& p, int h, int b, int tok) {
-  const int id = int4_page_id(p.pool, b, tok / kInt4Page);
-  return reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h) + 18 * 32 * kG + tok % kInt4Page * kG;
-}
 // Bit i: token i of 32, where lanes 2 x and 2 x + 1 hold flags of tokens 2 x and 2 x + 1.
 __device__ __forceinline__ uint32_t token_bits(bool even, bool odd) {
   const uint32_t e = __ballot_sync(0xffffffffu, even), o = __ballot_sync(0xffffffffu, odd);
   return ((e | e >> 1) & 0x55555555u) | ((o | o << 1) & 0xAAAAAAAAu);
 }
 
-// A warp's sums, weights (fragment order) and visible tokens, for add_apart.
-template <int D, int NT> struct Apart {
-  float acc[NT][D / 16][4], w[NT][4 * kSubs];
-  int vis[NT][2];
-};
-// Value groups that stay out of the product, added in fp32 to the columns that see
-// their token: those past the fp16 range (scaled to fit, they would cost the small
-// groups beside them their low bits), and NaN ones that only some columns see.
-// `apart` has the part's tokens with such groups.  The parameters are those of the
-// record: the pairs in shared memory hold 0 for these groups.  A call of its own on
-// copies: in the loop the registers it takes cost 1 % at D 128, 5 % with 16 columns.
-template <int D, int NT>
-__device__ __noinline__ void add_apart(const AttendParams& p, int h, int b, uint32_t apart, int base, int vis_min,
-                                       const uint32_t* codes, Apart<D, NT>& s) {
-  constexpr int kG = D / kInt4Group;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll 1
-  for (; apart != 0; apart &= apart - 1) {
-    const int k = __ffs(apart) - 1, tok = base + k;
-    const uint32_t* par = value_params<kG>(p, h, b, tok);
-    const uint32_t* words = codes + (k >> 3) * D + g * (D / 8) + ((k & 7) >> 1) * (D / 32) + (k & 1) * (D / 64);
-#pragma unroll 1
-    for (int col = 0; col < 2 * NT; ++col) {
-      const int nt = col >> 1, c = col & 1;
-      // row k & 7 of the scores' fragments holds the token
-      const float w = __shfl_sync(0xffffffffu, s.w[nt][2 * (k >> 3) + c], (k & 7) * 4 + t);
-      const bool seen = tok < s.vis[nt][c];
-#pragma unroll 1
-      for (int G = 0; G < kG; ++G) {
-        const uint32_t sz = par[G], four = words[G >> 1] >> (16 * (G & 1));
-        if (!seen || !stays_apart(sz, tok, vis_min)) continue;
+// Weights of 16 tokens (pr, spent: rows g and g + 8 of the scores' fragments) as the
+// product's B operand, columns by tokens, in kTerms fp16 numbers.
+template <int kTerms>
+__device__ __forceinline__ void weight_operand(float (&pr)[4], uint32_t (&b)[kTerms][2]) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {  // channel 4 g + n
-          float& a = s.acc[nt][2 * G + (n >> 1)][2 * (n & 1) + c];
-          a = fmaf(w, fmaf(static_cast<float>(four >> (4 * n) & 15u), half_lo(sz), half_hi(sz)), a);
-        }
+  for (int y = 0; y < kTerms; ++y)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w = pack_half2(pr[2 * k], pr[2 * k + 1]);
+      b[y][k] = transpose8x8(w);
+      if (y + 1 < kTerms) {
+        pr[2 * k] -= half_lo(w);
+        pr[2 * k + 1] -= half_hi(w);
       }
     }
+}
+// Values of channels 4 g + n of group G for a pair of tokens, from its code words
+// ([token][w]), scales and minima.
+template <int kG>
+__device__ __forceinline__ void value_operand(const uint32_t (&words)[kG], int G, uint32_t s2, uint32_t z2, uint32_t (&v)[4]) {
+  // bytes of the even and the odd token, as 1024 + byte
+  const uint32_t y = __byte_perm(words[G >> 1], words[kG / 2 + (G >> 1)], (G & 1) ? 0x7362 : 0x5140);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t even, odd;
+    two_codes(__byte_perm(y, 0x64646464u, k == 0 ? 0x4140 : 0x4342), even, odd);
+    v[2 * k] = hfma2(even, s2, z2);
+    v[2 * k + 1] = hfma2(odd, s2, z2);
   }
+}
+// sums += Values (two pairs of tokens) times weights.
+template <int D, int NT, int kTerms>
+__device__ __forceinline__ void add_values(float (&acc)[NT][D / 16][4], int G, const uint32_t (&v)[2][4],
+                                           const uint32_t (&pb)[NT][kTerms][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int y = 0; y < kTerms; ++y) {
+      mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][y][0], pb[nt][y][1]);
+      mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][y][0], pb[nt][y][1]);
+    }
+}
+
+// A warp's sums, weights (fragment order) and visible tokens, for add_apart.
+template <int D, int NT> struct Apart {
+  float acc[NT][D / 16][4], w[NT][kSubs][4];
+  int vis[NT][2];
+};
+// Value groups that stay out of the product; `apart` has the tokens of the part that
+// have some.  NaN ones that only some columns see become NaN in the sums of those.
+// Those that may pass the fp16 range are multiplied at 1/32, the others' parameters 0:
+// scaled together, the small groups would lose their low bits.  (A Value of such a
+// group, whose step is 2^11 or whose minimum 2^15, is right to 2^-20 or 2^-11 of itself.)
+// The parameters are the record's: the pairs in shared memory hold 0 for these
+// groups.  A call of its own on copies: the registers it takes in the loop cost the usual
+// half pages 1 % at D 128, 5 % with 16 columns.  8 x 32k tokens, 28 heads on 4, D 128,
+// take 104 us with such a group in every token, 89 in every 64th, 42 in none (in fp32,
+// token by token: 1071 and 90).
+template <typename T, int D, int NT>
+__device__ __noinline__ void add_apart(const AttendParams& p, int h, int b, uint32_t apart, int base, int vis_min,
+                                       const uint8_t* vcode, Apart<D, NT>& s) {
+  constexpr int kG = D / kInt4Group, kTerms = kWeightTerms<T>;
+  const int lane = threadIdx.x & 31, t = lane & 3, tok = base + lane;
+  uint32_t par[kG];  // the lane's token's
+#pragma unroll
+  for (int G = 0; G < kG; ++G) par[G] = 0;
+  if (apart >> lane & 1) {
+    const int id = int4_page_id(p.pool, b, tok / kInt4Page);  // known to be there
+    load_words<kG>(reinterpret_cast<const uint8_t*>(p.pool.words + int4_record(p.pool, id, h) + 18 * D +
+                                                    tok % kInt4Page * kG), par);
+  }
+  bool wide = false;
+#pragma unroll
+  for (int G = 0; G < kG; ++G) {
+    const uint32_t nan = __ballot_sync(0xffffffffu, tok >= vis_min && is_nan_param(par[G]));
+    const int first = nan != 0 ? base + __ffs(nan) - 1 : INT32_MAX;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (first < s.vis[nt][k & 1]) s.acc[nt][2 * G][k] = s.acc[nt][2 * G + 1][k] = NAN;
+    if (!is_wide_param(par[G])) par[G] = 0;
+    wide |= par[G] != 0;
+  }
+  if (!__any_sync(0xffffffffu, wide)) return;
+  float acc[NT][2 * kG][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int y = 0; y < 2 * kG; ++y)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[nt][y][k] = s.acc[nt][y][k] * 0.03125f;
+#pragma unroll 1
+  for (int sub = 0; sub < kSubs; ++sub) {
+    uint32_t pb[NT][kTerms][2], vw[2][kG];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) weight_operand<kTerms>(s.w[nt][sub], pb[nt]);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) load_words<kG>(vcode + (2 * sub + r) * (4 * D) + lane * (4 * kG), vw[r]);
+#pragma unroll
+    for (int G = 0; G < kG; ++G) {
+      uint32_t v[2][4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int k = sub * kTile + 8 * r + 2 * t;
+        const uint32_t e = __shfl_sync(0xffffffffu, par[G], k), o = __shfl_sync(0xffffffffu, par[G], k + 1);
+        value_operand<kG>(vw[r], G, hmul2(__byte_perm(e, o, 0x5410), 0x28002800u), hmul2(__byte_perm(e, o, 0x7632), 0x28002800u),
+                          v[r]);
+      }
+      add_values<D>(acc, G, v, pb);
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int y = 0; y < 2 * kG; ++y)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s.acc[nt][y][k] = acc[nt][y][k] * 32.0f;
 }
 
 // Adds 1 and returns what was there.  What the CTA wrote before the barrier ahead
@@ -285,7 +361,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   using C = AttendCfg<D, NT>;
   constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
-  constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 1;  // fp16 numbers that make up a weight
+  constexpr int kTerms = kWeightTerms<T>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int meta_s[kWarps][kStages];  // first token of each stage's part of a page, -1: nothing to do
   __shared__ int last_s;
@@ -671,17 +747,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             l[nt][0] = sum.x;
             l[nt][1] = sum.y;
           }
-#pragma unroll
-          for (int y = 0; y < kTerms; ++y)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t w = pack_half2(pr[2 * k], pr[2 * k + 1]);
-              pb[nt][y][k] = transpose8x8(w);
-              if (y + 1 < kTerms) {
-                pr[2 * k] -= half_lo(w);
-                pr[2 * k + 1] -= half_hi(w);
-              }
-            }
+          weight_operand<kTerms>(pr, pb[nt]);
         }
 
         // Values: codes of 16 tokens, pairs (2t, 2t + 1) of each half, and their parameters.
@@ -698,26 +764,8 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         for (int G = 0; G < kG; ++G) {
           uint32_t v[2][4];  // half, channel 4 g + n of the group
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t s2 = sz[r][2 * G], z2 = sz[r][2 * G + 1];
-            // bytes of the even and the odd token (words [token][w]), as 1024 + byte
-            const uint32_t y = __byte_perm(vw[r][G >> 1], vw[r][kG / 2 + (G >> 1)], (G & 1) ? 0x7362 : 0x5140);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              uint32_t even, odd;
-              two_codes(__byte_perm(y, 0x64646464u, k == 0 ? 0x4140 : 0x4342), even, odd);
-              v[r][2 * k] = hfma2(even, s2, z2);
-              v[r][2 * k + 1] = hfma2(odd, s2, z2);
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int y = 0; y < kTerms; ++y) {
-              mma16816(acc[nt][2 * G], v[0][0], v[0][1], v[1][0], v[1][1], pb[nt][y][0], pb[nt][y][1]);
-              mma16816(acc[nt][2 * G + 1], v[0][2], v[0][3], v[1][2], v[1][3], pb[nt][y][0], pb[nt][y][1]);
-            }
-          }
+          for (int r = 0; r < 2; ++r) value_operand<kG>(vw[r], G, sz[r][2 * G], sz[r][2 * G + 1], v[r]);
+          add_values<D>(acc, G, v, pb);
         }
       }
       if (apart != 0) {
@@ -731,11 +779,11 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
           for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) held.w[nt][4 * sub + k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
+            for (int k = 0; k < 4; ++k) held.w[nt][sub][k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
 #pragma unroll
           for (int c = 0; c < 2; ++c) held.vis[nt][c] = vis[nt][c];
         }
-        add_apart<D, NT>(p, h, b, apart, base, vis_min, reinterpret_cast<const uint32_t*>(stage + kCodes), held);
+        add_apart<T>(p, h, b, apart, base, vis_min, stage + kCodes, held);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
