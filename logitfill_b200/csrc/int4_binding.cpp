@@ -77,6 +77,8 @@ Pool make_pool(PyObject* pages_o, PyObject* table_o) {
     fail(PyExc_ValueError, "pages must be int32 [n_pages, n_kv, words] with word stride 1, got ", shape(pages));
   if (table.dim() != 2 || table.scalar_type() != at::kInt || table.stride(1) != 1)
     fail(PyExc_ValueError, "page_table must be int32 [batch, width] with entry stride 1, got ", shape(table));
+  if (pages.numel() == 0 || table.numel() == 0)
+    fail(PyExc_ValueError, "empty pool, batch or page table: pages ", shape(pages), ", page_table ", shape(table));
   if (!pages.is_cuda()) fail(PyExc_RuntimeError, "the 4-bit cache needs CUDA tensors (there is no CPU path)");
   if (table.device() != pages.device())
     fail(PyExc_RuntimeError, "page_table is on ", table.device(), ", pages on ", pages.device());

@@ -159,3 +159,18 @@ def test_sparse_with_a_negative_scaling(D, nq, H):
     _check(got, *_dense_reference(q, lengths, [L] * 3, sk, sv, -D ** -0.5, want), BF16, 2.0 ** -24)
     flipped, same = int4.int4_sparse_attention(-q, pages, bounds, table, _i32(lengths), D ** -0.5, 4, 1, 2)
     assert torch.equal(same, picked) and torch.equal(flipped, got)
+
+
+# ------------------------------------------------------------ empty pools
+
+def test_pools_without_pages_heads_or_sequences_are_refused():
+    pages, bounds = int4.alloc_pages(4, 2, 64), int4.alloc_bounds(4, 2, 64)
+    table, n = _i32([[0, 1], [2, 3]]), _i32([5, 5])
+    q = torch.zeros(2, 4, 64, dtype=BF16, device="cuda")
+    for p, b, t, m, x in ((pages[:, :0], bounds[:, :0], table, n, q), (pages[:0], bounds[:0], table, n, q),
+                          (pages[..., :0], bounds, table, n, q), (pages, bounds, table[:, :0], n, q),
+                          (pages, bounds, table[:0], n[:0], q[:0])):
+        for call in (lambda: int4.int4_attention(x, p, t, m, 1.0), lambda: int4.int4_select(x, p, b, t, m, 4),
+                     lambda: int4.int4_sparse_attention(x, p, b, t, m, 1.0, 4), lambda: int4.int4_read(p, t, m, 3)):
+            with pytest.raises(ValueError):
+                call()
