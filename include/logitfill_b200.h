@@ -387,7 +387,7 @@ typedef struct lf_int4_tokens {
 LF_API int lf_int4_write(const lf_int4_tokens* args, lf_stream_t stream);
 
 /* Read positions start[b] .. start[b] + tokens - 1 back into key and value; token i
- * is zero from counts[b] on. */
+ * is zero from counts[b] on, and where its position is below 0 (out of range). */
 LF_API int lf_int4_read(const lf_int4_tokens* args, lf_stream_t stream);
 
 /* Bounds records as fp32 values: out [n_pages][kv_heads][2][head_dim], upper then lower. */

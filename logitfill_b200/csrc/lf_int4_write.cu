@@ -410,13 +410,13 @@ __global__ void __launch_bounds__(kWriteThreads) int4_read_kernel(const __grid_c
   const int G = l >> 2, t = l & 3, u = G & 1, w = G >> 1;
   const int i0 = blockIdx.x * kInt4Page, last = min(i0 + kInt4Page, p.tokens);
   const int64_t pos0 = static_cast<int64_t>(start) + i0;
+  const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));  // slot of its page, rounded down
   auto record = [&](int x) -> const uint32_t* {  // of the first page, or of the one after
-    const int64_t page = pos0 >= 0 ? pos0 / kInt4Page + x : -1;
-    const int id = page < p.pool.table_width ? int4_page_id(p.pool, b, static_cast<int>(page)) : -1;
+    const int64_t page = (pos0 - k0) / kInt4Page + x;  // negative for a position below 0
+    const int id = page >= 0 && page < p.pool.table_width ? int4_page_id(p.pool, b, static_cast<int>(page)) : -1;
     return id < 0 ? nullptr : reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, h);
   };
   const uint32_t *rec0 = record(0), *rec1 = record(1);
-  const int k0 = static_cast<int>(pos0 & (kInt4Page - 1));
   T* key = static_cast<T*>(p.key) + b * p.k_seq + h * p.k_head + i0 * p.k_tok + 8 * l;
   T* value = static_cast<T*>(p.value) + b * p.v_seq + h * p.v_head + i0 * p.v_tok + 8 * l;
   constexpr int kAtOnce = 4;  // rows whose loads are in flight together (one: 38 us for the prompts above, four: 31.4)

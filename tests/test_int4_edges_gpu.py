@@ -174,3 +174,17 @@ def test_pools_without_pages_heads_or_sequences_are_refused():
                      lambda: int4.int4_sparse_attention(x, p, b, t, m, 1.0, 4), lambda: int4.int4_read(p, t, m, 3)):
             with pytest.raises(ValueError):
                 call()
+
+
+# ------------------------------------------------------------ negative positions
+
+@pytest.mark.parametrize("start", [-10, -64, -70, -300])
+def test_read_from_a_negative_position(start):
+    """Positions below 0 are zeros and reported; those from 0 on are read."""
+    D, T = 64, 150
+    pages, table, _, sk, sv = _filled(1, [T], 2, D)
+    status = _i32([0])
+    k, v = int4.int4_read(pages, table, _i32([start]), T - start, status=status)
+    assert int(status) != 0
+    assert not k[:, :, :-start].any() and not v[:, :, :-start].any()
+    assert np.array_equal(k[:, :, -start:].cpu().numpy(), sk) and np.array_equal(v[:, :, -start:].cpu().numpy(), sv)
