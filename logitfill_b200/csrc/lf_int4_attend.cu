@@ -25,7 +25,9 @@
 //
 // The work is one pass over the pages with a running maximum and sum.  The
 // maximum is moved only when a score passes it by 2^8 (p <= 2^15 fits), so most
-// tiles skip the rescaling.
+// tiles skip the rescaling.  It is kept in the scores' own units and enters as what
+// the minima's product starts from: scores come out relative to it, and no rounding of
+// a large product of score and scaling reaches the exponent.
 //
 // Split.  All pages of all units form one line, cut into equal ranges, one per
 // CTA (the lengths are read on the device, so nothing is planned on the host).
@@ -74,7 +76,7 @@ constexpr int kPart = kInt4Page / 2;  // tokens of a page that one warp takes
 constexpr int kSubs = kPart / kTile;
 constexpr float kLift = 7.0f;         // log2 of the weight that a running maximum stands for
 constexpr float kSlack = 8.0f;        // log2 a score may pass the running maximum by
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -3e38f;      // below any score
 constexpr int kMinPages = 4;          // places of a range at least: two pages for each pair of warps
 constexpr int kUnitCost = 6;          // empty places before a unit's pages (at 8 x 32k 16 cost 2 us more, 40 2.4)
 
@@ -122,10 +124,11 @@ __device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ void mma1688_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+// From one number per column.
+__device__ __forceinline__ void mma1688_from(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0, float from0, float from1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%7,%8};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
+      : "r"(a0), "r"(a1), "r"(b0), "f"(from0), "f"(from1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -514,9 +517,10 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // 2^kq brings the column's largest magnitude to [2^13, 2^14)
+      // 2^kq brings the column's largest magnitude to [2^13, 2^14) (below where the largest
+      // is under 2^-114: 2^127 is the last power there is)
       const int kq = most > 0.0f && most < INFINITY
-                         ? max(-100, min(100, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127)))
+                         ? min(127, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127))
                          : 0;
       const float up = pow2(kq) * flip;
       float sums[kG];
@@ -525,8 +529,8 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         sums[G] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          sums[G] += x[G][k];
           x[G][k] *= up;
+          sums[G] += x[G][k];
         }
         sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 1);
         sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 2);
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       float mine = 0.0f;
 #pragma unroll
       for (int G = 0; G < kG; ++G) mine = t == G ? sums[G] : mine;
-      mine *= pow2(kq - 10) * flip;
+      mine *= 0x1p-10f;
       const float hi = __half2float(__float2half_rn(mine));
       qz[nt] = pack_half2(hi, mine - hi);
 #pragma unroll
@@ -557,12 +561,13 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     for (int nt = 0; nt < NT; ++nt) vis_min = min(vis_min, min(vis[nt][0], vis[nt][1]));
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
-    float acc[NT][2 * kG][4], m[NT][2], l[NT][2];
+    float acc[NT][2 * kG][4], back[NT][2], l[NT][2];  // back: the running maxima, negated
+    bool fresh = true;  // before the first part
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        m[nt][k] = kNoMax;
+        back[nt][k] = 0.0f;
         l[nt][k] = 0.0f;
       }
 #pragma unroll
@@ -657,7 +662,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         float dot[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma1688_zero(x[sub][nt], kz[0], kz[1], qz[nt]);
+          mma1688_from(x[sub][nt], kz[0], kz[1], qz[nt], back[nt][0], back[nt][1]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) dot[nt][k] = 0.0f;
         }
@@ -697,9 +702,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           }
       }
 
-      // The running maxima (m lies kLift below), moved where a score passes one by more
-      // than the slack.
-      bool move = false;
+      // The running maxima, moved where a score passes one by more than the slack, and set
+      // by the first part (a column that sees nothing of it sees nothing of the later ones).
+      bool move = fresh;
       float most[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -708,7 +713,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           most[nt][k] = fmaxf(x[0][nt][k], x[0][nt][k + 2]);
 #pragma unroll
           for (int sub = 1; sub < kSubs; ++sub) most[nt][k] = fmaxf(most[nt][k], fmaxf(x[sub][nt][k], x[sub][nt][k + 2]));
-          move |= fmaf(most[nt][k], c2[nt][k], -m[nt][k]) > kLift + kSlack;
+          move |= most[nt][k] * c2[nt][k] > kSlack;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -716,19 +721,25 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           float fix[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float top = most[nt][k] * c2[nt][k];
+            float by = most[nt][k];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top - kLift, m[nt][k]);
-            fix[k] = ex2(m[nt][k] - top);
-            m[nt][k] = top;
+            for (int o = 4; o < 32; o <<= 1) by = fmaxf(by, __shfl_xor_sync(0xffffffffu, by, o));
+            if (!(by > (fresh ? -INFINITY : 0.0f))) by = 0.0f;
+            fix[k] = fresh ? 1.0f : ex2(-by * c2[nt][k]);
+            back[nt][k] -= by;
             l[nt][k] *= fix[k];
+#pragma unroll
+            for (int sub = 0; sub < kSubs; ++sub) {
+              x[sub][nt][k] -= by;
+              x[sub][nt][k + 2] -= by;
+            }
           }
 #pragma unroll
           for (int y = 0; y < 2 * kG; ++y)
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[nt][y][k] *= fix[k & 1];
         }
+        fresh = false;
       }
 
 #pragma unroll
@@ -739,7 +750,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           float pr[4];
 #pragma unroll
           for (int k = 0; k < 4; k += 2) {
-            float a0 = -m[nt][0], a1 = -m[nt][1];
+            float a0 = kLift, a1 = kLift;
             fma2(a0, a1, x[sub][nt][k], x[sub][nt][k + 1], c2[nt][0], c2[nt][1]);
             pr[k] = ex2(a0);
             pr[k + 1] = ex2(a1);
@@ -779,7 +790,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
           for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) held.w[nt][sub][k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], -m[nt][k & 1]));
+            for (int k = 0; k < 4; ++k) held.w[nt][sub][k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], kLift));
 #pragma unroll
           for (int c = 0; c < 2; ++c) held.vis[nt][c] = vis[nt][c];
         }
@@ -808,7 +819,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const int col = warp * kCol + nt * 8 + 2 * t + k;
         if (g == 0) {
-          top_w[col] = m[nt][k];
+          top_w[col] = sum == 0.0f ? kNoMax : fmaxf(-back[nt][k] * c2[nt][k], kNoMax);
           sum_w[col] = sum;
         }
 #pragma unroll

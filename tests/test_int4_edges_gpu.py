@@ -188,3 +188,33 @@ def test_read_from_a_negative_position(start):
     assert int(status) != 0
     assert not k[:, :, :-start].any() and not v[:, :, :-start].any()
     assert np.array_equal(k[:, :, -start:].cpu().numpy(), sk) and np.array_equal(v[:, :, -start:].cpu().numpy(), sv)
+
+
+# ------------------------------------------------------------ magnitudes of queries
+
+@pytest.mark.parametrize("D,nq", [(64, 3), (128, 14)])
+def test_queries_of_any_magnitude(D, nq):
+    """bf16 queries near both ends of their range."""
+    lengths = [300]
+    pages, table, _, sk, sv = _filled(1, lengths, 1, D)
+    for scale in (2.0 ** 118, 2.0 ** 100, 2.0 ** -60, 2.0 ** -120):
+        q = (_queries(1, 1, nq, 1, D).float() * scale).to(BF16)
+        got = int4.int4_attention(q, pages, table, _i32(lengths), 0.125 / scale)
+        want, weight = _dense_reference(q, lengths, [1], sk, sv, 0.125 / scale)
+        S = float(np.abs(q.double().cpu().numpy()).sum(-1).max() * np.abs(sk).max() * 0.125 / scale)
+        _check(got, want, weight * (1.0 + S * 2.0 ** -10), BF16, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("D,nq", [(64, 3), (128, 14)])
+def test_scores_that_are_all_far_below_zero(D, nq):
+    """Every score near -1e34: the nearest to zero takes all the weight."""
+    T = 300
+    g = torch.Generator().manual_seed(D)
+    key, value = torch.rand(1, 1, T, D, generator=g).cuda() + 0.5, torch.randn(1, 1, T, D, generator=g).cuda()
+    table, n = _table(1, 1, 5)
+    pages = _garbage(n, 1, D)
+    int4.int4_write(key, value, pages, table, _i32([0]))
+    sk, sv = ref.stored(key.double().cpu().numpy()), ref.stored(value.double().cpu().numpy())
+    q = (-(torch.rand(1, nq, 1, D, generator=g) + 0.5) * 2.0 ** 110).to(BF16).cuda()
+    got = int4.int4_attention(q, pages, table, _i32([T]), 0.125)
+    _check(got, *_dense_reference(q, [T], [1], sk, sv, 0.125), BF16, 2.0 ** -24)
