@@ -160,6 +160,7 @@ class Int4KVCache:
         self._owned = np.zeros(batch, np.int64)                   # pages each sequence holds
         self._end = np.zeros(batch, np.int64)
         self._start = np.zeros(batch, np.int64)
+        self._step = 0                                            # tokens of the step, at most
         self._free = list(range(n_pages - 1, -1, -1))
 
     @property
@@ -207,6 +208,7 @@ class Int4KVCache:
         if (n < 0).any():
             raise ValueError("counts must not be negative")
         self.reserve(self._end + n)
+        self._step = int(n.max())
         if torch.cuda.is_current_stream_capturing():
             if not uniform:
                 raise RuntimeError("a captured step takes the same number of tokens for every sequence")
@@ -229,7 +231,7 @@ class Int4KVCache:
         n = np.broadcast_to(np.asarray(lengths, np.int64), (self.batch,))
         if (n < 0).any() or (n > self._end).any():
             raise ValueError("truncate() takes lengths between 0 and the present ones")
-        self._start, self._end = n.copy(), n.copy()
+        self._start, self._end, self._step = n.copy(), n.copy(), 0
         self._upload(self._spans, np.stack([self._start, self._end, np.zeros_like(n)]))
 
     def release(self, seqs=None) -> None:
@@ -239,12 +241,16 @@ class Int4KVCache:
                 self._free.append(int(self._table[b, j]))
             self._table[b, :] = -1
             self._owned[b] = self._start[b] = self._end[b] = 0
+        self._step = int((self._end - self._start).max())
         self._upload(self.page_table, self._table)
         self._upload(self._spans, np.stack([self._start, self._end, self._end - self._start]))
 
     def write(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store this step's tokens of one layer: ``[batch, n_kv, T, head_dim]``,
-        the first ``counts[b]`` of sequence ``b``."""
+        the first ``counts[b]`` of sequence ``b`` (``T`` is the largest count at
+        least)."""
+        if key.dim() == 4:
+            self._check_step("key", key.shape[2])
         int4_write(key, value, self.pages[layer], self.page_table, self.start, self.counts,
                    None if self.bounds is None else self.bounds[layer], self.status)
 
@@ -260,22 +266,28 @@ class Int4KVCache:
 
     def attend(self, layer: int, query: torch.Tensor, scaling: float, out: torch.Tensor | None = None) -> torch.Tensor:
         """:func:`int4_attention` of this step's query tokens (the first
-        ``counts[b]`` of sequence ``b``)."""
-        self._check_heads(query)
+        ``counts[b]`` of sequence ``b``; all of the step's)."""
+        self._check_query(query)
         return int4_attention(query, self.pages[layer], self.page_table, self.end, scaling, self.counts, out, self.status)
 
     def attend_sparse(self, layer: int, query: torch.Tensor, scaling: float, top_pages: int, sink_pages: int = 1,
                       recent_pages: int = 2, out: torch.Tensor | None = None):
         """:func:`int4_sparse_attention` of this step's query tokens."""
-        self._check_heads(query)
         if self.bounds is None:
             raise RuntimeError("a sparse call needs a cache made with bounds=True")
+        self._check_query(query)
         return int4_sparse_attention(query, self.pages[layer], self.bounds[layer], self.page_table, self.end, scaling,
                                      top_pages, sink_pages, recent_pages, self.counts, out, self.status)
 
-    def _check_heads(self, query: torch.Tensor) -> None:
+    def _check_query(self, query: torch.Tensor) -> None:
         if query.dim() < 3 or query.shape[1] != self.n_q:
             raise ValueError(f"query must have {self.n_q} heads, got {tuple(query.shape)}")
+        self._check_step("query", query.shape[2] if query.dim() == 4 else 1)
+
+    def _check_step(self, name: str, tokens: int) -> None:
+        # extend() has counted the step's tokens already
+        if tokens < self._step:
+            raise ValueError(f"{name} has {tokens} tokens per sequence, the step has {self._step}")
 
     def check_status(self) -> None:
         """Raise if a kernel met a position outside its sequence's pages (synchronises)."""

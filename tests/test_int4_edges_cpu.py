@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from logitfill_b200 import int4
+from tests.test_int4_cpu import cpu_cache  # noqa: F401  (a fixture)
 
 
 def test_pools_without_pages_heads_or_sequences_are_refused():
@@ -17,3 +18,33 @@ def test_pools_without_pages_heads_or_sequences_are_refused():
             int4.int4_attention(x, p, t, m, 1.0)
         with pytest.raises(ValueError):
             int4.int4_read(p, t, m, 3)
+
+
+def test_cache_refuses_fewer_tokens_than_the_step_has(cpu_cache):  # noqa: F811
+    """The lengths already count the step's tokens: a write of fewer would leave slots
+    that later calls attend, and a query of fewer would be placed at the step's first
+    tokens.  What has the step's tokens gets as far as the kernel."""
+    c = cpu_cache
+    k, q = torch.zeros(3, 2, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 4, 4, 64, dtype=torch.bfloat16)
+
+    def check(step, refused):
+        c.extend(step)
+        for n in range(1, 5):
+            error = (ValueError, f"the step has {refused}") if n < refused else (RuntimeError, "CUDA")
+            for call in (lambda: c.write(0, k[:, :, :n], k[:, :, :n]), lambda: c.attend(0, q[:, :, :n], 1.0),
+                         lambda: c.attend_sparse(0, q[:, :, :n], 1.0, 4)):
+                with pytest.raises(error[0], match=error[1]):
+                    call()
+
+    check([3, 0, 1], 3)
+    check(2, 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        c.extend(1)
+        c.attend(0, q[:, :, 0], 1.0)
+    c.extend(2)
+    with pytest.raises(ValueError, match="the step has 2"):
+        c.attend(0, q[:, :, 0], 1.0)
+    c.truncate([1, 1, 1])   # no step is open: nothing of a query is attended, nothing is written
+    for call in (lambda: c.write(0, k, k), lambda: c.attend(0, q, 1.0)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
