@@ -236,7 +236,8 @@ class Int4KVCache:
 
     def release(self, seqs=None) -> None:
         """Empty the sequences ``seqs`` (default: all) and return their pages."""
-        for b in range(self.batch) if seqs is None else seqs:
+        every = range(self.batch)
+        for b in every if seqs is None else [every[s] for s in seqs]:   # all are looked up before the first is emptied
             for j in range(int(self._owned[b]) - 1, -1, -1):
                 self._free.append(int(self._table[b, j]))
             self._table[b, :] = -1

@@ -48,3 +48,17 @@ def test_cache_refuses_fewer_tokens_than_the_step_has(cpu_cache):  # noqa: F811
     for call in (lambda: c.write(0, k, k), lambda: c.attend(0, q, 1.0)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_release_of_a_sequence_that_is_not_there_changes_nothing(cpu_cache):  # noqa: F811
+    c = cpu_cache
+    c.extend([65, 10, 3])
+    table, start = c.page_table.clone(), c.start.clone()
+    for seqs in ([0, 3], [1, -4], [0, 1, "2"], [0, None]):
+        with pytest.raises((IndexError, TypeError)):
+            c.release(seqs)
+        assert c.free_pages == 4 and c.lengths.tolist() == [65, 10, 3]
+        assert torch.equal(c.page_table, table) and torch.equal(c.start, start)
+    c.release([0, 0, -1])   # twice, and from the end
+    assert c.free_pages == 7 and c.lengths.tolist() == [0, 10, 0] and c.end.tolist() == [0, 10, 0]
+    assert (c.page_table[0] == -1).all() and int((c.page_table >= 0).sum()) == 1
