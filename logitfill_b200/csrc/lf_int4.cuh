@@ -83,5 +83,9 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 
 // Checks the C ABI's pool and copies it for a kernel (lf_int4_write.cu).
 int check_int4_pool(const char* what, const lf_int4_pool& pool, int head_dim, Int4Pool& out);
+// lf_int4_select's checks alone, and the call itself for the queries times sign (1 or
+// -1) (lf_int4_select.cu).
+int check_int4_select(const lf_int4_query* a);
+int int4_select_pages(const lf_int4_query* a, float sign, cudaStream_t stream);
 
 }  // namespace lf

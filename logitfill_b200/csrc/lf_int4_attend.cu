@@ -69,6 +69,7 @@ struct AttendParams {
   float* partials;
   uint32_t* tickets;
   int32_t* status;
+  int sms;  // of the device (for the launch)
 };
 
 constexpr int kTile = 16;             // tokens of one tensor-core step
@@ -960,7 +961,7 @@ static size_t partial_bytes(int sms) {
 }
 
 template <typename T, int D, int NT, bool kSparse>
-static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
+static int launch_attend(AttendParams p, cudaStream_t stream) {
   using C = AttendCfg<D, NT>;
   const void* kern = reinterpret_cast<const void*>(int4_attend_kernel<T, D, NT, kSparse>);
   cudaError_t err = raise_smem_limit(kern, C::kSmem, true);
@@ -971,7 +972,7 @@ static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
   // No more CTAs than ranges there can be.
   const int64_t units = static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles;
   const int64_t pages = units * (kSparse ? p.slots : p.pool.table_width);
-  const int64_t ranges = (pages + units * kUnitCost + kMinPages - 1) / kMinPages, slots = static_cast<int64_t>(sms) * C::kCtas;
+  const int64_t ranges = (pages + units * kUnitCost + kMinPages - 1) / kMinPages, slots = static_cast<int64_t>(p.sms) * C::kCtas;
   void* args[] = {&p};
   err = launch_programmatic(kern, dim3(static_cast<unsigned>(ranges < slots ? ranges : slots)), dim3(C::kThreads), C::kSmem,
                             stream, args);
@@ -987,10 +988,10 @@ static int launch_attend(AttendParams p, int sms, cudaStream_t stream) {
 // (now 26.4 and 34.8).  Four column tiles in one at D 64 do not pay: 25 columns of
 // drafts 28.2 us, 25.2 in two tiles of 16.
 template <typename T, int D>
-static int launch_attend_by(const AttendParams& p, int sms, cudaStream_t stream) {
+static int launch_attend_by(const AttendParams& p, cudaStream_t stream) {
   if (p.cols <= 8)
-    return p.picked ? launch_attend<T, D, 1, true>(p, sms, stream) : launch_attend<T, D, 1, false>(p, sms, stream);
-  return p.picked ? launch_attend<T, D, 2, true>(p, sms, stream) : launch_attend<T, D, 2, false>(p, sms, stream);
+    return p.picked ? launch_attend<T, D, 1, true>(p, stream) : launch_attend<T, D, 1, false>(p, stream);
+  return p.picked ? launch_attend<T, D, 2, true>(p, stream) : launch_attend<T, D, 2, false>(p, stream);
 }
 static int tile_columns(int cols) { return cols <= 8 ? 8 : 16; }
 
@@ -1007,10 +1008,12 @@ extern "C" size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int 
   return lf::partial_bytes(lf::sm_count()) + (static_cast<size_t>(units) * 4 + 15) / 16 * 16;
 }
 
-extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
+namespace lf {
+
+// Checks the arguments and fills p; launches nothing.
+static int check_attend(const lf_int4_query* a, AttendParams& p) {
   LF_CHECK_ARG(a != nullptr, "lf_int4_attend: null arguments");
-  lf::AttendParams p;
-  const int bad = lf::check_int4_pool("lf_int4_attend", a->pool, a->head_dim, p.pool);
+  const int bad = check_int4_pool("lf_int4_attend", a->pool, a->head_dim, p.pool);
   if (bad != LF_OK) return bad;
   LF_CHECK_ARG(a->q && a->lengths && a->out, "lf_int4_attend: null pointer");
   LF_CHECK_SUPPORTED(a->dtype == LF_F16 || a->dtype == LF_BF16, "lf_int4_attend: dtype %d (fp16 or bf16)", a->dtype);
@@ -1024,8 +1027,11 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&
                    (a->out_seq_stride | a->out_head_stride | a->out_tok_stride) % 4 == 0,
                "lf_int4_attend: output rows must be 8-byte aligned");
-  const int sms = lf::sm_count();
-  if (sms <= 0) return lf::launch_status("lf_int4_attend");
+  p.sms = sm_count();
+  if (p.sms <= 0) {
+    set_error("lf_int4_attend: the current device's SMs cannot be counted");
+    return LF_ERR_CUDA;
+  }
   LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
                    a->workspace_bytes >= lf_int4_workspace_bytes(p.pool.batch, p.pool.kv_heads, a->n_q, a->q_len, a->head_dim),
                "lf_int4_attend: workspace of %zu bytes is missing, misaligned or too small", a->workspace_bytes);
@@ -1046,17 +1052,35 @@ extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
   p.out_tok = a->out_tok_stride;
   p.rows = sparse ? p.pool.batch * a->q_len : p.pool.batch;
   p.cols = sparse ? p.group : p.group * a->q_len;
-  p.col_tiles = (p.cols + lf::tile_columns(p.cols) - 1) / lf::tile_columns(p.cols);
+  p.col_tiles = (p.cols + tile_columns(p.cols) - 1) / tile_columns(p.cols);
   LF_CHECK_SUPPORTED(static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles <=
-                         (1 << 30) / ((sparse ? a->slots : p.pool.table_width) + lf::kUnitCost),
+                         (1 << 30) / ((sparse ? a->slots : p.pool.table_width) + kUnitCost),
                      "lf_int4_attend: %d sequences of %d pages are too many for one call", p.pool.batch,
                      p.pool.table_width);
   p.partials = static_cast<float*>(a->workspace);
-  p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + lf::partial_bytes(sms));
+  p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + partial_bytes(p.sms));
   p.status = a->status;
+  return LF_OK;
+}
+
+static int launch_attend(const lf_int4_query* a, const AttendParams& p, lf_stream_t stream) {
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == LF_F16)
-    return a->head_dim == 128 ? lf::launch_attend_by<__half, 128>(p, sms, s) : lf::launch_attend_by<__half, 64>(p, sms, s);
-  return a->head_dim == 128 ? lf::launch_attend_by<__nv_bfloat16, 128>(p, sms, s)
-                            : lf::launch_attend_by<__nv_bfloat16, 64>(p, sms, s);
+  if (a->dtype == LF_F16) return a->head_dim == 128 ? launch_attend_by<__half, 128>(p, s) : launch_attend_by<__half, 64>(p, s);
+  return a->head_dim == 128 ? launch_attend_by<__nv_bfloat16, 128>(p, s) : launch_attend_by<__nv_bfloat16, 64>(p, s);
+}
+
+}  // namespace lf
+
+extern "C" int lf_int4_attend(const lf_int4_query* a, lf_stream_t stream) {
+  lf::AttendParams p;
+  const int bad = lf::check_attend(a, p);
+  return bad != LF_OK ? bad : lf::launch_attend(a, p, stream);
+}
+
+extern "C" int lf_int4_attend_sparse(const lf_int4_query* a, lf_stream_t stream) {
+  lf::AttendParams p;
+  int bad = lf::check_int4_select(a);
+  if (bad == LF_OK) bad = lf::check_attend(a, p);
+  if (bad == LF_OK) bad = lf::int4_select_pages(a, a->scaling < 0.0f ? -1.0f : 1.0f, reinterpret_cast<cudaStream_t>(stream));
+  return bad != LF_OK ? bad : lf::launch_attend(a, p, stream);
 }

@@ -307,20 +307,18 @@ static int launch_select(SelectParams p, cudaStream_t stream) {
   return launch_status("lf_int4_select");
 }
 
-}  // namespace lf
-
-// The choice for the queries times sign.
-static int select_pages(const lf_int4_query* a, float sign, lf_stream_t stream) {
-  lf::SelectParams p;
+// Checks the arguments and fills p; launches nothing.
+static int check_select(const lf_int4_query* a, float sign, SelectParams& p) {
+  LF_CHECK_ARG(a != nullptr, "lf_int4_select: null arguments");
   p.sign = sign;
-  const int bad = lf::check_int4_pool("lf_int4_select", a->pool, a->head_dim, p.pool);
+  const int bad = check_int4_pool("lf_int4_select", a->pool, a->head_dim, p.pool);
   if (bad != LF_OK) return bad;
   LF_CHECK_ARG(a->q && a->bounds && a->lengths && a->picked, "lf_int4_select: null pointer");
   LF_CHECK_SUPPORTED(a->dtype == LF_F16 || a->dtype == LF_BF16, "lf_int4_select: query dtype %d (fp16 or bf16)", a->dtype);
   LF_CHECK_ARG(a->q_len > 0 && a->q_len <= 65535 && a->n_q > 0 && a->n_q % p.pool.kv_heads == 0,
                "lf_int4_select: q_len %d, %d query heads on %d KV heads", a->q_len, a->n_q, p.pool.kv_heads);
   p.group = a->n_q / p.pool.kv_heads;
-  LF_CHECK_SUPPORTED(p.group <= lf::kMaxGroup, "lf_int4_select: %d query heads per KV head (%d at most)", p.group, lf::kMaxGroup);
+  LF_CHECK_SUPPORTED(p.group <= kMaxGroup, "lf_int4_select: %d query heads per KV head (%d at most)", p.group, kMaxGroup);
   LF_CHECK_ARG(a->sink_pages >= 0 && a->recent_pages >= 1 && a->slots <= (1 << 24) &&
                    static_cast<int64_t>(a->sink_pages) + a->recent_pages <= a->slots,
                "lf_int4_select: sink %d, recent %d of %d pages (recent at least 1)", a->sink_pages, a->recent_pages,
@@ -331,8 +329,8 @@ static int select_pages(const lf_int4_query* a, float sign, lf_stream_t stream) 
                "lf_int4_select: bounds records must be 8-byte aligned");
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->q) & 15) == 0 && (a->q_seq_stride | a->q_head_stride | a->q_tok_stride) % 8 == 0,
                "lf_int4_select: query rows must be 16-byte aligned");
-  LF_CHECK_SUPPORTED(p.pool.table_width <= lf::kMaxSelectPages, "lf_int4_select: %d pages per sequence (%d at most)",
-                     p.pool.table_width, lf::kMaxSelectPages);
+  LF_CHECK_SUPPORTED(p.pool.table_width <= kMaxSelectPages, "lf_int4_select: %d pages per sequence (%d at most)",
+                     p.pool.table_width, kMaxSelectPages);
   p.q = a->q;
   p.q_seq = a->q_seq_stride;
   p.q_head = a->q_head_stride;
@@ -348,19 +346,24 @@ static int select_pages(const lf_int4_query* a, float sign, lf_stream_t stream) 
   p.recent = a->recent_pages;
   p.picked = a->picked;
   p.status = a->status;
-  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == LF_F16)
-    return a->head_dim == 128 ? lf::launch_select<__half, 128>(p, s) : lf::launch_select<__half, 64>(p, s);
-  return a->head_dim == 128 ? lf::launch_select<__nv_bfloat16, 128>(p, s) : lf::launch_select<__nv_bfloat16, 64>(p, s);
+  return LF_OK;
 }
+
+int check_int4_select(const lf_int4_query* a) {
+  SelectParams p;
+  return check_select(a, 1.0f, p);
+}
+
+int int4_select_pages(const lf_int4_query* a, float sign, cudaStream_t s) {
+  SelectParams p;
+  const int bad = check_select(a, sign, p);
+  if (bad != LF_OK) return bad;
+  if (a->dtype == LF_F16) return a->head_dim == 128 ? launch_select<__half, 128>(p, s) : launch_select<__half, 64>(p, s);
+  return a->head_dim == 128 ? launch_select<__nv_bfloat16, 128>(p, s) : launch_select<__nv_bfloat16, 64>(p, s);
+}
+
+}  // namespace lf
 
 extern "C" int lf_int4_select(const lf_int4_query* a, lf_stream_t stream) {
-  LF_CHECK_ARG(a != nullptr, "lf_int4_select: null arguments");
-  return select_pages(a, 1.0f, stream);
-}
-
-extern "C" int lf_int4_attend_sparse(const lf_int4_query* a, lf_stream_t stream) {
-  LF_CHECK_ARG(a != nullptr, "lf_int4_attend_sparse: null arguments");
-  const int bad = select_pages(a, a->scaling < 0.0f ? -1.0f : 1.0f, stream);
-  return bad != LF_OK ? bad : lf_int4_attend(a, stream);
+  return lf::int4_select_pages(a, 1.0f, reinterpret_cast<cudaStream_t>(stream));
 }

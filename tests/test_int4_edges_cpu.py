@@ -4,8 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from logitfill_b200 import int4
-from tests.test_int4_cpu import cpu_cache  # noqa: F401  (a fixture)
+from logitfill_b200 import _lib, int4
+from tests.test_int4_cpu import _query, cpu_cache  # noqa: F401  (cpu_cache: a fixture)
 
 
 def test_pools_without_pages_heads_or_sequences_are_refused():
@@ -62,3 +62,13 @@ def test_release_of_a_sequence_that_is_not_there_changes_nothing(cpu_cache):  # 
     c.release([0, 0, -1])   # twice, and from the end
     assert c.free_pages == 7 and c.lengths.tolist() == [0, 10, 0] and c.end.tolist() == [0, 10, 0]
     assert (c.page_table[0] == -1).all() and int((c.page_table >= 0).sum()) == 1
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are made up: nothing may be launched")
+@pytest.mark.parametrize("wrong", [dict(out=0), dict(os=(512, 62, 64)), dict(scaling=float("nan")), dict(slots=3, sink=1, recent=1, out=0)])
+def test_a_sparse_call_is_checked_before_its_first_launch(wrong):
+    """What only the attention refuses is refused before the choice of pages runs (whose
+    launch would fail here in another way)."""
+    so = _lib.lib()
+    assert so.lf_int4_attend_sparse(_query(**wrong), None) == _lib.LF_ERR_INVALID_ARGUMENT
+    assert b"lf_int4_attend" in so.lf_last_error()
