@@ -993,7 +993,7 @@ static int launch_attend_by(const AttendParams& p, cudaStream_t stream) {
     return p.picked ? launch_attend<T, D, 1, true>(p, stream) : launch_attend<T, D, 1, false>(p, stream);
   return p.picked ? launch_attend<T, D, 2, true>(p, stream) : launch_attend<T, D, 2, false>(p, stream);
 }
-static int tile_columns(int cols) { return cols <= 8 ? 8 : 16; }
+static int tile_columns(int64_t cols) { return cols <= 8 ? 8 : 16; }
 
 }  // namespace lf
 
@@ -1027,6 +1027,14 @@ static int check_attend(const lf_int4_query* a, AttendParams& p) {
   LF_CHECK_ARG((reinterpret_cast<uintptr_t>(a->out) & 7) == 0 &&
                    (a->out_seq_stride | a->out_head_stride | a->out_tok_stride) % 4 == 0,
                "lf_int4_attend: output rows must be 8-byte aligned");
+  const int64_t group = a->n_q / p.pool.kv_heads;
+  const int64_t rows = sparse ? static_cast<int64_t>(p.pool.batch) * a->q_len : p.pool.batch;
+  const int64_t cols = sparse ? group : group * a->q_len;
+  const int64_t per_tile = tile_columns(cols), col_tiles = (cols + per_tile - 1) / per_tile;
+  const int64_t pages = sparse ? a->slots : p.pool.table_width;
+  LF_CHECK_SUPPORTED(rows * p.pool.kv_heads <= (1 << 30) / (pages + kUnitCost) / col_tiles && cols <= (1 << 30),
+                     "lf_int4_attend: %d sequences of %lld pages are too many for one call", p.pool.batch,
+                     static_cast<long long>(pages));
   p.sms = sm_count();
   if (p.sms <= 0) {
     set_error("lf_int4_attend: the current device's SMs cannot be counted");
@@ -1040,7 +1048,10 @@ static int check_attend(const lf_int4_query* a, AttendParams& p) {
   p.q_head = a->q_head_stride;
   p.q_tok = a->q_tok_stride;
   p.q_len = a->q_len;
-  p.group = a->n_q / p.pool.kv_heads;
+  p.group = static_cast<int>(group);
+  p.rows = static_cast<int>(rows);
+  p.cols = static_cast<int>(cols);
+  p.col_tiles = static_cast<int>(col_tiles);
   p.lengths = a->lengths;
   p.counts = a->counts;
   p.picked = a->picked;
@@ -1050,13 +1061,6 @@ static int check_attend(const lf_int4_query* a, AttendParams& p) {
   p.out_seq = a->out_seq_stride;
   p.out_head = a->out_head_stride;
   p.out_tok = a->out_tok_stride;
-  p.rows = sparse ? p.pool.batch * a->q_len : p.pool.batch;
-  p.cols = sparse ? p.group : p.group * a->q_len;
-  p.col_tiles = (p.cols + tile_columns(p.cols) - 1) / tile_columns(p.cols);
-  LF_CHECK_SUPPORTED(static_cast<int64_t>(p.rows) * p.pool.kv_heads * p.col_tiles <=
-                         (1 << 30) / ((sparse ? a->slots : p.pool.table_width) + kUnitCost),
-                     "lf_int4_attend: %d sequences of %d pages are too many for one call", p.pool.batch,
-                     p.pool.table_width);
   p.partials = static_cast<float*>(a->workspace);
   p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + partial_bytes(p.sms));
   p.status = a->status;

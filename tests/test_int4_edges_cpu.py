@@ -72,3 +72,10 @@ def test_a_sparse_call_is_checked_before_its_first_launch(wrong):
     so = _lib.lib()
     assert so.lf_int4_attend_sparse(_query(**wrong), None) == _lib.LF_ERR_INVALID_ARGUMENT
     assert b"lf_int4_attend" in so.lf_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are made up: nothing may be launched")
+@pytest.mark.parametrize("large", [dict(batch=65535, q_len=65535), dict(n_q=1 << 30, q_len=65535), dict(batch=65535, table_width=1 << 20, table_stride=1 << 20, picked=0),
+                                   dict(slots=(1 << 31) - 1)])
+def test_sizes_whose_products_pass_32_bits_are_refused(large):
+    assert _lib.lib().lf_int4_attend(_query(**large), None) == _lib.LF_ERR_UNSUPPORTED
