@@ -10,7 +10,6 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblogitfill_b200.so"
-BINDING_PATH = LIB_PATH.with_name("int4_binding.so")
 
 (LF_OK, LF_ERR_INVALID_ARGUMENT, LF_ERR_UNSUPPORTED, LF_ERR_LAUNCH, LF_ERR_DEVICE_TIMEOUT, LF_ERR_OUT_OF_RANGE,
  LF_ERR_CUDA) = range(7)
@@ -115,15 +114,16 @@ def int4_binding():
     global _BINDING
     if _BINDING is None:
         lib()
-        if not BINDING_PATH.exists():
-            raise RuntimeError(
-                f"logitfill_b200 binding missing at {BINDING_PATH}; build it with "
-                "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
         import importlib.util
 
-        import torch  # noqa: F401  (its libraries are the binding's)
+        from logitfill_b200.build import binding_path
 
-        spec = importlib.util.spec_from_file_location("int4_binding", BINDING_PATH)
+        path = binding_path()   # (imports torch, whose libraries are the binding's)
+        if not path.exists():
+            raise RuntimeError(
+                f"logitfill_b200 binding missing at {path}; build it with "
+                "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
+        spec = importlib.util.spec_from_file_location("int4_binding", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         _BINDING = module

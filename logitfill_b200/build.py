@@ -20,7 +20,6 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB_NAME = "liblogitfill_b200.so"
-BINDING_NAME = "int4_binding.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -35,9 +34,19 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
+def binding_path() -> Path:
+    """The binding for this Python and this torch, whose C++ classes it is compiled
+    against: both are in the name."""
+    import sysconfig
+
+    import torch
+
+    return OUT_DIR / f"int4_binding.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
+
+
 def build_binding(verbose: bool = False, force: bool = False) -> Path:
     """g++ of the 4-bit cache's Python binding, linked to torch and the library."""
-    src, out, lib = CSRC / "int4_binding.cpp", OUT_DIR / BINDING_NAME, OUT_DIR / LIB_NAME
+    src, out, lib = CSRC / "int4_binding.cpp", binding_path(), OUT_DIR / LIB_NAME
     deps = (src, ROOT / "include" / "logitfill_b200.h", Path(__file__))
     if not force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return out

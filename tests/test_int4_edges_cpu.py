@@ -79,3 +79,14 @@ def test_a_sparse_call_is_checked_before_its_first_launch(wrong):
                                    dict(slots=(1 << 31) - 1)])
 def test_sizes_whose_products_pass_32_bits_are_refused(large):
     assert _lib.lib().lf_int4_attend(_query(**large), None) == _lib.LF_ERR_UNSUPPORTED
+
+
+def test_a_binding_of_another_torch_is_not_loaded(monkeypatch):
+    """It is compiled against torch's C++ classes: for another version there is none,
+    however old the file is."""
+    monkeypatch.setattr(_lib, "_BINDING", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0+none")
+    with pytest.raises(RuntimeError, match="binding missing"):
+        _lib.int4_binding()
+    monkeypatch.undo()
+    assert _lib.int4_binding() is _lib.int4_binding()
