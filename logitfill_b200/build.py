@@ -1,6 +1,7 @@
 """Build the sm_100a C-ABI library in-tree (``logitfill_b200/_lib/``).
 
-    python -m logitfill_b200.build          # or __graft_entry__.build()
+    python -m logitfill_b200.build                 # or __graft_entry__.build()
+    python logitfill_b200/build.py --library       # the C library alone: needs no torch
 
 nvcc cross-compiles for B200 without a GPU.  The shared library links the
 CUDA runtime statically and exports only the ``lf_*`` symbols declared in
@@ -80,6 +81,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
 
 
 def build_library(verbose: bool = False, force: bool = False) -> Path:
+    """Build the C library, which needs nvcc and its host compiler only."""
     OUT_DIR.mkdir(exist_ok=True)
     out = OUT_DIR / LIB_NAME
     srcs = sources()
@@ -118,5 +120,5 @@ def build_library(verbose: bool = False, force: bool = False) -> Path:
 
 
 if __name__ == "__main__":
-    path = build(verbose="-v" in sys.argv, force="-f" in sys.argv)
-    print(path)
+    make = build_library if "--library" in sys.argv else build
+    print(make(verbose="-v" in sys.argv, force="-f" in sys.argv))

@@ -1,6 +1,11 @@
 """CPU tests of the 4-bit cache's refusals and bookkeeping at the edges."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -90,3 +95,15 @@ def test_a_binding_of_another_torch_is_not_loaded(monkeypatch):
         _lib.int4_binding()
     monkeypatch.undo()
     assert _lib.int4_binding() is _lib.int4_binding()
+
+
+def test_the_library_builds_without_torch(tmp_path):
+    """A host that links the C library alone has neither torch nor its headers."""
+    (tmp_path / "torch.py").write_text("raise ImportError('no torch here')\n")
+    script = Path(_lib.__file__).with_name("build.py")
+    env = dict(os.environ, PYTHONPATH=str(tmp_path))
+    done = subprocess.run([sys.executable, str(script), "--library"], env=env, capture_output=True, text=True, timeout=900)
+    assert done.returncode == 0, done.stderr
+    assert done.stdout.split() == [str(_lib.LIB_PATH)]
+    done = subprocess.run([sys.executable, str(script)], env=env, capture_output=True, text=True, timeout=900)
+    assert done.returncode != 0 and "no torch here" in done.stderr   # the binding needs it
