@@ -341,8 +341,10 @@ LF_API int lf_gather_wait(uint32_t* flags, int layer, uint32_t expected, uint64_
  *           of word b * D + g * D/8 + t * D/32 + o * D/64 + w
  *   parameters: word k * D/32 + G, s in the low half, z in the high half
  * The page table gives sequence b's logical page j as pool page
- * table[b * table_stride + j]; sequences may share pages.  An entry outside
- * [0, n_pages) is never followed: the tokens there are skipped (written
+ * table[b * table_stride + j]; sequences may share pages that are not written any
+ * more (a common prefix): a page that a call writes to belongs to one of its
+ * sequences only, else two would store the same record, and its bounds, in no order.
+ * An entry outside [0, n_pages) is never followed: the tokens there are skipped (written
  * nowhere, read as zero, not attended) and LF_ERR_OUT_OF_RANGE goes to *status
  * (device int32, may be NULL).
  *

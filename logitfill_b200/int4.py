@@ -19,10 +19,12 @@ in 64-token pages that a page table orders into sequences.
 The functions take the tensors themselves: ``pages`` int32 ``[n_pages, n_kv,
 20 * head_dim]`` (see ``include/logitfill_b200.h`` for the record),
 ``page_table`` int32 ``[batch, width]``, lengths and positions int32
-``[batch]``, all on the GPU.  A page table entry outside the pool is never
-followed; with ``status`` (int32 ``[1]`` on the GPU) given, such an access sets
-it to a non-zero ``lf_status``.  Every launch goes to the current stream.
-There is no CPU or dense fallback; what the kernels do not implement raises
+``[batch]``, all on the GPU.  Sequences may share pages that are not written
+any more (a common prefix); a page that a call writes belongs to one of its
+sequences.  A page table entry outside the pool is never followed; with
+``status`` (int32 ``[1]`` on the GPU) given, such an access sets it to a
+non-zero ``lf_status``.  Every launch goes to the current stream.  There is no
+CPU or dense fallback; what the kernels do not implement raises
 ``NotImplementedError``, malformed arguments ``ValueError``.
 """
 from __future__ import annotations

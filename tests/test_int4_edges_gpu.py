@@ -8,7 +8,7 @@ import torch
 
 from logitfill_b200 import int4
 from tests import int4_reference as ref
-from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _garbage, _i32, _picks, _table
+from tests.test_int4_gpu import BF16, F16, ROUND, _dense_reference, _filled, _garbage, _i32, _kv, _picks, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +218,30 @@ def test_scores_that_are_all_far_below_zero(D, nq):
     q = (-(torch.rand(1, nq, 1, D, generator=g) + 0.5) * 2.0 ** 110).to(BF16).cuda()
     got = int4.int4_attention(q, pages, table, _i32([T]), 0.125)
     _check(got, *_dense_reference(q, [T], [1], sk, sv, 0.125), BF16, 2.0 ** -24)
+
+
+# ------------------------------------------------------------ shared pages
+
+@pytest.mark.parametrize("q_len", [1, 3])
+def test_sequences_that_share_a_prefix(q_len):
+    """Two sequences whose first pages are the same pool pages, each with its own tail."""
+    D, H, nq, shared, lengths = 128, 2, 14, 5, [5 * 64 + 70, 5 * 64 + 9]
+    table, n = _table(2, 2, 7)
+    table[1, :shared] = table[0, :shared]
+    pages, bounds = _garbage(n, H, D), int4.alloc_bounds(n, H, D)
+    k, v = _kv(3, 2, H, max(lengths), D)
+    k[1, :, :shared * 64], v[1, :, :shared * 64] = k[0, :, :shared * 64], v[0, :, :shared * 64]
+    # the prefix through one of its owners, then both tails
+    int4.int4_write(k[:1, :, :shared * 64], v[:1, :, :shared * 64], pages, table[:1], _i32([0]), bounds=bounds)
+    int4.int4_write(k[:, :, shared * 64:], v[:, :, shared * 64:], pages, table, _i32([shared * 64] * 2),
+                    _i32([m - shared * 64 for m in lengths]), bounds=bounds)
+    sk, sv = ref.stored(k.double().cpu().numpy()), ref.stored(v.double().cpu().numpy())
+    gk, gv = int4.int4_read(pages, table, _i32([0, 0]), min(lengths))
+    assert np.array_equal(gk.cpu().numpy(), sk[:, :, :min(lengths)]) and np.array_equal(gv.cpu().numpy(), sv[:, :, :min(lengths)])
+    q = _queries(1, 2, nq, q_len, D)
+    got = int4.int4_attention(q, pages, table, _i32(lengths), D ** -0.5)
+    _check(got, *_dense_reference(q, lengths, [q_len] * 2, sk, sv, D ** -0.5), BF16, 2.0 ** -24)
+    got, picked = int4.int4_sparse_attention(q, pages, bounds, table, _i32(lengths), D ** -0.5, 2, 1, 1)
+    want = _picks(q, sk, lengths, [q_len] * 2, 2, 1, 1)
+    assert np.array_equal(picked.cpu().numpy(), want)
+    _check(got, *_dense_reference(q, lengths, [q_len] * 2, sk, sv, D ** -0.5, want), BF16, 2.0 ** -24)
