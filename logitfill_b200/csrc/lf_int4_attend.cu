@@ -20,14 +20,14 @@
 // keep fewer bits: fp16 ends at steps of 2^-24.  So that a dominant token does not
 // press the rest of its warp's tokens below that, the largest weight is put at 2^7
 // and not at 1: what is lost of a weight is then 2^-32 of the warp's largest at most.
-// A Value group that may pass the fp16 range stays out of the product and gets one of
-// its own, at 1/32 (add_apart).
+// A Value group that may pass the fp16 range stays out of the product and is added in
+// fp32 at the end (add_apart).
 //
 // The work is one pass over the pages with a running maximum and sum.  The
 // maximum is moved only when a score passes it by 2^8 (p <= 2^15 fits), so most
-// tiles skip the rescaling.  It is kept in the scores' own units and enters as what
-// the minima's product starts from: scores come out relative to it, and no rounding of
-// a large product of score and scaling reaches the exponent.
+// tiles skip the rescaling.  It is kept in the units of the codes' products, whose sum
+// starts from it: scores come out relative to it, and no rounding of a large product
+// of score and scaling reaches the exponent.
 //
 // Split.  All pages of all units form one line, cut into equal ranges, one per
 // CTA (the lengths are read on the device, so nothing is planned on the host).
@@ -125,11 +125,10 @@ __device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// From one number per column.
-__device__ __forceinline__ void mma1688_from(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0, float from0, float from1) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%7,%8};"
+__device__ __forceinline__ void mma1688_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(b0), "f"(from0), "f"(from1));
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -197,12 +196,6 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[kWor
     w[0] = x.x; w[1] = x.y;
   }
 }
-// Bit i: token i of 32, where lanes 2 x and 2 x + 1 hold flags of tokens 2 x and 2 x + 1.
-__device__ __forceinline__ uint32_t token_bits(bool even, bool odd) {
-  const uint32_t e = __ballot_sync(0xffffffffu, even), o = __ballot_sync(0xffffffffu, odd);
-  return ((e | e >> 1) & 0x55555555u) | ((o | o << 1) & 0xAAAAAAAAu);
-}
-
 // Weights of 16 tokens (pr, spent: rows g and g + 8 of the scores' fragments) as the
 // product's B operand, columns by tokens, in kTerms fp16 numbers.
 template <int kTerms>
@@ -246,83 +239,6 @@ __device__ __forceinline__ void add_values(float (&acc)[NT][D / 16][4], int G, c
     }
 }
 
-// A warp's sums, weights (fragment order) and visible tokens, for add_apart.
-template <int D, int NT> struct Apart {
-  float acc[NT][D / 16][4], w[NT][kSubs][4];
-  int vis[NT][2];
-};
-// Value groups that stay out of the product; `apart` has the tokens of the part that
-// have some.  NaN ones that only some columns see become NaN in the sums of those.
-// Those that may pass the fp16 range are multiplied at 1/32, the others' parameters 0:
-// scaled together, the small groups would lose their low bits.  (A Value of such a
-// group, whose step is 2^11 or whose minimum 2^15, is right to 2^-20 or 2^-11 of itself.)
-// The parameters are the record's: the pairs in shared memory hold 0 for these
-// groups.  A call of its own on copies: the registers it takes in the loop cost the usual
-// half pages 1 % at D 128, 5 % with 16 columns.  8 x 32k tokens, 28 heads on 4, D 128,
-// take 104 us with such a group in every token, 89 in every 64th, 42 in none (in fp32,
-// token by token: 1071 and 90).
-template <typename T, int D, int NT>
-__device__ __noinline__ void add_apart(const AttendParams& p, int h, int b, uint32_t apart, int base, int vis_min,
-                                       const uint8_t* vcode, Apart<D, NT>& s) {
-  constexpr int kG = D / kInt4Group, kTerms = kWeightTerms<T>;
-  const int lane = threadIdx.x & 31, t = lane & 3, tok = base + lane;
-  uint32_t par[kG];  // the lane's token's
-#pragma unroll
-  for (int G = 0; G < kG; ++G) par[G] = 0;
-  if (apart >> lane & 1) {
-    const int id = int4_page_id(p.pool, b, tok / kInt4Page);  // known to be there
-    load_words<kG>(reinterpret_cast<const uint8_t*>(p.pool.words + int4_record(p.pool, id, h) + 18 * D +
-                                                    tok % kInt4Page * kG), par);
-  }
-  bool wide = false;
-#pragma unroll
-  for (int G = 0; G < kG; ++G) {
-    const uint32_t nan = __ballot_sync(0xffffffffu, tok >= vis_min && is_nan_param(par[G]));
-    const int first = nan != 0 ? base + __ffs(nan) - 1 : INT32_MAX;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (first < s.vis[nt][k & 1]) s.acc[nt][2 * G][k] = s.acc[nt][2 * G + 1][k] = NAN;
-    if (!is_wide_param(par[G])) par[G] = 0;
-    wide |= par[G] != 0;
-  }
-  if (!__any_sync(0xffffffffu, wide)) return;
-  float acc[NT][2 * kG][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[nt][y][k] = s.acc[nt][y][k] * 0.03125f;
-#pragma unroll 1
-  for (int sub = 0; sub < kSubs; ++sub) {
-    uint32_t pb[NT][kTerms][2], vw[2][kG];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) weight_operand<kTerms>(s.w[nt][sub], pb[nt]);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) load_words<kG>(vcode + (2 * sub + r) * (4 * D) + lane * (4 * kG), vw[r]);
-#pragma unroll
-    for (int G = 0; G < kG; ++G) {
-      uint32_t v[2][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int k = sub * kTile + 8 * r + 2 * t;
-        const uint32_t e = __shfl_sync(0xffffffffu, par[G], k), o = __shfl_sync(0xffffffffu, par[G], k + 1);
-        value_operand<kG>(vw[r], G, hmul2(__byte_perm(e, o, 0x5410), 0x28002800u), hmul2(__byte_perm(e, o, 0x7632), 0x28002800u),
-                          v[r]);
-      }
-      add_values<D>(acc, G, v, pb);
-    }
-  }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s.acc[nt][y][k] = acc[nt][y][k] * 32.0f;
-}
-
 // Adds 1 and returns what was there.  What the CTA wrote before the barrier ahead
 // of it is visible to whoever takes a later ticket.
 __device__ __forceinline__ uint32_t take_ticket(uint32_t* ticket) {
@@ -359,6 +275,81 @@ __device__ __forceinline__ int merge_pages(int total, int units) {
   return static_cast<int>(sqrtf(static_cast<float>(total / units) / 3.0f));
 }
 
+// A unit, as add_apart needs it.
+struct Unit {
+  int b, h, c0, i0, first, stop, length, count, seen_max, vis_min;
+  const int32_t* listed;  // pages of a sparse unit
+};
+// Value groups that stayed out of the products of a warp's pages, added in fp32 to its
+// sums in the merge buffer: those that may pass the fp16 range (scaled to fit it, they
+// would cost the small groups beside them their low bits), and NaN ones that only some
+// columns see.  It goes through the warp's pages again, token by token, with scores of
+// its own (top: the maxima that the sums are relative to, in log2).  Slow where there are
+// many: 8 x 32k tokens, 28 heads on 4, D 128, 42 us without any, 88 with one in every 64
+// tokens, 305 in every 4th, 940 in every one; a second product in the loop took 104 for
+// that, but cost the calls without any 3 %, for its registers.
+template <typename T, int D, int NT, bool kSparse>
+__device__ __noinline__ void add_apart(const AttendParams& p, const Unit& u, const int* vis, float* sums, const float* top) {
+  constexpr int kG = D / kInt4Group, kOwn = D / 32, kCol = 8 * NT, kPad = AttendCfg<D, NT>::kPad;
+  const int part = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31;
+  const int d = lane * kOwn, G = d / kInt4Group;  // the lane's channels: kOwn from d on
+  float q[kCol][kOwn];
+#pragma unroll
+  for (int col = 0; col < kCol; ++col) {
+    const int c = min(u.c0 + col, p.cols - 1), i = kSparse || p.q_len == 1 ? 0 : c / p.group;
+    const T* from = static_cast<const T*>(p.q) + u.b * p.q_seq + (u.h * p.group + c - i * p.group) * p.q_head +
+                    (u.i0 + i) * p.q_tok + d;
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) q[col][x] = Scalar<T>::load(from + x);
+  }
+#pragma unroll 1
+  for (int place = u.first + (threadIdx.x >> 6); place < u.stop; place += AttendCfg<D, NT>::kTeams) {
+    const int page = kSparse ? u.listed[place] : place;
+    if (page < 0 || page > (u.seen_max - 1) / kInt4Page) continue;  // (seen_max > 0: there was a group to add)
+    const int id = int4_page_id(p.pool, u.b, page), base = page * kInt4Page + part * kPart;
+    if (id < 0 || base >= u.seen_max) continue;
+    const uint32_t* rec = reinterpret_cast<const uint32_t*>(p.pool.words) + int4_record(p.pool, id, u.h);
+    bool apart = false;
+    if (base + lane < u.seen_max) {
+      uint32_t sz[kG];
+      load_words<kG>(reinterpret_cast<const uint8_t*>(rec + 18 * D + (part * kPart + lane) * kG), sz);
+#pragma unroll
+      for (int x = 0; x < kG; ++x) apart |= stays_apart(sz[x], base + lane, u.vis_min);
+    }
+#pragma unroll 1
+    for (uint32_t rest = __ballot_sync(0xffffffffu, apart); rest != 0; rest &= rest - 1) {
+      const int tok = base + __ffs(rest) - 1, k = tok % kInt4Page;
+      const uint32_t ksz = rec[8 * D + k * kG + G], vsz = rec[18 * D + k * kG + G];
+      const uint32_t kc = rec[k * (D / 8) + d % 32 / 8 * kG + G] >> (4 * (d % 8));
+      const uint32_t vc = rec[10 * D + (k >> 3) * D + d % 32 / 4 * (D / 8) + (k & 7) / 2 * kG + (k & 1) * (D / 64) + d / 64] >>
+                          (16 * (G & 1) + 4 * (d % 4));
+      float key[kOwn], value[kOwn], score[kCol];
+#pragma unroll
+      for (int x = 0; x < kOwn; ++x) {
+        key[x] = fmaf(static_cast<float>(kc >> (4 * x) & 15u), half_lo(ksz), half_hi(ksz));
+        value[x] = fmaf(static_cast<float>(vc >> (4 * x) & 15u), half_lo(vsz), half_hi(vsz));
+      }
+#pragma unroll
+      for (int col = 0; col < kCol; ++col) {
+        score[col] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kOwn; ++x) score[col] = fmaf(q[col][x], key[x], score[col]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) score[col] += __shfl_xor_sync(0xffffffffu, score[col], o);
+      }
+      if (stays_apart(vsz, tok, u.vis_min)) {
+#pragma unroll
+        for (int col = 0; col < kCol; ++col) {
+          if (tok >= vis[col]) continue;
+          const float w = ex2(fminf(fmaf(score[col], p.scale_log2, -top[col]), kSlack) + kLift);
+#pragma unroll
+          for (int x = 0; x < kOwn; ++x) sums[col * kPad + d + x] = fmaf(w, value[x], sums[col * kPad + d + x]);
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int D, int NT, bool kSparse>
 __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::kCtas)
     int4_attend_kernel(const __grid_constant__ AttendParams p) {
@@ -366,9 +357,12 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
   constexpr int kTerms = kWeightTerms<T>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];  // 128: 42.2 us at 16 bytes past that, 39.8 (8 x 32k, from Python)
   __shared__ int meta_s[kWarps][kStages];  // first token of each stage's part of a page, -1: nothing to do
   __shared__ int last_s;
+  __shared__ Unit unit_s;
+  __shared__ int vis_s[kWarps][kCol];  // tokens that each column sees
+  __shared__ int apart_s[kWarps];       // a Value group stayed out of the product
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = p.pool.kv_heads * p.col_tiles;
   grid_dep_wait();
@@ -495,7 +489,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     // Query fragments, sums and scales of this unit's columns.
     uint32_t qf[NT][2 * kG][2], qz[NT];
     float c2[NT][2];
-    int vis[NT][2];
+    int vis_min = INT32_MAX;
     const float flip = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -554,15 +548,16 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         // positive, so that a masked score's -inf stays one
         c2[nt][k] = fmaxf(pow2(10 - kc) * fabsf(p.scale_log2), 1e-36f);
         const int col = min(c0 + nt * 8 + 2 * t + k, p.cols - 1);
-        vis[nt][k] = int4_seen(length, count, i0 + token_of(col));
+        const int vis = int4_seen(length, count, i0 + token_of(col));
+        if (g == 0) vis_s[warp][nt * 8 + 2 * t + k] = vis;
+        vis_min = min(vis_min, vis);
       }
     }
-    int vis_min = INT32_MAX;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) vis_min = min(vis_min, min(vis[nt][0], vis[nt][1]));
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
-    float acc[NT][2 * kG][4], back[NT][2], l[NT][2];  // back: the running maxima, negated
+    if (tid == 0) unit_s = Unit{b, h, c0, i0, first, stop, length, count, seen_max, vis_min, listed};
+    if (lane == 0) apart_s[warp] = 0;
+    float acc[NT][2 * kG][4], back[NT][2], l[NT][2];  // back: the running maxima, negated, times 2^-14
     bool fresh = true;  // before the first part
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -591,7 +586,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
       // Value parameters in pairs of tokens, as the fragments take them: in place
       // of (s, z) of tokens 2 x and 2 x + 1 a lane writes (s, s'), (z, z').
-      uint32_t apart = 0;  // tokens with a Value group that stays out of the product (add_apart)
       {
         constexpr int kQ = kG / 2;  // groups of a lane: two lanes for each of the 16 pairs
         const int x = lane >> 1, q = lane & 1;
@@ -622,21 +616,14 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         }
         any_apart |= (most & 0x7FFFu) >= 0x7800u || (most & 0x7FFF0000u) >= 0x78000000u;  // 2^15: is_wide_param of one
         if (__any_sync(0xffffffffu, any_apart)) {
-          bool apart_e = false, apart_o = false;
+          if (lane == 0) apart_s[warp] = 1;
 #pragma unroll
           for (int k = 0; k < kQ; ++k) {
-            if (stays_apart(e[k], tok, vis_min)) {
-              apart_e = true;
-              e[k] = 0;
-            }
-            if (stays_apart(o[k], tok + 1, vis_min)) {
-              apart_o = true;
-              o[k] = 0;
-            }
+            if (stays_apart(e[k], tok, vis_min)) e[k] = 0;
+            if (stays_apart(o[k], tok + 1, vis_min)) o[k] = 0;
             s2[k] = __byte_perm(e[k], o[k], 0x5410);
             z2[k] = __byte_perm(e[k], o[k], 0x7632);
           }
-          apart = token_bits(apart_e, apart_o);
         }
         __syncwarp();  // every lane has read its words
         if constexpr (kQ == 2)
@@ -663,9 +650,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         float dot[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma1688_from(x[sub][nt], kz[0], kz[1], qz[nt], back[nt][0], back[nt][1]);
+          mma1688_zero(x[sub][nt], kz[0], kz[1], qz[nt]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) dot[nt][k] = 0.0f;
+          for (int k = 0; k < 4; ++k) dot[nt][k] = back[nt][k & 1];
         }
 #pragma unroll
         for (int G = 0; G < kG; ++G) {
@@ -699,7 +686,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k)
-                if (tok >= vis[nt][k]) x[sub][nt][2 * r + k] = -INFINITY;
+                if (tok >= vis_s[warp][nt * 8 + 2 * t + k]) x[sub][nt][2 * r + k] = -INFINITY;
           }
       }
 
@@ -727,7 +714,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             for (int o = 4; o < 32; o <<= 1) by = fmaxf(by, __shfl_xor_sync(0xffffffffu, by, o));
             if (!(by > (fresh ? -INFINITY : 0.0f))) by = 0.0f;
             fix[k] = fresh ? 1.0f : ex2(-by * c2[nt][k]);
-            back[nt][k] -= by;
+            back[nt][k] -= by * 0x1p-14f;
             l[nt][k] *= fix[k];
 #pragma unroll
             for (int sub = 0; sub < kSubs; ++sub) {
@@ -780,29 +767,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           add_values<D>(acc, G, v, pb);
         }
       }
-      if (apart != 0) {
-        Apart<D, NT> held;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) held.acc[nt][y][k] = acc[nt][y][k];
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) held.w[nt][sub][k] = ex2(fmaf(x[sub][nt][k], c2[nt][k & 1], kLift));
-#pragma unroll
-          for (int c = 0; c < 2; ++c) held.vis[nt][c] = vis[nt][c];
-        }
-        add_apart<T>(p, h, b, apart, base, vis_min, stage + kCodes, held);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int y = 0; y < 2 * kG; ++y)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[nt][y][k] = held.acc[nt][y][k];
-      }
     }
     cp_wait<0>();
     __syncthreads();  // the rings are free: the merge buffer takes their place
@@ -820,7 +784,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const int col = warp * kCol + nt * 8 + 2 * t + k;
         if (g == 0) {
-          top_w[col] = sum == 0.0f ? kNoMax : fmaxf(-back[nt][k] * c2[nt][k], kNoMax);
+          top_w[col] = sum == 0.0f ? kNoMax : fmaxf(-back[nt][k] * 16384.0f * c2[nt][k], kNoMax);
           sum_w[col] = sum;
         }
 #pragma unroll
@@ -828,6 +792,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           *reinterpret_cast<float4*>(merge + col * C::kPad + 32 * G + 4 * g) =
               make_float4(acc[nt][2 * G][k], acc[nt][2 * G][k + 2], acc[nt][2 * G + 1][k], acc[nt][2 * G + 1][k + 2]);
       }
+    __syncwarp();
+    if (apart_s[warp] != 0)
+      add_apart<T, D, NT, kSparse>(p, unit_s, vis_s[warp], merge + warp * kCol * C::kPad, top_w + warp * kCol);
     __syncthreads();
 
     const bool whole = first == 0 && stop == n_pages;
