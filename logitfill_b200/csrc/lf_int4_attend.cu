@@ -40,12 +40,13 @@
 // accumulator) and the last one to arrive (an atomic ticket) merges them in the
 // order of the ranges, so results do not depend on timing.
 //
-// Measured at 8 sequences of 32k tokens, 28 heads on 4, D 128, bf16 (168 MB): 41.6
-// us, 4.0 TB/s, 62 % of a plain copy's rate.  Of it 3.5 us pass before the first
-// page is there (lengths, table and pages are dependent loads), 4 after the last one
-// (partial, ticket, merge).  The loop takes 26 to 33; its copies alone end at 25, so
-// instructions and their latencies bound it: some 650 a warp for its 32 tokens, a third
-// of them the Values' dequantisation, issue slots 58 % busy with three warps a scheduler.
+// Measured at 8 sequences of 32k tokens, 28 heads on 4, D 128, bf16 (168 MB), replayed
+// in a graph: 41.7 us, 4.0 TB/s, 62 % of a plain copy's rate.  Of it 3.5 us pass before
+// the first page is there (lengths, table and pages are dependent loads), 4 after the
+// last one (partial, ticket, merge).  The loop takes 26 to 33 (traced in an earlier form
+// of it, of the same time); its copies alone end at 25, so instructions and their
+// latencies bound it: some 650 a warp for its 32 tokens, a third of them the Values'
+// dequantisation, issue slots 57 % busy with three warps a scheduler.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -79,7 +80,9 @@ constexpr float kLift = 7.0f;         // log2 of the weight that a running maxim
 constexpr float kSlack = 8.0f;        // log2 a score may pass the running maximum by
 constexpr float kNoMax = -3e38f;      // below any score
 constexpr int kMinPages = 4;          // places of a range at least: two pages for each pair of warps
-constexpr int kUnitCost = 6;          // empty places before a unit's pages (at 8 x 32k 16 cost 2 us more, 40 2.4)
+// Empty places before a unit's pages: at 8 x 32k 16 cost 2 us more than 6, 40 2.4 (fitted
+// before the merge had its present form, as merge_pages below; fewer than 6 not tried).
+constexpr int kUnitCost = 6;
 
 // CTAs of four warps, three an SM (168 registers a thread), or two with 16 columns
 // at D 128 (255), which hide each other's start and merge; the stages are what 227
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   constexpr int kG = D / kInt4Group, kCol = 8 * NT, kStages = C::kStages, kWarps = C::kWarps;
   constexpr int kCodes = C::kCodes, kPar = C::kPar;
   constexpr int kTerms = kWeightTerms<T>;
-  extern __shared__ __align__(128) uint8_t smem[];  // 128: 42.2 us at 16 bytes past that, 39.8 (8 x 32k, from Python)
+  extern __shared__ __align__(128) uint8_t smem[];  // 8 x 32k, from Python: 39.8 us; 42.2 at 112 past a multiple
   __shared__ int meta_s[kWarps][kStages];  // first token of each stage's part of a page, -1: nothing to do
   __shared__ int last_s;
   __shared__ Unit unit_s;

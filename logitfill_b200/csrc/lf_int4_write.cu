@@ -20,8 +20,8 @@
 // (66 us instead of 49).
 //
 // Measured for 16 sequences of 4096 bf16 tokens, 4 KV heads, D 128 (176 MB each
-// way): write 46.6 us (3.8 TB/s), of which loads and stores alone 32.9, parameters
-// 2.3, codes 5, bounds 6; the issue slots are 75 % busy.  Read 31.4 us (5.6 TB/s).
+// way): write 46.3 us (3.8 TB/s), of which loads and stores alone 32.9, parameters
+// 2.3, codes 5, bounds 6; the issue slots are 76 % busy.  Read 31.6 us (5.6 TB/s).
 // One token of 16 sequences: 2 to 3 us each, the latency of three dependent loads.
 #include <type_traits>
 
