@@ -458,6 +458,47 @@ LF_API int lf_int4_attend_sparse(const lf_int4_query* args, lf_stream_t stream);
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);
 LF_API size_t lf_int4_workspace_clear_from(void);
 
+/*
+ * ---- A prompt's way into the cache ----------------------------------------
+ *
+ * No counterpart in the reference, which leaves both steps to the model's own
+ * code (qwen2_attention.py:74-150).
+ */
+
+/* Arguments of lf_rotary_embed.  Strides in elements; channel stride 1. */
+typedef struct lf_rotary {
+  const void* q;          /* [batch][n_q][tokens][head_dim]                       */
+  void* q_out;
+  const void* k;          /* [batch][n_kv][tokens][head_dim]; not read where n_kv is 0 */
+  void* k_out;
+  int64_t q_seq_stride, q_head_stride, q_tok_stride;
+  int64_t q_out_seq_stride, q_out_head_stride, q_out_tok_stride;
+  int64_t k_seq_stride, k_head_stride, k_tok_stride;
+  int64_t k_out_seq_stride, k_out_head_stride, k_out_tok_stride;
+  const int64_t* freqs;   /* [part / 2] turns per position in units of 2^-64 turn (modulo one turn) */
+  const void* positions;  /* [batch][tokens] positions, or NULL: start[b] + t     */
+  int64_t pos_seq_stride, pos_tok_stride;
+  const int32_t* start;   /* [batch]; not read where positions are given          */
+  float magnitude;        /* factor of the rotated channels                       */
+  int32_t positions_64;   /* positions are int64 (else int32)                     */
+  int32_t dtype;          /* F32, F16 or BF16                                     */
+  int32_t head_dim;       /* 2 to 256                                             */
+  int32_t part;           /* rotated channels: the first `part`, even             */
+  int32_t interleaved;    /* pairs (2 i, 2 i + 1), else (i, i + part / 2)          */
+  int32_t transposed;     /* turn the other way                                   */
+  int32_t batch, tokens, n_q, n_kv;
+} lf_rotary;
+
+/*
+ * Rotary positions: the pair (x, y) number i of the rotated channels of a token at
+ * position p becomes magnitude * (x cos a - y sin a, y cos a + x sin a), a = 2 pi p
+ * freqs[i] / 2^64 (the other sign of a with transposed: the transposed map, which is
+ * also how a gradient goes back); the other channels are copied.  The product of
+ * position and frequency is taken modulo one turn in 64-bit whole numbers, so far
+ * positions lose nothing.  q_out may be q, and k_out k; they may not overlap otherwise.
+ */
+LF_API int lf_rotary_embed(const lf_rotary* args, lf_stream_t stream);
+
 /* Human-readable text of a status code; detail of the last failure on this thread. */
 LF_API const char* lf_status_string(int status);
 LF_API const char* lf_last_error(void);

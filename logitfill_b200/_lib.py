@@ -94,6 +94,7 @@ def lib() -> ctypes.CDLL:
         "lf_int4_attend_sparse": (c_int, [Q, P]),
         "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+        "lf_rotary_embed": (c_int, [Q, P]),
         "lf_status_string": (c_char_p, [c_int]),
         "lf_last_error": (c_char_p, []),
     }
@@ -105,7 +106,25 @@ def lib() -> ctypes.CDLL:
     return so
 
 
-_BINDING = None
+_BINDING = None          # the 4-bit cache's
+_PROMPT_BINDING = None
+
+
+def _load_binding(name: str):
+    lib()
+    import importlib.util
+
+    from logitfill_b200.build import binding_path
+
+    path = binding_path(name)   # (imports torch, whose libraries are the binding's)
+    if not path.exists():
+        raise RuntimeError(
+            f"logitfill_b200 binding missing at {path}; build it with "
+            "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
+    spec = importlib.util.spec_from_file_location(name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def int4_binding():
@@ -113,21 +132,16 @@ def int4_binding():
     built."""
     global _BINDING
     if _BINDING is None:
-        lib()
-        import importlib.util
-
-        from logitfill_b200.build import binding_path
-
-        path = binding_path()   # (imports torch, whose libraries are the binding's)
-        if not path.exists():
-            raise RuntimeError(
-                f"logitfill_b200 binding missing at {path}; build it with "
-                "`python -m logitfill_b200.build` (there is no CPU or Python fallback)")
-        spec = importlib.util.spec_from_file_location("int4_binding", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _BINDING = module
+        _BINDING = _load_binding("int4_binding")
     return _BINDING
+
+
+def prompt_binding():
+    """The same of a prompt's operators."""
+    global _PROMPT_BINDING
+    if _PROMPT_BINDING is None:
+        _PROMPT_BINDING = _load_binding("prompt_binding")
+    return _PROMPT_BINDING
 
 
 def check(status: int, what: str) -> None:

@@ -5,8 +5,9 @@
 
 nvcc cross-compiles for B200 without a GPU.  The shared library links the
 CUDA runtime statically and exports only the ``lf_*`` symbols declared in
-``include/logitfill_b200.h``.  The compiled Python binding of the 4-bit cache
-(``csrc/int4_binding.cpp``, against the installed torch) lies next to it.
+``include/logitfill_b200.h``.  The compiled Python bindings of the 4-bit cache
+(``csrc/int4_binding.cpp``) and of a prompt's operators
+(``csrc/prompt_binding.cpp``), against the installed torch, lie next to it.
 """
 from __future__ import annotations
 
@@ -35,46 +36,63 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def binding_path() -> Path:
-    """The binding for this Python and this torch, whose C++ classes it is compiled
+BINDINGS = ("int4_binding", "prompt_binding")
+
+
+def binding_path(name: str = "int4_binding") -> Path:
+    """The binding ``name`` for this Python and this torch, whose C++ classes it is compiled
     against: both are in the name."""
     import sysconfig
 
     import torch
 
-    return OUT_DIR / f"int4_binding.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
+    return OUT_DIR / f"{name}.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
 
 
 def build_binding(verbose: bool = False, force: bool = False) -> Path:
-    """g++ of the 4-bit cache's Python binding, linked to torch and the library."""
-    src, out, lib = CSRC / "int4_binding.cpp", binding_path(), OUT_DIR / LIB_NAME
-    deps = (src, ROOT / "include" / "logitfill_b200.h", Path(__file__))
-    if not force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
-        return out
+    """g++ of the Python bindings, linked to torch and the library; returns the
+    4-bit cache's path."""
+    lib = OUT_DIR / LIB_NAME
+    shared = (CSRC / "binding_common.h", ROOT / "include" / "logitfill_b200.h", Path(__file__))
+    stale = []
+    for name in BINDINGS:
+        src, out = CSRC / f"{name}.cpp", binding_path(name)
+        if force or not out.exists() or any(out.stat().st_mtime < d.stat().st_mtime for d in (src, *shared)):
+            stale.append((src, out))
+    if not stale:
+        return binding_path()
     import sysconfig
 
     import torch
 
     torch_dir = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1] / "include"
-    tmp = out.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(ROOT / "include"),
-           "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
-           "-isystem", str(cuda), "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp),
-           str(lib), "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-           "-Wl,-rpath,$ORIGIN"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if done.returncode != 0:
-        raise RuntimeError(f"g++ failed on {src.name}:\n{done.stdout}")
-    os.replace(tmp, out)
-    return out
+    running = []
+    for src, out in stale:
+        tmp = out.with_suffix(".so.tmp")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(ROOT / "include"),
+               "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+               "-isystem", str(cuda), "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp),
+               str(lib), "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+               "-Wl,-rpath,$ORIGIN"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        running.append((src, tmp, out, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for src, tmp, out, proc in running:
+        log = proc.communicate()[0]
+        if proc.returncode != 0:
+            failed.append(f"g++ failed on {src.name}:\n{log}")
+        else:
+            os.replace(tmp, out)
+    if failed:
+        raise RuntimeError("\n".join(failed))
+    return binding_path()
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Build the library and the binding; returns the library's path."""
+    """Build the library and the bindings; returns the library's path."""
     out = build_library(verbose, force)
     build_binding(verbose, force)
     return out

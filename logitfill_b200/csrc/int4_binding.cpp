@@ -6,64 +6,16 @@
 // through ctypes, 4.9 us so), which is why these functions have a compiled binding
 // next to the ctypes one of the rest.  It holds checks and bookkeeping only: the
 // kernels are in liblogitfill_b200.so, behind include/logitfill_b200.h.
-//
-// Errors: ValueError for malformed arguments, NotImplementedError for what the
-// kernels do not take, RuntimeError for tensors in the wrong place and CUDA
-// failures, TypeError for what is no tensor.  No C++ exception leaves a function.
-#include <Python.h>
+// (Checks and errors as binding_common.h says.)
+#include "binding_common.h"
 
-#include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/python_variable.h>
 
 #include <map>
 #include <mutex>
-#include <sstream>
-#include <string>
-#include <utility>
-
-#include "logitfill_b200.h"
 
 namespace {
-
-struct Fail {
-  PyObject* type;
-  std::string text;
-};
-template <typename... A>
-[[noreturn]] void fail(PyObject* type, const A&... parts) {
-  std::ostringstream s;
-  (s << ... << parts);
-  throw Fail{type, s.str()};
-}
-
-std::string shape(const at::Tensor& t) {
-  std::ostringstream s;
-  s << c10::toString(t.scalar_type()) << " [";
-  for (int64_t i = 0; i < t.dim(); ++i) s << (i ? ", " : "") << t.size(i);
-  s << "] on " << t.device();
-  return s.str();
-}
-
-const at::Tensor& tensor(PyObject* o, const char* name) {
-  if (!THPVariable_Check(o)) fail(PyExc_TypeError, name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
-}
-
-int type_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return LF_F32;
-    case at::kHalf: return LF_F16;
-    case at::kBFloat16: return LF_BF16;
-    default:
-      fail(PyExc_NotImplementedError, "dtype ", c10::toString(t), " is not supported (float32, float16, bfloat16)");
-  }
-}
 
 struct Pool {
   lf_int4_pool c;
@@ -132,34 +84,6 @@ int8_t* bounds_records(PyObject* o, const Pool& p, int64_t& page_stride, int64_t
   return static_cast<int8_t*>(t.data_ptr());
 }
 
-// t [B, H, T, D] with 16-byte aligned rows of channel stride 1 (a copy where it is
-// not), and its first three strides (0 where the extent is 1).
-at::Tensor aligned_rows(at::Tensor t, int64_t (&s)[3]) {
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
-    const auto address = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.stride(3) == 1 && address % 16 == 0 && (s[0] | s[1] | s[2]) * static_cast<int64_t>(t.element_size()) % 16 == 0) break;
-    t = t.clone(at::MemoryFormat::Contiguous);
-  }
-  return t;
-}
-
-// The device a call runs on made current, and its stream.
-struct Launch {
-  c10::cuda::OptionalCUDAGuard guard;
-  c10::cuda::CUDAStream stream;
-  explicit Launch(at::Device d) : guard(d), stream(c10::cuda::getCurrentCUDAStream(d.index())) {}
-  lf_stream_t raw() const { return reinterpret_cast<lf_stream_t>(stream.stream()); }
-};
-
-void check(int status, const char* what) {
-  if (status == LF_OK) return;
-  fail(status == LF_ERR_UNSUPPORTED        ? PyExc_NotImplementedError
-       : status == LF_ERR_INVALID_ARGUMENT ? PyExc_ValueError
-                                           : PyExc_RuntimeError,
-       what, ": ", lf_status_string(status), ": ", lf_last_error());
-}
-
 // Scratch of attention calls: partial results, then tickets that are zero between
 // calls.  Calls on one stream share one buffer (they run in order); a call being
 // captured in a CUDA graph gets its own, which the graph keeps and clears, so
@@ -186,32 +110,6 @@ Scratch workspace(const lf_int4_query& a, const Launch& on) {
     s.bytes = room;
   }
   return s;
-}
-
-template <typename F>
-PyObject* guarded(F&& body) noexcept {
-  try {
-    return body();
-  } catch (const Fail& f) {
-    PyErr_SetString(f.type, f.text.c_str());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  } catch (...) {
-    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
-  }
-  return nullptr;
-}
-
-void expect(Py_ssize_t got, Py_ssize_t want) {
-  if (got != want) fail(PyExc_TypeError, "expected ", want, " arguments, got ", got);
-}
-int64_t integer(PyObject* o, const char* name) {
-  const long long v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) {
-    PyErr_Clear();
-    fail(PyExc_TypeError, name, " must be an integer");
-  }
-  return v;
 }
 
 // write(key, value, pages, page_table, start, counts, bounds, status)
@@ -392,9 +290,6 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
-  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
-}
 PyMethodDef methods[] = {{"write", fast(write), METH_FASTCALL, nullptr},
                          {"read", fast(read), METH_FASTCALL, nullptr},
                          {"read_bounds", fast(read_bounds), METH_FASTCALL, nullptr},
