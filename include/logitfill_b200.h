@@ -499,6 +499,38 @@ typedef struct lf_rotary {
  */
 LF_API int lf_rotary_embed(const lf_rotary* args, lf_stream_t stream);
 
+/* Arguments of lf_prompt_attend.  Strides in elements; channel stride 1. */
+typedef struct lf_prompt {
+  const void* q;          /* [batch][n_q][tokens][head_dim]; packed: [n_q][tokens][head_dim] */
+  const void* k;          /* as q, with n_kv heads                                */
+  const void* v;
+  void* out;              /* as q                                                 */
+  int64_t q_seq_stride, q_head_stride, q_tok_stride;
+  int64_t k_seq_stride, k_head_stride, k_tok_stride;
+  int64_t v_seq_stride, v_head_stride, v_tok_stride;
+  int64_t out_seq_stride, out_head_stride, out_tok_stride;
+  const int32_t* starts;  /* [batch + 1] rows of the packed sequences' first tokens, or NULL: a padded batch */
+  const int32_t* counts;  /* [batch] tokens of each padded sequence, or NULL: all */
+  int32_t* status;        /* device word, or NULL                                 */
+  float scaling;
+  int32_t head_dim;       /* 64 or 128                                            */
+  int32_t dtype;          /* F16 or BF16                                          */
+  int32_t batch, tokens, n_q, n_kv;
+} lf_prompt;
+
+/*
+ * Attention of whole prompts over their own tokens: token i of a sequence sees its
+ * tokens 0 .. i (the mask of reference.py:18-27 without a past); q-head j reads KV head
+ * j / (n_q / n_kv), n_q / n_kv at most 128.  All rows 16-byte aligned, strides positive
+ * where there is more than one of a thing.
+ * Packed (starts given): sequence b is rows starts[b] .. starts[b + 1] - 1 of the one
+ * batch (the seq strides are not read); a sequence that would begin below 0, end past
+ * `tokens` or end before it begins is cut to what there is.  Rows of no sequence are
+ * neither read into a result nor written.
+ * Padded: sequence b is the first counts[b] tokens; the out rows behind them become 0.
+ */
+LF_API int lf_prompt_attend(const lf_prompt* args, lf_stream_t stream);
+
 /* Human-readable text of a status code; detail of the last failure on this thread. */
 LF_API const char* lf_status_string(int status);
 LF_API const char* lf_last_error(void);

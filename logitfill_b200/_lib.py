@@ -95,6 +95,7 @@ def lib() -> ctypes.CDLL:
         "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
         "lf_rotary_embed": (c_int, [Q, P]),
+        "lf_prompt_attend": (c_int, [Q, P]),
         "lf_status_string": (c_char_p, [c_int]),
         "lf_last_error": (c_char_p, []),
     }

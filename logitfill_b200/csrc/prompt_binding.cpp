@@ -157,7 +157,106 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-PyMethodDef methods[] = {{"rotary", fast(rotary), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// t with 16-byte aligned rows of channel stride 1 and no stride of 0 over more than one
+// row (a copy where it is not so).
+at::Tensor plain_rows(const at::Tensor& t) {
+  bool fits = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1) fits = fits && t.stride(d) > 0 && t.stride(d) * static_cast<int64_t>(t.element_size()) % 16 == 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+const int32_t* small_ints(PyObject* o, const char* name, int64_t count, const at::Device& on) {
+  const at::Tensor& t = tensor(o, name);
+  if (t.scalar_type() != at::kInt || t.dim() != 1 || (count >= 0 ? t.size(0) != count : t.size(0) < 1) || t.device() != on ||
+      !t.is_contiguous())
+    fail(PyExc_ValueError, name, " must be a contiguous int32 [", count >= 0 ? std::to_string(count) : "batch + 1", "] tensor on ", on,
+         ", got ", shape(t));
+  return static_cast<const int32_t*>(t.data_ptr());
+}
+
+// attend(query, key, value, scaling, starts, counts, out, status) -> out
+PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect(n, 8);
+    const at::Tensor &query = tensor(v[0], "query"), &key = tensor(v[1], "key"), &value = tensor(v[2], "value");
+    const bool packed = query.dim() == 3;
+    if (query.dim() != 3 && query.dim() != 4)
+      fail(PyExc_ValueError, "query must be [batch, heads, tokens, head_dim] or [tokens, heads, head_dim], got ", shape(query));
+    const int64_t T = query.size(packed ? 0 : 2), D = query.size(-1), nq = query.size(1);
+    const bool like = key.dim() == query.dim() && key.size(-1) == D && key.size(0) == query.size(0) && (packed || key.size(2) == T);
+    if (!like || key.sizes() != value.sizes() || key.scalar_type() != query.scalar_type() || value.scalar_type() != query.scalar_type())
+      fail(PyExc_ValueError, "key and value must be like the query but for their heads (", shape(query), "), got ", shape(key), " and ",
+           shape(value));
+    const int64_t nkv = key.size(1);
+    if (nq < 1 || nkv < 1 || nq % nkv) fail(PyExc_ValueError, nq, " query heads do not divide into ", nkv, " KV heads");
+    if (query.scalar_type() != at::kHalf && query.scalar_type() != at::kBFloat16)
+      fail(PyExc_NotImplementedError, "prompt attention takes fp16 or bf16, got ", c10::toString(query.scalar_type()));
+    if (!query.is_cuda()) fail(PyExc_RuntimeError, "prompt_attention needs CUDA tensors (there is no CPU path)");
+    if (key.device() != query.device() || value.device() != query.device())
+      fail(PyExc_RuntimeError, "key and value must be on ", query.device());
+    no_gradient(query, "query");
+    no_gradient(key, "key");
+    no_gradient(value, "value");
+    for (const int64_t x : {query.size(0), T, nq, D})
+      if (x > INT32_MAX) fail(PyExc_NotImplementedError, "an extent of ", x, " is too large");
+    lf_prompt a{};
+    a.batch = static_cast<int32_t>(packed ? 1 : query.size(0));
+    if (packed) {
+      if (v[5] != Py_None) fail(PyExc_ValueError, "packed sequences take starts, a padded batch counts");
+      if (v[4] != Py_None) {
+        a.starts = small_ints(v[4], "starts", -1, query.device());
+        const int64_t b = tensor(v[4], "starts").size(0) - 1;
+        if (b > INT32_MAX) fail(PyExc_NotImplementedError, "an extent of ", b, " is too large");
+        a.batch = static_cast<int32_t>(b);
+      }
+    } else {
+      if (v[4] != Py_None) fail(PyExc_ValueError, "packed sequences take starts, a padded batch counts");
+      if (v[5] != Py_None) a.counts = small_ints(v[5], "counts", query.size(0), query.device());
+    }
+    a.scaling = number(v[3], "scaling");
+    if (v[7] != Py_None) {
+      const at::Tensor& t = tensor(v[7], "status");
+      if (t.scalar_type() != at::kInt || t.numel() < 1 || t.device() != query.device())
+        fail(PyExc_ValueError, "status must be an int32 tensor on ", query.device(), ", got ", shape(t));
+      a.status = static_cast<int32_t*>(t.data_ptr());
+    }
+    const Launch on(query.device());
+    at::Tensor out;
+    if (v[6] == Py_None) {
+      out = at::empty_like(query);
+      if (plain_rows(out).data_ptr() != out.data_ptr()) out = at::empty(query.sizes(), query.options());
+    } else {
+      out = tensor(v[6], "out");
+      check_out(out, query, "out", "query");
+      if (overlap(out, query) || overlap(out, key) || overlap(out, value)) fail(PyExc_ValueError, "out shares memory with an input");
+    }
+    if (query.numel() == 0) return THPVariable_Wrap(std::move(out));
+    const at::Tensor q = plain_rows(query), k = plain_rows(key), x = plain_rows(value);
+    const auto place = [](const at::Tensor& y, int64_t& seq, int64_t& head, int64_t& tok) {
+      const Rows r(y);
+      seq = r.seq;
+      head = r.head;
+      tok = r.tok;
+      return y.data_ptr();
+    };
+    a.q = place(q, a.q_seq_stride, a.q_head_stride, a.q_tok_stride);
+    a.k = place(k, a.k_seq_stride, a.k_head_stride, a.k_tok_stride);
+    a.v = place(x, a.v_seq_stride, a.v_head_stride, a.v_tok_stride);
+    a.out = place(out, a.out_seq_stride, a.out_head_stride, a.out_tok_stride);
+    a.head_dim = static_cast<int32_t>(D);
+    a.dtype = type_code(q.scalar_type());
+    a.tokens = static_cast<int32_t>(T);
+    a.n_q = static_cast<int32_t>(nq);
+    a.n_kv = static_cast<int32_t>(nkv);
+    check(lf_prompt_attend(&a, on.raw()), "lf_prompt_attend");
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+PyMethodDef methods[] = {{"rotary", fast(rotary), METH_FASTCALL, nullptr},
+                         {"attend", fast(attend), METH_FASTCALL, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "prompt_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

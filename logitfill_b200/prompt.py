@@ -1,9 +1,12 @@
-"""A prompt's way into the cache: rotary positions of its queries and Keys.
+"""A prompt's way into the cache: rotary positions of its queries and Keys, and
+its attention over its own tokens.
 
 :func:`rotary_embed` turns the queries and Keys of a step to their positions,
 next to the caches' own attention: what :func:`logitfill_b200.int4.int4_write`
 or a layer's ``commit`` stores are turned Keys.  :func:`rotary_frequencies`
-makes the table it reads.
+makes the table it reads.  :func:`prompt_attention` is the causal attention of
+whole prompts in their original type, which both caches leave to their caller
+(:mod:`logitfill_b200.adapter` can run it).
 
 Tensors are ``[batch, heads, tokens, head_dim]``, or packed ``[tokens, heads,
 head_dim]``: the tokens of all sequences behind one another.  Every launch goes
@@ -93,4 +96,23 @@ def rotary_embed(query: torch.Tensor, key: torch.Tensor | None, freqs: torch.Ten
     return _lib.prompt_binding().rotary(query, key, freqs, positions, start, magnitude, interleaved, transposed, out)
 
 
-__all__ = ["rotary_frequencies", "rotary_embed"]
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float,
+                     starts: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of whole prompts over their own tokens: token ``i`` of a sequence
+    sees its tokens ``0 .. i``.  fp16 or bf16, ``head_dim`` 64 or 128, query head
+    ``j`` reading KV head ``j // (n_q // n_kv)`` (128 query heads to a KV head at
+    most); the result has the query's shape and type.
+
+    Packed, ``query`` ``[tokens, n_q, head_dim]`` and ``key``, ``value`` ``[tokens,
+    n_kv, head_dim]``: sequence ``b`` is rows ``starts[b] .. starts[b + 1] - 1``
+    (int32 ``[batch + 1]`` on the GPU; None: one sequence); sequences do not share
+    rows, and rows of no sequence are left as they were in ``out`` (undefined in a
+    new result).  Padded, ``[batch, heads, tokens, head_dim]``: sequence ``b`` has its
+    first ``counts[b]`` tokens (int32 ``[batch]``; None: all), and the rows behind
+    them become 0.  What lies in rows that a token does not see does not matter, NaN
+    and infinities included.  ``out`` may not share memory with an input."""
+    return _lib.prompt_binding().attend(query, key, value, scaling, starts, counts, out, status)
+
+
+__all__ = ["rotary_frequencies", "rotary_embed", "prompt_attention"]

@@ -215,3 +215,290 @@ def test_rotary_refusals():
     room = torch.zeros(200, 2, 64, dtype=BF16, device="cuda")
     with pytest.raises(ValueError, match="overlaps"):
         prompt.rotary_embed(room[:100], None, freqs, positions=torch.arange(100, device="cuda"), out=(room[50:150], None))
+
+
+# ------------------------------------------------------------ prompt attention
+#
+# Element by element within  u |out| + (u + 2 e + 2^-16) sum p |v| + n 2^-30 max |v|:
+# u is half a step of the type, for the output and for the weights that enter the
+# product with Value; e, the fp32 sums of a score: 128 products of 2^-24 each, scaled,
+# of the row's largest sum |q k|, in a weight and in the sum of weights; 2^-16 the
+# exponential, the running sums and their rescalings; the last term what fp16 weights
+# lose below their smallest step (2^-25 of weights whose largest is at 2^7, or 2^-1
+# where the running maximum lags by its slack of 2^8).
+
+def _prompts(seed, counts, n_q, n_kv, D, dtype=BF16, keys=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = max(sum(counts), 0)
+    q, k, v = (torch.randn(n, h, D, generator=g, device="cuda") for h in (n_q, n_kv, n_kv))
+    k[..., ::19] *= keys
+    return q.to(dtype), k.to(dtype), v.to(dtype)
+
+
+def _one(q, k, v, scaling, dtype):
+    """(out, bound) of one sequence: q [n, n_q, D], k and v [n, n_kv, D], in 64 bits."""
+    n, n_q, D = q.shape
+    group = n_q // k.shape[1]
+    out, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    later = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+    u = HALF_STEP[dtype]
+    for h in range(n_q):
+        a, b, c = q[:, h].double(), k[:, h // group].double(), v[:, h // group].double()
+        logits = (a @ b.T * scaling).masked_fill(later, -math.inf)
+        p = torch.softmax(logits, -1)
+        e = (a.abs() @ b.abs().T * abs(scaling)).masked_fill(later, 0).amax(-1, keepdim=True) * 128 * 2.0 ** -24
+        out[:, h] = p @ c
+        bound[:, h] = u * out[:, h].abs() + (u + 2 * e + 2.0 ** -16) * (p @ c.abs()) + n * 2.0 ** -30 * c.abs().max() + 2.0 ** -24
+    return out, bound
+
+
+def _check_prompts(got, q, k, v, counts, scaling, dtype):
+    at = 0
+    for c in counts:
+        if c:
+            want, bound = _one(q[at:at + c], k[at:at + c], v[at:at + c], scaling, dtype)
+            off = (got[at:at + c].double() - want).abs() - bound
+            assert bool((off <= 0).all()), f"{c} tokens: outside by {float(off.max()):.3g} at {(off == off.max()).nonzero()[0].tolist()}"
+        at += c
+
+
+def _starts(counts, device="cuda"):
+    return torch.tensor([sum(counts[:b]) for b in range(len(counts) + 1)], dtype=torch.int32, device=device)
+
+
+HEADS = [(28, 4), (8, 8), (16, 1), (40, 8), (9, 3)]
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64), (F16, 128), (BF16, 64)])
+def test_prompts_of_every_length(n_q, n_kv, dtype, D):
+    counts = [1, 2, 17, 0, 18, 19, 36, 37, 64, 127, 128, 129, 0, 255, 256, 257, 300]
+    q, k, v = _prompts(n_q + D, counts, n_q, n_kv, D, dtype)
+    got = prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts))
+    assert got.shape == q.shape and got.dtype == dtype
+    _check_prompts(got, q, k, v, counts, D ** -0.5, dtype)
+    # a sequence's result does not depend on its neighbours
+    at = sum(counts[:11])
+    alone = prompt.prompt_attention(q[at:at + 129], k[at:at + 129], v[at:at + 129], D ** -0.5)
+    assert torch.equal(alone, got[at:at + 129])
+
+
+@pytest.mark.parametrize("n_q,n_kv,D,dtype,counts", [(28, 4, 128, BF16, [2500]), (4, 2, 128, BF16, [1, 4097, 3]), (128, 1, 64, F16, [333]),
+                                                     (100, 1, 128, BF16, [70, 5]), (65, 1, 64, BF16, [40]), (12, 3, 64, F16, [1700, 900])])
+def test_longer_prompts_and_wide_groups(n_q, n_kv, D, dtype, counts):
+    q, k, v = _prompts(n_q, counts, n_q, n_kv, D, dtype)
+    _check_prompts(prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts)), q, k, v, counts, D ** -0.5, dtype)
+
+
+def test_many_short_sequences():
+    counts = [1 + b * 7 % 23 for b in range(700)]
+    q, k, v = _prompts(1, counts, 6, 2, 64, F16)
+    _check_prompts(prompt.prompt_attention(q, k, v, 0.125, starts=_starts(counts)), q, k, v, counts, 0.125, F16)
+
+
+@pytest.mark.parametrize("dtype,D,B,T,n_q,n_kv", [(BF16, 128, 3, 200, 14, 2), (F16, 64, 5, 37, 8, 8), (BF16, 64, 2, 513, 6, 1)])
+def test_padded_batches(dtype, D, B, T, n_q, n_kv):
+    """Padding holds NaN: it is not read into anything, and comes out as 0."""
+    counts = [T, 0, 1, T - 1, 20][:B] if B > 2 else [T - 130, T]
+    q, k, v = _prompts(T, [T] * B, n_q, n_kv, D, dtype)
+    q, k, v = (x.view(B, T, -1, D) for x in (q, k, v))
+    for x in (q, k, v):
+        for b, c in enumerate(counts):
+            x[b, c:] = float("nan")
+    device = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    for contiguous in (False, True):
+        a, b_, c_ = ((x.transpose(1, 2).contiguous() if contiguous else x.transpose(1, 2)) for x in (q, k, v))
+        got = prompt.prompt_attention(a, b_, c_, D ** -0.5, counts=device)
+        assert got.shape == (B, n_q, T, D)
+        for b, c in enumerate(counts):
+            assert not bool(got[b, :, c:].any())
+            if c:
+                _check_prompts(got[b].transpose(0, 1), q[b], k[b], v[b], [c], D ** -0.5, dtype)
+    full = [torch.nan_to_num(x.transpose(1, 2)) for x in (q, k, v)]
+    every = prompt.prompt_attention(*full, D ** -0.5)
+    for b in range(B):
+        _check_prompts(every[b].transpose(0, 1), *(x[b].transpose(0, 1) for x in full), [T], D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64)])
+def test_rows_of_no_sequence_stay_as_they_were(dtype, D):
+    """Rows before, between and behind the sequences, NaN in all of them."""
+    q, k, v = _prompts(2, [400], 10, 2, D, dtype)
+    starts = torch.tensor([30, 95, 95, 300], dtype=torch.int32, device="cuda")
+    for x in (q, k, v):
+        x[:30], x[300:] = float("nan"), float("inf")
+    out = torch.full_like(q, 7.0)
+    got = prompt.prompt_attention(q, k, v, D ** -0.5, starts=starts, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert bool((out[:30] == 7).all()) and bool((out[300:] == 7).all())
+    _check_prompts(out[30:300], q[30:300], k[30:300], v[30:300], [65, 0, 205], D ** -0.5, dtype)
+    # starts that leave the rows, or run backwards, are cut to what there is
+    for bad, spans in [((-50, 95, 90, 1 << 30), [(0, 95), (90, 400)]), ((300, 30, 2000000000, -5), [(30, 400)]), ((-9, -3), [])]:
+        out.fill_(7.0)
+        prompt.prompt_attention(*(torch.nan_to_num(x, 1.0, 1.0, 1.0) for x in (q, k, v)), D ** -0.5,
+                                starts=torch.tensor(bad, dtype=torch.int32, device="cuda"), out=out)
+        covered = torch.zeros(400, dtype=torch.bool)
+        for low, high in spans:
+            covered[low:high] = True
+        written = ~(out == 7).all(-1).all(-1).cpu()
+        assert torch.equal(written, covered)
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.09, 1e-30, 40.0, -700.0])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scalings_of_any_sign_and_size(scaling, dtype):
+    q, k, v = _prompts(4, [200, 77], 4, 2, 128, dtype, keys=1.0)
+    got = prompt.prompt_attention(q, k, v, scaling, starts=_starts([200, 77]))
+    if abs(scaling) < 1:
+        _check_prompts(got, q, k, v, [200, 77], scaling, dtype)
+    else:   # one token takes nearly all: where the best leads by more than the scores' error, it is the result
+        at = 0
+        for c in (200, 77):
+            for h in range(4):
+                a, b = q[at:at + c, h].double(), k[at:at + c, h // 2].double()
+                later = torch.ones(c, c, dtype=torch.bool, device="cuda").triu(1)
+                logits = (a @ b.T * scaling).masked_fill(later, -math.inf)
+                e = float((a.abs() @ b.abs().T).max()) * abs(scaling) * 128 * 2.0 ** -24
+                best = logits.topk(2, -1)
+                sure = best.values[:, 0] - best.values[:, 1] > 30 + 2 * e
+                assert int(sure.sum()) > c // 3
+                want = v[at:at + c, h // 2][best.indices[:, 0]]
+                assert torch.equal(got[at:at + c, h][sure], want[sure])
+            at += c
+
+
+def test_a_dominant_token_keeps_the_others():
+    """An attention sink with a small Value, others 10 to 16 below it: in fp16 weights their share would drop out
+    if the largest weight stood at 1."""
+    n, D = 500, 128
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for gap in (10.0, 16.0):
+        q = torch.ones(n, 2, D, dtype=F16, device="cuda")
+        k = torch.zeros(n, 1, D, dtype=F16, device="cuda")
+        k[0] = gap / D
+        v = (torch.randn(n, 1, D, generator=g, device="cuda").abs() + 1).to(F16)
+        v[0] = 0.0
+        got = prompt.prompt_attention(q, k, v, 1.0)
+        _check_prompts(got, q, k, v, [n], 1.0, F16)
+
+
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_that_rise_and_fall(rising):
+    """The running maximum moves at every tile, or only at the first."""
+    n, D = 1500, 128
+    q = torch.ones(n, 7, D, dtype=BF16, device="cuda")
+    ramp = torch.linspace(0, 120, n, device="cuda") / D
+    k = (ramp if rising else ramp.flip(0)).to(BF16).view(n, 1, 1).expand(n, 1, D).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    v = torch.randn(n, 1, D, generator=g, device="cuda").to(BF16)
+    _check_prompts(prompt.prompt_attention(q, k, v, 1.0), q, k, v, [n], 1.0, BF16)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("where", ["key", "value", "query"])
+def test_non_finite_rows_reach_only_who_sees_them(dtype, D, value, where):
+    counts = [300, 140]
+    q, k, v = _prompts(7, counts, 6, 2, D, dtype)
+    clean = prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts))
+    at = 133                      # inside a tile, of the first sequence, KV head 1
+    dict(key=k, value=v, query=q)[where][at, 1, 5] = value
+    got = prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts))
+    touched = torch.zeros(440, 6, D, dtype=torch.bool, device="cuda")
+    if where == "query":
+        touched[at, 1] = True
+    elif where == "key":
+        touched[at:300, 3:] = True
+    else:
+        touched[at:300, 3:, 5] = True
+    assert torch.equal(got[~touched], clean[~touched])
+    if where == "value":
+        assert not bool(torch.isfinite(got[touched]).any())
+    elif math.isnan(value):
+        assert bool(torch.isnan(got[touched]).all())
+
+
+def test_prompt_strides_and_unaligned_rows():
+    """Views of one projection's buffer, broadcast Keys, rows at odd offsets (copied first)."""
+    counts, D = [90, 41], 64
+    g = torch.Generator(device="cuda").manual_seed(8)
+    room = torch.randn(131 * (6 + 2 + 2) * D + 1, generator=g, device="cuda").to(BF16)
+    for shift in (0, 1):
+        both = room[shift:shift + 131 * 10 * D].view(131, 10, D)
+        q, k, v = both[:, :6], both[:, 6:8], both[:, 8:]
+        got = prompt.prompt_attention(q, k, v, 0.125, starts=_starts(counts))
+        _check_prompts(got, q, k, v, counts, 0.125, BF16)
+        want = prompt.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), 0.125, starts=_starts(counts))
+        assert torch.equal(got, want)
+    one = k[:, :1].expand(-1, 2, -1)
+    assert torch.equal(prompt.prompt_attention(q, one, v, 0.125), prompt.prompt_attention(q, one.contiguous(), v, 0.125))
+    # heads first in memory, an out of other strides
+    turned = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    out = torch.zeros(131, 8, D, dtype=BF16, device="cuda")[:, 1:7]
+    assert torch.equal(prompt.prompt_attention(*turned, 0.125, starts=_starts(counts), out=out), got)
+
+
+def test_prompt_streams_graphs_and_empty_calls():
+    counts, D = [300, 29, 171], 128
+    q, k, v = _prompts(9, counts, 8, 2, D)
+    starts = _starts(counts)
+    want = prompt.prompt_attention(q, k, v, 0.09, starts=starts)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [prompt.prompt_attention(q, k, v, 0.09, starts=starts) for _ in range(3)]
+    both = [prompt.prompt_attention(q, k, v, 0.09, starts=starts) for _ in range(3)]     # two streams at once
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(x, want) for x in got + both)
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        prompt.prompt_attention(q, k, v, 0.09, starts=starts, out=out)
+    graph.replay()
+    assert torch.equal(out, want)
+    starts.copy_(_starts([100, 350, 50]))     # the lengths are read when it runs
+    q.mul_(0.5)
+    graph.replay()
+    assert torch.equal(out, prompt.prompt_attention(q, k, v, 0.09, starts=starts)) and not torch.equal(out, want)
+    assert prompt.prompt_attention(q[:0], k[:0], v[:0], 1.0).shape == (0, 8, D)
+    assert prompt.prompt_attention(q[:0], k[:0], v[:0], 1.0, starts=starts).shape == (0, 8, D)
+    padded = [x.view(2, 250, -1, D).transpose(1, 2) for x in (q, k, v)]
+    assert prompt.prompt_attention(*(x[:0] for x in padded), 1.0).shape == (0, 8, 250, D)
+    assert not bool(prompt.prompt_attention(*padded, 1.0, counts=torch.tensor([0, -3], dtype=torch.int32, device="cuda")).any())
+
+
+def test_prompt_offsets_past_32_bits():
+    """Rows more than 2^31 elements apart."""
+    n, D, tok = 40, 64, 1 << 26
+    room = torch.empty(n * tok, dtype=BF16, device="cuda")
+    q = room.as_strided((n, 2, D), (tok, D, 1), 0)
+    k, v = room.as_strided((n, 1, D), (tok, D, 1), 1024), room.as_strided((n, 1, D), (tok, D, 1), 2048)
+    out = room.as_strided((n, 2, D), (tok, D, 1), 4096)
+    made = _prompts(10, [n], 2, 1, D)
+    for x, y in zip((q, k, v), made):
+        x.copy_(y)
+    prompt.prompt_attention(q, k, v, 0.125, out=out)
+    assert torch.equal(out, prompt.prompt_attention(*made, 0.125))
+    del room
+
+
+def test_prompt_refusals():
+    q, k, v = _prompts(11, [32], 8, 2, 64)
+    starts = _starts([20, 12])
+    p4 = [x.view(2, 16, -1, 64).transpose(1, 2) for x in (q, k, v)]
+    counts = torch.tensor([16, 3], dtype=torch.int32, device="cuda")
+    for error, args, kw in [
+            (ValueError, (q, k[:31], v, 1.0), {}), (ValueError, (q, k, v[:, :1], 1.0), {}), (ValueError, (q, k.half(), v, 1.0), {}),
+            (ValueError, (q[:, :7], k, v, 1.0), {}), (ValueError, (q[:, :0], k, v, 1.0), {}), (ValueError, (q[0], k[0], v[0], 1.0), {}),
+            (ValueError, (q, k, v, float("nan")), {}), (ValueError, (q, k, v, float("inf")), {}), (TypeError, (q, k, v, "1"), {}),
+            (ValueError, (q, k, v, 1.0), dict(counts=counts)), (ValueError, (*p4, 1.0), dict(starts=starts)),
+            (ValueError, (q, k, v, 1.0), dict(starts=starts.long())), (ValueError, (q, k, v, 1.0), dict(starts=starts[:0])),
+            (ValueError, (q, k, v, 1.0), dict(starts=starts.cpu())), (ValueError, (*p4, 1.0), dict(counts=counts[:1])),
+            (ValueError, (q, k, v, 1.0), dict(out=q)), (ValueError, (q, k, v, 1.0), dict(out=q.float())),
+            (ValueError, (q, k, v, 1.0), dict(out=torch.zeros(1, 8, 64, dtype=BF16, device="cuda").expand(32, 8, 64))),
+            (NotImplementedError, (q.float(), k.float(), v.float(), 1.0), {}), (RuntimeError, (q.cpu(), k, v, 1.0), {}),
+            (RuntimeError, (q, k.cpu(), v, 1.0), {}), (NotImplementedError, tuple(x[..., :32] for x in (q, k, v)) + (1.0,), {}),
+            (NotImplementedError, (q.repeat(1, 17, 1), k[:, :1], v[:, :1], 1.0), {}),
+            (NotImplementedError, (q.clone().requires_grad_(), k, v, 1.0), {}), (TypeError, (q, None, v, 1.0), {})]:
+        with pytest.raises(error):
+            prompt.prompt_attention(*args, **kw)
