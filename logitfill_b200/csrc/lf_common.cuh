@@ -13,6 +13,8 @@ namespace lf {
 // Per-thread error text for lf_last_error().
 void set_error(const char* fmt, ...);
 int launch_status(const char* what);
+// SMs of the current device (0 on error), asked once per device.
+int sm_count();
 // Raise kern's dynamic shared-memory limit on the current device to at least
 // `bytes` (optionally with the full shared-memory carveout).  The limit only
 // grows: launches and occupancy queries for different layouts share one

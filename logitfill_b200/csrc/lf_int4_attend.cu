@@ -47,7 +47,6 @@
 // of it, of the same time); its copies alone end at 25, so instructions and their
 // latencies bound it: some 650 a warp for its 32 tokens, a third of them the Values'
 // dequantisation, issue slots 57 % busy with three warps a scheduler.
-#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -910,16 +909,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   }
 }
 
-// SMs of the current device (0 on error), asked once per device.
-static int sm_count() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
-  n = known[dev].load(std::memory_order_relaxed);
-  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
-    known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
 // The partials: two records per CTA of the largest grid.
 static size_t partial_bytes(int sms) {
   using A = AttendCfg<128, 1>;

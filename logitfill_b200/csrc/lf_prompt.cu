@@ -1,7 +1,10 @@
 // Attention of whole prompts over their own tokens (lf_prompt_attend).
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "lf_common.cuh"
+#include "lf_flash.cuh"
 
 namespace lf {
 
@@ -74,24 +77,467 @@ __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok
   for (int x = 0; x < kOwn; ++x) Scalar<T>::store(out + d + x, sum == 0.0f ? 0.0f : acc[x] / sum);
 }
 
-// A warp to a row; rows of sequence blockIdx.z and q-head blockIdx.y.
+using namespace sm100;
+
+// Shared memory and barriers of a CTA.
+template <int D> struct PromptCfg {
+  static constexpr int kTile = 128 * D * 2;                      // bytes of 128 rows
+  static constexpr int kSlots = D == 128 ? 5 : 8;                // Key and Value tiles in flight
+  static constexpr int kSmem = 2 * kTile + kSlots * kTile + 1024;  // (aligned by hand)
+  static constexpr int kO = 256;                                 // TMEM columns: scores of both tiles, then outputs
+};
+constexpr int kPromptThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kScanWarp = 11;
+constexpr uint64_t kPromptWaitNs = 2000000000ull;
+
+// A piece of work: two query tiles of one KV head of one sequence.
+struct PromptItem {
+  int b, h;        // b < 0: no more
+  int tok;         // first token of the first tile
+  int tokens, rows;
+  int first;       // row of the sequence's first token
+  int n[2];        // Key tiles that each query tile sees
+};
+
+struct PromptShared {
+  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_ready[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
+  PromptItem item[2];
+  int bad[2];      // a Value that not all rows of a masked tile see is not finite
+  int scan_slot, scan_live, scan_item;  // for the scan: the Value tile, its rows of the sequence, the item's slot
+  int stop;        // a wait gave up
+  uint32_t tmem;
+};
+
+// Whether some row of the query tile that begins at token t0 does not see all of Key tile j.
+__device__ __forceinline__ bool tile_masked(int t0, int j) { return (j + 1) * 128 > t0 + 1; }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prompt_simple_kernel(const __grid_constant__ PromptParams p) {
-  grid_dep_wait();
-  const int h = blockIdx.y;
-  for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
-    const PromptSpan s = prompt_span(p, b);
-    const T* k = static_cast<const T*>(p.k) + b * p.k_seq + s.first * p.k_tok + h / p.group * p.k_head;
-    const T* v = static_cast<const T*>(p.v) + b * p.v_seq + s.first * p.v_tok + h / p.group * p.v_head;
-    for (int64_t i = blockIdx.x * 8 + (threadIdx.x >> 5); i < s.rows; i += gridDim.x * 8)
-      prompt_row<T, D>(static_cast<const T*>(p.q) + b * p.q_seq + (s.first + i) * p.q_tok + h * p.q_head, k, p.k_tok, v, p.v_tok,
-                       i < s.tokens ? static_cast<int>(i) + 1 : 0, p.scale_log2,
-                       static_cast<T*>(p.out) + b * p.o_seq + (s.first + i) * p.o_tok + h * p.o_head);
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                  const __grid_constant__ CUtensorMap v_map) {
+  using C = PromptCfg<D>;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  constexpr int kHalves = D / 64, kSlots = C::kSlots;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ PromptShared sh;
+  const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, ring = base + 2 * C::kTile;
+  uint8_t* ring_ptr = dynamic + (ring - smem_u32(dynamic));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int per_tile = 128 / p.group;  // tokens of a query tile
+
+  if (warp == kMmaWarp) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
   }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh.s_full[t], 1);
+      mbar_init(&sh.p_ready[t], 128);
+      mbar_init(&sh.o_done[t], 1);
+      mbar_init(&sh.item_full[t], 1);
+      mbar_init(&sh.item_empty[t], 10);
+    }
+    mbar_init(&sh.scan, 1);
+    mbar_init(&sh.scanned, 1);
+    mbar_init(&sh.last, 1);
+    sh.stop = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&sh.tmem), 0);
+  grid_dep_wait();
+
+  volatile int* stop = &sh.stop;
+  // Whole-warp wait: false once a wait of this CTA has given up.
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) {
+      const uint64_t t0 = globaltimer_ns();
+      for (uint32_t n = 1; !ok; ++n) {
+        ok = mbar_try_wait(bar, parity);
+        if (!ok && (n & 63u) == 0u && (*stop != 0 || globaltimer_ns() - t0 > kPromptWaitNs)) break;
+      }
+      if (!ok) *stop = 1;
+    }
+    return __all_sync(0xffffffffu, ok);
+  };
+  // The next item (number n of this CTA), copied from the plan's slot.
+  auto take = [&](uint32_t n, PromptItem& it) -> bool {
+    if (!wait(&sh.item_full[n & 1], (n >> 1) & 1)) return false;
+    it = sh.item[n & 1];
+    return it.b >= 0;
+  };
+  auto give = [&](uint32_t n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[n & 1]);
+  };
+
+  if (warp == kPlanWarp) {
+    // ---------------------------------------------------------------- plan
+    // Items in the order of falling cost: by their number of tokens before, over all
+    // sequences; a CTA takes them from alternating ends of rounds as wide as the grid.
+    const int span = 2 * per_tile;
+    auto pairs_of = [&](int b) { return (prompt_span(p, b).rows + span - 1) / span; };
+    // Items of one KV head at level x or above, over all sequences (64 bits: starts may be anything).
+    auto above = [&](int x) -> int64_t {
+      int64_t n = 0;
+      for (int b = lane; b < p.batch; b += 32) n += max(0, pairs_of(b) - x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      return n;
+    };
+    int most = 0;
+    for (int b = lane; b < p.batch; b += 32) most = max(most, pairs_of(b));
+    most = __reduce_max_sync(0xffffffffu, most);
+    const int64_t total = above(0) * p.n_kv;
+    uint32_t n = 0;
+    for (int64_t round = 0;; ++round, ++n) {
+      if (n >= 2 && !wait(&sh.item_empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
+      const int64_t x = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      PromptItem it;
+      it.b = -1;
+      if (x < total) {
+        int low = 0, high = most - 1;  // the level: the largest with more than x items at or above it
+        while (low < high) {
+          const int mid = (low + high + 1) >> 1;
+          if (above(mid) * p.n_kv > x) low = mid; else high = mid - 1;
+        }
+        const int64_t y = x - above(low + 1) * p.n_kv;
+        int64_t rank = y / p.n_kv;
+        it.h = static_cast<int>(y - rank * p.n_kv);
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+          const uint32_t has = __ballot_sync(0xffffffffu, b0 + lane < p.batch && pairs_of(b0 + lane) > low);
+          if (rank < __popc(has)) {
+            it.b = b0 + __fns(has, 0, static_cast<int>(rank) + 1);
+            break;
+          }
+          rank -= __popc(has);
+        }
+        const PromptSpan s = prompt_span(p, it.b);
+        it.first = static_cast<int>(s.first);
+        it.tokens = s.tokens;
+        it.rows = s.rows;
+        it.tok = low * span;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int t0 = it.tok + t * per_tile;
+          it.n[t] = t0 < s.tokens ? (min(t0 + per_tile, s.tokens) - 1) / 128 + 1 : 0;
+        }
+      }
+      if (lane == 0) {
+        sh.item[n & 1] = it;
+        sh.bad[n & 1] = 0;
+        mbar_arrive(&sh.item_full[n & 1]);
+      }
+      __syncwarp();
+      if (it.b < 0) break;
+    }
+  } else if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- copies
+    uint32_t load = 0, n_q = 0;  // tiles and query pairs copied so far
+    if (lane < 3) prefetch_map(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map);
+    PromptItem it;
+    bool ok = true;
+    for (uint32_t n = 0; ok && take(n, it); ++n) {
+      give(n);
+      const int steps = max(it.n[0], it.n[1]);
+      if (steps == 0) continue;
+      if (n_q > 0 && !(ok = wait(&sh.q_empty, (n_q - 1) & 1))) break;
+      ++n_q;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&sh.q_full, 2 * kHalves * per_tile * p.group * 128);
+        for (int t = 0; t < 2; ++t)
+          for (int c = 0; c < kHalves; ++c)
+            tma_load_4d(base + t * C::kTile + c * kHalfBytes, &q_map, 64 * c, it.h * p.group, it.first + it.tok + t * per_tile,
+                        p.starts != nullptr ? 0 : it.b, &sh.q_full);
+      }
+      __syncwarp();
+      for (int i = 0; i < 2 * steps; ++i, ++load) {
+        const int slot = load % kSlots, j = steps - 1 - (i >> 1);
+        if (load >= kSlots && !(ok = wait(&sh.kv_empty[slot], (load / kSlots - 1) & 1))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&sh.kv_full[slot], C::kTile);
+          for (int c = 0; c < kHalves; ++c)
+            tma_load_4d(ring + slot * C::kTile + c * kHalfBytes, (i & 1) ? &v_map : &k_map, 64 * c, it.first + 128 * j, it.h,
+                        p.starts != nullptr ? 0 : it.b, &sh.kv_full[slot]);
+        }
+        __syncwarp();
+      }
+    }
+    // Every copy and every arrival of the tensor core's has come in before the CTA ends
+    // (after a wait that gave up: as far as the limit goes).
+    for (int i = 0; i < kSlots; ++i) {
+      const uint32_t done = load / kSlots + (static_cast<uint32_t>(i) < load % kSlots ? 1 : 0);
+      if (done == 0) continue;
+      if (*stop == 0)
+        wait(&sh.kv_empty[i], (done - 1) & 1);
+      else
+        mbar_wait_bounded(&sh.kv_full[i], (done - 1) & 1, kPromptWaitNs);
+    }
+    if (n_q > 0) {
+      if (*stop == 0)
+        wait(&sh.q_empty, (n_q - 1) & 1);
+      else
+        mbar_wait_bounded(&sh.q_full, (n_q - 1) & 1, kPromptWaitNs);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- products
+    // Step s of the CTA: scores of Key tile (load 2 s) for both query tiles, after the
+    // output product of step s - 1 (Value tile, load 2 s - 1), tile by tile: while the
+    // softmax of one tile runs, the tensor core works for the other.
+    const uint32_t idesc_s = idesc_16(kBf16, 128, 128, false, p.scale_log2 < 0.0f), idesc_o = idesc_16(kBf16, 128, D, true, false);
+    uint32_t step = 0, n_q = 0, made[2] = {0, 0}, masked_steps = 0;
+    int live = 0;        // rows of the sequence in the step before's Value tile, where it is masked, else 0
+    uint32_t number = 0;  // and its item
+    bool had[2] = {false, false}, fresh[2] = {false, false};
+    auto output = [&](int t) -> bool {  // += weights of tile t times the Value tile of the step before
+      if (!wait(&sh.p_ready[t], made[t] & 1)) return false;
+      ++made[t];
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t v = swizzled_desc(ring + (2 * step - 1) % kSlots * C::kTile);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || k > 0);
+        mma_commit(&sh.o_done[t]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto value_there = [&]() -> bool {
+      const uint32_t load = 2 * step - 1;
+      if (!wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1)) return false;
+      if (live == 0) return true;
+      if (lane == 0) {
+        sh.scan_slot = load % kSlots;
+        sh.scan_live = live;
+        sh.scan_item = number & 1;
+        mbar_arrive(&sh.scan);
+      }
+      __syncwarp();
+      return wait(&sh.scanned, masked_steps++ & 1);
+    };
+    auto free_slot = [&](uint32_t load) {
+      if (elect_one()) mma_commit(&sh.kv_empty[load % kSlots]);
+      __syncwarp();
+    };
+    PromptItem it;
+    bool ok = true;
+    for (uint32_t n = 0; ok && take(n, it); ++n) {
+      give(n);
+      const int steps = max(it.n[0], it.n[1]);
+      if (steps == 0) continue;
+      for (int j = steps - 1; ok && j >= 0; --j) {
+        if (j == steps - 1) {
+          if (!(ok = wait(&sh.q_full, n_q & 1))) break;
+          ++n_q;
+        }
+        if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
+        if (step > 0 && !(ok = value_there())) break;
+        bool now[2], masked = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          now[t] = j < it.n[t];
+          masked |= now[t] && tile_masked(it.tok + t * per_tile, j);
+          if (had[t] && !(ok = output(t))) break;
+          if (now[t]) {
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t a = swizzled_desc(base + t * C::kTile), b = swizzled_desc(ring + 2 * step % kSlots * C::kTile);
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+                mma_16_ss(tmem + 128 * t, a + off, b + off, idesc_s, k > 0);
+              }
+              mma_commit(&sh.s_full[t]);
+            }
+            __syncwarp();
+            fresh[t] = j == it.n[t] - 1;
+          }
+        }
+        if (!ok) break;
+        had[0] = now[0];
+        had[1] = now[1];
+        live = masked ? min(128, it.tokens - 128 * j) : 0;
+        number = n;
+        if (step > 0) free_slot(2 * step - 1);
+        free_slot(2 * step);
+        if (j == 0) {
+          if (elect_one()) mma_commit(&sh.q_empty);
+          __syncwarp();
+        }
+        ++step;
+      }
+    }
+    if (ok && step > 0 && *stop == 0) {  // the last step's outputs
+      ok = value_there();
+      for (int t = 0; ok && t < 2; ++t) ok = !had[t] || output(t);
+      if (ok) free_slot(2 * step - 1);
+    }
+    if (lane == 0) {
+      sh.scan_slot = -1;
+      mbar_arrive(&sh.scan);
+    }
+    __syncwarp();
+    if (*stop != 0) {  // the products in flight, before their operands go
+      if (elect_one()) mma_commit(&sh.last);
+      __syncwarp();
+      mbar_wait_bounded(&sh.last, 0, kPromptWaitNs);
+    }
+  } else if (warp == kScanWarp) {
+    // ---------------------------------------------------------------- masked Value tiles
+    // A weight of 0 does not keep a NaN or an infinity out of a product.  Of the Value
+    // tiles that some row sees in part, rows behind the sequence are zeroed here, and a
+    // number that is not finite sends the item to prompt_row.
+    for (uint32_t n = 0; wait(&sh.scan, n & 1); ++n) {
+      const int slot = *const_cast<volatile int*>(&sh.scan_slot), live = *const_cast<volatile int*>(&sh.scan_live);
+      if (slot < 0) break;
+      uint4* tile = reinterpret_cast<uint4*>(ring_ptr + slot * C::kTile);
+      uint32_t seen = 0;
+#pragma unroll 8
+      for (int i = lane; i < C::kTile / 16; i += 32) {
+        if (i % 1024 / 8 >= live) {
+          tile[i] = make_uint4(0, 0, 0, 0);
+        } else {
+          const uint4 x = tile[i];  // an exponent of all ones carries into the sign's place
+          constexpr uint32_t kOne = kBf16 ? 0x00800080u : 0x04000400u;
+          seen |= (x.x & 0x7FFF7FFFu) + kOne;
+          seen |= (x.y & 0x7FFF7FFFu) + kOne;
+          seen |= (x.z & 0x7FFF7FFFu) + kOne;
+          seen |= (x.w & 0x7FFF7FFFu) + kOne;
+        }
+      }
+      if ((seen & 0x80008000u) != 0) sh.bad[*const_cast<volatile int*>(&sh.scan_item)] = 1;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.scanned);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, one tile a warpgroup
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
+    const int in_tile = r / p.group, head = r - in_tile * p.group;
+    // positive, so that a masked score's -inf stays one; a negative scaling negates the queries in the product
+    const float c = fmaxf(fabsf(p.scale_log2), 1e-36f);
+    uint32_t count = 0;  // score tiles so far
+    PromptItem it;
+    bool ok = true;
+    for (uint32_t n = 0; ok && take(n, it); ++n) {
+      const int t0 = it.tok + t * per_tile, token = t0 + in_tile;
+      RowState st = {-INFINITY, 0.0f};
+      for (int j = it.n[t] - 1; j >= 0; --j, ++count) {
+        if (!(ok = wait(&sh.s_full[t], count & 1))) break;
+        tc_fence_after();
+        const float fix = soften<T>(tm_s, c, tile_masked(t0, j), min(token + 1, it.tokens) - 128 * j, st);
+        if (j < it.n[t] - 1 && __any_sync(0xffffffffu, fix != 1.0f)) {
+          if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+          tc_fence_after();
+          rescale<D>(tm_o, fix);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_ready[t]);
+      }
+      if (!ok) break;
+      const bool stored = in_tile < per_tile && token < it.rows;
+      T* out = static_cast<T*>(p.out) + it.b * p.o_seq + (static_cast<int64_t>(it.first) + token) * p.o_tok +
+               (it.h * p.group + head) * p.o_head;
+      if (it.n[t] > 0) {
+        if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+        tc_fence_after();
+      }
+      if (it.n[t] > 0 && *const_cast<volatile int*>(&sh.bad[n & 1]) != 0) {
+        const T* k = static_cast<const T*>(p.k) + it.b * p.k_seq + it.first * p.k_tok + it.h * p.k_head;
+        const T* v = static_cast<const T*>(p.v) + it.b * p.v_seq + it.first * p.v_tok + it.h * p.v_head;
+        for (int i = 0; i < 32; ++i) {
+          const int x = (warp & 3) * 32 + i, tok = t0 + x / p.group, hd = it.h * p.group + x % p.group;
+          if (x >= per_tile * p.group || tok >= it.rows) break;
+          const int64_t row = static_cast<int64_t>(it.first) + tok;
+          prompt_row<T, D>(static_cast<const T*>(p.q) + it.b * p.q_seq + row * p.q_tok + hd * p.q_head, k, p.k_tok, v, p.v_tok,
+                           tok < it.tokens ? tok + 1 : 0, p.scale_log2, static_cast<T*>(p.out) + it.b * p.o_seq + row * p.o_tok + hd * p.o_head);
+        }
+      } else {
+        const bool live = it.n[t] > 0 && token < it.tokens && st.sum != 0.0f;  // else 0: a row behind the sequence
+        const float inv = 1.0f / st.sum;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          float o[32];
+          if (it.n[t] > 0) {
+            tmem_ld_x32(tm_o + 32 * i, o);
+            tmem_wait_ld();
+            tmem_settle(o);
+          }
+          if (stored) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = live ? o[x] * inv : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              uint4 w;
+              w.x = pack_two<T>(o[x], o[x + 1]);
+              w.y = pack_two<T>(o[x + 2], o[x + 3]);
+              w.z = pack_two<T>(o[x + 4], o[x + 5]);
+              w.w = pack_two<T>(o[x + 6], o[x + 7]);
+              *reinterpret_cast<uint4*>(out + 32 * i + x) = w;
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      give(n);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && sh.stop != 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_DEVICE_TIMEOUT);
 }
 
-template <typename T> static const void* prompt_kernel(int head_dim) {
-  return head_dim == 128 ? reinterpret_cast<const void*>(prompt_simple_kernel<T, 128>) : reinterpret_cast<const void*>(prompt_simple_kernel<T, 64>);
+// cuTensorMapEncodeTiled of the driver, found once.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static std::atomic<void*> known{nullptr};
+  void* f = known.load(std::memory_order_acquire);
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+      return nullptr;
+    known.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeTiled>(f);
+}
+// A map of [..] 16-bit elements: 64 channels wide boxes in the 128-byte swizzle; extents,
+// strides (elements) and box of the three dimensions over the channels.
+static bool make_map(CUtensorMap* map, const void* at, bool bf16, int D, const int64_t (&extent)[3], const int64_t (&stride)[3],
+                     const int (&box)[3]) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D)}, strides[3];
+  cuuint32_t boxes[4] = {64}, ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(extent[i]);
+    strides[i] = static_cast<cuuint64_t>(extent[i] > 1 ? stride[i] : D) * 2;
+    boxes[i + 1] = static_cast<cuuint32_t>(box[i]);
+  }
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(at), dims, strides, boxes,
+                ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+static const void* prompt_kernel_of(int head_dim) {
+  return head_dim == 128 ? reinterpret_cast<const void*>(prompt_kernel<T, 128>) : reinterpret_cast<const void*>(prompt_kernel<T, 64>);
 }
 
 }  // namespace lf
@@ -144,12 +590,33 @@ extern "C" int lf_prompt_attend(const lf_prompt* a, lf_stream_t stream) {
   p.n_q = a->n_q;
   p.n_kv = a->n_kv;
   p.group = a->n_q / a->n_kv;
-  const int64_t rows = (static_cast<int64_t>(a->tokens) + 7) / 8;
-  void* args[] = {&p};
-  const cudaError_t err = launch_programmatic(
-      a->dtype == LF_F16 ? prompt_kernel<__half>(a->head_dim) : prompt_kernel<__nv_bfloat16>(a->head_dim),
-      dim3(static_cast<unsigned>(rows < 65535 ? rows : 65535), a->n_q, a->batch < 65535 ? a->batch : 65535), dim3(256), 0,
-      reinterpret_cast<cudaStream_t>(stream), args);
+  const int sms = sm_count();
+  if (sms <= 0) {
+    set_error("lf_prompt_attend: the current device's SMs cannot be counted");
+    return LF_ERR_CUDA;
+  }
+  const bool packed = a->starts != nullptr, bf16 = a->dtype == LF_BF16;
+  const int per_tile = 128 / p.group, batches = packed ? 1 : a->batch;
+  CUtensorMap q_map, k_map, v_map;
+  if (!make_map(&q_map, a->q, bf16, a->head_dim, {a->n_q, a->tokens, batches}, {p.q_head, p.q_tok, p.q_seq}, {p.group, per_tile, 1}) ||
+      !make_map(&k_map, a->k, bf16, a->head_dim, {a->tokens, a->n_kv, batches}, {p.k_tok, p.k_head, p.k_seq}, {128, 1, 1}) ||
+      !make_map(&v_map, a->v, bf16, a->head_dim, {a->tokens, a->n_kv, batches}, {p.v_tok, p.v_head, p.v_seq}, {128, 1, 1})) {
+    set_error("lf_prompt_attend: the driver makes no tensor map of these rows");
+    return LF_ERR_CUDA;
+  }
+  // No more CTAs than items there can be (of sequences that do not overlap).
+  const int64_t span = 2 * per_tile;
+  const int64_t items = (packed ? a->tokens / span + a->batch : (a->tokens + span - 1) / span * a->batch) * a->n_kv;
+  const void* kern = bf16 ? prompt_kernel_of<__nv_bfloat16>(a->head_dim) : prompt_kernel_of<__half>(a->head_dim);
+  const int smem = a->head_dim == 128 ? PromptCfg<128>::kSmem : PromptCfg<64>::kSmem;
+  cudaError_t err = raise_smem_limit(kern, smem, true);
+  if (err != cudaSuccess) {
+    set_error("lf_prompt_attend: %s", cudaGetErrorString(err));
+    return LF_ERR_CUDA;
+  }
+  void* args[] = {&p, &q_map, &k_map, &v_map};
+  err = launch_programmatic(kern, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kPromptThreads), smem,
+                            reinterpret_cast<cudaStream_t>(stream), args);
   if (err != cudaSuccess) {
     set_error("lf_prompt_attend: %s", cudaGetErrorString(err));
     return LF_ERR_LAUNCH;

@@ -258,7 +258,7 @@ def _check_prompts(got, q, k, v, counts, scaling, dtype):
         if c:
             want, bound = _one(q[at:at + c], k[at:at + c], v[at:at + c], scaling, dtype)
             off = (got[at:at + c].double() - want).abs() - bound
-            assert bool((off <= 0).all()), f"{c} tokens: outside by {float(off.max()):.3g} at {(off == off.max()).nonzero()[0].tolist()}"
+            assert bool((off <= 0).all()), f"{c} tokens: outside by {float(off.max()):.3g} in {int((off > 0).sum())} places, {int(off.isnan().sum())} NaN"
         at += c
 
 
@@ -351,7 +351,12 @@ def test_scalings_of_any_sign_and_size(scaling, dtype):
     got = prompt.prompt_attention(q, k, v, scaling, starts=_starts([200, 77]))
     if abs(scaling) < 1:
         _check_prompts(got, q, k, v, [200, 77], scaling, dtype)
-    else:   # one token takes nearly all: where the best leads by more than the scores' error, it is the result
+    else:
+        # One token takes nearly all: where the best leads by more than the scores' error, it is the result.
+        # (First asked for to the last bit, which is wrong: its weight w, any number near the running maximum's,
+        # enters the product with Value as w (1 + d), |d| <= u, half a step of the type, and the sum in fp32 as
+        # w; the quotient v (1 + d) is then rounded once more: u |v| + u |v| (1 + u) in all.)
+        u = HALF_STEP[dtype]
         at = 0
         for c in (200, 77):
             for h in range(4):
@@ -362,8 +367,8 @@ def test_scalings_of_any_sign_and_size(scaling, dtype):
                 best = logits.topk(2, -1)
                 sure = best.values[:, 0] - best.values[:, 1] > 30 + 2 * e
                 assert int(sure.sum()) > c // 3
-                want = v[at:at + c, h // 2][best.indices[:, 0]]
-                assert torch.equal(got[at:at + c, h][sure], want[sure])
+                want = v[at:at + c, h // 2][best.indices[:, 0]].double()
+                assert bool(((got[at:at + c, h].double() - want).abs() <= (2 * u + 2 * u * u) * want.abs() + 2.0 ** -24)[sure].all())
             at += c
 
 
@@ -400,7 +405,7 @@ def test_scores_that_rise_and_fall(rising):
 def test_non_finite_rows_reach_only_who_sees_them(dtype, D, value, where):
     counts = [300, 140]
     q, k, v = _prompts(7, counts, 6, 2, D, dtype)
-    clean = prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts))
+    want = [torch.cat(x) for x in zip(*(_one(q[a:b], k[a:b], v[a:b], D ** -0.5, dtype) for a, b in ((0, 300), (300, 440))))]
     at = 133                      # inside a tile, of the first sequence, KV head 1
     dict(key=k, value=v, query=q)[where][at, 1, 5] = value
     got = prompt.prompt_attention(q, k, v, D ** -0.5, starts=_starts(counts))
@@ -411,7 +416,8 @@ def test_non_finite_rows_reach_only_who_sees_them(dtype, D, value, where):
         touched[at:300, 3:] = True
     else:
         touched[at:300, 3:, 5] = True
-    assert torch.equal(got[~touched], clean[~touched])
+    off = (got.double() - want[0]).abs() - want[1]     # tiles with such a row may be summed in another way: not bit for bit
+    assert bool((off[~touched] <= 0).all())
     if where == "value":
         assert not bool(torch.isfinite(got[touched]).any())
     elif math.isnan(value):
