@@ -455,6 +455,29 @@ LF_API int lf_int4_attend(const lf_int4_query* args, lf_stream_t stream);
  * the pages are those of the negated queries: the largest bounds on scaling q . K. */
 LF_API int lf_int4_attend_sparse(const lf_int4_query* args, lf_stream_t stream);
 
+/* Arguments of lf_int4_attend_prefix: those of lf_int4_attend (picked and its slots not
+ * read), and the sequences that share their first pages. */
+typedef struct lf_int4_prefix {
+  lf_int4_query query;
+  const int32_t* group;   /* [batch] group of each sequence; outside [0, groups): none */
+  const int32_t* shared;  /* [groups] first pages that a group's sequences share  */
+  void* workspace;        /* of its own, beside the query's                       */
+  size_t workspace_bytes;
+  int32_t groups;
+} lf_int4_prefix;
+
+/*
+ * lf_int4_attend for sequences that share a prefix.  The first shared[g] entries of the
+ * page table's rows are the same for all sequences of group g (the row of its lowest
+ * sequence is read), so these pages are read and unpacked once for all queries of the
+ * group.  The result is lf_int4_attend's, up to the order of its sums; a sequence that
+ * sees only part of its shared pages, or is in no group, is attended as well.
+ * workspace: lf_int4_prefix_workspace_bytes bytes, 16-byte aligned, of any content; calls
+ * that overlap on the GPU need one each (of both).
+ */
+LF_API int lf_int4_attend_prefix(const lf_int4_prefix* args, lf_stream_t stream);
+LF_API size_t lf_int4_prefix_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim, int groups);
+
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);
 LF_API size_t lf_int4_workspace_clear_from(void);
 

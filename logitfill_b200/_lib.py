@@ -92,6 +92,8 @@ def lib() -> ctypes.CDLL:
         "lf_int4_select": (c_int, [Q, P]),
         "lf_int4_attend": (c_int, [Q, P]),
         "lf_int4_attend_sparse": (c_int, [Q, P]),
+        "lf_int4_attend_prefix": (c_int, [Q, P]),
+        "lf_int4_prefix_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
         "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
         "lf_rotary_embed": (c_int, [Q, P]),

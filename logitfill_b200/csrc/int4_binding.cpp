@@ -92,9 +92,10 @@ struct Scratch {
   at::Tensor words;
   size_t bytes = 0;
 };
+using Held = std::map<std::pair<int, cudaStream_t>, Scratch>;
 Scratch workspace(const lf_int4_query& a, const Launch& on) {
   static std::mutex mu;
-  static auto* held = new std::map<std::pair<int, cudaStream_t>, Scratch>;  // outlives the CUDA context's teardown
+  static auto* held = new Held;  // outlives the CUDA context's teardown
   const size_t need = lf_int4_workspace_bytes(a.pool.batch, a.pool.kv_heads, a.n_q, a.q_len, a.head_dim);
   const auto options = at::TensorOptions().dtype(at::kByte).device(on.stream.device());
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
@@ -109,6 +110,20 @@ Scratch workspace(const lf_int4_query& a, const Launch& on) {
     s.words = at::zeros({static_cast<int64_t>(room)}, options);
     s.bytes = room;
   }
+  return s;
+}
+
+// The same for the records of calls with shared pages, whose content does not matter.
+Scratch prefix_workspace(const lf_int4_query& a, int groups, const Launch& on) {
+  static std::mutex mu;
+  static auto* held = new Held;
+  const size_t need = lf_int4_prefix_workspace_bytes(a.pool.batch, a.pool.kv_heads, a.n_q, a.q_len, a.head_dim, groups);
+  const auto options = at::TensorOptions().dtype(at::kByte).device(on.stream.device());
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return Scratch{at::empty({static_cast<int64_t>(need)}, options), need};
+  std::lock_guard<std::mutex> lock(mu);
+  Scratch& s = (*held)[{on.stream.device_index(), on.stream.stream()}];
+  if (s.bytes < need) s = Scratch{at::empty({static_cast<int64_t>(need)}, options), need};
   return s;
 }
 
@@ -203,6 +218,61 @@ PyObject* read_bounds(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// Query, lengths, counts, status and scaling of an attention call; returns the query as it is read.
+at::Tensor fill_query(lf_int4_query& a, const Pool& p, PyObject* query_o, PyObject* lengths, PyObject* scaling_o, PyObject* counts,
+                      PyObject* status) {
+  const at::Tensor& query = tensor(query_o, "query");
+  const int64_t B = p.c.batch, H = p.c.kv_heads, D = p.head_dim;
+  if ((query.dim() != 3 && query.dim() != 4) || query.size(0) != B || query.size(-1) != D || query.size(1) < 1 ||
+      query.numel() == 0)
+    fail(PyExc_ValueError, "query must be [", B, ", n_q, ", D, "] or [", B, ", n_q, q_len, ", D, "], got ", shape(query));
+  if (query.size(1) % H) fail(PyExc_ValueError, query.size(1), " query heads do not divide into ", H, " KV heads");
+  if (query.scalar_type() != at::kHalf && query.scalar_type() != at::kBFloat16)
+    fail(PyExc_NotImplementedError, "the 4-bit cache's attention takes fp16 or bf16 queries, got ",
+         c10::toString(query.scalar_type()));
+  if (query.device() != p.device) fail(PyExc_RuntimeError, "query is on ", query.device(), ", pages on ", p.device);
+  int64_t s[3];
+  const at::Tensor q = aligned_rows(query.dim() == 4 ? query : query.unsqueeze(2), s);
+  if (q.size(1) > INT32_MAX || q.size(2) > INT32_MAX) fail(PyExc_NotImplementedError, "too many queries");
+  a.pool = p.c;
+  a.q = q.data_ptr();
+  a.q_seq_stride = s[0];
+  a.q_head_stride = s[1];
+  a.q_tok_stride = s[2];
+  a.lengths = per_sequence(lengths, "lengths", p, false);
+  a.counts = per_sequence(counts, "counts", p, true);
+  a.status = status_word(status, p);
+  a.head_dim = p.head_dim;
+  a.dtype = type_code(q.scalar_type());
+  a.n_q = static_cast<int32_t>(q.size(1));
+  a.q_len = static_cast<int32_t>(q.size(2));
+  const double scaling = PyFloat_AsDouble(scaling_o);
+  if (scaling == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    fail(PyExc_TypeError, "scaling must be a number");
+  }
+  a.scaling = static_cast<float>(scaling);
+  return q;
+}
+
+// The output of an attention call: the caller's, or a new one.
+at::Tensor fill_out(lf_int4_query& a, const Pool& p, PyObject* out_o, const at::Tensor& query) {
+  at::Tensor out;
+  if (out_o == Py_None) {
+    out = at::empty(query.sizes(), query.options());
+  } else {
+    out = tensor(out_o, "out");
+    if (out.sizes() != query.sizes() || out.scalar_type() != query.scalar_type() || out.device() != p.device ||
+        out.stride(-1) != 1)
+      fail(PyExc_ValueError, "out must be like the query (", shape(query), ") with channel stride 1, got ", shape(out));
+  }
+  a.out = out.data_ptr();
+  a.out_seq_stride = p.c.batch > 1 ? out.stride(0) : 0;
+  a.out_head_stride = out.size(1) > 1 ? out.stride(1) : 0;
+  a.out_tok_stride = out.dim() == 4 && out.size(2) > 1 ? out.stride(2) : 0;
+  return out;
+}
+
 // attend(query, pages, page_table, lengths, scaling, counts, out, status) -> out
 // With (bounds, top, sink, recent) after these: chosen pages only, -> (out, picked).
 // With (bounds, top, sink, recent, True): only the choice, -> picked.
@@ -211,38 +281,9 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (n != 8 && n != 12 && n != 13) expect(n, 12);
     const bool sparse = n > 8, choose_only = n == 13 && PyObject_IsTrue(v[12]) == 1;
     const Pool p = make_pool(v[1], v[2]);
-    const at::Tensor& query = tensor(v[0], "query");
-    const int64_t B = p.c.batch, H = p.c.kv_heads, D = p.head_dim;
-    if ((query.dim() != 3 && query.dim() != 4) || query.size(0) != B || query.size(-1) != D || query.size(1) < 1 ||
-        query.numel() == 0)
-      fail(PyExc_ValueError, "query must be [", B, ", n_q, ", D, "] or [", B, ", n_q, q_len, ", D, "], got ", shape(query));
-    if (query.size(1) % H) fail(PyExc_ValueError, query.size(1), " query heads do not divide into ", H, " KV heads");
-    if (query.scalar_type() != at::kHalf && query.scalar_type() != at::kBFloat16)
-      fail(PyExc_NotImplementedError, "the 4-bit cache's attention takes fp16 or bf16 queries, got ",
-           c10::toString(query.scalar_type()));
-    if (query.device() != p.device) fail(PyExc_RuntimeError, "query is on ", query.device(), ", pages on ", p.device);
-    int64_t s[3];
-    const at::Tensor q = aligned_rows(query.dim() == 4 ? query : query.unsqueeze(2), s);
-    if (q.size(1) > INT32_MAX || q.size(2) > INT32_MAX) fail(PyExc_NotImplementedError, "too many queries");
     lf_int4_query a{};
-    a.pool = p.c;
-    a.q = q.data_ptr();
-    a.q_seq_stride = s[0];
-    a.q_head_stride = s[1];
-    a.q_tok_stride = s[2];
-    a.lengths = per_sequence(v[3], "lengths", p, false);
-    a.counts = per_sequence(v[5], "counts", p, true);
-    a.status = status_word(v[7], p);
-    a.head_dim = p.head_dim;
-    a.dtype = type_code(q.scalar_type());
-    a.n_q = static_cast<int32_t>(q.size(1));
-    a.q_len = static_cast<int32_t>(q.size(2));
-    const double scaling = PyFloat_AsDouble(v[4]);
-    if (scaling == -1.0 && PyErr_Occurred()) {
-      PyErr_Clear();
-      fail(PyExc_TypeError, "scaling must be a number");
-    }
-    a.scaling = static_cast<float>(scaling);
+    const at::Tensor q = fill_query(a, p, v[0], v[3], v[4], v[5], v[7]);
+    const int64_t B = p.c.batch, H = p.c.kv_heads;
     const Launch on(p.device);
 
     at::Tensor picked;
@@ -265,19 +306,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
       }
     }
 
-    at::Tensor out;
-    if (v[6] == Py_None) {
-      out = at::empty(query.sizes(), query.options());
-    } else {
-      out = tensor(v[6], "out");
-      if (out.sizes() != query.sizes() || out.scalar_type() != query.scalar_type() || out.device() != p.device ||
-          out.stride(-1) != 1)
-        fail(PyExc_ValueError, "out must be like the query (", shape(query), ") with channel stride 1, got ", shape(out));
-    }
-    a.out = out.data_ptr();
-    a.out_seq_stride = B > 1 ? out.stride(0) : 0;
-    a.out_head_stride = out.size(1) > 1 ? out.stride(1) : 0;
-    a.out_tok_stride = out.dim() == 4 && out.size(2) > 1 ? out.stride(2) : 0;
+    at::Tensor out = fill_out(a, p, v[6], tensor(v[0], "query"));
     const Scratch scratch = workspace(a, on);
     a.workspace = scratch.words.data_ptr();
     a.workspace_bytes = scratch.bytes;
@@ -290,10 +319,37 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// attend_prefix(query, pages, page_table, lengths, scaling, group, shared, counts, out, status) -> out
+PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect(n, 10);
+    const Pool p = make_pool(v[1], v[2]);
+    lf_int4_prefix a{};
+    const at::Tensor q = fill_query(a.query, p, v[0], v[3], v[4], v[7], v[9]);
+    a.group = per_sequence(v[5], "prefix_group", p, false);
+    const at::Tensor& shared = tensor(v[6], "prefix_pages");
+    if (shared.scalar_type() != at::kInt || shared.dim() != 1 || shared.device() != p.device || !shared.is_contiguous())
+      fail(PyExc_ValueError, "prefix_pages must be a contiguous int32 [groups] tensor on ", p.device, ", got ", shape(shared));
+    if (shared.size(0) > INT32_MAX) fail(PyExc_NotImplementedError, "too many groups");
+    a.shared = static_cast<const int32_t*>(shared.data_ptr());
+    a.groups = static_cast<int32_t>(shared.size(0));
+    const Launch on(p.device);
+    at::Tensor out = fill_out(a.query, p, v[8], tensor(v[0], "query"));
+    const Scratch scratch = workspace(a.query, on), records = prefix_workspace(a.query, a.groups, on);
+    a.query.workspace = scratch.words.data_ptr();
+    a.query.workspace_bytes = scratch.bytes;
+    a.workspace = records.words.data_ptr();
+    a.workspace_bytes = records.bytes;
+    check(lf_int4_attend_prefix(&a, on.raw()), "lf_int4_attend_prefix");
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyMethodDef methods[] = {{"write", fast(write), METH_FASTCALL, nullptr},
                          {"read", fast(read), METH_FASTCALL, nullptr},
                          {"read_bounds", fast(read_bounds), METH_FASTCALL, nullptr},
                          {"attend", fast(attend), METH_FASTCALL, nullptr},
+                         {"attend_prefix", fast(attend_prefix), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "int4_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

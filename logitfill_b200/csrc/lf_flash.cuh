@@ -5,6 +5,7 @@
 
 #include <cuda.h>
 
+#include "lf_common.cuh"
 #include "lf_tcgen05.cuh"
 
 namespace lf {
@@ -101,6 +102,22 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// Wait of a whole warp for a barrier's phase, with a limit: false once a wait of this CTA
+// has given up (*stop), for all lanes alike.
+constexpr uint64_t kTileWaitNs = 2000000000ull;
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t n = 1; !ok; ++n) {
+      ok = mbar_try_wait(bar, parity);
+      if (!ok && (n & 63u) == 0u && (*stop != 0 || globaltimer_ns() - t0 > kTileWaitNs)) break;
+    }
+    if (!ok) *stop = 1;
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 
 // The softmax of one 128 x 128 tile of scores, row by row (a thread to a row, TMEM lane =

@@ -81,8 +81,34 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+// Sequences that share their first pages (lf_int4_prefix.cu): what the plan kernel leaves
+// for the kernels behind it, in the call's workspace.
+struct PrefixGroup {
+  int pages;       // shared pages that are read once for the group (0: none)
+  int live;        // 0: a page was met that its members have to read themselves
+  int members, count;
+  int units, places;  // first unit, first place in the line of steps
+  int tiles, steps;   // row tiles of a KV head, Key tiles of a unit
+};
+struct PrefixSeq { int group, rank; };  // group -1: no shared pages
+struct PrefixPlan {
+  int* head;            // places in all, places of a CTA's range
+  PrefixGroup* groups;
+  PrefixSeq* seqs;
+  int* members;
+  float* records;
+};
+constexpr int kPrefixRows = 256;    // rows (query token, q-head) of a unit
+constexpr int kPrefixCost = 2;      // empty places before a unit's steps
+// Floats of a record: maxima, sums, accumulators.
+__host__ __device__ constexpr int64_t prefix_record(int D) { return kPrefixRows * (static_cast<int64_t>(D) + 2); }
+
 // Checks the C ABI's pool and copies it for a kernel (lf_int4_write.cu).
 int check_int4_pool(const char* what, const lf_int4_pool& pool, int head_dim, Int4Pool& out);
+// The suffix of a call with shared pages: lf_int4_attend from the shared pages' end on, and
+// the merge (lf_int4_attend.cu).
+int check_int4_attend(const lf_int4_query* a);
+int int4_attend_suffix(const lf_int4_query* a, const PrefixPlan& plan, cudaStream_t stream);
 // lf_int4_select's checks alone, and the call itself for the queries times sign (1 or
 // -1) (lf_int4_select.cu).
 int check_int4_select(const lf_int4_query* a);

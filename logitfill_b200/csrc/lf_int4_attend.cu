@@ -70,6 +70,7 @@ struct AttendParams {
   uint32_t* tickets;
   int32_t* status;
   int sms;  // of the device (for the launch)
+  PrefixPlan prefix;  // of a call with shared pages
 };
 
 constexpr int kTile = 16;             // tokens of one tensor-core step
@@ -262,12 +263,44 @@ __device__ __forceinline__ int row_tokens(const AttendParams& p, int r) {
   const int length = p.lengths[b], count = p.counts != nullptr ? p.counts[b] : p.q_len;
   return int4_seen(length, count, kSparse ? r - b * p.q_len : max(0, min(count, p.q_len) - 1));
 }
-// Pages of a row that sees `tokens`, at least 1, so that an empty row is visited
+// Pages of a row that sees `tokens`, behind its shared ones, at least 1, so that an empty row is visited
 // and zeroed.
 template <bool kSparse>
-__device__ __forceinline__ int row_pages(const AttendParams& p, int tokens) {
+__device__ __forceinline__ int row_pages(const AttendParams& p, int tokens, int shared) {
   const int n = tokens / kInt4Page + (tokens % kInt4Page != 0);
-  return max(1, min(n, kSparse ? p.slots : p.pool.table_width));
+  return max(1, min(n, kSparse ? p.slots : p.pool.table_width) - shared);
+}
+
+// Shared pages of sequence b, which are not among its own here.
+template <bool kPrefix>
+__device__ __forceinline__ int shared_pages(const AttendParams& p, int b) {
+  if constexpr (!kPrefix) return 0;
+  const int g = p.prefix.seqs[b].group;
+  return g >= 0 && p.prefix.groups[g].live != 0 ? p.prefix.groups[g].pages : 0;
+}
+
+// Adds the shared pages' part of row r of a group (KV head h, channels d .. d + 3) to a
+// maximum, sum and accumulators.
+template <int D>
+__device__ __forceinline__ void add_shared(const PrefixPlan& plan, const PrefixGroup& g, int h, int r, int d, float& top, float& sum, float4& v) {
+  const int unit = h * g.tiles + r / kPrefixRows, in = r % kPrefixRows, per = plan.head[1];
+  const int start = g.places + unit * (g.steps + kPrefixCost) + kPrefixCost;
+  const int first = start / per, n = (start + g.steps - 1) / per - first + 1;
+  const float* rec = plan.records + (g.units + unit + first) * prefix_record(D) + in;
+  float now = top;
+#pragma unroll 4
+  for (int x = 0; x < n; ++x) now = fmaxf(now, rec[x * prefix_record(D)]);
+  const float fix = ex2(top - now);
+  sum *= fix;
+  v = make_float4(v.x * fix, v.y * fix, v.z * fix, v.w * fix);
+  top = now;
+#pragma unroll 4
+  for (int x = 0; x < n; ++x) {
+    const float* at = rec + x * prefix_record(D);
+    const float f = ex2(at[0] - now);
+    sum = fmaf(f, at[kPrefixRows], sum);
+    add_scaled(v, f, *reinterpret_cast<const float4*>(at - in + 2 * kPrefixRows + static_cast<int64_t>(in) * D + d));
+  }
 }
 
 // Places of a range below which the merge costs more than the range: with n pages
@@ -281,6 +314,7 @@ __device__ __forceinline__ int merge_pages(int total, int units) {
 struct Unit {
   int b, h, c0, i0, first, stop, length, count, seen_max, vis_min;
   const int32_t* listed;  // pages of a sparse unit
+  int shared;             // pages before its first
 };
 // Value groups that stayed out of the products of a warp's pages, added in fp32 to its
 // sums in the merge buffer: those that may pass the fp16 range (scaled to fit it, they
@@ -306,7 +340,7 @@ __device__ __noinline__ void add_apart(const AttendParams& p, const Unit& u, con
   }
 #pragma unroll 1
   for (int place = u.first + (threadIdx.x >> 6); place < u.stop; place += AttendCfg<D, NT>::kTeams) {
-    const int page = kSparse ? u.listed[place] : place;
+    const int page = kSparse ? u.listed[place] : u.shared + place;
     if (page < 0 || page > (u.seen_max - 1) / kInt4Page) continue;  // (seen_max > 0: there was a group to add)
     const int id = int4_page_id(p.pool, u.b, page), base = page * kInt4Page + part * kPart;
     if (id < 0 || base >= u.seen_max) continue;
@@ -352,7 +386,7 @@ __device__ __noinline__ void add_apart(const AttendParams& p, const Unit& u, con
   }
 }
 
-template <typename T, int D, int NT, bool kSparse>
+template <typename T, int D, int NT, bool kSparse, bool kPrefix>
 __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::kCtas)
     int4_attend_kernel(const __grid_constant__ AttendParams p) {
   using C = AttendCfg<D, NT>;
@@ -371,7 +405,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 
   // The line of pages: its length, and the row where this CTA's range begins.
   auto places = [&](int r) {
-    return r < p.rows ? (row_pages<kSparse>(p, row_tokens<kSparse>(p, r)) + kUnitCost) * per_row : 0;
+    return r < p.rows ? (row_pages<kSparse>(p, row_tokens<kSparse>(p, r), shared_pages<kPrefix>(p, r)) + kUnitCost) * per_row : 0;
   };
   const int places0 = places(lane);
   int total = __reduce_add_sync(0xffffffffu, places0);
@@ -408,7 +442,8 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   int at = begin;
   while (at < end) {
     // ------------------------------------------------------------ one unit
-    const int seen_max = row_tokens<kSparse>(p, row), n_pages = row_pages<kSparse>(p, seen_max);
+    const int shared = shared_pages<kPrefix>(p, row);
+    const int seen_max = row_tokens<kSparse>(p, row), n_pages = row_pages<kSparse>(p, seen_max, shared);
     const int in_row = at - row_base, unit_in_row = in_row / (n_pages + kUnitCost);
     const int unit_begin = row_base + unit_in_row * (n_pages + kUnitCost) + kUnitCost;  // its first page's place
     const int unit_end = unit_begin + n_pages;
@@ -452,7 +487,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         if ((issued & 31) == 0) {
           ids = logicals = -1;
           if (issued + lane < mine_n) {
-            logicals = first + team + (issued + lane) * C::kTeams;
+            logicals = shared + first + team + (issued + lane) * C::kTeams;
             if constexpr (kSparse) logicals = listed[logicals];
             if (logicals >= 0 && seen_max > 0 && logicals <= (seen_max - 1) / kInt4Page) {
               ids = int4_page_id(p.pool, b, logicals);
@@ -557,7 +592,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     }
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
-    if (tid == 0) unit_s = Unit{b, h, c0, i0, first, stop, length, count, seen_max, vis_min, listed};
+    if (tid == 0) unit_s = Unit{b, h, c0, i0, first, stop, length, count, seen_max, vis_min, listed, shared};
     if (lane == 0) apart_s[warp] = 0;
     float acc[NT][2 * kG][4], back[NT][2], l[NT][2];  // back: the running maxima, negated, times 2^-14
     bool fresh = true;  // before the first part
@@ -813,6 +848,15 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       Scalar<T>::store(f.x + 3, v.w * inv);
       *reinterpret_cast<Four*>(o) = f;
     };
+    // What the shared pages gave, with a thread's share of the result in hand.
+    auto with_shared = [&](int col, int d, float& top, float& sum, float4& v) {
+      if constexpr (kPrefix) {
+        if (shared > 0 && c0 + col < p.cols) {
+          const PrefixSeq s = p.prefix.seqs[b];
+          add_shared<D>(p.prefix, p.prefix.groups[s.group], h, s.rank * p.cols + c0 + col, d, top, sum, v);
+        }
+      }
+    };
     // The partial of range x of this unit: the range that begins inside the unit
     // uses its CTA's first record, the unit's first range the second.
     const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per, parts = last_cta - first_cta + 1;
@@ -833,6 +877,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         add_scaled(v, f, *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d));
       }
       if (whole) {
+        with_shared(col, d, top, sum, v);
         store(col, d, v, sum);
       } else {
         *reinterpret_cast<float4*>(mine + 2 * kCol + col * D + d) = v;
@@ -901,6 +946,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {
           const int item = tid + it * C::kThreads;
+          with_shared(item / (D / 4), item % (D / 4) * 4, top[it], sum[it], v[it]);
           store(item / (D / 4), item % (D / 4) * 4, v[it], sum[it]);
         }
       }
@@ -919,10 +965,10 @@ static size_t partial_bytes(int sms) {
   return static_cast<size_t>(sms) * 2 * most * sizeof(float);
 }
 
-template <typename T, int D, int NT, bool kSparse>
+template <typename T, int D, int NT, bool kSparse, bool kPrefix = false>
 static int launch_attend(AttendParams p, cudaStream_t stream) {
   using C = AttendCfg<D, NT>;
-  const void* kern = reinterpret_cast<const void*>(int4_attend_kernel<T, D, NT, kSparse>);
+  const void* kern = reinterpret_cast<const void*>(int4_attend_kernel<T, D, NT, kSparse, kPrefix>);
   cudaError_t err = raise_smem_limit(kern, C::kSmem, true);
   if (err != cudaSuccess) {
     set_error("lf_int4_attend: %s", cudaGetErrorString(err));
@@ -948,6 +994,8 @@ static int launch_attend(AttendParams p, cudaStream_t stream) {
 // drafts 28.2 us, 25.2 in two tiles of 16.
 template <typename T, int D>
 static int launch_attend_by(const AttendParams& p, cudaStream_t stream) {
+  if (p.prefix.head != nullptr)
+    return p.cols <= 8 ? launch_attend<T, D, 1, false, true>(p, stream) : launch_attend<T, D, 2, false, true>(p, stream);
   if (p.cols <= 8)
     return p.picked ? launch_attend<T, D, 1, true>(p, stream) : launch_attend<T, D, 1, false>(p, stream);
   return p.picked ? launch_attend<T, D, 2, true>(p, stream) : launch_attend<T, D, 2, false>(p, stream);
@@ -1023,6 +1071,7 @@ static int check_attend(const lf_int4_query* a, AttendParams& p) {
   p.partials = static_cast<float*>(a->workspace);
   p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + partial_bytes(p.sms));
   p.status = a->status;
+  p.prefix = PrefixPlan{};
   return LF_OK;
 }
 
@@ -1030,6 +1079,19 @@ static int launch_attend(const lf_int4_query* a, const AttendParams& p, lf_strea
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a->dtype == LF_F16) return a->head_dim == 128 ? launch_attend_by<__half, 128>(p, s) : launch_attend_by<__half, 64>(p, s);
   return a->head_dim == 128 ? launch_attend_by<__nv_bfloat16, 128>(p, s) : launch_attend_by<__nv_bfloat16, 64>(p, s);
+}
+
+int check_int4_attend(const lf_int4_query* a) {
+  AttendParams p;
+  return check_attend(a, p);
+}
+
+int int4_attend_suffix(const lf_int4_query* a, const PrefixPlan& plan, cudaStream_t stream) {
+  AttendParams p;
+  const int bad = check_attend(a, p);
+  if (bad != LF_OK) return bad;
+  p.prefix = plan;
+  return launch_attend(a, p, reinterpret_cast<lf_stream_t>(stream));
 }
 
 }  // namespace lf

@@ -1,0 +1,618 @@
+// Attention over the 4-bit paged cache for sequences that share their first pages
+// (lf_int4_attend_prefix).
+//
+// Mathematics.  The shared tokens' part of a row's softmax (maximum, sum, accumulators)
+// is the same sum whether the row's sequence holds the pages or another does.  So the
+// queries of all sequences of a group are the rows of one product with the shared Keys,
+// one with the shared Values, and what lf_int4_attend would have read for every sequence
+// is read and unpacked once for 256 rows.  Three kernels:
+//   plan     the groups' members, and the line of all Key tiles of all units (256 rows of a
+//            KV head of a group), cut into equal ranges, one per CTA;
+//   prefix   the shared pages: every (unit, range) leaves a record of maxima, sums and
+//            accumulators;
+//   suffix   lf_int4_attend's kernel from the shared pages' end on, whose last step adds
+//            the unit's records (lf_int4_attend.cu).
+//
+// The product runs on tcgen05 with fp16 operands.  Codes become fp16 numbers code * s + z,
+// rounded once (2^-11); the queries of a row are scaled by a power of two, so that bf16 and
+// fp16 enter exactly.  A group whose numbers may pass the fp16 range (s 2^11 or |z| 2^15 at
+// least), or with a NaN, is not brought into it: the group of sequences is marked, and its
+// members read these pages themselves, in the suffix kernel, which can do that.
+//
+// Order of channels.  A word's nibbles n and n + 4 lie in one fp16 pair (w >> 4 n) &
+// 0x000f000f.  For Key, a sum over channels has no order: Keys and queries both take the
+// channels of a group of 8 as (0, 4), (1, 5), (2, 6), (3, 7).  For Value, the two are
+// channels 32 apart; the accumulators' columns come in the codes' order, and the record is
+// written in the channels'.
+#include <cmath>
+#include <type_traits>
+
+#include "lf_flash.cuh"
+#include "lf_int4.cuh"
+
+namespace lf {
+
+using namespace sm100;
+
+struct PrefixParams {
+  Int4Pool pool;
+  const void* q;
+  int64_t q_seq, q_head, q_tok;
+  int q_len, heads;               // query heads of a KV head
+  const int32_t *lengths, *counts, *group, *shared;
+  int groups, grid;
+  float scale_log2;
+  int32_t* status;
+  PrefixPlan plan;
+};
+
+// -------------------------------------------------------------------- plan
+
+constexpr int kMaxGroups = 4096;
+
+// Shared pages of group g that its `count` members read together.  One member with few
+// rows has nothing to share.
+__device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int count) {
+  if (count == 0 || (count == 1 && p.q_len * p.heads <= 16)) return 0;
+  return min(max(p.shared[g], 0), p.pool.table_width);
+}
+
+__global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_constant__ PrefixParams p) {
+  __shared__ int count_s[kMaxGroups], first_s[kMaxGroups];
+  const int lane = threadIdx.x;
+  grid_dep_wait();
+  for (int g = lane; g < p.groups; g += 32) count_s[g] = 0;
+  __syncwarp();
+  // Each sequence's rank among its group's.
+  for (int b0 = 0; b0 < p.pool.batch; b0 += 32) {
+    const int b = b0 + lane;
+    int g = b < p.pool.batch ? p.group[b] : -1;
+    if (g >= p.groups) g = -1;
+    if (g < 0) g = -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, g);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    const int rank = g >= 0 ? count_s[g] + before : -1;
+    __syncwarp();
+    if (g >= 0 && before == 0) count_s[g] += __popc(same);
+    __syncwarp();
+    if (b < p.pool.batch) p.plan.seqs[b] = PrefixSeq{g, rank};
+  }
+  // The groups' places in the lists and in the line.
+  int members = 0, units = 0, places = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    const int count = g < p.groups ? count_s[g] : 0;
+    const int pages = g < p.groups ? group_pages(p, g, count) : 0;
+    const int tiles = pages > 0 ? (count * p.q_len * p.heads + kPrefixRows - 1) / kPrefixRows : 0, steps = (pages + 1) / 2;
+    const int n_units = tiles * p.pool.kv_heads, n_places = n_units * (steps + kPrefixCost);
+    int m = count, u = n_units, x = n_places;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, m, o), b = __shfl_up_sync(0xffffffffu, u, o), c = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) {
+        m += a;
+        u += b;
+        x += c;
+      }
+    }
+    if (g < p.groups) {
+      first_s[g] = members + m - count;
+      p.plan.groups[g] = PrefixGroup{pages, pages > 0, members + m - count, count, units + u - n_units, places + x - n_places, tiles, steps};
+    }
+    members += __shfl_sync(0xffffffffu, m, 31);
+    units += __shfl_sync(0xffffffffu, u, 31);
+    places += __shfl_sync(0xffffffffu, x, 31);
+  }
+  __syncwarp();
+  for (int b = lane; b < p.pool.batch; b += 32) {
+    const PrefixSeq s = p.plan.seqs[b];  // (this lane's own store)
+    if (s.group >= 0) p.plan.members[first_s[s.group] + s.rank] = b;
+  }
+  if (lane == 0) {
+    p.plan.head[0] = places;
+    p.plan.head[1] = max(kPrefixCost + 1, (places + p.grid - 1) / p.grid);
+  }
+}
+
+// ------------------------------------------------------------ shared pages
+
+template <int D> struct PrefixCfg {
+  static constexpr int kTile = 128 * D * 2;                     // bytes of 128 fp16 rows
+  static constexpr int kSlots = D == 128 ? 3 : 6;               // Key and Value tiles
+  static constexpr int kRecord = 20 * D * 4;                    // bytes of a page
+  static constexpr int kStages = D == 128 ? 3 : 6;              // pairs of pages as they are in the pool
+  static constexpr int kSmem = 2 * kTile + kSlots * kTile + kStages * 2 * kRecord + 1024;  // (aligned by hand)
+  static constexpr int kO = 256;                                // TMEM columns: scores of both tiles, then outputs
+};
+constexpr int kPrefixThreads = 512;
+constexpr int kUnpackWarp = 8, kProductWarp = 12, kCopyWarp = 13;
+constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
+
+struct PrefixShared {
+  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_ready[2], o_done[2];
+  int stop;
+  uint32_t tmem;
+};
+
+// Steps of one unit that this CTA has.
+struct Piece { int g, h, tile, first, n, unit; };
+// The pieces of a CTA's range, in order; every lane of a warp calls it.
+struct Walk {
+  const PrefixPlan& plan;
+  int kv_heads, groups, at, end, g0;
+  PrefixGroup group;
+  int g;
+  __device__ __forceinline__ Walk(const PrefixPlan& plan, int kv_heads, int groups) : plan(plan), kv_heads(kv_heads), groups(groups), g0(0), g(-1) {
+    const int per = plan.head[1];
+    at = blockIdx.x * per;
+    end = min(plan.head[0], at + per);
+    group = PrefixGroup{};
+  }
+  __device__ __forceinline__ bool next(Piece& piece) {
+    while (at < end) {
+      while (g < 0 || at >= group.places + group.tiles * kv_heads * (group.steps + kPrefixCost)) {  // (places end behind `at`)
+        const int x = g0 + (threadIdx.x & 31);
+        bool past = false;
+        if (x < groups) {
+          const PrefixGroup y = plan.groups[x];
+          past = at < y.places + y.tiles * kv_heads * (y.steps + kPrefixCost);
+        }
+        const uint32_t any = __ballot_sync(0xffffffffu, past);
+        if (any != 0) {
+          g = g0 + __ffs(any) - 1;
+          group = plan.groups[g];
+        } else {
+          g0 += 32;
+          if (g0 >= groups) return false;
+        }
+      }
+      const int span = group.steps + kPrefixCost, x = (at - group.places) / span, start = group.places + x * span + kPrefixCost;
+      const int first = max(at, start), stop = min(end, start + group.steps);
+      at = max(stop, min(end, start));
+      if (first >= stop) continue;
+      piece = Piece{g, x / group.tiles, x % group.tiles, first - start, stop - first, group.units + x};
+      return true;
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ uint32_t hfma2_rn(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// The eight codes of a word times s2 plus z2 as fp16 pairs: codes (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t s2, uint32_t z2) {
+  uint32_t c[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t x = w >> (8 * k);
+    const uint32_t even = (x & 0x000F000Fu) | 0x64006400u, odd = (x & 0x00F000F0u) | 0x64006400u;  // 1024 + code, 1024 + 16 code
+    c[2 * k] = hfma2_rn(even, 0x3C003C00u, 0xE400E400u);     // - 1024
+    c[2 * k + 1] = hfma2_rn(odd, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
+  }
+  return make_uint4(hfma2_rn(c[0], s2, z2), hfma2_rn(c[1], s2, z2), hfma2_rn(c[2], s2, z2), hfma2_rn(c[3], s2, z2));
+}
+// Non-zero in a sign's place where a scale is 2^11 at least, a minimum 2^15, or one is not finite.
+__device__ __forceinline__ uint32_t wide_bits(uint32_t sz) { return (sz & 0x7FFF7FFFu) + 0x08001800u; }
+
+template <int kN> __device__ __forceinline__ void words_of(const uint8_t* at, uint32_t (&w)[kN]) {
+  if constexpr (kN == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(at);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
+    w[0] = x.x; w[1] = x.y;
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __grid_constant__ PrefixParams p) {
+  using C = PrefixCfg<D>;
+  constexpr int kSlots = C::kSlots, kStages = C::kStages, kG = D / kInt4Group;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ PrefixShared sh;
+  const uint32_t pad = ((smem_u32(dynamic) + 1023u) & ~1023u) - smem_u32(dynamic);
+  uint8_t* queries = dynamic + pad;
+  uint8_t* ring = queries + 2 * C::kTile;
+  uint8_t* raw = ring + kSlots * C::kTile;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  if (warp == kProductWarp) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.kv_full[i], 4);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh.raw_full[i], 1);
+      mbar_init(&sh.raw_empty[i], 4);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh.q_ready[t], 4);
+      mbar_init(&sh.s_full[t], 1);
+      mbar_init(&sh.p_ready[t], 128);
+      mbar_init(&sh.o_done[t], 1);
+    }
+    sh.stop = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&sh.tmem), 0);
+  grid_dep_wait();
+
+  volatile int* stop = &sh.stop;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, stop); };
+  const int per_member = p.q_len * p.heads;
+
+  if (warp == kCopyWarp) {
+    // ---------------------------------------------------------------- copies of pages
+    Walk walk(p.plan, p.pool.kv_heads, p.groups);
+    Piece piece;
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && walk.next(piece)) {
+      const int pages = walk.group.pages, leader = p.plan.members[walk.group.members];
+      const int32_t* words = p.pool.words + piece.h * p.pool.head_stride;
+      int ids = 0;
+      for (int i = 0; i < piece.n; ++i, ++n) {
+        const int page = 2 * (piece.first + i), two = page + 1 < pages ? 2 : 1;
+        if ((i & 15) == 0) {  // the ids of 32 pages, one a lane
+          ids = page + lane < pages ? int4_page_id(p.pool, leader, page + lane) : 0;
+          if (ids < 0) {
+            p.plan.groups[piece.g].live = 0;  // its members look for themselves
+            ids = 0;
+          }
+        }
+        const int stage = n % kStages;
+        if (n >= kStages && !(ok = wait(&sh.raw_empty[stage], (n / kStages - 1) & 1))) break;
+        const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + 1);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&sh.raw_full[stage], two * C::kRecord);
+          bulk_g2s(raw + stage * 2 * C::kRecord, words + id0 * p.pool.page_stride, C::kRecord, &sh.raw_full[stage]);
+          if (two == 2) bulk_g2s(raw + (2 * stage + 1) * C::kRecord, words + id1 * p.pool.page_stride, C::kRecord, &sh.raw_full[stage]);
+        }
+        __syncwarp();
+      }
+    }
+    for (int i = 0; i < kStages; ++i) {  // no copy outlives the CTA
+      const uint32_t used = n / kStages + (static_cast<uint32_t>(i) < n % kStages ? 1 : 0);
+      if (used != 0) mbar_wait_bounded(&sh.raw_full[i], (used - 1) & 1, kTileWaitNs);
+    }
+  } else if (warp >= kUnpackWarp && warp < kUnpackWarp + 4) {
+    // ---------------------------------------------------------------- pages to fp16 tiles
+    Walk walk(p.plan, p.pool.kv_heads, p.groups);
+    Piece piece;
+    uint32_t n = 0;
+    bool ok = true;
+    const int w = warp - kUnpackWarp;
+    while (ok && walk.next(piece)) {
+      const int pages = walk.group.pages;
+      uint32_t wide = 0;
+      for (int i = 0; i < piece.n; ++i, ++n) {
+        const int stage = n % kStages, page = 2 * (piece.first + i);
+        if (!(ok = wait(&sh.raw_full[stage], (n / kStages) & 1))) break;
+#pragma unroll 1
+        for (int value = 0; value < 2; ++value) {
+          const uint32_t load = 2 * n + value, slot = load % kSlots;
+          if (load >= kSlots && !(ok = wait(&sh.kv_empty[slot], (load / kSlots - 1) & 1))) break;
+          uint8_t* tile = ring + slot * C::kTile;
+#pragma unroll
+          for (int part = 0; part < 4; ++part) {
+            // 16 words' rows at a time: warp w and part give 8 tokens of a page
+            const int block = part * 4 + w, half = block >> 3, b = block & 7;  // half: which page; b: its 8 tokens
+            const uint8_t* rec = raw + (2 * stage + half) * C::kRecord + value * 40 * D;
+            const bool there = page + half < pages;
+            if (value == 0) {
+              // Key: lane = (token, t), its kG words the groups' channels 8 t .. 8 t + 7.  Tokens x and
+              // x + 4 in a quarter of the warp store to different banks.
+              const int t = lane & 3, tok = 8 * b + ((lane >> 2) & 1) * 4 + (lane >> 3), row = half * 64 + tok;
+              uint32_t code[kG], sz[kG];
+              words_of<kG>(rec + (tok * (D / 8) + t * kG) * 4, code);
+              words_of<kG>(rec + 32 * D + tok * kG * 4, sz);
+#pragma unroll
+              for (int G = 0; G < kG; ++G) {
+                wide |= there ? wide_bits(sz[G]) : 0u;
+                const uint32_t s2 = __byte_perm(sz[G], 0, 0x1010), z2 = __byte_perm(sz[G], 0, 0x3232);
+                const uint4 x = there ? unpack_word(code[G], s2, z2) : make_uint4(0, 0, 0, 0);
+                const int chunk = 4 * (G & 1) + t;
+                *reinterpret_cast<uint4*>(tile + (G >> 1) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4)) = x;
+              }
+            } else {
+              // Value: lane = (t, g), its words [token 2 t + o][w]: channels 64 w + 32 u + 4 g + n.
+              const int g = lane & 7, t = lane >> 3;
+              uint32_t code[kG], sz[2][kG];
+              words_of<kG>(rec + (b * D + g * (D / 8) + t * kG) * 4, code);
+              words_of<kG>(rec + 32 * D + (8 * b + 2 * t) * kG * 4, sz[0]);
+              words_of<kG>(rec + 32 * D + (8 * b + 2 * t + 1) * kG * 4, sz[1]);
+#pragma unroll
+              for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int x = 0; x < kG / 2; ++x) {
+                  const uint32_t a = sz[o][2 * x], c = sz[o][2 * x + 1];
+                  wide |= there ? (wide_bits(a) | wide_bits(c)) : 0u;
+                  const uint32_t s2 = __byte_perm(a, c, 0x5410), z2 = __byte_perm(a, c, 0x7632);
+                  const int row = half * 64 + 8 * b + 2 * t + o;
+                  const uint4 y = there ? unpack_word(code[o * (kG / 2) + x], s2, z2) : make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(tile + x * kHalfBytes + row * 128 + ((g ^ (row & 7)) << 4)) = y;
+                }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.kv_full[slot]);
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.raw_empty[stage]);
+      }
+      if ((wide & 0x80008000u) != 0) p.plan.groups[piece.g].live = 0;
+    }
+  } else if (warp == kProductWarp) {
+    // ---------------------------------------------------------------- products
+    // As prompt attention's: scores of step s after the outputs of step s - 1, tile by tile.
+    Walk walk(p.plan, p.pool.kv_heads, p.groups);
+    Piece piece;
+    const uint32_t idesc_s = idesc_16(false, 128, 128, false, false), idesc_o = idesc_16(false, 128, D, true, false);
+    const uint32_t ring_a = smem_u32(ring), queries_a = smem_u32(queries);
+    uint32_t step = 0, made[2] = {0, 0}, asked[2] = {0, 0};
+    bool had[2] = {false, false}, fresh = false, ok = true;
+    auto output = [&](int t) -> bool {
+      if (!wait(&sh.p_ready[t], made[t] & 1)) return false;
+      ++made[t];
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t v = swizzled_desc(ring_a + (2 * step - 1) % kSlots * C::kTile);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || k > 0);
+        mma_commit(&sh.o_done[t]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto free_slot = [&](uint32_t load) {
+      if (elect_one()) mma_commit(&sh.kv_empty[load % kSlots]);
+      __syncwarp();
+    };
+    while (ok && walk.next(piece)) {
+      const int rows = walk.group.count * per_member - piece.tile * kPrefixRows;
+      const bool now[2] = {true, rows > 128};
+      for (int i = 0; i < piece.n; ++i) {
+        const uint32_t load = 2 * step;
+        if (!(ok = wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1))) break;
+        if (step > 0 && !(ok = wait(&sh.kv_full[(load - 1) % kSlots], ((load - 1) / kSlots) & 1))) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (had[t] && !(ok = output(t))) break;
+          if (!now[t]) continue;
+          if (i == 0 && !(ok = wait(&sh.q_ready[t], asked[t]++ & 1))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t a = swizzled_desc(queries_a + t * C::kTile), b = swizzled_desc(ring_a + load % kSlots * C::kTile);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+              mma_16_ss(tmem + 128 * t, a + off, b + off, idesc_s, k > 0);
+            }
+            mma_commit(&sh.s_full[t]);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (step > 0) free_slot(load - 1);
+        free_slot(load);
+        had[0] = now[0];
+        had[1] = now[1];
+        fresh = i == 0;
+        ++step;
+      }
+    }
+    if (ok && step > 0 && *stop == 0) {  // the last step's outputs
+      const uint32_t load = 2 * step - 1;
+      ok = wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1);
+      for (int t = 0; ok && t < 2; ++t) ok = !had[t] || output(t);
+      if (ok) free_slot(load);
+    }
+    // No product, and no arrival of one, outlives the CTA.
+    for (uint32_t i = 0; i < kSlots; ++i) {
+      const uint32_t used = 2 * step / kSlots + (i < 2 * step % kSlots ? 1 : 0);
+      if (used != 0) mbar_wait_bounded(&sh.kv_empty[i], (used - 1) & 1, kTileWaitNs);
+    }
+  } else if (warp < kUnpackWarp) {
+    // ---------------------------------------------------------------- softmax, one tile a warpgroup
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
+    Walk walk(p.plan, p.pool.kv_heads, p.groups);
+    Piece piece;
+    uint32_t count = 0;
+    bool ok = true;
+    while (ok && walk.next(piece)) {
+      const int row = piece.tile * kPrefixRows + t * 128 + r, rows = walk.group.count * per_member;
+      if (piece.tile * kPrefixRows + t * 128 >= rows) continue;
+      // ---- the row's query, as fp16 at a power of two
+      float c = 1e-36f;
+      int vis = walk.group.pages * kInt4Page;
+      {
+        uint4 x[D / 8];
+        float most = 0.0f;
+        if (row < rows) {
+          const int m = row / per_member, in = row - m * per_member, i = in / p.heads, b = p.plan.members[walk.group.members + m];
+          const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (piece.h * p.heads + in - i * p.heads) * p.q_head + i * p.q_tok;
+          vis = min(vis, int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i));
+#pragma unroll
+          for (int k = 0; k < D / 8; ++k) x[k] = *reinterpret_cast<const uint4*>(q + 8 * k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < D / 8; ++k) x[k] = make_uint4(0, 0, 0, 0);
+        }
+        auto number = [&](uint32_t v, bool high) {
+          if constexpr (std::is_same<T, __half>::value) return high ? half_hi(v) : half_lo(v);
+          return __uint_as_float(high ? v & 0xFFFF0000u : v << 16);
+        };
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) most = fmaxf(most, fmaxf(fabsf(number(v[y], false)), fabsf(number(v[y], true))));
+        }
+        // 2^kq brings the largest magnitude to [2^13, 2^14), or as near as 2^126 does
+        const int kq = most > 0.0f && most < INFINITY ? min(126, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127)) : 0;
+        const float up = p.scale_log2 < 0.0f ? -pow2(kq) : pow2(kq);
+        c = fmaxf(pow2(-kq) * fabsf(p.scale_log2), 1e-36f);  // positive, so that a masked score's -inf stays one
+        uint8_t* tile = queries + t * C::kTile + r * 128;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          float f[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) f[y] = number(v[y >> 1], y & 1) * up;
+          const uint4 w = make_uint4(pack_two<__half>(f[0], f[4]), pack_two<__half>(f[1], f[5]), pack_two<__half>(f[2], f[6]),
+                                     pack_two<__half>(f[3], f[7]));
+          *reinterpret_cast<uint4*>(tile + (k >> 3) * kHalfBytes + (((k & 7) ^ (r & 7)) << 4)) = w;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_ready[t]);
+      const int vis_min = __reduce_min_sync(0xffffffffu, vis);
+      // ---- its steps
+      RowState st = {-INFINITY, 0.0f};
+      for (int i = 0; i < piece.n; ++i, ++count) {
+        const int at = (piece.first + i) * 128;
+        if (!(ok = wait(&sh.s_full[t], count & 1))) break;
+        tc_fence_after();
+        const float fix = soften<__half>(tm_s, c, at + 128 > vis_min, vis - at, st);
+        if (i > 0 && __any_sync(0xffffffffu, fix != 1.0f)) {
+          if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+          tc_fence_after();
+          rescale<D>(tm_o, fix);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_ready[t]);
+      }
+      if (!ok || !(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+      tc_fence_after();
+      // ---- its record
+      float* rec = p.plan.records + (piece.unit + static_cast<int64_t>(blockIdx.x)) * prefix_record(D);
+      const int in = t * 128 + r;
+      float* acc = rec + 2 * kPrefixRows + static_cast<int64_t>(in) * D;
+      if (row < rows) {
+        rec[in] = st.top == -INFINITY ? kNoScore : fmaxf(st.top, kNoScore);
+        rec[kPrefixRows + in] = st.sum;
+      }
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        float o[32];
+        tmem_ld_x32(tm_o + 32 * x, o);
+        tmem_wait_ld();
+        tmem_settle(o);
+        if (row < rows) {
+          // column 64 w + 8 g + 2 n + u is channel 64 w + 32 u + 4 g + n
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              *reinterpret_cast<float4*>(acc + 64 * (x >> 1) + 32 * u + 4 * (4 * (x & 1) + g)) =
+                  make_float4(o[8 * g + u], o[8 * g + 2 + u], o[8 * g + 4 + u], o[8 * g + 6 + u]);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kProductWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && sh.stop != 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_DEVICE_TIMEOUT);
+}
+
+// ------------------------------------------------------------------- host
+
+// Bytes of the plan's lists, and records that there can be.
+static size_t plan_bytes(int batch, int groups) {
+  return (16 + static_cast<size_t>(groups) * sizeof(PrefixGroup) + static_cast<size_t>(batch) * (sizeof(PrefixSeq) + 4) + 255) / 256 * 256;
+}
+static int64_t most_records(int64_t batch, int64_t kv_heads, int64_t heads, int64_t q_len, int64_t groups, int64_t sms) {
+  return (batch * q_len * heads / kPrefixRows + (groups < batch ? groups : batch)) * kv_heads + sms;
+}
+
+template <typename T>
+static const void* prefix_kernel_of(int head_dim) {
+  return head_dim == 128 ? reinterpret_cast<const void*>(int4_prefix_kernel<T, 128>) : reinterpret_cast<const void*>(int4_prefix_kernel<T, 64>);
+}
+
+}  // namespace lf
+
+extern "C" size_t lf_int4_prefix_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim, int groups) {
+  if (batch <= 0 || kv_heads <= 0 || n_q < kv_heads || q_len <= 0 || head_dim <= 0 || groups < 0) return 0;
+  return lf::plan_bytes(batch, groups) + static_cast<size_t>(lf::most_records(batch, kv_heads, n_q / kv_heads, q_len, groups, lf::sm_count())) *
+                                             lf::prefix_record(head_dim) * 4;
+}
+
+extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream) {
+  using namespace lf;
+  LF_CHECK_ARG(a != nullptr, "lf_int4_attend_prefix: null arguments");
+  const lf_int4_query& q = a->query;
+  LF_CHECK_ARG(q.picked == nullptr, "lf_int4_attend_prefix: pages were picked");
+  const int bad = check_int4_attend(&q);
+  if (bad != LF_OK) return bad;
+  LF_CHECK_ARG(a->groups >= 0 && (a->groups == 0 || (a->group && a->shared)), "lf_int4_attend_prefix: null pointer");
+  LF_CHECK_SUPPORTED(a->groups <= kMaxGroups, "lf_int4_attend_prefix: %d groups (%d at most)", a->groups, kMaxGroups);
+  if (a->groups == 0) return lf_int4_attend(&q, stream);
+  PrefixParams p;
+  const int ok = check_int4_pool("lf_int4_attend_prefix", q.pool, q.head_dim, p.pool);
+  if (ok != LF_OK) return ok;
+  p.q = q.q;
+  p.q_seq = q.q_seq_stride;
+  p.q_head = q.q_head_stride;
+  p.q_tok = q.q_tok_stride;
+  p.q_len = q.q_len;
+  p.heads = q.n_q / p.pool.kv_heads;
+  p.lengths = q.lengths;
+  p.counts = q.counts;
+  p.group = a->group;
+  p.shared = a->shared;
+  p.groups = a->groups;
+  p.scale_log2 = q.scaling * 1.4426950408889634f;
+  p.status = q.status;
+  const int sms = sm_count();
+  const int64_t records = most_records(p.pool.batch, p.pool.kv_heads, p.heads, p.q_len, p.groups, sms);
+  const int64_t steps = (p.pool.table_width + 1) / 2 + kPrefixCost;
+  LF_CHECK_SUPPORTED(records <= (1 << 30) / steps && static_cast<int64_t>(p.pool.batch) * p.q_len * p.heads <= (1 << 30),
+                     "lf_int4_attend_prefix: %d sequences of %d pages are too many for one call", p.pool.batch, p.pool.table_width);
+  LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
+                   a->workspace_bytes >= lf_int4_prefix_workspace_bytes(p.pool.batch, p.pool.kv_heads, q.n_q, p.q_len, q.head_dim, p.groups),
+               "lf_int4_attend_prefix: workspace of %zu bytes is missing, misaligned or too small", a->workspace_bytes);
+  uint8_t* at = static_cast<uint8_t*>(a->workspace);
+  p.plan.head = reinterpret_cast<int*>(at);
+  p.plan.groups = reinterpret_cast<PrefixGroup*>(at + 16);
+  p.plan.seqs = reinterpret_cast<PrefixSeq*>(p.plan.groups + p.groups);
+  p.plan.members = reinterpret_cast<int*>(p.plan.seqs + p.pool.batch);
+  p.plan.records = reinterpret_cast<float*>(at + plan_bytes(p.pool.batch, p.groups));
+  const int64_t most_steps = (records - sms) * steps;
+  p.grid = static_cast<int>(most_steps < sms ? most_steps : sms);
+
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const void* kern = q.dtype == LF_F16 ? prefix_kernel_of<__half>(q.head_dim) : prefix_kernel_of<__nv_bfloat16>(q.head_dim);
+  const int smem = q.head_dim == 128 ? PrefixCfg<128>::kSmem : PrefixCfg<64>::kSmem;
+  cudaError_t err = raise_smem_limit(kern, smem, true);
+  void* args[] = {&p};
+  if (err == cudaSuccess)
+    err = launch_programmatic(reinterpret_cast<const void*>(int4_prefix_plan_kernel), dim3(1), dim3(32), 0, s, args);
+  if (err == cudaSuccess) err = launch_programmatic(kern, dim3(p.grid), dim3(kPrefixThreads), smem, s, args);
+  if (err != cudaSuccess) {
+    set_error("lf_int4_attend_prefix: %s", cudaGetErrorString(err));
+    return LF_ERR_LAUNCH;
+  }
+  return int4_attend_suffix(&q, p.plan, s);
+}

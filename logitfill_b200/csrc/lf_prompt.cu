@@ -88,7 +88,6 @@ template <int D> struct PromptCfg {
 };
 constexpr int kPromptThreads = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kScanWarp = 11;
-constexpr uint64_t kPromptWaitNs = 2000000000ull;
 
 // A piece of work: two query tiles of one KV head of one sequence.
 struct PromptItem {
@@ -156,19 +155,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   grid_dep_wait();
 
   volatile int* stop = &sh.stop;
-  // Whole-warp wait: false once a wait of this CTA has given up.
-  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-      const uint64_t t0 = globaltimer_ns();
-      for (uint32_t n = 1; !ok; ++n) {
-        ok = mbar_try_wait(bar, parity);
-        if (!ok && (n & 63u) == 0u && (*stop != 0 || globaltimer_ns() - t0 > kPromptWaitNs)) break;
-      }
-      if (!ok) *stop = 1;
-    }
-    return __all_sync(0xffffffffu, ok);
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, stop); };
   // The next item (number n of this CTA), copied from the plan's slot.
   auto take = [&](uint32_t n, PromptItem& it) -> bool {
     if (!wait(&sh.item_full[n & 1], (n >> 1) & 1)) return false;
@@ -280,13 +267,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (*stop == 0)
         wait(&sh.kv_empty[i], (done - 1) & 1);
       else
-        mbar_wait_bounded(&sh.kv_full[i], (done - 1) & 1, kPromptWaitNs);
+        mbar_wait_bounded(&sh.kv_full[i], (done - 1) & 1, kTileWaitNs);
     }
     if (n_q > 0) {
       if (*stop == 0)
         wait(&sh.q_empty, (n_q - 1) & 1);
       else
-        mbar_wait_bounded(&sh.q_full, (n_q - 1) & 1, kPromptWaitNs);
+        mbar_wait_bounded(&sh.q_full, (n_q - 1) & 1, kTileWaitNs);
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- products
@@ -390,7 +377,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (*stop != 0) {  // the products in flight, before their operands go
       if (elect_one()) mma_commit(&sh.last);
       __syncwarp();
-      mbar_wait_bounded(&sh.last, 0, kPromptWaitNs);
+      mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
     }
   } else if (warp == kScanWarp) {
     // ---------------------------------------------------------------- masked Value tiles

@@ -13,6 +13,8 @@ in 64-token pages that a page table orders into sequences.
 * :func:`int4_select` scores a sequence's pages by a bound on their attention
   scores and picks the best for each query token and KV head, and
   :func:`int4_sparse_attention` attends over the picked pages only;
+* :func:`int4_prefix_attention` reads the pages that sequences share once for
+  all of them;
 * :class:`Int4KVCache` keeps the pools, the page table and the lengths of a
   batch of sequences, for every layer of a model.
 
@@ -120,6 +122,24 @@ def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torc
     visible, every page is read and the result is the dense one."""
     return _lib.int4_binding().attend(query, pages, page_table, lengths, scaling, counts, out, status, bounds, top_pages,
                                       sink_pages, recent_pages)
+
+
+def int4_prefix_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                          scaling: float, prefix_group: torch.Tensor, prefix_pages: torch.Tensor,
+                          counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                          status: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`int4_attention` where sequences share their first pages (a system
+    prompt, a document that several ask about, or, for one sequence with many
+    query tokens, its own history): the shared pages are read and unpacked once
+    for all of a group's queries.
+
+    ``prefix_group`` (int32 ``[batch]``) names each sequence's group (outside ``0 ..
+    groups - 1``: none), ``prefix_pages`` (int32 ``[groups]``) how many of their
+    first page table entries a group's sequences have in common; the entries of
+    its lowest sequence are read.  Both are read on the GPU.  The result is
+    :func:`int4_attention`'s up to the order of sums, for any lengths."""
+    return _lib.int4_binding().attend_prefix(query, pages, page_table, lengths, scaling, prefix_group, prefix_pages, counts, out,
+                                             status)
 
 
 class Int4KVCache:
@@ -301,4 +321,4 @@ class Int4KVCache:
 
 
 __all__ = ["PAGE_TOKENS", "GROUP", "record_words", "bounds_bytes", "alloc_pages", "alloc_bounds", "int4_write",
-           "int4_read", "int4_read_bounds", "int4_attention", "int4_select", "int4_sparse_attention", "Int4KVCache"]
+           "int4_read", "int4_read_bounds", "int4_attention", "int4_select", "int4_sparse_attention", "int4_prefix_attention", "Int4KVCache"]
