@@ -21,6 +21,10 @@ int sm_count();
 // kernel, and lowering it for a small layout would fail a larger one later.
 cudaError_t raise_smem_limit(const void* kern, int bytes, bool max_carveout);
 
+// Whether kern has `regs` registers a thread, which its own split of them counts on
+// (asked once per kernel and device).
+bool launched_with(const void* kern, int regs);
+
 template <typename T> struct Scalar;
 template <> struct Scalar<float> {
   static __device__ __forceinline__ float load(const float* p) { return *p; }

@@ -5,6 +5,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "lf_common.cuh"
 #include "lf_tcgen05.cuh"
 
@@ -69,16 +71,29 @@ __device__ __forceinline__ void tmem_settle(float* r) {
     "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]),
     "+f"(r[31]));
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+// 16 columns, waited for.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
+        "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+// A warpgroup's registers per thread from here on; the sum over the block may not pass what
+// it was launched with, or the raise would wait
+// for good (launched_with).
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Two numbers rounded to T, the first in the low half.
 template <typename T> __device__ __forceinline__ uint32_t pack_two(float lo, float hi);
@@ -124,6 +139,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // row).  Weights stand at 2^kLift for the running maximum.  It is moved only where a
 // score passes it by 2^kSlack, so most tiles skip the rescaling of the output.
 constexpr float kSlack = 8.0f;
+#ifndef LF_POLY
+#define LF_POLY 3
+#endif
+constexpr int kPolyPairs = LF_POLY;
 template <typename T> constexpr float kLift = 0.0f;
 // fp16 ends at steps of 2^-24: with the largest weight at 2^7, what is lost of a small
 // weight is 2^-32 of it at most (and 2^(7 + 8) still fits).
@@ -131,15 +150,25 @@ template <> constexpr float kLift<__half> = 7.0f;
 
 struct RowState {
   float top;  // running maximum times c, -inf before any score
-  float sum;  // of the weights
+  float sum;  // of the weights; NaN once a score was NaN or +inf
+  __device__ __forceinline__ bool empty() const { return top == -INFINITY && sum == sum; }  // nothing above -inf was seen
 };
 
-// Scores of the row's 128 columns, of which the first `seen` are visible (masked: whether
-// that is to be looked at), from s to weights in T at the same TMEM columns.  c > 0.
-// Returns the factor that the output so far has to be multiplied by (1 mostly).
-template <typename T>
-__device__ __forceinline__ float soften(uint32_t tmem_s, float c, bool masked, int seen, RowState& st) {
-  float s[128];
+__device__ __forceinline__ float max_nan2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The row's 128 scores, of which the first `seen` are visible (masked: whether that is to
+// be looked at), and the row's maximum with them.  c > 0.  Returns the factor that the
+// output so far has to be multiplied by (1 mostly).
+__device__ __forceinline__ float row_scores(uint32_t tmem_s, float (&s)[128], float c, bool masked, int seen, RowState& st) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) tmem_ld_x32(tmem_s + 32 * i, s + 32 * i);
   tmem_wait_ld();
@@ -151,52 +180,112 @@ __device__ __forceinline__ float soften(uint32_t tmem_s, float c, bool masked, i
   }
   float most[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) most[k] = fmaxf(s[k], s[k + 4]);
+  for (int k = 0; k < 4; ++k) most[k] = s[k];
 #pragma unroll
-  for (int i = 8; i < 128; i += 8)
+  for (int i = 4; i < 124; i += 8)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) most[k] = fmaxf(fmaxf(most[k], s[i + k]), s[i + k + 4]);
-  const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * c;
+    for (int k = 0; k < 4; ++k) most[k] = max3_nan(most[k], s[i + k], s[i + k + 4]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) most[k] = max_nan2(most[k], s[124 + k]);
+  const float now = max3_nan(max_nan2(most[0], most[1]), most[2], most[3]) * c;
   float fix = 1.0f;
   if (now > st.top + kSlack) {  // (the first score of a row always: top is -inf)
     fix = ex2(st.top - now);
     st.top = now;
     st.sum *= fix;
   }
+  if (!(now < INFINITY)) st.sum = NAN;  // a score that is NaN or +inf makes the row's result NaN
+  return fix;
+}
+
+// 2^x for x >= -126 without the special function unit: x = n + r with |r| <= 1/2 (the
+// nearest whole number by adding 1.5 * 2^23), 2^r by its minimax polynomial (relative
+// error; found with Remez' algorithm), n added to the exponent.  Within 7.5e-5 (degree 3)
+// and 2.7e-6 (degree 4): below a weight's own rounding to bf16 (2^-9) and fp16 (2^-12).
+template <int kDegree>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 n = __fadd2_rn(x, magic);
+  const float2 whole = __fadd2_rn(n, make_float2(-12582912.0f, -12582912.0f));
+  const float2 r = __ffma2_rn(whole, make_float2(-1.0f, -1.0f), x);
+  auto step = [&](float2 y, float k) { return __ffma2_rn(y, r, make_float2(k, k)); };
+  float2 y;
+  if constexpr (kDegree == 3) {
+    y = step(make_float2(0.05517166906f, 0.05517166906f), 0.2426111222f);
+    y = step(step(y, 0.6932609855f), 0.9999280735f);
+  } else {
+    static_assert(kDegree == 4, "polynomials of degree 3 and 4");
+    y = step(make_float2(0.009570101912f, 0.009570101912f), 0.05591786032f);
+    y = step(step(step(y, 0.2402474483f), 0.6931218147f), 0.9999992614f);
+  }
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// Weights of the scores' quarter `part` (32 columns), stored in T at the row's columns 16 part
+// of tmem_s.  kPoly of every 8 pairs go by the polynomial: the special function unit gives 16
+// results a cycle, as long as the tensor core takes for both products of them.
+template <typename T, int kPoly>
+__device__ __forceinline__ void row_weights(uint32_t tmem_s, const float (&s)[128], int part, float c, RowState& st) {
   // The product of maximum and c is rounded once, and taken as it is everywhere: it
   // cancels in the quotient of output and sum.
   const float base = kLift<T> - (st.top == -INFINITY ? 0.0f : st.top);
   float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+  uint32_t w[16];
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    uint32_t w[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float2 x = __ffma2_rn(make_float2(s[64 * part + 2 * i], s[64 * part + 2 * i + 1]), make_float2(c, c), make_float2(base, base));
-      const float2 e = make_float2(ex2(x.x), ex2(x.y));
-      sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-      w[i] = pack_two<T>(e.x, e.y);
-    }
-    tmem_st_x32(tmem_s + 32 * part, w);
+  for (int i = 0; i < 16; ++i) {
+    const float2 x = __ffma2_rn(make_float2(s[32 * part + 2 * i], s[32 * part + 2 * i + 1]), make_float2(c, c), make_float2(base, base));
+    const float2 e = i % 8 < kPoly ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(x) : make_float2(ex2(x.x), ex2(x.y));
+    sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+    w[i] = pack_two<T>(e.x, e.y);
   }
+  tmem_st_x16(tmem_s + 16 * part, w);
   st.sum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-  return fix;
 }
 
 // The output rows so far times their factors.
 template <int D>
 __device__ __forceinline__ void rescale(uint32_t tmem_o, float fix) {
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    float o[32];
-    tmem_ld_x32(tmem_o + 32 * i, o);
-    tmem_wait_ld();
-    tmem_settle(o);
-    uint32_t w[32];
+  for (int i = 0; i < D / 16; ++i) {
+    float o[16];
+    tmem_ld_x16(tmem_o + 16 * i, o);
+    uint32_t w[16];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * fix);
-    tmem_st_x32(tmem_o + 32 * i, w);
+    for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * fix);
+    tmem_st_x16(tmem_o + 16 * i, w);
   }
+}
+
+// A thread's part of a warpgroup's row tile: scores to weights, in two halves (the product
+// with Value begins when the first is there).  wait(): the output product before is done
+// (asked for where the output has to be rescaled, not for a fresh one); false on a limit.
+template <typename T, int D, typename Wait>
+__device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, float c, bool masked, int seen, bool fresh, RowState& st,
+                                            uint64_t* half, uint64_t* ready, Wait&& wait) {
+  float s[128];
+  const float fix = row_scores(tmem_s, s, c, masked, seen, st);
+  if (!fresh && __any_sync(0xffffffffu, fix != 1.0f)) {
+    if (!wait()) return false;
+    tc_fence_after();
+    rescale<D>(tmem_o, fix);
+  }
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+    if (masked)  // a masked score's weight is 0, not 2^-126
+      row_weights<T, 0>(tmem_s, s, part, c, st);
+    else
+      row_weights<T, kPolyPairs>(tmem_s, s, part, c, st);
+    if (part & 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(part == 1 ? half : ready);
+    }
+  }
+  return true;
 }
 
 }  // namespace sm100

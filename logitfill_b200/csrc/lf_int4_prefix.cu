@@ -125,11 +125,15 @@ template <int D> struct PrefixCfg {
   static constexpr int kO = 256;                                // TMEM columns: scores of both tiles, then outputs
 };
 constexpr int kPrefixThreads = 512;
+// Registers a thread: 128 at launch (all that 512 threads can have), then split by what the
+// warpgroups hold: a row of 128 scores, four words and their parameters, counters.
+constexpr int kPrefixLaunchRegs = 128, kRowRegs = 192, kUnpackRegs = 80, kOtherRegs = 48;
+static_assert(256 * kRowRegs + 128 * (kUnpackRegs + kOtherRegs) <= kPrefixThreads * kPrefixLaunchRegs, "more registers than the block has");
 constexpr int kUnpackWarp = 8, kProductWarp = 12, kCopyWarp = 13;
 constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
 
 struct PrefixShared {
-  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_ready[2], o_done[2];
+  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_half[2], p_ready[2], o_done[2];
   int stop;
   uint32_t tmem;
 };
@@ -235,7 +239,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_ready[t], 4);
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_ready[t], 128);
+      mbar_init(&sh.p_half[t], 4);
+      mbar_init(&sh.p_ready[t], 4);
       mbar_init(&sh.o_done[t], 1);
     }
     sh.stop = 0;
@@ -253,6 +258,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
 
   if (warp == kCopyWarp) {
     // ---------------------------------------------------------------- copies of pages
+    fewer_registers<kOtherRegs>();
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
     uint32_t n = 0;
@@ -287,6 +293,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     }
   } else if (warp >= kUnpackWarp && warp < kUnpackWarp + 4) {
     // ---------------------------------------------------------------- pages to fp16 tiles
+    fewer_registers<kUnpackRegs>();
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
     uint32_t n = 0;
@@ -356,6 +363,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     }
   } else if (warp == kProductWarp) {
     // ---------------------------------------------------------------- products
+    fewer_registers<kOtherRegs>();
     // As prompt attention's: scores of step s after the outputs of step s - 1, tile by tile.
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
@@ -364,17 +372,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     uint32_t step = 0, made[2] = {0, 0}, asked[2] = {0, 0};
     bool had[2] = {false, false}, fresh = false, ok = true;
     auto output = [&](int t) -> bool {
-      if (!wait(&sh.p_ready[t], made[t] & 1)) return false;
-      ++made[t];
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t v = swizzled_desc(ring_a + (2 * step - 1) % kSlots * C::kTile);
+      for (int part = 0; part < 2; ++part) {
+        if (!wait(part == 0 ? &sh.p_half[t] : &sh.p_ready[t], made[t] & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v = swizzled_desc(ring_a + (2 * step - 1) % kSlots * C::kTile);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || k > 0);
-        mma_commit(&sh.o_done[t]);
+          for (int k = 4 * part; k < 4 * part + 4; ++k)
+            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || k > 0);
+          if (part == 1) mma_commit(&sh.o_done[t]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ++made[t];
       return true;
     };
     auto free_slot = [&](uint32_t load) {
@@ -427,6 +437,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     }
   } else if (warp < kUnpackWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
+    more_registers<kRowRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
@@ -488,15 +499,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         const int at = (piece.first + i) * 128;
         if (!(ok = wait(&sh.s_full[t], count & 1))) break;
         tc_fence_after();
-        const float fix = soften<__half>(tm_s, c, at + 128 > vis_min, vis - at, st);
-        if (i > 0 && __any_sync(0xffffffffu, fix != 1.0f)) {
-          if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
-          tc_fence_after();
-          rescale<D>(tm_o, fix);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sh.p_ready[t]);
+        if (!(ok = soften_tile<__half, D>(tm_s, tm_o, c, at + 128 > vis_min, vis - at, i == 0, st, &sh.p_half[t], &sh.p_ready[t],
+                                          [&] { return wait(&sh.o_done[t], (count - 1) & 1); })))
+          break;
       }
       if (!ok || !(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
       tc_fence_after();
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       float* acc = rec + 2 * kPrefixRows + static_cast<int64_t>(in) * D;
       if (row < rows) {
         rec[in] = st.top == -INFINITY ? kNoScore : fmaxf(st.top, kNoScore);
-        rec[kPrefixRows + in] = st.sum;
+        rec[kPrefixRows + in] = st.empty() ? 0.0f : st.sum;
       }
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
@@ -526,6 +531,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       }
       tc_fence_before();
     }
+  } else {
+    fewer_registers<kOtherRegs>();  // (of a warpgroup, all warps at once)
   }
   tc_fence_before();
   __syncthreads();
@@ -606,6 +613,10 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   const void* kern = q.dtype == LF_F16 ? prefix_kernel_of<__half>(q.head_dim) : prefix_kernel_of<__nv_bfloat16>(q.head_dim);
   const int smem = q.head_dim == 128 ? PrefixCfg<128>::kSmem : PrefixCfg<64>::kSmem;
   cudaError_t err = raise_smem_limit(kern, smem, true);
+  if (!launched_with(kern, kPrefixLaunchRegs)) {
+    set_error("lf_int4_attend_prefix: the kernel was not built for %d registers a thread", kPrefixLaunchRegs);
+    return LF_ERR_LAUNCH;
+  }
   void* args[] = {&p};
   if (err == cudaSuccess)
     err = launch_programmatic(reinterpret_cast<const void*>(int4_prefix_plan_kernel), dim3(1), dim3(32), 0, s, args);

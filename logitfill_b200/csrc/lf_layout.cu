@@ -36,6 +36,21 @@ cudaError_t raise_smem_limit(const void* kern, int bytes, bool max_carveout) {
   return e;
 }
 
+bool launched_with(const void* kern, int regs) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, int> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[std::make_pair(kern, dev)];
+  if (n == 0) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return false;
+    n = a.numRegs;
+  }
+  return n == regs;
+}
+
 cudaError_t launch_programmatic(const void* kern, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                 void** args) {
   cudaLaunchAttribute attr[1];

@@ -87,6 +87,10 @@ template <int D> struct PromptCfg {
   static constexpr int kO = 256;                                 // TMEM columns: scores of both tiles, then outputs
 };
 constexpr int kPromptThreads = 384;
+// Registers a thread: 168 at launch (all that 384 threads can have), then moved to the
+// softmax, whose row of 128 scores stays in registers.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kPromptThreads * kLaunchRegs, "more registers than the block has");
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kScanWarp = 11;
 
 // A piece of work: two query tiles of one KV head of one sequence.
@@ -99,7 +103,7 @@ struct PromptItem {
 };
 
 struct PromptShared {
-  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_ready[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
+  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
   PromptItem item[2];
   int bad[2];      // a Value that not all rows of a masked tile see is not finite
   int scan_slot, scan_live, scan_item;  // for the scan: the Value tile, its rows of the sequence, the item's slot
@@ -137,7 +141,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     mbar_init(&sh.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_ready[t], 128);
+      mbar_init(&sh.p_half[t], 4);
+      mbar_init(&sh.p_ready[t], 4);
       mbar_init(&sh.o_done[t], 1);
       mbar_init(&sh.item_full[t], 1);
       mbar_init(&sh.item_empty[t], 10);
@@ -169,6 +174,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp == kPlanWarp) {
     // ---------------------------------------------------------------- plan
+    fewer_registers<kOtherRegs>();
     // Items in the order of falling cost: by their number of tokens before, over all
     // sequences; a CTA takes them from alternating ends of rounds as wide as the grid.
     const int span = 2 * per_tile;
@@ -229,6 +235,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else if (warp == kLoadWarp) {
     // ---------------------------------------------------------------- copies
+    fewer_registers<kOtherRegs>();
     uint32_t load = 0, n_q = 0;  // tiles and query pairs copied so far
     if (lane < 3) prefetch_map(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map);
     PromptItem it;
@@ -277,6 +284,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- products
+    fewer_registers<kOtherRegs>();
     // Step s of the CTA: scores of Key tile (load 2 s) for both query tiles, after the
     // output product of step s - 1 (Value tile, load 2 s - 1), tile by tile: while the
     // softmax of one tile runs, the tensor core works for the other.
@@ -286,17 +294,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     uint32_t number = 0;  // and its item
     bool had[2] = {false, false}, fresh[2] = {false, false};
     auto output = [&](int t) -> bool {  // += weights of tile t times the Value tile of the step before
-      if (!wait(&sh.p_ready[t], made[t] & 1)) return false;
-      ++made[t];
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t v = swizzled_desc(ring + (2 * step - 1) % kSlots * C::kTile);
+      for (int part = 0; part < 2; ++part) {
+        if (!wait(part == 0 ? &sh.p_half[t] : &sh.p_ready[t], made[t] & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v = swizzled_desc(ring + (2 * step - 1) % kSlots * C::kTile);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || k > 0);
-        mma_commit(&sh.o_done[t]);
+          for (int k = 4 * part; k < 4 * part + 4; ++k)
+            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || k > 0);
+          if (part == 1) mma_commit(&sh.o_done[t]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ++made[t];
       return true;
     };
     auto value_there = [&]() -> bool {
@@ -381,6 +391,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else if (warp == kScanWarp) {
     // ---------------------------------------------------------------- masked Value tiles
+    fewer_registers<kOtherRegs>();
     // A weight of 0 does not keep a NaN or an infinity out of a product.  Of the Value
     // tiles that some row sees in part, rows behind the sequence are zeroed here, and a
     // number that is not finite sends the item to prompt_row.
@@ -409,6 +420,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
+    more_registers<kSoftmaxRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
     const int in_tile = r / p.group, head = r - in_tile * p.group;
@@ -423,15 +435,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int j = it.n[t] - 1; j >= 0; --j, ++count) {
         if (!(ok = wait(&sh.s_full[t], count & 1))) break;
         tc_fence_after();
-        const float fix = soften<T>(tm_s, c, tile_masked(t0, j), min(token + 1, it.tokens) - 128 * j, st);
-        if (j < it.n[t] - 1 && __any_sync(0xffffffffu, fix != 1.0f)) {
-          if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
-          tc_fence_after();
-          rescale<D>(tm_o, fix);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sh.p_ready[t]);
+        if (!(ok = soften_tile<T, D>(tm_s, tm_o, c, tile_masked(t0, j), min(token + 1, it.tokens) - 128 * j, j == it.n[t] - 1, st,
+                                     &sh.p_half[t], &sh.p_ready[t], [&] { return wait(&sh.o_done[t], (count - 1) & 1); })))
+          break;
       }
       if (!ok) break;
       const bool stored = in_tile < per_tile && token < it.rows;
@@ -452,7 +458,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                            tok < it.tokens ? tok + 1 : 0, p.scale_log2, static_cast<T*>(p.out) + it.b * p.o_seq + row * p.o_tok + hd * p.o_head);
         }
       } else {
-        const bool live = it.n[t] > 0 && token < it.tokens && st.sum != 0.0f;  // else 0: a row behind the sequence
+        // else 0: a row behind the sequence, or one of no score above -inf
+        const bool live = it.n[t] > 0 && token < it.tokens && !st.empty();
         const float inv = 1.0f / st.sum;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -600,6 +607,10 @@ extern "C" int lf_prompt_attend(const lf_prompt* a, lf_stream_t stream) {
   if (err != cudaSuccess) {
     set_error("lf_prompt_attend: %s", cudaGetErrorString(err));
     return LF_ERR_CUDA;
+  }
+  if (!launched_with(kern, kLaunchRegs)) {
+    set_error("lf_prompt_attend: the kernel was not built for %d registers a thread", kLaunchRegs);
+    return LF_ERR_LAUNCH;
   }
   void* args[] = {&p, &q_map, &k_map, &v_map};
   err = launch_programmatic(kern, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kPromptThreads), smem,
