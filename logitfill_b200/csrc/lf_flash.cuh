@@ -135,9 +135,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
-// The softmax of one 128 x 128 tile of scores, row by row (a thread to a row, TMEM lane =
-// row).  Weights stand at 2^kLift for the running maximum.  It is moved only where a
-// score passes it by 2^kSlack, so most tiles skip the rescaling of the output.
+// The softmax of one 128 x 128 tile of scores by 8 warps: two threads to a row (TMEM lane =
+// row), 64 columns each.  One thread to a row has its 128 exponentials in a chain that
+// the tensor core waits for: 3500 cycles a step of two tiles, against 2048 of its own;
+// four warps to a scheduler also cover one another's latencies.  Weights stand at
+// 2^kLift for the running maximum.  It is moved only where a score passes it by 2^kSlack,
+// so most tiles skip the rescaling of the output.
 constexpr float kSlack = 8.0f;
 #ifndef LF_POLY
 #define LF_POLY 3
@@ -165,29 +168,58 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// The row's 128 scores, of which the first `seen` are visible (masked: whether that is to
-// be looked at), and the row's maximum with them.  c > 0.  Returns the factor that the
-// output so far has to be multiplied by (1 mostly).
-__device__ __forceinline__ float row_scores(uint32_t tmem_s, float (&s)[128], float c, bool masked, int seen, RowState& st) {
+// What the two threads of a row tell one another: a number each, by way of shared memory
+// and a barrier that all 8 warps of the tile arrive at.
+struct Pair {
+  float* mine;
+  const float* other;
+  uint64_t* met;
+  uint32_t phase;
+  template <typename Wait>
+  __device__ __forceinline__ bool meet(Wait&& wait) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(met);
+    return wait(met, phase++ & 1);
+  }
+  // The next exchange may begin once the other thread has read this one's number: after
+  // another meeting, or a barrier that it arrives at later.
+  template <typename Wait>
+  __device__ __forceinline__ bool exchange(float x, float& y, Wait&& wait) {
+    *const_cast<volatile float*>(mine) = x;
+    if (!meet(wait)) return false;
+    y = *const_cast<const volatile float*>(other);
+    return true;
+  }
+};
+
+// This thread's 64 scores, of which the first `seen` are visible (masked: whether that is to
+// be looked at).  Returns their largest (NaN where one is).
+__device__ __forceinline__ float row_scores(uint32_t tmem_s, float (&s)[64], bool masked, int seen) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_ld_x32(tmem_s + 32 * i, s + 32 * i);
+  for (int i = 0; i < 2; ++i) tmem_ld_x32(tmem_s + 32 * i, s + 32 * i);
   tmem_wait_ld();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_settle(s + 32 * i);
+  for (int i = 0; i < 2; ++i) tmem_settle(s + 32 * i);
   if (masked) {
 #pragma unroll
-    for (int i = 0; i < 128; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+    for (int i = 0; i < 64; ++i) s[i] = i < seen ? s[i] : -INFINITY;
   }
   float most[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) most[k] = s[k];
 #pragma unroll
-  for (int i = 4; i < 124; i += 8)
+  for (int i = 4; i < 60; i += 8)
 #pragma unroll
     for (int k = 0; k < 4; ++k) most[k] = max3_nan(most[k], s[i + k], s[i + k + 4]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) most[k] = max_nan2(most[k], s[124 + k]);
-  const float now = max3_nan(max_nan2(most[0], most[1]), most[2], most[3]) * c;
+  for (int k = 0; k < 4; ++k) most[k] = max_nan2(most[k], s[60 + k]);
+  return max3_nan(max_nan2(most[0], most[1]), most[2], most[3]);
+}
+
+// The row's maximum moved by its tile's largest score (c > 0).  Returns the factor that
+// the output so far has to be multiplied by (1 mostly).
+__device__ __forceinline__ float move_top(float most, float c, RowState& st) {
+  const float now = most * c;
   float fix = 1.0f;
   if (now > st.top + kSlack) {  // (the first score of a row always: top is -inf)
     fix = ex2(st.top - now);
@@ -224,11 +256,11 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
 }
 
-// Weights of the scores' quarter `part` (32 columns), stored in T at the row's columns 16 part
-// of tmem_s.  kPoly of every 8 pairs go by the polynomial: the special function unit gives 16
-// results a cycle, as long as the tensor core takes for both products of them.
+// Weights of 32 scores, stored in T at 16 columns.  kPoly of every 8 pairs go by the
+// polynomial: the special function unit gives 16 results a cycle, as long as the tensor
+// core takes for both products of them.
 template <typename T, int kPoly>
-__device__ __forceinline__ void row_weights(uint32_t tmem_s, const float (&s)[128], int part, float c, RowState& st) {
+__device__ __forceinline__ void row_weights(uint32_t tmem_p, const float* s, float c, RowState& st) {
   // The product of maximum and c is rounded once, and taken as it is everywhere: it
   // cancels in the quotient of output and sum.
   const float base = kLift<T> - (st.top == -INFINITY ? 0.0f : st.top);
@@ -236,20 +268,20 @@ __device__ __forceinline__ void row_weights(uint32_t tmem_s, const float (&s)[12
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float2 x = __ffma2_rn(make_float2(s[32 * part + 2 * i], s[32 * part + 2 * i + 1]), make_float2(c, c), make_float2(base, base));
+    const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(base, base));
     const float2 e = i % 8 < kPoly ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(x) : make_float2(ex2(x.x), ex2(x.y));
     sum[i & 1] = __fadd2_rn(sum[i & 1], e);
     w[i] = pack_two<T>(e.x, e.y);
   }
-  tmem_st_x16(tmem_s + 16 * part, w);
+  tmem_st_x16(tmem_p, w);
   st.sum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
-// The output rows so far times their factors.
-template <int D>
+// kN columns of the output rows so far times their factors.
+template <int kN>
 __device__ __forceinline__ void rescale(uint32_t tmem_o, float fix) {
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
+  for (int i = 0; i < kN / 16; ++i) {
     float o[16];
     tmem_ld_x16(tmem_o + 16 * i, o);
     uint32_t w[16];
@@ -259,33 +291,45 @@ __device__ __forceinline__ void rescale(uint32_t tmem_o, float fix) {
   }
 }
 
-// A thread's part of a warpgroup's row tile: scores to weights, in two halves (the product
-// with Value begins when the first is there).  wait(): the output product before is done
-// (asked for where the output has to be rescaled, not for a fresh one); false on a limit.
+// A thread's part of a tile: columns 64 half .. of its row's scores to weights (which take
+// the first 64 columns' place, two to a column), first 32 columns, then 32: the output
+// product over these may begin when `early`, then `ready` is complete (8 warps each).
+// fresh: the row's first tile; done: the barrier of the output product before, at parity.
+// wait(barrier, parity) is false once a limit ran out, and so is the result then.
 template <typename T, int D, typename Wait>
-__device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, float c, bool masked, int seen, bool fresh, RowState& st,
-                                            uint64_t* half, uint64_t* ready, Wait&& wait) {
-  float s[128];
-  const float fix = row_scores(tmem_s, s, c, masked, seen, st);
+__device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, int half, float c, bool masked, int seen, bool fresh,
+                                            RowState& st, Pair& pair, uint64_t* early, uint64_t* ready, uint64_t* done, uint32_t parity,
+                                            Wait&& wait) {
+  float s[64], other;
+  const float most = row_scores(tmem_s + 64 * half, s, masked, seen - 64 * half);
+  if (!pair.exchange(most, other, wait)) return false;
+  const float fix = move_top(max_nan2(most, other), c, st);
   if (!fresh && __any_sync(0xffffffffu, fix != 1.0f)) {
-    if (!wait()) return false;
+    if (!wait(done, parity)) return false;
     tc_fence_after();
-    rescale<D>(tmem_o, fix);
+    rescale<D / 2>(tmem_o + D / 2 * half, fix);
   }
 #pragma unroll
-  for (int part = 0; part < 4; ++part) {
+  for (int part = 0; part < 2; ++part) {
     if (masked)  // a masked score's weight is 0, not 2^-126
-      row_weights<T, 0>(tmem_s, s, part, c, st);
+      row_weights<T, 0>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
     else
-      row_weights<T, kPolyPairs>(tmem_s, s, part, c, st);
-    if (part & 1) {
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(part == 1 ? half : ready);
-    }
+      row_weights<T, kPolyPairs>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(part == 0 ? early : ready);
   }
   return true;
+}
+
+// The row's sum, of both its threads' (the next exchange may follow at once).
+template <typename Wait>
+__device__ __forceinline__ bool join_sums(RowState& st, Pair& pair, Wait&& wait) {
+  float other;
+  if (!pair.exchange(st.sum, other, wait)) return false;
+  st.sum += other;
+  return pair.meet(wait);
 }
 
 }  // namespace sm100

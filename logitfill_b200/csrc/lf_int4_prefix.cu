@@ -124,18 +124,19 @@ template <int D> struct PrefixCfg {
   static constexpr int kSmem = 2 * kTile + kSlots * kTile + kStages * 2 * kRecord + 1024;  // (aligned by hand)
   static constexpr int kO = 256;                                // TMEM columns: scores of both tiles, then outputs
 };
-constexpr int kPrefixThreads = 512;
-// Registers a thread: 128 at launch (all that 512 threads can have), then split by what the
-// warpgroups hold: a row of 128 scores, four words and their parameters, counters.
-constexpr int kPrefixLaunchRegs = 128, kRowRegs = 192, kUnpackRegs = 80, kOtherRegs = 48;
-static_assert(256 * kRowRegs + 128 * (kUnpackRegs + kOtherRegs) <= kPrefixThreads * kPrefixLaunchRegs, "more registers than the block has");
-constexpr int kUnpackWarp = 8, kProductWarp = 12, kCopyWarp = 13;
+constexpr int kPrefixThreads = 768;
+// Registers a thread: 80 at launch, then split by what the warpgroups hold: 64 scores of a
+// row, four words and their parameters, counters.
+constexpr int kPrefixLaunchRegs = 80, kRowRegs = 96, kUnpackRegs = 64, kOtherRegs = 32;
+static_assert(512 * kRowRegs + 128 * (kUnpackRegs + kOtherRegs) <= kPrefixThreads * kPrefixLaunchRegs, "more registers than the block has");
+constexpr int kUnpackWarp = 16, kProductWarp = 20, kCopyWarp = 21;
 constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
 
 struct PrefixShared {
-  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_half[2], p_ready[2], o_done[2];
+  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2];
   int stop;
   uint32_t tmem;
+  float told[2][2][128];  // between the two threads of a row
 };
 
 // Steps of one unit that this CTA has.
@@ -237,10 +238,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       mbar_init(&sh.raw_empty[i], 4);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&sh.q_ready[t], 4);
+      mbar_init(&sh.q_ready[t], 8);
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_half[t], 4);
-      mbar_init(&sh.p_ready[t], 4);
+      mbar_init(&sh.p_early[t], 8);
+      mbar_init(&sh.p_ready[t], 8);
+      mbar_init(&sh.met[t], 8);
       mbar_init(&sh.o_done[t], 1);
     }
     sh.stop = 0;
@@ -373,13 +375,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     bool had[2] = {false, false}, fresh = false, ok = true;
     auto output = [&](int t) -> bool {
       for (int part = 0; part < 2; ++part) {
-        if (!wait(part == 0 ? &sh.p_half[t] : &sh.p_ready[t], made[t] & 1)) return false;
+        if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t v = swizzled_desc(ring_a + (2 * step - 1) % kSlots * C::kTile);
 #pragma unroll
-          for (int k = 4 * part; k < 4 * part + 4; ++k)
-            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || k > 0);
+          for (int i = 0; i < 4; ++i) {  // keys 64 half + 32 part ..
+            const int k = 4 * (i >> 1) + 2 * part + (i & 1);
+            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || part + i > 0);
+          }
           if (part == 1) mma_commit(&sh.o_done[t]);
         }
         __syncwarp();
@@ -438,8 +442,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   } else if (warp < kUnpackWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
     more_registers<kRowRegs>();
-    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
+    Pair pair = {&sh.told[t][half][r], &sh.told[t][half ^ 1][r], &sh.met[t], 0};
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
     uint32_t count = 0;
@@ -447,46 +452,49 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     while (ok && walk.next(piece)) {
       const int row = piece.tile * kPrefixRows + t * 128 + r, rows = walk.group.count * per_member;
       if (piece.tile * kPrefixRows + t * 128 >= rows) continue;
-      // ---- the row's query, as fp16 at a power of two
+      // ---- the row's query, as fp16 at a power of two: each thread half of its channels
       float c = 1e-36f;
       int vis = walk.group.pages * kInt4Page;
       {
-        uint4 x[D / 8];
-        float most = 0.0f;
+        uint4 x[D / 16];
+        float most = 0.0f, other;
         if (row < rows) {
           const int m = row / per_member, in = row - m * per_member, i = in / p.heads, b = p.plan.members[walk.group.members + m];
-          const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (piece.h * p.heads + in - i * p.heads) * p.q_head + i * p.q_tok;
+          const T* q = static_cast<const T*>(p.q) + b * p.q_seq + (piece.h * p.heads + in - i * p.heads) * p.q_head + i * p.q_tok + D / 2 * half;
           vis = min(vis, int4_seen(p.lengths[b], p.counts != nullptr ? p.counts[b] : p.q_len, i));
 #pragma unroll
-          for (int k = 0; k < D / 8; ++k) x[k] = *reinterpret_cast<const uint4*>(q + 8 * k);
+          for (int k = 0; k < D / 16; ++k) x[k] = *reinterpret_cast<const uint4*>(q + 8 * k);
         } else {
 #pragma unroll
-          for (int k = 0; k < D / 8; ++k) x[k] = make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < D / 16; ++k) x[k] = make_uint4(0, 0, 0, 0);
         }
         auto number = [&](uint32_t v, bool high) {
           if constexpr (std::is_same<T, __half>::value) return high ? half_hi(v) : half_lo(v);
           return __uint_as_float(high ? v & 0xFFFF0000u : v << 16);
         };
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
+        for (int k = 0; k < D / 16; ++k) {
           const uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) most = fmaxf(most, fmaxf(fabsf(number(v[y], false)), fabsf(number(v[y], true))));
         }
+        if (!(ok = pair.exchange(most, other, wait))) break;
+        most = fmaxf(most, other);
         // 2^kq brings the largest magnitude to [2^13, 2^14), or as near as 2^126 does
         const int kq = most > 0.0f && most < INFINITY ? min(126, 13 - (static_cast<int>(__float_as_uint(most) >> 23) - 127)) : 0;
         const float up = p.scale_log2 < 0.0f ? -pow2(kq) : pow2(kq);
         c = fmaxf(pow2(-kq) * fabsf(p.scale_log2), 1e-36f);  // positive, so that a masked score's -inf stays one
         uint8_t* tile = queries + t * C::kTile + r * 128;
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
+        for (int k = 0; k < D / 16; ++k) {
           const uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
           float f[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) f[y] = number(v[y >> 1], y & 1) * up;
           const uint4 w = make_uint4(pack_two<__half>(f[0], f[4]), pack_two<__half>(f[1], f[5]), pack_two<__half>(f[2], f[6]),
                                      pack_two<__half>(f[3], f[7]));
-          *reinterpret_cast<uint4*>(tile + (k >> 3) * kHalfBytes + (((k & 7) ^ (r & 7)) << 4)) = w;
+          const int chunk = D / 16 * half + k;
+          *reinterpret_cast<uint4*>(tile + (chunk >> 3) * kHalfBytes + (((chunk & 7) ^ (r & 7)) << 4)) = w;
         }
       }
       fence_proxy_async_smem();
@@ -499,22 +507,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         const int at = (piece.first + i) * 128;
         if (!(ok = wait(&sh.s_full[t], count & 1))) break;
         tc_fence_after();
-        if (!(ok = soften_tile<__half, D>(tm_s, tm_o, c, at + 128 > vis_min, vis - at, i == 0, st, &sh.p_half[t], &sh.p_ready[t],
-                                          [&] { return wait(&sh.o_done[t], (count - 1) & 1); })))
+        if (!(ok = soften_tile<__half, D>(tm_s, tm_o, half, c, at + 128 > vis_min, vis - at, i == 0, st, pair, &sh.p_early[t], &sh.p_ready[t],
+                                          &sh.o_done[t], (count - 1) & 1, wait)))
           break;
       }
-      if (!ok || !(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+      if (!ok || !(ok = join_sums(st, pair, wait))) break;
+      if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
       tc_fence_after();
       // ---- its record
       float* rec = p.plan.records + (piece.unit + static_cast<int64_t>(blockIdx.x)) * prefix_record(D);
       const int in = t * 128 + r;
       float* acc = rec + 2 * kPrefixRows + static_cast<int64_t>(in) * D;
-      if (row < rows) {
+      if (row < rows && half == 0) {
         rec[in] = st.top == -INFINITY ? kNoScore : fmaxf(st.top, kNoScore);
         rec[kPrefixRows + in] = st.empty() ? 0.0f : st.sum;
       }
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
+      for (int y = 0; y < D / 64; ++y) {
+        const int x = D / 64 * half + y;
         float o[32];
         tmem_ld_x32(tm_o + 32 * x, o);
         tmem_wait_ld();

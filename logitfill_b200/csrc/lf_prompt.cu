@@ -16,6 +16,7 @@ struct PromptParams {
   int32_t* status;
   float scale_log2;
   int batch, tokens, n_q, n_kv, group;
+  int wide_out;  // out rows are 32-byte aligned
 };
 
 // Rows of sequence b: its first, how many tokens it has, and how many out rows it covers.
@@ -83,15 +84,15 @@ using namespace sm100;
 template <int D> struct PromptCfg {
   static constexpr int kTile = 128 * D * 2;                      // bytes of 128 rows
   static constexpr int kSlots = D == 128 ? 5 : 8;                // Key and Value tiles in flight
-  static constexpr int kSmem = 2 * kTile + kSlots * kTile + 1024;  // (aligned by hand)
+  static constexpr int kSmem = 2 * kTile + kSlots * kTile + 3072;  // with what the roles share, and room to align
   static constexpr int kO = 256;                                 // TMEM columns: scores of both tiles, then outputs
 };
-constexpr int kPromptThreads = 384;
-// Registers a thread: 168 at launch (all that 384 threads can have), then moved to the
-// softmax, whose row of 128 scores stays in registers.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kPromptThreads * kLaunchRegs, "more registers than the block has");
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kScanWarp = 11;
+constexpr int kPromptThreads = 640;
+// Registers a thread: 96 at launch, then split between the softmax, whose 64 scores stay in
+// registers, and the others.
+constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
+static_assert(512 * kSoftmaxRegs + 128 * kOtherRegs <= kPromptThreads * kLaunchRegs, "more registers than the block has");
+constexpr int kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18, kScanWarp = 19;
 
 // A piece of work: two query tiles of one KV head of one sequence.
 struct PromptItem {
@@ -103,13 +104,26 @@ struct PromptItem {
 };
 
 struct PromptShared {
-  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
+  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_early[2], p_ready[2], met[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
   PromptItem item[2];
   int bad[2];      // a Value that not all rows of a masked tile see is not finite
   int scan_slot, scan_live, scan_item;  // for the scan: the Value tile, its rows of the sequence, the item's slot
   int stop;        // a wait gave up
   uint32_t tmem;
+  float told[2][2][128];  // between the two threads of a row
 };
+
+// 32 bytes of a row: one store where rows are 32-byte aligned (a whole sector by one lane).
+template <typename T> __device__ __forceinline__ void store_row(T* at, const uint32_t (&w)[8], int wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(at + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
 
 // Whether some row of the query tile that begins at token t0 does not see all of Key tile j.
 __device__ __forceinline__ bool tile_masked(int t0, int j) { return (j + 1) * 128 > t0 + 1; }
@@ -121,10 +135,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = PromptCfg<D>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   constexpr int kHalves = D / 64, kSlots = C::kSlots;
-  extern __shared__ uint8_t dynamic[];
-  __shared__ PromptShared sh;
-  const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, ring = base + 2 * C::kTile;
-  uint8_t* ring_ptr = dynamic + (ring - smem_u32(dynamic));
+  extern __shared__ __align__(1024) uint8_t dynamic[];
+  const uint32_t base = smem_u32(dynamic), ring = base + 2 * C::kTile;
+  uint8_t* ring_ptr = dynamic + 2 * C::kTile;
+  PromptShared& sh = *reinterpret_cast<PromptShared*>(ring_ptr + kSlots * C::kTile);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int per_tile = 128 / p.group;  // tokens of a query tile
 
@@ -141,11 +155,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     mbar_init(&sh.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_half[t], 4);
-      mbar_init(&sh.p_ready[t], 4);
+      mbar_init(&sh.p_early[t], 8);
+      mbar_init(&sh.p_ready[t], 8);
+      mbar_init(&sh.met[t], 8);
       mbar_init(&sh.o_done[t], 1);
       mbar_init(&sh.item_full[t], 1);
-      mbar_init(&sh.item_empty[t], 10);
+      mbar_init(&sh.item_empty[t], 18);
     }
     mbar_init(&sh.scan, 1);
     mbar_init(&sh.scanned, 1);
@@ -295,13 +310,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     bool had[2] = {false, false}, fresh[2] = {false, false};
     auto output = [&](int t) -> bool {  // += weights of tile t times the Value tile of the step before
       for (int part = 0; part < 2; ++part) {
-        if (!wait(part == 0 ? &sh.p_half[t] : &sh.p_ready[t], made[t] & 1)) return false;
+        if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t v = swizzled_desc(ring + (2 * step - 1) % kSlots * C::kTile);
 #pragma unroll
-          for (int k = 4 * part; k < 4 * part + 4; ++k)
-            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || k > 0);
+          for (int i = 0; i < 4; ++i) {  // keys 64 half + 32 part ..
+            const int k = 4 * (i >> 1) + 2 * part + (i & 1);
+            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || part + i > 0);
+          }
           if (part == 1) mma_commit(&sh.o_done[t]);
         }
         __syncwarp();
@@ -421,36 +438,42 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   } else {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
     more_registers<kSoftmaxRegs>();
-    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), tm_s = mine + 128 * t, tm_o = mine + C::kO + t * D;
-    const int in_tile = r / p.group, head = r - in_tile * p.group;
+    Pair pair = {&sh.told[t][half][r], &sh.told[t][half ^ 1][r], &sh.met[t], 0};
     // positive, so that a masked score's -inf stays one; a negative scaling negates the queries in the product
     const float c = fmaxf(fabsf(p.scale_log2), 1e-36f);
     uint32_t count = 0;  // score tiles so far
-    PromptItem it;
     bool ok = true;
-    for (uint32_t n = 0; ok && take(n, it); ++n) {
-      const int t0 = it.tok + t * per_tile, token = t0 + in_tile;
+    for (uint32_t n = 0; ok && wait(&sh.item_full[n & 1], (n >> 1) & 1); ++n) {
+      volatile const PromptItem& it = sh.item[n & 1];  // (read where it is needed: registers are short here)
+      if (it.b < 0) break;
+      const int steps = it.n[t], t0 = it.tok + t * per_tile;
       RowState st = {-INFINITY, 0.0f};
-      for (int j = it.n[t] - 1; j >= 0; --j, ++count) {
-        if (!(ok = wait(&sh.s_full[t], count & 1))) break;
-        tc_fence_after();
-        if (!(ok = soften_tile<T, D>(tm_s, tm_o, c, tile_masked(t0, j), min(token + 1, it.tokens) - 128 * j, j == it.n[t] - 1, st,
-                                     &sh.p_half[t], &sh.p_ready[t], [&] { return wait(&sh.o_done[t], (count - 1) & 1); })))
-          break;
+      {
+        const int sees = min(t0 + r / p.group + 1, it.tokens);
+        for (int j = steps - 1; j >= 0; --j, ++count) {
+          if (!(ok = wait(&sh.s_full[t], count & 1))) break;
+          tc_fence_after();
+          if (!(ok = soften_tile<T, D>(tm_s, tm_o, half, c, tile_masked(t0, j), sees - 128 * j, j == steps - 1, st, pair, &sh.p_early[t],
+                                       &sh.p_ready[t], &sh.o_done[t], (count - 1) & 1, wait)))
+            break;
+        }
       }
       if (!ok) break;
+      const int in_tile = r / p.group, head = r - in_tile * p.group, token = t0 + in_tile;
       const bool stored = in_tile < per_tile && token < it.rows;
       T* out = static_cast<T*>(p.out) + it.b * p.o_seq + (static_cast<int64_t>(it.first) + token) * p.o_tok +
-               (it.h * p.group + head) * p.o_head;
-      if (it.n[t] > 0) {
+               (it.h * p.group + head) * p.o_head + D / 2 * half;
+      if (steps > 0) {
+        if (!(ok = join_sums(st, pair, wait))) break;
         if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
         tc_fence_after();
       }
-      if (it.n[t] > 0 && *const_cast<volatile int*>(&sh.bad[n & 1]) != 0) {
+      if (steps > 0 && *const_cast<volatile int*>(&sh.bad[n & 1]) != 0) {
         const T* k = static_cast<const T*>(p.k) + it.b * p.k_seq + it.first * p.k_tok + it.h * p.k_head;
         const T* v = static_cast<const T*>(p.v) + it.b * p.v_seq + it.first * p.v_tok + it.h * p.v_head;
-        for (int i = 0; i < 32; ++i) {
+        for (int i = half; i < 32; i += 2) {
           const int x = (warp & 3) * 32 + i, tok = t0 + x / p.group, hd = it.h * p.group + x % p.group;
           if (x >= per_tile * p.group || tok >= it.rows) break;
           const int64_t row = static_cast<int64_t>(it.first) + tok;
@@ -459,28 +482,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       } else {
         // else 0: a row behind the sequence, or one of no score above -inf
-        const bool live = it.n[t] > 0 && token < it.tokens && !st.empty();
+        const bool live = steps > 0 && token < it.tokens && !st.empty();
         const float inv = 1.0f / st.sum;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
-          float o[32];
-          if (it.n[t] > 0) {
-            tmem_ld_x32(tm_o + 32 * i, o);
-            tmem_wait_ld();
-            tmem_settle(o);
-          }
+          float o[16];
+          if (steps > 0) tmem_ld_x16(tm_o + D / 2 * half + 16 * i, o);
           if (stored) {
+            uint32_t w[8];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = live ? o[x] * inv : 0.0f;
-#pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-              uint4 w;
-              w.x = pack_two<T>(o[x], o[x + 1]);
-              w.y = pack_two<T>(o[x + 2], o[x + 3]);
-              w.z = pack_two<T>(o[x + 4], o[x + 5]);
-              w.w = pack_two<T>(o[x + 6], o[x + 7]);
-              *reinterpret_cast<uint4*>(out + 32 * i + x) = w;
-            }
+            for (int x = 0; x < 8; ++x) w[x] = live ? pack_two<T>(o[2 * x] * inv, o[2 * x + 1] * inv) : 0u;
+            store_row(out + 16 * i, w, p.wide_out);
           }
         }
       }
@@ -584,6 +596,7 @@ extern "C" int lf_prompt_attend(const lf_prompt* a, lf_stream_t stream) {
   p.n_q = a->n_q;
   p.n_kv = a->n_kv;
   p.group = a->n_q / a->n_kv;
+  p.wide_out = reinterpret_cast<uintptr_t>(a->out) % 32 == 0 && (p.o_seq | p.o_head | p.o_tok) % 16 == 0;
   const int sms = sm_count();
   if (sms <= 0) {
     set_error("lf_prompt_attend: the current device's SMs cannot be counted");
