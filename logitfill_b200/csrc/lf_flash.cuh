@@ -119,20 +119,56 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
-// Wait of a whole warp for a barrier's phase, with a limit: false once a wait of this CTA
-// has given up (*stop), for all lanes alike.
-constexpr uint64_t kTileWaitNs = 2000000000ull;
+// Wait of a whole warp for a barrier's phase, with a limit (of tries: reading a clock
+// between them costs more than the wait): false once a wait of this CTA has given up
+// (*stop), for all lanes alike.
+constexpr uint32_t kMostTries = 1u << 24;
+constexpr uint64_t kTileWaitNs = 2000000000ull;  // of the waits at a CTA's end
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
   bool ok = mbar_try_wait(bar, parity);
-  if (!ok) {
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t n = 1; !ok; ++n) {
-      ok = mbar_try_wait(bar, parity);
-      if (!ok && (n & 63u) == 0u && (*stop != 0 || globaltimer_ns() - t0 > kTileWaitNs)) break;
+  for (uint32_t n = 1; !ok; ++n) {
+    ok = mbar_try_wait(bar, parity);
+    if ((n & 1023u) == 0u && !ok && (*stop != 0 || n >= kMostTries)) {
+      *stop = 1;
+      break;
     }
-    if (!ok) *stop = 1;
   }
   return __all_sync(0xffffffffu, ok);
+}
+
+// Products of one tile (128 rows), issued by one lane of the calling warp.
+// Scores: queries times Keys, D channels of 128 rows each in shared memory.  `full` completes
+// with them, and so with everything that this warp issued before.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t tmem_s, uint32_t queries, uint32_t keys, uint32_t idesc, uint64_t* full) {
+  if (elect_one()) {
+    const uint64_t a = swizzled_desc(queries), b = swizzled_desc(keys);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+      mma_16_ss(tmem_s, a + off, b + off, idesc, k > 0);
+    }
+    mma_commit(full);
+  }
+  __syncwarp();
+}
+// Outputs: weights (in the scores' place) times Values, keys 64 half + 32 part .. of both
+// halves.  done: as full, or null.
+__device__ __forceinline__ void issue_outputs(uint32_t tmem_o, uint32_t tmem_p, uint32_t values, uint32_t idesc, int part, bool fresh, uint64_t* done) {
+  if (elect_one()) {
+    const uint64_t v = swizzled_desc(values);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 4 * (i >> 1) + 2 * part + (i & 1);
+      mma_16_ts(tmem_o, tmem_p + 8 * k, v + k * (16 * 128 >> 4), idesc, !fresh || part + i > 0);
+    }
+    if (done != nullptr) mma_commit(done);
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void arrive_once(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // The softmax of one 128 x 128 tile of scores by 8 warps: two threads to a row (TMEM lane =
@@ -142,10 +178,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // 2^kLift for the running maximum.  It is moved only where a score passes it by 2^kSlack,
 // so most tiles skip the rescaling of the output.
 constexpr float kSlack = 8.0f;
-#ifndef LF_POLY
-#define LF_POLY 3
-#endif
-constexpr int kPolyPairs = LF_POLY;
 template <typename T> constexpr float kLift = 0.0f;
 // fp16 ends at steps of 2^-24: with the largest weight at 2^7, what is lost of a small
 // weight is 2^-32 of it at most (and 2^(7 + 8) still fits).
@@ -177,8 +209,7 @@ struct Pair {
   uint32_t phase;
   template <typename Wait>
   __device__ __forceinline__ bool meet(Wait&& wait) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(met);
+    arrive_once(met);
     return wait(met, phase++ & 1);
   }
   // The next exchange may begin once the other thread has read this one's number: after
@@ -293,32 +324,29 @@ __device__ __forceinline__ void rescale(uint32_t tmem_o, float fix) {
 
 // A thread's part of a tile: columns 64 half .. of its row's scores to weights (which take
 // the first 64 columns' place, two to a column), first 32 columns, then 32: the output
-// product over these may begin when `early`, then `ready` is complete (8 warps each).
-// fresh: the row's first tile; done: the barrier of the output product before, at parity.
+// product over these may begin when `early`, then `ready` has 8 warps' arrivals.
+// fresh: the row's first tile.  (The output product before is done: it was issued before
+// these scores, whose barrier the caller has seen.)
 // wait(barrier, parity) is false once a limit ran out, and so is the result then.
-template <typename T, int D, typename Wait>
+// on_masked() is called on a masked tile before its first weights are handed over.
+template <typename T, int D, int kPoly, typename Wait, typename Masked>
 __device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, int half, float c, bool masked, int seen, bool fresh,
-                                            RowState& st, Pair& pair, uint64_t* early, uint64_t* ready, uint64_t* done, uint32_t parity,
-                                            Wait&& wait) {
+                                            RowState& st, Pair& pair, uint64_t* early, uint64_t* ready, Wait&& wait, Masked&& on_masked) {
   float s[64], other;
   const float most = row_scores(tmem_s + 64 * half, s, masked, seen - 64 * half);
   if (!pair.exchange(most, other, wait)) return false;
   const float fix = move_top(max_nan2(most, other), c, st);
-  if (!fresh && __any_sync(0xffffffffu, fix != 1.0f)) {
-    if (!wait(done, parity)) return false;
-    tc_fence_after();
-    rescale<D / 2>(tmem_o + D / 2 * half, fix);
-  }
+  if (masked && !on_masked()) return false;
+  if (!fresh && __any_sync(0xffffffffu, fix != 1.0f)) rescale<D / 2>(tmem_o + D / 2 * half, fix);
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     if (masked)  // a masked score's weight is 0, not 2^-126
       row_weights<T, 0>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
     else
-      row_weights<T, kPolyPairs>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
+      row_weights<T, kPoly>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
     tmem_wait_st();
     tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(part == 0 ? early : ready);
+    arrive_once(part == 0 ? early : ready);
   }
   return true;
 }

@@ -133,7 +133,7 @@ constexpr int kUnpackWarp = 16, kProductWarp = 20, kCopyWarp = 21;
 constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
 
 struct PrefixShared {
-  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2];
+  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2], last;
   int stop;
   uint32_t tmem;
   float told[2][2][128];  // between the two threads of a row
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       mbar_init(&sh.met[t], 8);
       mbar_init(&sh.o_done[t], 1);
     }
+    mbar_init(&sh.last, 1);
     sh.stop = 0;
     fence_mbar_init();
   }
@@ -370,74 +371,52 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
     const uint32_t idesc_s = idesc_16(false, 128, 128, false, false), idesc_o = idesc_16(false, 128, D, true, false);
-    const uint32_t ring_a = smem_u32(ring), queries_a = smem_u32(queries);
+    const uint32_t ring_a = smem_u32(ring);
     uint32_t step = 0, made[2] = {0, 0}, asked[2] = {0, 0};
-    bool had[2] = {false, false}, fresh = false, ok = true;
-    auto output = [&](int t) -> bool {
+    bool had[2] = {false, false}, fresh = false, ends = false, ok = true;
+    auto output = [&](int t) -> bool {  // of the step before
+      if (!had[t]) return true;
+      const uint32_t load = 2 * step - 1, slot = load % kSlots;
+      if (!wait(&sh.kv_full[slot], (load / kSlots) & 1)) return false;
       for (int part = 0; part < 2; ++part) {
         if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
-        if (elect_one()) {
-          const uint64_t v = swizzled_desc(ring_a + (2 * step - 1) % kSlots * C::kTile);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // keys 64 half + 32 part ..
-            const int k = 4 * (i >> 1) + 2 * part + (i & 1);
-            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh || part + i > 0);
-          }
-          if (part == 1) mma_commit(&sh.o_done[t]);
-        }
-        __syncwarp();
+        issue_outputs(tmem + C::kO + t * D, tmem + 128 * t, ring_a + slot * C::kTile, idesc_o, part, fresh, ends && part == 1 ? &sh.o_done[t] : nullptr);
       }
       ++made[t];
       return true;
     };
-    auto free_slot = [&](uint32_t load) {
-      if (elect_one()) mma_commit(&sh.kv_empty[load % kSlots]);
-      __syncwarp();
+    auto scores = [&](int t) {
+      tc_fence_after();
+      issue_scores<D>(tmem + 128 * t, smem_u32(queries) + t * C::kTile, ring_a + 2 * step % kSlots * C::kTile, idesc_s, &sh.s_full[t]);
     };
     while (ok && walk.next(piece)) {
-      const int rows = walk.group.count * per_member - piece.tile * kPrefixRows;
-      const bool now[2] = {true, rows > 128};
-      for (int i = 0; i < piece.n; ++i) {
-        const uint32_t load = 2 * step;
-        if (!(ok = wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1))) break;
-        if (step > 0 && !(ok = wait(&sh.kv_full[(load - 1) % kSlots], ((load - 1) / kSlots) & 1))) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (had[t] && !(ok = output(t))) break;
-          if (!now[t]) continue;
-          if (i == 0 && !(ok = wait(&sh.q_ready[t], asked[t]++ & 1))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t a = swizzled_desc(queries_a + t * C::kTile), b = swizzled_desc(ring_a + load % kSlots * C::kTile);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
-              mma_16_ss(tmem + 128 * t, a + off, b + off, idesc_s, k > 0);
-            }
-            mma_commit(&sh.s_full[t]);
-          }
-          __syncwarp();
+      const bool two = piece.tile * kPrefixRows + 128 < walk.group.count * per_member;
+      for (int i = 0; i < piece.n; ++i, ++step) {
+        if (i == 0) {  // (new queries are made only after the outputs of the piece before)
+          if (step > 0 && !(ok = output(0) && output(1))) break;
+          if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1) && wait(&sh.q_ready[0], asked[0]++ & 1))) break;
+          scores(0);
+          if (two && !(ok = wait(&sh.q_ready[1], asked[1]++ & 1))) break;
+          if (two) scores(1);
+        } else {
+          if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
+          if (!(ok = output(0))) break;
+          scores(0);
+          if (!(ok = output(1))) break;
+          if (two) scores(1);
         }
-        if (!ok) break;
-        if (step > 0) free_slot(load - 1);
-        free_slot(load);
-        had[0] = now[0];
-        had[1] = now[1];
+        had[0] = true;
+        had[1] = two;
         fresh = i == 0;
-        ++step;
+        ends = i == piece.n - 1;
       }
     }
-    if (ok && step > 0 && *stop == 0) {  // the last step's outputs
-      const uint32_t load = 2 * step - 1;
-      ok = wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1);
-      for (int t = 0; ok && t < 2; ++t) ok = !had[t] || output(t);
-      if (ok) free_slot(load);
-    }
-    // No product, and no arrival of one, outlives the CTA.
-    for (uint32_t i = 0; i < kSlots; ++i) {
-      const uint32_t used = 2 * step / kSlots + (i < 2 * step % kSlots ? 1 : 0);
-      if (used != 0) mbar_wait_bounded(&sh.kv_empty[i], (used - 1) & 1, kTileWaitNs);
+    if (ok && step > 0 && *stop == 0 && output(0)) output(1);  // the last step's
+    if (*stop != 0) {  // the products in flight, before their operands go
+      if (elect_one()) mma_commit(&sh.last);
+      __syncwarp();
+      mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
     }
   } else if (warp < kUnpackWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
@@ -447,10 +426,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     Pair pair = {&sh.told[t][half][r], &sh.told[t][half ^ 1][r], &sh.met[t], 0};
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
     Piece piece;
-    uint32_t count = 0;
+    uint32_t count = 0, pieces = 0, steps = 0;
+    const bool frees = (warp & 7) == 0;
     bool ok = true;
     while (ok && walk.next(piece)) {
       const int row = piece.tile * kPrefixRows + t * 128 + r, rows = walk.group.count * per_member;
+      const uint32_t before = steps;  // of the CTA
+      steps += piece.n;
       if (piece.tile * kPrefixRows + t * 128 >= rows) continue;
       // ---- the row's query, as fp16 at a power of two: each thread half of its channels
       float c = 1e-36f;
@@ -507,12 +489,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         const int at = (piece.first + i) * 128;
         if (!(ok = wait(&sh.s_full[t], count & 1))) break;
         tc_fence_after();
-        if (!(ok = soften_tile<__half, D>(tm_s, tm_o, half, c, at + 128 > vis_min, vis - at, i == 0, st, pair, &sh.p_early[t], &sh.p_ready[t],
-                                          &sh.o_done[t], (count - 1) & 1, wait)))
+        if (frees && (t == 1 || rows - piece.tile * kPrefixRows <= 128)) {
+          // The step's last scores are done, and with them all products before: the Key tile
+          // is free, and the Value tile of the step before.
+          const uint32_t load = 2 * (before + i);
+          arrive_once(&sh.kv_empty[load % kSlots]);
+          if (load > 0) arrive_once(&sh.kv_empty[(load - 1) % kSlots]);
+        }
+        if (!(ok = soften_tile<__half, D, 0>(tm_s, tm_o, half, c, at + 128 > vis_min, vis - at, i == 0, st, pair, &sh.p_early[t], &sh.p_ready[t],
+                                          wait, [] { return true; })))
           break;
       }
       if (!ok || !(ok = join_sums(st, pair, wait))) break;
-      if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+      if (!(ok = wait(&sh.o_done[t], pieces++ & 1))) break;
       tc_fence_after();
       // ---- its record
       float* rec = p.plan.records + (piece.unit + static_cast<int64_t>(blockIdx.x)) * prefix_record(D);

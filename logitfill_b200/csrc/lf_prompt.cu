@@ -92,7 +92,10 @@ constexpr int kPromptThreads = 640;
 // registers, and the others.
 constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
 static_assert(512 * kSoftmaxRegs + 128 * kOtherRegs <= kPromptThreads * kLaunchRegs, "more registers than the block has");
-constexpr int kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18, kScanWarp = 19;
+// Of every 8 pairs of exponentials, those by the polynomial.  8192 tokens, 28 heads on 4,
+// D 128: none 420 us, two 414, three 418.
+constexpr int kPolyPairs = 2;
+constexpr int kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18;
 
 // A piece of work: two query tiles of one KV head of one sequence.
 struct PromptItem {
@@ -104,10 +107,9 @@ struct PromptItem {
 };
 
 struct PromptShared {
-  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_early[2], p_ready[2], met[2], o_done[2], item_full[2], item_empty[2], scan, scanned, last;
+  uint64_t kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_early[2], p_ready[2], met[2], o_done[2], item_full[2], item_empty[2], last;
   PromptItem item[2];
   int bad[2];      // a Value that not all rows of a masked tile see is not finite
-  int scan_slot, scan_live, scan_item;  // for the scan: the Value tile, its rows of the sequence, the item's slot
   int stop;        // a wait gave up
   uint32_t tmem;
   float told[2][2][128];  // between the two threads of a row
@@ -123,6 +125,28 @@ template <typename T> __device__ __forceinline__ void store_row(T* at, const uin
     *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(at + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   }
+}
+
+// A weight of 0 does not keep a NaN or an infinity out of a product.  So of a Value tile
+// that some row sees in part, the 256 threads of a query tile zero the rows behind the
+// sequence, and a number that is not finite is reported: it sends the item to prompt_row.
+template <typename T, int D> __device__ __forceinline__ bool scan_value(uint8_t* tile, int live) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) {
+    const int i = (threadIdx.x & 255) + 256 * x;  // 16 bytes; 8 of them a row, 1024 a half
+    uint4* at = reinterpret_cast<uint4*>(tile) + i;
+    const uint4 y = *at;
+    if (i % 1024 / 8 >= live) {  // (the other query tile's threads may have done it: then it is only read)
+      if ((y.x | y.y | y.z | y.w) != 0) *at = make_uint4(0, 0, 0, 0);
+    } else {
+      // an exponent of all ones carries into the sign's place
+      constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+      seen |= ((y.x & 0x7FFF7FFFu) + kOne) | ((y.y & 0x7FFF7FFFu) + kOne) | ((y.z & 0x7FFF7FFFu) + kOne) | ((y.w & 0x7FFF7FFFu) + kOne);
+    }
+  }
+  fence_proxy_async_smem();
+  return (seen & 0x80008000u) != 0;
 }
 
 // Whether some row of the query tile that begins at token t0 does not see all of Key tile j.
@@ -153,6 +177,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.last, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.s_full[t], 1);
       mbar_init(&sh.p_early[t], 8);
@@ -162,9 +187,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&sh.item_full[t], 1);
       mbar_init(&sh.item_empty[t], 18);
     }
-    mbar_init(&sh.scan, 1);
-    mbar_init(&sh.scanned, 1);
-    mbar_init(&sh.last, 1);
     sh.stop = 0;
     fence_mbar_init();
   }
@@ -281,161 +303,77 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         __syncwarp();
       }
     }
-    // Every copy and every arrival of the tensor core's has come in before the CTA ends
-    // (after a wait that gave up: as far as the limit goes).
+    // No copy outlives the CTA (after a wait that gave up: as far as the limit goes).
     for (int i = 0; i < kSlots; ++i) {
-      const uint32_t done = load / kSlots + (static_cast<uint32_t>(i) < load % kSlots ? 1 : 0);
-      if (done == 0) continue;
-      if (*stop == 0)
-        wait(&sh.kv_empty[i], (done - 1) & 1);
-      else
-        mbar_wait_bounded(&sh.kv_full[i], (done - 1) & 1, kTileWaitNs);
+      const uint32_t used = load / kSlots + (static_cast<uint32_t>(i) < load % kSlots ? 1 : 0);
+      if (used != 0) mbar_wait_bounded(&sh.kv_full[i], (used - 1) & 1, kTileWaitNs);
     }
-    if (n_q > 0) {
-      if (*stop == 0)
-        wait(&sh.q_empty, (n_q - 1) & 1);
-      else
-        mbar_wait_bounded(&sh.q_full, (n_q - 1) & 1, kTileWaitNs);
-    }
+    if (n_q > 0) mbar_wait_bounded(&sh.q_full, (n_q - 1) & 1, kTileWaitNs);
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- products
     fewer_registers<kOtherRegs>();
     // Step s of the CTA: scores of Key tile (load 2 s) for both query tiles, after the
     // output product of step s - 1 (Value tile, load 2 s - 1), tile by tile: while the
-    // softmax of one tile runs, the tensor core works for the other.
+    // softmax of one tile runs, the tensor core works for the other.  The only commits are
+    // the scores' and an item's last outputs' (each takes this warp over 100 cycles): what
+    // else a tile's scores say is done, the softmax passes on.
     const uint32_t idesc_s = idesc_16(kBf16, 128, 128, false, p.scale_log2 < 0.0f), idesc_o = idesc_16(kBf16, 128, D, true, false);
-    uint32_t step = 0, n_q = 0, made[2] = {0, 0}, masked_steps = 0;
-    int live = 0;        // rows of the sequence in the step before's Value tile, where it is masked, else 0
-    uint32_t number = 0;  // and its item
-    bool had[2] = {false, false}, fresh[2] = {false, false};
-    auto output = [&](int t) -> bool {  // += weights of tile t times the Value tile of the step before
+    uint32_t step = 0, n_q = 0, made[2] = {0, 0};
+    bool had[2] = {false, false}, fresh[2] = {false, false}, ends = false;
+    auto output = [&](int t) -> bool {  // of the step before
+      if (!had[t]) return true;
+      const uint32_t load = 2 * step - 1, slot = load % kSlots;
+      if (!wait(&sh.kv_full[slot], (load / kSlots) & 1)) return false;
       for (int part = 0; part < 2; ++part) {
         if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
-        if (elect_one()) {
-          const uint64_t v = swizzled_desc(ring + (2 * step - 1) % kSlots * C::kTile);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // keys 64 half + 32 part ..
-            const int k = 4 * (i >> 1) + 2 * part + (i & 1);
-            mma_16_ts(tmem + C::kO + t * D, tmem + 128 * t + 8 * k, v + k * (16 * 128 >> 4), idesc_o, !fresh[t] || part + i > 0);
-          }
-          if (part == 1) mma_commit(&sh.o_done[t]);
-        }
-        __syncwarp();
+        issue_outputs(tmem + C::kO + t * D, tmem + 128 * t, ring + slot * C::kTile, idesc_o, part, fresh[t], ends && part == 1 ? &sh.o_done[t] : nullptr);
       }
       ++made[t];
       return true;
     };
-    auto value_there = [&]() -> bool {
-      const uint32_t load = 2 * step - 1;
-      if (!wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1)) return false;
-      if (live == 0) return true;
-      if (lane == 0) {
-        sh.scan_slot = load % kSlots;
-        sh.scan_live = live;
-        sh.scan_item = number & 1;
-        mbar_arrive(&sh.scan);
-      }
-      __syncwarp();
-      return wait(&sh.scanned, masked_steps++ & 1);
-    };
-    auto free_slot = [&](uint32_t load) {
-      if (elect_one()) mma_commit(&sh.kv_empty[load % kSlots]);
-      __syncwarp();
+    auto scores = [&](int t) {
+      tc_fence_after();
+      issue_scores<D>(tmem + 128 * t, base + t * C::kTile, ring + 2 * step % kSlots * C::kTile, idesc_s, &sh.s_full[t]);
     };
     PromptItem it;
     bool ok = true;
     for (uint32_t n = 0; ok && take(n, it); ++n) {
       give(n);
       const int steps = max(it.n[0], it.n[1]);
-      if (steps == 0) continue;
-      for (int j = steps - 1; ok && j >= 0; --j) {
-        if (j == steps - 1) {
-          if (!(ok = wait(&sh.q_full, n_q & 1))) break;
-          ++n_q;
+      if (steps == 0) {  // (nothing later may wait for an item to come: the softmax needs these to let it go)
+        if (!(ok = output(0) && output(1))) break;
+        had[0] = had[1] = false;
+      }
+      for (int j = steps - 1; j >= 0; --j, ++step) {
+        const bool now[2] = {j < it.n[0], j < it.n[1]};
+        if (j == steps - 1) {  // the outputs of the item before do not wait for this one's queries
+          if (step > 0 && !(ok = output(0) && output(1))) break;
+          if (!(ok = wait(&sh.q_full, n_q++ & 1) && wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
+          if (now[0]) scores(0);
+          if (now[1]) scores(1);
+        } else {
+          if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
+          if (!(ok = output(0))) break;
+          if (now[0]) scores(0);
+          if (!(ok = output(1))) break;
+          if (now[1]) scores(1);
         }
-        if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
-        if (step > 0 && !(ok = value_there())) break;
-        bool now[2], masked = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          now[t] = j < it.n[t];
-          masked |= now[t] && tile_masked(it.tok + t * per_tile, j);
-          if (had[t] && !(ok = output(t))) break;
-          if (now[t]) {
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t a = swizzled_desc(base + t * C::kTile), b = swizzled_desc(ring + 2 * step % kSlots * C::kTile);
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
-                mma_16_ss(tmem + 128 * t, a + off, b + off, idesc_s, k > 0);
-              }
-              mma_commit(&sh.s_full[t]);
-            }
-            __syncwarp();
-            fresh[t] = j == it.n[t] - 1;
-          }
+          had[t] = now[t];
+          fresh[t] = j == it.n[t] - 1;
         }
-        if (!ok) break;
-        had[0] = now[0];
-        had[1] = now[1];
-        live = masked ? min(128, it.tokens - 128 * j) : 0;
-        number = n;
-        if (step > 0) free_slot(2 * step - 1);
-        free_slot(2 * step);
-        if (j == 0) {
-          if (elect_one()) mma_commit(&sh.q_empty);
-          __syncwarp();
-        }
-        ++step;
+        ends = j == 0;
       }
     }
-    if (ok && step > 0 && *stop == 0) {  // the last step's outputs
-      ok = value_there();
-      for (int t = 0; ok && t < 2; ++t) ok = !had[t] || output(t);
-      if (ok) free_slot(2 * step - 1);
-    }
-    if (lane == 0) {
-      sh.scan_slot = -1;
-      mbar_arrive(&sh.scan);
-    }
-    __syncwarp();
+    if (ok && step > 0 && *stop == 0 && output(0)) output(1);  // the last step's
     if (*stop != 0) {  // the products in flight, before their operands go
       if (elect_one()) mma_commit(&sh.last);
       __syncwarp();
       mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
     }
-  } else if (warp == kScanWarp) {
-    // ---------------------------------------------------------------- masked Value tiles
-    fewer_registers<kOtherRegs>();
-    // A weight of 0 does not keep a NaN or an infinity out of a product.  Of the Value
-    // tiles that some row sees in part, rows behind the sequence are zeroed here, and a
-    // number that is not finite sends the item to prompt_row.
-    for (uint32_t n = 0; wait(&sh.scan, n & 1); ++n) {
-      const int slot = *const_cast<volatile int*>(&sh.scan_slot), live = *const_cast<volatile int*>(&sh.scan_live);
-      if (slot < 0) break;
-      uint4* tile = reinterpret_cast<uint4*>(ring_ptr + slot * C::kTile);
-      uint32_t seen = 0;
-#pragma unroll 8
-      for (int i = lane; i < C::kTile / 16; i += 32) {
-        if (i % 1024 / 8 >= live) {
-          tile[i] = make_uint4(0, 0, 0, 0);
-        } else {
-          const uint4 x = tile[i];  // an exponent of all ones carries into the sign's place
-          constexpr uint32_t kOne = kBf16 ? 0x00800080u : 0x04000400u;
-          seen |= (x.x & 0x7FFF7FFFu) + kOne;
-          seen |= (x.y & 0x7FFF7FFFu) + kOne;
-          seen |= (x.z & 0x7FFF7FFFu) + kOne;
-          seen |= (x.w & 0x7FFF7FFFu) + kOne;
-        }
-      }
-      if ((seen & 0x80008000u) != 0) sh.bad[*const_cast<volatile int*>(&sh.scan_item)] = 1;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.scanned);
-    }
-  } else {
+  } else if (warp < kMmaWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
     more_registers<kSoftmaxRegs>();
     const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
@@ -443,31 +381,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     Pair pair = {&sh.told[t][half][r], &sh.told[t][half ^ 1][r], &sh.met[t], 0};
     // positive, so that a masked score's -inf stays one; a negative scaling negates the queries in the product
     const float c = fmaxf(fabsf(p.scale_log2), 1e-36f);
-    uint32_t count = 0;  // score tiles so far
+    uint32_t count = 0, items = 0, before = 0;  // score tiles and items with some so far, steps of the items before
+    const bool frees = (warp & 7) == 0;
     bool ok = true;
     for (uint32_t n = 0; ok && wait(&sh.item_full[n & 1], (n >> 1) & 1); ++n) {
       volatile const PromptItem& it = sh.item[n & 1];  // (read where it is needed: registers are short here)
       if (it.b < 0) break;
-      const int steps = it.n[t], t0 = it.tok + t * per_tile;
+      const int steps = it.n[t], all = max(it.n[0], it.n[1]), t0 = it.tok + t * per_tile;
       RowState st = {-INFINITY, 0.0f};
       {
         const int sees = min(t0 + r / p.group + 1, it.tokens);
         for (int j = steps - 1; j >= 0; --j, ++count) {
           if (!(ok = wait(&sh.s_full[t], count & 1))) break;
           tc_fence_after();
-          if (!(ok = soften_tile<T, D>(tm_s, tm_o, half, c, tile_masked(t0, j), sees - 128 * j, j == steps - 1, st, pair, &sh.p_early[t],
-                                       &sh.p_ready[t], &sh.o_done[t], (count - 1) & 1, wait)))
+          const uint32_t load = 2 * (before + all - 1 - j);  // of the Key tile; the Value tile is the next
+          if (frees && (t == 1 || j >= it.n[1])) {
+            // The step's last scores are done, and with them all products before: the Key
+            // tile is free, the Value tile of the step before, after the last step the queries.
+            arrive_once(&sh.kv_empty[load % kSlots]);
+            if (load > 0) arrive_once(&sh.kv_empty[(load - 1) % kSlots]);
+            if (j == 0) arrive_once(&sh.q_empty);
+          }
+          if (!(ok = soften_tile<T, D, kPolyPairs>(tm_s, tm_o, half, c, tile_masked(t0, j), sees - 128 * j, j == steps - 1, st, pair, &sh.p_early[t], &sh.p_ready[t], wait, [&] {
+                                         const uint32_t slot = (load + 1) % kSlots;
+                                         if (!wait(&sh.kv_full[slot], ((load + 1) / kSlots) & 1)) return false;
+                                         if (scan_value<T, D>(ring_ptr + slot * C::kTile, min(128, it.tokens - 128 * j))) sh.bad[n & 1] = 1;
+                                         return true;
+                                       })))
             break;
         }
       }
       if (!ok) break;
+      before += all;
       const int in_tile = r / p.group, head = r - in_tile * p.group, token = t0 + in_tile;
       const bool stored = in_tile < per_tile && token < it.rows;
       T* out = static_cast<T*>(p.out) + it.b * p.o_seq + (static_cast<int64_t>(it.first) + token) * p.o_tok +
                (it.h * p.group + head) * p.o_head + D / 2 * half;
       if (steps > 0) {
         if (!(ok = join_sums(st, pair, wait))) break;
-        if (!(ok = wait(&sh.o_done[t], (count - 1) & 1))) break;
+        if (!(ok = wait(&sh.o_done[t], items++ & 1))) break;
         tc_fence_after();
       }
       if (steps > 0 && *const_cast<volatile int*>(&sh.bad[n & 1]) != 0) {
@@ -499,6 +451,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       tc_fence_before();
       give(n);
     }
+  } else {
+    fewer_registers<kOtherRegs>();  // (of a warpgroup, all warps at once)
   }
   tc_fence_before();
   __syncthreads();

@@ -320,6 +320,20 @@ def test_padded_batches(dtype, D, B, T, n_q, n_kv):
         _check_prompts(every[b].transpose(0, 1), *(x[b].transpose(0, 1) for x in full), [T], D ** -0.5, dtype)
 
 
+def test_padding_alone_between_prompts():
+    """Many tiles of nothing but padding before, between and after those with tokens."""
+    counts, T, D = [0, 3, 0, 0, 1500, 0], 1500, 128
+    q, k, v = _prompts(21, [T] * 6, 4, 2, D)
+    q, k, v = (x.view(6, T, -1, D).transpose(1, 2) for x in (q, k, v))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = prompt.prompt_attention(q, k, v, 0.09, counts=torch.tensor(counts, dtype=torch.int32, device="cuda"), status=status)
+    assert int(status) == 0
+    for b, c in enumerate(counts):
+        assert not bool(got[b, :, c:].any())
+        if c:
+            _check_prompts(got[b].transpose(0, 1), *(x[b].transpose(0, 1) for x in (q, k, v)), [c], 0.09, BF16)
+
+
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64)])
 def test_rows_of_no_sequence_stay_as_they_were(dtype, D):
     """Rows before, between and behind the sequences, NaN in all of them."""
