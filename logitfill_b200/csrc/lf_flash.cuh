@@ -137,30 +137,34 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 // Products of one tile (128 rows), issued by one lane of the calling warp.
-// Scores: queries times Keys, D channels of 128 rows each in shared memory.  `full` completes
-// with them, and so with everything that this warp issued before.
+// Scores: queries times Keys, D channels of 128 rows each in shared memory (+=: to what is
+// there).  `full`, if given, completes with them, and so with everything that this warp
+// issued before.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t tmem_s, uint32_t queries, uint32_t keys, uint32_t idesc, uint64_t* full) {
+__device__ __forceinline__ void issue_scores(uint32_t tmem_s, uint32_t queries, uint32_t keys, uint32_t idesc, bool add, uint64_t* full) {
   if (elect_one()) {
     const uint64_t a = swizzled_desc(queries), b = swizzled_desc(keys);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const uint32_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
-      mma_16_ss(tmem_s, a + off, b + off, idesc, k > 0);
+      mma_16_ss(tmem_s, a + off, b + off, idesc, add || k > 0);
     }
-    mma_commit(full);
+    if (full != nullptr) mma_commit(full);
   }
   __syncwarp();
 }
-// Outputs: weights (in the scores' place) times Values, keys 64 half + 32 part .. of both
-// halves.  done: as full, or null.
+// Outputs: weights (in the scores' place, kTerms numbers each) times Values, keys 64 half +
+// 32 part .. of both halves.  done: as full, or null.
+template <int kTerms>
 __device__ __forceinline__ void issue_outputs(uint32_t tmem_o, uint32_t tmem_p, uint32_t values, uint32_t idesc, int part, bool fresh, uint64_t* done) {
   if (elect_one()) {
     const uint64_t v = swizzled_desc(values);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = 4 * (i >> 1) + 2 * part + (i & 1);
-      mma_16_ts(tmem_o, tmem_p + 8 * k, v + k * (16 * 128 >> 4), idesc, !fresh || part + i > 0);
+#pragma unroll
+      for (int x = 0; x < kTerms; ++x)
+        mma_16_ts(tmem_o, tmem_p + 64 * x + 8 * k, v + k * (16 * 128 >> 4), idesc, !fresh || part + i + x > 0);
     }
     if (done != nullptr) mma_commit(done);
   }
@@ -287,24 +291,37 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
 }
 
-// Weights of 32 scores, stored in T at 16 columns.  kPoly of every 8 pairs go by the
-// polynomial: the special function unit gives 16 results a cycle, as long as the tensor
-// core takes for both products of them.
-template <typename T, int kPoly>
+// Weights of 32 scores, stored in T at 16 columns, and with kTerms 2 what T's rounding left
+// of them 64 columns on.  kPoly of every 8 pairs go by the polynomial: the special function
+// unit gives 16 results a cycle, as long as the tensor core takes for both products of them.
+template <typename T, int kPoly, int kTerms>
 __device__ __forceinline__ void row_weights(uint32_t tmem_p, const float* s, float c, RowState& st) {
   // The product of maximum and c is rounded once, and taken as it is everywhere: it
   // cancels in the quotient of output and sum.
   const float base = kLift<T> - (st.top == -INFINITY ? 0.0f : st.top);
   float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-  uint32_t w[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(base, base));
-    const float2 e = i % 8 < kPoly ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(x) : make_float2(ex2(x.x), ex2(x.y));
-    sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-    w[i] = pack_two<T>(e.x, e.y);
+  for (int part = 0; part < kTerms; ++part) {  // (two terms: 8 columns at a time, for registers)
+    uint32_t w[16 / kTerms], low[8];
+#pragma unroll
+    for (int i = 0; i < 16 / kTerms; ++i) {
+      const int at = 16 * part / kTerms + i;
+      const float2 x = __ffma2_rn(make_float2(s[2 * at], s[2 * at + 1]), make_float2(c, c), make_float2(base, base));
+      const float2 e = at % 8 < kPoly ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(x) : make_float2(ex2(x.x), ex2(x.y));
+      sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+      w[i] = pack_two<T>(e.x, e.y);
+      if constexpr (kTerms == 2) {
+        const float2 r = __fadd2_rn(e, make_float2(-half_bits_to_float(w[i] & 0xFFFFu), -half_bits_to_float(w[i] >> 16)));
+        low[i] = pack_two<T>(r.x, r.y);
+      }
+    }
+    if constexpr (kTerms == 1) {
+      tmem_st_x16(tmem_p, w);
+    } else {
+      tmem_st_x8(tmem_p + 8 * part, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+      tmem_st_x8(tmem_p + 64 + 8 * part, low[0], low[1], low[2], low[3], low[4], low[5], low[6], low[7]);
+    }
   }
-  tmem_st_x16(tmem_p, w);
   st.sum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
@@ -329,7 +346,7 @@ __device__ __forceinline__ void rescale(uint32_t tmem_o, float fix) {
 // these scores, whose barrier the caller has seen.)
 // wait(barrier, parity) is false once a limit ran out, and so is the result then.
 // on_masked() is called on a masked tile before its first weights are handed over.
-template <typename T, int D, int kPoly, typename Wait, typename Masked>
+template <typename T, int D, int kPoly, int kTerms, typename Wait, typename Masked>
 __device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, int half, float c, bool masked, int seen, bool fresh,
                                             RowState& st, Pair& pair, uint64_t* early, uint64_t* ready, Wait&& wait, Masked&& on_masked) {
   float s[64], other;
@@ -341,9 +358,9 @@ __device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, in
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     if (masked)  // a masked score's weight is 0, not 2^-126
-      row_weights<T, 0>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
+      row_weights<T, 0, kTerms>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
     else
-      row_weights<T, kPoly>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
+      row_weights<T, kPoly, kTerms>(tmem_s + 32 * half + 16 * part, s + 32 * part, c, st);
     tmem_wait_st();
     tc_fence_before();
     arrive_once(part == 0 ? early : ready);

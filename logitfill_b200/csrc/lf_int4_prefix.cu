@@ -15,7 +15,10 @@
 //
 // The product runs on tcgen05 with fp16 operands.  Codes become fp16 numbers code * s + z,
 // rounded once (2^-11); the queries of a row are scaled by a power of two, so that bf16 and
-// fp16 enter exactly.  A group whose numbers may pass the fp16 range (s 2^11 or |z| 2^15 at
+// fp16 enter exactly.  With an fp16 output, whose own rounding is as fine, Keys and weights
+// enter as sums of two fp16 numbers, in two products: error against 64 bits 0.00053 of the
+// result with one number each (0.0002 is the output's rounding alone), 0.00031 with two for
+// the Keys, 0.00028 with two for both.  A group whose numbers may pass the fp16 range (s 2^11 or |z| 2^15 at
 // least), or with a NaN, is not brought into it: the group of sequences is marked, and its
 // members read these pages themselves, in the suffix kernel, which can do that.
 //
@@ -124,12 +127,14 @@ template <int D> struct PrefixCfg {
   static constexpr int kSmem = 2 * kTile + kSlots * kTile + kStages * 2 * kRecord + 1024;  // (aligned by hand)
   static constexpr int kO = 256;                                // TMEM columns: scores of both tiles, then outputs
 };
-constexpr int kPrefixThreads = 768;
-// Registers a thread: 80 at launch, then split by what the warpgroups hold: 64 scores of a
-// row, four words and their parameters, counters.
-constexpr int kPrefixLaunchRegs = 80, kRowRegs = 96, kUnpackRegs = 64, kOtherRegs = 32;
-static_assert(512 * kRowRegs + 128 * (kUnpackRegs + kOtherRegs) <= kPrefixThreads * kPrefixLaunchRegs, "more registers than the block has");
-constexpr int kUnpackWarp = 16, kProductWarp = 20, kCopyWarp = 21;
+constexpr int kPrefixThreads = 896;
+// Registers a thread: 72 at launch, then split by what the warpgroups hold: 64 scores of a
+// row, a few words and their parameters, counters.
+constexpr int kPrefixLaunchRegs = 72, kRowRegs = 88, kUnpackRegs = 56, kOtherRegs = 32;
+constexpr int kUnpackWarps = 8;
+static_assert(512 * kRowRegs + 32 * kUnpackWarps * kUnpackRegs + 128 * kOtherRegs <= kPrefixThreads * kPrefixLaunchRegs,
+              "more registers than the block has");
+constexpr int kUnpackWarp = 16, kProductWarp = kUnpackWarp + kUnpackWarps, kCopyWarp = kProductWarp + 1;
 constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
 
 struct PrefixShared {
@@ -182,22 +187,62 @@ struct Walk {
   }
 };
 
+// fp16 numbers that make up a Key, and a weight.
+template <typename T> constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 1;
+
 __device__ __forceinline__ uint32_t hfma2_rn(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// The eight codes of a word times s2 plus z2 as fp16 pairs: codes (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t s2, uint32_t z2) {
-  uint32_t c[4];
+__device__ __forceinline__ uint32_t hadd2_rn(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hsub2_rn(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2_rn(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A word's eight codes as fp16 pairs: codes (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ void codes_of(uint32_t w, uint32_t (&c)[4]) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint32_t x = w >> (8 * k);
     const uint32_t even = (x & 0x000F000Fu) | 0x64006400u, odd = (x & 0x00F000F0u) | 0x64006400u;  // 1024 + code, 1024 + 16 code
-    c[2 * k] = hfma2_rn(even, 0x3C003C00u, 0xE400E400u);     // - 1024
+    c[2 * k] = hsub2_rn(even, 0x64006400u);
     c[2 * k + 1] = hfma2_rn(odd, 0x2C002C00u, 0xD400D400u);  // / 16 - 64
   }
+}
+// code * s2 + z2, rounded once.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t s2, uint32_t z2) {
+  uint32_t c[4];
+  codes_of(w, c);
   return make_uint4(hfma2_rn(c[0], s2, z2), hfma2_rn(c[1], s2, z2), hfma2_rn(c[2], s2, z2), hfma2_rn(c[3], s2, z2));
+}
+// The same as the sum of two fp16 numbers, of which this is the first (low: the second).
+// x = RN(code s) and r = code s - x, exact by an fma; a = RN(x + z) and what it leaves out,
+// exact by Knuth's two-sum; the second number is that and r, rounded.
+template <bool kLow> __device__ __forceinline__ uint4 unpack_word_exactly(uint32_t w, uint32_t s2, uint32_t z2) {
+  uint32_t c[4], y[4];
+  codes_of(w, c);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t x = hmul2_rn(c[k], s2), a = hadd2_rn(x, z2);
+    if constexpr (kLow) {
+      const uint32_t r = hfma2_rn(c[k], s2, x ^ 0x80008000u), b = hsub2_rn(a, x);
+      y[k] = hadd2_rn(hadd2_rn(hsub2_rn(x, hsub2_rn(a, b)), hsub2_rn(z2, b)), r);
+    } else {
+      y[k] = a;
+    }
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
 }
 // Non-zero in a sign's place where a scale is 2^11 at least, a minimum 2^15, or one is not finite.
 __device__ __forceinline__ uint32_t wide_bits(uint32_t sz) { return (sz & 0x7FFF7FFFu) + 0x08001800u; }
@@ -216,6 +261,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __grid_constant__ PrefixParams p) {
   using C = PrefixCfg<D>;
   constexpr int kSlots = C::kSlots, kStages = C::kStages, kG = D / kInt4Group;
+  constexpr int kLoads = kTerms<T> + 1;  // tiles of a step: the Key's terms, then Value
   extern __shared__ uint8_t dynamic[];
   __shared__ PrefixShared sh;
   const uint32_t pad = ((smem_u32(dynamic) + 1023u) & ~1023u) - smem_u32(dynamic);
@@ -230,12 +276,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&sh.kv_full[i], 4);
+      mbar_init(&sh.kv_full[i], kUnpackWarps);
       mbar_init(&sh.kv_empty[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.raw_full[i], 1);
-      mbar_init(&sh.raw_empty[i], 4);
+      mbar_init(&sh.raw_empty[i], kUnpackWarps);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_ready[t], 8);
@@ -294,7 +340,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       const uint32_t used = n / kStages + (static_cast<uint32_t>(i) < n % kStages ? 1 : 0);
       if (used != 0) mbar_wait_bounded(&sh.raw_full[i], (used - 1) & 1, kTileWaitNs);
     }
-  } else if (warp >= kUnpackWarp && warp < kUnpackWarp + 4) {
+  } else if (warp >= kUnpackWarp && warp < kUnpackWarp + kUnpackWarps) {
     // ---------------------------------------------------------------- pages to fp16 tiles
     fewer_registers<kUnpackRegs>();
     Walk walk(p.plan, p.pool.kv_heads, p.groups);
@@ -309,17 +355,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         const int stage = n % kStages, page = 2 * (piece.first + i);
         if (!(ok = wait(&sh.raw_full[stage], (n / kStages) & 1))) break;
 #pragma unroll 1
-        for (int value = 0; value < 2; ++value) {
-          const uint32_t load = 2 * n + value, slot = load % kSlots;
+        for (int kind = 0; kind < kLoads; ++kind) {  // the Key's terms, then Value
+          const bool value = kind == kLoads - 1;
+          const uint32_t load = kLoads * n + kind, slot = load % kSlots;
           if (load >= kSlots && !(ok = wait(&sh.kv_empty[slot], (load / kSlots - 1) & 1))) break;
           uint8_t* tile = ring + slot * C::kTile;
 #pragma unroll
-          for (int part = 0; part < 4; ++part) {
-            // 16 words' rows at a time: warp w and part give 8 tokens of a page
-            const int block = part * 4 + w, half = block >> 3, b = block & 7;  // half: which page; b: its 8 tokens
-            const uint8_t* rec = raw + (2 * stage + half) * C::kRecord + value * 40 * D;
+          for (int part = 0; part < 16 / kUnpackWarps; ++part) {
+            // 8 tokens of a page at a time
+            const int block = part * kUnpackWarps + w, half = block >> 3, b = block & 7;  // half: which page; b: its 8 tokens
+            const uint8_t* rec = raw + (2 * stage + half) * C::kRecord + (value ? 40 * D : 0);
             const bool there = page + half < pages;
-            if (value == 0) {
+            if (!value) {
               // Key: lane = (token, t), its kG words the groups' channels 8 t .. 8 t + 7.  Tokens x and
               // x + 4 in a quarter of the warp store to different banks.
               const int t = lane & 3, tok = 8 * b + ((lane >> 2) & 1) * 4 + (lane >> 3), row = half * 64 + tok;
@@ -330,7 +377,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
               for (int G = 0; G < kG; ++G) {
                 wide |= there ? wide_bits(sz[G]) : 0u;
                 const uint32_t s2 = __byte_perm(sz[G], 0, 0x1010), z2 = __byte_perm(sz[G], 0, 0x3232);
-                const uint4 x = there ? unpack_word(code[G], s2, z2) : make_uint4(0, 0, 0, 0);
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (there) {
+                  if constexpr (kLoads == 2)
+                    x = unpack_word(code[G], s2, z2);
+                  else
+                    x = kind == 0 ? unpack_word_exactly<false>(code[G], s2, z2) : unpack_word_exactly<true>(code[G], s2, z2);
+                }
                 const int chunk = 4 * (G & 1) + t;
                 *reinterpret_cast<uint4*>(tile + (G >> 1) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4)) = x;
               }
@@ -376,31 +429,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     bool had[2] = {false, false}, fresh = false, ends = false, ok = true;
     auto output = [&](int t) -> bool {  // of the step before
       if (!had[t]) return true;
-      const uint32_t load = 2 * step - 1, slot = load % kSlots;
+      const uint32_t load = kLoads * step - 1, slot = load % kSlots;
       if (!wait(&sh.kv_full[slot], (load / kSlots) & 1)) return false;
       for (int part = 0; part < 2; ++part) {
         if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
-        issue_outputs(tmem + C::kO + t * D, tmem + 128 * t, ring_a + slot * C::kTile, idesc_o, part, fresh, ends && part == 1 ? &sh.o_done[t] : nullptr);
+        issue_outputs<kTerms<T>>(tmem + C::kO + t * D, tmem + 128 * t, ring_a + slot * C::kTile, idesc_o, part, fresh, ends && part == 1 ? &sh.o_done[t] : nullptr);
       }
       ++made[t];
       return true;
     };
+    auto keys_there = [&]() -> bool {
+      for (uint32_t load = kLoads * step; load < kLoads * step + kLoads - 1; ++load)
+        if (!wait(&sh.kv_full[load % kSlots], (load / kSlots) & 1)) return false;
+      return true;
+    };
     auto scores = [&](int t) {
       tc_fence_after();
-      issue_scores<D>(tmem + 128 * t, smem_u32(queries) + t * C::kTile, ring_a + 2 * step % kSlots * C::kTile, idesc_s, &sh.s_full[t]);
+#pragma unroll
+      for (int x = 0; x < kLoads - 1; ++x)
+        issue_scores<D>(tmem + 128 * t, smem_u32(queries) + t * C::kTile, ring_a + (kLoads * step + x) % kSlots * C::kTile, idesc_s, x > 0,
+                        x == kLoads - 2 ? &sh.s_full[t] : nullptr);
     };
     while (ok && walk.next(piece)) {
       const bool two = piece.tile * kPrefixRows + 128 < walk.group.count * per_member;
       for (int i = 0; i < piece.n; ++i, ++step) {
         if (i == 0) {  // (new queries are made only after the outputs of the piece before)
           if (step > 0 && !(ok = output(0) && output(1))) break;
-          if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1) && wait(&sh.q_ready[0], asked[0]++ & 1))) break;
+          if (!(ok = keys_there() && wait(&sh.q_ready[0], asked[0]++ & 1))) break;
           scores(0);
           if (two && !(ok = wait(&sh.q_ready[1], asked[1]++ & 1))) break;
           if (two) scores(1);
         } else {
-          if (!(ok = wait(&sh.kv_full[2 * step % kSlots], (2 * step / kSlots) & 1))) break;
+          if (!(ok = keys_there())) break;
           if (!(ok = output(0))) break;
           scores(0);
           if (!(ok = output(1))) break;
@@ -492,11 +553,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         if (frees && (t == 1 || rows - piece.tile * kPrefixRows <= 128)) {
           // The step's last scores are done, and with them all products before: the Key tile
           // is free, and the Value tile of the step before.
-          const uint32_t load = 2 * (before + i);
-          arrive_once(&sh.kv_empty[load % kSlots]);
+          const uint32_t load = kLoads * (before + i);
+#pragma unroll
+          for (int x = 0; x < kLoads - 1; ++x) arrive_once(&sh.kv_empty[(load + x) % kSlots]);
           if (load > 0) arrive_once(&sh.kv_empty[(load - 1) % kSlots]);
         }
-        if (!(ok = soften_tile<__half, D, 0>(tm_s, tm_o, half, c, at + 128 > vis_min, vis - at, i == 0, st, pair, &sh.p_early[t], &sh.p_ready[t],
+        if (!(ok = soften_tile<__half, D, 0, kTerms<T>>(tm_s, tm_o, half, c, at + 128 > vis_min, vis - at, i == 0, st, pair, &sh.p_early[t], &sh.p_ready[t],
                                           wait, [] { return true; })))
           break;
       }

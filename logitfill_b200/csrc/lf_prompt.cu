@@ -327,14 +327,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int part = 0; part < 2; ++part) {
         if (!wait(part == 0 ? &sh.p_early[t] : &sh.p_ready[t], made[t] & 1)) return false;
         tc_fence_after();
-        issue_outputs(tmem + C::kO + t * D, tmem + 128 * t, ring + slot * C::kTile, idesc_o, part, fresh[t], ends && part == 1 ? &sh.o_done[t] : nullptr);
+        issue_outputs<1>(tmem + C::kO + t * D, tmem + 128 * t, ring + slot * C::kTile, idesc_o, part, fresh[t], ends && part == 1 ? &sh.o_done[t] : nullptr);
       }
       ++made[t];
       return true;
     };
     auto scores = [&](int t) {
       tc_fence_after();
-      issue_scores<D>(tmem + 128 * t, base + t * C::kTile, ring + 2 * step % kSlots * C::kTile, idesc_s, &sh.s_full[t]);
+      issue_scores<D>(tmem + 128 * t, base + t * C::kTile, ring + 2 * step % kSlots * C::kTile, idesc_s, false, &sh.s_full[t]);
     };
     PromptItem it;
     bool ok = true;
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (load > 0) arrive_once(&sh.kv_empty[(load - 1) % kSlots]);
             if (j == 0) arrive_once(&sh.q_empty);
           }
-          if (!(ok = soften_tile<T, D, kPolyPairs>(tm_s, tm_o, half, c, tile_masked(t0, j), sees - 128 * j, j == steps - 1, st, pair, &sh.p_early[t], &sh.p_ready[t], wait, [&] {
+          if (!(ok = soften_tile<T, D, kPolyPairs, 1>(tm_s, tm_o, half, c, tile_masked(t0, j), sees - 128 * j, j == steps - 1, st, pair, &sh.p_early[t], &sh.p_ready[t], wait, [&] {
                                          const uint32_t slot = (load + 1) % kSlots;
                                          if (!wait(&sh.kv_full[slot], ((load + 1) / kSlots) & 1)) return false;
                                          if (scan_value<T, D>(ring_ptr + slot * C::kTile, min(128, it.tokens - 128 * j))) sh.bad[n & 1] = 1;
