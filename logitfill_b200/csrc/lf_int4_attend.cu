@@ -279,27 +279,61 @@ __device__ __forceinline__ int shared_pages(const AttendParams& p, int b) {
   return g >= 0 && p.prefix.groups[g].live != 0 ? p.prefix.groups[g].pages : 0;
 }
 
-// Adds the shared pages' part of row r of a group (KV head h, channels d .. d + 3) to a
-// maximum, sum and accumulators.
-template <int D>
-__device__ __forceinline__ void add_shared(const PrefixPlan& plan, const PrefixGroup& g, int h, int r, int d, float& top, float& sum, float4& v) {
-  const int unit = h * g.tiles + r / kPrefixRows, in = r % kPrefixRows, per = plan.head[1];
-  const int start = g.places + unit * (g.steps + kPrefixCost) + kPrefixCost;
-  const int first = start / per, n = (start + g.steps - 1) / per - first + 1;
-  const float* rec = plan.records + (g.units + unit + first) * prefix_record(D) + in;
-  float now = top;
-#pragma unroll 4
-  for (int x = 0; x < n; ++x) now = fmaxf(now, rec[x * prefix_record(D)]);
-  const float fix = ex2(top - now);
-  sum *= fix;
-  v = make_float4(v.x * fix, v.y * fix, v.z * fix, v.w * fix);
-  top = now;
-#pragma unroll 4
-  for (int x = 0; x < n; ++x) {
-    const float* at = rec + x * prefix_record(D);
-    const float f = ex2(at[0] - now);
-    sum = fmaf(f, at[kPrefixRows], sum);
-    add_scaled(v, f, *reinterpret_cast<const float4*>(at - in + 2 * kPrefixRows + static_cast<int64_t>(in) * D + d));
+// Where the records of a unit's first column are.
+struct SharedRows {
+  const PrefixGroup* group;  // null: no shared pages
+  int row, h, per;
+};
+// Adds the shared pages' part of kItems rows (row[k] of the group, channels d[k] .. d[k] + 3)
+// to their maxima, sums and accumulators.
+template <int D, int kItems>
+__device__ __forceinline__ void add_shared(const PrefixPlan& plan, const SharedRows& where, const int (&row)[kItems], const int (&d)[kItems],
+                                           float (&top)[kItems], float (&sum)[kItems], float4 (&v)[kItems]) {
+  constexpr int kAhead = kItems <= 2 ? 4 : 2;  // parts whose loads wait for memory together, of all items
+  const PrefixGroup& g = *where.group;
+  const float* rec[kItems];
+  int n[kItems], most = 0;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int x = where.h * g.tiles + row[k] / kPrefixRows, start = g.start(x), first = start / where.per;
+    n[k] = (start + g.weight(x) * (g.steps - 1)) / where.per - first + 1;
+    most = max(most, n[k]);
+    rec[k] = plan.records + (g.units + x + first) * prefix_record(D) + row[k] % kPrefixRows;
+  }
+#pragma unroll 1
+  for (int x0 = 0; x0 < most; x0 += kAhead) {
+    float tops[kAhead][kItems], sums[kAhead][kItems];
+    float4 parts[kAhead][kItems];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x)
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        tops[x][k] = kNoMax;
+        sums[x][k] = 0.0f;
+        parts[x][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (x0 + x < n[k]) {
+          const float* at = rec[k] + (x0 + x) * prefix_record(D);
+          tops[x][k] = at[0];
+          sums[x][k] = at[kPrefixRows];
+          parts[x][k] = *reinterpret_cast<const float4*>(at + 2 * kPrefixRows + row[k] % kPrefixRows * static_cast<int64_t>(D - 1) + d[k]);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      float now = top[k];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) now = fmaxf(now, tops[x][k]);
+      const float fix = ex2(top[k] - now);
+      top[k] = now;
+      sum[k] *= fix;
+      v[k] = make_float4(v[k].x * fix, v[k].y * fix, v[k].z * fix, v[k].w * fix);
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const float f = ex2(tops[x][k] - now);
+        sum[k] = fmaf(f, sums[x][k], sum[k]);
+        add_scaled(v[k], f, parts[x][k]);
+      }
+    }
   }
 }
 
@@ -398,6 +432,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
   __shared__ int last_s;
   __shared__ Unit unit_s;
   __shared__ int vis_s[kWarps][kCol];  // tokens that each column sees
+  __shared__ SharedRows rows_s;
   __shared__ int apart_s[kWarps];       // a Value group stayed out of the product
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = p.pool.kv_heads * p.col_tiles;
@@ -592,6 +627,15 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
     }
     vis_min = __reduce_min_sync(0xffffffffu, vis_min);
 
+    if constexpr (kPrefix) {
+      if (tid == 0) {
+        rows_s.group = nullptr;
+        if (shared > 0) {
+          const PrefixSeq s = p.prefix.seqs[b];
+          rows_s = SharedRows{p.prefix.groups + s.group, s.rank * p.cols + c0, h, p.prefix.head[1]};
+        }
+      }
+    }
     if (tid == 0) unit_s = Unit{b, h, c0, i0, first, stop, length, count, seen_max, vis_min, listed, shared};
     if (lane == 0) apart_s[warp] = 0;
     float acc[NT][2 * kG][4], back[NT][2], l[NT][2];  // back: the running maxima, negated, times 2^-14
@@ -848,21 +892,27 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
       Scalar<T>::store(f.x + 3, v.w * inv);
       *reinterpret_cast<Four*>(o) = f;
     };
-    // What the shared pages gave, with a thread's share of the result in hand.
-    auto with_shared = [&](int col, int d, float& top, float& sum, float4& v) {
-      if constexpr (kPrefix) {
-        if (shared > 0 && c0 + col < p.cols) {
-          const PrefixSeq s = p.prefix.seqs[b];
-          add_shared<D>(p.prefix, p.prefix.groups[s.group], h, s.rank * p.cols + c0 + col, d, top, sum, v);
-        }
-      }
-    };
     // The partial of range x of this unit: the range that begins inside the unit
     // uses its CTA's first record, the unit's first range the second.
     const int first_cta = unit_begin / per, last_cta = (unit_end - 1) / per, parts = last_cta - first_cta + 1;
     auto record = [&](int x) { return p.partials + (2 * static_cast<int64_t>(x) + (x == first_cta)) * C::kRecord; };
     float* mine = record(blockIdx.x);
     constexpr int kItems = kCol * D / 4 / C::kThreads;  // (column, four channels) a thread merges
+    // The thread's items with what the shared pages gave, stored.
+    auto store_shared = [&](float (&top)[kItems], float (&sum)[kItems], float4 (&v)[kItems]) {
+      int row[kItems], d[kItems];
+#pragma unroll
+      for (int it = 0; it < kItems; ++it) {
+        const int item = tid + it * C::kThreads;
+        row[it] = rows_s.row + min(item / (D / 4), p.cols - 1 - c0);
+        d[it] = item % (D / 4) * 4;
+      }
+      if (rows_s.group != nullptr) add_shared<D>(p.prefix, rows_s, row, d, top, sum, v);
+#pragma unroll
+      for (int it = 0; it < kItems; ++it) store((tid + it * C::kThreads) / (D / 4), d[it], v[it], sum[it]);
+    };
+    float tops[kItems], sums[kItems];
+    float4 all[kItems];
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
       const int item = tid + it * C::kThreads, col = item / (D / 4), d = item % (D / 4) * 4;
@@ -877,8 +927,13 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
         add_scaled(v, f, *reinterpret_cast<const float4*>(merge + (w * kCol + col) * C::kPad + d));
       }
       if (whole) {
-        with_shared(col, d, top, sum, v);
-        store(col, d, v, sum);
+        if constexpr (kPrefix) {
+          tops[it] = top;
+          sums[it] = sum;
+          all[it] = v;
+        } else {
+          store(col, d, v, sum);
+        }
       } else {
         *reinterpret_cast<float4*>(mine + 2 * kCol + col * D + d) = v;
         if (d == 0) {
@@ -886,6 +941,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
           mine[kCol + col] = sum;
         }
       }
+    }
+    if constexpr (kPrefix) {
+      if (whole) store_shared(tops, sums, all);
     }
     if (!whole) {
       __syncthreads();
@@ -943,11 +1001,14 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kThreads, AttendCfg<D, NT>::
             }
           __syncthreads();
         }
+        if constexpr (kPrefix) {
+          store_shared(top, sum, v);
+        } else {
 #pragma unroll
-        for (int it = 0; it < kItems; ++it) {
-          const int item = tid + it * C::kThreads;
-          with_shared(item / (D / 4), item % (D / 4) * 4, top[it], sum[it], v[it]);
-          store(item / (D / 4), item % (D / 4) * 4, v[it], sum[it]);
+          for (int it = 0; it < kItems; ++it) {
+            const int item = tid + it * C::kThreads;
+            store(item / (D / 4), item % (D / 4) * 4, v[it], sum[it]);
+          }
         }
       }
     }

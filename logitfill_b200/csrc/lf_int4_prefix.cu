@@ -53,15 +53,18 @@ struct PrefixParams {
 
 constexpr int kMaxGroups = 4096;
 
-// Shared pages of group g that its `count` members read together.  One member with few
-// rows has nothing to share.
-__device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int count) {
+// Shared pages of group g that its `count` members (one of them `any`) read together.  One
+// member with few rows has nothing to share.
+__device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int count, int any) {
   if (count == 0 || (count == 1 && p.q_len * p.heads <= 16)) return 0;
+  // All pages of one member are its own: the complete ones (what a page's unwritten slots
+  // hold may not be read here) are read in this way, its queries' own tokens among them.
+  if (count == 1) return min(max(p.lengths[any], 0) / kInt4Page, p.pool.table_width);
   return min(max(p.shared[g], 0), p.pool.table_width);
 }
 
 __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_constant__ PrefixParams p) {
-  __shared__ int count_s[kMaxGroups], first_s[kMaxGroups];
+  __shared__ int count_s[kMaxGroups], first_s[kMaxGroups], any_s[kMaxGroups];
   const int lane = threadIdx.x;
   grid_dep_wait();
   for (int g = lane; g < p.groups; g += 32) count_s[g] = 0;
@@ -76,7 +79,10 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
     const int before = __popc(same & ((1u << lane) - 1u));
     const int rank = g >= 0 ? count_s[g] + before : -1;
     __syncwarp();
-    if (g >= 0 && before == 0) count_s[g] += __popc(same);
+    if (g >= 0 && before == 0) {
+      count_s[g] += __popc(same);
+      any_s[g] = b;
+    }
     __syncwarp();
     if (b < p.pool.batch) p.plan.seqs[b] = PrefixSeq{g, rank};
   }
@@ -85,9 +91,10 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane;
     const int count = g < p.groups ? count_s[g] : 0;
-    const int pages = g < p.groups ? group_pages(p, g, count) : 0;
+    const int pages = g < p.groups ? group_pages(p, g, count, any_s[g]) : 0;
     const int tiles = pages > 0 ? (count * p.q_len * p.heads + kPrefixRows - 1) / kPrefixRows : 0, steps = (pages + 1) / 2;
-    const int n_units = tiles * p.pool.kv_heads, n_places = n_units * (steps + kPrefixCost);
+    const int last = tiles > 0 && count * p.q_len * p.heads - (tiles - 1) * kPrefixRows <= kPrefixRows / 2 ? 1 : 2;
+    const int n_units = tiles * p.pool.kv_heads, n_places = tiles > 0 ? p.pool.kv_heads * prefix_head_places(tiles, steps, last) : 0;
     int m = count, u = n_units, x = n_places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -100,7 +107,7 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
     }
     if (g < p.groups) {
       first_s[g] = members + m - count;
-      p.plan.groups[g] = PrefixGroup{pages, pages > 0, members + m - count, count, units + u - n_units, places + x - n_places, tiles, steps};
+      p.plan.groups[g] = PrefixGroup{pages, pages > 0, members + m - count, count, units + u - n_units, places + x - n_places, tiles, steps, last, {}};
     }
     members += __shfl_sync(0xffffffffu, m, 31);
     units += __shfl_sync(0xffffffffu, u, 31);
@@ -113,19 +120,19 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
   }
   if (lane == 0) {
     p.plan.head[0] = places;
-    p.plan.head[1] = max(kPrefixCost + 1, (places + p.grid - 1) / p.grid);
+    p.plan.head[1] = max(2, (places + p.grid - 1) / p.grid);
   }
 }
 
 // ------------------------------------------------------------ shared pages
 
 template <int D> struct PrefixCfg {
-  static constexpr int kTile = 128 * D * 2;                     // bytes of 128 fp16 rows
-  static constexpr int kSlots = D == 128 ? 3 : 6;               // Key and Value tiles
-  static constexpr int kRecord = 20 * D * 4;                    // bytes of a page
-  static constexpr int kStages = D == 128 ? 3 : 6;              // pairs of pages as they are in the pool
-  static constexpr int kSmem = 2 * kTile + kSlots * kTile + kStages * 2 * kRecord + 1024;  // (aligned by hand)
-  static constexpr int kO = 256;                                // TMEM columns: scores of both tiles, then outputs
+  static constexpr int kTile = 128 * D * 2;        // bytes of 128 fp16 rows
+  static constexpr int kSlots = D == 128 ? 4 : 8;  // Key and Value tiles
+  static constexpr int kRaw = 40 * D;              // bytes of a page's Keys or Values: codes, then parameters
+  static constexpr int kStages = D == 128 ? 3 : 8;  // two pages' Keys or Values, as they are in the pool
+  static constexpr int kSmem = 2 * kTile + kSlots * kTile + kStages * 2 * kRaw + 3072;  // with what the roles share
+  static constexpr int kO = 256;                   // TMEM columns: scores of both tiles, then outputs
 };
 constexpr int kPrefixThreads = 896;
 // Registers a thread: 72 at launch, then split by what the warpgroups hold: 64 scores of a
@@ -134,11 +141,11 @@ constexpr int kPrefixLaunchRegs = 72, kRowRegs = 88, kUnpackRegs = 56, kOtherReg
 constexpr int kUnpackWarps = 8;
 static_assert(512 * kRowRegs + 32 * kUnpackWarps * kUnpackRegs + 128 * kOtherRegs <= kPrefixThreads * kPrefixLaunchRegs,
               "more registers than the block has");
-constexpr int kUnpackWarp = 16, kProductWarp = kUnpackWarp + kUnpackWarps, kCopyWarp = kProductWarp + 1;
+constexpr int kUnpackWarp = 16, kProductWarp = kUnpackWarp + kUnpackWarps, kCopyWarp = kProductWarp + 1, kCheckWarp = kProductWarp + 2;
 constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: below any score
 
 struct PrefixShared {
-  uint64_t raw_full[6], raw_empty[6], kv_full[6], kv_empty[6], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2], last;
+  uint64_t raw_full[8], raw_empty[8], kv_full[8], kv_empty[8], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2], last;
   int stop;
   uint32_t tmem;
   float told[2][2][128];  // between the two threads of a row
@@ -158,16 +165,15 @@ struct Walk {
     end = min(plan.head[0], at + per);
     group = PrefixGroup{};
   }
+  __device__ __forceinline__ int group_end(const PrefixGroup& y) const {
+    return y.tiles > 0 ? y.places + kv_heads * prefix_head_places(y.tiles, y.steps, y.last) : y.places;
+  }
+  // A step belongs to the range that its first place lies in.
   __device__ __forceinline__ bool next(Piece& piece) {
     while (at < end) {
-      while (g < 0 || at >= group.places + group.tiles * kv_heads * (group.steps + kPrefixCost)) {  // (places end behind `at`)
+      while (g < 0 || at >= group_end(group)) {
         const int x = g0 + (threadIdx.x & 31);
-        bool past = false;
-        if (x < groups) {
-          const PrefixGroup y = plan.groups[x];
-          past = at < y.places + y.tiles * kv_heads * (y.steps + kPrefixCost);
-        }
-        const uint32_t any = __ballot_sync(0xffffffffu, past);
+        const uint32_t any = __ballot_sync(0xffffffffu, x < groups && at < group_end(plan.groups[min(x, groups - 1)]));
         if (any != 0) {
           g = g0 + __ffs(any) - 1;
           group = plan.groups[g];
@@ -176,11 +182,13 @@ struct Walk {
           if (g0 >= groups) return false;
         }
       }
-      const int span = group.steps + kPrefixCost, x = (at - group.places) / span, start = group.places + x * span + kPrefixCost;
-      const int first = max(at, start), stop = min(end, start + group.steps);
-      at = max(stop, min(end, start));
+      const int per_head = prefix_head_places(group.tiles, group.steps, group.last), in = at - group.places, h = in / per_head;
+      const int tile = min((in - h * per_head) / (2 * group.steps + kPrefixCost), group.tiles - 1), x = h * group.tiles + tile;
+      const int w = group.weight(x), start = group.start(x), unit_end = start + w * group.steps;
+      const int first = (max(at, start) - start + w - 1) / w, stop = min(group.steps, max(0, end - start + w - 1) / w);
+      at = min(end, unit_end);
       if (first >= stop) continue;
-      piece = Piece{g, x / group.tiles, x % group.tiles, first - start, stop - first, group.units + x};
+      piece = Piece{g, h, tile, first, stop - first, group.units + x};
       return true;
     }
     return false;
@@ -262,12 +270,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   using C = PrefixCfg<D>;
   constexpr int kSlots = C::kSlots, kStages = C::kStages, kG = D / kInt4Group;
   constexpr int kLoads = kTerms<T> + 1;  // tiles of a step: the Key's terms, then Value
-  extern __shared__ uint8_t dynamic[];
-  __shared__ PrefixShared sh;
-  const uint32_t pad = ((smem_u32(dynamic) + 1023u) & ~1023u) - smem_u32(dynamic);
-  uint8_t* queries = dynamic + pad;
+  extern __shared__ __align__(1024) uint8_t dynamic[];
+  uint8_t* queries = dynamic;
   uint8_t* ring = queries + 2 * C::kTile;
   uint8_t* raw = ring + kSlots * C::kTile;
+  PrefixShared& sh = *reinterpret_cast<PrefixShared*>(raw + kStages * 2 * C::kRaw);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == kProductWarp) {
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.raw_full[i], 1);
-      mbar_init(&sh.raw_empty[i], kUnpackWarps);
+      mbar_init(&sh.raw_empty[i], kUnpackWarps + 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_ready[t], 8);
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       const int pages = walk.group.pages, leader = p.plan.members[walk.group.members];
       const int32_t* words = p.pool.words + piece.h * p.pool.head_stride;
       int ids = 0;
-      for (int i = 0; i < piece.n; ++i, ++n) {
+      for (int i = 0; i < piece.n; ++i) {
         const int page = 2 * (piece.first + i), two = page + 1 < pages ? 2 : 1;
         if ((i & 15) == 0) {  // the ids of 32 pages, one a lane
           ids = page + lane < pages ? int4_page_id(p.pool, leader, page + lane) : 0;
@@ -325,15 +332,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
             ids = 0;
           }
         }
-        const int stage = n % kStages;
-        if (n >= kStages && !(ok = wait(&sh.raw_empty[stage], (n / kStages - 1) & 1))) break;
         const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + 1);
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&sh.raw_full[stage], two * C::kRecord);
-          bulk_g2s(raw + stage * 2 * C::kRecord, words + id0 * p.pool.page_stride, C::kRecord, &sh.raw_full[stage]);
-          if (two == 2) bulk_g2s(raw + (2 * stage + 1) * C::kRecord, words + id1 * p.pool.page_stride, C::kRecord, &sh.raw_full[stage]);
+        for (int value = 0; ok && value < 2; ++value, ++n) {
+          const int stage = n % kStages;
+          if (n >= kStages && !(ok = wait(&sh.raw_empty[stage], (n / kStages - 1) & 1))) break;
+          if (elect_one()) {
+            const int32_t* from = words + value * 10 * D;
+            mbar_arrive_expect_tx(&sh.raw_full[stage], two * C::kRaw);
+            bulk_g2s(raw + stage * 2 * C::kRaw, from + id0 * p.pool.page_stride, C::kRaw, &sh.raw_full[stage]);
+            if (two == 2) bulk_g2s(raw + (2 * stage + 1) * C::kRaw, from + id1 * p.pool.page_stride, C::kRaw, &sh.raw_full[stage]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
       }
     }
     for (int i = 0; i < kStages; ++i) {  // no copy outlives the CTA
@@ -350,21 +361,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     const int w = warp - kUnpackWarp;
     while (ok && walk.next(piece)) {
       const int pages = walk.group.pages;
-      uint32_t wide = 0;
-      for (int i = 0; i < piece.n; ++i, ++n) {
-        const int stage = n % kStages, page = 2 * (piece.first + i);
-        if (!(ok = wait(&sh.raw_full[stage], (n / kStages) & 1))) break;
+      for (int i = 0; ok && i < piece.n; ++i, ++n) {
+        const int page = 2 * (piece.first + i);
 #pragma unroll 1
         for (int kind = 0; kind < kLoads; ++kind) {  // the Key's terms, then Value
           const bool value = kind == kLoads - 1;
-          const uint32_t load = kLoads * n + kind, slot = load % kSlots;
+          const uint32_t load = kLoads * n + kind, slot = load % kSlots, unit = 2 * n + value, stage = unit % kStages;
+          if (!(ok = wait(&sh.raw_full[stage], (unit / kStages) & 1))) break;
           if (load >= kSlots && !(ok = wait(&sh.kv_empty[slot], (load / kSlots - 1) & 1))) break;
           uint8_t* tile = ring + slot * C::kTile;
 #pragma unroll
           for (int part = 0; part < 16 / kUnpackWarps; ++part) {
             // 8 tokens of a page at a time
             const int block = part * kUnpackWarps + w, half = block >> 3, b = block & 7;  // half: which page; b: its 8 tokens
-            const uint8_t* rec = raw + (2 * stage + half) * C::kRecord + (value ? 40 * D : 0);
+            const uint8_t* rec = raw + (2 * stage + half) * C::kRaw;
             const bool there = page + half < pages;
             if (!value) {
               // Key: lane = (token, t), its kG words the groups' channels 8 t .. 8 t + 7.  Tokens x and
@@ -375,7 +385,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
               words_of<kG>(rec + 32 * D + tok * kG * 4, sz);
 #pragma unroll
               for (int G = 0; G < kG; ++G) {
-                wide |= there ? wide_bits(sz[G]) : 0u;
                 const uint32_t s2 = __byte_perm(sz[G], 0, 0x1010), z2 = __byte_perm(sz[G], 0, 0x3232);
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (there) {
@@ -388,8 +397,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
                 *reinterpret_cast<uint4*>(tile + (G >> 1) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4)) = x;
               }
             } else {
-              // Value: lane = (t, g), its words [token 2 t + o][w]: channels 64 w + 32 u + 4 g + n.
-              const int g = lane & 7, t = lane >> 3;
+              // Value: lane = (g, t), its words [token 2 t + o][w]: channels 64 w + 32 u + 4 g + n.
+              const int t = lane & 3, g = lane >> 2;
               uint32_t code[kG], sz[2][kG];
               words_of<kG>(rec + (b * D + g * (D / 8) + t * kG) * 4, code);
               words_of<kG>(rec + 32 * D + (8 * b + 2 * t) * kG * 4, sz[0]);
@@ -399,7 +408,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
 #pragma unroll
                 for (int x = 0; x < kG / 2; ++x) {
                   const uint32_t a = sz[o][2 * x], c = sz[o][2 * x + 1];
-                  wide |= there ? (wide_bits(a) | wide_bits(c)) : 0u;
                   const uint32_t s2 = __byte_perm(a, c, 0x5410), z2 = __byte_perm(a, c, 0x7632);
                   const int row = half * 64 + 8 * b + 2 * t + o;
                   const uint4 y = there ? unpack_word(code[o * (kG / 2) + x], s2, z2) : make_uint4(0, 0, 0, 0);
@@ -408,12 +416,32 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
             }
           }
           fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.kv_full[slot]);
+          arrive_once(&sh.kv_full[slot]);
+          if (kind >= kLoads - 2) arrive_once(&sh.raw_empty[stage]);  // the Key's last term, and Value
         }
-        if (!ok) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.raw_empty[stage]);
+      }
+    }
+  } else if (warp == kCheckWarp) {
+    // ---------------------------------------------------------------- parameters out of fp16's range
+    fewer_registers<kOtherRegs>();
+    Walk walk(p.plan, p.pool.kv_heads, p.groups);
+    Piece piece;
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && walk.next(piece)) {
+      uint32_t wide = 0;
+      for (int i = 0; ok && i < 2 * piece.n; ++i, ++n) {
+        const int stage = n % kStages, two = 2 * (piece.first + i / 2) + 1 < walk.group.pages ? 2 : 1;
+        if (!(ok = wait(&sh.raw_full[stage], (n / kStages) & 1))) break;
+        for (int half = 0; half < two; ++half) {
+          const uint4* at = reinterpret_cast<const uint4*>(raw + (2 * stage + half) * C::kRaw + 32 * D) + lane;
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            const uint4 y = at[32 * x];
+            wide |= wide_bits(y.x) | wide_bits(y.y) | wide_bits(y.z) | wide_bits(y.w);
+          }
+        }
+        arrive_once(&sh.raw_empty[stage]);
       }
       if ((wide & 0x80008000u) != 0) p.plan.groups[piece.g].live = 0;
     }
@@ -655,7 +683,7 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   p.status = q.status;
   const int sms = sm_count();
   const int64_t records = most_records(p.pool.batch, p.pool.kv_heads, p.heads, p.q_len, p.groups, sms);
-  const int64_t steps = (p.pool.table_width + 1) / 2 + kPrefixCost;
+  const int64_t steps = 2 * ((p.pool.table_width + 1) / 2) + kPrefixCost;
   LF_CHECK_SUPPORTED(records <= (1 << 30) / steps && static_cast<int64_t>(p.pool.batch) * p.q_len * p.heads <= (1 << 30),
                      "lf_int4_attend_prefix: %d sequences of %d pages are too many for one call", p.pool.batch, p.pool.table_width);
   LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
