@@ -188,10 +188,13 @@ template <typename T> constexpr float kLift = 0.0f;
 template <> constexpr float kLift<__half> = 7.0f;
 
 struct RowState {
-  float top;  // running maximum times c, -inf before any score
-  float sum;  // of the weights; NaN once a score was NaN or +inf
+  float top;   // running maximum of the scores times c, -inf before any
+  float sum;   // of the weights; NaN once a score was NaN or +inf
+  bool large;  // a maximum was so large that the rounding of its product with c reaches the exponent
   __device__ __forceinline__ bool empty() const { return top == -INFINITY && sum == sum; }  // nothing above -inf was seen
 };
+__device__ __forceinline__ RowState no_scores() { return RowState{-INFINITY, 0.0f, false}; }
+constexpr float kLargeTop = 1024.0f;  // 2^-14 of an exponent is lost from here on
 
 __device__ __forceinline__ float max_nan2(float a, float b) {
   float r;
@@ -260,11 +263,11 @@ __device__ __forceinline__ float move_top(float most, float c, RowState& st) {
     fix = ex2(st.top - now);
     st.top = now;
     st.sum *= fix;
+    st.large |= fabsf(now) >= kLargeTop && now < INFINITY;
   }
   if (!(now < INFINITY)) st.sum = NAN;  // a score that is NaN or +inf makes the row's result NaN
   return fix;
 }
-
 // 2^x for x >= -126 without the special function unit: x = n + r with |r| <= 1/2 (the
 // nearest whole number by adding 1.5 * 2^23), 2^r by its minimax polynomial (relative
 // error; found with Remez' algorithm), n added to the exponent.  Within 7.5e-5 (degree 3)
@@ -296,8 +299,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // unit gives 16 results a cycle, as long as the tensor core takes for both products of them.
 template <typename T, int kPoly, int kTerms>
 __device__ __forceinline__ void row_weights(uint32_t tmem_p, const float* s, float c, RowState& st) {
-  // The product of maximum and c is rounded once, and taken as it is everywhere: it
-  // cancels in the quotient of output and sum.
+  // The product of maximum and c is rounded once, and taken as it is everywhere: it cancels
+  // in the quotient of output and sum.  (Rows of RowState::large are done again elsewhere.)
   const float base = kLift<T> - (st.top == -INFINITY ? 0.0f : st.top);
   float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll

@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       if (lane == 0) mbar_arrive(&sh.q_ready[t]);
       const int vis_min = __reduce_min_sync(0xffffffffu, vis);
       // ---- its steps
-      RowState st = {-INFINITY, 0.0f};
+      RowState st = no_scores();
       for (int i = 0; i < piece.n; ++i, ++count) {
         const int at = (piece.first + i) * 128;
         if (!(ok = wait(&sh.s_full[t], count & 1))) break;
@@ -590,6 +590,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
                                           wait, [] { return true; })))
           break;
       }
+      if (__any_sync(0xffffffffu, st.large && row < rows) && lane == 0) p.plan.groups[piece.g].live = 0;
       if (!ok || !(ok = join_sums(st, pair, wait))) break;
       if (!(ok = wait(&sh.o_done[t], pieces++ & 1))) break;
       tc_fence_after();

@@ -34,6 +34,8 @@ template <typename T, int D>
 __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok, const T* v, int64_t v_tok, int n, float scale_log2, T* out) {
   constexpr int kOwn = D / 32, kAhead = 4;
   const int d = (threadIdx.x & 31) * kOwn;
+  // positive, so that -inf stays one; the difference to the maximum before the product
+  const float c = fmaxf(fabsf(scale_log2), 1e-36f), sign = scale_log2 < 0.0f ? -1.0f : 1.0f;
   float qx[kOwn], acc[kOwn], top = -INFINITY, sum = 0.0f;
 #pragma unroll
   for (int x = 0; x < kOwn; ++x) {
@@ -56,10 +58,10 @@ __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok
     float now = top;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      s[u] *= scale_log2;
+      s[u] *= sign;
       if (j + u < n) now = fmaxf(now, s[u]);
     }
-    const float base = now == -INFINITY ? 0.0f : now, fix = exp2f(top - base);
+    const float base = now == -INFINITY ? 0.0f : now, fix = exp2f((top - base) * c);
     sum *= fix;
 #pragma unroll
     for (int x = 0; x < kOwn; ++x) acc[x] *= fix;
@@ -67,7 +69,7 @@ __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (j + u >= n) break;
-      const float w = exp2f(s[u] - base);
+      const float w = exp2f((s[u] - base) * c);
       sum += w;
       const T* row = v + (j + u) * v_tok + d;
 #pragma unroll
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       volatile const PromptItem& it = sh.item[n & 1];  // (read where it is needed: registers are short here)
       if (it.b < 0) break;
       const int steps = it.n[t], all = max(it.n[0], it.n[1]), t0 = it.tok + t * per_tile;
-      RowState st = {-INFINITY, 0.0f};
+      RowState st = no_scores();
       {
         const int sees = min(t0 + r / p.group + 1, it.tokens);
         for (int j = steps - 1; j >= 0; --j, ++count) {
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!(ok = wait(&sh.o_done[t], items++ & 1))) break;
         tc_fence_after();
       }
-      if (steps > 0 && *const_cast<volatile int*>(&sh.bad[n & 1]) != 0) {
+      if (steps > 0 && (*const_cast<volatile int*>(&sh.bad[n & 1]) != 0 || __any_sync(0xffffffffu, st.large && stored && token < it.tokens))) {
         const T* k = static_cast<const T*>(p.k) + it.b * p.k_seq + it.first * p.k_tok + it.h * p.k_head;
         const T* v = static_cast<const T*>(p.v) + it.b * p.v_seq + it.first * p.v_tok + it.h * p.v_head;
         for (int i = half; i < 32; i += 2) {

@@ -217,6 +217,40 @@ def test_queries_of_any_size(size):
     batch.check(batch.run(q, 0.09 / size), q, 0.09 / size)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, BF16)])
+def test_scores_that_are_all_far_below_zero(D, dtype):
+    """Every score far below zero, down to -1e34: the nearest to zero takes all the weight, wherever it lies."""
+    batch = Batch(21, [0] * 4, [7], [70, 1, 64, 300], 1, D, dtype)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for table, start, tokens in ([batch.table[:1], 0, 448], *[(batch.table[b:b + 1], 448, t) for b, t in enumerate([70, 1, 64, 300])]):
+        key, value = torch.rand(1, 1, tokens, D, generator=g, device="cuda") + 0.5, torch.randn(1, 1, tokens, D, generator=g, device="cuda")
+        int4.int4_write(key, value, batch.pages, table, _i32([start]))
+    for size in ((1e3, 6e4) if dtype == F16 else (1e3, 1e9, 2.0 ** 110)):
+        q = (-(torch.rand(4, 6, 1, D, generator=g, device="cuda") + 0.5) * size).to(dtype)
+        got = batch.run(q, 0.125)
+        k, v = batch.values()
+        for b in range(4):
+            n = batch.lengths[b]
+            logits = q[b, :, 0].double() @ k[b, 0, :n].T * 0.125
+            best = logits.topk(2, -1)
+            # a score is off by its Keys' rounding (bf16 queries: 2^-11) and its fp32 sums
+            e = (q[b, :, 0].double().abs() @ k[b, 0, :n].abs().T).amax(-1) * 0.125 * (2.0 ** -11 + 128 * 2.0 ** -24)
+            sure = best.values[:, 0] - best.values[:, 1] > 30 + 2 * e
+            want = v[b, 0][best.indices[:, 0]]
+            off = (got[b, :, 0].double() - want).abs()
+            # weight and Value rounded to fp16, the output to its type
+            fine = torch.isfinite(q[b, :, 0]).all(-1)         # (fp16 ends at 65504: some queries of 6e4 * 1.5 are infinite)
+            assert bool((off <= (HALF_STEP[dtype] + 2.0 ** -10 + 2.0 ** -12) * want.abs() + 2.0 ** -20)[sure & fine].all())
+            assert bool(torch.isfinite(got[b, fine]).all())
+            # and no result leaves what the Values near the best span
+            near = logits >= (best.values[:, :1] - 40 - 2 * e.view(-1, 1))
+            for h in fine.nonzero()[:, 0].tolist():
+                span = v[b, 0, :n][near[h]]
+                low, high = span.amin(0), span.amax(0)
+                slack = 2.0 ** -7 * torch.maximum(low.abs(), high.abs()) + 2.0 ** -8
+                assert bool(((got[b, h, 0].double() >= low - slack) & (got[b, h, 0].double() <= high + slack)).all())
+
+
 def test_non_finite_queries_stay_in_their_rows():
     batch = Batch(15, [0] * 4, [5], [70, 1, 64, 8], 2, 64, F16)
     q = batch.query(13, 6, 1)

@@ -386,6 +386,32 @@ def test_scalings_of_any_sign_and_size(scaling, dtype):
             at += c
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("size", [3e2, 1e4, 2.0 ** 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_magnitude(dtype, D, size, sign):
+    """Scores up to 1e5 and 1e19, all above or all below zero, over several tiles: a weight is what the difference
+    of two scores says.  Keys are whole multiples of one direction, so that the scores are exact in fp32."""
+    n = 600
+    g = torch.Generator(device="cuda").manual_seed(7)
+    step = torch.randint(1, 60, (n, 1, 1), generator=g, device="cuda").float()
+    k = (step * torch.ones(n, 1, D, device="cuda")).to(dtype)
+    q = torch.full((n, 3, D), float(sign), dtype=dtype, device="cuda")
+    v = torch.randn(n, 1, D, generator=g, device="cuda").to(dtype)
+    scaling = size / 60 / D
+    got = prompt.prompt_attention(q, k, v, scaling)
+    # exact scores D * step * sign, whole numbers: the only error is fp32's in the difference's product with the scaling
+    logits = (sign * D * step[:, 0, 0].double() * float(torch.tensor(scaling, dtype=torch.float32))).view(1, n).expand(n, n)
+    p = torch.softmax(logits.masked_fill(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf), -1)
+    vv, u = v[:, 0].double(), HALF_STEP[dtype]
+    want = p @ vv
+    # in an exponent of size x (at most 25 where a weight counts) 3 roundings of 2^-24 x; kLargeTop 2^10 leaves 2^-14
+    bound = u * want.abs() + (u + 2.0 ** -13) * (p @ vv.abs()) + 2.0 ** -24
+    for h in range(3):
+        off = (got[:, h].double() - want).abs() - bound
+        assert bool((off <= 0).all()), float(off.max())
+
+
 def test_a_dominant_token_keeps_the_others():
     """An attention sink with a small Value, others 10 to 16 below it: in fp16 weights their share would drop out
     if the largest weight stood at 1."""
