@@ -21,7 +21,8 @@ EXPORTS = (
     "lf_decode", "lf_decode_multi", "lf_decode_max_splits_multi", "lf_commit_token", "lf_selftest_wait", "lf_selftest_divide",
     "lf_ipc_alloc", "lf_ipc_free", "lf_ipc_handle", "lf_ipc_open", "lf_ipc_close", "lf_decode_merge_gather",
     "lf_gather_signals", "lf_gather_wait", "lf_int4_write", "lf_int4_read", "lf_int4_read_bounds", "lf_int4_select",
-    "lf_int4_attend", "lf_int4_attend_sparse", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from", "lf_status_string", "lf_last_error",
+    "lf_int4_attend", "lf_int4_attend_sparse", "lf_int4_attend_prefix", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from",
+    "lf_int4_prefix_workspace_bytes", "lf_rotary_embed", "lf_prompt_attend", "lf_status_string", "lf_last_error",
 )
 
 

@@ -24,6 +24,11 @@ Differences from the reference, each deliberate:
 * A decode step whose cache reports a length other than the packed history's
   raises ``ValueError`` instead of running with wrong rotary positions; pass
   ``past_key_values=adapter.make_cache()``.
+* ``prompt="kernel"`` runs the first prefill of a sequence with
+  :func:`logitfill_b200.prompt.prompt_attention` instead of the model's own
+  attention (``"dense"``, the default): causal attention of an unpadded prompt,
+  fp16 or bf16, head_dim 64 or 128; an attention mask, a sliding window, dropout
+  or a gradient raises.
 * ``backend="fake"`` (fake quantization in the dense cache, the reference's
   correctness path) is not part of this package and raises
   ``NotImplementedError``; ``backend="packed"`` is the default here.
@@ -49,6 +54,16 @@ def _head_dim(config) -> int:
     return int(getattr(config, "head_dim", None) or config.hidden_size // n_q)
 
 
+def _sliding_window(attn):
+    window = getattr(attn, "sliding_window", None)
+    if window is None:
+        cfg = attn.config
+        if (getattr(cfg, "use_sliding_window", False) and getattr(cfg, "sliding_window", None) is not None
+                and attn.layer_idx >= getattr(cfg, "max_window_layers", 0)):
+            window = cfg.sliding_window
+    return window
+
+
 def _dense_attention(attn, query, key, value, attention_mask, kwargs):
     """The model's configured attention implementation (sdpa, eager, ...)
     on ``[B, heads, T, D]`` states; returns ``[B, q_len, heads, D]``
@@ -63,12 +78,7 @@ def _dense_attention(attn, query, key, value, attention_mask, kwargs):
         fn = ALL_ATTENTION_FUNCTIONS.get_interface(impl, eager_attention_forward)
     else:
         fn = ALL_ATTENTION_FUNCTIONS.get(impl, eager_attention_forward)
-    window = getattr(attn, "sliding_window", None)
-    if window is None:
-        cfg = attn.config
-        if (getattr(cfg, "use_sliding_window", False) and getattr(cfg, "sliding_window", None) is not None
-                and attn.layer_idx >= getattr(cfg, "max_window_layers", 0)):
-            window = cfg.sliding_window
+    window = _sliding_window(attn)
     out, _ = fn(attn, query, key, value, attention_mask,
                 dropout=0.0 if not attn.training else attn.attention_dropout,
                 scaling=attn.scaling, sliding_window=window, **kwargs)
@@ -119,6 +129,18 @@ def _make_forward(adapter: "DeepSeekQwenKVAdapter", layer_idx: int):
     return forward
 
 
+def _prompt_attention(attn, query, key, value, attention_mask, kwargs):
+    """The first prefill by the prompt kernel; returns ``[B, q_len, heads, D]``."""
+    from logitfill_b200.prompt import prompt_attention
+
+    if attention_mask is not None:
+        raise NotImplementedError("prompt='kernel' takes unpadded prompts without an attention mask "
+                                  "(attn_implementation='sdpa' builds none for them)")
+    if _sliding_window(attn) is not None or (attn.training and attn.attention_dropout):
+        raise NotImplementedError("prompt='kernel' has neither a sliding window nor dropout")
+    return prompt_attention(query, key, value, attn.scaling).transpose(1, 2)
+
+
 def _packed_branch(attn, adapter, layer_idx, query, key, value, attention_mask, cache, kwargs):
     """qwen2_attention.py:223-256."""
     manager = adapter.packed_manager()
@@ -126,7 +148,8 @@ def _packed_branch(attn, adapter, layer_idx, query, key, value, attention_mask, 
     if past == 0 and layer_idx == 0:
         manager.reset()
     if past == 0:
-        out = _dense_attention(attn, query, key, value, attention_mask, kwargs)
+        first = _prompt_attention if adapter.prompt == "kernel" else _dense_attention
+        out = first(attn, query, key, value, attention_mask, kwargs)
     else:
         if layer_idx == 0 and cache is not None and not isinstance(cache, LogitFillCache):
             seen = int(cache.get_seq_length()) if hasattr(cache, "get_seq_length") else -1
@@ -151,7 +174,8 @@ class DeepSeekQwenKVAdapter:
     (deepseek_qwen.py:21-149)."""
 
     def __init__(self, model: nn.Module, group_size: int = 128, page_size: Optional[int] = None,
-                 v_group_size: Optional[int] = None, bit_v: int = 2, backend: str = "packed"):
+                 v_group_size: Optional[int] = None, bit_v: int = 2, backend: str = "packed",
+                 prompt: str = "dense"):
         if model.__class__.__name__ != "Qwen2ForCausalLM":
             raise TypeError(f"DeepSeek-R1-Distill-Qwen-7B is Qwen2ForCausalLM, got {model.__class__.__name__}")
         if group_size < 1:
@@ -160,6 +184,9 @@ class DeepSeekQwenKVAdapter:
             raise ValueError(f"backend must be fake or packed, got {backend}")
         if backend == "fake":
             raise NotImplementedError("this package implements backend='packed' only")
+        if prompt not in ("dense", "kernel"):
+            raise ValueError(f"prompt must be dense or kernel, got {prompt}")
+        self.prompt = prompt
         self.model = model
         self.group_size = int(group_size)
         self.page_size = self.group_size if page_size is None else int(page_size)

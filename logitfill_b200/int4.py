@@ -35,6 +35,7 @@ import numpy as np
 import torch
 
 from logitfill_b200 import _lib
+from logitfill_b200.prompt import rotary_embed
 
 PAGE_TOKENS = 64   # tokens of a page
 GROUP = 32         # channels that share a scale and a minimum
@@ -151,7 +152,9 @@ class Int4KVCache:
     value)`` and ``attend(layer, query, scaling)``: ``extend`` makes room for
     the step's tokens, ``write`` stores them behind the tokens of the steps
     before, ``attend`` sees both.  Pages come from a free list and go back with
-    ``release``.
+    ``release``.  ``rotate`` turns a step's queries and Keys to their positions;
+    ``share`` gives a sequence's complete pages to others that begin as it does,
+    and ``attend_shared`` reads such pages once for all of them.
 
     Capturing a step in a CUDA graph: ``reserve`` pages for all tokens to come,
     capture ``extend(n)`` (an int) with the rest of the step, and call
@@ -184,6 +187,9 @@ class Int4KVCache:
         self._start = np.zeros(batch, np.int64)
         self._step = 0                                            # tokens of the step, at most
         self._free = list(range(n_pages - 1, -1, -1))
+        self._refs = np.zeros(n_pages, np.int64)                  # sequences that hold each page
+        self.prefix_group = torch.arange(batch, dtype=torch.int32, device=self.device)   # for int4_prefix_attention
+        self.prefix_pages = torch.zeros(batch, dtype=torch.int32, device=self.device)
 
     @property
     def n_layers(self) -> int:
@@ -214,7 +220,8 @@ class Int4KVCache:
             raise RuntimeError(f"{int(need.sum())} pages are needed, {len(self._free)} are free")
         for b in np.flatnonzero(need):
             for j in range(int(self._owned[b]), int(want[b])):
-                self._table[b, j] = self._free.pop()
+                self._table[b, j] = page = self._free.pop()
+                self._refs[page] = 1
             self._owned[b] = want[b]
         self._upload(self.page_table, self._table)
 
@@ -253,20 +260,74 @@ class Int4KVCache:
         n = np.broadcast_to(np.asarray(lengths, np.int64), (self.batch,))
         if (n < 0).any() or (n > self._end).any():
             raise ValueError("truncate() takes lengths between 0 and the present ones")
+        for b in range(self.batch):   # what comes next would be written over these
+            if (self._refs[self._table[b, int(n[b]) // PAGE_TOKENS:int(self._owned[b])]] > 1).any():
+                raise ValueError(f"sequence {b} shares pages past token {int(n[b])}")
         self._start, self._end, self._step = n.copy(), n.copy(), 0
         self._upload(self._spans, np.stack([self._start, self._end, np.zeros_like(n)]))
 
     def release(self, seqs=None) -> None:
-        """Empty the sequences ``seqs`` (default: all) and return their pages."""
+        """Empty the sequences ``seqs`` (default: all) and return the pages that no
+        other sequence shares."""
         every = range(self.batch)
         for b in every if seqs is None else [every[s] for s in seqs]:   # all are looked up before the first is emptied
             for j in range(int(self._owned[b]) - 1, -1, -1):
-                self._free.append(int(self._table[b, j]))
+                page = int(self._table[b, j])
+                self._refs[page] -= 1
+                if self._refs[page] == 0:
+                    self._free.append(page)
             self._table[b, :] = -1
             self._owned[b] = self._start[b] = self._end[b] = 0
         self._step = int((self._end - self._start).max())
         self._upload(self.page_table, self._table)
         self._upload(self._spans, np.stack([self._start, self._end, self._end - self._start]))
+        self._regroup()
+
+    def share(self, source: int, seqs, tokens: int | None = None) -> int:
+        """Let the empty sequences ``seqs`` begin with the first ``tokens`` tokens of
+        ``source`` (default: all it has), in whole pages: they hold the same pages,
+        which are written no more.  Returns the tokens that are shared; the others
+        go on behind them.  The pages' tokens must have been written, or be written
+        on this stream before they are read."""
+        every = range(self.batch)
+        source, seqs = every[source], [every[s] for s in seqs]
+        if len(set(seqs)) < len(seqs) or source in seqs:
+            raise ValueError("a sequence is named twice")
+        if any(self._owned[b] or self._end[b] for b in seqs):
+            raise ValueError("sequences that begin with shared pages must be empty (release them first)")
+        have = int(self._end[source])
+        tokens = have if tokens is None else int(tokens)
+        if tokens < 0 or tokens > have:
+            raise ValueError(f"sequence {source} has {have} tokens, {tokens} were to be shared")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("share the pages before the capture")
+        n = tokens // PAGE_TOKENS
+        for b in seqs:
+            self._table[b, :n] = self._table[source, :n]
+            self._refs[self._table[source, :n]] += 1
+            self._owned[b] = n
+            self._start[b] = self._end[b] = n * PAGE_TOKENS
+        self._upload(self.page_table, self._table)
+        self._upload(self._spans, np.stack([self._start, self._end, self._end - self._start]))
+        self._regroup()
+        return n * PAGE_TOKENS
+
+    def _regroup(self) -> None:
+        """Sequences that begin with the same page are one group, named by its lowest;
+        the pages that all of it have in common are read once."""
+        group, pages, leader = np.arange(self.batch), np.zeros(self.batch, np.int64), {}
+        for b in range(self.batch):
+            first = int(self._table[b, 0])
+            if first < 0 or self._refs[first] < 2:
+                continue
+            a = leader.setdefault(first, b)
+            group[b] = a
+            same = int(min(self._owned[a], self._owned[b])) if a != b else int(self._owned[b])
+            differs = np.flatnonzero(self._table[a, :same] != self._table[b, :same])
+            same = int(differs[0]) if len(differs) else same
+            pages[a] = same if a == b else min(int(pages[a]), same)
+        self._upload(self.prefix_group, group)
+        self._upload(self.prefix_pages, pages)
 
     def write(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store this step's tokens of one layer: ``[batch, n_kv, T, head_dim]``,
@@ -292,6 +353,20 @@ class Int4KVCache:
         ``counts[b]`` of sequence ``b``; all of the step's)."""
         self._check_query(query)
         return int4_attention(query, self.pages[layer], self.page_table, self.end, scaling, self.counts, out, self.status)
+
+    def rotate(self, query: torch.Tensor, key: torch.Tensor | None, freqs: torch.Tensor, magnitude: float = 1.0,
+               interleaved: bool = False, out: tuple | None = None):
+        """:func:`logitfill_b200.prompt.rotary_embed` of this step's queries and Keys, ``[batch,
+        heads, T, head_dim]``, to their positions in the sequences (read on the GPU)."""
+        return rotary_embed(query, key, freqs, start=self.start, magnitude=magnitude, interleaved=interleaved, out=out)
+
+    def attend_shared(self, layer: int, query: torch.Tensor, scaling: float, out: torch.Tensor | None = None) -> torch.Tensor:
+        """:meth:`attend` by way of :func:`int4_prefix_attention`: pages that sequences
+        share are read once for all of them.  (For a chunk of a prompt, many query
+        tokens of one sequence, its own pages are read once for all of those.)"""
+        self._check_query(query)
+        return int4_prefix_attention(query, self.pages[layer], self.page_table, self.end, scaling, self.prefix_group,
+                                     self.prefix_pages, self.counts, out, self.status)
 
     def attend_sparse(self, layer: int, query: torch.Tensor, scaling: float, top_pages: int, sink_pages: int = 1,
                       recent_pages: int = 2, out: torch.Tensor | None = None):

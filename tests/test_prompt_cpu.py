@@ -1,0 +1,261 @@
+"""CPU tests of a prompt's operators and of shared prefixes: refusals before any
+launch, the frequency tables, the cache's bookkeeping of shared pages."""
+from __future__ import annotations
+
+import math
+import re
+import struct
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from logitfill_b200 import _lib, int4, prompt
+from logitfill_b200.adapter import DeepSeekQwenKVAdapter
+from tests.qwen_cases import tiny_qwen2
+from tests.test_int4_cpu import QUERY, _query
+
+HEADER = (Path(__file__).resolve().parents[1] / "include" / "logitfill_b200.h").read_text()
+INVALID, UNSUPPORTED, OK = _lib.LF_ERR_INVALID_ARGUMENT, _lib.LF_ERR_UNSUPPORTED, _lib.LF_OK
+FAKE = 1 << 20   # never dereferenced: validation fails first
+
+ROTARY = struct.Struct("@4P12qPP2qPf10i0q")
+PROMPT = struct.Struct("@4P12q3Pf6i0q")
+
+
+def _fields(name):
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), HEADER, re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    out = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        kind, names = re.match(r"(?:const )?([\w]+\s*\*?)\s*(.*)", decl, re.S).groups()
+        out += [(kind.replace(" ", ""), n.strip()) for n in names.split(",")]
+    return out
+
+
+@pytest.mark.parametrize("name,packed", [("lf_rotary", ROTARY), ("lf_prompt", PROMPT)])
+def test_packed_structs_follow_the_header(name, packed):
+    code = {"void*": "P", "int32_t*": "P", "int64_t*": "P", "int64_t": "q", "int32_t": "i", "float": "f"}
+    spelled = re.sub(r"(\d+)([a-zA-Z])", lambda m: int(m.group(1)) * m.group(2), packed.format.lstrip("@"))
+    assert spelled == "".join(code[k] for k, _ in _fields(name))
+
+
+def _rotary(**over):
+    f = dict(q=FAKE, q_out=FAKE, k=FAKE, k_out=FAKE, strides=(512, 64, 1024) * 4, freqs=FAKE, positions=FAKE, ps=0, pt=1, start=0,
+             magnitude=1.0, p64=1, dtype=_lib.LF_BF16, head_dim=64, part=64, interleaved=0, transposed=0, batch=1, tokens=4, n_q=8, n_kv=2)
+    f.update(over)
+    flat = []
+    for v in f.values():
+        flat += list(v) if isinstance(v, tuple) else [v]
+    return ROTARY.pack(*flat)
+
+
+def _prompt(**over):
+    f = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, strides=(0, 64, 512, 0, 64, 128, 0, 64, 128, 0, 64, 512), starts=FAKE, counts=0, status=0,
+             scaling=0.125, head_dim=64, dtype=_lib.LF_BF16, batch=2, tokens=9, n_q=8, n_kv=2)
+    f.update(over)
+    flat = []
+    for v in f.values():
+        flat += list(v) if isinstance(v, tuple) else [v]
+    return PROMPT.pack(*flat)
+
+
+def test_rotary_validates_before_launch():
+    f = _lib.lib().lf_rotary_embed
+    assert f(None, None) == INVALID
+    assert f(_rotary(tokens=0), None) == OK and f(_rotary(batch=0), None) == OK and f(_rotary(n_q=0, n_kv=0), None) == OK
+    for bad in (dict(q=0), dict(q_out=0), dict(k=0), dict(freqs=0), dict(positions=0), dict(part=0), dict(part=63), dict(part=66),
+                dict(tokens=-1), dict(n_q=-1), dict(dtype=5), dict(magnitude=math.nan), dict(magnitude=math.inf)):
+        assert f(_rotary(**bad), None) == INVALID, bad
+    for much in (dict(head_dim=258), dict(head_dim=0, part=2), dict(n_q=70000), dict(batch=1 << 30, tokens=1 << 30)):
+        assert f(_rotary(**much), None) == UNSUPPORTED, much
+
+
+def test_prompt_attention_validates_before_launch():
+    f = _lib.lib().lf_prompt_attend
+    assert f(None, None) == INVALID
+    assert f(_prompt(tokens=0), None) == OK and f(_prompt(batch=0), None) == OK
+    for bad in (dict(q=0), dict(out=0), dict(q=FAKE + 8), dict(n_q=7), dict(n_kv=0), dict(tokens=-1), dict(scaling=math.inf),
+                dict(scaling=3.2e38), dict(strides=(0, 60, 512, 0, 64, 128, 0, 64, 128, 0, 64, 512)),
+                dict(strides=(0, 64, 512, 0, 64, 0, 0, 64, 128, 0, 64, 512)), dict(strides=(0, 64, -512, 0, 64, 128, 0, 64, 128, 0, 64, 512)),
+                dict(starts=0)):   # (a padded batch without a sequence stride)
+        assert f(_prompt(**bad), None) == INVALID, bad
+    for much in (dict(head_dim=96), dict(dtype=_lib.LF_F32), dict(n_q=258), dict(n_q=65536, n_kv=65536)):
+        assert f(_prompt(**much), None) == UNSUPPORTED, much
+    assert b"lf_prompt_attend" in _lib.lib().lf_last_error()
+
+
+def _prefix(query=None, **over):
+    f = dict(group=FAKE, shared=FAKE, ws=FAKE, ws_bytes=1 << 40, groups=2)
+    f.update(over)
+    return _query(**dict(dict(picked=0), **(query or {}))) + struct.pack("@PPPNi0q", *f.values())
+
+
+def test_prefix_attention_validates_before_launch():
+    assert QUERY.size % 8 == 0
+    f = _lib.lib().lf_int4_attend_prefix
+    assert f(None, None) == INVALID
+    for bad in (dict(group=0), dict(shared=0), dict(groups=-1)):
+        assert f(_prefix(**bad), None) in (INVALID, _lib.LF_ERR_CUDA), bad     # (without a GPU its SMs cannot be counted)
+    for bad in (dict(q=0), dict(picked=FAKE), dict(n_q=9), dict(out=0), dict(lengths=0), dict(pages=FAKE + 4)):
+        assert f(_prefix(bad), None) == INVALID, bad
+    assert f(_prefix(dict(head_dim=96)), None) == UNSUPPORTED
+    so = _lib.lib()
+    assert so.lf_int4_prefix_workspace_bytes(0, 8, 40, 1, 128, 1) == 0 == so.lf_int4_prefix_workspace_bytes(1, 8, 7, 1, 128, 1)
+    record = 256 * (128 + 2) * 4
+    few, many = (so.lf_int4_prefix_workspace_bytes(64, 8, 40, q, 128, 1) for q in (1, 256))
+    # 64 sequences' rows (5 heads on a KV head) of 255 query tokens more, in records of 256
+    assert many - few == 8 * (64 * 5 * 256 // 256 - 64 * 5 // 256) * record
+
+
+# ------------------------------------------------------------ frequencies
+
+def _radians(freqs):
+    return [f / 2.0 ** 64 * 2 * math.pi for f in freqs.tolist()]
+
+
+@pytest.mark.parametrize("part,base", [(128, 10000.0), (64, 1e6), (2, 5e5), (34, 10000.0)])
+def test_frequencies_without_scaling(part, base):
+    freqs, magnitude = prompt.rotary_frequencies(part, base, device="cpu")
+    assert freqs.dtype == torch.int64 and magnitude == 1.0
+    for i, got in enumerate(_radians(freqs)):
+        want = base ** (-2 * i / part)
+        assert abs(got - want) <= 2.0 ** -50 * want + 2.0 ** -61   # fp64, then steps of 2^-64 turns
+    linear, magnitude = prompt.rotary_frequencies(part, base, dict(type="linear", factor=4.0), device="cpu")
+    assert magnitude == 1.0
+    assert all(abs(4 * a - b) <= 2.0 ** -60 for a, b in zip(_radians(linear), _radians(freqs)))
+
+
+def test_frequencies_stretched_in_part():
+    """Peng et al.: pairs that turn often keep their frequency, slow ones are divided, a ramp between."""
+    scaling = dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=4096)
+    plain = _radians(prompt.rotary_frequencies(128, device="cpu")[0])
+    freqs, magnitude = prompt.rotary_frequencies(128, scaling=scaling, device="cpu")
+    got = _radians(freqs)
+    assert magnitude == pytest.approx(0.1 * math.log(8.0) + 1.0)
+    turns = [4096 * f / (2 * math.pi) for f in plain]
+    for i, (g, f, t) in enumerate(zip(got, plain, turns)):
+        assert f / 8 * (1 - 1e-12) <= g <= f * (1 + 1e-12)
+        if t > 40:
+            assert g == pytest.approx(f, rel=1e-12), i
+        if t < 0.8:
+            assert g == pytest.approx(f / 8, rel=1e-12), i
+    assert all(a > b for a, b in zip(got, got[1:]))
+    again, m = prompt.rotary_frequencies(128, scaling=dict(scaling, attention_factor=1.5), device="cpu")
+    assert m == 1.5 and torch.equal(again, freqs)
+
+
+def test_frequencies_match_the_installed_transformers():
+    from transformers import Qwen2Config
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+
+    rope = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768, rope_theta=1e6)
+    config = Qwen2Config(hidden_size=512, num_attention_heads=4, max_position_embeddings=131072, rope_theta=1e6, rope_parameters=rope)
+    want, factor = ROPE_INIT_FUNCTIONS["yarn"](config, torch.device("cpu"))
+    got, magnitude = prompt.rotary_frequencies(128, 1e6, rope, device="cpu")
+    assert magnitude == pytest.approx(factor)
+    # its table is fp32: a power and a product, a few roundings of 2^-24
+    assert np.allclose(_radians(got), want.double().numpy(), rtol=2.0 ** -20, atol=0)
+
+
+def test_frequency_refusals():
+    for bad in (0, 3, -2):
+        with pytest.raises(ValueError):
+            prompt.rotary_frequencies(bad, device="cpu")
+    for bad in (0.0, -1.0, math.inf):
+        with pytest.raises(ValueError):
+            prompt.rotary_frequencies(64, bad, device="cpu")
+    yarn = dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=4096)
+    for error, scaling in [(NotImplementedError, dict(rope_type="dynamic", factor=2.0)), (ValueError, dict(rope_type="linear", factor=0.5)),
+                           (KeyError, dict(rope_type="linear")), (NotImplementedError, dict(yarn, mscale=1.0)),
+                           (NotImplementedError, dict(yarn, truncate=False)), (ValueError, dict(yarn, original_max_position_embeddings=0))]:
+        with pytest.raises(error):
+            prompt.rotary_frequencies(64, scaling=scaling, device="cpu")
+
+
+def test_functions_refuse_cpu_tensors():
+    q, k = torch.zeros(4, 8, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    freqs, _ = prompt.rotary_frequencies(64, device="cpu")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        prompt.rotary_embed(q, k, freqs, positions=torch.arange(4))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        prompt.prompt_attention(q, k, k, 0.125)
+    with pytest.raises(TypeError):
+        prompt.prompt_attention(q, k, [1], 0.125)
+    with pytest.raises(ValueError):
+        prompt.prompt_attention(q, k[:3], k[:3], 0.125)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        n = torch.zeros(1, dtype=torch.int32)
+        int4.int4_prefix_attention(q[:1], torch.zeros(4, 2, 1280, dtype=torch.int32), torch.zeros(1, 2, dtype=torch.int32), n, 1.0, n, n)
+
+
+# ------------------------------------------------------------ shared pages in the cache
+
+@pytest.fixture
+def cache(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(int4.Int4KVCache, "_upload", lambda self, t, host: t.copy_(torch.from_numpy(np.asarray(host).astype(np.int32))))
+    return int4.Int4KVCache(1, 4, 4, 2, 64, n_pages=12, max_tokens=400, device="cpu")
+
+
+def test_sharing_bookkeeping(cache):
+    c = cache
+    assert c.prefix_group.tolist() == [0, 1, 2, 3] and c.prefix_pages.tolist() == [0, 0, 0, 0]
+    c.extend([200, 0, 0, 0])
+    assert c.share(0, [2, 3]) == 192 and c.free_pages == 8
+    assert c.lengths.tolist() == [200, 0, 192, 192] and c.start.tolist() == [0, 0, 192, 192] and c.counts.tolist() == [200, 0, 0, 0]
+    assert torch.equal(c.page_table[2, :3], c.page_table[0, :3]) and (c.page_table[2, 3:] == -1).all()
+    assert c.prefix_group.tolist() == [0, 1, 0, 0] and c.prefix_pages.tolist() == [3, 0, 0, 0]
+    c.extend([1, 5, 1, 130])
+    assert c.free_pages == 8 - 1 - 1 - 3
+    rows = [[int(x) for x in row if x >= 0] for row in c.page_table]
+    assert len(rows[0]) == 4 and len(rows[2]) == 4 and len(rows[3]) == 6 and len(rows[1]) == 1
+    own = rows[0][3:] + rows[1] + rows[2][3:] + rows[3][3:]
+    assert len(set(own)) == len(own) and not set(own) & set(rows[0][:3])
+    with pytest.raises(ValueError, match="shares"):
+        c.truncate([200, 5, 191, 300])
+    with pytest.raises(ValueError, match="shares"):
+        c.truncate([100, 5, 193, 300])
+    c.truncate([192, 5, 192, 300])          # behind the shared pages
+    c.release([0])
+    assert c.prefix_group.tolist() == [0, 1, 2, 2] and c.prefix_pages.tolist() == [0, 0, 3, 0]
+    c.release([2])
+    assert c.prefix_group.tolist() == [0, 1, 2, 3] and c.prefix_pages.tolist() == [0, 0, 0, 0]
+    c.truncate([0, 5, 0, 10])               # nobody shares these now
+    c.release()
+    assert c.free_pages == 12 and sorted(c._free) == list(range(12)) and not c._refs.any()
+
+
+def test_sharing_a_part_and_sharing_on(cache):
+    c = cache
+    c.extend([300, 0, 0, 0])
+    assert c.share(0, [1], tokens=130) == 128
+    c.extend([0, 100, 0, 0])
+    assert c.share(1, [2]) == 192            # two pages of the first, one of its own
+    assert c.prefix_group.tolist() == [0, 0, 0, 3] and c.prefix_pages.tolist() == [2, 0, 0, 0]
+    assert c.share(0, [3], tokens=63) == 0 and c.lengths.tolist() == [300, 228, 192, 0]
+    for bad in (dict(source=0, seqs=[0]), dict(source=0, seqs=[3, 3]), dict(source=0, seqs=[1]), dict(source=0, seqs=[3], tokens=301),
+                dict(source=0, seqs=[3], tokens=-1)):
+        with pytest.raises(ValueError):
+            c.share(**bad)
+    with pytest.raises(IndexError):
+        c.share(0, [4])
+    c.reserve([0, 0, 0, 64])
+    with pytest.raises(ValueError, match="empty"):
+        c.share(0, [3])
+
+
+def test_adapter_takes_the_prompt_kernel_by_name():
+    model = tiny_qwen2(n_q=4, n_kv=2, head_dim=64, layers=1, vocab=32, seed=1)
+    assert DeepSeekQwenKVAdapter(model, group_size=64).prompt == "dense"
+    with pytest.raises(ValueError, match="prompt"):
+        DeepSeekQwenKVAdapter(model, group_size=64, prompt="fast")
+    a = DeepSeekQwenKVAdapter(model, group_size=64, prompt="kernel").attach()
+    a._packed = type("Empty", (), dict(seq_len=0, layer_length=lambda self, i: 0, reset=lambda self: None))()
+    ids = torch.zeros(1, 5, dtype=torch.long)
+    with torch.no_grad(), pytest.raises((NotImplementedError, RuntimeError)):   # fp32 on the CPU: no fallback
+        model(input_ids=ids)
+    masked = torch.tensor([[0, 1, 1, 1, 1]])
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="mask"):
+        model(input_ids=ids, attention_mask=masked)
