@@ -39,6 +39,28 @@ template <> struct Scalar<__nv_bfloat16> {
   static __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 };
 
+// Two numbers rounded to T, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack_two(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_two<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack_two<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Both numbers of a word.
+template <typename T> __device__ __forceinline__ float2 unpack_two(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack_two<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack_two<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
 __device__ __forceinline__ float half_bits_to_float(uint16_t bits) {
   return __half2float(__ushort_as_half(bits));
 }

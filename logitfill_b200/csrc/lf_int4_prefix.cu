@@ -66,6 +66,7 @@ __device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int cou
 __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_constant__ PrefixParams p) {
   __shared__ int count_s[kMaxGroups], first_s[kMaxGroups], any_s[kMaxGroups];
   const int lane = threadIdx.x;
+  grid_dep_trigger();  // the prefix kernel's CTAs may start: they wait for this one before they read
   grid_dep_wait();
   for (int g = lane; g < p.groups; g += 32) count_s[g] = 0;
   __syncwarp();
@@ -306,6 +307,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&sh.tmem), 0);
+  grid_dep_trigger();  // all CTAs of this grid run at once, so the suffix kernel's take nothing that one needs
   grid_dep_wait();
 
   volatile int* stop = &sh.stop;

@@ -12,9 +12,11 @@
 // What bounds it: every element is read and written once and the angles are shared by a
 // token's heads, so a large call is bound by HBM.  A thread keeps the cosines and sines
 // of its pairs (16 bytes of channels and their partners) in registers and walks over the
-// token's heads, four in flight; its angles are worked out while the first loads are on
-// their way, with no shared memory and no barrier.  In small calls there are as many
-// threads to a token as it has heads, so that each makes one round of loads.
+// token's heads, four in flight.  The block's angles are worked out once, each by one
+// thread, while the first loads are on their way, and handed over in shared memory: with
+// each thread working out its own, 16384 tokens of 32 heads, D 128, took 90 us (the
+// arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
+// token as it has heads, so that each makes one round of loads.
 #include <cmath>
 
 #include "lf_common.cuh"
@@ -37,6 +39,7 @@ struct RotaryParams {
 };
 
 constexpr int kRotaryThreads = 256, kRotaryAhead = 4;
+
 constexpr int64_t kRotaryFill = 148 * 2048;  // threads that a B200 holds at once
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T x[N]; };
@@ -54,12 +57,81 @@ __device__ __forceinline__ void turn_of(uint64_t phase, float& c, float& s) {
   s = minus_s ? -s : s;
 }
 
+// Sequence and token of a token of all sequences.  (A 64-bit division is some 100
+// instructions: as many as the rest of what a thread does for a head.)
+__device__ __forceinline__ void split(const RotaryParams& p, int64_t token, int64_t& b, int64_t& t) {
+  if (p.total <= INT32_MAX) {
+    b = static_cast<uint32_t>(token) / static_cast<uint32_t>(p.tokens);
+    t = static_cast<uint32_t>(token) - static_cast<uint32_t>(b) * p.tokens;
+  } else {
+    b = token / p.tokens;
+    t = token - b * p.tokens;
+  }
+}
+
+// Pairs (u, w) turned: two of them at a time.
+__device__ __forceinline__ void turn_two(float2& u, float2& w, float2 c, float2 s) {
+  const float2 a = __fmul2_rn(w, make_float2(-s.x, -s.y)), b = __fmul2_rn(u, s);
+  u = __ffma2_rn(u, c, a);
+  w = __ffma2_rn(w, c, b);
+}
+// N pairs, of vectors x and y (half pairs).
+template <typename T, int N>
+__device__ __forceinline__ void turn_halves(Pack<T, N>& x, Pack<T, N>& y, const float (&c)[N], const float (&s)[N]) {
+  if constexpr (N == 1) {
+    const float u = Scalar<T>::load(x.x), w = Scalar<T>::load(y.x);
+    Scalar<T>::store(x.x, fmaf(u, c[0], -w * s[0]));
+    Scalar<T>::store(y.x, fmaf(w, c[0], u * s[0]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float2 u, w;
+      if constexpr (sizeof(T) == 4) {
+        u = make_float2(x.x[i], x.x[i + 1]);
+        w = make_float2(y.x[i], y.x[i + 1]);
+      } else {
+        u = unpack_two<T>(reinterpret_cast<uint32_t*>(x.x)[i / 2]);
+        w = unpack_two<T>(reinterpret_cast<uint32_t*>(y.x)[i / 2]);
+      }
+      turn_two(u, w, make_float2(c[i], c[i + 1]), make_float2(s[i], s[i + 1]));
+      if constexpr (sizeof(T) == 4) {
+        x.x[i] = u.x;
+        x.x[i + 1] = u.y;
+        y.x[i] = w.x;
+        y.x[i + 1] = w.y;
+      } else {
+        reinterpret_cast<uint32_t*>(x.x)[i / 2] = pack_two<T>(u.x, u.y);
+        reinterpret_cast<uint32_t*>(y.x)[i / 2] = pack_two<T>(w.x, w.y);
+      }
+    }
+  }
+}
+// N / 2 pairs of one vector (adjacent pairs).
+template <typename T, int N>
+__device__ __forceinline__ void turn_adjacent(Pack<T, N>& x, const float (&c)[N / 2], const float (&s)[N / 2]) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    float2 u;
+    if constexpr (sizeof(T) == 4)
+      u = make_float2(x.x[2 * i], x.x[2 * i + 1]);
+    else
+      u = unpack_two<T>(reinterpret_cast<uint32_t*>(x.x)[i]);
+    u = make_float2(fmaf(u.x, c[i], -u.y * s[i]), fmaf(u.y, c[i], u.x * s[i]));
+    if constexpr (sizeof(T) == 4) {
+      x.x[2 * i] = u.x;
+      x.x[2 * i + 1] = u.y;
+    } else {
+      reinterpret_cast<uint32_t*>(x.x)[i] = pack_two<T>(u.x, u.y);
+    }
+  }
+}
+
 // N elements a vector.  Half pairs: item v < part / 2 / N is the vectors at N v and N v +
 // part / 2.  Adjacent pairs: item v < part / N is the vector at N v; for N = 1, item v <
 // part / 2 is the elements at 2 v and 2 v + 1.  The items behind them are vectors of
 // channels that are copied.
 template <typename T, int N, bool kAdjacent>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr bool kInside = kAdjacent && N > 1;  // both channels of a pair in one vector
   constexpr int kPairs = kInside ? N / 2 : N;
   using Vec = Pack<T, N>;
@@ -67,67 +139,99 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   const int first_head = slot % p.head_lanes, in_block = slot / p.head_lanes;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * p.per_block + in_block;
   grid_dep_wait();
-  if (in_block >= p.per_block || token >= p.total) return;
-  const int64_t b = token / p.tokens, t = token - b * p.tokens;
+  const bool mine = in_block < p.per_block && token < p.total;
+  int64_t b, t;
+  split(p, token, b, t);
   const int turning = kInside ? p.part / N : p.part / 2 / N;
   const bool turns = v < turning;
   // The item's channel, and its partner's.
   const int at = !turns ? p.part + (v - turning) * N : kAdjacent && !kInside ? 2 * v : v * N;
   const int other = kAdjacent ? at + 1 : at + p.part / 2;
-  const T *q = static_cast<const T*>(p.q) + b * p.q_seq + t * p.q_tok, *k = static_cast<const T*>(p.k) + b * p.k_seq + t * p.k_tok;
-  T *qo = static_cast<T*>(p.q_out) + b * p.qo_seq + t * p.qo_tok, *ko = static_cast<T*>(p.k_out) + b * p.ko_seq + t * p.ko_tok;
-  auto source = [&](int h) { return h < p.n_q ? q + h * p.q_head : k + (h - p.n_q) * p.k_head; };
-  auto target = [&](int h) { return h < p.n_q ? qo + h * p.qo_head : ko + (h - p.n_q) * p.ko_head; };
+  // This thread's rows: of the queries from its first head on, then of the Keys.
+  struct Rows {
+    const T* in;
+    T* out;
+    int64_t in_step, out_step;
+    int n;
+  } rows[2];
+  const int first_k = first_head < p.n_q ? first_head + (p.n_q - first_head + p.head_lanes - 1) / p.head_lanes * p.head_lanes - p.n_q
+                                         : first_head - p.n_q;
+  const int n_kv = p.heads - p.n_q;
+  rows[0] = Rows{static_cast<const T*>(p.q) + b * p.q_seq + t * p.q_tok + first_head * p.q_head,
+                 static_cast<T*>(p.q_out) + b * p.qo_seq + t * p.qo_tok + first_head * p.qo_head, p.head_lanes * p.q_head,
+                 p.head_lanes * p.qo_head, mine && first_head < p.n_q ? (p.n_q - first_head + p.head_lanes - 1) / p.head_lanes : 0};
+  rows[1] = Rows{static_cast<const T*>(p.k) + b * p.k_seq + t * p.k_tok + first_k * p.k_head,
+                 static_cast<T*>(p.k_out) + b * p.ko_seq + t * p.ko_tok + first_k * p.ko_head, p.head_lanes * p.k_head,
+                 p.head_lanes * p.ko_head, mine && first_k < n_kv ? (n_kv - first_k + p.head_lanes - 1) / p.head_lanes : 0};
 
   Vec x[kRotaryAhead], y[kRotaryAhead];
-  auto load = [&](int h0) {
+  auto load = [&](const Rows& r) {
 #pragma unroll
     for (int j = 0; j < kRotaryAhead; ++j) {
-      const int h = h0 + j * p.head_lanes;
-      if (h >= p.heads) break;
-      x[j] = *reinterpret_cast<const Vec*>(source(h) + at);
-      if (!kInside && turns) y[j] = *reinterpret_cast<const Vec*>(source(h) + other);
+      if (j >= r.n) break;
+      x[j] = *reinterpret_cast<const Vec*>(r.in + j * r.in_step + at);
+      if (!kInside && turns) y[j] = *reinterpret_cast<const Vec*>(r.in + j * r.in_step + other);
     }
   };
-  load(first_head);
+  const bool k_first = rows[0].n == 0;
+  if (k_first)
+    load(rows[1]);
+  else
+    load(rows[0]);
 
-  float c[kPairs], s[kPairs];
-  if (turns) {
+  // The block's tokens' angles, each by one thread.  Pair i of item v lies at place i *
+  // turning + v of its token, so that a warp's reads do not meet in a bank.
+  __shared__ float2 turn_s[kRotaryThreads * 8];
+  const int pairs = p.part / 2;
+  for (int x = threadIdx.x; x < p.per_block * pairs; x += kRotaryThreads) {
+    const int which = x / pairs, pair = x - which * pairs;
+    const int64_t tok = static_cast<int64_t>(blockIdx.x) * p.per_block + which;
+    if (tok >= p.total) break;
+    int64_t bb, tt;
+    split(p, tok, bb, tt);
     int64_t position;
     if (p.positions == nullptr)
-      position = static_cast<int64_t>(p.start[b]) + t;
+      position = static_cast<int64_t>(p.start[bb]) + tt;
     else if (p.positions_64)
-      position = static_cast<const int64_t*>(p.positions)[b * p.pos_seq + t * p.pos_tok];
+      position = static_cast<const int64_t*>(p.positions)[bb * p.pos_seq + tt * p.pos_tok];
     else
-      position = static_cast<const int32_t*>(p.positions)[b * p.pos_seq + t * p.pos_tok];
+      position = static_cast<const int32_t*>(p.positions)[bb * p.pos_seq + tt * p.pos_tok];
+    float c, s;
+    turn_of(static_cast<uint64_t>(position) * static_cast<uint64_t>(p.freqs[pair]), c, s);
+    turn_s[which * pairs + pair % kPairs * turning + pair / kPairs] = make_float2(c * p.magnitude, s * p.sign);
+  }
+  __syncthreads();
+  if (!mine) return;
+  float c[kPairs], s[kPairs];
+  if (turns) {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const int pair = v * kPairs + i;
-      turn_of(static_cast<uint64_t>(position) * static_cast<uint64_t>(p.freqs[pair]), c[i], s[i]);
-      c[i] *= p.magnitude;
-      s[i] *= p.sign;
+      const float2 y = turn_s[in_block * pairs + i * turning + v];
+      c[i] = y.x;
+      s[i] = y.y;
     }
   }
-  for (int h0 = first_head; h0 < p.heads; h0 += kRotaryAhead * p.head_lanes) {
-    if (h0 != first_head) load(h0);
+  bool loaded = true;
+  auto go = [&](Rows r) {
+    for (; r.n > 0; r.n -= kRotaryAhead, r.in += kRotaryAhead * r.in_step, r.out += kRotaryAhead * r.out_step) {
+      if (!loaded) load(r);
+      loaded = false;
 #pragma unroll
-    for (int j = 0; j < kRotaryAhead; ++j) {
-      const int h = h0 + j * p.head_lanes;
-      if (h >= p.heads) break;
-      if (turns) {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          T& first = x[j].x[kInside ? 2 * i : i];
-          T& second = kInside ? x[j].x[kInside ? 2 * i + 1 : 0] : y[j].x[i];
-          const float u = Scalar<T>::load(&first), w = Scalar<T>::load(&second);
-          Scalar<T>::store(&first, fmaf(u, c[i], -w * s[i]));
-          Scalar<T>::store(&second, fmaf(w, c[i], u * s[i]));
+      for (int j = 0; j < kRotaryAhead; ++j) {
+        if (j >= r.n) break;
+        if (turns) {
+          if constexpr (kInside)
+            turn_adjacent<T, N>(x[j], c, s);
+          else
+            turn_halves<T, N>(x[j], y[j], c, s);
+          if (!kInside) *reinterpret_cast<Vec*>(r.out + j * r.out_step + other) = y[j];
         }
-        if (!kInside) *reinterpret_cast<Vec*>(target(h) + other) = y[j];
+        *reinterpret_cast<Vec*>(r.out + j * r.out_step + at) = x[j];
       }
-      *reinterpret_cast<Vec*>(target(h) + at) = x[j];
     }
-  }
+  };
+  go(rows[0]);
+  go(rows[1]);
 }
 
 template <typename T>
@@ -200,8 +304,8 @@ extern "C" int lf_rotary_embed(const lf_rotary* a, lf_stream_t stream) {
   p.per_row = wide ? (a->interleaved ? a->part : a->part / 2) / lanes + (a->head_dim - a->part) / lanes : a->head_dim - a->part / 2;
 
   // Threads to a token and item: as many as there are heads in a small call (a thread makes
-  // one load and store), down to one for each kRotaryAhead heads once the threads fill the
-  // GPU.  Measured at 16 x 1 tokens, 32 heads: see the figures below the kernel.
+  // one round of loads), down to one for each kRotaryAhead heads once the threads fill the
+  // GPU.  16384 tokens, 32 heads: 57 us so, 59 with 8 heads to a thread, 61 with 16.
   const int slots = kRotaryThreads / p.per_row;
   int lanes_heads = p.heads;
   while (lanes_heads > 1 && static_cast<int64_t>(p.total) * p.per_row * lanes_heads > kRotaryFill && lanes_heads * kRotaryAhead > p.heads)
