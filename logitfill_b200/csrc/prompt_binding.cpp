@@ -4,7 +4,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/ops/empty_strided.h>
 
 #include <cmath>
 
@@ -41,6 +41,13 @@ struct Rows {
 
 at::Tensor channels_last(const at::Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// A new tensor like t: with its strides where it has no gaps (a projection's transposed
+// view stays one), else contiguous.
+at::Tensor new_like(const at::Tensor& t) {
+  if (t.is_non_overlapping_and_dense()) return at::empty_strided(t.sizes(), t.strides(), t.options());
+  return at::empty(t.sizes(), t.options());
 }
 
 // Whether two tensors are known to share memory (strided views of one buffer whose gaps
@@ -125,8 +132,8 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const at::Tensor q = channels_last(query), k = with_key ? channels_last(key) : none;
     at::Tensor q_out, k_out;
     if (v[8] == Py_None) {
-      q_out = at::empty_like(q);
-      if (with_key) k_out = at::empty_like(k);
+      q_out = new_like(q);
+      if (with_key) k_out = new_like(k);
     } else {
       if (!PyTuple_Check(v[8]) || PyTuple_GET_SIZE(v[8]) != 2) fail(PyExc_TypeError, "out must be a tuple (query, key)");
       q_out = tensor(PyTuple_GET_ITEM(v[8], 0), "out[0]");
@@ -224,7 +231,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const Launch on(query.device());
     at::Tensor out;
     if (v[6] == Py_None) {
-      out = at::empty_like(query);
+      out = new_like(query);
       if (plain_rows(out).data_ptr() != out.data_ptr()) out = at::empty(query.sizes(), query.options());
     } else {
       out = tensor(v[6], "out");
