@@ -464,6 +464,7 @@ typedef struct lf_int4_prefix {
   void* workspace;        /* of its own, beside the query's                       */
   size_t workspace_bytes;
   int32_t groups;
+  int32_t always;         /* 0: where reading them once is expected to be faster   */
 } lf_int4_prefix;
 
 /*

@@ -319,12 +319,13 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// attend_prefix(query, pages, page_table, lengths, scaling, group, shared, counts, out, status) -> out
+// attend_prefix(query, pages, page_table, lengths, scaling, group, shared, counts, out, status, always) -> out
 PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    expect(n, 10);
+    expect(n, 11);
     const Pool p = make_pool(v[1], v[2]);
     lf_int4_prefix a{};
+    a.always = PyObject_IsTrue(v[10]) == 1;
     const at::Tensor q = fill_query(a.query, p, v[0], v[3], v[4], v[7], v[9]);
     a.group = per_sequence(v[5], "prefix_group", p, false);
     const at::Tensor& shared = tensor(v[6], "prefix_pages");

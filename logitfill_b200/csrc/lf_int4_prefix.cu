@@ -43,7 +43,7 @@ struct PrefixParams {
   int64_t q_seq, q_head, q_tok;
   int q_len, heads;               // query heads of a KV head
   const int32_t *lengths, *counts, *group, *shared;
-  int groups, grid;
+  int groups, grid, head_dim, always;
   float scale_log2;
   int32_t* status;
   PrefixPlan plan;
@@ -53,14 +53,39 @@ struct PrefixParams {
 
 constexpr int kMaxGroups = 4096;
 
-// Shared pages of group g that its `count` members (one of them `any`) read together.  One
-// member with few rows has nothing to share.
+// Whether the shared pages are read once, or by each sequence as lf_int4_attend does, is a
+// matter of sizes.  In ns on a B200: a page costs lf_int4_attend's kernel about 2 for up to 8
+// query columns and 2.9 for 16 (D 128; half at D 64), every time it is read; a place of the
+// line costs 5 here, and the two kernels more and the records 26000.  Measured in us, that
+// kernel / these three, D 128, bf16, replayed: 28 heads on 4, one token each, 8192 shared
+// tokens: 16 sequences 25 / 30, 32 sequences 41 / 37; 32768 tokens: 4 sequences 28 / 37,
+// 8: 41 / 39, 16: 69 / 41, 32: 127 / 54; 40 heads on 8, 8192 tokens: 8 sequences 25 / 28,
+// 16: 41 / 29; one sequence behind 32768 tokens, 28 heads on 4: 8 tokens 37 / 45, 16: 50 / 48,
+// 32: 85 / 56, 128: 298 / 124.
+constexpr int64_t kPrefixFixedNs = 26000;
+__host__ __device__ __forceinline__ int64_t visit_ns(int64_t pages, int columns, int head_dim) {
+  return pages * ((columns + 15) / 16) * (columns <= 8 ? 20 : 29) * head_dim / 1280;
+}
+
+// Shared pages of group g that its `count` members (one of them `any`) have.
 __device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int count, int any) {
-  if (count == 0 || (count == 1 && p.q_len * p.heads <= 16)) return 0;
+  if (count == 0) return 0;
   // All pages of one member are its own: the complete ones (what a page's unwritten slots
   // hold may not be read here) are read in this way, its queries' own tokens among them.
-  if (count == 1) return min(max(p.lengths[any], 0) / kInt4Page, p.pool.table_width);
+  if (count == 1) return p.q_len * p.heads <= 16 ? 0 : min(max(p.lengths[any], 0) / kInt4Page, p.pool.table_width);
   return min(max(p.shared[g], 0), p.pool.table_width);
+}
+// What a group's shared pages take in the line, and what reading them once saves.
+struct GroupCost { int tiles, steps, last, places; int64_t saved; };
+__device__ __forceinline__ GroupCost group_cost(const PrefixParams& p, int pages, int count) {
+  GroupCost c;
+  const int rows = count * p.q_len * p.heads;
+  c.tiles = pages > 0 ? (rows + kPrefixRows - 1) / kPrefixRows : 0;
+  c.steps = (pages + 1) / 2;
+  c.last = c.tiles > 0 && rows - (c.tiles - 1) * kPrefixRows <= kPrefixRows / 2 ? 1 : 2;
+  c.places = c.tiles > 0 ? p.pool.kv_heads * prefix_head_places(c.tiles, c.steps, c.last) : 0;
+  c.saved = visit_ns(static_cast<int64_t>(pages) * count * p.pool.kv_heads, p.q_len * p.heads, p.head_dim) - 5 * static_cast<int64_t>(c.places);
+  return c;
 }
 
 __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_constant__ PrefixParams p) {
@@ -87,15 +112,24 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
     __syncwarp();
     if (b < p.pool.batch) p.plan.seqs[b] = PrefixSeq{g, rank};
   }
+  // Whether it pays in all.
+  int64_t saved = 0;
+  for (int g = lane; g < p.groups; g += 32) {
+    const int count = count_s[g], pages = group_pages(p, g, count, any_s[g]);
+    saved += max(static_cast<int64_t>(0), group_cost(p, pages, count).saved);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) saved += __shfl_xor_sync(0xffffffffu, saved, o);
+  const bool pays = p.always || saved > kPrefixFixedNs;
   // The groups' places in the lists and in the line.
   int members = 0, units = 0, places = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane;
     const int count = g < p.groups ? count_s[g] : 0;
-    const int pages = g < p.groups ? group_pages(p, g, count, any_s[g]) : 0;
-    const int tiles = pages > 0 ? (count * p.q_len * p.heads + kPrefixRows - 1) / kPrefixRows : 0, steps = (pages + 1) / 2;
-    const int last = tiles > 0 && count * p.q_len * p.heads - (tiles - 1) * kPrefixRows <= kPrefixRows / 2 ? 1 : 2;
-    const int n_units = tiles * p.pool.kv_heads, n_places = tiles > 0 ? p.pool.kv_heads * prefix_head_places(tiles, steps, last) : 0;
+    int pages = pays && g < p.groups ? group_pages(p, g, count, any_s[g]) : 0;
+    if (!p.always && group_cost(p, pages, count).saved <= 0) pages = 0;
+    const GroupCost cost = group_cost(p, pages, count);
+    const int tiles = cost.tiles, steps = cost.steps, last = cost.last, n_units = tiles * p.pool.kv_heads, n_places = cost.places;
     int m = count, u = n_units, x = n_places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -667,7 +701,9 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   if (bad != LF_OK) return bad;
   LF_CHECK_ARG(a->groups >= 0 && (a->groups == 0 || (a->group && a->shared)), "lf_int4_attend_prefix: null pointer");
   LF_CHECK_SUPPORTED(a->groups <= kMaxGroups, "lf_int4_attend_prefix: %d groups (%d at most)", a->groups, kMaxGroups);
-  if (a->groups == 0) return lf_int4_attend(&q, stream);
+  const int columns = q.q_len * (q.n_q / q.pool.kv_heads);
+  const bool small = visit_ns(static_cast<int64_t>(q.pool.batch) * q.pool.kv_heads * q.pool.table_width, columns, q.head_dim) <= kPrefixFixedNs;
+  if (a->groups == 0 || (small && !a->always)) return lf_int4_attend(&q, stream);
   PrefixParams p;
   const int ok = check_int4_pool("lf_int4_attend_prefix", q.pool, q.head_dim, p.pool);
   if (ok != LF_OK) return ok;
@@ -682,6 +718,8 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   p.group = a->group;
   p.shared = a->shared;
   p.groups = a->groups;
+  p.head_dim = q.head_dim;
+  p.always = a->always;
   p.scale_log2 = q.scaling * 1.4426950408889634f;
   p.status = q.status;
   const int sms = sm_count();

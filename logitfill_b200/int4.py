@@ -128,7 +128,7 @@ def int4_sparse_attention(query: torch.Tensor, pages: torch.Tensor, bounds: torc
 def int4_prefix_attention(query: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                           scaling: float, prefix_group: torch.Tensor, prefix_pages: torch.Tensor,
                           counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                          status: torch.Tensor | None = None) -> torch.Tensor:
+                          status: torch.Tensor | None = None, always: bool = False) -> torch.Tensor:
     """:func:`int4_attention` where sequences share their first pages (a system
     prompt, a document that several ask about, or, for one sequence with many
     query tokens, its own history): the shared pages are read and unpacked once
@@ -138,9 +138,11 @@ def int4_prefix_attention(query: torch.Tensor, pages: torch.Tensor, page_table: 
     groups - 1``: none), ``prefix_pages`` (int32 ``[groups]``) how many of their
     first page table entries a group's sequences have in common; the entries of
     its lowest sequence are read.  Both are read on the GPU.  The result is
-    :func:`int4_attention`'s up to the order of sums, for any lengths."""
+    :func:`int4_attention`'s up to the order of sums, for any lengths.  Where few
+    sequences share few pages, each reads them itself, which is faster then
+    (``always``: never)."""
     return _lib.int4_binding().attend_prefix(query, pages, page_table, lengths, scaling, prefix_group, prefix_pages, counts, out,
-                                             status)
+                                             status, always)
 
 
 class Int4KVCache:

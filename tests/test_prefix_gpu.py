@@ -61,8 +61,9 @@ class Batch:
         return torch.randn(len(self.group), n_q, q_len, self.D, generator=g, device="cuda").to(dtype or self.dtype)
 
     def run(self, q, scaling, counts=None, **kw):
+        """The shared pages read once, whatever the sizes (where it does not pay, a call leaves them to int4_attention)."""
         return int4.int4_prefix_attention(q, self.pages, self.table, _i32(self.lengths), scaling, _i32(self.group), _i32(self.shared),
-                                          counts=None if counts is None else _i32(counts), **kw)
+                                          counts=None if counts is None else _i32(counts), **dict(dict(always=True), **kw))
 
     def values(self):
         """Key and Value [B, H, tokens, D] that the pages hold, in 64 bits."""
@@ -140,6 +141,24 @@ def test_long_prefixes_in_many_ranges():
     assert all(torch.equal(batch.run(q, 0.0884), got) for _ in range(3))     # no result depends on timing
 
 
+def test_where_it_does_not_pay():
+    """Few sequences, few pages: the call is int4_attention's, bit for bit; many of both are not, and right too; groups of
+    both kinds in one call."""
+    batch = Batch(22, [0, 0, 1, -1], [9, 4], [70, 1, 64, 30], 2, 128)
+    q = batch.query(19, 8, 1)
+    plain = int4.int4_attention(q, batch.pages, batch.table, _i32(batch.lengths), 0.09)
+    assert torch.equal(batch.run(q, 0.09, always=False), plain)
+    batch = Batch(23, [0] * 40 + [1, 1], [300, 2], [70 - b for b in range(42)], 4, 128)
+    q = batch.query(20, 28, 1)
+    got = batch.run(q, 0.0884, always=False)
+    batch.check(got, q, 0.0884)
+    assert torch.equal(got[:40], batch.run(q, 0.0884)[:40])
+    # few shared pages in wide tables: planned on the GPU, and left to the sequences there
+    batch = Batch(24, [0] * 40, [2], [70 - b for b in range(40)], 4, 64, F16, spare=600)
+    q = batch.query(21, 28, 1)
+    batch.check(batch.run(q, 0.125, always=False), q, 0.125)
+
+
 def test_many_groups():
     groups = 70
     group = [b * 29 % (groups + 1) - 1 for b in range(150)]
@@ -172,7 +191,7 @@ def test_more_shared_pages_named_than_are_written():
     q = batch.query(9, 8, 1)
     want, bound = batch.want(q, 0.09)
     for named in (4, 1 << 30, -5, 0):
-        got = int4.int4_prefix_attention(q, batch.pages, batch.table, _i32([192, 192, 192]), 0.09, _i32([0, 0, 0]), _i32([min(named, 3) if named == 4 else named]))
+        got = int4.int4_prefix_attention(q, batch.pages, batch.table, _i32([192, 192, 192]), 0.09, _i32([0, 0, 0]), _i32([named]), always=True)
         alike = int4.int4_attention(q, batch.pages, batch.table, _i32([192, 192, 192]), 0.09)
         w, b = batch.want(q, 0.09, lengths=[192, 192, 192])
         assert bool(((got.double() - w).abs() <= b).all()) and bool(((alike.double() - w).abs() <= b).all())
@@ -301,7 +320,7 @@ def test_strides_streams_and_graphs():
     for o in outs:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            int4.int4_prefix_attention(q, batch.pages, batch.table, lengths, 0.09, group, shared, out=o)
+            int4.int4_prefix_attention(q, batch.pages, batch.table, lengths, 0.09, group, shared, out=o, always=True)
         graphs.append(graph)
     for _ in range(2):
         for graph in graphs:
@@ -310,7 +329,7 @@ def test_strides_streams_and_graphs():
     lengths -= 1                                     # read when it runs
     group[1] = -1
     graphs[0].replay()
-    direct = int4.int4_prefix_attention(q, batch.pages, batch.table, lengths, 0.09, group, shared)
+    direct = int4.int4_prefix_attention(q, batch.pages, batch.table, lengths, 0.09, group, shared, always=True)
     assert torch.equal(outs[0], direct) and not torch.equal(direct, want)
 
 

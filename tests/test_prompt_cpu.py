@@ -87,9 +87,9 @@ def test_prompt_attention_validates_before_launch():
 
 
 def _prefix(query=None, **over):
-    f = dict(group=FAKE, shared=FAKE, ws=FAKE, ws_bytes=1 << 40, groups=2)
+    f = dict(group=FAKE, shared=FAKE, ws=FAKE, ws_bytes=1 << 40, groups=2, always=1)
     f.update(over)
-    return _query(**dict(dict(picked=0), **(query or {}))) + struct.pack("@PPPNi0q", *f.values())
+    return _query(**dict(dict(picked=0), **(query or {}))) + struct.pack("@PPPNii0q", *f.values())
 
 
 def test_prefix_attention_validates_before_launch():
