@@ -89,12 +89,8 @@ struct PrefixGroup {
   int members, count;
   int units, places;  // first unit, first place in the line
   int tiles, steps;   // row tiles of a KV head, Key tiles of a unit
-  int last;           // places of a step of a KV head's last unit (1: it has one half's rows)
-  int pad[3];
 
-  // Unit x of the group (KV head x / tiles, row tile x % tiles): places of a step, and its
-  // first step's place.
-  __device__ __forceinline__ int weight(int x) const { return x % tiles == tiles - 1 ? last : 2; }
+  // Place of the first step of unit x of the group (KV head x / tiles, row tile x % tiles).
   __device__ __forceinline__ int start(int x) const;
 };
 struct PrefixSeq { int group, rank; };  // group -1: no shared pages
@@ -106,15 +102,12 @@ struct PrefixPlan {
   float* records;
 };
 constexpr int kPrefixRows = 256;    // rows (query token, q-head) of a unit, in two halves
-constexpr int kPrefixCost = 4;      // empty places before a unit's steps: what taking it up costs
-// Places of a KV head's units.
-__device__ __forceinline__ int prefix_head_places(int tiles, int steps, int last) {
-  return (tiles - 1) * (2 * steps + kPrefixCost) + last * steps + kPrefixCost;
-}
-__device__ __forceinline__ int PrefixGroup::start(int x) const {
-  const int h = x / tiles;
-  return places + h * prefix_head_places(tiles, steps, last) + (x - h * tiles) * (2 * steps + kPrefixCost) + kPrefixCost;
-}
+// Empty places before a unit's steps: what taking it up costs, in steps.  (A unit of 128 rows
+// takes nearly as long for a step as one of 256, 2.2 us and 2.6 at D 128: what bounds the
+// former is the unpacking of pages.  Its steps taken by both row tiles in turn, with a
+// record each, were no faster.)
+constexpr int kPrefixCost = 2;
+__device__ __forceinline__ int PrefixGroup::start(int x) const { return places + x * (steps + kPrefixCost) + kPrefixCost; }
 // Floats of a record: maxima, sums, accumulators.
 __host__ __device__ constexpr int64_t prefix_record(int D) { return kPrefixRows * (static_cast<int64_t>(D) + 2); }
 

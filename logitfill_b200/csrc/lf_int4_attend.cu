@@ -296,7 +296,7 @@ __device__ __forceinline__ void add_shared(const PrefixPlan& plan, const SharedR
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int x = where.h * g.tiles + row[k] / kPrefixRows, start = g.start(x), first = start / where.per;
-    n[k] = (start + g.weight(x) * (g.steps - 1)) / where.per - first + 1;
+    n[k] = (start + g.steps - 1) / where.per - first + 1;
     most = max(most, n[k]);
     rec[k] = plan.records + (g.units + x + first) * prefix_record(D) + row[k] % kPrefixRows;
   }

@@ -43,7 +43,7 @@ struct PrefixParams {
   int64_t q_seq, q_head, q_tok;
   int q_len, heads;               // query heads of a KV head
   const int32_t *lengths, *counts, *group, *shared;
-  int groups, grid, head_dim, always;
+  int groups, grid, head_dim, fp16, always;
   float scale_log2;
   int32_t* status;
   PrefixPlan plan;
@@ -55,17 +55,19 @@ constexpr int kMaxGroups = 4096;
 
 // Whether the shared pages are read once, or by each sequence as lf_int4_attend does, is a
 // matter of sizes.  In ns on a B200: a page costs lf_int4_attend's kernel about 2 for up to 8
-// query columns and 2.9 for 16 (D 128; half at D 64), every time it is read; a place of the
-// line costs 5 here, and the two kernels more and the records 26000.  Measured in us, that
-// kernel / these three, D 128, bf16, replayed: 28 heads on 4, one token each, 8192 shared
-// tokens: 16 sequences 25 / 30, 32 sequences 41 / 37; 32768 tokens: 4 sequences 28 / 37,
-// 8: 41 / 39, 16: 69 / 41, 32: 127 / 54; 40 heads on 8, 8192 tokens: 8 sequences 25 / 28,
-// 16: 41 / 29; one sequence behind 32768 tokens, 28 heads on 4: 8 tokens 37 / 45, 16: 50 / 48,
-// 32: 85 / 56, 128: 298 / 124.
-constexpr int64_t kPrefixFixedNs = 26000;
+// query columns and 2.9 for 16 (D 128; half at D 64), every time it is read; a Key tile of a
+// unit costs 16 here, 30 with the two terms of fp16 (D 64: 11 and 16), and the two kernels
+// more and the records 17000 (D 64: 12500).  Measured in us, that kernel / these three,
+// replayed.  28 heads on 4, D 128, bf16, one token each: 8192 shared tokens, 16 sequences
+// 25 / 30, 32 sequences 41 / 37; 32768 tokens, 4 sequences 28 / 37, 8: 41 / 39, 16: 69 / 41,
+// 32: 127 / 54.  40 heads on 8: 8192 tokens, 8 sequences 25 / 28, 16: 41 / 29; 32768 tokens, 4
+// sequences 41 / 48, 8: 69 / 48; fp16, 8: 75 / 81, 16: 140 / 82.  One sequence behind 32768
+// tokens, 28 heads on 4, bf16: 8 query tokens 37 / 45, 16: 50 / 48, 32: 85 / 56, 128: 298 / 124.
 __host__ __device__ __forceinline__ int64_t visit_ns(int64_t pages, int columns, int head_dim) {
   return pages * ((columns + 15) / 16) * (columns <= 8 ? 20 : 29) * head_dim / 1280;
 }
+__host__ __device__ __forceinline__ int tile_ns(int head_dim, bool fp16) { return head_dim == 128 ? (fp16 ? 30 : 16) : (fp16 ? 16 : 11); }
+__host__ __device__ __forceinline__ int64_t fixed_ns(int head_dim) { return head_dim == 128 ? 17000 : 12500; }
 
 // Shared pages of group g that its `count` members (one of them `any`) have.
 __device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int count, int any) {
@@ -76,15 +78,15 @@ __device__ __forceinline__ int group_pages(const PrefixParams& p, int g, int cou
   return min(max(p.shared[g], 0), p.pool.table_width);
 }
 // What a group's shared pages take in the line, and what reading them once saves.
-struct GroupCost { int tiles, steps, last, places; int64_t saved; };
+struct GroupCost { int tiles, steps, places; int64_t saved; };
 __device__ __forceinline__ GroupCost group_cost(const PrefixParams& p, int pages, int count) {
   GroupCost c;
   const int rows = count * p.q_len * p.heads;
   c.tiles = pages > 0 ? (rows + kPrefixRows - 1) / kPrefixRows : 0;
   c.steps = (pages + 1) / 2;
-  c.last = c.tiles > 0 && rows - (c.tiles - 1) * kPrefixRows <= kPrefixRows / 2 ? 1 : 2;
-  c.places = c.tiles > 0 ? p.pool.kv_heads * prefix_head_places(c.tiles, c.steps, c.last) : 0;
-  c.saved = visit_ns(static_cast<int64_t>(pages) * count * p.pool.kv_heads, p.q_len * p.heads, p.head_dim) - 5 * static_cast<int64_t>(c.places);
+  c.places = c.tiles * p.pool.kv_heads * (c.steps + kPrefixCost);
+  c.saved = visit_ns(static_cast<int64_t>(pages) * count * p.pool.kv_heads, p.q_len * p.heads, p.head_dim) -
+            static_cast<int64_t>(c.places) * tile_ns(p.head_dim, p.fp16);
   return c;
 }
 
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) saved += __shfl_xor_sync(0xffffffffu, saved, o);
-  const bool pays = p.always || saved > kPrefixFixedNs;
+  const bool pays = p.always || saved > fixed_ns(p.head_dim);
   // The groups' places in the lists and in the line.
   int members = 0, units = 0, places = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
     int pages = pays && g < p.groups ? group_pages(p, g, count, any_s[g]) : 0;
     if (!p.always && group_cost(p, pages, count).saved <= 0) pages = 0;
     const GroupCost cost = group_cost(p, pages, count);
-    const int tiles = cost.tiles, steps = cost.steps, last = cost.last, n_units = tiles * p.pool.kv_heads, n_places = cost.places;
+    const int tiles = cost.tiles, steps = cost.steps, n_units = tiles * p.pool.kv_heads, n_places = cost.places;
     int m = count, u = n_units, x = n_places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
     }
     if (g < p.groups) {
       first_s[g] = members + m - count;
-      p.plan.groups[g] = PrefixGroup{pages, pages > 0, members + m - count, count, units + u - n_units, places + x - n_places, tiles, steps, last, {}};
+      p.plan.groups[g] = PrefixGroup{pages, pages > 0, members + m - count, count, units + u - n_units, places + x - n_places, tiles, steps};
     }
     members += __shfl_sync(0xffffffffu, m, 31);
     units += __shfl_sync(0xffffffffu, u, 31);
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(32) int4_prefix_plan_kernel(const __grid_const
   }
   if (lane == 0) {
     p.plan.head[0] = places;
-    p.plan.head[1] = max(2, (places + p.grid - 1) / p.grid);
+    p.plan.head[1] = max(1, (places + p.grid - 1) / p.grid);
   }
 }
 
@@ -201,9 +203,8 @@ struct Walk {
     group = PrefixGroup{};
   }
   __device__ __forceinline__ int group_end(const PrefixGroup& y) const {
-    return y.tiles > 0 ? y.places + kv_heads * prefix_head_places(y.tiles, y.steps, y.last) : y.places;
+    return y.places + y.tiles * kv_heads * (y.steps + kPrefixCost);
   }
-  // A step belongs to the range that its first place lies in.
   __device__ __forceinline__ bool next(Piece& piece) {
     while (at < end) {
       while (g < 0 || at >= group_end(group)) {
@@ -217,13 +218,11 @@ struct Walk {
           if (g0 >= groups) return false;
         }
       }
-      const int per_head = prefix_head_places(group.tiles, group.steps, group.last), in = at - group.places, h = in / per_head;
-      const int tile = min((in - h * per_head) / (2 * group.steps + kPrefixCost), group.tiles - 1), x = h * group.tiles + tile;
-      const int w = group.weight(x), start = group.start(x), unit_end = start + w * group.steps;
-      const int first = (max(at, start) - start + w - 1) / w, stop = min(group.steps, max(0, end - start + w - 1) / w);
-      at = min(end, unit_end);
+      const int span = group.steps + kPrefixCost, x = (at - group.places) / span, start = group.start(x);
+      const int first = max(at, start) - start, stop = min(end - start, group.steps);
+      at = min(end, start + group.steps);
       if (first >= stop) continue;
-      piece = Piece{g, h, tile, first, stop - first, group.units + x};
+      piece = Piece{g, x / group.tiles, x % group.tiles, first, stop - first, group.units + x};
       return true;
     }
     return false;
@@ -702,7 +701,7 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   LF_CHECK_ARG(a->groups >= 0 && (a->groups == 0 || (a->group && a->shared)), "lf_int4_attend_prefix: null pointer");
   LF_CHECK_SUPPORTED(a->groups <= kMaxGroups, "lf_int4_attend_prefix: %d groups (%d at most)", a->groups, kMaxGroups);
   const int columns = q.q_len * (q.n_q / q.pool.kv_heads);
-  const bool small = visit_ns(static_cast<int64_t>(q.pool.batch) * q.pool.kv_heads * q.pool.table_width, columns, q.head_dim) <= kPrefixFixedNs;
+  const bool small = visit_ns(static_cast<int64_t>(q.pool.batch) * q.pool.kv_heads * q.pool.table_width, columns, q.head_dim) <= fixed_ns(q.head_dim);
   if (a->groups == 0 || (small && !a->always)) return lf_int4_attend(&q, stream);
   PrefixParams p;
   const int ok = check_int4_pool("lf_int4_attend_prefix", q.pool, q.head_dim, p.pool);
@@ -719,12 +718,13 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   p.shared = a->shared;
   p.groups = a->groups;
   p.head_dim = q.head_dim;
+  p.fp16 = q.dtype == LF_F16;
   p.always = a->always;
   p.scale_log2 = q.scaling * 1.4426950408889634f;
   p.status = q.status;
   const int sms = sm_count();
   const int64_t records = most_records(p.pool.batch, p.pool.kv_heads, p.heads, p.q_len, p.groups, sms);
-  const int64_t steps = 2 * ((p.pool.table_width + 1) / 2) + kPrefixCost;
+  const int64_t steps = (p.pool.table_width + 1) / 2 + kPrefixCost;
   LF_CHECK_SUPPORTED(records <= (1 << 30) / steps && static_cast<int64_t>(p.pool.batch) * p.q_len * p.heads <= (1 << 30),
                      "lf_int4_attend_prefix: %d sequences of %d pages are too many for one call", p.pool.batch, p.pool.table_width);
   LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
