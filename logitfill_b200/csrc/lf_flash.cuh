@@ -106,18 +106,21 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
-// Wait of a whole warp for a barrier's phase, with a limit (of tries: reading a clock
-// between them costs more than the wait): false once a wait of this CTA has given up
-// (*stop), for all lanes alike.
-constexpr uint32_t kMostTries = 1u << 24;
-constexpr uint64_t kTileWaitNs = 2000000000ull;  // of the waits at a CTA's end
+// Wait of a whole warp for a barrier's phase, with a limit: false once a wait of this CTA
+// has given up (*stop), for all lanes alike.  The clock is read once in 1024 tries.
+constexpr uint64_t kTileWaitNs = 2000000000ull;
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
   bool ok = mbar_try_wait(bar, parity);
+  uint64_t since = 0;
   for (uint32_t n = 1; !ok; ++n) {
     ok = mbar_try_wait(bar, parity);
-    if ((n & 1023u) == 0u && !ok && (*stop != 0 || n >= kMostTries)) {
-      *stop = 1;
-      break;
+    if ((n & 1023u) == 0u && !ok) {
+      const uint64_t now = globaltimer_ns();
+      if (since == 0) since = now;
+      if (*stop != 0 || now - since > kTileWaitNs) {
+        *stop = 1;
+        break;
+      }
     }
   }
   return __all_sync(0xffffffffu, ok);
