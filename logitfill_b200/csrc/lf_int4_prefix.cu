@@ -18,8 +18,9 @@
 // fp16 enter exactly.  With an fp16 output, whose own rounding is as fine, Keys and weights
 // enter as sums of two fp16 numbers, in two products: error against 64 bits 0.00053 of the
 // result with one number each (0.0002 is the output's rounding alone), 0.00031 with two for
-// the Keys, 0.00028 with two for both.  A group whose numbers may pass the fp16 range (s 2^11 or |z| 2^15 at
-// least), or with a NaN, is not brought into it: the group of sequences is marked, and its
+// the Keys, 0.00028 with two for both.  Numbers that may pass the fp16 range (a scale of 2^11
+// or a minimum of 2^15 at least), a NaN, a page that is not in the pool, or scores too
+// large for the exponent are not done here: the group of sequences is marked, and its
 // members read these pages themselves, in the suffix kernel, which can do that.
 //
 // Order of channels.  A word's nibbles n and n + 4 lie in one fp16 pair (w >> 4 n) &
@@ -27,6 +28,20 @@
 // channels of a group of 8 as (0, 4), (1, 5), (2, 6), (3, 7).  For Value, the two are
 // channels 32 apart; the accumulators' columns come in the codes' order, and the record is
 // written in the channels'.
+//
+// Roles of the prefix kernel (28 warps, one CTA an SM): 16 softmax warps and one for the
+// products, as in lf_prompt.cu; one copies pages (cp.async.bulk, Keys and Values apart, the
+// ids of 32 pages at a time); 8 unpack them into swizzled fp16 tiles, K-major for Key and
+// MN-major for Value, 16 bytes a store without bank conflicts; one looks for parameters out
+// of range.
+//
+// What bounds it.  A chunk of 512 tokens behind 32768, 28 heads on 4, D 128, bf16: 285 us,
+// 851 TFLOP/s, 51 % of the measured 1680; 262 of it in the prefix kernel, 2.6 us a step of
+// 256 rows, where prompt attention's takes 2.0: the softmax warps share the issue slots
+// with the unpacking (48 % busy).  64 sequences behind 16384 tokens, 40 heads on 8: 76 us
+// (under the profiler: plan 6, prefix 56, suffix and merge 27); 320 rows to a KV head fill
+// a unit of 256 and a quarter of another.  The chunk took 424 us with four warps unpacking
+// and three tiles in the ring, 342 with eight warps, 285 with four tiles.
 #include <cmath>
 #include <type_traits>
 

@@ -16,7 +16,9 @@
 // thread, while the first loads are on their way, and handed over in shared memory: with
 // each thread working out its own, 16384 tokens of 32 heads, D 128, took 90 us (the
 // arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
-// token as it has heads, so that each makes one round of loads.
+// token as it has heads, so that each makes one round of loads.  16384 tokens of 32 heads, D
+// 128, bf16: 55 us replayed, 4.9 TB/s, 75 % of a plain copy's rate; 16 tokens: 5.3 us from
+// Python, the host's issue.
 #include <cmath>
 
 #include "lf_common.cuh"
