@@ -8,6 +8,7 @@
 
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
@@ -69,6 +70,14 @@ at::Tensor aligned_rows(at::Tensor t, int64_t (&s)[3]) {
   return t;
 }
 
+// Whether two tensors are known to share memory (strided views of one buffer whose gaps
+// hold the other are not: q and k of one projection).
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  const at::MemOverlapStatus s = at::get_overlap_status(x, y);
+  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+}
+
 // The device a call runs on made current, and its stream.
 struct Launch {
   c10::cuda::OptionalCUDAGuard guard;
@@ -109,6 +118,15 @@ int64_t integer(PyObject* o, const char* name) {
     fail(PyExc_TypeError, name, " must be an integer");
   }
   return v;
+}
+
+bool truth(PyObject* o, const char* name) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    fail(PyExc_TypeError, name, " must be true or false");
+  }
+  return v != 0;
 }
 
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {

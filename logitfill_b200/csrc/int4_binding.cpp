@@ -279,7 +279,7 @@ at::Tensor fill_out(lf_int4_query& a, const Pool& p, PyObject* out_o, const at::
 PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 8 && n != 12 && n != 13) expect(n, 12);
-    const bool sparse = n > 8, choose_only = n == 13 && PyObject_IsTrue(v[12]) == 1;
+    const bool sparse = n > 8, choose_only = n == 13 && truth(v[12], "choose_only");
     const Pool p = make_pool(v[1], v[2]);
     lf_int4_query a{};
     const at::Tensor q = fill_query(a, p, v[0], v[3], v[4], v[5], v[7]);
@@ -325,7 +325,7 @@ PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
     expect(n, 11);
     const Pool p = make_pool(v[1], v[2]);
     lf_int4_prefix a{};
-    a.always = PyObject_IsTrue(v[10]) == 1;
+    a.always = truth(v[10], "always");
     const at::Tensor q = fill_query(a.query, p, v[0], v[3], v[4], v[7], v[9]);
     a.group = per_sequence(v[5], "prefix_group", p, false);
     const at::Tensor& shared = tensor(v[6], "prefix_pages");
@@ -336,6 +336,8 @@ PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
     a.groups = static_cast<int32_t>(shared.size(0));
     const Launch on(p.device);
     at::Tensor out = fill_out(a.query, p, v[8], tensor(v[0], "query"));
+    if (at::has_internal_overlap(out) == at::MemOverlap::Yes) fail(PyExc_ValueError, "out overlaps itself");
+    if (overlap(out, q)) fail(PyExc_ValueError, "out shares memory with the query");
     const Scratch scratch = workspace(a.query, on), records = prefix_workspace(a.query, a.groups, on);
     a.query.workspace = scratch.words.data_ptr();
     a.query.workspace_bytes = scratch.bytes;

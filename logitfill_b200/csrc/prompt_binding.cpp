@@ -2,7 +2,6 @@
 // (Checks and errors as binding_common.h says; why they are compiled, int4_binding.cpp.)
 #include "binding_common.h"
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty_strided.h>
 
@@ -48,14 +47,6 @@ at::Tensor channels_last(const at::Tensor& t) {
 at::Tensor new_like(const at::Tensor& t) {
   if (t.is_non_overlapping_and_dense()) return at::empty_strided(t.sizes(), t.strides(), t.options());
   return at::empty(t.sizes(), t.options());
-}
-
-// Whether two tensors are known to share memory (strided views of one buffer whose gaps
-// hold the other are not: q and k of one projection).
-bool overlap(const at::Tensor& x, const at::Tensor& y) {
-  if (x.numel() == 0 || y.numel() == 0) return false;
-  const at::MemOverlapStatus s = at::get_overlap_status(x, y);
-  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
 }
 
 // out given by the caller for x: like it, and written once.
@@ -125,8 +116,8 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
       a.start = static_cast<const int32_t*>(at_.data_ptr());
     }
     a.magnitude = number(v[5], "magnitude");
-    a.interleaved = PyObject_IsTrue(v[6]) == 1;
-    a.transposed = PyObject_IsTrue(v[7]) == 1;
+    a.interleaved = truth(v[6], "interleaved");
+    a.transposed = truth(v[7], "transposed");
 
     const Launch on(query.device());
     const at::Tensor q = channels_last(query), k = with_key ? channels_last(key) : none;

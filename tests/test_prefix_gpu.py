@@ -357,7 +357,8 @@ def test_no_groups_and_refusals():
     for error, change in [(ValueError, dict(prefix_group=_i32([0]))), (ValueError, dict(prefix_group=_i32([0, 0]).long())),
                           (ValueError, dict(prefix_pages=_i32([[1]]))), (ValueError, dict(prefix_pages=_i32([1]).cpu())),
                           (TypeError, dict(prefix_pages=None)), (TypeError, dict(prefix_group=None)), (ValueError, dict(scaling=math.nan)),
-                          (ValueError, dict(query=q[:, :5])), (NotImplementedError, dict(query=q.float())),
+                          (ValueError, dict(out=q)), (ValueError, dict(out=q[:, :, :1])), (TypeError, dict(always=_i32([1, 2]))),
+                          (ValueError, dict(out=q[:1].expand(2, -1, -1, -1))), (ValueError, dict(query=q[:, :5])), (NotImplementedError, dict(query=q.float())),
                           (NotImplementedError, dict(prefix_pages=_i32([1] * 4097)))]:
         with pytest.raises(error):
             int4.int4_prefix_attention(**dict(args, **change))

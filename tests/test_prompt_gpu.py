@@ -91,6 +91,21 @@ def test_batches_and_starts(B, T, dtype):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,part,tokens,n_q,n_kv,dtype", [
+    (128, 128, 300, 28, 4, BF16), (128, 128, 1101, 40, 8, F16), (256, 256, 333, 17, 1, F32), (64, 32, 1500, 9, 0, BF16),
+    (80, 48, 999, 31, 2, F16), (256, 2, 200, 3, 1, BF16), (128, 64, 2049, 1, 3, F32)])
+def test_calls_that_fill_the_gpu(interleaved, D, part, tokens, n_q, n_kv, dtype):
+    """Blocks of both sizes, several heads to a thread, heads that are no multiple of those."""
+    g = torch.Generator().manual_seed(tokens)
+    q, k = (torch.randn(tokens, h, D, generator=g).to(dtype).cuda() for h in (n_q, n_kv))
+    at = torch.randint(0, 70000, (tokens,), generator=g)
+    freqs, _ = prompt.rotary_frequencies(part)
+    gq, gk = prompt.rotary_embed(q, k, freqs, positions=at.cuda(), interleaved=interleaved)
+    _check_turned(gq, q, at.tolist(), freqs, 1.0, interleaved)
+    _check_turned(gk, k, at.tolist(), freqs, 1.0, interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("D,part,shift", [(128, 128, 0), (64, 32, 0), (128, 128, 1), (96, 40, 3)])
 def test_in_place_and_unaligned(interleaved, D, part, shift):
     """Queries and Keys of one projection's buffer, at any element offset, turned where they lie."""
@@ -207,6 +222,7 @@ def test_rotary_refusals():
             (ValueError, (q, q, freqs), dict(start=start, out=(q, q))), (TypeError, (q, 3, freqs), ok),
             (ValueError, (q, k, freqs), dict(start=start, out=(torch.zeros(1, 8, 3, 64, dtype=BF16, device="cuda").expand(2, -1, -1, -1), k))),
             (NotImplementedError, (q.double(), None, freqs), ok), (RuntimeError, (q, k.cpu(), freqs), ok),
+            (TypeError, (q, k, freqs), dict(start=start, interleaved=start)), (TypeError, (q, k, freqs), dict(start=start, transposed=start)),
             (NotImplementedError, (q.float().requires_grad_(), None, freqs), ok)]:
         with pytest.raises(error):
             prompt.rotary_embed(*args, **kw)
