@@ -14,11 +14,11 @@
 // of its pairs (16 bytes of channels and their partners) in registers and walks over the
 // token's heads, four in flight.  The block's angles are worked out once, each by one
 // thread, while the first loads are on their way, and handed over in shared memory: with
-// each thread working out its own, 16384 tokens of 32 heads, D 128, took 90 us (the
-// arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
+// each thread working out its own, 16384 tokens of 32 heads, D 128, took 90 us in place of
+// 57 (the arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
 // token as it has heads, so that each makes one round of loads.  16384 tokens of 32 heads, D
-// 128, bf16: 55 us replayed, 4.9 TB/s, 75 % of a plain copy's rate; 16 tokens: 5.3 us from
-// Python, the host's issue.
+// 128, bf16: 46 us replayed, 5.9 TB/s, 90 % of a plain copy's rate (D 256: 6.3 TB/s; fp32: 6.4);
+// 16 tokens: 2.5 us replayed, 5.3 from Python, the host's issue.
 #include <cmath>
 
 #include "lf_common.cuh"
@@ -40,7 +40,14 @@ struct RotaryParams {
   int per_row, head_lanes, per_block;  // items of a head's row, threads to a token and item, tokens of a block
 };
 
-constexpr int kRotaryThreads = 256, kRotaryAhead = 4;
+constexpr int kRotaryAhead = 4;
+
+// Threads of a block.  In a large call small blocks wait less at their barrier for the angles:
+// 16384 tokens of 32 heads, D 128, bf16, take 46 us with 64 threads and 52 with 256, 600
+// tokens 3.5 and 4.9, 300 (a quarter of the GPU's threads) 3.2 with either.  A small call
+// wants a token's heads in one block: 16 tokens take 2.5 us with 256 threads and 2.9 with 64.
+// Rows of single elements (up to 255 items) need 256.  (Replayed 20 or 40 times in a graph.)
+constexpr int kSmallBlock = 64, kLargeBlock = 256;
 
 constexpr int64_t kRotaryFill = 148 * 2048;  // threads that a B200 holds at once
 
@@ -133,7 +140,7 @@ __device__ __forceinline__ void turn_adjacent(Pack<T, N>& x, const float (&c)[N 
 // part / 2 is the elements at 2 v and 2 v + 1.  The items behind them are vectors of
 // channels that are copied.
 template <typename T, int N, bool kAdjacent>
-__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kLargeBlock, 3) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr bool kInside = kAdjacent && N > 1;  // both channels of a pair in one vector
   constexpr int kPairs = kInside ? N / 2 : N;
   using Vec = Pack<T, N>;
@@ -183,9 +190,9 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_
 
   // The block's tokens' angles, each by one thread.  Pair i of item v lies at place i *
   // turning + v of its token, so that a warp's reads do not meet in a bank.
-  __shared__ float2 turn_s[kRotaryThreads * 8];
+  extern __shared__ float2 turn_s[];
   const int pairs = p.part / 2;
-  for (int x = threadIdx.x; x < p.per_block * pairs; x += kRotaryThreads) {
+  for (int x = threadIdx.x; x < p.per_block * pairs; x += blockDim.x) {
     const int which = x / pairs, pair = x - which * pairs;
     const int64_t tok = static_cast<int64_t>(blockIdx.x) * p.per_block + which;
     if (tok >= p.total) break;
@@ -307,11 +314,13 @@ extern "C" int lf_rotary_embed(const lf_rotary* a, lf_stream_t stream) {
 
   // Threads to a token and item: as many as there are heads in a small call (a thread makes
   // one round of loads), down to one for each kRotaryAhead heads once the threads fill the
-  // GPU.  16384 tokens, 32 heads: 57 us so, 59 with 8 heads to a thread, 61 with 16.
-  const int slots = kRotaryThreads / p.per_row;
+  // GPU.  16384 tokens, 32 heads, blocks of 256: 57 us so, 59 with 8 heads to a thread, 61
+  // with 16.
   int lanes_heads = p.heads;
   while (lanes_heads > 1 && static_cast<int64_t>(p.total) * p.per_row * lanes_heads > kRotaryFill && lanes_heads * kRotaryAhead > p.heads)
     lanes_heads = (lanes_heads + 1) / 2;
+  const bool large = static_cast<int64_t>(p.total) * p.per_row * p.heads > kRotaryFill / 4;
+  const int threads = wide && large ? kSmallBlock : kLargeBlock, slots = threads / p.per_row;
   p.head_lanes = lanes_heads < slots ? lanes_heads : slots;
   p.per_block = slots / p.head_lanes;
   const int64_t blocks = (p.total + p.per_block - 1) / p.per_block;
@@ -320,7 +329,8 @@ extern "C" int lf_rotary_embed(const lf_rotary* a, lf_stream_t stream) {
                      : a->dtype == LF_F16 ? rotary_kernel_of<__half>(a->interleaved != 0, wide)
                                           : rotary_kernel_of<__nv_bfloat16>(a->interleaved != 0, wide);
   void* args[] = {&p};
-  const cudaError_t err = launch_programmatic(kern, dim3(static_cast<unsigned>(blocks)), dim3(kRotaryThreads), 0,
+  const cudaError_t err = launch_programmatic(kern, dim3(static_cast<unsigned>(blocks)), dim3(threads),
+                                              static_cast<size_t>(p.per_block) * (p.part / 2) * sizeof(float2),
                                               reinterpret_cast<cudaStream_t>(stream), args);
   if (err != cudaSuccess) {
     set_error("lf_rotary_embed: %s", cudaGetErrorString(err));
