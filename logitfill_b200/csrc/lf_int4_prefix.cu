@@ -283,23 +283,21 @@ __device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t s2, uint32_t z
   codes_of(w, c);
   return make_uint4(hfma2_rn(c[0], s2, z2), hfma2_rn(c[1], s2, z2), hfma2_rn(c[2], s2, z2), hfma2_rn(c[3], s2, z2));
 }
-// The same as the sum of two fp16 numbers, of which this is the first (low: the second).
-// x = RN(code s) and r = code s - x, exact by an fma; a = RN(x + z) and what it leaves out,
-// exact by Knuth's two-sum; the second number is that and r, rounded.
-template <bool kLow> __device__ __forceinline__ uint4 unpack_word_exactly(uint32_t w, uint32_t s2, uint32_t z2) {
-  uint32_t c[4], y[4];
+// The same as the sum of two fp16 numbers.  x = RN(code s) and r = code s - x, exact by an
+// fma; a = RN(x + z) and what it leaves out, exact by Knuth's two-sum; the second number is
+// that and r, rounded.
+__device__ __forceinline__ void unpack_word_exactly(uint32_t w, uint32_t s2, uint32_t z2, uint4& high, uint4& low) {
+  uint32_t c[4], y[4], e[4];
   codes_of(w, c);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t x = hmul2_rn(c[k], s2), a = hadd2_rn(x, z2);
-    if constexpr (kLow) {
-      const uint32_t r = hfma2_rn(c[k], s2, x ^ 0x80008000u), b = hsub2_rn(a, x);
-      y[k] = hadd2_rn(hadd2_rn(hsub2_rn(x, hsub2_rn(a, b)), hsub2_rn(z2, b)), r);
-    } else {
-      y[k] = a;
-    }
+    const uint32_t x = hmul2_rn(c[k], s2), r = hfma2_rn(c[k], s2, x ^ 0x80008000u);
+    y[k] = hadd2_rn(x, z2);
+    const uint32_t b = hsub2_rn(y[k], x);
+    e[k] = hadd2_rn(hadd2_rn(hsub2_rn(x, hsub2_rn(y[k], b)), hsub2_rn(z2, b)), r);
   }
-  return make_uint4(y[0], y[1], y[2], y[3]);
+  high = make_uint4(y[0], y[1], y[2], y[3]);
+  low = make_uint4(e[0], e[1], e[2], e[3]);
 }
 // Non-zero in a sign's place where a scale is 2^11 at least, a minimum 2^15, or one is not finite.
 __device__ __forceinline__ uint32_t wide_bits(uint32_t sz) { return (sz & 0x7FFF7FFFu) + 0x08001800u; }
@@ -414,12 +412,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       for (int i = 0; ok && i < piece.n; ++i, ++n) {
         const int page = 2 * (piece.first + i);
 #pragma unroll 1
-        for (int kind = 0; kind < kLoads; ++kind) {  // the Key's terms, then Value
-          const bool value = kind == kLoads - 1;
-          const uint32_t load = kLoads * n + kind, slot = load % kSlots, unit = 2 * n + value, stage = unit % kStages;
+        for (int value = 0; value < 2; ++value) {  // the Key's terms, then Value
+          const uint32_t load = kLoads * n + (value ? kLoads - 1 : 0), slot = load % kSlots, unit = 2 * n + value, stage = unit % kStages;
+          const uint32_t next = (load + 1) % kSlots;  // of a Key's second term
           if (!(ok = wait(&sh.raw_full[stage], (unit / kStages) & 1))) break;
           if (load >= kSlots && !(ok = wait(&sh.kv_empty[slot], (load / kSlots - 1) & 1))) break;
-          uint8_t* tile = ring + slot * C::kTile;
+          if (kLoads == 3 && !value && load + 1 >= kSlots && !(ok = wait(&sh.kv_empty[next], ((load + 1) / kSlots - 1) & 1))) break;
+          uint8_t *tile = ring + slot * C::kTile, *second = ring + next * C::kTile;
 #pragma unroll
           for (int part = 0; part < 16 / kUnpackWarps; ++part) {
             // 8 tokens of a page at a time
@@ -436,15 +435,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
 #pragma unroll
               for (int G = 0; G < kG; ++G) {
                 const uint32_t s2 = __byte_perm(sz[G], 0, 0x1010), z2 = __byte_perm(sz[G], 0, 0x3232);
-                uint4 x = make_uint4(0, 0, 0, 0);
+                uint4 x = make_uint4(0, 0, 0, 0), y = x;
                 if (there) {
                   if constexpr (kLoads == 2)
                     x = unpack_word(code[G], s2, z2);
                   else
-                    x = kind == 0 ? unpack_word_exactly<false>(code[G], s2, z2) : unpack_word_exactly<true>(code[G], s2, z2);
+                    unpack_word_exactly(code[G], s2, z2, x, y);
                 }
-                const int chunk = 4 * (G & 1) + t;
-                *reinterpret_cast<uint4*>(tile + (G >> 1) * kHalfBytes + row * 128 + ((chunk ^ (row & 7)) << 4)) = x;
+                const int at = (G >> 1) * kHalfBytes + row * 128 + (((4 * (G & 1) + t) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(tile + at) = x;
+                if constexpr (kLoads == 3) *reinterpret_cast<uint4*>(second + at) = y;
               }
             } else {
               // Value: lane = (g, t), its words [token 2 t + o][w]: channels 64 w + 32 u + 4 g + n.
@@ -467,7 +467,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
           }
           fence_proxy_async_smem();
           arrive_once(&sh.kv_full[slot]);
-          if (kind >= kLoads - 2) arrive_once(&sh.raw_empty[stage]);  // the Key's last term, and Value
+          if (kLoads == 3 && !value) arrive_once(&sh.kv_full[next]);
+          arrive_once(&sh.raw_empty[stage]);
         }
       }
     }
