@@ -35,13 +35,16 @@
 // MN-major for Value, 16 bytes a store without bank conflicts; one looks for parameters out
 // of range.
 //
-// What bounds it.  A chunk of 512 tokens behind 32768, 28 heads on 4, D 128, bf16: 285 us,
-// 851 TFLOP/s, 51 % of the measured 1680; 262 of it in the prefix kernel, 2.6 us a step of
-// 256 rows, where prompt attention's takes 2.0: the softmax warps share the issue slots
-// with the unpacking (48 % busy).  64 sequences behind 16384 tokens, 40 heads on 8: 76 us
-// (under the profiler: plan 6, prefix 56, suffix and merge 27); 320 rows to a KV head fill
-// a unit of 256 and a quarter of another.  The chunk took 424 us with four warps unpacking
-// and three tiles in the ring, 342 with eight warps, 285 with four tiles.
+// What bounds it.  A chunk of 512 tokens behind 32768, 28 heads on 4, D 128, bf16: 281 us,
+// 864 TFLOP/s, 51 % of the measured 1680 (replayed; back to back 298).  A step takes 2.35 us
+// with 256 rows (1.2 of products), 1.98 with 128 and 1.86 with 32: with one tile the chain of
+// scores, softmax and outputs is not hidden, with two it is in part.  Unpacking is behind it:
+// half of it left out took 2.27 and 1.97.  (fp16 outputs: 4.6 and 3.5; with each term of a Key
+// unpacked in a pass of its own 5.4 and 4.1; D 64: 2.6 and 2.4, was 3.1 and 2.3.)  64 sequences
+// behind 16384 tokens, 40 heads on 8: 76 us (under the profiler: plan 6, prefix 56, suffix and
+// merge 27); 320 rows to a KV head fill a unit of 256 and a quarter of another.  The chunk
+// took 424 us with four warps unpacking and three tiles in the ring, 342 with eight warps, 285
+// with four tiles.
 #include <cmath>
 #include <type_traits>
 
@@ -71,17 +74,17 @@ constexpr int kMaxGroups = 4096;
 // Whether the shared pages are read once, or by each sequence as lf_int4_attend does, is a
 // matter of sizes.  In ns on a B200: a page costs lf_int4_attend's kernel about 2 for up to 8
 // query columns and 2.9 for 16 (D 128; half at D 64), every time it is read; a Key tile of a
-// unit costs 16 here, 30 with the two terms of fp16 (D 64: 11 and 16), and the two kernels
+// unit costs 16 here, 23 with the two terms of fp16 (D 64: 11 and 16), and the two kernels
 // more and the records 17000 (D 64: 12500).  Measured in us, that kernel / these three,
 // replayed.  28 heads on 4, D 128, bf16, one token each: 8192 shared tokens, 16 sequences
 // 25 / 30, 32 sequences 41 / 37; 32768 tokens, 4 sequences 28 / 37, 8: 41 / 39, 16: 69 / 41,
 // 32: 127 / 54.  40 heads on 8: 8192 tokens, 8 sequences 25 / 28, 16: 41 / 29; 32768 tokens, 4
-// sequences 41 / 48, 8: 69 / 48; fp16, 8: 75 / 81, 16: 140 / 82.  One sequence behind 32768
+// sequences 41 / 48, 8: 69 / 48; fp16, 8: 75 / 69, 16: 140 / 72.  One sequence behind 32768
 // tokens, 28 heads on 4, bf16: 8 query tokens 37 / 45, 16: 50 / 48, 32: 85 / 56, 128: 298 / 124.
 __host__ __device__ __forceinline__ int64_t visit_ns(int64_t pages, int columns, int head_dim) {
   return pages * ((columns + 15) / 16) * (columns <= 8 ? 20 : 29) * head_dim / 1280;
 }
-__host__ __device__ __forceinline__ int tile_ns(int head_dim, bool fp16) { return head_dim == 128 ? (fp16 ? 30 : 16) : (fp16 ? 16 : 11); }
+__host__ __device__ __forceinline__ int tile_ns(int head_dim, bool fp16) { return head_dim == 128 ? (fp16 ? 23 : 16) : (fp16 ? 16 : 11); }
 __host__ __device__ __forceinline__ int64_t fixed_ns(int head_dim) { return head_dim == 128 ? 17000 : 12500; }
 
 // Shared pages of group g that its `count` members (one of them `any`) have.
