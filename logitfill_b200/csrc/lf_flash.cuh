@@ -210,7 +210,9 @@ struct Pair {
     return wait(met, phase++ & 1);
   }
   // The next exchange may begin once the other thread has read this one's number: after
-  // another meeting, or a barrier that it arrives at later.
+  // another meeting, or a barrier that it arrives at later.  (The next step's scores are
+  // such a barrier, and the last step's outputs: both come behind the weights of all 8 warps,
+  // which each hands over behind its read.)
   template <typename Wait>
   __device__ __forceinline__ bool exchange(float x, float& y, Wait&& wait) {
     *const_cast<volatile float*>(mine) = x;
@@ -361,7 +363,8 @@ __device__ __forceinline__ bool soften_tile(uint32_t tmem_s, uint32_t tmem_o, in
   return true;
 }
 
-// The row's sum, of both its threads' (the next exchange may follow at once).
+// The row's sum, of both its threads': called once the row's outputs are done, which keeps it
+// behind the last step's exchange.  (The next exchange may follow at once.)
 template <typename Wait>
 __device__ __forceinline__ bool join_sums(RowState& st, Pair& pair, Wait&& wait) {
   float other;

@@ -645,8 +645,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
           break;
       }
       if (__any_sync(0xffffffffu, st.large && row < rows) && lane == 0) p.plan.groups[piece.g].live = 0;
-      if (!ok || !(ok = join_sums(st, pair, wait))) break;
-      if (!(ok = wait(&sh.o_done[t], pieces++ & 1))) break;
+      if (!ok || !(ok = wait(&sh.o_done[t], pieces++ & 1))) break;
+      if (!(ok = join_sums(st, pair, wait))) break;
       tc_fence_after();
       // ---- its record
       float* rec = p.plan.records + (piece.unit + static_cast<int64_t>(blockIdx.x)) * prefix_record(D);

@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       T* out = static_cast<T*>(p.out) + it.b * p.o_seq + (static_cast<int64_t>(it.first) + token) * p.o_tok +
                (it.h * p.group + head) * p.o_head + D / 2 * half;
       if (steps > 0) {
-        if (!(ok = join_sums(st, pair, wait))) break;
         if (!(ok = wait(&sh.o_done[t], items++ & 1))) break;
+        if (!(ok = join_sums(st, pair, wait))) break;
         tc_fence_after();
       }
       if (steps > 0 && (*const_cast<volatile int*>(&sh.bad[n & 1]) != 0 || __any_sync(0xffffffffu, st.large && stored && token < it.tokens))) {
