@@ -406,11 +406,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
     }
     if (ok && step > 0 && *stop == 0 && output(0)) output(1);  // the last step's
-    if (*stop != 0) {  // the products in flight, before their operands go
-      if (elect_one()) mma_commit(&sh.last);
-      __syncwarp();
-      mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
-    }
   } else if (warp < kMmaWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
     more_registers<kSoftmaxRegs>();
@@ -496,6 +491,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
+    if (sh.stop != 0) {  // a wait gave up, of any role: products may be in flight, and end before their operands go
+      if (elect_one()) mma_commit(&sh.last);
+      __syncwarp();
+      mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
+    }
     tmem_dealloc(tmem, 512);
   }
   if (threadIdx.x == 0 && sh.stop != 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_DEVICE_TIMEOUT);

@@ -1,5 +1,6 @@
 """CPU model of what the two threads of a row of scores tell one another in the tensor-core
-attention kernels: every interleaving of both, over the steps that their source has.
+attention kernels: every interleaving of both, over the steps that their source has; and the
+order in which a CTA of theirs ends.
 
 A row's threads exchange numbers by way of one slot each.  The order of writes, meetings,
 reads and of the waits between them is read from the sources (lf_flash.cuh, lf_prompt.cu,
@@ -110,3 +111,14 @@ def test_the_model_finds_an_exchange_that_waits_for_nothing():
     step = ["scores", "write", "arrive", "await", "read", "ready"]
     assert _stale_read(step + ["write", "arrive", "await", "read", "outputs"]) == (4, 1, 2)
     assert _stale_read(step + ["outputs", "write", "arrive", "await", "read"]) is None
+
+
+@pytest.mark.parametrize("kernel", ["lf_prompt.cu", "lf_int4_prefix.cu"])
+def test_products_in_flight_end_before_the_cta(kernel):
+    """Any role may give up while products run whose end only the softmax would have waited for: what decides
+    whether they are waited for is read when no role can give up any more, before tensor memory goes."""
+    text = _code((CSRC / kernel).read_text())
+    joined = text.rindex("__syncthreads();")
+    asked, committed, gone = text.rindex("if (sh.stop != 0)", 0, text.rindex("tmem_dealloc")), text.index("mma_commit(&sh.last)"), text.rindex("tmem_dealloc")
+    assert text.count("mma_commit(&sh.last)") == 1
+    assert joined < asked < committed < text.index("mbar_wait_bounded(&sh.last", committed) < gone
