@@ -129,8 +129,9 @@ def _make_forward(adapter: "DeepSeekQwenKVAdapter", layer_idx: int):
     return forward
 
 
-def _prompt_attention(attn, query, key, value, attention_mask, kwargs):
-    """The first prefill by the prompt kernel; returns ``[B, q_len, heads, D]``."""
+def _prompt_attention(attn, manager, query, key, value, attention_mask):
+    """The first prefill by the prompt kernel, which reports to the cache's status word
+    (``check_status``); returns ``[B, q_len, heads, D]``."""
     from logitfill_b200.prompt import prompt_attention
 
     if attention_mask is not None:
@@ -138,7 +139,9 @@ def _prompt_attention(attn, query, key, value, attention_mask, kwargs):
                                   "(attn_implementation='sdpa' builds none for them)")
     if _sliding_window(attn) is not None or (attn.training and attn.attention_dropout):
         raise NotImplementedError("prompt='kernel' has neither a sliding window nor dropout")
-    return prompt_attention(query, key, value, attn.scaling).transpose(1, 2)
+    if not query.is_cuda:
+        raise RuntimeError("prompt='kernel' needs a model on the GPU (there is no CPU path)")
+    return prompt_attention(query, key, value, attn.scaling, status=manager.cache.status).transpose(1, 2)
 
 
 def _packed_branch(attn, adapter, layer_idx, query, key, value, attention_mask, cache, kwargs):
@@ -148,8 +151,10 @@ def _packed_branch(attn, adapter, layer_idx, query, key, value, attention_mask, 
     if past == 0 and layer_idx == 0:
         manager.reset()
     if past == 0:
-        first = _prompt_attention if adapter.prompt == "kernel" else _dense_attention
-        out = first(attn, query, key, value, attention_mask, kwargs)
+        if adapter.prompt == "kernel":
+            out = _prompt_attention(attn, manager, query, key, value, attention_mask)
+        else:
+            out = _dense_attention(attn, query, key, value, attention_mask, kwargs)
     else:
         if layer_idx == 0 and cache is not None and not isinstance(cache, LogitFillCache):
             seen = int(cache.get_seq_length()) if hasattr(cache, "get_seq_length") else -1
