@@ -270,6 +270,14 @@ LF_API int lf_decode_noalloc(const lf_layout* layout, const int32_t* rows, const
 LF_API int lf_selftest_wait(int32_t* status, int64_t limit_ns, int arrive, lf_stream_t stream);
 
 /*
+ * The same of the wait of the tensor-core attention kernels, whose limit is on a time in
+ * which nothing moves: a second warp works for busy_ns, which it shows, then arrives or not.
+ * *status becomes LF_OK where the wait ends by the arrival, LF_ERR_DEVICE_TIMEOUT where it
+ * gives up and a second wait of the CTA does so too.  Limit and work of 1 s at most.
+ */
+LF_API int lf_selftest_tile_wait(int32_t* status, int64_t limit_ns, int64_t busy_ns, int arrive, lf_stream_t stream);
+
+/*
  * Self-test of K1's per-element arithmetic (no counterpart in the reference;
  * it checks the restatement of layout.py:12-18).  For i < n (device arrays):
  * quotient[i] = (x[i] - lo[i]) / scale[i] as K1 computes it (IEEE subtract,

@@ -18,7 +18,7 @@ LF_F32, LF_F16, LF_BF16 = 0, 1, 2
 EXPORTS = (
     "lf_layout_init", "lf_pack_pages", "lf_dequantize", "lf_decode_workspace_bytes",
     "lf_decode_max_splits", "lf_decode_occupancy", "lf_decode_partial", "lf_decode_noalloc", "lf_decode_merge",
-    "lf_decode", "lf_decode_multi", "lf_decode_max_splits_multi", "lf_commit_token", "lf_selftest_wait", "lf_selftest_divide",
+    "lf_decode", "lf_decode_multi", "lf_decode_max_splits_multi", "lf_commit_token", "lf_selftest_wait", "lf_selftest_tile_wait", "lf_selftest_divide",
     "lf_ipc_alloc", "lf_ipc_free", "lf_ipc_handle", "lf_ipc_open", "lf_ipc_close", "lf_decode_merge_gather",
     "lf_gather_signals", "lf_gather_wait", "lf_int4_write", "lf_int4_read", "lf_int4_read_bounds", "lf_int4_select",
     "lf_int4_attend", "lf_int4_attend_sparse", "lf_int4_attend_prefix", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from",
@@ -77,6 +77,7 @@ def lib() -> ctypes.CDLL:
         "lf_commit_token": (c_int, [L, P, P, P, P, P, c_int64, c_int64, P, P, c_int, P, P, c_int64, c_int64, c_int,
                                     P, P, P]),
         "lf_selftest_wait": (c_int, [P, c_int64, c_int, P]),
+        "lf_selftest_tile_wait": (c_int, [P, c_int64, c_int64, c_int, P]),
         "lf_selftest_divide": (c_int, [P, P, P, c_int64, c_int, P, P, P]),
         "lf_ipc_alloc": (c_int, [c_size_t, P]),
         "lf_ipc_free": (c_int, [P]),

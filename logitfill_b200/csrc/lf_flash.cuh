@@ -106,19 +106,29 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// How the waits of a CTA end before their time, in its shared memory.
+struct Waits {
+  int stop;        // one gave up
+  uint32_t moves;  // counts up while a role is at work that others wait for, however long it takes
+};
 // Wait of a whole warp for a barrier's phase, with a limit: false once a wait of this CTA
-// has given up (*stop), for all lanes alike.  The clock is read once in 1024 tries.
+// has given up, for all lanes alike.  The limit is on a time in which nothing moves: work
+// that may take longer (prompt_row's) counts up Waits::moves.  The clock is read once in
+// 1024 tries.
 constexpr uint64_t kTileWaitNs = 2000000000ull;
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile Waits* waits, uint64_t limit_ns = kTileWaitNs) {
   bool ok = mbar_try_wait(bar, parity);
   uint64_t since = 0;
+  uint32_t moves = 0;
   for (uint32_t n = 1; !ok; ++n) {
     ok = mbar_try_wait(bar, parity);
     if ((n & 1023u) == 0u && !ok) {
       const uint64_t now = globaltimer_ns();
-      if (since == 0) since = now;
-      if (*stop != 0 || now - since > kTileWaitNs) {
-        *stop = 1;
+      const uint32_t seen = waits->moves;
+      if (since == 0 || seen != moves) since = now;
+      moves = seen;
+      if (waits->stop != 0 || now - since > limit_ns) {
+        waits->stop = 1;
         break;
       }
     }

@@ -201,7 +201,7 @@ constexpr float kNoScore = -3e38f;  // the maximum of a row that sees nothing: b
 
 struct PrefixShared {
   uint64_t raw_full[8], raw_empty[8], kv_full[8], kv_empty[8], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2], last;
-  int stop;
+  Waits waits;
   uint32_t tmem;
   float told[2][2][128];  // between the two threads of a row
 };
@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
       mbar_init(&sh.o_done[t], 1);
     }
     mbar_init(&sh.last, 1);
-    sh.stop = 0;
+    sh.waits.stop = 0;
+    sh.waits.moves = 0;
     fence_mbar_init();
   }
   tc_fence_before();
@@ -359,8 +360,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   grid_dep_trigger();  // all CTAs of this grid run at once, so the suffix kernel's take nothing that one needs
   grid_dep_wait();
 
-  volatile int* stop = &sh.stop;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, stop); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, &sh.waits); };
   const int per_member = p.q_len * p.heads;
 
   if (warp == kCopyWarp) {
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
         ends = i == piece.n - 1;
       }
     }
-    if (ok && step > 0 && *stop == 0 && output(0)) output(1);  // the last step's
+    if (ok && step > 0 && *const_cast<volatile int*>(&sh.waits.stop) == 0 && output(0)) output(1);  // the last step's
   } else if (warp < kUnpackWarp) {
     // ---------------------------------------------------------------- softmax, one tile a warpgroup
     more_registers<kRowRegs>();
@@ -677,14 +677,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   __syncthreads();
   if (warp == kProductWarp) {
     tc_fence_after();
-    if (sh.stop != 0) {  // a wait gave up, of any role: products may be in flight, and end before their operands go
+    if (sh.waits.stop != 0) {  // a wait gave up, of any role: products may be in flight, and end before their operands go
       if (elect_one()) mma_commit(&sh.last);
       __syncwarp();
       mbar_wait_bounded(&sh.last, 0, kTileWaitNs);
     }
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && sh.stop != 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_DEVICE_TIMEOUT);
+  if (threadIdx.x == 0 && sh.waits.stop != 0 && p.status != nullptr) atomicExch(p.status, LF_ERR_DEVICE_TIMEOUT);
 }
 
 // ------------------------------------------------------------------- host

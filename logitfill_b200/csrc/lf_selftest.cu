@@ -5,7 +5,7 @@
 // LF_ERR_DEVICE_TIMEOUT in the status word and returns: the failure path is
 // exercised with no fault, trap or hang, and the context stays usable.
 #include "lf_common.cuh"
-#include "lf_tcgen05.cuh"
+#include "lf_flash.cuh"
 
 namespace lf {
 
@@ -28,6 +28,47 @@ extern "C" int lf_selftest_wait(int32_t* status, int64_t limit_ns, int arrive, l
   lf::selftest_wait_kernel<<<1, 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       status, static_cast<uint64_t>(limit_ns), arrive);
   return lf::launch_status("lf_selftest_wait");
+}
+
+// The same of the wait of the tensor-core attention kernels (warp_wait).  One warp waits; the
+// other counts up Waits::moves for busy_ns, then arrives on the barrier or not.  Their limit
+// is on a time in which nothing moves.
+namespace lf {
+
+__global__ void selftest_tile_wait_kernel(int32_t* status, uint64_t limit_ns, uint64_t busy_ns, int arrive) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ sm100::Waits waits;
+  if (threadIdx.x == 0) {
+    sm100::mbar_init(&bar, 1);
+    sm100::fence_mbar_init();
+    waits.stop = 0;
+    waits.moves = 0;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const bool done = sm100::warp_wait(&bar, 0, &waits, limit_ns);
+    // (a wait that gives up ends all others of its CTA as well)
+    const bool again = sm100::warp_wait(&bar, 0, &waits, limit_ns);
+    if (threadIdx.x == 0) *status = done && again && waits.stop == 0 ? LF_OK : !done && !again && waits.stop == 1 ? LF_ERR_DEVICE_TIMEOUT : -1;
+  } else if (threadIdx.x == 32) {
+    const uint64_t since = sm100::globaltimer_ns();
+    for (uint32_t n = 0; n < (1u << 27) && sm100::globaltimer_ns() - since < busy_ns; ++n) {
+      if ((n & 1023u) == 0u) atomicAdd(&waits.moves, 1u);
+    }
+    if (arrive) sm100::mbar_arrive(&bar);
+  }
+}
+
+}  // namespace lf
+
+extern "C" int lf_selftest_tile_wait(int32_t* status, int64_t limit_ns, int64_t busy_ns, int arrive, lf_stream_t stream) {
+  LF_CHECK_ARG(status != nullptr, "lf_selftest_tile_wait: null status");
+  LF_CHECK_ARG(limit_ns > 0 && limit_ns <= 1000000000LL && busy_ns >= 0 && busy_ns <= 1000000000LL,
+               "lf_selftest_tile_wait: limit %lld ns and work of %lld ns (1 s at most)", static_cast<long long>(limit_ns),
+               static_cast<long long>(busy_ns));
+  lf::selftest_tile_wait_kernel<<<1, 64, 0, reinterpret_cast<cudaStream_t>(stream)>>>(status, static_cast<uint64_t>(limit_ns),
+                                                                                     static_cast<uint64_t>(busy_ns), arrive);
+  return lf::launch_status("lf_selftest_tile_wait");
 }
 
 // Self-test of K1's per-element division: for each (x, lo, scale) triple the

@@ -3,6 +3,8 @@ limit of their waits, how it is reported, and what must not reach it.  No test f
 hangs the GPU: a wait runs out on a flag that nothing sets, and the kernel returns."""
 from __future__ import annotations
 
+import time
+
 import pytest
 import torch
 
@@ -39,3 +41,51 @@ def test_the_adapter_reports_a_prefill_that_gave_up(monkeypatch):
     with pytest.raises(RuntimeError, match="timed out"):
         a.packed_manager().cache.check_status()
     a.detach()
+
+
+MS = 1_000_000
+
+
+def _tile_wait(limit_ns, busy_ns, arrive):
+    status = torch.full((1,), 77, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    since = time.perf_counter()
+    _lib.check(_lib.lib().lf_selftest_tile_wait(_lib.ptr(status), limit_ns, busy_ns, int(arrive), _lib.stream_handle(status.device)),
+               "lf_selftest_tile_wait")
+    torch.cuda.synchronize()
+    return int(status), time.perf_counter() - since
+
+
+@pytest.mark.parametrize("limit,busy,arrive,want", [(50 * MS, 0, True, "LF_OK"), (20 * MS, 0, False, "LF_ERR_DEVICE_TIMEOUT"),
+                                                    (10 * MS, 200 * MS, True, "LF_OK"), (10 * MS, 100 * MS, False, "LF_ERR_DEVICE_TIMEOUT")])
+def test_the_limit_is_on_a_time_in_which_nothing_moves(limit, busy, arrive, want):
+    status, took = _tile_wait(limit, busy, arrive)
+    assert status == getattr(_lib, want)
+    assert took >= (busy if arrive else busy + limit) * 1e-9 and took < 3.0
+    # the context is as good as before
+    assert float(torch.ones(8, device="cuda").sum()) == 8.0
+
+
+def test_rows_that_take_longer_than_the_limit():
+    """A Value that not all rows of a tile may see is NaN: its rows are done one by one, 16 to a warp over all Keys,
+    which takes seconds here.  The roles that wait meanwhile do not give up."""
+    n, D = 3 << 18, 64
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q, k, v = (torch.randn(n, 1, D, generator=g, device="cuda").to(BF16) for _ in range(3))
+    v += 2.0                                             # (results of 2, not of the small mean of many signs)
+    v[n - 1] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    prompt.prompt_attention(q, k, v, 0.125, out=out, status=status)
+    assert int(status) == _lib.LF_OK
+    assert bool(out[n - 1].isnan().all()) and bool(torch.isfinite(out[:n - 1]).all())
+    assert not bool((out == 7.0).all(-1).any())          # every row was written
+    u = 2.0 ** -8
+    for i in (0, 129, 200001, n - 257, n - 256, n - 129, n - 128, n - 2):
+        a, b, c = q[i, 0].double(), k[:i + 1, 0].double(), v[:i + 1, 0].double()
+        p = torch.softmax(b @ a * 0.125, 0)
+        # the bound of the operator's own tests; n 2^-30 for fp32 sums of n terms, whose roundings go both ways
+        # (some sqrt(n) 2^-24 of the sum, far less)
+        e = float((b.abs() @ a.abs()).max()) * 0.125 * D * 2.0 ** -24
+        bound = u * (p @ c).abs() + (u + 2 * e + 2.0 ** -16 + n * 2.0 ** -30) * (p @ c.abs()) + 2.0 ** -24
+        assert bool(((out[i, 0].double() - p @ c).abs() <= bound).all()), i

@@ -119,6 +119,7 @@ def test_products_in_flight_end_before_the_cta(kernel):
     whether they are waited for is read when no role can give up any more, before tensor memory goes."""
     text = _code((CSRC / kernel).read_text())
     joined = text.rindex("__syncthreads();")
-    asked, committed, gone = text.rindex("if (sh.stop != 0)", 0, text.rindex("tmem_dealloc")), text.index("mma_commit(&sh.last)"), text.rindex("tmem_dealloc")
+    committed, gone = text.index("mma_commit(&sh.last)"), text.rindex("tmem_dealloc")
+    asked = [m.start() for m in re.finditer(r"if \(sh\.[\w.]*stop != 0\)", text[:committed])][-1]
     assert text.count("mma_commit(&sh.last)") == 1
     assert joined < asked < committed < text.index("mbar_wait_bounded(&sh.last", committed) < gone
