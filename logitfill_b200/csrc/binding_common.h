@@ -10,8 +10,10 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -46,6 +48,15 @@ std::string shape(const at::Tensor& t) {
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) fail(PyExc_TypeError, name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
   return THPVariable_Unpack(o);
+}
+
+// For operators that record no gradient, of either direction: a result that silently dropped
+// it would be wrong.
+[[maybe_unused]] void no_gradient(const at::Tensor& t, const char* what) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    fail(PyExc_NotImplementedError, what, " requires a gradient, which this operator does not record: call it under torch.no_grad()");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    fail(PyExc_NotImplementedError, what, " has a forward-mode tangent, which this operator does not carry on");
 }
 
 int type_code(at::ScalarType t) {

@@ -323,6 +323,8 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
 PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect(n, 11);
+    no_gradient(tensor(v[0], "query"), "query");
+    if (v[8] != Py_None) no_gradient(tensor(v[8], "out"), "out");
     const Pool p = make_pool(v[1], v[2]);
     lf_int4_prefix a{};
     a.always = truth(v[10], "always");

@@ -2,7 +2,6 @@
 // (Checks and errors as binding_common.h says; why they are compiled, int4_binding.cpp.)
 #include "binding_common.h"
 
-#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty_strided.h>
 
 #include <cmath>
@@ -16,13 +15,6 @@ float number(PyObject* o, const char* name) {
     fail(PyExc_TypeError, name, " must be a number");
   }
   return static_cast<float>(v);
-}
-
-// The operators have no backward pass of their own: a result that silently dropped its
-// gradient would be wrong.
-void no_gradient(const at::Tensor& t, const char* what) {
-  if (t.requires_grad() && at::GradMode::is_enabled())
-    fail(PyExc_NotImplementedError, what, " requires a gradient, which this operator does not record: call it under torch.no_grad()");
 }
 
 // A tensor's strides over (sequence, head, token), 0 where the extent is 1: [batch, heads,
@@ -82,6 +74,9 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
       no_gradient(key, "key");
     }
     no_gradient(query, "query");
+    if (v[8] != Py_None && PyTuple_Check(v[8]))
+      for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(v[8]); ++i)
+        if (PyObject* o = PyTuple_GET_ITEM(v[8], i); o != Py_None) no_gradient(tensor(o, "out"), "out");
     if (!query.is_cuda()) fail(PyExc_RuntimeError, "rotary_embed needs CUDA tensors (there is no CPU path)");
     if (freqs.dim() != 1 || freqs.scalar_type() != at::kLong || !freqs.is_contiguous() || freqs.size(0) < 1 || 2 * freqs.size(0) > D ||
         freqs.device() != query.device())
@@ -190,12 +185,13 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (nq < 1 || nkv < 1 || nq % nkv) fail(PyExc_ValueError, nq, " query heads do not divide into ", nkv, " KV heads");
     if (query.scalar_type() != at::kHalf && query.scalar_type() != at::kBFloat16)
       fail(PyExc_NotImplementedError, "prompt attention takes fp16 or bf16, got ", c10::toString(query.scalar_type()));
-    if (!query.is_cuda()) fail(PyExc_RuntimeError, "prompt_attention needs CUDA tensors (there is no CPU path)");
-    if (key.device() != query.device() || value.device() != query.device())
-      fail(PyExc_RuntimeError, "key and value must be on ", query.device());
     no_gradient(query, "query");
     no_gradient(key, "key");
     no_gradient(value, "value");
+    if (v[6] != Py_None) no_gradient(tensor(v[6], "out"), "out");
+    if (!query.is_cuda()) fail(PyExc_RuntimeError, "prompt_attention needs CUDA tensors (there is no CPU path)");
+    if (key.device() != query.device() || value.device() != query.device())
+      fail(PyExc_RuntimeError, "key and value must be on ", query.device());
     for (const int64_t x : {query.size(0), T, nq, D})
       if (x > INT32_MAX) fail(PyExc_NotImplementedError, "an extent of ", x, " is too large");
     lf_prompt a{};

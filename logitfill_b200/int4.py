@@ -140,7 +140,8 @@ def int4_prefix_attention(query: torch.Tensor, pages: torch.Tensor, page_table: 
     its lowest sequence are read.  Both are read on the GPU.  The result is
     :func:`int4_attention`'s up to the order of sums, for any lengths.  Where few
     sequences share few pages, each reads them itself, which is faster then
-    (``always``: never)."""
+    (``always``: never).  No gradient is recorded: a query that requires one, or
+    has a forward-mode tangent, raises ``NotImplementedError``."""
     return _lib.int4_binding().attend_prefix(query, pages, page_table, lengths, scaling, prefix_group, prefix_pages, counts, out,
                                              status, always)
 

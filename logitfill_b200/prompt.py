@@ -10,9 +10,9 @@ whole prompts in their original type, which both caches leave to their caller
 
 Tensors are ``[batch, heads, tokens, head_dim]``, or packed ``[tokens, heads,
 head_dim]``: the tokens of all sequences behind one another.  Every launch goes
-to the current stream.  There is no CPU or dense fallback and no backward pass;
-what the kernels do not implement raises ``NotImplementedError``, malformed
-arguments ``ValueError``.
+to the current stream.  There is no CPU or dense fallback and no backward pass
+(a tensor that requires a gradient, or has a forward-mode tangent, is refused); what the
+kernels do not implement raises ``NotImplementedError``, malformed arguments ``ValueError``.
 """
 from __future__ import annotations
 

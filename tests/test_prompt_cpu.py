@@ -190,6 +190,39 @@ def test_functions_refuse_cpu_tensors():
         int4.int4_prefix_attention(q[:1], torch.zeros(4, 2, 1280, dtype=torch.int32), torch.zeros(1, 2, dtype=torch.int32), n, 1.0, n, n)
 
 
+def test_gradients_are_refused():
+    """None of the three records a gradient, of either direction: dropping one silently would be wrong."""
+    from torch.autograd import forward_ad
+
+    q, k = torch.zeros(4, 8, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    freqs, _ = prompt.rotary_frequencies(64, device="cpu")
+    n, table, pages = torch.zeros(4, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2, 1280, dtype=torch.int32)
+    calls = {
+        "rotary query": lambda x: prompt.rotary_embed(x, k, freqs, positions=torch.arange(4)),
+        "rotary key": lambda x: prompt.rotary_embed(k, x, freqs, positions=torch.arange(4)),
+        "rotary out": lambda x: prompt.rotary_embed(q, None, freqs, positions=torch.arange(4), out=(x, None)),
+        "prompt query": lambda x: prompt.prompt_attention(x, k, k, 0.125),
+        "prompt key": lambda x: prompt.prompt_attention(q, x, q, 0.125),
+        "prompt value": lambda x: prompt.prompt_attention(q, q, x, 0.125),
+        "prompt out": lambda x: prompt.prompt_attention(q, k, k, 0.125, out=x),
+        "prefix query": lambda x: int4.int4_prefix_attention(x, pages, table, n, 1.0, n, n),
+        "prefix out": lambda x: int4.int4_prefix_attention(q, pages, table, n, 1.0, n, n, out=x),
+    }
+    for name, call in calls.items():
+        with pytest.raises(NotImplementedError, match="gradient"):
+            call(q.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call(q.clone().requires_grad_())
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(q.clone(), torch.ones_like(q))
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):     # (no_grad does not end this mode)
+                call(dual)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(q.clone())
+
+
 # ------------------------------------------------------------ shared pages in the cache
 
 @pytest.fixture
