@@ -191,6 +191,7 @@ class Int4KVCache:
         self._step = 0                                            # tokens of the step, at most
         self._free = list(range(n_pages - 1, -1, -1))
         self._refs = np.zeros(n_pages, np.int64)                  # sequences that hold each page
+        self._common = np.zeros(batch, np.int64)                  # first pages of each that others hold too
         self.prefix_group = torch.arange(batch, dtype=torch.int32, device=self.device)   # for int4_prefix_attention
         self.prefix_pages = torch.zeros(batch, dtype=torch.int32, device=self.device)
 
@@ -263,9 +264,9 @@ class Int4KVCache:
         n = np.broadcast_to(np.asarray(lengths, np.int64), (self.batch,))
         if (n < 0).any() or (n > self._end).any():
             raise ValueError("truncate() takes lengths between 0 and the present ones")
-        for b in range(self.batch):   # what comes next would be written over these
-            if (self._refs[self._table[b, int(n[b]) // PAGE_TOKENS:int(self._owned[b])]] > 1).any():
-                raise ValueError(f"sequence {b} shares pages past token {int(n[b])}")
+        cut = np.flatnonzero(n // PAGE_TOKENS < self._common)   # what comes next would be written over these
+        if len(cut):
+            raise ValueError(f"sequence {cut[0]} shares pages past token {int(n[cut[0]])}")
         self._start, self._end, self._step = n.copy(), n.copy(), 0
         self._upload(self._spans, np.stack([self._start, self._end, np.zeros_like(n)]))
 
@@ -318,17 +319,25 @@ class Int4KVCache:
     def _regroup(self) -> None:
         """Sequences that begin with the same page are one group, named by its lowest;
         the pages that all of it have in common are read once."""
-        group, pages, leader = np.arange(self.batch), np.zeros(self.batch, np.int64), {}
-        for b in range(self.batch):
-            first = int(self._table[b, 0])
-            if first < 0 or self._refs[first] < 2:
-                continue
-            a = leader.setdefault(first, b)
-            group[b] = a
-            same = int(min(self._owned[a], self._owned[b])) if a != b else int(self._owned[b])
-            differs = np.flatnonzero(self._table[a, :same] != self._table[b, :same])
-            same = int(differs[0]) if len(differs) else same
-            pages[a] = same if a == b else min(int(pages[a]), same)
+        first = self._table[:, 0]
+        rows = np.flatnonzero((first >= 0) & (self._refs[first] > 1))
+        if not len(rows) and not self._common.any():
+            return   # as before: no sequence shares anything
+        group, pages = np.arange(self.batch), np.zeros(self.batch, np.int64)
+        self._common[:] = 0
+        if len(rows):
+            _, leader, which = np.unique(first[rows], return_index=True, return_inverse=True)
+            leader = rows[leader[which]]   # each row's group: its lowest sequence
+            table = self._table[:, :int(self._owned[rows].max())]
+            held = table[rows] >= 0
+
+            def leading(yes):   # how many of a row's first entries are so
+                return np.where(yes.all(1), yes.shape[1], np.argmin(yes, 1))
+
+            self._common[rows] = leading(held & (self._refs[table[rows]] > 1))
+            group[rows] = leader
+            pages[leader] = self.width
+            np.minimum.at(pages, leader, leading(held & (table[rows] == table[leader])))
         self._upload(self.prefix_group, group)
         self._upload(self.prefix_pages, pages)
 

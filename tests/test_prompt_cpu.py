@@ -5,6 +5,7 @@ from __future__ import annotations
 import math
 import re
 import struct
+import time
 from pathlib import Path
 
 import numpy as np
@@ -277,6 +278,76 @@ def test_sharing_a_part_and_sharing_on(cache):
     c.reserve([0, 0, 0, 64])
     with pytest.raises(ValueError, match="empty"):
         c.share(0, [3])
+
+
+def test_many_sequences_cost_no_more_than_before_pages_could_be_shared(cache, monkeypatch):
+    """truncate() runs at every step of drafts, release() at every end of a sequence: neither walks over the batch in
+    Python, and where nothing is shared the groups stay as they were, without a copy to the GPU."""
+    many = int4.Int4KVCache(1, 2048, 4, 2, 64, n_pages=2 * 2048, max_tokens=640, device="cpu")
+    many.extend(70)
+    copied = []
+    real = many._upload
+    monkeypatch.setattr(many, "_upload", lambda t, host: (copied.append(t), real(t, host)), raising=False)
+
+    def fastest(call):
+        took = []
+        for _ in range(20):
+            since = time.perf_counter()
+            call()
+            took.append(time.perf_counter() - since)
+        return min(took)
+
+    # 17 us each on the build machine, truncate 6 ms and release 0.5 ms when they walked
+    assert fastest(lambda: many.truncate(70)) < 1e-3
+    assert fastest(lambda: many.release([5])) < 2e-4
+    assert not any(t is many.prefix_group or t is many.prefix_pages for t in copied)
+    many.share(0, [5])
+    assert int(many.prefix_group[5]) == 0 and int(many.prefix_pages[0]) == 1
+    with pytest.raises(ValueError, match="shares"):
+        many.truncate(np.where(np.arange(2048) == 5, 63, many.lengths))
+    assert fastest(lambda: many.truncate(many.lengths)) < 1e-3
+
+
+def test_groups_follow_any_order_of_sharing_and_release(cache):
+    """Against the groups counted page by page."""
+    rng = np.random.default_rng(3)
+    c = int4.Int4KVCache(1, 7, 4, 2, 64, n_pages=80, max_tokens=700, device="cpu")
+    for step in range(300):
+        b = int(rng.integers(7))
+        if c.lengths[b] == 0 and rng.random() < 0.6:
+            sources = [a for a in range(7) if c.lengths[a]]
+            if sources:
+                c.share(int(rng.choice(sources)), [b], None if rng.random() < 0.5 else 64 * int(rng.integers(0, 1 + min(c.lengths[sources]) // 64)))
+        elif rng.random() < 0.4:
+            c.release([b])
+        else:
+            n = np.zeros(7, np.int64)
+            n[b] = rng.integers(1, 150)
+            if (c.lengths + n).max() < 700 and c.free_pages > 3:
+                c.extend(n)
+        rows = [[int(p) for p in row if p >= 0] for row in c.page_table]
+        held = [p for row in rows for p in row]
+        groups = {}
+        for a, row in enumerate(rows):
+            if row and held.count(row[0]) > 1:
+                groups.setdefault(row[0], []).append(a)
+        want_group, want_pages = list(range(7)), [0] * 7
+        for members in groups.values():
+            common = 0
+            while all(len(rows[a]) > common and rows[a][common] == rows[members[0]][common] for a in members):
+                common += 1
+            for a in members:
+                want_group[a] = members[0]
+            want_pages[members[0]] = common
+        assert c.prefix_group.tolist() == want_group and c.prefix_pages.tolist() == want_pages
+        for a, row in enumerate(rows):
+            first_own = next((j for j, p in enumerate(row) if held.count(p) == 1), len(row))
+            if first_own:
+                with pytest.raises(ValueError, match="shares"):
+                    c.truncate(np.where(np.arange(7) == a, min(64 * first_own - 1, int(c.lengths[a])), c.lengths))
+            before = c.lengths
+            c.truncate(before)
+    assert c.free_pages + len(set(held)) == 80
 
 
 def test_adapter_takes_the_prompt_kernel_by_name():
