@@ -39,6 +39,7 @@ from logitfill_b200.prompt import rotary_embed
 
 PAGE_TOKENS = 64   # tokens of a page
 GROUP = 32         # channels that share a scale and a minimum
+MAX_GROUPS = 4096  # groups of sequences that share pages, of one call
 
 
 def record_words(head_dim: int) -> int:
@@ -135,7 +136,7 @@ def int4_prefix_attention(query: torch.Tensor, pages: torch.Tensor, page_table: 
     for all of a group's queries.
 
     ``prefix_group`` (int32 ``[batch]``) names each sequence's group (outside ``0 ..
-    groups - 1``: none), ``prefix_pages`` (int32 ``[groups]``) how many of their
+    groups - 1``: none), ``prefix_pages`` (int32 ``[groups]``, ``MAX_GROUPS`` at most) how many of their
     first page table entries a group's sequences have in common; the entries of
     its lowest sequence are read.  Both are read on the GPU.  The result is
     :func:`int4_attention`'s up to the order of sums, for any lengths.  Where few
@@ -192,8 +193,8 @@ class Int4KVCache:
         self._free = list(range(n_pages - 1, -1, -1))
         self._refs = np.zeros(n_pages, np.int64)                  # sequences that hold each page
         self._common = np.zeros(batch, np.int64)                  # first pages of each that others hold too
-        self.prefix_group = torch.arange(batch, dtype=torch.int32, device=self.device)   # for int4_prefix_attention
-        self.prefix_pages = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self.prefix_pages = torch.zeros(min(batch, MAX_GROUPS), dtype=torch.int32, device=self.device)   # for int4_prefix_attention
+        self.prefix_group = torch.from_numpy(self._numbered(np.arange(batch))[0].astype(np.int32)).to(self.device)
 
     @property
     def n_layers(self) -> int:
@@ -338,8 +339,22 @@ class Int4KVCache:
             group[rows] = leader
             pages[leader] = self.width
             np.minimum.at(pages, leader, leading(held & (table[rows] == table[leader])))
+        group, names = self._numbered(group)
         self._upload(self.prefix_group, group)
-        self._upload(self.prefix_pages, pages)
+        self._upload(self.prefix_pages, pages[names])
+
+    def _numbered(self, group: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+        """(each sequence's group as a call takes it, the lowest sequence of each group).
+        Groups that go by their lowest sequence's number as long as there are numbers for
+        all; else groups of several come first, and what is past the last number is in none
+        (its sequences read their pages themselves)."""
+        if self.batch <= MAX_GROUPS:
+            return group, np.arange(self.batch)
+        size = np.bincount(group, minlength=self.batch)
+        names = np.argsort(-np.minimum(size, 2), kind="stable")[:MAX_GROUPS]   # (sequences that lead no group: size 0, last)
+        number = np.full(self.batch, -1)
+        number[names] = np.arange(len(names))
+        return number[group], names
 
     def write(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store this step's tokens of one layer: ``[batch, n_kv, T, head_dim]``,
@@ -407,5 +422,5 @@ class Int4KVCache:
             _lib.check(code, "4-bit cache kernel")
 
 
-__all__ = ["PAGE_TOKENS", "GROUP", "record_words", "bounds_bytes", "alloc_pages", "alloc_bounds", "int4_write",
+__all__ = ["PAGE_TOKENS", "GROUP", "MAX_GROUPS", "record_words", "bounds_bytes", "alloc_pages", "alloc_bounds", "int4_write",
            "int4_read", "int4_read_bounds", "int4_attention", "int4_select", "int4_sparse_attention", "int4_prefix_attention", "Int4KVCache"]

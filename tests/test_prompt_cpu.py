@@ -350,6 +350,25 @@ def test_groups_follow_any_order_of_sharing_and_release(cache):
     assert c.free_pages + len(set(held)) == 80
 
 
+def test_groups_of_a_batch_with_more_sequences_than_numbers(cache, monkeypatch):
+    """A call takes MAX_GROUPS groups: those of several sequences are numbered first, what is left over is in none."""
+    n = int4.MAX_GROUPS + 900
+    many = int4.Int4KVCache(1, n, 1, 1, 64, n_pages=n + 50, max_tokens=64 * 3, device="cpu")
+    assert many.prefix_pages.shape == (int4.MAX_GROUPS,)
+    assert many.prefix_group.tolist() == [b if b < int4.MAX_GROUPS else -1 for b in range(n)]
+    counts = np.zeros(n, np.int64)
+    counts[[4500, 10, 3]] = 130, 64, 70
+    many.extend(counts)
+    many.share(4500, [4501, 7], 128)
+    many.share(10, [4990])
+    group, pages = many.prefix_group.tolist(), many.prefix_pages.tolist()
+    assert group[7] == group[4500] == group[4501] == 0 and pages[0] == 2 and group[10] == group[4990] == 1 and pages[1] == 1
+    rest = [b for b in range(n) if b not in (7, 4500, 4501, 10, 4990)]
+    assert [group[b] for b in rest] == [2 + i if 2 + i < int4.MAX_GROUPS else -1 for i in range(len(rest))] and not any(pages[2:])
+    many.release([4500, 7, 4990])
+    assert many.prefix_group.tolist() == [b if b < int4.MAX_GROUPS else -1 for b in range(n)] and not many.prefix_pages.any()
+
+
 def test_adapter_takes_the_prompt_kernel_by_name():
     model = tiny_qwen2(n_q=4, n_kv=2, head_dim=64, layers=1, vocab=32, seed=1)
     assert DeepSeekQwenKVAdapter(model, group_size=64).prompt == "dense"

@@ -182,3 +182,28 @@ def test_model_prefill_by_the_prompt_kernel():
     with pytest.raises(NotImplementedError, match="gradient"):
         model(input_ids=ids, use_cache=True, past_key_values=a.make_cache())
     a.detach()
+
+
+def test_more_sequences_than_groups_of_a_call():
+    """attend_shared takes any batch that attend takes."""
+    B = 4096 + 37
+    cache = Int4KVCache(1, B, 2, 1, 64, n_pages=B + 40, max_tokens=192)
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def step(counts, T):
+        q, k, v = (torch.randn(B, h, T, 64, generator=g, device="cuda").to(BF16) for h in (2, 1, 1))
+        cache.extend(counts)
+        cache.write(0, k, v)
+        return q
+
+    step([130 if b == 4100 else 0 for b in range(B)], 130)
+    cache.share(4100, range(20, 50), 128)
+    q = step(1, 1)
+    shared, plain = cache.attend_shared(0, q, 0.125), cache.attend(0, q, 0.125)
+    hk, hv = cache.read(0)
+    for b in (0, 19, 20, 49, 50, 4095, 4096, 4100, B - 1):
+        n = int(cache.lengths[b])
+        for got in (shared, plain):
+            _inside(got[b], _attended(q[b], hk[b, :, :n], hv[b, :, :n], 0.125, [n]))
+    assert float((shared.float() - plain.float()).abs().max()) <= 2.0 ** -5    # (either within the bound above: a few units)
+    cache.check_status()
