@@ -481,10 +481,14 @@ typedef struct lf_int4_prefix {
  * sequence is read), so these pages are read and unpacked once for all queries of the
  * group.  The result is lf_int4_attend's, up to the order of its sums; a sequence that
  * sees only part of its shared pages, or is in no group, is attended as well.
- * workspace: lf_int4_prefix_workspace_bytes bytes, 16-byte aligned, of any content; calls
- * that overlap on the GPU need one each (of both).
+ * workspace: 16-byte aligned, of any content; calls that overlap on the GPU need one each (of
+ * both).  lf_int4_prefix_workspace_need says how many bytes this call needs, with the current
+ * device's SMs (its pointers are not looked at): none where each sequence will read its pages
+ * itself whatever the groups turn out to be.  lf_int4_prefix_workspace_bytes is enough for any
+ * call of these sizes.
  */
 LF_API int lf_int4_attend_prefix(const lf_int4_prefix* args, lf_stream_t stream);
+LF_API size_t lf_int4_prefix_workspace_need(const lf_int4_prefix* args);
 LF_API size_t lf_int4_prefix_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim, int groups);
 
 LF_API size_t lf_int4_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim);

@@ -22,7 +22,7 @@ EXPORTS = (
     "lf_ipc_alloc", "lf_ipc_free", "lf_ipc_handle", "lf_ipc_open", "lf_ipc_close", "lf_decode_merge_gather",
     "lf_gather_signals", "lf_gather_wait", "lf_int4_write", "lf_int4_read", "lf_int4_read_bounds", "lf_int4_select",
     "lf_int4_attend", "lf_int4_attend_sparse", "lf_int4_attend_prefix", "lf_int4_workspace_bytes", "lf_int4_workspace_clear_from",
-    "lf_int4_prefix_workspace_bytes", "lf_rotary_embed", "lf_prompt_attend", "lf_status_string", "lf_last_error",
+    "lf_int4_prefix_workspace_bytes", "lf_int4_prefix_workspace_need", "lf_rotary_embed", "lf_prompt_attend", "lf_status_string", "lf_last_error",
 )
 
 
@@ -96,6 +96,7 @@ def lib() -> ctypes.CDLL:
         "lf_int4_attend_sparse": (c_int, [Q, P]),
         "lf_int4_attend_prefix": (c_int, [Q, P]),
         "lf_int4_prefix_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+        "lf_int4_prefix_workspace_need": (c_size_t, [Q]),
         "lf_int4_workspace_clear_from": (c_size_t, []),
         "lf_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
         "lf_rotary_embed": (c_int, [Q, P]),

@@ -114,10 +114,11 @@ Scratch workspace(const lf_int4_query& a, const Launch& on) {
 }
 
 // The same for the records of calls with shared pages, whose content does not matter.
-Scratch prefix_workspace(const lf_int4_query& a, int groups, const Launch& on) {
+Scratch prefix_workspace(const lf_int4_prefix& a, const Launch& on) {
   static std::mutex mu;
   static auto* held = new Held;
-  const size_t need = lf_int4_prefix_workspace_bytes(a.pool.batch, a.pool.kv_heads, a.n_q, a.q_len, a.head_dim, groups);
+  const size_t need = lf_int4_prefix_workspace_need(&a);
+  if (need == 0) return Scratch{};
   const auto options = at::TensorOptions().dtype(at::kByte).device(on.stream.device());
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return Scratch{at::empty({static_cast<int64_t>(need)}, options), need};
@@ -340,10 +341,10 @@ PyObject* attend_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
     at::Tensor out = fill_out(a.query, p, v[8], tensor(v[0], "query"));
     if (at::has_internal_overlap(out) == at::MemOverlap::Yes) fail(PyExc_ValueError, "out overlaps itself");
     if (overlap(out, q)) fail(PyExc_ValueError, "out shares memory with the query");
-    const Scratch scratch = workspace(a.query, on), records = prefix_workspace(a.query, a.groups, on);
+    const Scratch scratch = workspace(a.query, on), records = prefix_workspace(a, on);
     a.query.workspace = scratch.words.data_ptr();
     a.query.workspace_bytes = scratch.bytes;
-    a.workspace = records.words.data_ptr();
+    if (records.bytes != 0) a.workspace = records.words.data_ptr();
     a.workspace_bytes = records.bytes;
     check(lf_int4_attend_prefix(&a, on.raw()), "lf_int4_attend_prefix");
     return THPVariable_Wrap(std::move(out));

@@ -689,12 +689,42 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
 
 // ------------------------------------------------------------------- host
 
-// Bytes of the plan's lists, and records that there can be.
+// Bytes of the plan's lists.
 static size_t plan_bytes(int batch, int groups) {
   return (16 + static_cast<size_t>(groups) * sizeof(PrefixGroup) + static_cast<size_t>(batch) * (sizeof(PrefixSeq) + 4) + 255) / 256 * 256;
 }
-static int64_t most_records(int64_t batch, int64_t kv_heads, int64_t heads, int64_t q_len, int64_t groups, int64_t sms) {
-  return (batch * q_len * heads / kPrefixRows + (groups < batch ? groups : batch)) * kv_heads + sms;
+// The fewest members of a group whose pages are read once (plan kernel: group_pages, group_cost).
+// Where sizes decide, n members save something only where n visits of P pages take longer than
+// the steps of one unit at least, of which there are more than P / 2:
+// n A D / 1280 > tile_ns / 2, with visit_ns' factor A.  So records are few where queries are
+// many: a row of records for each of 1024 sequences that might share would be 1 GB for 8 KV
+// heads, D 128; by this rule it is 0.2.
+static int64_t least_members(int64_t columns, int head_dim, bool fp16, bool always) {
+  const int64_t least = columns <= 16 ? 2 : 1;
+  if (always) return least;
+  const int64_t a = (columns + 15) / 16 * (columns <= 8 ? 20 : 29), n = 640 * tile_ns(head_dim, fp16) / (a * head_dim) + 1;
+  return n > least ? n : least;
+}
+// Records that there can be: one of each unit and CTA that meet, no more than units and CTAs.
+static int64_t most_units(int64_t batch, int64_t kv_heads, int64_t columns, int64_t groups, int64_t least) {
+  const int64_t most_groups = batch / least;  // that read pages once
+  return most_groups == 0 ? 0 : (batch * columns / kPrefixRows + (groups < most_groups ? groups : most_groups)) * kv_heads;
+}
+static size_t prefix_bytes(int64_t batch, int64_t groups, int64_t units, int head_dim) {
+  return plan_bytes(static_cast<int>(batch), static_cast<int>(groups)) +
+         static_cast<size_t>(units + sm_count()) * prefix_record(head_dim) * 4;
+}
+// Units that a call may have; 0 where each sequence reads its pages itself, whatever the groups are.
+static int64_t call_units(const lf_int4_prefix& a) {
+  const lf_int4_query& q = a.query;
+  if (a.groups <= 0 || a.groups > kMaxGroups || q.pool.kv_heads <= 0 || q.pool.batch <= 0 || q.q_len <= 0 || q.n_q < q.pool.kv_heads || q.head_dim <= 0)
+    return 0;
+  const int64_t columns = static_cast<int64_t>(q.q_len) * (q.n_q / q.pool.kv_heads);
+  if (columns * q.pool.batch > (1 << 30)) return 0;  // (refused)
+  const bool small =
+      visit_ns(static_cast<int64_t>(q.pool.batch) * q.pool.kv_heads * q.pool.table_width, static_cast<int>(columns), q.head_dim) <= fixed_ns(q.head_dim);
+  if (small && !a.always) return 0;
+  return most_units(q.pool.batch, q.pool.kv_heads, columns, a.groups, least_members(columns, q.head_dim, q.dtype == LF_F16, a.always != 0));
 }
 
 template <typename T>
@@ -706,8 +736,14 @@ static const void* prefix_kernel_of(int head_dim) {
 
 extern "C" size_t lf_int4_prefix_workspace_bytes(int batch, int kv_heads, int n_q, int q_len, int head_dim, int groups) {
   if (batch <= 0 || kv_heads <= 0 || n_q < kv_heads || q_len <= 0 || head_dim <= 0 || groups < 0) return 0;
-  return lf::plan_bytes(batch, groups) + static_cast<size_t>(lf::most_records(batch, kv_heads, n_q / kv_heads, q_len, groups, lf::sm_count())) *
-                                             lf::prefix_record(head_dim) * 4;
+  const int64_t columns = static_cast<int64_t>(q_len) * (n_q / kv_heads);
+  return lf::prefix_bytes(batch, groups, lf::most_units(batch, kv_heads, columns, groups, lf::least_members(columns, head_dim, false, true)), head_dim);
+}
+
+extern "C" size_t lf_int4_prefix_workspace_need(const lf_int4_prefix* a) {
+  if (a == nullptr) return 0;
+  const int64_t units = lf::call_units(*a);
+  return units == 0 ? 0 : lf::prefix_bytes(a->query.pool.batch, a->groups, units, a->query.head_dim);
 }
 
 extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream) {
@@ -719,9 +755,8 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   if (bad != LF_OK) return bad;
   LF_CHECK_ARG(a->groups >= 0 && (a->groups == 0 || (a->group && a->shared)), "lf_int4_attend_prefix: null pointer");
   LF_CHECK_SUPPORTED(a->groups <= kMaxGroups, "lf_int4_attend_prefix: %d groups (%d at most)", a->groups, kMaxGroups);
-  const int columns = q.q_len * (q.n_q / q.pool.kv_heads);
-  const bool small = visit_ns(static_cast<int64_t>(q.pool.batch) * q.pool.kv_heads * q.pool.table_width, columns, q.head_dim) <= fixed_ns(q.head_dim);
-  if (a->groups == 0 || (small && !a->always)) return lf_int4_attend(&q, stream);
+  const int64_t units = call_units(*a);
+  if (units == 0) return lf_int4_attend(&q, stream);
   PrefixParams p;
   const int ok = check_int4_pool("lf_int4_attend_prefix", q.pool, q.head_dim, p.pool);
   if (ok != LF_OK) return ok;
@@ -742,12 +777,12 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   p.scale_log2 = q.scaling * 1.4426950408889634f;
   p.status = q.status;
   const int sms = sm_count();
-  const int64_t records = most_records(p.pool.batch, p.pool.kv_heads, p.heads, p.q_len, p.groups, sms);
+  const int64_t records = units + sms;
   const int64_t steps = (p.pool.table_width + 1) / 2 + kPrefixCost;
   LF_CHECK_SUPPORTED(records <= (1 << 30) / steps && static_cast<int64_t>(p.pool.batch) * p.q_len * p.heads <= (1 << 30),
                      "lf_int4_attend_prefix: %d sequences of %d pages are too many for one call", p.pool.batch, p.pool.table_width);
   LF_CHECK_ARG(a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0 &&
-                   a->workspace_bytes >= lf_int4_prefix_workspace_bytes(p.pool.batch, p.pool.kv_heads, q.n_q, p.q_len, q.head_dim, p.groups),
+                   a->workspace_bytes >= prefix_bytes(p.pool.batch, p.groups, units, q.head_dim),
                "lf_int4_attend_prefix: workspace of %zu bytes is missing, misaligned or too small", a->workspace_bytes);
   uint8_t* at = static_cast<uint8_t*>(a->workspace);
   p.plan.head = reinterpret_cast<int*>(at);
@@ -755,7 +790,7 @@ extern "C" int lf_int4_attend_prefix(const lf_int4_prefix* a, lf_stream_t stream
   p.plan.seqs = reinterpret_cast<PrefixSeq*>(p.plan.groups + p.groups);
   p.plan.members = reinterpret_cast<int*>(p.plan.seqs + p.pool.batch);
   p.plan.records = reinterpret_cast<float*>(at + plan_bytes(p.pool.batch, p.groups));
-  const int64_t most_steps = (records - sms) * steps;
+  const int64_t most_steps = units * steps;
   p.grid = static_cast<int>(most_steps < sms ? most_steps : sms);
 
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

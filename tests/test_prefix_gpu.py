@@ -375,3 +375,25 @@ def test_offsets_past_32_bits():
     want = batch.run(q, 0.09)
     batch.pages, batch.table = pages, torch.where(batch.table >= 0, batch.table + far, batch.table)
     assert torch.equal(batch.run(q, 0.09), want)
+
+
+def test_workspace_of_many_groups_that_share_little():
+    """A group for every sequence, few of which share: no record for each, and none for calls that int4_attention takes."""
+    B, H, D = 500, 8, 128
+    batch = Batch(25, [b // 2 if b < 20 else b for b in range(B)], [2 if x < 10 else 0 for x in range(B)], [1 + b % 3 for b in range(B)], H, D)
+    q = batch.query(22, 16, 1)
+    lengths, group, shared = _i32(batch.lengths), _i32(batch.group), _i32(batch.shared)
+    wide = torch.full((B, 300), -1, dtype=torch.int32, device="cuda")
+    wide[:, :batch.table.shape[1]] = batch.table
+    for n, always, most in ((4, False, 0), (B, False, 150 << 20), (B, True, 330 << 20)):
+        stream = torch.cuda.Stream()
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            int4.int4_attention(q[:n], batch.pages, wide[:n], lengths[:n], 0.09, out=out[:n])      # its own workspace
+            before = torch.cuda.memory_allocated()
+            int4.int4_prefix_attention(q[:n], batch.pages, wide[:n], lengths[:n], 0.09, group[:n], shared, out=out[:n], always=always)
+            assert torch.cuda.memory_allocated() - before <= most
+        torch.cuda.synchronize()
+        want, bound = batch.want(q, 0.09)
+        assert bool(((out.double() - want).abs() <= bound)[:n].all()) and not bool(out[n:].any())

@@ -110,6 +110,66 @@ def test_prefix_attention_validates_before_launch():
     assert many - few == 8 * (64 * 5 * 256 // 256 - 64 * 5 // 256) * record
 
 
+def _need(batch=64, kv_heads=8, n_q=40, q_len=1, head_dim=128, dtype=None, width=1000, groups=64, always=0):
+    query = dict(q_len=q_len, n_q=n_q, head_dim=head_dim, dtype=_lib.LF_BF16 if dtype is None else dtype)
+    pool = dict(batch=batch, kv_heads=kv_heads, table_width=width)
+    return _lib.lib().lf_int4_prefix_workspace_need(_prefix(dict(query, **pool), groups=groups, always=always))
+
+
+def test_prefix_attention_asks_for_no_more_workspace_than_groups_may_use():
+    so = _lib.lib()
+    record = 256 * (128 + 2) * 4
+    any_call = so.lf_int4_prefix_workspace_bytes(1024, 8, 40, 1, 128, 1024)
+    assert any_call < 0.6e9                                   # pairs of sequences, at most
+    assert _need(batch=1024, groups=1024) < 0.26e9            # five sequences read a page once sooner than each for itself
+    assert _need(batch=64, groups=64) < 15e6
+    assert _need(batch=64, groups=64) >= (64 * 5 // 256 + 12) * 8 * record
+    for none in (dict(width=3, batch=4), dict(batch=4, groups=4), dict(groups=0), dict(groups=4097), dict(q_len=0), dict(n_q=7)):
+        assert _need(**none) == 0, none
+    assert _need(batch=4, groups=4, always=1) > 0 and _need(batch=1, groups=1, q_len=512, n_q=28, kv_heads=4) > 0
+    assert so.lf_int4_prefix_workspace_need(None) == 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_no_groups_fill_more_units_than_a_call_has_room_for(seed):
+    """The plan's rule (which groups read their pages once, and how many units of 256 rows that makes), over random
+    groups, lengths and shapes, against the room that a call asks for."""
+    rng = np.random.default_rng(seed)
+    tried = 0
+    for _ in range(400):
+        D, fp16, always = int(rng.choice([64, 128])), bool(rng.integers(2)), bool(rng.integers(2))
+        kv_heads, heads, q_len = int(rng.choice([1, 2, 8])), int(rng.choice([1, 2, 5, 7, 16, 40])), int(rng.choice([1, 1, 2, 3, 9, 64]))
+        batch = int(rng.integers(1, 200))
+        groups = int(rng.integers(1, 200))
+        width = int(rng.choice([1, 7, 100, 1000, 5000]))
+        columns = heads * q_len
+        visit = lambda pages: pages * ((columns + 15) // 16) * (20 if columns <= 8 else 29) * D // 1280  # noqa: E731
+        tile = {(128, False): 16, (128, True): 23, (64, False): 11, (64, True): 16}[D, fp16]
+        fewest = rng.integers(1, 12)
+        count = np.bincount(rng.integers(0, max(1, min(groups, batch // fewest)), batch), minlength=groups)
+        units = 0
+        for c in count:
+            if c == 0 or (c == 1 and columns <= 16):
+                continue
+            pages = width if rng.random() < 0.7 else int(rng.integers(0, width + 1))
+            tiles = -(-int(c) * columns // 256) if pages else 0
+            places = tiles * kv_heads * ((pages + 1) // 2 + 2)
+            if pages and (always or visit(pages * int(c) * kv_heads) - places * tile > 0):
+                units += tiles * kv_heads
+        need = _need(batch, kv_heads, kv_heads * heads, q_len, D, _lib.LF_F16 if fp16 else _lib.LF_BF16, width, groups, int(always))
+        small = visit(batch * kv_heads * width) <= (17000 if D == 128 else 12500) and not always
+        if small:
+            assert need == 0
+            continue
+        lists = (16 + 32 * groups + 12 * batch + 255) // 256 * 256
+        record = 256 * (D + 2) * 4
+        room = (need - lists) // record if need else 0      # (no SMs here: the records of units alone)
+        assert room >= units, (D, fp16, always, kv_heads, heads, q_len, batch, groups, width)
+        assert need <= _lib.lib().lf_int4_prefix_workspace_bytes(batch, kv_heads, kv_heads * heads, q_len, D, groups)
+        tried += units > 0
+    assert tried > 50
+
+
 # ------------------------------------------------------------ frequencies
 
 def _radians(freqs):
