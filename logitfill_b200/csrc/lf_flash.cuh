@@ -108,26 +108,25 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 
 // How the waits of a CTA end before their time, in its shared memory.
 struct Waits {
+  uint64_t moved;  // when a role was last seen at work that others wait for, however long it takes (globaltimer)
   int stop;        // one gave up
-  uint32_t moves;  // counts up while a role is at work that others wait for, however long it takes
 };
 // Wait of a whole warp for a barrier's phase, with a limit: false once a wait of this CTA
-// has given up, for all lanes alike.  The limit is on a time in which nothing moves: work
-// that may take longer (prompt_row's) counts up Waits::moves.  The clock is read once in
-// 1024 tries.
+// has given up, for all lanes alike.  The clock is read once in 1024 tries.  kMoves: the limit
+// is on a time in which nothing moves; work that may take longer (prompt_row's) writes
+// Waits::moved.  (The other kernel does without: looked at there too, it took 283 us for a
+// chunk in place of 272.)
 constexpr uint64_t kTileWaitNs = 2000000000ull;
+template <bool kMoves>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile Waits* waits, uint64_t limit_ns = kTileWaitNs) {
   bool ok = mbar_try_wait(bar, parity);
   uint64_t since = 0;
-  uint32_t moves = 0;
   for (uint32_t n = 1; !ok; ++n) {
     ok = mbar_try_wait(bar, parity);
     if ((n & 1023u) == 0u && !ok) {
       const uint64_t now = globaltimer_ns();
-      const uint32_t seen = waits->moves;
-      if (since == 0 || seen != moves) since = now;
-      moves = seen;
-      if (waits->stop != 0 || now - since > limit_ns) {
+      if (since == 0) since = now;
+      if (waits->stop != 0 || (now - since > limit_ns && (!kMoves || static_cast<int64_t>(now - waits->moved) > static_cast<int64_t>(limit_ns)))) {
         waits->stop = 1;
         break;
       }

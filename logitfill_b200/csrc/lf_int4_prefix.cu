@@ -203,7 +203,7 @@ struct PrefixShared {
   uint64_t raw_full[8], raw_empty[8], kv_full[8], kv_empty[8], q_ready[2], s_full[2], p_early[2], p_ready[2], met[2], o_done[2], last;
   Waits waits;
   uint32_t tmem;
-  float told[2][2][128];  // between the two threads of a row
+  alignas(128) float told[2][2][128];  // between the two threads of a row
 };
 
 // Steps of one unit that this CTA has.
@@ -350,7 +350,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
     }
     mbar_init(&sh.last, 1);
     sh.waits.stop = 0;
-    sh.waits.moves = 0;
     fence_mbar_init();
   }
   tc_fence_before();
@@ -360,7 +359,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) int4_prefix_kernel(const __
   grid_dep_trigger();  // all CTAs of this grid run at once, so the suffix kernel's take nothing that one needs
   grid_dep_wait();
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, &sh.waits); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait<false>(bar, parity, &sh.waits); };
   const int per_member = p.q_len * p.heads;
 
   if (warp == kCopyWarp) {

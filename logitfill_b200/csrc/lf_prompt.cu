@@ -66,11 +66,11 @@ __device__ __forceinline__ PromptSpan prompt_span(const PromptParams& p, int b) 
 }
 
 // One row by one warp: q over the first n keys, in fp32; the lane keeps D / 32 channels.
-// What waits for the row meanwhile learns from `moves` that it comes on: a warp has 16 rows of
+// What waits for the row meanwhile learns from `moved` that it comes on: a warp has 16 rows of
 // some 0.2 us a key, which is more than the waits' limit from some hundred thousand keys on.
 template <typename T, int D>
 __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok, const T* v, int64_t v_tok, int n, float scale_log2, T* out,
-                                           uint32_t* moves) {
+                                           volatile uint64_t* moved) {
   constexpr int kOwn = D / 32, kAhead = 4;
   const int d = (threadIdx.x & 31) * kOwn;
   // positive, so that -inf stays one; the difference to the maximum before the product
@@ -82,7 +82,7 @@ __device__ __forceinline__ void prompt_row(const T* q, const T* k, int64_t k_tok
     acc[x] = 0.0f;
   }
   for (int j = 0; j < n; j += kAhead) {
-    if (j % 4096 == 0 && (threadIdx.x & 31) == 0) atomicAdd(moves, 1u);
+    if (j % 4096 == 0 && (threadIdx.x & 31) == 0) *moved = sm100::globaltimer_ns();
     float s[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -154,7 +154,7 @@ struct PromptShared {
   int bad[2];      // a Value that not all rows of a masked tile see is not finite
   Waits waits;
   uint32_t tmem;
-  float told[2][2][128];  // between the two threads of a row
+  alignas(128) float told[2][2][128];  // between the two threads of a row
 };
 
 // 32 bytes of a row: one store where rows are 32-byte aligned (a whole sector by one lane).
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&sh.item_full[t], 1);
       mbar_init(&sh.item_empty[t], 18);
     }
+    sh.waits.moved = 0;
     sh.waits.stop = 0;
-    sh.waits.moves = 0;
     fence_mbar_init();
   }
   tc_fence_before();
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&sh.tmem), 0);
   grid_dep_wait();
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, &sh.waits); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait<true>(bar, parity, &sh.waits); };
   // The next item (number n of this CTA), copied from the plan's slot.
   auto take = [&](uint32_t n, PromptItem& it) -> bool {
     if (!wait(&sh.item_full[n & 1], (n >> 1) & 1)) return false;
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (x >= per_tile * p.group || tok >= it.rows) break;
           const int64_t row = static_cast<int64_t>(it.first) + tok;
           prompt_row<T, D>(static_cast<const T*>(p.q) + it.b * p.q_seq + row * p.q_tok + hd * p.q_head, k, p.k_tok, v, p.v_tok,
-                           tok < it.tokens ? tok + 1 : 0, p.scale_log2, static_cast<T*>(p.out) + it.b * p.o_seq + row * p.o_tok + hd * p.o_head, &sh.waits.moves);
+                           tok < it.tokens ? tok + 1 : 0, p.scale_log2, static_cast<T*>(p.out) + it.b * p.o_seq + row * p.o_tok + hd * p.o_head, &sh.waits.moved);
         }
       } else {
         // else 0: a row behind the sequence, or one of no score above -inf

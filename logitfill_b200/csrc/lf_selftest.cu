@@ -31,7 +31,7 @@ extern "C" int lf_selftest_wait(int32_t* status, int64_t limit_ns, int arrive, l
 }
 
 // The same of the wait of the tensor-core attention kernels (warp_wait).  One warp waits; the
-// other counts up Waits::moves for busy_ns, then arrives on the barrier or not.  Their limit
+// other writes Waits::moved for busy_ns, then arrives on the barrier or not.  Their limit
 // is on a time in which nothing moves.
 namespace lf {
 
@@ -41,19 +41,22 @@ __global__ void selftest_tile_wait_kernel(int32_t* status, uint64_t limit_ns, ui
   if (threadIdx.x == 0) {
     sm100::mbar_init(&bar, 1);
     sm100::fence_mbar_init();
+    waits.moved = 0;
     waits.stop = 0;
-    waits.moves = 0;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
-    const bool done = sm100::warp_wait(&bar, 0, &waits, limit_ns);
+    const bool done = sm100::warp_wait<true>(&bar, 0, &waits, limit_ns);
     // (a wait that gives up ends all others of its CTA as well)
-    const bool again = sm100::warp_wait(&bar, 0, &waits, limit_ns);
+    const bool again = sm100::warp_wait<true>(&bar, 0, &waits, limit_ns);
     if (threadIdx.x == 0) *status = done && again && waits.stop == 0 ? LF_OK : !done && !again && waits.stop == 1 ? LF_ERR_DEVICE_TIMEOUT : -1;
   } else if (threadIdx.x == 32) {
     const uint64_t since = sm100::globaltimer_ns();
-    for (uint32_t n = 0; n < (1u << 27) && sm100::globaltimer_ns() - since < busy_ns; ++n) {
-      if ((n & 1023u) == 0u) atomicAdd(&waits.moves, 1u);
+    volatile uint64_t* moved = &waits.moved;
+    uint64_t now = since;
+    for (uint32_t n = 0; n < (1u << 27) && now - since < busy_ns; ++n) {
+      if ((n & 1023u) == 0u) *moved = now;
+      now = sm100::globaltimer_ns();
     }
     if (arrive) sm100::mbar_arrive(&bar);
   }
