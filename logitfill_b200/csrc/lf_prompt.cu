@@ -270,6 +270,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int b = lane; b < p.batch; b += 32) most = max(most, pairs_of(b));
     most = __reduce_max_sync(0xffffffffu, most);
     const int64_t total = above(0) * p.n_kv;
+    // The level of the last item, the level's first item and the next one's, and how far into
+    // the sequences its search went, with how many of the level it passed: items come in
+    // order, so none is searched from the start again.  (65000 sequences of one token, 8 KV
+    // heads: 1315 ms so, by the square of their number, and 11 this way.)
+    int low = 0, b0 = 0, passed = 0;
+    int64_t level_first = 0, level_end = 0;
     uint32_t n = 0;
     for (int64_t round = 0;; ++round, ++n) {
       if (n >= 2 && !wait(&sh.item_empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
@@ -277,23 +283,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       PromptItem it;
       it.b = -1;
       if (x < total) {
-        int low = 0, high = most - 1;  // the level: the largest with more than x items at or above it
-        while (low < high) {
-          const int mid = (low + high + 1) >> 1;
-          if (above(mid) * p.n_kv > x) low = mid; else high = mid - 1;
+        if (x >= level_end) {
+          int high = most - 1;  // the level: the largest with more than x items at or above it
+          low = 0;
+          while (low < high) {
+            const int mid = (low + high + 1) >> 1;
+            if (above(mid) * p.n_kv > x) low = mid; else high = mid - 1;
+          }
+          level_first = low + 1 < most ? above(low + 1) * p.n_kv : 0;
+          level_end = low > 0 ? above(low) * p.n_kv : total;
+          b0 = 0;
+          passed = 0;
         }
-        const int64_t y = x - above(low + 1) * p.n_kv;
-        int64_t rank = y / p.n_kv;
-        it.h = static_cast<int>(y - rank * p.n_kv);
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int64_t y = x - level_first;
+        const int rank = static_cast<int>(y / p.n_kv);  // among the level's sequences
+        it.h = static_cast<int>(y - static_cast<int64_t>(rank) * p.n_kv);
+        for (; b0 < p.batch; b0 += 32) {
           const uint32_t has = __ballot_sync(0xffffffffu, b0 + lane < p.batch && pairs_of(b0 + lane) > low);
-          if (rank < __popc(has)) {
-            it.b = b0 + __fns(has, 0, static_cast<int>(rank) + 1);
+          if (rank - passed < __popc(has)) {
+            it.b = b0 + __fns(has, 0, rank - passed + 1);
             break;
           }
-          rank -= __popc(has);
+          passed += __popc(has);
         }
-        const PromptSpan s = prompt_span(p, it.b);
+        const PromptSpan s = prompt_span(p, max(it.b, 0));
         it.first = static_cast<int>(s.first);
         it.tokens = s.tokens;
         it.rows = s.rows;

@@ -89,3 +89,37 @@ def test_rows_that_take_longer_than_the_limit():
         e = float((b.abs() @ a.abs()).max()) * 0.125 * D * 2.0 ** -24
         bound = u * (p @ c).abs() + (u + 2 * e + 2.0 ** -16 + n * 2.0 ** -30) * (p @ c.abs()) + 2.0 ** -24
         assert bool(((out[i, 0].double() - p @ c).abs() <= bound).all()), i
+
+
+def test_very_many_sequences():
+    """The plan's time goes with the number of sequences, not with its square (3 s for these, were each item searched
+    among all sequences), and deals every one of them out."""
+    n, H, D = 100000, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(13)
+    counts = torch.tensor([1, 0, 2, 1, 1], device="cuda").repeat(n // 5)
+    counts[77] = 700                                     # and one with several items, in levels of its own
+    starts = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    starts[1:] = counts.cumsum(0)
+    rows = int(starts[-1])
+    q, k, v = (torch.randn(rows, H, D, generator=g, device="cuda").to(BF16) for _ in range(3))
+    out = torch.full_like(q, 7.0)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    prompt.prompt_attention(q, k, v, 0.125, starts=starts, out=out, status=status)
+    end.record()
+    torch.cuda.synchronize()
+    assert int(status) == _lib.LF_OK and begin.elapsed_time(end) < 500
+    first = starts[:-1].long()[counts == 1]
+    assert torch.equal(out[first], v[first])             # a token that sees itself alone
+    first = starts[:-1].long()[counts == 2]
+    assert torch.equal(out[first], v[first])
+    a, u = q[first + 1].double(), 2.0 ** -8
+    p = torch.softmax(torch.stack([(a * k[first].double()).sum(-1), (a * k[first + 1].double()).sum(-1)], -1) * 0.125, -1).unsqueeze(-1)
+    x, y = v[first].double(), v[first + 1].double()
+    want, size = p[..., 0, :] * x + p[..., 1, :] * y, p[..., 0, :] * x.abs() + p[..., 1, :] * y.abs()
+    e = (a.abs() * torch.maximum(k[first].abs(), k[first + 1].abs()).double()).sum(-1, keepdim=True) * 0.125 * D * 2.0 ** -24
+    assert bool(((out[first + 1].double() - want).abs() <= u * want.abs() + (u + 2 * e + 2.0 ** -16) * size + 2.0 ** -24).all())
+    at = int(starts[77])
+    alone = prompt.prompt_attention(q[at:at + 700], k[at:at + 700], v[at:at + 700], 0.125)
+    assert torch.equal(out[at:at + 700], alone)
