@@ -463,8 +463,8 @@ LF_API int lf_int4_attend(const lf_int4_query* args, lf_stream_t stream);
  * the pages are those of the negated queries: the largest bounds on scaling q . K. */
 LF_API int lf_int4_attend_sparse(const lf_int4_query* args, lf_stream_t stream);
 
-/* Arguments of lf_int4_attend_prefix: those of lf_int4_attend (picked and its slots not
- * read), and the sequences that share their first pages. */
+/* Arguments of lf_int4_attend_prefix: those of lf_int4_attend (picked must be NULL), and
+ * the sequences that share their first pages. */
 typedef struct lf_int4_prefix {
   lf_int4_query query;
   const int32_t* group;   /* [batch] group of each sequence; outside [0, groups): none */
@@ -479,8 +479,12 @@ typedef struct lf_int4_prefix {
  * lf_int4_attend for sequences that share a prefix.  The first shared[g] entries of the
  * page table's rows are the same for all sequences of group g (the row of its lowest
  * sequence is read), so these pages are read and unpacked once for all queries of the
- * group.  The result is lf_int4_attend's, up to the order of its sums; a sequence that
- * sees only part of its shared pages, or is in no group, is attended as well.
+ * group.  A sequence that sees only part of its shared pages, or is in no group, is attended
+ * as well.  The result is lf_int4_attend's within roundings: where pages are read once, a Key
+ * and a Value code * scale + minimum, and a softmax weight, enter their products as fp16
+ * numbers (lf_int4_attend keeps codes and parameters apart; 2^-11 each, so that a score is
+ * off by up to 2^-11 of scaling sum |q k|); with an fp16 output Keys and weights as the sums
+ * of two.
  * workspace: 16-byte aligned, of any content; calls that overlap on the GPU need one each (of
  * both).  lf_int4_prefix_workspace_need says how many bytes this call needs, with the current
  * device's SMs (its pointers are not looked at): none where each sequence will read its pages

@@ -103,8 +103,8 @@ struct PrefixPlan {
 };
 constexpr int kPrefixRows = 256;    // rows (query token, q-head) of a unit, in two halves
 // Empty places before a unit's steps: what taking it up costs, in steps.  (A unit of 128 rows
-// takes nearly as long for a step as one of 256, 2.2 us and 2.6 at D 128: what bounds the
-// former is the unpacking of pages.  Its steps taken by both row tiles in turn, with a
+// takes nearly as long for a step as one of 256, 1.98 us and 2.35 at D 128, bf16: the chain of
+// scores, softmax and outputs of one tile.  Its steps taken by both row tiles in turn, with a
 // record each, were no faster.)
 constexpr int kPrefixCost = 2;
 __device__ __forceinline__ int PrefixGroup::start(int x) const { return places + x * (steps + kPrefixCost) + kPrefixCost; }

@@ -36,7 +36,7 @@
 // of range.
 //
 // What bounds it.  A chunk of 512 tokens behind 32768, 28 heads on 4, D 128, bf16: 281 us,
-// 864 TFLOP/s, 51 % of the measured 1680 (replayed; back to back 298).  A step takes 2.35 us
+// 864 TFLOP/s, 51 % of the measured 1680 (replayed; 272 to 288 by the GPU; back to back 297).  A step takes 2.35 us
 // with 256 rows (1.2 of products), 1.98 with 128 and 1.86 with 32: with one tile the chain of
 // scores, softmax and outputs is not hidden, with two it is in part.  Unpacking is behind it:
 // half of it left out took 2.27 and 1.97.  (fp16 outputs: 4.6 and 3.5; with each term of a Key

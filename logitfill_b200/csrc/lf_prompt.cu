@@ -27,14 +27,15 @@
 // Order of work.  The plan deals items out by falling cost over all sequences, from
 // alternating ends, without atomics: results do not depend on timing.
 //
-// What bounds it.  4 x 4096 tokens, 28 heads on 4, D 128, bf16: 444 us, 1083 TFLOP/s, 64 %
+// What bounds it.  4 x 4096 tokens, 28 heads on 4, D 128, bf16: 450 us, 1068 TFLOP/s, 64 %
 // of the measured 1680; one prompt of 8192: 414 us, 1163 TFLOP/s, 69 % (replayed in a
-// graph, with pauses; back to back under the power cap 527 and 487).  A step of both tiles
-// takes some 3700 cycles, 2048 of them products (tensor cores 51 % busy over the launch,
-// issue slots 49 %): the exponentials, 2048 cycles of the special function unit without
-// the polynomial, the other instructions of the softmax and the hand-overs between the
-// roles overlap in part only.  Without any softmax the same loop takes 377 us, with its
-// products cut to a quarter as well 237.
+// graph, with pauses; 3 % more on some GPUs; back to back under the power cap 526 and 486).
+// A step of both tiles takes some 3700 cycles, 2048 of them products (tensor cores 49 % busy
+// over the launch of one prompt of 4096, issue slots 48 %): the exponentials, 2048 cycles of
+// the special function unit without the polynomial, the other instructions of the softmax
+// and the hand-overs between the roles overlap in part only.  (When 8192 tokens took 446 us,
+// the loop without any softmax took 377, and with its products cut to a quarter as well 237:
+// hand-overs alone were over half of a step.)
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -51,7 +52,7 @@ struct PromptParams {
   const int32_t *starts, *counts;
   int32_t* status;
   float scale_log2;
-  int batch, tokens, n_q, n_kv, group;
+  int batch, tokens, n_kv, group;
   int wide_out;  // out rows are 32-byte aligned
 };
 
@@ -255,7 +256,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // ---------------------------------------------------------------- plan
     fewer_registers<kOtherRegs>();
     // Items in the order of falling cost: by their number of tokens before, over all
-    // sequences; a CTA takes them from alternating ends of rounds as wide as the grid.
+    // sequences (a padded sequence's rows behind its tokens among them, which cost little);
+    // a CTA takes them from alternating ends of rounds as wide as the grid.
     const int span = 2 * per_tile;
     auto pairs_of = [&](int b) { return (prompt_span(p, b).rows + span - 1) / span; };
     // Items of one KV head at level x or above, over all sequences (64 bits: starts may be anything).
@@ -602,7 +604,6 @@ extern "C" int lf_prompt_attend(const lf_prompt* a, lf_stream_t stream) {
   p.scale_log2 = a->scaling * 1.4426950408889634f;
   p.batch = a->batch;
   p.tokens = a->tokens;
-  p.n_q = a->n_q;
   p.n_kv = a->n_kv;
   p.group = a->n_q / a->n_kv;
   p.wide_out = reinterpret_cast<uintptr_t>(a->out) % 32 == 0 && (p.o_seq | p.o_head | p.o_tok) % 16 == 0;

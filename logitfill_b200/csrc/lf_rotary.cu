@@ -13,9 +13,9 @@
 // token's heads, so a large call is bound by HBM.  A thread keeps the cosines and sines
 // of its pairs (16 bytes of channels and their partners) in registers and walks over the
 // token's heads, four in flight.  The block's angles are worked out once, each by one
-// thread, while the first loads are on their way, and handed over in shared memory: with
-// each thread working out its own, 16384 tokens of 32 heads, D 128, took 90 us in place of
-// 57 (the arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
+// thread, while the first loads are on their way, and handed over in shared memory: when
+// that brought 16384 tokens of 32 heads, D 128, to 57 us, each thread working out its own had
+// taken 90 (the arithmetic of 8 angles for 4 heads).  In small calls there are as many threads to a
 // token as it has heads, so that each makes one round of loads.  16384 tokens of 32 heads, D
 // 128, bf16: 46 us replayed, 5.9 TB/s, 90 % of a plain copy's rate (D 256: 6.3 TB/s; fp32: 6.4);
 // 16 tokens: 2.5 us replayed, 5.3 from Python, the host's issue.
@@ -35,7 +35,7 @@ struct RotaryParams {
   int64_t pos_seq, pos_tok;
   const int32_t* start;
   float magnitude, sign;
-  int positions_64, head_dim, part, tokens, n_q, heads;
+  int positions_64, part, tokens, n_q, heads;
   int64_t total;                      // tokens of all sequences
   int per_row, head_lanes, per_block;  // items of a head's row, threads to a token and item, tokens of a block
 };
@@ -293,7 +293,6 @@ extern "C" int lf_rotary_embed(const lf_rotary* a, lf_stream_t stream) {
   p.magnitude = a->magnitude;
   p.sign = a->transposed ? -a->magnitude : a->magnitude;
   p.positions_64 = a->positions_64;
-  p.head_dim = a->head_dim;
   p.part = a->part;
   p.tokens = a->tokens;
   p.n_q = a->n_q;
@@ -314,8 +313,7 @@ extern "C" int lf_rotary_embed(const lf_rotary* a, lf_stream_t stream) {
 
   // Threads to a token and item: as many as there are heads in a small call (a thread makes
   // one round of loads), down to one for each kRotaryAhead heads once the threads fill the
-  // GPU.  16384 tokens, 32 heads, blocks of 256: 57 us so, 59 with 8 heads to a thread, 61
-  // with 16.
+  // GPU.  16384 tokens, 32 heads, when that took 57 us: 59 with 8 heads to a thread, 61 with 16.
   int lanes_heads = p.heads;
   while (lanes_heads > 1 && static_cast<int64_t>(p.total) * p.per_row * lanes_heads > kRotaryFill && lanes_heads * kRotaryAhead > p.heads)
     lanes_heads = (lanes_heads + 1) / 2;

@@ -357,7 +357,7 @@ def test_many_sequences_cost_no_more_than_before_pages_could_be_shared(cache, mo
             took.append(time.perf_counter() - since)
         return min(took)
 
-    # 17 us each on the build machine, truncate 6 ms and release 0.5 ms when they walked
+    # some 20 us each; truncate 6 ms and release 0.5 ms when they walked
     assert fastest(lambda: many.truncate(70)) < 1e-3
     assert fastest(lambda: many.release([5])) < 2e-4
     assert not any(t is many.prefix_group or t is many.prefix_pages for t in copied)
