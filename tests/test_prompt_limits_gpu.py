@@ -104,6 +104,7 @@ def test_very_many_sequences():
     q, k, v = (torch.randn(rows, H, D, generator=g, device="cuda").to(BF16) for _ in range(3))
     out = torch.full_like(q, 7.0)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    prompt.prompt_attention(q[:9], k[:9], v[:9], 0.125)   # (the first call of a process loads the kernel)
     begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     begin.record()
     prompt.prompt_attention(q, k, v, 0.125, starts=starts, out=out, status=status)
