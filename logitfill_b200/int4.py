@@ -422,7 +422,8 @@ class Int4KVCache:
         """Raise if a kernel met a position outside its sequence's pages (synchronises)."""
         code = int(self.status.item())
         if code:
-            self.status.zero_()
+            with torch.inference_mode():   # (the word may have been made in it)
+                self.status.zero_()
             _lib.check(code, "4-bit cache kernel")
 
 

@@ -262,7 +262,8 @@ class PackedKVCache:
         """Raise if a kernel reported a device-side failure (synchronises)."""
         code = int(self.status.item())
         if code:
-            self.status.zero_()
+            with torch.inference_mode():   # (the word may have been made in it)
+                self.status.zero_()
             _lib.check(code, "packed KV kernel")
 
     def length(self, b: int = 0, layer_idx: int = 0) -> int:

@@ -14,6 +14,7 @@ import torch
 
 from logitfill_b200 import _lib, int4, prompt
 from logitfill_b200.adapter import DeepSeekQwenKVAdapter
+from logitfill_b200.packed import PackedKVCache
 from tests.qwen_cases import tiny_qwen2
 from tests.test_int4_cpu import QUERY, _query
 
@@ -427,6 +428,17 @@ def test_groups_of_a_batch_with_more_sequences_than_numbers(cache, monkeypatch):
     assert [group[b] for b in rest] == [2 + i if 2 + i < int4.MAX_GROUPS else -1 for i in range(len(rest))] and not any(pages[2:])
     many.release([4500, 7, 4990])
     assert many.prefix_group.tolist() == [b if b < int4.MAX_GROUPS else -1 for b in range(n)] and not many.prefix_pages.any()
+
+
+@pytest.mark.parametrize("cls", [int4.Int4KVCache, PackedKVCache])
+@pytest.mark.parametrize("inference", [False, True])
+def test_status_is_raised_wherever_the_cache_was_made(cls, inference):
+    """A cache that was made in inference mode (an adapter makes its at the first forward) is asked outside of it."""
+    with torch.inference_mode(inference):
+        holder = type("Holder", (), dict(status=torch.full((1,), _lib.LF_ERR_DEVICE_TIMEOUT, dtype=torch.int32)))()
+    with pytest.raises(RuntimeError, match="timed out"):
+        cls.check_status(holder)
+    cls.check_status(holder)      # and is clean behind it
 
 
 def test_adapter_takes_the_prompt_kernel_by_name():
